@@ -413,10 +413,10 @@ def _plain_tables(slots, old, new, free, count, table, page, max_rows, parents, 
     behind = torch.cumsum(need, 0)
     padded = (new - old + multiple - 1) // multiple * multiple
     ends = torch.cumsum(padded, 0)
-    forked = torch.zeros(table.shape[0], dtype=torch.bool, device=table.device)
-    forked[slots.clamp(0, table.shape[0] - 1)] = fork
+    named = torch.zeros(table.shape[0], dtype=torch.bool, device=table.device)
+    named[slots.clamp(0, table.shape[0] - 1)] = True  # a parent is no request of the same call
     valid = (slots > 0) & (slots < table.shape[0]) & (old >= 0) & (new >= old) & (parents < table.shape[0])
-    valid &= ~(fork & forked[parents.clamp(0, table.shape[0] - 1)])
+    valid &= ~(fork & named[parents.clamp(0, table.shape[0] - 1)])
     order = torch.sort(slots).values
     twice = (order[1:] == order[:-1]).any()
     status = ((behind[-1] > count[0]).int() + 2 * (blocks > columns).any().int() + 4 * (ends[-1] > max_rows).int()
