@@ -19,7 +19,7 @@ _LIB_DIR = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib")
 LIB_PATH = os.path.join(_LIB_DIR, "libfp_paged_kv.so")
 HOST_PATH = os.path.join(_LIB_DIR, "fp_host.so")
 
-FP_ABI_VERSION = 10
+FP_ABI_VERSION = 11
 NOALLOC_SCRATCH_BYTES = 64 << 20  # FP_NOALLOC_SCRATCH_BYTES
 FP_DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 FP_INDEX = {torch.int32: 0, torch.int64: 1}
@@ -79,6 +79,21 @@ SIGNATURES = {
     "fp_paged_prefill_workspace_bytes": (c_int64, [c_int32, c_int32, c_int32, c_int32, c_int]),
     "fp_paged_prefill_uncut_keys": (c_int32, [c_int32, c_int32, c_int32, c_int32, c_int32, c_int]),
 }
+
+SIGNATURES["fp_step_tables"] = (c_int, [
+    c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_int64, c_void_p, c_int64, c_int64,
+    c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+    c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_void_p])
+SIGNATURES["fp_copy_pages"] = (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int32, c_int32,
+                                       c_int, c_void_p])
+SIGNATURES["fp_shared_decode_plan_bytes"] = (c_int64, [c_int32] * 5)
+SIGNATURES["fp_shared_decode_workspace_bytes"] = (c_int64, [c_int32] * 5)
+SIGNATURES["fp_shared_decode_plan"] = (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p] + [c_int32] * 7
+                                       + [c_void_p, c_int64, c_void_p])
+SIGNATURES["fp_paged_decode_shared"] = (c_int, [
+    c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int,
+    c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64,
+    c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int64, c_int32, c_float, c_int, c_void_p])
 
 SIGNATURES["fp_probe_mfma_softmax"] = (c_int, [c_int, c_int, c_int, c_int, c_void_p, c_int64, c_void_p])
 SIGNATURES["fp_paged_decode_plan"] = SIGNATURES["fp_paged_decode"]

@@ -5,7 +5,9 @@ caller leaves an output or workspace argument out, and none synchronises.
 
 from __future__ import annotations
 
+import contextlib
 import math
+from typing import NamedTuple
 
 import torch
 from torch import Tensor
@@ -482,3 +484,242 @@ def prefill_uncut_keys(Lq: int, Hq: int, Hc: int, D: int, page_size: int, dtype:
     n = int(N.lib().fp_paged_prefill_uncut_keys(Lq, Hq, Hc, D, page_size, N.dtype_code(dtype)))
     N.check(n, "fp_paged_prefill_uncut_keys")
     return n
+
+
+# ----------------------------------------------------------------- many requests on one cached prefix
+
+def _on(device: torch.device):
+    """The launch goes to the current device: that of the tensors, whichever is current."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _same_device(what: str, *tensors) -> torch.device:
+    N.require_cuda(*tensors)
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) != 1:
+        raise RuntimeError(f"{what}: the tensors are on different devices: {sorted(map(str, devices))}")
+    return devices.pop()
+
+
+def _vector(what: str, name: str, t: Tensor, n: int | None, *dtypes: torch.dtype) -> Tensor:
+    if t.dtype not in dtypes or t.dim() != 1 or (n is not None and t.shape[0] != n):
+        raise RuntimeError(f"{what}: {name} must be {' or '.join(str(d)[6:] for d in dtypes)} "
+                           f"[{'n' if n is None else n}], got {str(t.dtype)[6:]} {list(t.shape)}")
+    return t.contiguous()
+
+
+def _page_table(what: str, page_table: Tensor) -> None:
+    if page_table.dtype != torch.int64 or page_table.dim() != 2 or page_table.stride(1) != 1:
+        raise RuntimeError(f"{what}: page_table must be int64 [max_batch, blocks] with a dense last axis")
+
+
+class StepTables(NamedTuple):
+    """What `step_tables` makes besides the rows of the page table; see there."""
+
+    batch_idx: Tensor
+    input_pos: Tensor
+    slot_map: Tensor
+    row_starts: Tensor
+    free_left: Tensor
+    copy_src: Tensor
+    copy_dst: Tensor
+    copy_rows: Tensor
+    status: Tensor
+
+    REPORTS = ("the free list has too few pages", "a request is longer than a row of the page table",
+               "the rows of the requests exceed max_rows",
+               "a request names a slot outside the table or another one's, its lengths are negative, shrink or do not fit 31 bits, "
+               "its parent is a request of the same call or outside the table, or free_count lies outside the free list")
+
+    def check(self) -> "StepTables":
+        """Wait for the launch and raise if it refused the step."""
+        bits = int(self.status.item())
+        if bits:
+            raise RuntimeError("step_tables: " + "; ".join(r for i, r in enumerate(self.REPORTS) if bits >> i & 1))
+        return self
+
+
+def step_tables(slots: Tensor, old_lens: Tensor, new_lens: Tensor, free_pages: Tensor, free_count: Tensor,
+                page_table: Tensor, page_size: int, max_rows: int, *, parents: Tensor | None = None,
+                row_multiple: int = 1, inverse: Tensor | None = None) -> StepTables:
+    """Rows of the page table, packed rows and slot map of a step from the lengths of its requests, in one launch.
+
+    Request b grows the sequence in cache slot `slots[b]` (int64) from `old_lens[b]` to `new_lens[b]` tokens (int32 or int64).
+    Pages come from the end of the first `free_count[0]` (int32 [1]) of `free_pages` (int64), in the order in which
+    `PagedKVCache.reserve`, called request by request, takes them, and go to `page_table` [max_batch, blocks], in place
+    (`inverse` [max_batch, pages], optional: the inverse map along with it).  `parents[b]` > 0 (int64) makes the request a fork
+    of that slot: its first `old_lens[b]` tokens are the parent's, whose whole pages it shares; the page in which the prefix
+    ends is its own, and `copy_src`, `copy_dst`, `copy_rows` [B] say what `copy_pages` has to copy for it (-1, -1, 0: nothing).
+
+    Returned rows, `max_rows` of them: `batch_idx` (int64) and `input_pos` (int32) of every new token, request after request,
+    each one's rows padded to a multiple of `row_multiple` - what a packed prefill step is given -, and `slot_map` (int64), the
+    row page * page_size + position % page_size of the pool's planes; padding is 0, 0, 0.  `row_starts` [B + 1] int32,
+    `free_left` [1] int32: the next `free_count`.  `status` [1] int32: not 0 means that nothing was done, and `check()`
+    waits and says why."""
+    what = "step_tables"
+    device = _same_device(what, slots, old_lens, new_lens, free_pages, free_count, page_table, parents, inverse)
+    slots = _vector(what, "slots", slots, None, torch.int64)
+    B = slots.shape[0]
+    old_lens = _vector(what, "old_lens", old_lens, B, torch.int32, torch.int64)
+    new_lens = _vector(what, "new_lens", new_lens, B, old_lens.dtype)
+    if parents is not None:
+        parents = _vector(what, "parents", parents, B, torch.int64)
+    free_pages = _vector(what, "free_pages", free_pages, None, torch.int64)
+    free_count = _vector(what, "free_count", free_count, 1, torch.int32)
+    _page_table(what, page_table)
+    if inverse is not None and (inverse.dtype != torch.int64 or inverse.dim() != 2 or inverse.stride(1) != 1
+                                or inverse.shape[0] != page_table.shape[0]):
+        raise RuntimeError(f"{what}: inverse must be int64 [max_batch, pages] with a dense last axis")
+    if max_rows < 0 or row_multiple < 1:
+        raise RuntimeError(f"{what}: max_rows {max_rows}, row_multiple {row_multiple}")
+    with _on(device):
+        long = lambda n: torch.empty(n, dtype=torch.int64, device=device)
+        whole = lambda n: torch.empty(n, dtype=torch.int32, device=device)
+        made = StepTables(long(max_rows), whole(max_rows), long(max_rows), whole(B + 1), whole(1), long(B), long(B), whole(B),
+                          whole(1))
+        rc = N.lib().fp_step_tables(
+            slots.data_ptr(), old_lens.data_ptr(), new_lens.data_ptr(), N.index_code(old_lens),
+            None if parents is None else parents.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(), free_pages.shape[0],
+            page_table.data_ptr(), page_table.stride(0), None if inverse is None else inverse.data_ptr(),
+            0 if inverse is None else inverse.stride(0), 0 if inverse is None else inverse.shape[1],
+            *(t.data_ptr() for t in made), B, max_rows, row_multiple, page_size, page_table.shape[1], page_table.shape[0],
+            N.stream_ptr(device))
+    N.check(rc, "fp_step_tables")
+    return made
+
+
+def copy_pages(pool: Tensor, src: Tensor, dst: Tensor, rows: Tensor, page_size: int) -> None:
+    """Copy the first `rows[i]` (int32) rows of page `src[i]` to page `dst[i]` (int64) in every plane of `pool` [..., n_slots, D].
+
+    An entry with a page outside the pool (-1: nothing to copy) or without rows is left out, and so are an entry whose
+    destination is a source of the call and one whose destination an entry before it has: every source is copied as it was."""
+    what = "copy_pages"
+    device = _same_device(what, pool, src, dst, rows)
+    if pool.dim() < 2 or not pool.is_contiguous():
+        raise RuntimeError(f"{what}: the pool must be contiguous [..., n_slots, D]")
+    if page_size < 1:
+        raise RuntimeError(f"{what}: page_size {page_size}")
+    src = _vector(what, "src", src, None, torch.int64)
+    n = src.shape[0]
+    dst = _vector(what, "dst", dst, n, torch.int64)
+    rows = _vector(what, "rows", rows, n, torch.int32)
+    n_slots, D = pool.shape[-2:]
+    if pool.numel() == 0:
+        return
+    with _on(device):
+        rc = N.lib().fp_copy_pages(pool.data_ptr(), src.data_ptr(), dst.data_ptr(), rows.data_ptr(), n,
+                                   pool.numel() // (n_slots * D), n_slots, D, page_size, N.dtype_code(pool.dtype),
+                                   N.stream_ptr(device))
+    N.check(rc, "fp_copy_pages")
+
+
+def shared_decode_plan_bytes(B: int, S: int, *, q_heads: int, cached_heads: int, head_dim: int) -> int:
+    """Bytes of the plan of a `paged_decode_shared` step of this shape."""
+    n = int(N.lib().fp_shared_decode_plan_bytes(B, S, q_heads, cached_heads, head_dim))
+    N.check(n, "fp_shared_decode_plan_bytes")
+    return n
+
+
+def shared_decode_workspace_bytes(B: int, S: int, *, q_heads: int, cached_heads: int, head_dim: int) -> int:
+    """Bytes of workspace that `paged_decode_shared` needs for this shape, whatever the lengths are."""
+    n = int(N.lib().fp_shared_decode_workspace_bytes(B, S, q_heads, cached_heads, head_dim))
+    N.check(n, "fp_shared_decode_workspace_bytes")
+    return n
+
+
+def _shared_step(what: str, batch_idx: Tensor, input_pos: Tensor, prefix_ids: Tensor, prefix_lens: Tensor):
+    batch_idx = _vector(what, "batch_idx", batch_idx, None, torch.int64)
+    B = batch_idx.shape[0]
+    if input_pos.dtype not in (torch.int32, torch.int64) or input_pos.dim() not in (1, 2) or input_pos.shape[0] != B:
+        raise RuntimeError(f"{what}: input_pos must be int32 or int64 [B] or [B, S] with B = {B}, got {list(input_pos.shape)}")
+    prefix_ids = _vector(what, "prefix_ids", prefix_ids, None, torch.int32)
+    prefix_lens = _vector(what, "prefix_lens", prefix_lens, prefix_ids.shape[0], torch.int32)
+    return batch_idx, input_pos.contiguous(), prefix_ids, prefix_lens, input_pos.shape[1] if input_pos.dim() == 2 else 1
+
+
+def _byte_buffer(what: str, name: str, t: Tensor | None, need: int, device) -> Tensor:
+    if t is None:
+        return torch.empty(need, dtype=torch.uint8, device=device)
+    if t.dtype != torch.uint8 or not t.is_contiguous() or t.numel() < need:
+        raise RuntimeError(f"{what}: {name} must be a contiguous uint8 tensor of at least {need} bytes")
+    return t
+
+
+def shared_decode_plan(batch_idx: Tensor, input_pos: Tensor, prefix_ids: Tensor, prefix_lens: Tensor, *, q_heads: int,
+                       cached_heads: int, head_dim: int, max_context: int, plan: Tensor | None = None) -> Tensor:
+    """The plan of a `paged_decode_shared` step, made once for all layers: which sequences share a prefix and how the work
+    is cut.  Arguments as there; `plan`: a uint8 tensor of `shared_decode_plan_bytes(...)` bytes to write it to."""
+    what = "shared_decode_plan"
+    device = _same_device(what, batch_idx, input_pos, prefix_ids, prefix_lens, plan)
+    batch_idx, input_pos, prefix_ids, prefix_lens, S = _shared_step(what, batch_idx, input_pos, prefix_ids, prefix_lens)
+    B, shape = batch_idx.shape[0], dict(q_heads=q_heads, cached_heads=cached_heads, head_dim=head_dim)
+    with _on(device):
+        plan = _byte_buffer(what, "plan", plan, shared_decode_plan_bytes(B, S, **shape), device)
+        rc = N.lib().fp_shared_decode_plan(
+            batch_idx.data_ptr(), input_pos.data_ptr(), N.index_code(input_pos), prefix_ids.data_ptr(), prefix_lens.data_ptr(),
+            B, S, q_heads, cached_heads, head_dim, prefix_ids.shape[0], max_context, plan.data_ptr(), plan.numel(),
+            N.stream_ptr(device))
+    N.check(rc, "fp_shared_decode_plan")
+    return plan
+
+
+def paged_decode_shared(q: Tensor, pool_k: Tensor, pool_v: Tensor, page_table: Tensor, batch_idx: Tensor, input_pos: Tensor,
+                        prefix_ids: Tensor, prefix_lens: Tensor, page_size: int, max_context: int, *,
+                        scale: float | None = None, sinks: Tensor | None = None, plan: Tensor | None = None,
+                        workspace: Tensor | None = None, out: Tensor | None = None,
+                        lse: Tensor | None = None) -> tuple[Tensor, Tensor]:
+    """Attention of a batch's newest tokens over the paged cache; keys that sequences of the batch begin with in common are read once.
+
+    q [B, Hq, S, D], S tokens a sequence (1 in a decode step); pools [Hc, N, D]; `input_pos` [B] or [B, S]: token j of sequence
+    b sees the cached positions 0 .. input_pos[b, j], and -1 is no token (out 0, lse -inf).  `prefix_ids`, `prefix_lens`
+    [max_batch] int32 by cache slot: slots with the same id > 0 hold the same keys and values at the positions below the smallest
+    of their prefix_lens, in the same pages or in copies.  Returns out like q and lse [B, Hq, S].
+
+    `plan`: what `shared_decode_plan` made for this step (positions, slots and table unchanged since); without one the call
+    makes it.  `workspace`: `shared_decode_workspace_bytes(...)` bytes, for one launch at a time.  `sinks` [Hq] float32 gates
+    the output as in `paged_decode`."""
+    what = "paged_decode_shared"
+    device = _same_device(what, q, pool_k, pool_v, page_table, batch_idx, input_pos, prefix_ids, prefix_lens, sinks, plan,
+                          workspace, out, lse)
+    if q.dim() != 4 or pool_k.dim() != 3:
+        raise RuntimeError(f"{what}: q must be [B, Hq, S, D] and the pools [Hc, N, D]")
+    B, Hq, S, D = q.shape
+    Hc, n_slots, Dp = pool_k.shape
+    if Dp != D or pool_v.shape != pool_k.shape or pool_k.dtype != q.dtype or pool_v.dtype != q.dtype:
+        raise RuntimeError(f"{what}: q / pool shape or dtype mismatch")
+    if not (pool_k.is_contiguous() and pool_v.is_contiguous()):
+        raise RuntimeError(f"{what}: pool planes must be contiguous [H, N, D]")
+    _page_table(what, page_table)
+    batch_idx, input_pos, prefix_ids, prefix_lens, tokens = _shared_step(what, batch_idx, input_pos, prefix_ids, prefix_lens)
+    if batch_idx.shape[0] != B or tokens != S:
+        raise RuntimeError(f"{what}: batch_idx and input_pos are of {batch_idx.shape[0]} sequences of {tokens} tokens, q is of "
+                           f"{B} of {S}")
+    if prefix_ids.shape[0] != page_table.shape[0]:
+        raise RuntimeError(f"{what}: prefix_ids and prefix_lens need one entry per row of page_table ({page_table.shape[0]})")
+    q = _rows(q)
+    shape = dict(q_heads=Hq, cached_heads=Hc, head_dim=D)
+    with _on(device):
+        if plan is None:
+            plan = shared_decode_plan(batch_idx, input_pos, prefix_ids, prefix_lens, max_context=max_context, **shape)
+        workspace = _byte_buffer(what, "workspace", workspace, shared_decode_workspace_bytes(B, S, **shape), device)
+        if out is None:
+            out = torch.empty_like(q)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.stride(3) != 1:
+            raise RuntimeError(f"{what}: out must be like q, with dense rows")
+        if lse is None:
+            lse = torch.empty((B, Hq, S), dtype=torch.float32, device=device)
+        elif lse.shape != (B, Hq, S) or lse.dtype != torch.float32 or not lse.is_contiguous():
+            raise RuntimeError(f"{what}: lse must be contiguous float32 [B, Hq, S]")
+        if plan.dtype != torch.uint8 or not plan.is_contiguous():
+            raise RuntimeError(f"{what}: plan must be a contiguous uint8 tensor")
+        rc = N.lib().fp_paged_decode_shared(
+            q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), pool_k.data_ptr(), pool_v.data_ptr(), page_table.data_ptr(),
+            page_table.stride(0), batch_idx.data_ptr(), input_pos.data_ptr(), N.index_code(input_pos), out.data_ptr(),
+            out.stride(0), out.stride(1), out.stride(2), lse.data_ptr(), _sinks_ptr(sinks, Hq, device), workspace.data_ptr(),
+            workspace.numel(), plan.data_ptr(), plan.numel(), B, S, Hq, Hc, D, page_size, page_table.shape[1],
+            page_table.shape[0], n_slots, max_context, 1.0 / math.sqrt(D) if scale is None else scale, N.dtype_code(q.dtype),
+            N.stream_ptr(device))
+    N.check(rc, "fp_paged_decode_shared")
+    return out, lse

@@ -44,7 +44,7 @@
 extern "C" {
 #endif
 
-#define FP_ABI_VERSION 10
+#define FP_ABI_VERSION 11
 
 /* element types of pool / q / k / v */
 #define FP_DTYPE_F32 0
@@ -537,6 +537,97 @@ int fp_paged_prefill(const void* q, int64_t q_stride_row, int64_t q_stride_h,
  */
 int fp_probe_mfma_softmax(int mode, int waves_per_simd, int workgroups, int iters, float* out, int64_t out_floats,
                           void* stream);
+
+/* ---- many requests on one cached prefix (ABI 11; the reference has no counterpart but where one is named) ---- */
+
+/*
+ * Page tables, packed rows and slot map of a step, from the lengths of its requests: what a host loop over
+ * PagedKVCache.reserve (paged_attention.py:115-164) and the engine's lists of a packed prefill step
+ * (paged_inference.py:637-672) come to, in one launch without the host.
+ *
+ *   slots      [B] int64 cache slot of each request: 1 .. max_batch - 1, each at most once
+ *   old_lens, new_lens  [B] int32/int64 (len_index_type): tokens of the request in the cache before and after the step
+ *   parents    NULL, or [B] int64: a slot > 0 makes the request a fork, whose first old_lens[b] tokens are those of that slot.  Its
+ *              whole pages are shared: the blocks 0 .. old / P - 1 of the parent's row are copied as they are.  The page the prefix ends in
+ *              is the fork's own (copy_src .. copy_rows: what fp_copy_pages takes).  A parent is no request of the same call and
+ *              has these blocks mapped
+ *   free_pages [n_free] int64, of which the first free_count[0] are free.  Pages are taken from the end, request by request, in
+ *              the order in which reserve takes them: block have + i of request b gets free_pages[count - off_b - need_b + i]
+ *   page_table [max_batch, n_pages] int64: the blocks behind those a request has are written, of a fork also the shared ones;
+ *              nothing else is
+ *   inverse    NULL, or [max_batch, inv_cols] int64 (physical_to_logical): inverse[slot, page] = block for every block written
+ *   batch_idx, input_pos, slot_map  [max_rows] int64, int32, int64: the tokens old .. new - 1 of every request, request after
+ *              request, each one's rows padded to row_multiple: cache slot, position, and page * P + position % P (the row of the pool's
+ *              planes).  Padding and what is behind the last request: 0, 0, 0, the reserved page
+ *   row_starts [B + 1] int32: first row of each request; last, the rows of all
+ *   free_left  [1] int32: free pages left; another address than free_count, whose next value it is
+ *   copy_src, copy_dst, copy_rows  [B] int64, int64, int32: page to copy, page to copy it to, rows of it; -1, -1, 0 where there is none
+ *   status     [1] int32: 0, or why NOTHING was done (tables untouched, rows all padding, free_left = free_count, row_starts all 0):
+ *              bit 0 pages are short, bit 1 a request is longer than a row of the table, bit 2 the rows exceed max_rows,
+ *              bit 3 a bad request (slot out of range or named twice, old < 0, new < old, new >= 2^31, parent >= max_batch or itself a
+ *              request of the call) or free_count outside 0 .. n_free
+ * B <= 4096, max_batch <= 131072.
+ */
+int fp_step_tables(const int64_t* slots, const void* old_lens, const void* new_lens, int len_index_type,
+                   const int64_t* parents, const int64_t* free_pages, const int32_t* free_count, int32_t n_free,
+                   int64_t* page_table, int64_t pt_row_stride,
+                   int64_t* inverse, int64_t inv_row_stride, int64_t inv_cols,
+                   int64_t* batch_idx, int32_t* input_pos, int64_t* slot_map, int32_t* row_starts, int32_t* free_left,
+                   int64_t* copy_src, int64_t* copy_dst, int32_t* copy_rows, int32_t* status,
+                   int32_t B, int32_t max_rows, int32_t row_multiple,
+                   int32_t page_size, int32_t n_pages, int32_t max_batch, void* stream);
+
+/*
+ * Copies the first rows of pages to other pages, in every plane of a pool (all layers, K and V, all heads):
+ *   pool[p, dst[i] * P + t, :] = pool[p, src[i] * P + t, :]   for t < min(rows[i], P)
+ *
+ *   pool       [n_planes, n_slots, D] contiguous
+ *   src, dst   [n] int64 pages; an entry with a page outside 0 .. n_slots / P - 1, or rows[i] <= 0, is left out (fp_step_tables
+ *              leaves -1 where there is nothing to copy)
+ *   rows       [n] int32
+ * Left out are also an entry whose dst is the src of a valid entry (its own included) and one whose dst a valid entry before it has:
+ * every source is copied as it was before the call, whatever the order.  n <= 65535.
+ */
+int fp_copy_pages(void* pool, const int64_t* src, const int64_t* dst, const int32_t* rows, int32_t n,
+                  int64_t n_planes, int64_t n_slots, int32_t D, int32_t page_size, int dtype, void* stream);
+
+/*
+ * Attention of a batch's newest tokens where sequences begin with the same keys: a picture that many requests ask about.
+ * The keys of such a prefix are read once for all its sequences, not once for each.
+ *
+ *   q          [B, Hq, S, D], element strides (b, h, s): S tokens per sequence, 1 in a decode step
+ *   input_pos  [B, S] contiguous, int32/int64: token j of sequence b attends logical positions 0 .. input_pos[b, j] (at most
+ *              max_context - 1); every such key is in the cache already.  input_pos < 0: no token, out = 0, lse = -inf
+ *   prefix_ids, prefix_lens  [max_batch] int32 by cache slot: slots with the same id > 0 have the same keys and values at the positions
+ *              0 .. (smallest of their prefix_lens) - 1, be it in the same pages or in copies of them.  An id <= 0 shares with nobody
+ *   out        [B, Hq, S, D], element strides (b, h, s); lse [B, Hq, S] float32 contiguous
+ *   sinks, scale, page_table, batch_idx, pool_k, pool_v, n_slots  as fp_paged_decode
+ * Results are those of fp_paged_decode for each token, up to the order of the sums; with a false prefix_ids they are not: a shared key
+ * is read through the table row of any of the sequences.
+ *
+ * fp_shared_decode_plan, once per step, finds the sequences that share and cuts the work; every layer's fp_paged_decode_shared with the
+ * same B, S, Hq, Hc, D and max_context takes the plan.  batch_idx, input_pos and the rows of page_table must not change in between: a launch
+ * that meets a plan of another shape, or of other slots or positions for a row, leaves NaN in out and lse there.
+ * Plan and workspace are memory of the caller (16-byte aligned), one launch at a time; nothing in them needs clearing.
+ * Hq / Hc in {1, 2, 4, 8}, D in {64, 128}, B <= 4096, S <= 1024.  Both may be captured in a graph.
+ */
+int64_t fp_shared_decode_plan_bytes(int32_t B, int32_t S, int32_t Hq, int32_t Hc, int32_t D);
+int64_t fp_shared_decode_workspace_bytes(int32_t B, int32_t S, int32_t Hq, int32_t Hc, int32_t D);
+int fp_shared_decode_plan(const int64_t* batch_idx, const void* input_pos, int pos_index_type,
+                          const int32_t* prefix_ids, const int32_t* prefix_lens,
+                          int32_t B, int32_t S, int32_t Hq, int32_t Hc, int32_t D,
+                          int32_t max_batch, int32_t max_context,
+                          void* plan, int64_t plan_bytes, void* stream);
+int fp_paged_decode_shared(const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_s,
+                           const void* pool_k, const void* pool_v,
+                           const int64_t* page_table, int64_t pt_row_stride,
+                           const int64_t* batch_idx, const void* input_pos, int pos_index_type,
+                           void* out, int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_s,
+                           float* lse, const float* sinks,
+                           void* workspace, int64_t workspace_bytes, const void* plan, int64_t plan_bytes,
+                           int32_t B, int32_t S, int32_t Hq, int32_t Hc, int32_t D,
+                           int32_t page_size, int32_t n_pages, int32_t max_batch, int64_t n_slots,
+                           int32_t max_context, float scale, int dtype, void* stream);
 
 #ifdef __cplusplus
 }

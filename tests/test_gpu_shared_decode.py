@@ -1,0 +1,183 @@
+"""Attention of a batch whose sequences share prefixes, against float64 (tolerances: SharedBatch.expect)."""
+
+import pytest
+import torch
+
+from falcon_perception_amd import ops
+from tests.shared_cases import SharedBatch
+
+pytestmark = pytest.mark.gpu
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def one_each(groups, behind, n=1):
+    return [(g, k, n) for g, k in zip(groups, behind)]
+
+
+SHAPES = {
+    # a single sequence, with and without a prefix; one key
+    "one_key": ([], [(-1, 1, 1)]),
+    "one_alone": ([], [(-1, 77, 1)]),
+    "one_with_prefix": ([130], [(0, 5, 1)]),
+    # all of the batch on one prefix that ends inside a page and a tile
+    "picture": ([203], one_each([0] * 7, [1, 2, 17, 64, 65, 130, 33])),
+    # groups of many sizes, loners between them, in no order
+    "mixed": ([65, 257, 128, 1], one_each([2, -1, 0, 1, 2, -1, 1, 3, 0, 3, 2, -1, 3], [3, 300, 9, 70, 1, 1, 128, 5, 64, 63, 40, 129, 1])),
+    # more rows than a tile of queries
+    "many": ([300], one_each([0] * 75, [1 + 7 * i % 50 for i in range(75)])),
+    # keys of the prefix only: the token itself is its last key
+    "nothing_behind": ([192], [(0, 1, 1), (0, 1, 1), (0, 1, 1)]),
+    "long": ([2111], one_each([0, 0, 0, -1], [700, 3, 1, 1500])),
+}
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("D,Hq,Hc", [(128, 4, 2), (64, 8, 1), (128, 8, 2), (64, 2, 2)])
+@pytest.mark.parametrize("shape", list(SHAPES))
+def test_a_token_each(shape, D, Hq, Hc, dtype):
+    prefixes, sequences = SHAPES[shape]
+    case = SharedBatch(11, prefixes, sequences, Hq=Hq, Hc=Hc, D=D, P=64, dtype=dtype).on()
+    case.check(case.call(ops))
+
+
+@pytest.mark.parametrize("P", [1, 16, 48, 100, 128, 256])
+def test_page_sizes(P):
+    case = SharedBatch(12, [150, 97], one_each([0, 1, 0, -1, 1, 0], [5, 40, 130, 99, 1, 17]), Hq=4, Hc=2, D=128, P=P, dtype=BF16).on()
+    case.check(case.call(ops))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("D,Hq,Hc", [(128, 4, 2), (64, 8, 1), (64, 1, 1)])
+@pytest.mark.parametrize("tokens", [2, 5, 17, 70])
+def test_several_tokens(tokens, D, Hq, Hc, dtype):
+    """Prompts of different lengths behind their pictures, padded to the longest; one sequence has no token at all."""
+    seqs = [(0, tokens, tokens), (0, tokens + 3, 1), (-1, tokens, max(1, tokens // 2)), (1, 2 * tokens, tokens), (1, 9, min(9, tokens)),
+            (0, 4, 0)]
+    case = SharedBatch(13, [190, 64], seqs, Hq=Hq, Hc=Hc, D=D, P=32, dtype=dtype, S=tokens).on()
+    case.check(case.call(ops))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_sink_gate_and_scale(dtype):
+    case = SharedBatch(14, [100], one_each([0, 0, -1], [20, 90, 33]), Hq=8, Hc=2, D=64, P=64, dtype=dtype).on()
+    sinks = torch.randn(8, generator=case.gen)
+    case.check(case.call(ops, sinks=sinks.cuda(), scale=0.21), sinks=sinks, scale=0.21)
+
+
+def test_rows_that_see_less_than_the_prefix():
+    """A sequence whose position lies inside the shared prefix sees its keys up to there, and int64 positions are the same."""
+    case = SharedBatch(15, [300], one_each([0] * 5, [3, 50, 9, 1, 1]), Hq=4, Hc=2, D=128, P=64, dtype=BF16).on()
+    case.pos[1, 0], case.pos[2, 0], case.pos[3, 0] = 0, 131, 298
+    case.pos_d = case.pos.cuda()
+    got = case.call(ops)
+    case.check(got)
+    again = case.call(ops, pos=case.pos_d.long())
+    assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+
+
+def test_no_token_and_slots_outside_the_table():
+    case = SharedBatch(16, [100], one_each([0] * 4, [3, 50, 9, 20]), Hq=4, Hc=2, D=128, P=64, dtype=BF16).on()
+    case.pos[1, 0] = -1
+    case.pos_d = case.pos.cuda()
+    case.batch_idx_d[2] = case.max_batch
+    case.batch_idx_d[3] = -5
+    got = case.call(ops)
+    case.pos[2, 0] = case.pos[3, 0] = -1
+    case.check(got)
+
+
+def test_max_context_bounds_the_keys():
+    case = SharedBatch(17, [100], one_each([0] * 4, [3, 50, 9, 200]), Hq=4, Hc=2, D=128, P=64, dtype=BF16).on()
+    got = case.call(ops, max_context=109)
+    case.check(got, pos=case.pos.clamp(max=108))
+
+
+def test_smallest_length_of_a_group_counts():
+    """Members whose prefix lengths differ share the smallest of them; an id of 0 or below shares with nobody."""
+    case = SharedBatch(18, [300], one_each([0] * 6, [30, 50, 9, 1, 77, 6]), Hq=4, Hc=2, D=128, P=64, dtype=BF16)
+    case.lens[case.batch_idx[2]] = 133
+    case.lens[case.batch_idx[4]] = -3
+    case.ids[case.batch_idx[4]] = 0
+    case.ids[case.batch_idx[5]] = -3
+    case.on()
+    case.check(case.call(ops))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_strides(dtype):
+    """q as a slice of a projection, out as rows of a projection's input, table rows of a wider table."""
+    case = SharedBatch(19, [90], one_each([0, 0, -1, 0], [20, 90, 33, 4]), Hq=8, Hc=2, D=64, P=32, dtype=dtype).on()
+    want = case.call(ops)
+    wide = torch.randn(4, 1, 12, 64, device="cuda").to(dtype)
+    wide[:, :, 2:10] = case.q_d.transpose(1, 2)
+    out = torch.full((4, 1, 9, 64), 7.0, device="cuda", dtype=dtype)
+    case.table_d = torch.cat([case.table_d, torch.full_like(case.table_d, 10 ** 12)], 1)[:, :case.columns]
+    got = case.call(ops, q=wide[:, :, 2:10].transpose(1, 2), out=out[:, :, :8].transpose(1, 2))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert (out[:, :, 8] == 7).all()
+
+
+def test_unmapped_pages_are_the_reserved_page():
+    """As in paged_decode: a block without a page reads page 0."""
+    case = SharedBatch(20, [], [(-1, 200, 1), (-1, 90, 1)], Hq=4, Hc=2, D=128, P=64, dtype=BF16)
+    case.pool[:, :, :64] = torch.randn(case.pool[:, :, :64].shape, generator=case.gen).to(BF16)
+    case.table[case.batch_idx[0], 1] = -1
+    for i in range(2):
+        case.keys[0][i][:, 64:128] = case.pool[i][:, :64]
+    case.on()
+    case.check(case.call(ops))
+
+
+def test_equal_to_paged_decode():
+    """The same step through the operator that reads every copy; the two differ by the order of their sums."""
+    case = SharedBatch(21, [400, 129], one_each([0, 1, 0, -1, 1], [20, 90, 33, 4, 300]), Hq=8, Hc=4, D=128, P=128, dtype=BF16).on()
+    got = case.call(ops)
+    plain = ops.paged_decode(case.q_d, case.pool_d[0].nan_to_num(), case.pool_d[1].nan_to_num(), case.table_d, case.batch_idx_d,
+                             case.pos_d.view(-1), 128, case.columns * 128)
+    case.check(got)
+    case.check(plain)
+
+
+def test_scores_of_any_size():
+    """Scores spread over hundreds: the running maximum moves, and most probabilities vanish."""
+    for dtype in (BF16, F16, F32):
+        case = SharedBatch(22, [300], one_each([0, 0, -1], [20, 90, 333]), Hq=4, Hc=2, D=128, P=64, dtype=dtype, spread=5.0).on()
+        case.check(case.call(ops))
+
+
+def test_an_empty_batch():
+    case = SharedBatch(23, [], [(-1, 3, 1)], Hq=4, Hc=2, D=128, P=64, dtype=BF16).on()
+    out, lse = ops.paged_decode_shared(case.q_d[:0], case.pool_d[0], case.pool_d[1], case.table_d, case.batch_idx_d[:0],
+                                       case.pos_d[:0], case.ids_d, case.lens_d, 64, 64)
+    assert out.shape == (0, 4, 1, 128) and lse.shape == (0, 4, 1)
+
+
+def test_refusals():
+    case = SharedBatch(24, [64], [(0, 3, 1), (0, 5, 1)], Hq=4, Hc=2, D=128, P=64, dtype=BF16).on()
+    call = lambda **kw: case.call(ops, **kw)
+    with pytest.raises(RuntimeError, match="workspace must be"):
+        call(workspace=torch.empty(16, dtype=torch.uint8, device="cuda"))
+    with pytest.raises(RuntimeError, match="plan of 16 bytes is too small"):
+        call(plan=torch.empty(16, dtype=torch.uint8, device="cuda"))
+    with pytest.raises(RuntimeError, match="GPU only"):
+        call(q=case.q)
+    with pytest.raises(RuntimeError, match="dtype mismatch"):
+        call(q=case.q_d.half())
+    with pytest.raises(RuntimeError, match="of 2 sequences of 1 tokens"):
+        call(q=case.q_d.repeat(1, 1, 2, 1))
+    with pytest.raises(RuntimeError, match="query heads per cache head"):
+        call(q=case.q_d.repeat(1, 3, 1, 1))
+    with pytest.raises(RuntimeError, match="int32 or int64"):
+        call(pos=case.pos_d.float())
+    with pytest.raises(RuntimeError, match="sinks must be"):
+        call(sinks=torch.zeros(3, device="cuda"))
+    with pytest.raises(RuntimeError, match="max_context"):
+        call(max_context=0)
+    with pytest.raises(RuntimeError, match="out must be like q"):
+        call(out=torch.empty(2, 4, 1, 64, dtype=BF16, device="cuda"))
+    with pytest.raises(RuntimeError, match="head_dim"):
+        ops.shared_decode_plan(case.batch_idx_d, case.pos_d, case.ids_d, case.lens_d, q_heads=4, cached_heads=2, head_dim=96,
+                               max_context=64)
+    with pytest.raises(RuntimeError, match="prefix_lens must be"):
+        ops.shared_decode_plan(case.batch_idx_d, case.pos_d, case.ids_d, case.lens_d[1:], q_heads=4, cached_heads=2, head_dim=64,
+                               max_context=64)
