@@ -1,18 +1,324 @@
 // Attention of a batch's newest tokens over the paged cache, where sequences of the batch begin with the same keys.
 //
 //   out[b, h, j] = sum over t <= p of softmax_t(scale q.k_t) v_t,   p = input_pos[b, j]
-#include "fp_common.h"
+// The softmax over a sequence's keys is two: over the prefix that its group shares and over the keys behind it, joined by
+// their maxima and sums.  Over the prefix all rows of the group - its sequences' tokens times the query heads of a cached
+// head - are the columns of one matrix product, so that a shared key is read once for up to 64 rows, not once a sequence.
+//
+// Three launches: the plan once per step, then for every layer the products and the join.
+//  * Plan (one workgroup): finds the groups, and makes tiles of up to 64 rows over one range of keys: the prefix of a group
+//    by its rows, the keys behind it by the rows of one sequence.  The tiles' keys, in units of 64, are laid end to end and
+//    cut evenly over two workgroups a CU, so a workgroup streams the same number of keys whatever the lengths are; a tile
+//    that a cut goes through leaves a partial result for each of its pieces.
+//  * Products: a workgroup of 4 wavefronts takes the pieces of its cut, one cached head.  The wavefronts have the same rows
+//    and take the stages of keys in turn, each from a ring of its own in LDS that global_load_lds fills, without a barrier:
+//      S^T = K Q^T    keys are the M rows of the matrix product and queries its columns, so a lane has the scores of
+//                     one query and a K operand read from LDS serves up to four blocks of 16 columns
+//      O^T += V^T P^T  P^T is in the B operand's layout as the scores leave the first product; V^T comes out of LDS
+//                     through the transpose read (fp32: by reading four neighbours of a row for four blocks of O^T)
+//    The states of the four wavefronts meet in LDS at the end of a piece.
+//  * Join: a row's pieces, by their maxima and sums, in 32 bits.
+#include "decode_common.h"
 
 #include <math.h>
 
 namespace {
 
+using fp_decode::fast_exp2;
+using fp_decode::kLn2;
+using fp_decode::kLog2e;
+using fp_decode::safe_max;
+
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int kMaxSequences = 4096;
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kMaxSequences = 2048;
+constexpr int kMaxRows = 1 << 20;      // B * S * heads of a group
+constexpr int kMaxContext = 1 << 21;   // with the rows: units of all tiles fit 31 bits
+constexpr int kTileRows = 64;
+constexpr int kUnit = 64;              // keys: what the cut is made of
+constexpr int kMinUnits = 2;           // a workgroup's share at least
+constexpr int kMinShared = 64;         // keys of a prefix that are worth a tile of their own
+constexpr int kSegPages = 1024;        // page ids held in LDS
+constexpr float kMaxSlack = 6.f;       // the reference point of the exponentials may lag the maximum by this much (log2)
+constexpr int kMagic = 0x5ade0001;
 
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+// ------------------------------------------------------------------------------------------------------------ plan
+// ints: header, sequences, members of the groups, workgroups, tiles
+struct Header {
+  int magic, B, S, Hq, Hc, max_batch, max_context;
+  int len;      // units a workgroup
+  int n_wg;     // workgroups that have a share
+  int n_tiles;
+  int pad[6];
+};
+struct Sequence {
+  int slot, keys;      // -1: not a slot; keys any of its tokens sees
+  int prefix_tile;     // first tile of its group, -1: shares with nobody
+  int prefix_row;      // its first row among the group's
+  int own_tile;        // first tile of the keys behind the prefix, -1: none
+  int pad[3];
+};
+struct Share {
+  int tile, offset, units, pad;  // first tile, units of it that belong to workgroups before, units to do
+};
+struct Tile {
+  int slot;            // row of the page table
+  int base;            // >= 0: a prefix, place of the group in the list of members; < 0: -1 - sequence
+  int row0, n_rows;    // of the group's or the sequence's rows
+  int t_begin, t_end;  // keys
+  int first_wg;        // workgroup of the first piece
+  int n_pieces;
+  int part;            // workspace row of the first piece's first row; piece after piece
+  int pad[3];
+};
+
+struct Layout {
+  int n_wg, max_tiles, rows;  // rows: of a sequence and cached head
+  int64_t seqs, members, shares, tiles, bytes;  // byte offsets
+  int64_t part_rows;
+};
+
+Layout layout_of(int B, int S, int Hq, int Hc) {
+  Layout l;
+  l.n_wg = 2 * fp::compute_units() / Hc;
+  if (l.n_wg < 1) l.n_wg = 1;
+  l.rows = S * (Hq / Hc);
+  // ceil(members * rows / 64) summed over groups of two or more; every sequence's own
+  l.max_tiles = static_cast<int>(static_cast<int64_t>(B) * l.rows / kTileRows + B / 2 + 1 +
+                                 static_cast<int64_t>(B) * ((l.rows + kTileRows - 1) / kTileRows));
+  l.seqs = sizeof(Header);
+  l.members = l.seqs + static_cast<int64_t>(B) * sizeof(Sequence);
+  l.shares = l.members + (static_cast<int64_t>(B) * 4 + 15) / 16 * 16;
+  l.tiles = l.shares + static_cast<int64_t>(l.n_wg) * sizeof(Share);
+  l.bytes = l.tiles + static_cast<int64_t>(l.max_tiles) * sizeof(Tile);
+  l.part_rows = 2ll * B * l.rows + static_cast<int64_t>(kTileRows) * l.n_wg;
+  return l;
+}
+
+struct PlanArgs {
+  const int64_t* batch_idx;
+  const void* input_pos;
+  int pos_i64;
+  const int32_t* ids;
+  const int32_t* lens;
+  int B, S, Hq, Hc, rows, max_batch, max_context, n_wg, max_tiles;
+  char* plan;
+  int64_t seqs, members, shares, tiles;
+};
+
+__device__ __forceinline__ int units_of(int keys) { return (keys + kUnit - 1) / kUnit; }
+
+// last i of 0 .. n - 1 with at[i] <= x (at[0] is 0)
+__device__ __forceinline__ int last_at_or_below(const int* at, int n, int x) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (at[mid] <= x) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+__global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
+  extern __shared__ int s_mem[];
+  const int Bp = (a.B + 3) & ~3;
+  int* const s_id = s_mem;             // prefix id, 0: none
+  int* const s_keys = s_id + Bp;       // keys the sequence's tokens see
+  int* const s_len = s_keys + Bp;      // its prefix length
+  int* const s_shared = s_len + Bp;    // shared keys of its group, 0: none
+  int* const s_count = s_shared + Bp;  // members, at the group's first sequence (its leader), elsewhere 0
+  int* const s_rank = s_count + Bp;    // place among the members
+  int* const s_lead = s_rank + Bp;
+  int* const s_ptile = s_lead + Bp;    // sums over the sequences before: prefix tiles, their units, members
+  int* const s_punit = s_ptile + Bp;
+  int* const s_pmem = s_punit + Bp;
+  int* const s_sunit = s_pmem + Bp;    // units of own tiles (tiles: see own_tiles)
+  int* const s_stile = s_sunit + Bp;
+  __shared__ int s_sum[16][5];
+  const int tid = threadIdx.x, n_thr = blockDim.x, lane = tid & 63, wave = tid >> 6;
+
+  for (int b = tid; b < Bp; b += n_thr) {
+    int id = 0, keys = 0, len = 0;
+    if (b < a.B) {
+      const int64_t slot = a.batch_idx[b];
+      const bool valid = slot >= 0 && slot < a.max_batch;
+      for (int j = 0; j < a.S; ++j) {
+        int64_t p = fp::load_index(a.input_pos, static_cast<int64_t>(b) * a.S + j, a.pos_i64) + 1;
+        p = p < 0 ? 0 : p > a.max_context ? a.max_context : p;
+        keys = max(keys, static_cast<int>(p));
+      }
+      if (!valid) keys = 0;
+      if (keys > 0) {
+        id = max(a.ids[slot], 0);
+        len = max(a.lens[slot], 0);
+      }
+      Sequence* const q = reinterpret_cast<Sequence*>(a.plan + a.seqs) + b;
+      q->slot = valid ? static_cast<int>(slot) : -1;
+      q->keys = keys;
+    }
+    s_id[b] = id;
+    s_keys[b] = keys;
+    s_len[b] = len;
+  }
+  __syncthreads();
+
+  // groups: every sequence looks at all of them (LDS broadcasts, four ids at a time)
+  for (int b = tid; b < a.B; b += n_thr) {
+    const int id = s_id[b];
+    int lead = b, rank = 0, count = 0, shortest = INT32_MAX, longest = 0;
+    if (id > 0) {
+      for (int j = 0; j < Bp; j += 4) {
+        const i32x4 four = *reinterpret_cast<const i32x4*>(s_id + j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (four[i] != id) continue;
+          ++count;
+          rank += j + i < b;
+          lead = min(lead, j + i);
+          shortest = min(shortest, s_len[j + i]);
+          longest = max(longest, s_keys[j + i]);
+        }
+      }
+    }
+    const int shared = count >= 2 ? min(shortest, longest) : 0;
+    const bool shares = shared >= kMinShared;
+    s_shared[b] = shares ? shared : 0;
+    s_count[b] = shares && lead == b ? count : 0;
+    s_rank[b] = rank;
+    s_lead[b] = lead;
+  }
+  __syncthreads();
+
+  // sums over the sequences before, consecutive ones a thread
+  const int own_tiles = (a.rows + kTileRows - 1) / kTileRows;
+  const int per = (a.B + n_thr - 1) / n_thr, b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
+  int x[5] = {0, 0, 0, 0, 0};
+  const auto add = [&](int b) {
+    const int c = s_count[b];
+    if (c > 0) {
+      const int n = (c * a.rows + kTileRows - 1) / kTileRows;
+      x[0] += n;
+      x[1] += n * units_of(s_shared[b]);
+      x[2] += c;
+    }
+    const int own = s_keys[b] - s_shared[b];
+    if (own > 0) {
+      x[3] += own_tiles * units_of(own);
+      x[4] += own_tiles;
+    }
+  };
+  for (int b = b0; b < b1; ++b) add(b);
+  int total[5], before[5];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) {
+    int up = x[i];
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int y = __shfl_up(up, off);
+      if (lane >= off) up += y;
+    }
+    if (lane == 63) s_sum[wave][i] = up;
+    before[i] = up - x[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 5; ++i) total[i] = 0;
+  for (int w = 0; w < n_thr / 64; ++w)
+#pragma unroll
+    for (int i = 0; i < 5; ++i) {
+      if (w < wave) before[i] += s_sum[w][i];
+      total[i] += s_sum[w][i];
+    }
+#pragma unroll
+  for (int i = 0; i < 5; ++i) x[i] = before[i];
+  for (int b = b0; b < b1; ++b) {
+    s_ptile[b] = x[0];
+    s_punit[b] = x[1];
+    s_pmem[b] = x[2];
+    s_sunit[b] = x[3];
+    s_stile[b] = x[4];
+    add(b);
+  }
+  __syncthreads();
+
+  const int p_tiles = total[0], n_tiles = p_tiles + total[4], units = total[1] + total[3];
+  const int len = max(kMinUnits, (units + a.n_wg - 1) / a.n_wg), n_wg = (units + len - 1) / len;
+  if (tid == 0) {
+    Header* const h = reinterpret_cast<Header*>(a.plan);
+    h->magic = kMagic;
+    h->B = a.B, h->S = a.S, h->Hq = a.Hq, h->Hc = a.Hc, h->max_batch = a.max_batch, h->max_context = a.max_context;
+    h->len = len, h->n_wg = n_wg, h->n_tiles = n_tiles;
+  }
+  for (int b = tid; b < a.B; b += n_thr) {
+    Sequence* const q = reinterpret_cast<Sequence*>(a.plan + a.seqs) + b;
+    const int lead = s_lead[b];
+    const bool shares = s_shared[b] > 0;
+    q->prefix_tile = shares ? s_ptile[lead] : -1;
+    q->prefix_row = shares ? s_rank[b] * a.rows : 0;
+    q->own_tile = s_keys[b] > s_shared[b] ? p_tiles + s_stile[b] : -1;
+    if (shares) reinterpret_cast<int*>(a.plan + a.members)[s_pmem[lead] + s_rank[b]] = b;
+  }
+  // workspace rows: a tile has those of the tiles before it, each once, and 64 for every cut up to its first key
+  const int64_t all_shared_rows = static_cast<int64_t>(total[2]) * a.rows;
+  for (int i = tid; i < n_tiles; i += n_thr) {
+    Tile t;
+    int n_units, from;
+    int64_t rows_before;
+    if (i < p_tiles) {
+      const int b = last_at_or_below(s_ptile, a.B, i), k = i - s_ptile[b], all = s_count[b] * a.rows;
+      n_units = units_of(s_shared[b]);
+      from = s_punit[b] + k * n_units;
+      t.base = s_pmem[b];
+      t.slot = static_cast<int>(a.batch_idx[b]);
+      t.row0 = k * kTileRows;
+      t.n_rows = min(kTileRows, all - t.row0);
+      t.t_begin = 0;
+      t.t_end = s_shared[b];
+      rows_before = static_cast<int64_t>(s_pmem[b]) * a.rows + t.row0;
+    } else {
+      const int b = last_at_or_below(s_stile, a.B, i - p_tiles), k = i - p_tiles - s_stile[b];
+      n_units = units_of(s_keys[b] - s_shared[b]);
+      from = total[1] + s_sunit[b] + k * n_units;
+      t.base = -1 - b;
+      t.slot = static_cast<int>(a.batch_idx[b]);
+      t.row0 = k * kTileRows;
+      t.n_rows = min(kTileRows, a.rows - t.row0);
+      t.t_begin = s_shared[b];
+      t.t_end = s_keys[b];
+      rows_before = all_shared_rows + static_cast<int64_t>(b) * a.rows + t.row0;
+    }
+    t.first_wg = from / len;
+    t.n_pieces = (from + n_units - 1) / len - t.first_wg + 1;
+    t.part = static_cast<int>(rows_before + static_cast<int64_t>(kTileRows) * t.first_wg);
+    t.pad[0] = t.pad[1] = t.pad[2] = 0;
+    reinterpret_cast<Tile*>(a.plan + a.tiles)[i] = t;
+  }
+  for (int w = tid; w < a.n_wg; w += n_thr) {
+    Share s{0, 0, 0, 0};
+    const int from = w * len;
+    if (w < n_wg) {
+      s.units = min(len, units - from);
+      if (from < total[1]) {
+        const int b = last_at_or_below(s_punit, a.B, from), n = units_of(s_shared[b]), off = from - s_punit[b];
+        s.tile = s_ptile[b] + off / n;
+        s.offset = off % n;
+      } else {
+        const int b = last_at_or_below(s_sunit, a.B, from - total[1]), n = units_of(s_keys[b] - s_shared[b]);
+        const int off = from - total[1] - s_sunit[b];
+        s.tile = p_tiles + s_stile[b] + off / n;
+        s.offset = off % n;
+      }
+    }
+    reinterpret_cast<Share*>(a.plan + a.shares)[w] = s;
+  }
+}
+
+// -------------------------------------------------------------------------------------------------------- products
 struct SharedArgs {
   const char* q;
   int64_t qs_b, qs_h, qs_s;  // bytes
@@ -33,59 +339,639 @@ struct SharedArgs {
   int64_t n_slots;
   int max_context;
   float qscale;  // scale * log2(e)
+  int rows, group, group_shift;  // rows of a sequence and cached head, query heads of a cached head
+  const char* plan;
+  int64_t seqs, members, shares, tiles;
+  float* ws_acc;  // [part rows, Hc, D]
+  float* ws_ml;   // [part rows, Hc, 2]
 };
 
-template <typename T>
-__device__ __forceinline__ float wave_sum(T x) {
-#pragma unroll
-  for (int off = 32; off; off >>= 1) x += __shfl_xor(x, off);
-  return x;
+struct BF16 {
+  using type = __bf16;
+  typedef __bf16 vec8 __attribute__((ext_vector_type(8)));
+  static constexpr int kBytes = 2;
+  // sets the elements of w that are infinite or NaN to 0; whether there are any
+  static __device__ __forceinline__ bool drop_infinities(uint32_t& w) {
+    const bool lo = (w & 0x7f80u) == 0x7f80u, hi = (w & 0x7f800000u) == 0x7f800000u;
+    w &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+    return lo || hi;
+  }
+  // Added to the exponents: the probabilities stay at 1 and below although the reference point lags the maximum, so that a product
+  // with the largest V of the type stays in fp32.
+  static constexpr float kHeadroom = -kMaxSlack;
+  static __device__ __forceinline__ f32x4 mfma_k32(const v4u& a, const v4u& b, const f32x4& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vec8, a), __builtin_bit_cast(vec8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x4 mfma_k16(const s16x4& a, const s16x4& b, const f32x4& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    typedef __bf16 vec2 __attribute__((ext_vector_type(2)));
+    const vec2 v = {static_cast<__bf16>(lo), static_cast<__bf16>(hi)};
+    return __builtin_bit_cast(uint32_t, v);
+  }
+  static __device__ __forceinline__ float above_zero(float p) { return p; }  // fp32's exponents: no p rounds to 0
+  static __device__ __forceinline__ float to_float(uint32_t bits) { return __uint_as_float(bits << 16); }
+  static __device__ __forceinline__ float round(float v) { return static_cast<float>(static_cast<__bf16>(v)); }
+};
+struct F16 {
+  using type = _Float16;
+  typedef _Float16 vec4 __attribute__((ext_vector_type(4)));
+  typedef _Float16 vec8 __attribute__((ext_vector_type(8)));
+  static constexpr int kBytes = 2;
+  static __device__ __forceinline__ bool drop_infinities(uint32_t& w) {
+    const bool lo = (w & 0x7c00u) == 0x7c00u, hi = (w & 0x7c000000u) == 0x7c000000u;
+    w &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+    return lo || hi;
+  }
+  // probabilities up to 2^(8 + kMaxSlack): below the largest f16, and small ones stay normal numbers longer
+  static constexpr float kHeadroom = 8.f;
+  static __device__ __forceinline__ f32x4 mfma_k32(const v4u& a, const v4u& b, const f32x4& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vec8, a), __builtin_bit_cast(vec8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x4 mfma_k16(const s16x4& a, const s16x4& b, const f32x4& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(vec4, a), __builtin_bit_cast(vec4, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    typedef _Float16 vec2 __attribute__((ext_vector_type(2)));
+    const vec2 v = {static_cast<_Float16>(lo), static_cast<_Float16>(hi)};
+    return __builtin_bit_cast(uint32_t, v);
+  }
+  // a probability that would round to 0 becomes the smallest number of the type (2^-32 of the largest), so that an infinite V
+  // element still meets something above 0
+  static __device__ __forceinline__ float above_zero(float p) { return fmaxf(p, fminf(p * 0x1p+102f, 0x1p-24f)); }
+  static __device__ __forceinline__ float to_float(uint32_t bits) {
+    return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(bits)));
+  }
+  static __device__ __forceinline__ float round(float v) { return static_cast<float>(static_cast<_Float16>(v)); }
+};
+struct F32 {
+  using type = float;
+  static constexpr int kBytes = 4;
+  static constexpr float kHeadroom = -kMaxSlack;
+  static __device__ __forceinline__ bool drop_infinities(uint32_t& w) {
+    const bool odd = (w & 0x7f800000u) == 0x7f800000u;
+    if (odd) w = 0;
+    return odd;
+  }
+  static __device__ __forceinline__ float round(float v) { return v; }
+};
+
+__device__ __forceinline__ s16x4 lds_read_tr(const char* p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p));
+}
+
+// this wavefront's staging loads but the `kLater` issued last have landed in LDS
+template <int kLater>
+__device__ __forceinline__ void wait_staged() {
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(kLater) : "memory");
+}
+
+// Stages: TS rows of K, then TS rows of V.  16-byte chunk c of K's row r sits at c ^ k_swz(r) (the score product reads one chunk of
+// 16 consecutive rows); of 16-bit V, 32-byte region c of row r at c ^ v_swz(r) (a transpose read takes one region of 16
+// rows); fp32's V is read along its rows and stays in order.
+template <typename E, int D>
+struct Geo {
+  static constexpr bool k16 = E::kBytes == 2;
+  static constexpr int ROWB = D * E::kBytes;
+  static constexpr int CPR = ROWB / 16;            // 16-byte chunks of a row
+  static constexpr int R32 = ROWB / 32;
+  static constexpr int RPI = 64 / CPR;             // rows of one load instruction
+  static constexpr int TS = ROWB == 128 ? 32 : 16;  // keys of a stage
+  static constexpr int HALF = TS * ROWB;           // bytes of a stage's K
+  static constexpr int NI = HALF / 1024;           // load instructions of a stage's K
+  static constexpr int NB = TS / 16;               // blocks of 16 keys
+  static constexpr int DB = D / 16;                // blocks of 16 rows of O^T
+  static constexpr int QV = ROWB / 64;             // 16-byte operand registers of a query row
+  static constexpr int RING = 2 * 2 * HALF;        // two stages a wavefront
+  static constexpr int PASS = RING / (16 * D * 4) < 4 ? RING / (16 * D * 4) : 4;  // column blocks whose states fit a ring
+  static __device__ __forceinline__ int k_swz(int r) { return CPR == 8 ? (r >> 1) & 7 : r & 15; }
+  static __device__ __forceinline__ int v_swz(int r) { return !k16 ? 0 : CPR == 16 ? r & 7 : (r >> 1) & 3; }
+};
+
+template <typename E>
+__device__ __forceinline__ void store4(char* p, const f32x4& v) {
+  if constexpr (E::kBytes == 4)
+    *reinterpret_cast<f32x4*>(p) = v;
+  else
+    *reinterpret_cast<uint2*>(p) = uint2{E::pack2(v[0], v[1]), E::pack2(v[2], v[3])};
+}
+
+// keys of token j of sequence b
+__device__ __forceinline__ int keys_of(const SharedArgs& a, int b, int j) {
+  const int64_t p = fp::load_index(a.input_pos, static_cast<int64_t>(b) * a.S + j, a.pos_i64) + 1;
+  return p < 0 ? 0 : p > a.max_context ? a.max_context : static_cast<int>(p);
 }
 
 template <typename E, int D>
-__global__ __launch_bounds__(kThreads) void shared_decode_simple(const SharedArgs a) {
-  constexpr int V = D / 64;
-  __shared__ float s_acc[kWaves][D], s_ml[kWaves][2];
-  const int hq = blockIdx.x, b = blockIdx.y / a.S, s = blockIdx.y % a.S, hc = hq / (a.Hq / a.Hc);
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t trow = a.batch_idx[b];
-  int64_t L = fp::load_index(a.input_pos, static_cast<int64_t>(b) * a.S + s, a.pos_i64);
-  L = L < 0 || trow < 0 || trow >= a.max_batch ? 0 : L >= a.max_context ? a.max_context : L + 1;
-  const E* q = reinterpret_cast<const E*>(a.q + b * a.qs_b + hq * a.qs_h + s * a.qs_s) + lane * V;
-  float qv[V], acc[V], m = -INFINITY, l = 0.f;
-  for (int i = 0; i < V; ++i) qv[i] = static_cast<float>(q[i]), acc[i] = 0.f;
-  for (int64_t t = wave; t < L; t += kWaves) {
+struct Shared {
+  using G = Geo<E, D>;
+  __attribute__((aligned(1024))) char ring[kWaves][G::RING];
+  int pages[kSegPages];
+  float ml[kWaves][kTileRows][2];
+  int limit[kWaves][kTileRows];  // keys of the columns' rows, each wavefront's own copy
+  int tainted;  // an element of V that is not finite was left out
+};
+
+// x, worked out again where it is used: what follows from it is not kept in registers through the loops around.
+__device__ __forceinline__ int anew(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+// The kernel's arguments (its first parameter) read again where they are used: scalar registers that carried them through the
+// loop over the keys would be spilled into vector registers.
+__device__ __forceinline__ const SharedArgs& reread() {
+  auto p = (const __attribute__((address_space(4))) SharedArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const SharedArgs*)p;
+}
+
+// Token and head of row r of a tile.
+__device__ __forceinline__ void find_row(const SharedArgs& a, const Tile& tile, int r, int* b, int* j, int* g) {
+  const uint32_t rr = tile.row0 + r;
+  uint32_t x = rr;
+  if (tile.base >= 0) {
+    const uint32_t m = rr / static_cast<uint32_t>(a.rows);
+    x = rr - m * a.rows;
+    *b = reinterpret_cast<const int*>(a.plan + a.members)[tile.base + m];
+  } else {
+    *b = -1 - tile.base;
+  }
+  *j = static_cast<int>(x >> a.group_shift);
+  *g = static_cast<int>(x & (a.group - 1));
+}
+
+// What the products left out of row r: the infinities and NaN of the V rows of keys [t0, t1) that it sees, elements 4 c .. 4 c + 3.
+template <typename E, int D>
+__device__ __forceinline__ void add_infinities(const SharedArgs& a, const Tile& tile, int r, int t0, int t1,
+                                                         const char* vplane, int c, f32x4& num) {
+  int b, j, g;
+  find_row(a, tile, r, &b, &j, &g);
+  const int end = min(t1, keys_of(a, b, j));
+  for (int t = t0; t < end; ++t) {
     int64_t blk;
     int off;
     a.pd.split(t, blk, off);
-    int64_t page = blk < a.n_pages ? a.page_table[trow * a.pt_row_stride + blk] : 0;
+    int64_t page = blk < a.n_pages ? a.page_table[static_cast<int64_t>(tile.slot) * a.pt_row_stride + blk] : 0;
     if (page < 0 || page >= a.pool_pages) page = 0;
-    const int64_t row = (static_cast<int64_t>(hc) * a.n_slots + page * a.pd.page_size + off) * D + lane * V;
-    float x = 0.f;
-    for (int i = 0; i < V; ++i) x += qv[i] * static_cast<float>(reinterpret_cast<const E*>(a.pool_k)[row + i]);
-    x = wave_sum(x) * a.qscale;
-    const float mn = fmaxf(m, x), ms = mn == -INFINITY ? 0.f : mn;
-    const float keep = exp2f(m - ms), p = exp2f(x - ms);
-    l = l * keep + p;
-    for (int i = 0; i < V; ++i) acc[i] = acc[i] * keep + p * static_cast<float>(reinterpret_cast<const E*>(a.pool_v)[row + i]);
-    m = mn;
+    const char* const at = vplane + ((page * a.pd.page_size + off) * D + c * 4) * E::kBytes;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float v = static_cast<float>(reinterpret_cast<const typename E::type*>(at)[k]);
+      if (!(fabsf(v) < INFINITY)) num[k] += v;
+    }
   }
-  for (int i = 0; i < V; ++i) s_acc[wave][lane * V + i] = acc[i];
-  if (lane == 0) s_ml[wave][0] = m, s_ml[wave][1] = l;
-  __syncthreads();
-  float mn = -INFINITY, den = 0.f;
-  for (int w = 0; w < kWaves; ++w) mn = fmaxf(mn, s_ml[w][0]);
-  const float ms = mn == -INFINITY ? 0.f : mn;
-  for (int w = 0; w < kWaves; ++w) den += s_ml[w][1] * exp2f(s_ml[w][0] - ms);
-  const float lse = (mn + log2f(den)) * kLn2;
-  for (int d = threadIdx.x; d < D; d += kThreads) {
-    float num = 0.f;
-    for (int w = 0; w < kWaves; ++w) num += s_acc[w][d] * exp2f(s_ml[w][0] - ms);
-    float o = L == 0 ? 0.f : num / den;
-    if (a.sinks && L > 0) o = static_cast<float>(static_cast<E>(o)) / (1.f + expf(a.sinks[hq] - lse));
-    reinterpret_cast<E*>(a.out + b * a.os_b + hq * a.os_h + s * a.os_s)[d] = static_cast<E>(o);
+}
+
+// One piece: the rows of a tile over its keys [t0, t1).  CB blocks of 16 columns; kSplit: at most 8 rows, in columns 0 .. 7 and again in
+// 8 .. 15, whose probabilities carry what the rounding of the first left over.
+template <typename E, int D, int CB, bool kSplit>
+__device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh, const Tile& tile, const int piece, const int t0,
+                                          const int t1) {
+  using G = Geo<E, D>;
+  const int tid = anew(threadIdx.x), lane = tid & 63, hc = blockIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, grp = lane >> 4;
+  const bool prefix = tile.base >= 0;
+  char* const ring = sh.ring[wave];
+  const char* const kplane = a.pool_k + static_cast<int64_t>(hc) * a.n_slots * G::ROWB;
+  const char* const vplane = a.pool_v + static_cast<int64_t>(hc) * a.n_slots * G::ROWB;
+  const int64_t* const table = a.page_table + static_cast<int64_t>(tile.slot) * a.pt_row_stride;
+
+  // rows: query operands and limits of this lane's columns.  A column without a row repeats row 0, sees everything and is not stored.
+  v4u q[CB][G::QV];
+  int least = INT32_MAX;
+#pragma unroll
+  for (int cb = 0; cb < CB; ++cb) {
+    const SharedArgs& a = reread();
+    const int r = kSplit ? col & 7 : cb * 16 + col;
+    const bool on = r < tile.n_rows;
+    int b, j, g;
+    find_row(a, tile, on ? r : 0, &b, &j, &g);
+    const int h = hc * a.group + g;
+    const int lim = on ? keys_of(a, b, j) : INT32_MAX;
+    least = min(least, lim);
+    if (grp == 0) sh.limit[wave][cb * 16 + col] = lim;
+    const char* const src = a.q + b * a.qs_b + h * a.qs_h + j * a.qs_s + grp * 16;
+#pragma unroll
+    for (int kk = 0; kk < G::QV; ++kk) q[cb][kk] = *reinterpret_cast<const v4u*>(src + kk * 64);
   }
-  if (threadIdx.x == 0) a.lse[(static_cast<int64_t>(b) * a.Hq + hq) * a.S + s] = L == 0 ? -INFINITY : lse;
+  least = -fp::wave_max(-least);
+  if (tid == 0) sh.tainted = 0;  // ahead of the barriers of the first segment
+
+  f32x4 o[CB][G::DB];
+  float m[CB], l[CB];
+#pragma unroll
+  for (int cb = 0; cb < CB; ++cb) {
+    m[cb] = -INFINITY;
+    l[cb] = 0.f;
+#pragma unroll
+    for (int db = 0; db < G::DB; ++db) o[cb][db] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // byte offset inside row r of a stage of what goes to position p of the row
+  const auto k_off = [](int p, int r) { return static_cast<uint32_t>((p ^ G::k_swz(r)) * 16); };
+  const auto v_off = [](int p, int r) {
+    return static_cast<uint32_t>(G::k16 ? (p ^ G::v_swz(r) * 2) * 16 : p * 16);
+  };
+  const bool aligned_pages = a.pd.shift >= 0 && a.pd.page_size % G::TS == 0;
+
+  for (int seg0 = t0; seg0 < t1;) {
+    int64_t blk0;
+    int off0, seg1 = t1;
+    a.pd.split(seg0, blk0, off0);
+    {
+      const int64_t room = (blk0 + kSegPages) * a.pd.page_size - seg0;
+      if (room < t1 - seg0) seg1 = seg0 + static_cast<int>(room) / (kWaves * G::TS) * (kWaves * G::TS);
+      int64_t last;
+      int unused;
+      a.pd.split(seg1 - 1, last, unused);
+      __syncthreads();  // the page ids before are no longer read
+      for (int i = tid; i <= static_cast<int>(last - blk0); i += kThreads) {
+        int64_t page = 0;
+        if (blk0 + i < a.n_pages) page = table[blk0 + i];
+        if (page < 0 || page >= a.pool_pages) page = 0;  // as paged_decode: the reserved page
+        sh.pages[i] = static_cast<int>(page);
+      }
+      __syncthreads();
+    }
+
+    const auto issue = [&](int c0, char* stage) {
+      const int at_lane = anew(lane), lrow = at_lane / G::CPR, lpos = at_lane % G::CPR;
+      if (aligned_pages && c0 % G::TS == 0 && c0 + G::TS <= seg1) {
+        const int page = __builtin_amdgcn_readfirstlane(sh.pages[(c0 >> a.pd.shift) - static_cast<int>(blk0)]);
+        const int64_t slot = static_cast<int64_t>(page) * a.pd.page_size + (c0 & (a.pd.page_size - 1));
+        if (prefix) {  // other tiles read these rows, too
+#pragma unroll
+          for (int i = 0; i < G::NI; ++i) fp::load_to_lds(kplane + slot * G::ROWB, (i * G::RPI + lrow) * G::ROWB + k_off(lpos, i * G::RPI + lrow), stage + i * 1024);
+#pragma unroll
+          for (int i = 0; i < G::NI; ++i)
+            fp::load_to_lds(vplane + slot * G::ROWB, (i * G::RPI + lrow) * G::ROWB + v_off(lpos, i * G::RPI + lrow), stage + G::HALF + i * 1024);
+        } else {
+#pragma unroll
+          for (int i = 0; i < G::NI; ++i) fp::load_to_lds_nt(kplane + slot * G::ROWB, (i * G::RPI + lrow) * G::ROWB + k_off(lpos, i * G::RPI + lrow), stage + i * 1024);
+#pragma unroll
+          for (int i = 0; i < G::NI; ++i)
+            fp::load_to_lds_nt(vplane + slot * G::ROWB, (i * G::RPI + lrow) * G::ROWB + v_off(lpos, i * G::RPI + lrow), stage + G::HALF + i * 1024);
+        }
+      } else {  // pages that do not hold whole stages, the last keys: row by row.  A row past the range repeats its last one and is masked
+#pragma nounroll
+        for (int i = 0; i < G::NI; ++i) {  // one at a time: their addresses would be registers of the whole loop
+          const int r = i * G::RPI + lrow;
+          const int t = min(c0 + r, seg1 - 1);
+          int64_t blk;
+          int off;
+          a.pd.split(t, blk, off);
+          const int64_t at = (static_cast<int64_t>(sh.pages[blk - blk0]) * a.pd.page_size + off) * G::ROWB;
+          fp::load_to_lds(kplane + at + k_off(lpos, r), stage + i * 1024);
+          fp::load_to_lds(vplane + at + v_off(lpos, r), stage + G::HALF + i * 1024);
+        }
+      }
+    };
+
+    // stages wave, wave + 4, ... of the segment
+    const int n_stages = (seg1 - seg0 + G::TS - 1) / G::TS;
+    if (wave < n_stages) issue(seg0 + wave * G::TS, ring);
+    if (wave + kWaves < n_stages) issue(seg0 + (wave + kWaves) * G::TS, ring + 2 * G::HALF);
+#pragma nounroll
+    for (int s = wave, buf = 0; s < n_stages; s += kWaves, buf ^= 1) {
+      const int c0 = seg0 + s * G::TS;
+      char* const k_lds = ring + buf * 2 * G::HALF;
+      char* const v_lds = k_lds + G::HALF;
+      if (s + kWaves < n_stages) wait_staged<2 * G::NI>(); else wait_staged<0>();
+      // scores of this lane's columns: keys 16 * blk + 4 * grp + 0 .. 3
+      f32x4 sc[CB][G::NB];
+      const int lane_now = anew(lane);
+#pragma unroll
+      for (int blk = 0; blk < G::NB; ++blk) {
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) sc[cb][blk] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const int r = blk * 16 + (lane_now & 15);
+        const uint32_t at = r * G::ROWB + ((lane_now >> 4) ^ G::k_swz(r)) * 16;
+#pragma unroll
+        for (int kk = 0; kk < G::QV; ++kk) {
+          const v4u ka = *reinterpret_cast<const v4u*>(k_lds + (at ^ (kk * 64)));
+#pragma unroll
+          for (int cb = 0; cb < CB; ++cb) {
+            if constexpr (G::k16) {
+              sc[cb][blk] = E::mfma_k32(ka, q[cb][kk], sc[cb][blk]);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                sc[cb][blk] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(ka[e]), __uint_as_float(q[cb][kk][e]), sc[cb][blk], 0, 0, 0);
+            }
+          }
+        }
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) sc[cb][blk] *= a.qscale;
+      }
+      if (c0 + G::TS > min(seg1, least)) {
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) {
+          const int end = min(sh.limit[wave][cb * 16 + col], seg1);
+#pragma unroll
+          for (int blk = 0; blk < G::NB; ++blk)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (c0 + blk * 16 + grp * 4 + j >= end) sc[cb][blk][j] = -INFINITY;
+        }
+        // V rows past the range become 0: a probability of 0 against an infinity would be NaN.  So do the elements that are not
+        // finite of rows which only some columns see; these columns get them at the end.
+#pragma nounroll
+        for (int i = 0; i < G::NI; ++i) {
+          const int t = c0 + i * G::RPI + anew(lane) / G::CPR;
+          if (t < least) continue;
+          v4u* const at = reinterpret_cast<v4u*>(v_lds + i * 1024 + lane * 16);
+          v4u w = {0, 0, 0, 0};
+          if (t < seg1) {
+            w = *at;
+            bool odd = false;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t two = w[c];
+              odd |= E::drop_infinities(two);
+              w[c] = two;
+            }
+            if (!odd) continue;
+            sh.tainted = 1;
+          }
+          *at = w;
+        }
+        asm volatile("" : : : "memory");  // a wavefront's LDS instructions are executed in order
+      }
+      // Reference point of the exponentials, per column: moves only when the column's maximum has outgrown it by kMaxSlack, so most
+      // stages need no exchange between the lanes of a column and no rescale.
+      float cand[CB];
+      bool grown = false;
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb) {
+        cand[cb] = sc[cb][0][0];
+#pragma unroll
+        for (int blk = 0; blk < G::NB; ++blk)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) cand[cb] = fmaxf(cand[cb], sc[cb][blk][j]);
+        grown |= cand[cb] > m[cb] + (E::kHeadroom + kMaxSlack);
+      }
+      if (__any(grown)) {
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) {
+          cand[cb] = fmaxf(cand[cb], __shfl_xor(cand[cb], 16));
+          cand[cb] = fmaxf(cand[cb], __shfl_xor(cand[cb], 32));
+          if (cand[cb] > m[cb] + (E::kHeadroom + kMaxSlack)) {
+            const float m_new = cand[cb] - E::kHeadroom, alpha = fast_exp2(m[cb] - m_new);
+            l[cb] *= alpha;
+#pragma unroll
+            for (int db = 0; db < G::DB; ++db) o[cb][db] *= alpha;
+            m[cb] = m_new;
+          }
+        }
+      }
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb) {
+        const float ms = safe_max(m[cb]);  // no key above -inf so far: its probabilities are 0
+#pragma unroll
+        for (int blk = 0; blk < G::NB; ++blk)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            sc[cb][blk][j] = fast_exp2(sc[cb][blk][j] - ms);
+            l[cb] += sc[cb][blk][j];
+          }
+      }
+      if constexpr (G::k16) {
+#pragma unroll
+        for (int blk = 0; blk < G::NB; ++blk) {
+          s16x4 pb[CB];
+#pragma unroll
+          for (int cb = 0; cb < CB; ++cb) {
+            uint32_t w[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const float p0 = sc[cb][blk][2 * j], p1 = sc[cb][blk][2 * j + 1];
+              w[j] = E::pack2(E::above_zero(p0), E::above_zero(p1));
+              if constexpr (kSplit) {
+                const uint32_t rest = E::pack2(p0 - E::to_float(w[j] & 0xffffu), p1 - E::to_float(w[j] >> 16));
+                if (col >= 8) w[j] = rest;
+              }
+            }
+            pb[cb] = __builtin_bit_cast(s16x4, uint2{w[0], w[1]});
+          }
+          // lanes 4 j + c of a 16-lane block name elements 4 c .. of key 4 * grp + j and receive element `col` of the four keys
+          const int r = blk * 16 + (lane_now >> 4) * 4 + ((lane_now & 15) >> 2);
+          const uint32_t at = r * G::ROWB + G::v_swz(r) * 32 + (lane_now & 3) * 8;
+#pragma unroll
+          for (int db = 0; db < G::DB; ++db) {
+            const s16x4 va = lds_read_tr(v_lds + (at ^ (db * 32)));
+#pragma unroll
+            for (int cb = 0; cb < CB; ++cb) o[cb][db] = E::mfma_k16(va, pb[cb], o[cb][db]);
+          }
+        }
+      } else {
+        // element e of four neighbours of a V row is the operand of block e of O^T: row i of block 4 h + e is d = 64 h + 4 i + e
+#pragma unroll
+        for (int blk = 0; blk < G::NB; ++blk)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int r = blk * 16 + (lane_now >> 4) * 4 + j;
+#pragma unroll
+            for (int h = 0; h < D / 64; ++h) {
+              const f32x4 va = *reinterpret_cast<const f32x4*>(v_lds + r * G::ROWB + h * 256 + (lane_now & 15) * 16);
+#pragma unroll
+              for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  o[cb][4 * h + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(va[e], sc[cb][blk][j], o[cb][4 * h + e], 0, 0, 0);
+            }
+          }
+      }
+      if (s + 2 * kWaves < n_stages) {
+        asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // every operand of this stage has left LDS
+        issue(c0 + 2 * kWaves * G::TS, ring + buf * 2 * G::HALF);
+      }
+    }
+    seg0 = seg1;
+  }
+
+  // The wavefronts' states meet in LDS, PASS column blocks at a time, chunks permuted against bank conflicts.
+#pragma unroll
+  for (int cb = 0; cb < CB; ++cb) {
+    if constexpr (kSplit) {
+      // both halves of the columns together.  Against an infinite V element what rounding left over is 0 or negative, and the sum would
+      // be NaN: the upper half stands.
+#pragma unroll
+      for (int db = 0; db < G::DB; ++db)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float rest = fp_decode::dpp<0x128>(o[cb][db][j]);  // row_ror:8, lane ^ 8
+          if ((__float_as_uint(o[cb][db][j]) & 0x7f800000u) != 0x7f800000u) o[cb][db][j] += rest;
+        }
+    }
+    l[cb] += __shfl_xor(l[cb], 16);
+    l[cb] += __shfl_xor(l[cb], 32);
+    if (grp == 0) {
+      sh.ml[wave][cb * 16 + col][0] = m[cb];
+      sh.ml[wave][cb * 16 + col][1] = l[cb];
+    }
+  }
+  const SharedArgs& e = reread();
+  const bool sole = !prefix && tile.n_pieces == 1 && tile.t_begin == 0;  // nothing to join: the result itself
+  constexpr int C4 = D / 4;  // 16-byte chunks of a row of O
+#pragma unroll
+  for (int cb0 = 0; cb0 < CB; cb0 += G::PASS) {
+    if (cb0 > 0) __syncthreads();  // the pass before has been read
+#pragma unroll
+    for (int i = 0; i < G::PASS && cb0 + i < CB; ++i) {
+      const int cb = cb0 + i;
+      f32x4* const acc = reinterpret_cast<f32x4*>(ring) + (i * 16 + col) * C4;
+#pragma unroll
+      for (int db = 0; db < G::DB; ++db) {
+        if constexpr (G::k16) {
+          acc[(db * 4 + grp) ^ col] = o[cb][db];
+        } else if (db % 4 == 0) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            acc[(db * 4 + grp * 4 + j) ^ col] = f32x4{o[cb][db][j], o[cb][db + 1][j], o[cb][db + 2][j], o[cb][db + 3][j]};
+        }
+      }
+    }
+    __syncthreads();
+    constexpr int kRows = G::PASS < CB ? G::PASS * 16 : CB * 16;
+    for (int i = tid; i < kRows * C4; i += kThreads) {
+      const int row = i / C4, c = i % C4, r = cb0 * 16 + row;
+      if (r >= tile.n_rows) break;
+      float mn = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) mn = fmaxf(mn, sh.ml[w][r][0]);
+      const float ms = safe_max(mn);
+      f32x4 num = {0.f, 0.f, 0.f, 0.f};
+      float den = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float wgt = fast_exp2(sh.ml[w][r][0] - ms);
+        num += reinterpret_cast<const f32x4*>(sh.ring[w])[row * C4 + (c ^ (row & 15))] * wgt;
+        den += sh.ml[w][r][1] * wgt;
+      }
+      if (sh.tainted) add_infinities<E, D>(e, tile, r, max(t0, least), t1, e.pool_v + static_cast<int64_t>(hc) * e.n_slots * G::ROWB, c, num);
+      if (sole) {
+        const int b = -1 - tile.base, x = tile.row0 + r, j = x >> e.group_shift, h = hc * e.group + (x & (e.group - 1));
+        const bool any = keys_of(e, b, j) > 0;
+        const float lse = (mn + log2f(den)) * kLn2;
+        f32x4 res;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) res[k] = any ? fp_decode::sink_gate<E>(num[k] / den, lse, e.sinks, h) : 0.f;
+        store4<E>(e.out + b * e.os_b + h * e.os_h + j * e.os_s + c * 4 * E::kBytes, res);
+        if (c == 0) e.lse[(static_cast<int64_t>(b) * e.Hq + h) * e.S + j] = any ? lse : -INFINITY;
+      } else {
+        const int64_t p = (static_cast<int64_t>(tile.part) + static_cast<int64_t>(piece) * tile.n_rows + r) * e.Hc + hc;
+        *reinterpret_cast<f32x4*>(e.ws_acc + p * D + c * 4) = num;
+        if (c == 0) *reinterpret_cast<float2*>(e.ws_ml + p * 2) = float2{mn, den};
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ bool plan_fits(const SharedArgs& a, const Header& h) {
+  return h.magic == kMagic && h.B == a.B && h.S == a.S && h.Hq == a.Hq && h.Hc == a.Hc && h.max_batch == a.max_batch &&
+         h.max_context == a.max_context;
+}
+
+// A record of the plan, which no launch that reads it writes: scalar loads.
+template <typename T>
+__device__ __forceinline__ T load_record(const char* p) {
+  typedef const __attribute__((address_space(4))) int* ints;
+  const ints from = (ints)p;
+  T t;
+  int* const to = reinterpret_cast<int*>(&t);
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(T) / 4); ++i) to[i] = from[i];
+  return t;
+}
+
+template <typename E, int D>
+__global__ __launch_bounds__(kThreads, (sizeof(Shared<E, D>) <= 80 * 1024 ? 2 : 1)) void shared_products_kernel(const SharedArgs a) {
+  __shared__ Shared<E, D> sh;
+  const int w = blockIdx.y;
+  const Header h = load_record<Header>(a.plan);
+  const Share share = load_record<Share>(a.plan + a.shares + w * static_cast<int64_t>(sizeof(Share)));
+  if (!plan_fits(a, h) || w >= h.n_wg) return;
+  int left = share.units, offset = share.offset;
+  for (int i = share.tile; left > 0 && i < h.n_tiles; ++i, offset = 0) {
+    const Tile t = load_record<Tile>(a.plan + a.tiles + i * static_cast<int64_t>(sizeof(Tile)));
+    const int units = min(left, units_of(t.t_end - t.t_begin) - offset);
+    const int t0 = t.t_begin + offset * kUnit, t1 = min(t.t_end, t0 + units * kUnit), piece = w - t.first_wg;
+    if (i != share.tile) __syncthreads();  // the piece before has left LDS
+    if (Geo<E, D>::k16 && t.n_rows <= 8)
+      run_piece<E, D, 1, Geo<E, D>::k16>(a, sh, t, piece, t0, t1);
+    else if (t.n_rows <= 16)
+      run_piece<E, D, 1, false>(a, sh, t, piece, t0, t1);
+    else if (t.n_rows <= 32)
+      run_piece<E, D, 2, false>(a, sh, t, piece, t0, t1);
+    else
+      run_piece<E, D, 4, false>(a, sh, t, piece, t0, t1);
+    left -= units;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------ join
+// D / 4 lanes a row.
+template <typename E, int D>
+__global__ __launch_bounds__(kThreads) void shared_join_kernel(const SharedArgs a) {
+  constexpr int LPR = D / 4;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / LPR) + threadIdx.x / LPR;
+  const int c = threadIdx.x % LPR;
+  if (row >= static_cast<int64_t>(a.B) * a.S * a.Hq) return;
+  const int h = static_cast<int>(row % a.Hq);
+  const int64_t bj = row / a.Hq;
+  const int b = static_cast<int>(bj / a.S), j = static_cast<int>(bj % a.S);
+  const Header head = *reinterpret_cast<const Header*>(a.plan);
+  const bool fits = plan_fits(a, head);
+  const Sequence s = reinterpret_cast<const Sequence*>(a.plan + a.seqs)[b];
+  const int keys = keys_of(a, b, j);
+  const int64_t slot = a.batch_idx[b];
+  const bool valid = slot >= 0 && slot < a.max_batch;
+  f32x4 res = {0.f, 0.f, 0.f, 0.f};
+  float lse = -INFINITY;
+  if (!fits || (valid && (s.slot != slot || keys > s.keys)) || (!valid && s.slot >= 0)) {
+    lse = NAN;  // the plan is of another step
+    res = f32x4{NAN, NAN, NAN, NAN};
+  } else if (valid && keys > 0) {
+    const Tile* const tiles = reinterpret_cast<const Tile*>(a.plan + a.tiles);
+    const int hc = h >> a.group_shift, x = (j << a.group_shift) + (h & (a.group - 1));
+    float m = -INFINITY, den = 0.f;
+    f32x4 num = {0.f, 0.f, 0.f, 0.f};
+    const auto join = [&](const Tile& t, int r) {
+      for (int k = 0; k < t.n_pieces; ++k) {
+        const int64_t p = (static_cast<int64_t>(t.part) + static_cast<int64_t>(k) * t.n_rows + r) * a.Hc + hc;
+        const float2 ml = *reinterpret_cast<const float2*>(a.ws_ml + p * 2);
+        const f32x4 acc = *reinterpret_cast<const f32x4*>(a.ws_acc + p * D + c * 4);
+        const float mn = fmaxf(m, ml.x), ms = safe_max(mn), keep = fast_exp2(m - ms), w = fast_exp2(ml.x - ms);
+        den = den * keep + ml.y * w;
+        num = num * keep + acc * w;
+        m = mn;
+      }
+    };
+    if (s.prefix_tile >= 0) {
+      const int rr = s.prefix_row + x;
+      join(tiles[s.prefix_tile + rr / kTileRows], rr % kTileRows);
+    }
+    if (s.own_tile >= 0) {
+      const Tile t = tiles[s.own_tile + x / kTileRows];
+      if (s.prefix_tile < 0 && t.n_pieces == 1) return;  // stored already
+      join(t, x % kTileRows);
+    }
+    lse = (m + log2f(den)) * kLn2;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) res[k] = fp_decode::sink_gate<E>(num[k] / den, lse, a.sinks, h);
+  }
+  store4<E>(a.out + b * a.os_b + h * a.os_h + j * a.os_s + c * 4 * E::kBytes, res);
+  if (c == 0) a.lse[(static_cast<int64_t>(b) * a.Hq + h) * a.S + j] = lse;
+}
+
+template <typename E, int D>
+void launch(const SharedArgs& a, int n_wg, hipStream_t st) {
+  hipLaunchKernelGGL((shared_products_kernel<E, D>), dim3(a.Hc, n_wg), dim3(kThreads), 0, st, a);
+  const int64_t rows = static_cast<int64_t>(a.B) * a.S * a.Hq, per = kThreads / (D / 4);
+  hipLaunchKernelGGL((shared_join_kernel<E, D>), dim3(static_cast<unsigned>((rows + per - 1) / per)), dim3(kThreads), 0, st, a);
 }
 
 int check_shape(const char* what, int B, int S, int Hq, int Hc, int D) {
@@ -95,8 +981,9 @@ int check_shape(const char* what, int B, int S, int Hq, int Hc, int D) {
   if (D != 64 && D != 128) return fp::fail(FP_ERR_UNSUPPORTED, "%s: head_dim %d (64 or 128)", what, D);
   if (G != 1 && G != 2 && G != 4 && G != 8)
     return fp::fail(FP_ERR_UNSUPPORTED, "%s: %d query heads per cache head (1, 2, 4 or 8)", what, G);
-  if (B > kMaxSequences || S > 1024)
-    return fp::fail(FP_ERR_UNSUPPORTED, "%s: at most %d sequences of 1024 tokens (got %d of %d)", what, kMaxSequences, B, S);
+  if (B > kMaxSequences || static_cast<int64_t>(B) * S * G > kMaxRows)
+    return fp::fail(FP_ERR_UNSUPPORTED, "%s: at most %d sequences and %d rows a cached head (got %d of %d tokens, %d heads)", what,
+                    kMaxSequences, kMaxRows, B, S, G);
   return FP_OK;
 }
 
@@ -104,12 +991,12 @@ int check_shape(const char* what, int B, int S, int Hq, int Hc, int D) {
 
 extern "C" int64_t fp_shared_decode_plan_bytes(int32_t B, int32_t S, int32_t Hq, int32_t Hc, int32_t D) {
   if (const int rc = check_shape("fp_shared_decode_plan_bytes", B, S, Hq, Hc, D)) return rc;
-  return 64;
+  return layout_of(B, S, Hq, Hc).bytes;
 }
 
 extern "C" int64_t fp_shared_decode_workspace_bytes(int32_t B, int32_t S, int32_t Hq, int32_t Hc, int32_t D) {
   if (const int rc = check_shape("fp_shared_decode_workspace_bytes", B, S, Hq, Hc, D)) return rc;
-  return 64;
+  return layout_of(B, S, Hq, Hc).part_rows * Hc * (D + 2) * static_cast<int64_t>(sizeof(float));
 }
 
 extern "C" int fp_shared_decode_plan(const int64_t* batch_idx, const void* input_pos, int pos_index_type,
@@ -120,6 +1007,8 @@ extern "C" int fp_shared_decode_plan(const int64_t* batch_idx, const void* input
   if (const int rc = check_shape(what, B, S, Hq, Hc, D)) return rc;
   if (max_batch <= 0 || max_context <= 0)
     return fp::fail(FP_ERR_INVALID_ARGUMENT, "%s: max_batch %d, max_context %d", what, max_batch, max_context);
+  if (max_context > kMaxContext)
+    return fp::fail(FP_ERR_UNSUPPORTED, "%s: max_context %d, at most %d", what, max_context, kMaxContext);
   if (pos_index_type != FP_INDEX_I32 && pos_index_type != FP_INDEX_I64)
     return fp::fail(FP_ERR_INVALID_ARGUMENT, "%s: pos_index_type %d", what, pos_index_type);
   if (B == 0) return FP_OK;
@@ -128,8 +1017,19 @@ extern "C" int fp_shared_decode_plan(const int64_t* batch_idx, const void* input
   if (plan_bytes < fp_shared_decode_plan_bytes(B, S, Hq, Hc, D) || !fp::aligned(plan, 16))
     return fp::fail(FP_ERR_WORKSPACE, "%s: the plan needs %lld bytes, 16-byte aligned (got %lld)", what,
                     static_cast<long long>(fp_shared_decode_plan_bytes(B, S, Hq, Hc, D)), static_cast<long long>(plan_bytes));
-  (void)stream;
-  return FP_OK;
+  const Layout l = layout_of(B, S, Hq, Hc);
+  const PlanArgs a{batch_idx, input_pos, pos_index_type, prefix_ids, prefix_lens, B, S, Hq, Hc, l.rows, max_batch, max_context,
+                   l.n_wg, l.max_tiles, static_cast<char*>(plan), l.seqs, l.members, l.shares, l.tiles};
+  int threads = (B + 63) / 64 * 64;
+  threads = threads < 256 ? 256 : threads > 1024 ? 1024 : threads;
+  const size_t lds = 12 * static_cast<size_t>((B + 3) & ~3) * sizeof(int);
+  if (lds > 64 * 1024) {
+    static const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(shared_plan_kernel),
+                                                          hipFuncAttributeMaxDynamicSharedMemorySize, 12 * kMaxSequences * sizeof(int));
+    if (allowed != hipSuccess) return fp::fail(FP_ERR_LAUNCH, "%s: %s", what, hipGetErrorString(allowed));
+  }
+  hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3(threads), lds, static_cast<hipStream_t>(stream), a);
+  return fp::check_launch(what);
 }
 
 extern "C" int fp_paged_decode_shared(const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_s,
@@ -149,6 +1049,8 @@ extern "C" int fp_paged_decode_shared(const void* q, int64_t q_stride_b, int64_t
       n_slots / page_size > INT32_MAX)
     return fp::fail(FP_ERR_INVALID_ARGUMENT, "%s: bad sizes (page_size=%d n_pages=%d max_batch=%d n_slots=%lld max_context=%d)",
                     what, page_size, n_pages, max_batch, static_cast<long long>(n_slots), max_context);
+  if (max_context > kMaxContext)
+    return fp::fail(FP_ERR_UNSUPPORTED, "%s: max_context %d, at most %d", what, max_context, kMaxContext);
   if (pos_index_type != FP_INDEX_I32 && pos_index_type != FP_INDEX_I64)
     return fp::fail(FP_ERR_INVALID_ARGUMENT, "%s: pos_index_type %d", what, pos_index_type);
   if (B == 0) return FP_OK;
@@ -164,25 +1066,28 @@ extern "C" int fp_paged_decode_shared(const void* q, int64_t q_stride_b, int64_t
   if (!workspace || workspace_bytes < need || !fp::aligned(workspace, 16))
     return fp::fail(FP_ERR_WORKSPACE, "%s: workspace of %lld bytes, 16-byte aligned, is needed (got %lld)", what,
                     static_cast<long long>(need), static_cast<long long>(workspace_bytes));
+  const Layout l = layout_of(B, S, Hq, Hc);
+  const int G = Hq / Hc;
+  float* const acc = static_cast<float*>(workspace);
   const SharedArgs a{static_cast<const char*>(q), q_stride_b * e, q_stride_h * e, q_stride_s * e,
                      static_cast<const char*>(pool_k), static_cast<const char*>(pool_v), page_table, pt_row_stride, batch_idx,
                      input_pos, pos_index_type, static_cast<char*>(out), out_stride_b * e, out_stride_h * e, out_stride_s * e,
                      lse, sinks, B, S, Hq, Hc, fp::PageDiv(page_size), n_pages, max_batch,
-                     static_cast<int>(n_slots / page_size), n_slots, max_context, scale * kLog2e};
-  const dim3 grid(Hq, B * S), block(kThreads);
+                     static_cast<int>(n_slots / page_size), n_slots, max_context, scale * kLog2e, l.rows, G, fp::log2_exact(G),
+                     static_cast<const char*>(plan), l.seqs, l.members, l.shares, l.tiles, acc, acc + l.part_rows * Hc * D};
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const auto go = [&](auto element) {
     using E = decltype(element);
     if (D == 64)
-      hipLaunchKernelGGL((shared_decode_simple<E, 64>), grid, block, 0, st, a);
+      launch<E, 64>(a, l.n_wg, st);
     else
-      hipLaunchKernelGGL((shared_decode_simple<E, 128>), grid, block, 0, st, a);
+      launch<E, 128>(a, l.n_wg, st);
   };
   if (dtype == FP_DTYPE_F32)
-    go(float{});
+    go(F32{});
   else if (dtype == FP_DTYPE_BF16)
-    go(__bf16{});
+    go(BF16{});
   else
-    go(_Float16{});
+    go(F16{});
   return fp::check_launch(what);
 }

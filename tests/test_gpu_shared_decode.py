@@ -181,3 +181,106 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="prefix_lens must be"):
         ops.shared_decode_plan(case.batch_idx_d, case.pos_d, case.ids_d, case.lens_d[1:], q_heads=4, cached_heads=2, head_dim=64,
                                max_context=64)
+
+
+def test_a_plan_serves_all_layers_and_another_steps_plan_gives_nan():
+    case = SharedBatch(25, [100], one_each([0, 0, -1, 0], [20, 90, 33, 4]), Hq=4, Hc=2, D=128, P=64, dtype=BF16).on()
+    shape = dict(q_heads=4, cached_heads=2, head_dim=128, max_context=case.columns * 64)
+    plan = ops.shared_decode_plan(case.batch_idx_d, case.pos_d, case.ids_d, case.lens_d, **shape)
+    want = case.call(ops)
+    ws = torch.empty(ops.shared_decode_workspace_bytes(4, 1, q_heads=4, cached_heads=2, head_dim=128), dtype=torch.uint8, device="cuda")
+    for _ in range(3):
+        got = case.call(ops, plan=plan, workspace=ws)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    # one sequence has moved on: its row is NaN, the others' are what they are
+    later = case.pos_d.clone()
+    later[1] += 1
+    got = case.call(ops, plan=plan, pos=later)
+    assert got[0][1].isnan().all() and got[1][1].isnan().all()
+    keep = [0, 2, 3]
+    assert torch.equal(got[0][keep], want[0][keep])
+    # a plan of another limit, and memory that holds none
+    for other in (ops.shared_decode_plan(case.batch_idx_d, case.pos_d, case.ids_d, case.lens_d, **{**shape, "max_context": 7}),
+                  torch.zeros_like(plan)):
+        got = case.call(ops, plan=other)
+        assert got[0].isnan().all() and got[1].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+def test_values_hidden_from_some_rows(value, dtype):
+    """A V row (and a K row) that is not finite reaches the tokens that see its key and no other."""
+    seqs = [(0, 20, 20), (0, 7, 3), (-1, 90, 15)]
+    case = SharedBatch(26, [130], seqs, Hq=8, Hc=2, D=64, P=64, dtype=dtype, S=20).on()
+    want = case.call(ops)
+    case.check(want)
+    # the key of token 11 of sequence 0 and of token 4 of sequence 2
+    for b, t in ((0, 130 + 11), (2, 75 + 4)):
+        page = int(case.table[case.batch_idx[b], t // 64])
+        case.pool_d[1][1, page * 64 + t % 64, 5] = value
+    got = case.call(ops)
+    touched = torch.zeros_like(want[0], dtype=torch.bool)
+    touched[0, 4:, 11:, 5] = True
+    touched[2, 4:, 4:, 5] = True
+    assert torch.equal(torch.where(touched, 0, got[0]), torch.where(touched, 0, want[0]))
+    hit = got[0][touched]
+    hit = hit[~(want[0][touched] == 0)]  # padding tokens of sequence 2
+    assert (hit.isnan() if value != value else hit == value).all()
+    assert torch.equal(got[1], want[1])
+
+
+def test_graph_replays():
+    """Plan and two layers captured once; the step's lengths, groups and rows change between the replays."""
+    case = SharedBatch(27, [300, 200], one_each([0, 0, 1, -1, 1, 0], [20, 90, 33, 400, 5, 64]), Hq=4, Hc=2, D=128, P=64, dtype=BF16).on()
+    shape = dict(q_heads=4, cached_heads=2, head_dim=128)
+    ws = torch.empty(ops.shared_decode_workspace_bytes(6, 1, **shape), dtype=torch.uint8, device="cuda")
+    plan = torch.empty(ops.shared_decode_plan_bytes(6, 1, **shape), dtype=torch.uint8, device="cuda")
+    case.q2 = torch.randn(case.q.shape, generator=case.gen).to(BF16).cuda()
+
+    def step():
+        ops.shared_decode_plan(case.batch_idx_d, case.pos_d, case.ids_d, case.lens_d, max_context=case.columns * 64, plan=plan, **shape)
+        return case.call(ops, plan=plan, workspace=ws), case.call(ops, q=case.q2, plan=plan, workspace=ws)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        made = step()
+    pos, lens, ids = case.pos.clone(), case.lens.clone(), case.ids.clone()
+    for turn in range(4):
+        case.pos_d.copy_((pos - 3 * turn).clamp(min=-1))
+        case.lens_d.copy_((lens - 40 * turn).clamp(min=0))
+        case.ids_d.copy_(ids if turn % 2 == 0 else ids * 0)
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = step()
+        for a, b in zip(made, eager):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+        case.check(eager[0], pos=case.pos_d.cpu())
+
+
+def test_another_stream_and_many_pages():
+    """Page ids that do not fit LDS at once (pages of one token), on a stream of its own."""
+    case = SharedBatch(28, [2500], one_each([0, 0, -1], [20, 1700, 3000]), Hq=2, Hc=1, D=64, P=1, dtype=F16).on()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        got = case.call(ops)
+    torch.cuda.synchronize()
+    case.check(got)
+
+
+@pytest.mark.parametrize("B", [257, 1000])
+def test_many_sequences(B):
+    groups = [b % 41 - 1 for b in range(B)]
+    case = SharedBatch(29, [64 + 3 * g for g in range(40)], one_each(groups, [1 + b % 90 for b in range(B)]), Hq=2, Hc=1, D=64, P=32,
+                       dtype=BF16).on()
+    case.check(case.call(ops))
+
+
+def test_long_prefixes_and_uneven_heads():
+    """Three cached heads: the cut is for a number of workgroups that divides nothing evenly."""
+    case = SharedBatch(30, [5000, 1333], one_each([0, 1, 0, 0, 1], [700, 3, 1, 50, 2222]), Hq=6, Hc=3, D=128, P=128, dtype=BF16).on()
+    case.check(case.call(ops))
