@@ -1,4 +1,4 @@
-// The calls an eager layer makes (append, decode step, prefill attention) from PyTorch tensors to the C ABI of
+// The calls an eager layer or step makes (append, decode step, prefill attention, tables and attention of shared prefixes) from PyTorch tensors to the C ABI of
 // include/fp_paged_kv.h, as a Python module.
 //
 // Bound by the host: a layer of a small eager step is shorter on the GPU than its calls are in Python, where every pointer, size
@@ -17,6 +17,7 @@
 #include <torch/version.h>
 
 #include <exception>
+#include <initializer_list>
 
 #include "fp_paged_kv.h"
 
@@ -46,6 +47,13 @@ bool is_table(const at::Tensor& t) { return t.dim() == 2 && t.scalar_type() == a
 bool is_indices(const at::Tensor& t, int64_t n) { return t.scalar_type() == at::kLong && t.is_contiguous() && t.numel() == n; }
 bool is_bytes(const at::Tensor& t) { return t.scalar_type() == at::kByte && t.is_contiguous(); }
 bool dense_rows(const at::Tensor& t) { return t.stride(t.dim() - 1) == 1; }
+
+// All of them (null: not given) lie on the device of this index, which the caller says is current.
+bool on_device(int64_t device, std::initializer_list<const at::Tensor*> tensors) {
+  for (const at::Tensor* t : tensors)
+    if (t && t->get_device() != device) return false;
+  return true;
+}
 
 // Other Python threads run while this one allocates and launches, which may wait (for a full queue, or for memory).
 struct Unlocked {
@@ -237,6 +245,142 @@ PyObject* prefill_unguarded(PyObject* const* args) {
   return pair(out, lse);
 }
 
+bool is_vector(const at::Tensor& t, at::ScalarType type, int64_t n) {
+  return t.dim() == 1 && t.scalar_type() == type && t.is_contiguous() && t.size(0) == n;
+}
+
+// batch_idx, input_pos, prefix_ids, prefix_lens: the step of an attention over shared prefixes
+bool is_shared_step(const at::Tensor& bidx, const at::Tensor& pos, const at::Tensor& ids, const at::Tensor& lens) {
+  return bidx.dim() == 1 && is_indices(bidx, bidx.size(0)) && index_code(pos) >= 0 && pos.is_contiguous() &&
+         (pos.dim() == 1 || pos.dim() == 2) && pos.size(0) == bidx.size(0) && ids.dim() == 1 &&
+         is_vector(ids, at::kInt, ids.size(0)) && is_vector(lens, at::kInt, ids.size(0));
+}
+
+// batch_idx, input_pos, prefix_ids, prefix_lens, q_heads, cached_heads, head_dim, max_context, plan, device, stream -> True
+PyObject* shared_plan_unguarded(PyObject* const* args) {
+  Args a{args};
+  const at::Tensor *bidx = a.tensor(), *pos = a.tensor(), *ids = a.tensor(), *lens = a.tensor();
+  const int64_t Hq = a.integer(), Hc = a.integer(), D = a.integer(), max_context = a.integer();
+  const at::Tensor* plan = a.tensor();
+  const int64_t device = a.integer(), stream = a.integer();
+  if (!a.ok || !is_shared_step(*bidx, *pos, *ids, *lens) || !is_bytes(*plan) || !on_device(device, {bidx, pos, ids, lens, plan}))
+    Py_RETURN_NONE;
+  int rc;
+  {
+    const Unlocked others;
+    rc = fp_shared_decode_plan(static_cast<const int64_t*>(bidx->data_ptr()), pos->data_ptr(), index_code(*pos),
+                               static_cast<const int32_t*>(ids->data_ptr()), static_cast<const int32_t*>(lens->data_ptr()),
+                               bidx->size(0), pos->dim() == 2 ? pos->size(1) : 1, Hq, Hc, D, ids->size(0), max_context,
+                               plan->data_ptr(), plan->numel(), reinterpret_cast<void*>(stream));
+  }
+  if (rc < 0) return fail("fp_shared_decode_plan", rc);
+  Py_RETURN_TRUE;
+}
+
+// q, pool_k, pool_v, page_table, batch_idx, input_pos, prefix_ids, prefix_lens, page_size, max_context, scale, sinks, plan, workspace,
+// device, stream -> (out, lse)
+PyObject* shared_unguarded(PyObject* const* args) {
+  Args a{args};
+  const at::Tensor *q = a.tensor(), *pk = a.tensor(), *pv = a.tensor(), *table = a.tensor(), *bidx = a.tensor(), *pos = a.tensor(),
+                   *ids = a.tensor(), *lens = a.tensor();
+  const int64_t page_size = a.integer(), max_context = a.integer();
+  const double scale = a.number();
+  const at::Tensor *sinks = a.maybe_tensor(), *plan = a.tensor(), *ws = a.tensor();
+  const int64_t device = a.integer(), stream = a.integer();
+  if (!a.ok) Py_RETURN_NONE;
+  const int dt = dtype_code(*q);
+  if (dt < 0 || q->dim() != 4 || pk->dim() != 3 || pk->sizes() != pv->sizes() || pk->size(2) != q->size(3) ||
+      pk->scalar_type() != q->scalar_type() || pv->scalar_type() != q->scalar_type() || !pk->is_contiguous() || !pv->is_contiguous() ||
+      !q->is_contiguous() || !is_table(*table) || !is_shared_step(*bidx, *pos, *ids, *lens) || !is_bytes(*plan) || !is_bytes(*ws))
+    Py_RETURN_NONE;
+  const int64_t B = q->size(0), Hq = q->size(1), S = q->size(2), D = q->size(3), Hc = pk->size(0);
+  if (bidx->size(0) != B || (pos->dim() == 2 ? pos->size(1) : 1) != S || ids->size(0) != table->size(0) ||
+      (sinks && !is_vector(*sinks, at::kFloat, Hq)) || !on_device(device, {q, pk, pv, table, bidx, pos, ids, lens, sinks, plan, ws}))
+    Py_RETURN_NONE;
+  at::Tensor out, lse;
+  int rc;
+  {
+    const Unlocked others;
+    out = at::empty({B, Hq, S, D}, q->options());
+    lse = at::empty({B, Hq, S}, q->options().dtype(at::kFloat));
+    rc = fp_paged_decode_shared(
+        q->data_ptr(), q->stride(0), q->stride(1), q->stride(2), pk->data_ptr(), pv->data_ptr(),
+        static_cast<const int64_t*>(table->data_ptr()), table->stride(0), static_cast<const int64_t*>(bidx->data_ptr()), pos->data_ptr(),
+        index_code(*pos), out.data_ptr(), out.stride(0), out.stride(1), out.stride(2), static_cast<float*>(lse.data_ptr()),
+        sinks ? static_cast<const float*>(sinks->data_ptr()) : nullptr, ws->data_ptr(), ws->numel(), plan->data_ptr(), plan->numel(), B,
+        S, Hq, Hc, D, page_size, table->size(1), table->size(0), pk->size(1), max_context, static_cast<float>(scale), dt,
+        reinterpret_cast<void*>(stream));
+  }
+  if (rc < 0) return fail("fp_paged_decode_shared", rc);
+  return pair(out, lse);
+}
+
+// slots, old_lens, new_lens, free_pages, free_count, page_table, page_size, max_rows, parents, row_multiple, inverse, device, stream ->
+// the nine tensors of StepTables
+PyObject* tables_unguarded(PyObject* const* args) {
+  Args a{args};
+  const at::Tensor *slots = a.tensor(), *before = a.tensor(), *after = a.tensor(), *pages = a.tensor(), *count = a.tensor(),
+                   *table = a.tensor();
+  const int64_t page_size = a.integer(), rows = a.integer();
+  const at::Tensor* parents = a.maybe_tensor();
+  const int64_t multiple = a.integer();
+  const at::Tensor* inverse = a.maybe_tensor();
+  const int64_t device = a.integer(), stream = a.integer();
+  if (!a.ok || slots->dim() != 1 || pages->dim() != 1 || rows < 0 || multiple < 1) Py_RETURN_NONE;
+  const int64_t B = slots->size(0);
+  if (!is_vector(*slots, at::kLong, B) || index_code(*before) < 0 || !is_vector(*before, before->scalar_type(), B) ||
+      !is_vector(*after, before->scalar_type(), B) || !is_vector(*pages, at::kLong, pages->size(0)) || !is_vector(*count, at::kInt, 1) ||
+      !is_table(*table) || (parents && !is_vector(*parents, at::kLong, B)) ||
+      (inverse && (!is_table(*inverse) || inverse->size(0) != table->size(0))) ||
+      !on_device(device, {slots, before, after, pages, count, table, parents, inverse}))
+    Py_RETURN_NONE;
+  at::Tensor made[9];
+  int rc;
+  {
+    const Unlocked others;
+    const auto options = slots->options(), whole = options.dtype(at::kInt);
+    const int64_t sizes[9] = {rows, rows, rows, B + 1, 1, B, B, B, 1};
+    const bool is_long[9] = {true, false, true, false, false, true, true, false, false};
+    for (int i = 0; i < 9; ++i) made[i] = at::empty({sizes[i]}, is_long[i] ? options : whole);
+    const auto at = [&](int i) { return made[i].data_ptr(); };
+    rc = fp_step_tables(static_cast<const int64_t*>(slots->data_ptr()), before->data_ptr(), after->data_ptr(), index_code(*before),
+                        parents ? static_cast<const int64_t*>(parents->data_ptr()) : nullptr, static_cast<const int64_t*>(pages->data_ptr()),
+                        static_cast<const int32_t*>(count->data_ptr()), pages->size(0), static_cast<int64_t*>(table->data_ptr()),
+                        table->stride(0), inverse ? static_cast<int64_t*>(inverse->data_ptr()) : nullptr, inverse ? inverse->stride(0) : 0,
+                        inverse ? inverse->size(1) : 0, static_cast<int64_t*>(at(0)), static_cast<int32_t*>(at(1)),
+                        static_cast<int64_t*>(at(2)), static_cast<int32_t*>(at(3)), static_cast<int32_t*>(at(4)),
+                        static_cast<int64_t*>(at(5)), static_cast<int64_t*>(at(6)), static_cast<int32_t*>(at(7)),
+                        static_cast<int32_t*>(at(8)), B, rows, multiple, page_size, table->size(1), table->size(0),
+                        reinterpret_cast<void*>(stream));
+  }
+  if (rc < 0) return fail("fp_step_tables", rc);
+  PyObject* const t = PyTuple_New(9);
+  if (!t) return nullptr;
+  for (int i = 0; i < 9; ++i) PyTuple_SET_ITEM(t, i, THPVariable_Wrap(made[i]));
+  return t;
+}
+
+// pool, src, dst, rows, page_size, device, stream -> True
+PyObject* copy_unguarded(PyObject* const* args) {
+  Args a{args};
+  const at::Tensor *pool = a.tensor(), *src = a.tensor(), *dst = a.tensor(), *rows = a.tensor();
+  const int64_t page_size = a.integer(), device = a.integer(), stream = a.integer();
+  if (!a.ok || dtype_code(*pool) < 0 || pool->dim() < 2 || !pool->is_contiguous() || pool->numel() == 0 || src->dim() != 1 ||
+      !is_vector(*src, at::kLong, src->size(0)) || !is_vector(*dst, at::kLong, src->size(0)) ||
+      !is_vector(*rows, at::kInt, src->size(0)) || page_size < 1 || !on_device(device, {pool, src, dst, rows}))
+    Py_RETURN_NONE;
+  const int64_t D = pool->size(-1), n_slots = pool->size(-2);
+  int rc;
+  {
+    const Unlocked others;
+    rc = fp_copy_pages(pool->data_ptr(), static_cast<const int64_t*>(src->data_ptr()), static_cast<const int64_t*>(dst->data_ptr()),
+                       static_cast<const int32_t*>(rows->data_ptr()), src->size(0), pool->numel() / (n_slots * D), n_slots, D, page_size,
+                       dtype_code(*pool), reinterpret_cast<void*>(stream));
+  }
+  if (rc < 0) return fail("fp_copy_pages", rc);
+  Py_RETURN_TRUE;
+}
+
 // A C++ exception (an allocation that failed) becomes a Python one.
 template <PyObject* (*kCall)(PyObject* const*), Py_ssize_t kArgs>
 PyObject* guarded(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -251,7 +395,9 @@ PyObject* guarded(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 #define FP_METHOD(name, call, n) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<call, n>)), METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {FP_METHOD("append", append_unguarded, 11), FP_METHOD("decode", decode_unguarded, 19),
-                          FP_METHOD("prefill", prefill_unguarded, 14), {nullptr, nullptr, 0, nullptr}};
+                          FP_METHOD("prefill", prefill_unguarded, 14),
+                          FP_METHOD("shared_plan", shared_plan_unguarded, 11), FP_METHOD("shared", shared_unguarded, 16),
+                          FP_METHOD("tables", tables_unguarded, 13), FP_METHOD("copy_pages", copy_unguarded, 7), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "fp_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

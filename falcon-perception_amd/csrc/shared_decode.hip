@@ -36,7 +36,8 @@ constexpr int kMaxRows = 1 << 20;      // B * S * heads of a group
 constexpr int kMaxContext = 1 << 21;   // with the rows: units of all tiles fit 31 bits
 constexpr int kTileRows = 64;
 constexpr int kUnit = 64;              // keys: what the cut is made of
-constexpr int kMinUnits = 2;           // a workgroup's share at least
+constexpr int kLeadUnits = 3;          // what a tile costs before its first key and behind its last, in units
+constexpr int kMinUnits = 4;           // a workgroup's share at least
 constexpr int kMinShared = 64;         // keys of a prefix that are worth a tile of their own
 constexpr int kSegPages = 1024;        // page ids held in LDS
 constexpr float kMaxSlack = 6.f;       // the reference point of the exponentials may lag the maximum by this much (log2)
@@ -64,9 +65,6 @@ struct Sequence {
   int own_tile;        // first tile of the keys behind the prefix, -1: none
   int pad[3];
 };
-struct Share {
-  int tile, offset, units, pad;  // first tile, units of it that belong to workgroups before, units to do
-};
 struct Tile {
   int slot;            // row of the page table
   int base;            // >= 0: a prefix, place of the group in the list of members; < 0: -1 - sequence
@@ -76,6 +74,10 @@ struct Tile {
   int n_pieces;
   int part;            // workspace row of the first piece's first row; piece after piece
   int pad[3];
+};
+struct Share {
+  int tile, offset, units, pad;  // first tile, units of it (lead included) that belong to workgroups before, units to do
+  Tile first;                    // the first tile itself: a trip to memory less
 };
 
 struct Layout {
@@ -139,6 +141,7 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   int* const s_pmem = s_punit + Bp;
   int* const s_sunit = s_pmem + Bp;    // units of own tiles (tiles: see own_tiles)
   int* const s_stile = s_sunit + Bp;
+  int* const s_slot = s_stile + Bp;
   __shared__ int s_sum[16][5];
   const int tid = threadIdx.x, n_thr = blockDim.x, lane = tid & 63, wave = tid >> 6;
 
@@ -158,7 +161,7 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
         len = max(a.lens[slot], 0);
       }
       Sequence* const q = reinterpret_cast<Sequence*>(a.plan + a.seqs) + b;
-      q->slot = valid ? static_cast<int>(slot) : -1;
+      q->slot = s_slot[b] = valid ? static_cast<int>(slot) : -1;
       q->keys = keys;
     }
     s_id[b] = id;
@@ -203,12 +206,12 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
     if (c > 0) {
       const int n = (c * a.rows + kTileRows - 1) / kTileRows;
       x[0] += n;
-      x[1] += n * units_of(s_shared[b]);
+      x[1] += n * (kLeadUnits + units_of(s_shared[b]));
       x[2] += c;
     }
     const int own = s_keys[b] - s_shared[b];
     if (own > 0) {
-      x[3] += own_tiles * units_of(own);
+      x[3] += own_tiles * (kLeadUnits + units_of(own));
       x[4] += own_tiles;
     }
   };
@@ -264,56 +267,56 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
     if (shares) reinterpret_cast<int*>(a.plan + a.members)[s_pmem[lead] + s_rank[b]] = b;
   }
   // workspace rows: a tile has those of the tiles before it, each once, and 64 for every cut up to its first key
-  const int64_t all_shared_rows = static_cast<int64_t>(total[2]) * a.rows;
-  for (int i = tid; i < n_tiles; i += n_thr) {
+  const int all_shared_rows = total[2] * a.rows;
+  const auto tile_at = [&](int i) {
     Tile t;
-    int n_units, from;
-    int64_t rows_before;
+    int n_units, from, rows_before;
     if (i < p_tiles) {
       const int b = last_at_or_below(s_ptile, a.B, i), k = i - s_ptile[b], all = s_count[b] * a.rows;
       n_units = units_of(s_shared[b]);
-      from = s_punit[b] + k * n_units;
+      from = s_punit[b] + k * (kLeadUnits + n_units);
       t.base = s_pmem[b];
-      t.slot = static_cast<int>(a.batch_idx[b]);
+      t.slot = s_slot[b];
       t.row0 = k * kTileRows;
       t.n_rows = min(kTileRows, all - t.row0);
       t.t_begin = 0;
       t.t_end = s_shared[b];
-      rows_before = static_cast<int64_t>(s_pmem[b]) * a.rows + t.row0;
+      rows_before = s_pmem[b] * a.rows + t.row0;
     } else {
       const int b = last_at_or_below(s_stile, a.B, i - p_tiles), k = i - p_tiles - s_stile[b];
       n_units = units_of(s_keys[b] - s_shared[b]);
-      from = total[1] + s_sunit[b] + k * n_units;
+      from = total[1] + s_sunit[b] + k * (kLeadUnits + n_units);
       t.base = -1 - b;
-      t.slot = static_cast<int>(a.batch_idx[b]);
+      t.slot = s_slot[b];
       t.row0 = k * kTileRows;
       t.n_rows = min(kTileRows, a.rows - t.row0);
       t.t_begin = s_shared[b];
       t.t_end = s_keys[b];
-      rows_before = all_shared_rows + static_cast<int64_t>(b) * a.rows + t.row0;
+      rows_before = all_shared_rows + b * a.rows + t.row0;
     }
-    t.first_wg = from / len;
-    t.n_pieces = (from + n_units - 1) / len - t.first_wg + 1;
-    t.part = static_cast<int>(rows_before + static_cast<int64_t>(kTileRows) * t.first_wg);
+    t.first_wg = (from + kLeadUnits) / len;
+    t.n_pieces = (from + kLeadUnits + n_units - 1) / len - t.first_wg + 1;
+    t.part = rows_before + kTileRows * t.first_wg;
     t.pad[0] = t.pad[1] = t.pad[2] = 0;
-    reinterpret_cast<Tile*>(a.plan + a.tiles)[i] = t;
-  }
-  for (int w = tid; w < a.n_wg; w += n_thr) {
-    Share s{0, 0, 0, 0};
+    return t;
+  };
+  for (int i = tid; i < n_tiles; i += n_thr) reinterpret_cast<Tile*>(a.plan + a.tiles)[i] = tile_at(i);
+  for (int w = tid; w < n_wg; w += n_thr) {
+    Share s;
     const int from = w * len;
-    if (w < n_wg) {
-      s.units = min(len, units - from);
-      if (from < total[1]) {
-        const int b = last_at_or_below(s_punit, a.B, from), n = units_of(s_shared[b]), off = from - s_punit[b];
-        s.tile = s_ptile[b] + off / n;
-        s.offset = off % n;
-      } else {
-        const int b = last_at_or_below(s_sunit, a.B, from - total[1]), n = units_of(s_keys[b] - s_shared[b]);
-        const int off = from - total[1] - s_sunit[b];
-        s.tile = p_tiles + s_stile[b] + off / n;
-        s.offset = off % n;
-      }
+    s.units = min(len, units - from);
+    s.pad = 0;
+    if (from < total[1]) {
+      const int b = last_at_or_below(s_punit, a.B, from), n = kLeadUnits + units_of(s_shared[b]), off = from - s_punit[b];
+      s.tile = s_ptile[b] + off / n;
+      s.offset = off % n;
+    } else {
+      const int b = last_at_or_below(s_sunit, a.B, from - total[1]), n = kLeadUnits + units_of(s_keys[b] - s_shared[b]);
+      const int off = from - total[1] - s_sunit[b];
+      s.tile = p_tiles + s_stile[b] + off / n;
+      s.offset = off % n;
     }
+    s.first = tile_at(s.tile);
     reinterpret_cast<Share*>(a.plan + a.shares)[w] = s;
   }
 }
@@ -895,11 +898,17 @@ __global__ __launch_bounds__(kThreads, (sizeof(Shared<E, D>) <= 80 * 1024 ? 2 : 
   const Share share = load_record<Share>(a.plan + a.shares + w * static_cast<int64_t>(sizeof(Share)));
   if (!plan_fits(a, h) || w >= h.n_wg) return;
   int left = share.units, offset = share.offset;
-  for (int i = share.tile; left > 0 && i < h.n_tiles; ++i, offset = 0) {
-    const Tile t = load_record<Tile>(a.plan + a.tiles + i * static_cast<int64_t>(sizeof(Tile)));
-    const int units = min(left, units_of(t.t_end - t.t_begin) - offset);
-    const int t0 = t.t_begin + offset * kUnit, t1 = min(t.t_end, t0 + units * kUnit), piece = w - t.first_wg;
-    if (i != share.tile) __syncthreads();  // the piece before has left LDS
+  bool busy = false;
+  Tile t = share.first;
+  for (int i = share.tile;;) {
+    const int all = units_of(t.t_end - t.t_begin), piece = w - t.first_wg;
+    const int from = max(0, offset - kLeadUnits), to = min(all, offset + left - kLeadUnits);
+    const int t0 = t.t_begin + from * kUnit, t1 = min(t.t_end, t.t_begin + to * kUnit);
+    left -= kLeadUnits + all - offset;
+    offset = 0;
+    if (to > from) {
+    if (busy) __syncthreads();  // the piece before has left LDS
+    busy = true;
     if (Geo<E, D>::k16 && t.n_rows <= 8)
       run_piece<E, D, 1, Geo<E, D>::k16>(a, sh, t, piece, t0, t1);
     else if (t.n_rows <= 16)
@@ -908,12 +917,15 @@ __global__ __launch_bounds__(kThreads, (sizeof(Shared<E, D>) <= 80 * 1024 ? 2 : 
       run_piece<E, D, 2, false>(a, sh, t, piece, t0, t1);
     else
       run_piece<E, D, 4, false>(a, sh, t, piece, t0, t1);
-    left -= units;
+    }
+    if (left <= kLeadUnits || ++i >= h.n_tiles) break;  // the lead alone has no key
+    t = load_record<Tile>(a.plan + a.tiles + i * static_cast<int64_t>(sizeof(Tile)));
   }
 }
 
 // ------------------------------------------------------------------------------------------------------------ join
 // D / 4 lanes a row.
+constexpr int kBatch = 8;
 template <typename E, int D>
 __global__ __launch_bounds__(kThreads) void shared_join_kernel(const SharedArgs a) {
   constexpr int LPR = D / 4;
@@ -939,25 +951,48 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(const SharedArgs 
     const int hc = h >> a.group_shift, x = (j << a.group_shift) + (h & (a.group - 1));
     float m = -INFINITY, den = 0.f;
     f32x4 num = {0.f, 0.f, 0.f, 0.f};
-    const auto join = [&](const Tile& t, int r) {
-      for (int k = 0; k < t.n_pieces; ++k) {
-        const int64_t p = (static_cast<int64_t>(t.part) + static_cast<int64_t>(k) * t.n_rows + r) * a.Hc + hc;
-        const float2 ml = *reinterpret_cast<const float2*>(a.ws_ml + p * 2);
-        const f32x4 acc = *reinterpret_cast<const f32x4*>(a.ws_acc + p * D + c * 4);
-        const float mn = fmaxf(m, ml.x), ms = safe_max(mn), keep = fast_exp2(m - ms), w = fast_exp2(ml.x - ms);
-        den = den * keep + ml.y * w;
-        num = num * keep + acc * w;
-        m = mn;
-      }
-    };
+    // the prefix's pieces, then those of its own keys: kBatch of them are on their way at once
+    int n_shared = 0, n_own = 0;
+    int64_t at = 0, step = 0, own_at = 0, own_step = 0;  // rows of the workspace
     if (s.prefix_tile >= 0) {
       const int rr = s.prefix_row + x;
-      join(tiles[s.prefix_tile + rr / kTileRows], rr % kTileRows);
+      const Tile t = tiles[s.prefix_tile + rr / kTileRows];
+      n_shared = t.n_pieces;
+      at = t.part + rr % kTileRows;
+      step = t.n_rows;
     }
     if (s.own_tile >= 0) {
       const Tile t = tiles[s.own_tile + x / kTileRows];
       if (s.prefix_tile < 0 && t.n_pieces == 1) return;  // stored already
-      join(t, x % kTileRows);
+      n_own = t.n_pieces;
+      own_at = t.part + x % kTileRows;
+      own_step = t.n_rows;
+    }
+    const int n = n_shared + n_own;
+    for (int k0 = 0; k0 < n; k0 += kBatch) {
+      float2 ml[kBatch];
+      f32x4 acc[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int k = min(k0 + i, n - 1);
+        const int64_t p = (k < n_shared ? at + k * step : own_at + (k - n_shared) * own_step) * a.Hc + hc;
+        ml[i] = *reinterpret_cast<const float2*>(a.ws_ml + p * 2);
+        acc[i] = *reinterpret_cast<const f32x4*>(a.ws_acc + p * D + c * 4);
+      }
+      float mn = m;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) mn = fmaxf(mn, ml[i].x);
+      const float ms = safe_max(mn), keep = fast_exp2(m - ms);
+      den *= keep;
+      num *= keep;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        if (k0 + i >= n) break;
+        const float w = fast_exp2(ml[i].x - ms);
+        den += ml[i].y * w;
+        num += acc[i] * w;
+      }
+      m = mn;
     }
     lse = (m + log2f(den)) * kLn2;
 #pragma unroll
@@ -1022,10 +1057,10 @@ extern "C" int fp_shared_decode_plan(const int64_t* batch_idx, const void* input
                    l.n_wg, l.max_tiles, static_cast<char*>(plan), l.seqs, l.members, l.shares, l.tiles};
   int threads = (B + 63) / 64 * 64;
   threads = threads < 256 ? 256 : threads > 1024 ? 1024 : threads;
-  const size_t lds = 12 * static_cast<size_t>((B + 3) & ~3) * sizeof(int);
+  const size_t lds = 13 * static_cast<size_t>((B + 3) & ~3) * sizeof(int);
   if (lds > 64 * 1024) {
     static const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(shared_plan_kernel),
-                                                          hipFuncAttributeMaxDynamicSharedMemorySize, 12 * kMaxSequences * sizeof(int));
+                                                          hipFuncAttributeMaxDynamicSharedMemorySize, 13 * kMaxSequences * sizeof(int));
     if (allowed != hipSuccess) return fp::fail(FP_ERR_LAUNCH, "%s: %s", what, hipGetErrorString(allowed));
   }
   hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3(threads), lds, static_cast<hipStream_t>(stream), a);

@@ -495,6 +495,14 @@ def _on(device: torch.device):
     return torch.cuda.device(device)
 
 
+def _current(t: Tensor) -> int:
+    """The index of the tensor's device where that is the current one, else -1: what the calls in C++ serve."""
+    if not t.is_cuda:
+        return -1
+    index = t.get_device()
+    return index if index == torch.cuda.current_device() else -1
+
+
 def _same_device(what: str, *tensors) -> torch.device:
     N.require_cuda(*tensors)
     devices = {t.device for t in tensors if t is not None}
@@ -558,6 +566,12 @@ def step_tables(slots: Tensor, old_lens: Tensor, new_lens: Tensor, free_pages: T
     row page * page_size + position % page_size of the pool's planes; padding is 0, 0, 0.  `row_starts` [B + 1] int32,
     `free_left` [1] int32: the next `free_count`.  `status` [1] int32: not 0 means that nothing was done, and `check()`
     waits and says why."""
+    index = _current(slots)
+    if index >= 0:
+        made = N.host().tables(slots, old_lens, new_lens, free_pages, free_count, page_table, page_size, max_rows, parents,
+                               row_multiple, inverse, index, N.raw_stream(index))
+        if made is not None:
+            return StepTables(*made)
     what = "step_tables"
     device = _same_device(what, slots, old_lens, new_lens, free_pages, free_count, page_table, parents, inverse)
     slots = _vector(what, "slots", slots, None, torch.int64)
@@ -595,6 +609,9 @@ def copy_pages(pool: Tensor, src: Tensor, dst: Tensor, rows: Tensor, page_size: 
 
     An entry with a page outside the pool (-1: nothing to copy) or without rows is left out, and so are an entry whose
     destination is a source of the call and one whose destination an entry before it has: every source is copied as it was."""
+    index = _current(pool)
+    if index >= 0 and N.host().copy_pages(pool, src, dst, rows, page_size, index, N.raw_stream(index)):
+        return
     what = "copy_pages"
     device = _same_device(what, pool, src, dst, rows)
     if pool.dim() < 2 or not pool.is_contiguous():
@@ -651,6 +668,10 @@ def shared_decode_plan(batch_idx: Tensor, input_pos: Tensor, prefix_ids: Tensor,
                        cached_heads: int, head_dim: int, max_context: int, plan: Tensor | None = None) -> Tensor:
     """The plan of a `paged_decode_shared` step, made once for all layers: which sequences share a prefix and how the work
     is cut.  Arguments as there; `plan`: a uint8 tensor of `shared_decode_plan_bytes(...)` bytes to write it to."""
+    index = _current(batch_idx)
+    if index >= 0 and plan is not None and N.host().shared_plan(batch_idx, input_pos, prefix_ids, prefix_lens, q_heads, cached_heads,
+                                                                head_dim, max_context, plan, index, N.raw_stream(index)):
+        return plan
     what = "shared_decode_plan"
     device = _same_device(what, batch_idx, input_pos, prefix_ids, prefix_lens, plan)
     batch_idx, input_pos, prefix_ids, prefix_lens, S = _shared_step(what, batch_idx, input_pos, prefix_ids, prefix_lens)
@@ -680,6 +701,13 @@ def paged_decode_shared(q: Tensor, pool_k: Tensor, pool_v: Tensor, page_table: T
     `plan`: what `shared_decode_plan` made for this step (positions, slots and table unchanged since); without one the call
     makes it.  `workspace`: `shared_decode_workspace_bytes(...)` bytes, for one launch at a time.  `sinks` [Hq] float32 gates
     the output as in `paged_decode`."""
+    index = _current(q)
+    if index >= 0 and out is None and lse is None and plan is not None and workspace is not None:
+        got = N.host().shared(q, pool_k, pool_v, page_table, batch_idx, input_pos, prefix_ids, prefix_lens, page_size, max_context,
+                              1.0 / math.sqrt(q.shape[-1]) if scale is None else scale, sinks, plan, workspace, index,
+                              N.raw_stream(index))
+        if got is not None:
+            return got
     what = "paged_decode_shared"
     device = _same_device(what, q, pool_k, pool_v, page_table, batch_idx, input_pos, prefix_ids, prefix_lens, sinks, plan,
                           workspace, out, lse)
