@@ -50,13 +50,12 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 
 // ------------------------------------------------------------------------------------------------------------ plan
-// ints: header, sequences, members of the groups, workgroups, tiles
+// ints: header, sequences, tokens of the groups and of the other sequences, each token's place, workgroups, tiles
 struct Header {
   int magic, B, S, Hq, Hc, max_batch, max_context;
-  int len;      // units a workgroup
   int n_wg;     // workgroups that have a share
   int n_tiles;
-  int pad[6];
+  int pad[7];
 };
 struct Sequence {
   int slot, keys;      // -1: not a slot; keys any of its tokens sees
@@ -67,22 +66,23 @@ struct Sequence {
 };
 struct Tile {
   int slot;            // row of the page table
-  int base;            // >= 0: a prefix, place of the group in the list of members; < 0: -1 - sequence
+  int base;            // place of its group's or sequence's first token in the list
   int row0, n_rows;    // of the group's or the sequence's rows
   int t_begin, t_end;  // keys
-  int first_wg;        // workgroup of the first piece
   int n_pieces;
   int part;            // workspace row of the first piece's first row; piece after piece
+  int shared;          // of a group
   int pad[3];
 };
 struct Share {
-  int tile, offset, units, pad;  // first tile, units of it (lead included) that belong to workgroups before, units to do
-  Tile first;                    // the first tile itself: a trip to memory less
+  int tile, offset, units;  // first tile, units of it (lead included) that belong to workgroups before, units to do
+  int piece;                // of the first tile; the others begin here
+  Tile first;               // the first tile itself: a trip to memory less
 };
 
 struct Layout {
   int n_wg, max_tiles, rows;  // rows: of a sequence and cached head
-  int64_t seqs, members, shares, tiles, bytes;  // byte offsets
+  int64_t seqs, tokens, place, shares, tiles, bytes;  // byte offsets
   int64_t part_rows;
 };
 
@@ -91,17 +91,23 @@ Layout layout_of(int B, int S, int Hq, int Hc) {
   l.n_wg = 2 * fp::compute_units() / Hc;
   if (l.n_wg < 1) l.n_wg = 1;
   l.rows = S * (Hq / Hc);
-  // ceil(members * rows / 64) summed over groups of two or more; every sequence's own
+  // ceil(rows / 64) summed over groups of two or more; every sequence's own
   l.max_tiles = static_cast<int>(static_cast<int64_t>(B) * l.rows / kTileRows + B / 2 + 1 +
                                  static_cast<int64_t>(B) * ((l.rows + kTileRows - 1) / kTileRows));
+  const int64_t list = (static_cast<int64_t>(B) * S * 4 + 15) / 16 * 16;
   l.seqs = sizeof(Header);
-  l.members = l.seqs + static_cast<int64_t>(B) * sizeof(Sequence);
-  l.shares = l.members + (static_cast<int64_t>(B) * 4 + 15) / 16 * 16;
+  l.tokens = l.seqs + static_cast<int64_t>(B) * sizeof(Sequence);
+  l.place = l.tokens + list;
+  l.shares = l.place + list;
   l.tiles = l.shares + static_cast<int64_t>(l.n_wg) * sizeof(Share);
   l.bytes = l.tiles + static_cast<int64_t>(l.max_tiles) * sizeof(Tile);
-  l.part_rows = 2ll * B * l.rows + static_cast<int64_t>(kTileRows) * l.n_wg;
+  l.part_rows = 3ll * B * l.rows + static_cast<int64_t>(kTileRows) * l.n_wg;
   return l;
 }
+
+// A token of the lists: sequence and place in it (kMaxSequences and kMaxRows bound both).
+constexpr int kTokenShift = 20;
+static_assert(kMaxSequences <= 1 << (31 - kTokenShift) && kMaxRows <= 1 << kTokenShift, "a token is one int");
 
 struct PlanArgs {
   const int64_t* batch_idx;
@@ -109,9 +115,9 @@ struct PlanArgs {
   int pos_i64;
   const int32_t* ids;
   const int32_t* lens;
-  int B, S, Hq, Hc, rows, max_batch, max_context, n_wg, max_tiles;
+  int B, S, Hq, Hc, group, max_batch, max_context, n_wg;
   char* plan;
-  int64_t seqs, members, shares, tiles;
+  int64_t seqs, tokens, place, shares, tiles;
 };
 
 __device__ __forceinline__ int units_of(int keys) { return (keys + kUnit - 1) / kUnit; }
@@ -126,195 +132,304 @@ __device__ __forceinline__ int last_at_or_below(const int* at, int n, int x) {
   return lo;
 }
 
+// keys that token j of sequence b sees, 0: no token
+__device__ __forceinline__ int plan_keys(const PlanArgs& a, int b, int j) {
+  const int64_t p = fp::load_index(a.input_pos, static_cast<int64_t>(b) * a.S + j, a.pos_i64) + 1;
+  return p < 0 ? 0 : p > a.max_context ? a.max_context : static_cast<int>(p);
+}
+
+// Sums over the threads before this one and over all, of N numbers a thread.
+template <int N>
+__device__ __forceinline__ void block_sums(const int (&x)[N], int (&before)[N], int (&total)[N], int* s_sum) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int up = fp_decode::scan_lanes(x[i]);
+    if (lane == 63) s_sum[wave * N + i] = up;
+    before[i] = up - x[i];
+    total[i] = 0;
+  }
+  __syncthreads();
+  for (int w = 0; w < static_cast<int>(blockDim.x) / 64; ++w)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int y = s_sum[w * N + i];
+      if (w < wave) before[i] += y;
+      total[i] += y;
+    }
+  __syncthreads();
+}
+
+constexpr int kPlanArrays = 15;
+
 __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   extern __shared__ int s_mem[];
   const int Bp = (a.B + 3) & ~3;
   int* const s_id = s_mem;             // prefix id, 0: none
   int* const s_keys = s_id + Bp;       // keys the sequence's tokens see
   int* const s_len = s_keys + Bp;      // its prefix length
-  int* const s_shared = s_len + Bp;    // shared keys of its group, 0: none
-  int* const s_count = s_shared + Bp;  // members, at the group's first sequence (its leader), elsewhere 0
-  int* const s_rank = s_count + Bp;    // place among the members
+  int* const s_tok = s_len + Bp;       // its tokens
+  int* const s_shared = s_tok + Bp;    // shared keys of its group, 0: none
+  int* const s_count = s_shared + Bp;  // tokens of the group, at its first sequence (its leader), elsewhere 0
+  int* const s_rank = s_count + Bp;    // tokens of the members before
   int* const s_lead = s_rank + Bp;
-  int* const s_ptile = s_lead + Bp;    // sums over the sequences before: prefix tiles, their units, members
-  int* const s_punit = s_ptile + Bp;
-  int* const s_pmem = s_punit + Bp;
-  int* const s_sunit = s_pmem + Bp;    // units of own tiles (tiles: see own_tiles)
-  int* const s_stile = s_sunit + Bp;
-  int* const s_slot = s_stile + Bp;
-  __shared__ int s_sum[16][5];
-  const int tid = threadIdx.x, n_thr = blockDim.x, lane = tid & 63, wave = tid >> 6;
+  int* const s_slot = s_lead + Bp;
+  int* const s_ptile = s_slot + Bp;    // sums over the sequences before: tiles of prefixes,
+  int* const s_base = s_ptile + Bp;    //   tokens of groups or of sequences that share nothing: place in the list
+  int* const s_stile = s_base + Bp;    //   tiles of own keys,
+  int* const s_unit = s_stile + Bp;    //   units of prefixes that are cut with everything else,
+  int* const s_own = s_unit + Bp;      //   units of own keys,
+  int* const s_wg = s_own + Bp;        //   workgroups of prefixes that are cut by themselves
+  __shared__ int s_sum[16 * 7], s_pick[1];
+  const int tid = threadIdx.x, n_thr = blockDim.x, lane = tid & 63, wave = tid >> 6, n_waves = n_thr / 64;
+  Sequence* const seqs = reinterpret_cast<Sequence*>(a.plan + a.seqs);
 
-  for (int b = tid; b < Bp; b += n_thr) {
-    int id = 0, keys = 0, len = 0;
-    if (b < a.B) {
-      const int64_t slot = a.batch_idx[b];
-      const bool valid = slot >= 0 && slot < a.max_batch;
-      for (int j = 0; j < a.S; ++j) {
-        int64_t p = fp::load_index(a.input_pos, static_cast<int64_t>(b) * a.S + j, a.pos_i64) + 1;
-        p = p < 0 ? 0 : p > a.max_context ? a.max_context : p;
-        keys = max(keys, static_cast<int>(p));
-      }
-      if (!valid) keys = 0;
-      if (keys > 0) {
-        id = max(a.ids[slot], 0);
-        len = max(a.lens[slot], 0);
-      }
-      Sequence* const q = reinterpret_cast<Sequence*>(a.plan + a.seqs) + b;
-      q->slot = s_slot[b] = valid ? static_cast<int>(slot) : -1;
-      q->keys = keys;
-    }
-    s_id[b] = id;
+  const auto put = [&](int b, int keys, int tokens) {
+    const int64_t slot = b < a.B ? a.batch_idx[b] : -1;
+    const bool valid = slot >= 0 && slot < a.max_batch;
+    if (!valid) keys = tokens = 0;
+    s_id[b] = keys > 0 ? max(a.ids[slot], 0) : 0;
+    s_len[b] = keys > 0 ? max(a.lens[slot], 0) : 0;
     s_keys[b] = keys;
-    s_len[b] = len;
+    s_tok[b] = tokens;
+    s_slot[b] = valid ? static_cast<int>(slot) : -1;
+  };
+  if (a.S == 1) {
+    for (int b = tid; b < Bp; b += n_thr) {
+      const int keys = b < a.B ? plan_keys(a, b, 0) : 0;
+      put(b, keys, keys > 0);
+    }
+  } else {  // a wavefront a sequence
+    for (int b = wave; b < Bp; b += n_waves) {
+      int keys = 0, tokens = 0;
+      for (int j0 = 0; j0 < a.S && b < a.B; j0 += 64) {
+        const int k = j0 + lane < a.S ? plan_keys(a, b, j0 + lane) : 0;
+        keys = max(keys, fp::wave_max(k));
+        tokens += __popcll(__ballot(k > 0));
+      }
+      if (lane == 0) put(b, keys, tokens);
+    }
   }
   __syncthreads();
 
   // groups: every sequence looks at all of them (LDS broadcasts, four ids at a time)
   for (int b = tid; b < a.B; b += n_thr) {
     const int id = s_id[b];
-    int lead = b, rank = 0, count = 0, shortest = INT32_MAX, longest = 0;
+    int lead = b, rank = 0, members = 0, tokens = 0, shortest = INT32_MAX, longest = 0;
     if (id > 0) {
       for (int j = 0; j < Bp; j += 4) {
         const i32x4 four = *reinterpret_cast<const i32x4*>(s_id + j);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           if (four[i] != id) continue;
-          ++count;
-          rank += j + i < b;
+          ++members;
+          tokens += s_tok[j + i];
+          rank += j + i < b ? s_tok[j + i] : 0;
           lead = min(lead, j + i);
           shortest = min(shortest, s_len[j + i]);
           longest = max(longest, s_keys[j + i]);
         }
       }
     }
-    const int shared = count >= 2 ? min(shortest, longest) : 0;
+    const int shared = members >= 2 ? min(shortest, longest) : 0;
     const bool shares = shared >= kMinShared;
     s_shared[b] = shares ? shared : 0;
-    s_count[b] = shares && lead == b ? count : 0;
-    s_rank[b] = rank;
+    s_count[b] = shares && lead == b ? tokens : 0;
+    s_rank[b] = shares ? rank : 0;
     s_lead[b] = lead;
   }
   __syncthreads();
 
+  const auto tiles_of = [&](int tokens) { return (tokens * a.group + kTileRows - 1) / kTileRows; };
   // sums over the sequences before, consecutive ones a thread
-  const int own_tiles = (a.rows + kTileRows - 1) / kTileRows;
   const int per = (a.B + n_thr - 1) / n_thr, b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
-  int x[5] = {0, 0, 0, 0, 0};
+  int x[7] = {0, 0, 0, 0, 0, 0, 0}, before[7], total[7];
   const auto add = [&](int b) {
-    const int c = s_count[b];
+    const int c = s_count[b], own = s_keys[b] - s_shared[b];
     if (c > 0) {
-      const int n = (c * a.rows + kTileRows - 1) / kTileRows;
-      x[0] += n;
-      x[1] += n * (kLeadUnits + units_of(s_shared[b]));
-      x[2] += c;
+      x[0] += tiles_of(c);
+      x[1] += c;
+      x[4] += tiles_of(c) * (kLeadUnits + units_of(s_shared[b]));
+      x[5] += tiles_of(c) > 1;
     }
-    const int own = s_keys[b] - s_shared[b];
     if (own > 0) {
-      x[3] += own_tiles * (kLeadUnits + units_of(own));
-      x[4] += own_tiles;
+      x[2] += tiles_of(s_tok[b]);
+      x[4] += tiles_of(s_tok[b]) * (kLeadUnits + units_of(own));
     }
+    if (s_shared[b] == 0) x[3] += s_tok[b];
+    x[6] += s_tok[b];
   };
   for (int b = b0; b < b1; ++b) add(b);
-  int total[5], before[5];
+  block_sums(x, before, total, s_sum);
+  const int p_tiles = total[0], n_tiles = p_tiles + total[2], shared_tokens = total[1], n_multi = total[5], all_units = total[4];
 #pragma unroll
-  for (int i = 0; i < 5; ++i) {
-    int up = x[i];
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int y = __shfl_up(up, off);
-      if (lane >= off) up += y;
-    }
-    if (lane == 63) s_sum[wave][i] = up;
-    before[i] = up - x[i];
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 5; ++i) total[i] = 0;
-  for (int w = 0; w < n_thr / 64; ++w)
-#pragma unroll
-    for (int i = 0; i < 5; ++i) {
-      if (w < wave) before[i] += s_sum[w][i];
-      total[i] += s_sum[w][i];
-    }
-#pragma unroll
-  for (int i = 0; i < 5; ++i) x[i] = before[i];
+  for (int i = 0; i < 7; ++i) x[i] = before[i];
   for (int b = b0; b < b1; ++b) {
     s_ptile[b] = x[0];
-    s_punit[b] = x[1];
-    s_pmem[b] = x[2];
-    s_sunit[b] = x[3];
-    s_stile[b] = x[4];
+    s_base[b] = s_shared[b] > 0 ? x[1] : shared_tokens + x[3];  // of a group: right at its leader
+    s_stile[b] = x[2];
+    s_len[b] = x[6];  // tokens of the sequences before; the prefix lengths are no longer needed
+    if (s_count[b] > 0 && tiles_of(s_count[b]) > 1) s_wg[x[5]] = b;  // a list for the moment
     add(b);
+  }
+  if (tid == 0) s_pick[0] = -1;
+  __syncthreads();
+
+  // The cut: `len` units a workgroup.  A prefix of several tiles is cut by itself, all its tiles at the same keys, and the pieces of one
+  // range of keys go to consecutive workgroups, which run at the same time and find what the first of them loads in their XCD's L2.
+  // (Laid end to end its tiles read all keys once each from beyond L2.)  That takes some more workgroups, so `len` is the
+  // shortest of 64 lengths, a lane each, for which there are enough.
+  const int shortest_len = max(kMinUnits, (all_units + a.n_wg - 1) / a.n_wg);
+  const auto pieces_at = [&](int b, int len) {  // 0: cut with everything else
+    const int n = units_of(s_shared[b]);
+    return tiles_of(s_count[b]) > 1 && 2 * (kLeadUnits + n) >= len ? (n + len - kLeadUnits - 1) / (len - kLeadUnits) : 0;
+  };
+  if (wave == 0 && n_multi > 0) {
+    const int len = shortest_len + (shortest_len * lane + 31) / 32;
+    int need = 0, rest = all_units;
+    for (int i = 0; i < n_multi; ++i) {
+      const int b = s_wg[i], n = pieces_at(b, len);
+      need += n * tiles_of(s_count[b]);
+      if (n > 0) rest -= tiles_of(s_count[b]) * (kLeadUnits + units_of(s_shared[b]));
+    }
+    const unsigned long long enough = __ballot(need + (rest + len - 1) / len <= a.n_wg);
+    if (enough != 0 && lane == 0) s_pick[0] = __builtin_ctzll(enough);
+  }
+  __syncthreads();
+  const int pick = s_pick[0];
+  const int len = pick < 0 ? shortest_len : shortest_len + (shortest_len * pick + 31) / 32;
+  const auto pieces_of = [&](int b) { return pick < 0 ? 0 : pieces_at(b, len); };
+  int y[4] = {0, 0, 0, 0}, y_before[4], y_total[4];
+  const auto add_cut = [&](int b) {
+    const int c = s_count[b], own = s_keys[b] - s_shared[b];
+    if (c > 0) {
+      const int n = pieces_of(b);
+      if (n > 0) {
+        y[0] += n * tiles_of(c);
+        y[3] += (n - 1) * tiles_of(c);
+      } else {
+        y[1] += tiles_of(c) * (kLeadUnits + units_of(s_shared[b]));
+      }
+    }
+    if (own > 0) y[2] += tiles_of(s_tok[b]) * (kLeadUnits + units_of(own));
+  };
+  for (int b = b0; b < b1; ++b) add_cut(b);
+  block_sums(y, y_before, y_total, s_sum);
+  const int wg0 = y_total[0], prefix_units = y_total[1], units = prefix_units + y_total[2];
+  const int n_wg = wg0 + (units + len - 1) / len;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = y_before[i];
+  for (int b = b0; b < b1; ++b) {
+    s_wg[b] = y[0];
+    s_unit[b] = y[1];
+    s_own[b] = y[2];
+    if (s_count[b] > 0) s_id[b] = y[3];  // cuts of the groups before; the ids are no longer needed
+    add_cut(b);
   }
   __syncthreads();
 
-  const int p_tiles = total[0], n_tiles = p_tiles + total[4], units = total[1] + total[3];
-  const int len = max(kMinUnits, (units + a.n_wg - 1) / a.n_wg), n_wg = (units + len - 1) / len;
   if (tid == 0) {
     Header* const h = reinterpret_cast<Header*>(a.plan);
     h->magic = kMagic;
     h->B = a.B, h->S = a.S, h->Hq = a.Hq, h->Hc = a.Hc, h->max_batch = a.max_batch, h->max_context = a.max_context;
-    h->len = len, h->n_wg = n_wg, h->n_tiles = n_tiles;
+    h->n_wg = n_wg, h->n_tiles = n_tiles;
   }
+  int* const tokens = reinterpret_cast<int*>(a.plan + a.tokens);
+  int* const place = reinterpret_cast<int*>(a.plan + a.place);
+  const auto base_of = [&](int b) { return s_shared[b] > 0 ? s_base[s_lead[b]] + s_rank[b] : s_base[b]; };
   for (int b = tid; b < a.B; b += n_thr) {
-    Sequence* const q = reinterpret_cast<Sequence*>(a.plan + a.seqs) + b;
     const int lead = s_lead[b];
     const bool shares = s_shared[b] > 0;
-    q->prefix_tile = shares ? s_ptile[lead] : -1;
-    q->prefix_row = shares ? s_rank[b] * a.rows : 0;
-    q->own_tile = s_keys[b] > s_shared[b] ? p_tiles + s_stile[b] : -1;
-    if (shares) reinterpret_cast<int*>(a.plan + a.members)[s_pmem[lead] + s_rank[b]] = b;
+    seqs[b] = Sequence{s_slot[b], s_keys[b], shares ? s_ptile[lead] : -1, s_rank[b] * a.group,
+                       s_keys[b] > s_shared[b] ? p_tiles + s_stile[b] : -1, {0, 0, 0}};
+    if (a.S == 1 && s_tok[b] > 0) tokens[base_of(b)] = b << kTokenShift;
   }
-  // workspace rows: a tile has those of the tiles before it, each once, and 64 for every cut up to its first key
-  const int all_shared_rows = total[2] * a.rows;
+  if (a.S > 1) {
+    for (int b = wave; b < a.B; b += n_waves) {
+      int n = 0;
+      const int base = base_of(b), all = s_tok[b];
+      for (int j0 = 0; j0 < a.S; j0 += 64) {
+        const int j = j0 + lane;
+        const bool on = all > 0 && j < a.S && plan_keys(a, b, j) > 0;
+        const unsigned long long who = __ballot(on);
+        const int at = n + __popcll(who & ((1ull << lane) - 1));
+        if (on && at < all) tokens[base + at] = b << kTokenShift | j;
+        if (j < a.S) place[b * a.S + j] = on ? at : -1;
+        n += __popcll(who);
+      }
+    }
+  }
+  // Workspace rows: behind those of the tiles before it, each once, and 64 for every cut up to a tile's first key; tiles that are cut by
+  // themselves first, then the others along their axis.
+  const int rest_part = shared_tokens * a.group + kTileRows * wg0;
   const auto tile_at = [&](int i) {
     Tile t;
-    int n_units, from, rows_before;
+    int n_units, from = 0, cut = 0, rows_before;
     if (i < p_tiles) {
-      const int b = last_at_or_below(s_ptile, a.B, i), k = i - s_ptile[b], all = s_count[b] * a.rows;
+      const int b = last_at_or_below(s_ptile, a.B, i), k = i - s_ptile[b];
       n_units = units_of(s_shared[b]);
-      from = s_punit[b] + k * (kLeadUnits + n_units);
-      t.base = s_pmem[b];
+      cut = pieces_of(b);
+      t.part = cut > 0 ? s_id[b] + k * (cut - 1) : 0;
+      from = s_unit[b] + k * (kLeadUnits + n_units);
+      t.base = s_base[b];
       t.slot = s_slot[b];
       t.row0 = k * kTileRows;
-      t.n_rows = min(kTileRows, all - t.row0);
+      t.n_rows = min(kTileRows, s_count[b] * a.group - t.row0);
       t.t_begin = 0;
       t.t_end = s_shared[b];
-      rows_before = s_pmem[b] * a.rows + t.row0;
+      t.shared = 1;
+      rows_before = s_base[b] * a.group + t.row0 + (cut > 0 ? 0 : rest_part);
     } else {
       const int b = last_at_or_below(s_stile, a.B, i - p_tiles), k = i - p_tiles - s_stile[b];
       n_units = units_of(s_keys[b] - s_shared[b]);
-      from = total[1] + s_sunit[b] + k * (kLeadUnits + n_units);
-      t.base = -1 - b;
+      from = prefix_units + s_own[b] + k * (kLeadUnits + n_units);
+      t.base = base_of(b);
       t.slot = s_slot[b];
       t.row0 = k * kTileRows;
-      t.n_rows = min(kTileRows, a.rows - t.row0);
+      t.n_rows = min(kTileRows, s_tok[b] * a.group - t.row0);
       t.t_begin = s_shared[b];
       t.t_end = s_keys[b];
-      rows_before = all_shared_rows + b * a.rows + t.row0;
+      t.shared = 0;
+      rows_before = rest_part + (shared_tokens + s_len[b]) * a.group + t.row0;
     }
-    t.first_wg = (from + kLeadUnits) / len;
-    t.n_pieces = (from + kLeadUnits + n_units - 1) / len - t.first_wg + 1;
-    t.part = rows_before + kTileRows * t.first_wg;
+    if (cut > 0) {
+      t.n_pieces = cut;
+    } else {
+      const int first = (from + kLeadUnits) / len;
+      t.n_pieces = (from + kLeadUnits + n_units - 1) / len - first + 1;
+      t.part = first;
+    }
+    t.part = rows_before + kTileRows * t.part;
     t.pad[0] = t.pad[1] = t.pad[2] = 0;
     return t;
   };
   for (int i = tid; i < n_tiles; i += n_thr) reinterpret_cast<Tile*>(a.plan + a.tiles)[i] = tile_at(i);
   for (int w = tid; w < n_wg; w += n_thr) {
     Share s;
-    const int from = w * len;
-    s.units = min(len, units - from);
-    s.pad = 0;
-    if (from < total[1]) {
-      const int b = last_at_or_below(s_punit, a.B, from), n = kLeadUnits + units_of(s_shared[b]), off = from - s_punit[b];
-      s.tile = s_ptile[b] + off / n;
-      s.offset = off % n;
+    if (w < wg0) {
+      const int b = last_at_or_below(s_wg, a.B, w), n = tiles_of(s_count[b]), k = (w - s_wg[b]) / n, i = (w - s_wg[b]) % n;
+      const int all = units_of(s_shared[b]), n_pieces = pieces_of(b);
+      const int from = static_cast<int>(static_cast<int64_t>(all) * k / n_pieces);
+      s.tile = s_ptile[b] + i;
+      s.offset = kLeadUnits + from;
+      s.units = static_cast<int>(static_cast<int64_t>(all) * (k + 1) / n_pieces) - from;
+      s.piece = k;
     } else {
-      const int b = last_at_or_below(s_sunit, a.B, from - total[1]), n = kLeadUnits + units_of(s_keys[b] - s_shared[b]);
-      const int off = from - total[1] - s_sunit[b];
-      s.tile = p_tiles + s_stile[b] + off / n;
-      s.offset = off % n;
+      const int from = (w - wg0) * len;
+      int start;
+      s.units = min(len, units - from);
+      if (from < prefix_units) {
+        const int b = last_at_or_below(s_unit, a.B, from), n = kLeadUnits + units_of(s_shared[b]), off = from - s_unit[b];
+        s.tile = s_ptile[b] + off / n;
+        s.offset = off % n;
+      } else {
+        const int b = last_at_or_below(s_own, a.B, from - prefix_units), n = kLeadUnits + units_of(s_keys[b] - s_shared[b]);
+        const int off = from - prefix_units - s_own[b];
+        s.tile = p_tiles + s_stile[b] + off / n;
+        s.offset = off % n;
+      }
+      start = from - s.offset + kLeadUnits;  // of the tile's first key
+      s.piece = max(0, (from - start / len * len) / len);
     }
     s.first = tile_at(s.tile);
     reinterpret_cast<Share*>(a.plan + a.shares)[w] = s;
@@ -342,9 +457,9 @@ struct SharedArgs {
   int64_t n_slots;
   int max_context;
   float qscale;  // scale * log2(e)
-  int rows, group, group_shift;  // rows of a sequence and cached head, query heads of a cached head
+  int group, group_shift;  // query heads of a cached head
   const char* plan;
-  int64_t seqs, members, shares, tiles;
+  int64_t seqs, tokens, place, shares, tiles;
   float* ws_acc;  // [part rows, Hc, D]
   float* ws_ml;   // [part rows, Hc, 2]
 };
@@ -492,17 +607,10 @@ __device__ __forceinline__ const SharedArgs& reread() {
 
 // Token and head of row r of a tile.
 __device__ __forceinline__ void find_row(const SharedArgs& a, const Tile& tile, int r, int* b, int* j, int* g) {
-  const uint32_t rr = tile.row0 + r;
-  uint32_t x = rr;
-  if (tile.base >= 0) {
-    const uint32_t m = rr / static_cast<uint32_t>(a.rows);
-    x = rr - m * a.rows;
-    *b = reinterpret_cast<const int*>(a.plan + a.members)[tile.base + m];
-  } else {
-    *b = -1 - tile.base;
-  }
-  *j = static_cast<int>(x >> a.group_shift);
-  *g = static_cast<int>(x & (a.group - 1));
+  const int x = tile.row0 + r, token = reinterpret_cast<const int*>(a.plan + a.tokens)[tile.base + (x >> a.group_shift)];
+  *b = token >> kTokenShift;
+  *j = token & ((1 << kTokenShift) - 1);
+  *g = x & (a.group - 1);
 }
 
 // What the products left out of row r: the infinities and NaN of the V rows of keys [t0, t1) that it sees, elements 4 c .. 4 c + 3.
@@ -536,7 +644,7 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
   const int tid = anew(threadIdx.x), lane = tid & 63, hc = blockIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
-  const bool prefix = tile.base >= 0;
+  const bool prefix = tile.shared != 0;
   char* const ring = sh.ring[wave];
   const char* const kplane = a.pool_k + static_cast<int64_t>(hc) * a.n_slots * G::ROWB;
   const char* const vplane = a.pool_v + static_cast<int64_t>(hc) * a.n_slots * G::ROWB;
@@ -856,7 +964,9 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
       }
       if (sh.tainted) add_infinities<E, D>(e, tile, r, max(t0, least), t1, e.pool_v + static_cast<int64_t>(hc) * e.n_slots * G::ROWB, c, num);
       if (sole) {
-        const int b = -1 - tile.base, x = tile.row0 + r, j = x >> e.group_shift, h = hc * e.group + (x & (e.group - 1));
+        int b, j, g;
+        find_row(e, tile, r, &b, &j, &g);
+        const int h = hc * e.group + g;
         const bool any = keys_of(e, b, j) > 0;
         const float lse = (mn + log2f(den)) * kLn2;
         f32x4 res;
@@ -897,11 +1007,11 @@ __global__ __launch_bounds__(kThreads, (sizeof(Shared<E, D>) <= 80 * 1024 ? 2 : 
   const Header h = load_record<Header>(a.plan);
   const Share share = load_record<Share>(a.plan + a.shares + w * static_cast<int64_t>(sizeof(Share)));
   if (!plan_fits(a, h) || w >= h.n_wg) return;
-  int left = share.units, offset = share.offset;
+  int left = share.units, offset = share.offset, piece = share.piece;
   bool busy = false;
   Tile t = share.first;
   for (int i = share.tile;;) {
-    const int all = units_of(t.t_end - t.t_begin), piece = w - t.first_wg;
+    const int all = units_of(t.t_end - t.t_begin);
     const int from = max(0, offset - kLeadUnits), to = min(all, offset + left - kLeadUnits);
     const int t0 = t.t_begin + from * kUnit, t1 = min(t.t_end, t.t_begin + to * kUnit);
     left -= kLeadUnits + all - offset;
@@ -919,6 +1029,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(Shared<E, D>) <= 80 * 1024 ? 2 : 
       run_piece<E, D, 4, false>(a, sh, t, piece, t0, t1);
     }
     if (left <= kLeadUnits || ++i >= h.n_tiles) break;  // the lead alone has no key
+    piece = 0;
     t = load_record<Tile>(a.plan + a.tiles + i * static_cast<int64_t>(sizeof(Tile)));
   }
 }
@@ -941,14 +1052,16 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(const SharedArgs 
   const int keys = keys_of(a, b, j);
   const int64_t slot = a.batch_idx[b];
   const bool valid = slot >= 0 && slot < a.max_batch;
+  const int at_b = !fits || a.S == 1 ? 0 : reinterpret_cast<const int*>(a.plan + a.place)[bj];  // place among the sequence's tokens
+  const bool missing = at_b < 0;
   f32x4 res = {0.f, 0.f, 0.f, 0.f};
   float lse = -INFINITY;
-  if (!fits || (valid && (s.slot != slot || keys > s.keys)) || (!valid && s.slot >= 0)) {
+  if (!fits || (valid && (s.slot != slot || keys > s.keys || (keys > 0 && missing))) || (!valid && s.slot >= 0)) {
     lse = NAN;  // the plan is of another step
     res = f32x4{NAN, NAN, NAN, NAN};
   } else if (valid && keys > 0) {
     const Tile* const tiles = reinterpret_cast<const Tile*>(a.plan + a.tiles);
-    const int hc = h >> a.group_shift, x = (j << a.group_shift) + (h & (a.group - 1));
+    const int hc = h >> a.group_shift, x = (at_b << a.group_shift) + (h & (a.group - 1));
     float m = -INFINITY, den = 0.f;
     f32x4 num = {0.f, 0.f, 0.f, 0.f};
     // the prefix's pieces, then those of its own keys: kBatch of them are on their way at once
@@ -1053,14 +1166,14 @@ extern "C" int fp_shared_decode_plan(const int64_t* batch_idx, const void* input
     return fp::fail(FP_ERR_WORKSPACE, "%s: the plan needs %lld bytes, 16-byte aligned (got %lld)", what,
                     static_cast<long long>(fp_shared_decode_plan_bytes(B, S, Hq, Hc, D)), static_cast<long long>(plan_bytes));
   const Layout l = layout_of(B, S, Hq, Hc);
-  const PlanArgs a{batch_idx, input_pos, pos_index_type, prefix_ids, prefix_lens, B, S, Hq, Hc, l.rows, max_batch, max_context,
-                   l.n_wg, l.max_tiles, static_cast<char*>(plan), l.seqs, l.members, l.shares, l.tiles};
+  const PlanArgs a{batch_idx, input_pos, pos_index_type, prefix_ids, prefix_lens, B, S, Hq, Hc, Hq / Hc, max_batch, max_context,
+                   l.n_wg, static_cast<char*>(plan), l.seqs, l.tokens, l.place, l.shares, l.tiles};
   int threads = (B + 63) / 64 * 64;
-  threads = threads < 256 ? 256 : threads > 1024 ? 1024 : threads;
-  const size_t lds = 13 * static_cast<size_t>((B + 3) & ~3) * sizeof(int);
+  threads = S > 1 || threads > 1024 ? 1024 : threads < 256 ? 256 : threads;  // a wavefront a sequence, or a thread
+  const size_t lds = kPlanArrays * static_cast<size_t>((B + 3) & ~3) * sizeof(int);
   if (lds > 64 * 1024) {
     static const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(shared_plan_kernel),
-                                                          hipFuncAttributeMaxDynamicSharedMemorySize, 13 * kMaxSequences * sizeof(int));
+                                                          hipFuncAttributeMaxDynamicSharedMemorySize, kPlanArrays * kMaxSequences * sizeof(int));
     if (allowed != hipSuccess) return fp::fail(FP_ERR_LAUNCH, "%s: %s", what, hipGetErrorString(allowed));
   }
   hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3(threads), lds, static_cast<hipStream_t>(stream), a);
@@ -1108,8 +1221,8 @@ extern "C" int fp_paged_decode_shared(const void* q, int64_t q_stride_b, int64_t
                      static_cast<const char*>(pool_k), static_cast<const char*>(pool_v), page_table, pt_row_stride, batch_idx,
                      input_pos, pos_index_type, static_cast<char*>(out), out_stride_b * e, out_stride_h * e, out_stride_s * e,
                      lse, sinks, B, S, Hq, Hc, fp::PageDiv(page_size), n_pages, max_batch,
-                     static_cast<int>(n_slots / page_size), n_slots, max_context, scale * kLog2e, l.rows, G, fp::log2_exact(G),
-                     static_cast<const char*>(plan), l.seqs, l.members, l.shares, l.tiles, acc, acc + l.part_rows * Hc * D};
+                     static_cast<int>(n_slots / page_size), n_slots, max_context, scale * kLog2e, G, fp::log2_exact(G),
+                     static_cast<const char*>(plan), l.seqs, l.tokens, l.place, l.shares, l.tiles, acc, acc + l.part_rows * Hc * D};
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const auto go = [&](auto element) {
     using E = decltype(element);

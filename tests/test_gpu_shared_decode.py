@@ -284,3 +284,26 @@ def test_long_prefixes_and_uneven_heads():
     """Three cached heads: the cut is for a number of workgroups that divides nothing evenly."""
     case = SharedBatch(30, [5000, 1333], one_each([0, 1, 0, 0, 1], [700, 3, 1, 50, 2222]), Hq=6, Hc=3, D=128, P=128, dtype=BF16).on()
     case.check(case.call(ops))
+
+
+@pytest.mark.parametrize("D,Hq,Hc,dtype", [(128, 4, 2, BF16), (64, 16, 2, F16), (128, 8, 2, F32)])
+def test_prefixes_of_several_tiles_beside_others(D, Hq, Hc, dtype):
+    """Groups whose rows fill several tiles are cut by themselves, small ones and own keys together; some are too short for that."""
+    groups = [0] * 90 + [1] * 70 + [2] * 3 + [3] * 40 + [-1] * 7
+    order = torch.randperm(len(groups), generator=torch.Generator().manual_seed(3)).tolist()
+    groups = [groups[i] for i in order]
+    case = SharedBatch(31, [1500, 640, 2000, 70], one_each(groups, [1 + 13 * i % 60 for i in range(len(groups))]), Hq=Hq, Hc=Hc, D=D,
+                       P=64, dtype=dtype).on()
+    case.check(case.call(ops))
+
+
+def test_tokens_in_any_places():
+    """Tokens need not come first in their rows: -1 may stand anywhere."""
+    case = SharedBatch(32, [190, 300], [(0, 70, 70), (0, 70, 70), (1, 80, 70), (-1, 90, 70), (1, 71, 70)], Hq=4, Hc=2, D=64, P=32,
+                       dtype=BF16, S=70)
+    case.pos[torch.rand(case.pos.shape, generator=case.gen) < 0.4] = -1
+    case.pos[1] = -1
+    case.pos[2, :66] = -1
+    case.on()
+    case.check(case.call(ops))
+    case.check(case.call(ops, pos=case.pos_d.long()))
