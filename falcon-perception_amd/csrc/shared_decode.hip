@@ -36,7 +36,6 @@ constexpr int kMaxRows = 1 << 20;      // B * S * heads of a group
 constexpr int kMaxContext = 1 << 21;   // with the rows: units of all tiles fit 31 bits
 constexpr int kTileRows = 64;
 constexpr int kUnit = 64;              // keys: what the cut is made of
-constexpr int kLeadUnits = 3;          // what a tile costs before its first key and behind its last, in units
 constexpr int kMinUnits = 4;           // a workgroup's share at least
 constexpr int kMinShared = 64;         // keys of a prefix that are worth a tile of their own
 constexpr int kSegPages = 1024;        // page ids held in LDS
@@ -72,7 +71,8 @@ struct Tile {
   int n_pieces;
   int part;            // workspace row of the first piece's first row; piece after piece
   int shared;          // of a group
-  int pad[3];
+  int lead;            // units that stand for what it costs before its first key and behind its last
+  int pad[2];
 };
 struct Share {
   int tile, offset, units;  // first tile, units of it (lead included) that belong to workgroups before, units to do
@@ -120,6 +120,9 @@ struct PlanArgs {
   int64_t seqs, tokens, place, shares, tiles;
 };
 
+// What a tile costs before its first key and behind its last, in units.
+__device__ __forceinline__ int lead_of(int rows) { return rows <= 32 ? 3 : 5; }
+
 __device__ __forceinline__ int units_of(int keys) { return (keys + kUnit - 1) / kUnit; }
 
 // last i of 0 .. n - 1 with at[i] <= x (at[0] is 0)
@@ -141,22 +144,20 @@ __device__ __forceinline__ int plan_keys(const PlanArgs& a, int b, int j) {
 // Sums over the threads before this one and over all, of N numbers a thread.
 template <int N>
 __device__ __forceinline__ void block_sums(const int (&x)[N], int (&before)[N], int (&total)[N], int* s_sum) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n_waves = blockDim.x >> 6;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int up = fp_decode::scan_lanes(x[i]);
     if (lane == 63) s_sum[wave * N + i] = up;
     before[i] = up - x[i];
-    total[i] = 0;
   }
   __syncthreads();
-  for (int w = 0; w < static_cast<int>(blockDim.x) / 64; ++w)
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int y = s_sum[w * N + i];
-      if (w < wave) before[i] += y;
-      total[i] += y;
-    }
+  for (int i = 0; i < N; ++i) {  // the wavefronts' sums, one a lane
+    const int y = lane < n_waves ? s_sum[lane * N + i] : 0, up = fp_decode::scan_lanes(y);
+    total[i] = __builtin_amdgcn_readlane(up, 63);
+    before[i] += __builtin_amdgcn_readlane(up, wave) - __builtin_amdgcn_readlane(y, wave);
+  }
   __syncthreads();
 }
 
@@ -183,63 +184,78 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   __shared__ int s_sum[16 * 7], s_pick[1];
   const int tid = threadIdx.x, n_thr = blockDim.x, lane = tid & 63, wave = tid >> 6, n_waves = n_thr / 64;
   Sequence* const seqs = reinterpret_cast<Sequence*>(a.plan + a.seqs);
-
-  const auto put = [&](int b, int keys, int tokens) {
+  // until the sums below, these three hold a group's sequences, shortest prefix length and most keys, at its first sequence
+  int* const s_members = s_ptile;
+  int* const s_shortest = s_base;
+  int* const s_longest = s_stile;
+  for (int b = tid; b < Bp; b += n_thr) {
     const int64_t slot = b < a.B ? a.batch_idx[b] : -1;
     const bool valid = slot >= 0 && slot < a.max_batch;
-    if (!valid) keys = tokens = 0;
-    s_id[b] = keys > 0 ? max(a.ids[slot], 0) : 0;
-    s_len[b] = keys > 0 ? max(a.lens[slot], 0) : 0;
+    const int keys = a.S == 1 && valid ? plan_keys(a, b, 0) : 0;
+    s_id[b] = valid ? max(a.ids[slot], 0) : 0;
+    s_len[b] = valid ? max(a.lens[slot], 0) : 0;
     s_keys[b] = keys;
-    s_tok[b] = tokens;
+    s_tok[b] = keys > 0;
     s_slot[b] = valid ? static_cast<int>(slot) : -1;
-  };
-  if (a.S == 1) {
-    for (int b = tid; b < Bp; b += n_thr) {
-      const int keys = b < a.B ? plan_keys(a, b, 0) : 0;
-      put(b, keys, keys > 0);
-    }
-  } else {  // a wavefront a sequence
-    for (int b = wave; b < Bp; b += n_waves) {
-      int keys = 0, tokens = 0;
-      for (int j0 = 0; j0 < a.S && b < a.B; j0 += 64) {
-        const int k = j0 + lane < a.S ? plan_keys(a, b, j0 + lane) : 0;
-        keys = max(keys, fp::wave_max(k));
-        tokens += __popcll(__ballot(k > 0));
-      }
-      if (lane == 0) put(b, keys, tokens);
-    }
+    s_lead[b] = b;
+    s_rank[b] = s_count[b] = s_members[b] = s_longest[b] = 0;
+    s_shortest[b] = INT32_MAX;
   }
   __syncthreads();
+  if (a.S > 1) {
+    for (int i = tid; i < a.B * a.S; i += n_thr) {
+      const int b = static_cast<uint32_t>(i) / static_cast<uint32_t>(a.S), keys = s_slot[b] < 0 ? 0 : plan_keys(a, b, i - b * a.S);
+      if (keys > 0) {
+        atomicMax(&s_keys[b], keys);
+        atomicAdd(&s_tok[b], 1);
+      }
+    }
+    __syncthreads();
+  }
 
-  // groups: every sequence looks at all of them (LDS broadcasts, four ids at a time)
-  for (int b = tid; b < a.B; b += n_thr) {
-    const int id = s_id[b];
-    int lead = b, rank = 0, members = 0, tokens = 0, shortest = INT32_MAX, longest = 0;
-    if (id > 0) {
-      for (int j = 0; j < Bp; j += 4) {
-        const i32x4 four = *reinterpret_cast<const i32x4*>(s_id + j);
+  // Groups.  The first sequence with the same id leads, and a sequence's place is behind the tokens of those before it: sequences
+  // look at all before them, four at a time, some threads a sequence.  A sequence without a token belongs to no group.
+  {
+    const int wide = (a.B + 63) & ~63, parts = max(1, n_thr / wide), part = tid / wide;
+    const int quads = (Bp / 4 + parts - 1) / parts;  // that a thread looks at
+    for (int b = parts > 1 ? tid - part * wide : tid; b < a.B && part < parts; b += n_thr) {
+      const int id = s_tok[b] > 0 ? s_id[b] : 0;
+      if (id == 0) continue;
+      int lead = b, rank = 0;
+      const int from = parts > 1 ? part * quads * 4 : 0, to = min(b, from + quads * 4);
+      for (int j = from; j < to; j += 4) {
+        const i32x4 ids = *reinterpret_cast<const i32x4*>(s_id + j), toks = *reinterpret_cast<const i32x4*>(s_tok + j);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if (four[i] != id) continue;
-          ++members;
-          tokens += s_tok[j + i];
-          rank += j + i < b ? s_tok[j + i] : 0;
-          lead = min(lead, j + i);
-          shortest = min(shortest, s_len[j + i]);
-          longest = max(longest, s_keys[j + i]);
+          const int tokens = ids[i] == id && j + i < b ? toks[i] : 0;
+          rank += tokens;
+          lead = min(lead, tokens > 0 ? j + i : b);
         }
       }
+      if (lead < b) atomicMin(&s_lead[b], lead);
+      if (rank > 0) atomicAdd(&s_rank[b], rank);
     }
-    const int shared = members >= 2 ? min(shortest, longest) : 0;
-    const bool shares = shared >= kMinShared;
+  }
+  __syncthreads();
+  for (int b = tid; b < a.B; b += n_thr) {
+    if (s_id[b] == 0 || s_tok[b] == 0) continue;
+    const int lead = s_lead[b];
+    atomicAdd(&s_count[lead], s_tok[b]);
+    atomicAdd(&s_members[lead], 1);
+    atomicMin(&s_shortest[lead], s_len[b]);
+    atomicMax(&s_longest[lead], s_keys[b]);
+  }
+  __syncthreads();
+  for (int b = tid; b < a.B; b += n_thr) {
+    const int lead = s_lead[b], shared = s_members[lead] >= 2 ? min(s_shortest[lead], s_longest[lead]) : 0;
+    const bool shares = s_tok[b] > 0 && s_id[b] > 0 && shared >= kMinShared;
     s_shared[b] = shares ? shared : 0;
-    s_count[b] = shares && lead == b ? tokens : 0;
-    s_rank[b] = shares ? rank : 0;
-    s_lead[b] = lead;
+    if (!shares) s_rank[b] = 0;
+    if (!shares || lead != b) s_count[b] = 0;
   }
   __syncthreads();
 
+  const auto lead_for = [&](int tokens) { return lead_of(tokens * a.group); };
   const auto tiles_of = [&](int tokens) { return (tokens * a.group + kTileRows - 1) / kTileRows; };
   // sums over the sequences before, consecutive ones a thread
   const int per = (a.B + n_thr - 1) / n_thr, b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
@@ -249,12 +265,12 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
     if (c > 0) {
       x[0] += tiles_of(c);
       x[1] += c;
-      x[4] += tiles_of(c) * (kLeadUnits + units_of(s_shared[b]));
+      x[4] += tiles_of(c) * (lead_for(c) + units_of(s_shared[b]));
       x[5] += tiles_of(c) > 1;
     }
     if (own > 0) {
       x[2] += tiles_of(s_tok[b]);
-      x[4] += tiles_of(s_tok[b]) * (kLeadUnits + units_of(own));
+      x[4] += tiles_of(s_tok[b]) * (lead_for(s_tok[b]) + units_of(own));
     }
     if (s_shared[b] == 0) x[3] += s_tok[b];
     x[6] += s_tok[b];
@@ -282,7 +298,8 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   const int shortest_len = max(kMinUnits, (all_units + a.n_wg - 1) / a.n_wg);
   const auto pieces_at = [&](int b, int len) {  // 0: cut with everything else
     const int n = units_of(s_shared[b]);
-    return tiles_of(s_count[b]) > 1 && 2 * (kLeadUnits + n) >= len ? (n + len - kLeadUnits - 1) / (len - kLeadUnits) : 0;
+    const int lead = lead_for(s_count[b]), room = max(1, len - lead);
+    return tiles_of(s_count[b]) > 1 && 2 * (lead + n) >= len ? (n + room - 1) / room : 0;
   };
   if (wave == 0 && n_multi > 0) {
     const int len = shortest_len + (shortest_len * lane + 31) / 32;
@@ -290,7 +307,7 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
     for (int i = 0; i < n_multi; ++i) {
       const int b = s_wg[i], n = pieces_at(b, len);
       need += n * tiles_of(s_count[b]);
-      if (n > 0) rest -= tiles_of(s_count[b]) * (kLeadUnits + units_of(s_shared[b]));
+      if (n > 0) rest -= tiles_of(s_count[b]) * (lead_for(s_count[b]) + units_of(s_shared[b]));
     }
     const unsigned long long enough = __ballot(need + (rest + len - 1) / len <= a.n_wg);
     if (enough != 0 && lane == 0) s_pick[0] = __builtin_ctzll(enough);
@@ -308,10 +325,10 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
         y[0] += n * tiles_of(c);
         y[3] += (n - 1) * tiles_of(c);
       } else {
-        y[1] += tiles_of(c) * (kLeadUnits + units_of(s_shared[b]));
+        y[1] += tiles_of(c) * (lead_for(c) + units_of(s_shared[b]));
       }
     }
-    if (own > 0) y[2] += tiles_of(s_tok[b]) * (kLeadUnits + units_of(own));
+    if (own > 0) y[2] += tiles_of(s_tok[b]) * (lead_for(s_tok[b]) + units_of(own));
   };
   for (int b = b0; b < b1; ++b) add_cut(b);
   block_sums(y, y_before, y_total, s_sum);
@@ -370,7 +387,8 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
       n_units = units_of(s_shared[b]);
       cut = pieces_of(b);
       t.part = cut > 0 ? s_id[b] + k * (cut - 1) : 0;
-      from = s_unit[b] + k * (kLeadUnits + n_units);
+      t.lead = lead_for(s_count[b]);
+      from = s_unit[b] + k * (t.lead + n_units);
       t.base = s_base[b];
       t.slot = s_slot[b];
       t.row0 = k * kTileRows;
@@ -382,7 +400,8 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
     } else {
       const int b = last_at_or_below(s_stile, a.B, i - p_tiles), k = i - p_tiles - s_stile[b];
       n_units = units_of(s_keys[b] - s_shared[b]);
-      from = prefix_units + s_own[b] + k * (kLeadUnits + n_units);
+      t.lead = lead_for(s_tok[b]);
+      from = prefix_units + s_own[b] + k * (t.lead + n_units);
       t.base = base_of(b);
       t.slot = s_slot[b];
       t.row0 = k * kTileRows;
@@ -395,40 +414,46 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
     if (cut > 0) {
       t.n_pieces = cut;
     } else {
-      const int first = (from + kLeadUnits) / len;
-      t.n_pieces = (from + kLeadUnits + n_units - 1) / len - first + 1;
+      const int first = (from + t.lead) / len;
+      t.n_pieces = (from + t.lead + n_units - 1) / len - first + 1;
       t.part = first;
     }
     t.part = rows_before + kTileRows * t.part;
-    t.pad[0] = t.pad[1] = t.pad[2] = 0;
+    t.pad[0] = t.pad[1] = 0;
     return t;
   };
-  for (int i = tid; i < n_tiles; i += n_thr) reinterpret_cast<Tile*>(a.plan + a.tiles)[i] = tile_at(i);
-  for (int w = tid; w < n_wg; w += n_thr) {
+  for (int i = tid; i < n_wg + n_tiles; i += n_thr) {
+    if (i >= n_wg) {
+      reinterpret_cast<Tile*>(a.plan + a.tiles)[i - n_wg] = tile_at(i - n_wg);
+      continue;
+    }
+    const int w = i;
     Share s;
     if (w < wg0) {
-      const int b = last_at_or_below(s_wg, a.B, w), n = tiles_of(s_count[b]), k = (w - s_wg[b]) / n, i = (w - s_wg[b]) % n;
+      const int b = last_at_or_below(s_wg, a.B, w), n = tiles_of(s_count[b]), k = (w - s_wg[b]) / n;
       const int all = units_of(s_shared[b]), n_pieces = pieces_of(b);
       const int from = static_cast<int>(static_cast<int64_t>(all) * k / n_pieces);
-      s.tile = s_ptile[b] + i;
-      s.offset = kLeadUnits + from;
+      s.tile = s_ptile[b] + (w - s_wg[b]) % n;
+      s.offset = lead_for(s_count[b]) + from;
       s.units = static_cast<int>(static_cast<int64_t>(all) * (k + 1) / n_pieces) - from;
       s.piece = k;
     } else {
       const int from = (w - wg0) * len;
-      int start;
+      int lead, start;
       s.units = min(len, units - from);
       if (from < prefix_units) {
-        const int b = last_at_or_below(s_unit, a.B, from), n = kLeadUnits + units_of(s_shared[b]), off = from - s_unit[b];
+        const int b = last_at_or_below(s_unit, a.B, from), n = lead_for(s_count[b]) + units_of(s_shared[b]), off = from - s_unit[b];
+        lead = lead_for(s_count[b]);
         s.tile = s_ptile[b] + off / n;
         s.offset = off % n;
       } else {
-        const int b = last_at_or_below(s_own, a.B, from - prefix_units), n = kLeadUnits + units_of(s_keys[b] - s_shared[b]);
+        const int b = last_at_or_below(s_own, a.B, from - prefix_units), n = lead_for(s_tok[b]) + units_of(s_keys[b] - s_shared[b]);
+        lead = lead_for(s_tok[b]);
         const int off = from - prefix_units - s_own[b];
         s.tile = p_tiles + s_stile[b] + off / n;
         s.offset = off % n;
       }
-      start = from - s.offset + kLeadUnits;  // of the tile's first key
+      start = from - s.offset + lead;  // of the tile's first key
       s.piece = max(0, (from - start / len * len) / len);
     }
     s.first = tile_at(s.tile);
@@ -586,7 +611,8 @@ struct Shared {
   using G = Geo<E, D>;
   __attribute__((aligned(1024))) char ring[kWaves][G::RING];
   int pages[kSegPages];
-  float ml[kWaves][kTileRows][2];
+  __attribute__((aligned(8))) float ml[kWaves][kTileRows][2];
+  float joined[kTileRows][2];    // maximum and sum of all wavefronts
   int limit[kWaves][kTileRows];  // keys of the columns' rows, each wavefront's own copy
   int tainted;  // an element of V that is not finite was left out
 };
@@ -653,20 +679,42 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
   // rows: query operands and limits of this lane's columns.  A column without a row repeats row 0, sees everything and is not stored.
   v4u q[CB][G::QV];
   int least = INT32_MAX;
-#pragma unroll
-  for (int cb = 0; cb < CB; ++cb) {
+  {
+    // two trips to memory: the tokens, then what they name
     const SharedArgs& a = reread();
-    const int r = kSplit ? col & 7 : cb * 16 + col;
-    const bool on = r < tile.n_rows;
-    int b, j, g;
-    find_row(a, tile, on ? r : 0, &b, &j, &g);
-    const int h = hc * a.group + g;
-    const int lim = on ? keys_of(a, b, j) : INT32_MAX;
-    least = min(least, lim);
-    if (grp == 0) sh.limit[wave][cb * 16 + col] = lim;
-    const char* const src = a.q + b * a.qs_b + h * a.qs_h + j * a.qs_s + grp * 16;
+    const int* const tokens = reinterpret_cast<const int*>(a.plan + a.tokens) + tile.base;
+    int x[CB], token[CB];
 #pragma unroll
-    for (int kk = 0; kk < G::QV; ++kk) q[cb][kk] = *reinterpret_cast<const v4u*>(src + kk * 64);
+    for (int cb = 0; cb < CB; ++cb) {
+      const int r = kSplit ? col & 7 : cb * 16 + col;
+      x[cb] = tile.row0 + (r < tile.n_rows ? r : 0);
+      token[cb] = tokens[x[cb] >> a.group_shift];
+    }
+    int64_t pos[CB];
+    const auto at = [&](int cb) { return static_cast<int64_t>(token[cb] >> kTokenShift) * a.S + (token[cb] & ((1 << kTokenShift) - 1)); };
+    if (a.pos_i64) {
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb) pos[cb] = static_cast<const int64_t*>(a.input_pos)[at(cb)];
+    } else {
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb) pos[cb] = static_cast<const int32_t*>(a.input_pos)[at(cb)];
+    }
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) {
+      const int b = token[cb] >> kTokenShift, j = token[cb] & ((1 << kTokenShift) - 1), h = hc * a.group + (x[cb] & (a.group - 1));
+      const char* const src = a.q + b * a.qs_b + h * a.qs_h + j * a.qs_s + grp * 16;
+#pragma unroll
+      for (int kk = 0; kk < G::QV; ++kk) q[cb][kk] = *reinterpret_cast<const v4u*>(src + kk * 64);
+    }
+    __builtin_amdgcn_sched_barrier(0);  // all of them are on their way before the first is waited for
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) {
+      const int r = kSplit ? col & 7 : cb * 16 + col;
+      const int64_t keys = pos[cb] < 0 ? 0 : pos[cb] >= a.max_context ? a.max_context : pos[cb] + 1;
+      const int lim = r < tile.n_rows ? static_cast<int>(keys) : INT32_MAX;
+      least = min(least, lim);
+      if (grp == 0) sh.limit[wave][cb * 16 + col] = lim;
+    }
   }
   least = -fp::wave_max(-least);
   if (tid == 0) sh.tainted = 0;  // ahead of the barriers of the first segment
@@ -706,6 +754,12 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
         sh.pages[i] = static_cast<int>(page);
       }
       __syncthreads();
+      // The query rows are waited for here.  At their first use, inside the loop over the stages, the wait would be one of every
+      // stage, and for the stages on their way, too, of which the compiler does not know.
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+        for (int kk = 0; kk < G::QV; ++kk) asm volatile("" : "+v"(q[cb][kk]));
     }
 
     const auto issue = [&](int c0, char* stage) {
@@ -903,7 +957,8 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
     seg0 = seg1;
   }
 
-  // The wavefronts' states meet in LDS, PASS column blocks at a time, chunks permuted against bank conflicts.
+  // The wavefronts' states meet in LDS: maxima and sums first, then the accumulators, scaled to the common maximum, PASS column blocks
+  // at a time, chunks permuted against bank conflicts.
 #pragma unroll
   for (int cb = 0; cb < CB; ++cb) {
     if constexpr (kSplit) {
@@ -919,10 +974,25 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
     }
     l[cb] += __shfl_xor(l[cb], 16);
     l[cb] += __shfl_xor(l[cb], 32);
-    if (grp == 0) {
-      sh.ml[wave][cb * 16 + col][0] = m[cb];
-      sh.ml[wave][cb * 16 + col][1] = l[cb];
+    if (grp == 0) *reinterpret_cast<float2*>(sh.ml[wave][cb * 16 + col]) = float2{m[cb], l[cb]};
+  }
+  __syncthreads();
+#pragma unroll
+  for (int cb = 0; cb < CB; ++cb) {
+    float2 ml[kWaves];
+    float mn = -INFINITY, den = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      ml[w] = *reinterpret_cast<const float2*>(sh.ml[w][cb * 16 + col]);
+      mn = fmaxf(mn, ml[w].x);
     }
+    const float ms = safe_max(mn);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) den += ml[w].y * fast_exp2(ml[w].x - ms);
+    if (wave == 0 && grp == 0) *reinterpret_cast<float2*>(sh.joined[cb * 16 + col]) = float2{mn, den};
+    const float scale = fast_exp2(m[cb] - ms);
+#pragma unroll
+    for (int db = 0; db < G::DB; ++db) o[cb][db] *= scale;
   }
   const SharedArgs& e = reread();
   const bool sole = !prefix && tile.n_pieces == 1 && tile.t_begin == 0;  // nothing to join: the result itself
@@ -950,18 +1020,11 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
     for (int i = tid; i < kRows * C4; i += kThreads) {
       const int row = i / C4, c = i % C4, r = cb0 * 16 + row;
       if (r >= tile.n_rows) break;
-      float mn = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) mn = fmaxf(mn, sh.ml[w][r][0]);
-      const float ms = safe_max(mn);
+      const float2 ml = *reinterpret_cast<const float2*>(sh.joined[r]);
+      const float mn = ml.x, den = ml.y;
       f32x4 num = {0.f, 0.f, 0.f, 0.f};
-      float den = 0.f;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        const float wgt = fast_exp2(sh.ml[w][r][0] - ms);
-        num += reinterpret_cast<const f32x4*>(sh.ring[w])[row * C4 + (c ^ (row & 15))] * wgt;
-        den += sh.ml[w][r][1] * wgt;
-      }
+      for (int w = 0; w < kWaves; ++w) num += reinterpret_cast<const f32x4*>(sh.ring[w])[row * C4 + (c ^ (row & 15))];
       if (sh.tainted) add_infinities<E, D>(e, tile, r, max(t0, least), t1, e.pool_v + static_cast<int64_t>(hc) * e.n_slots * G::ROWB, c, num);
       if (sole) {
         int b, j, g;
@@ -1012,9 +1075,9 @@ __global__ __launch_bounds__(kThreads, (sizeof(Shared<E, D>) <= 80 * 1024 ? 2 : 
   Tile t = share.first;
   for (int i = share.tile;;) {
     const int all = units_of(t.t_end - t.t_begin);
-    const int from = max(0, offset - kLeadUnits), to = min(all, offset + left - kLeadUnits);
+    const int from = max(0, offset - t.lead), to = min(all, offset + left - t.lead);
     const int t0 = t.t_begin + from * kUnit, t1 = min(t.t_end, t.t_begin + to * kUnit);
-    left -= kLeadUnits + all - offset;
+    left -= t.lead + all - offset;
     offset = 0;
     if (to > from) {
     if (busy) __syncthreads();  // the piece before has left LDS
@@ -1028,7 +1091,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(Shared<E, D>) <= 80 * 1024 ? 2 : 
     else
       run_piece<E, D, 4, false>(a, sh, t, piece, t0, t1);
     }
-    if (left <= kLeadUnits || ++i >= h.n_tiles) break;  // the lead alone has no key
+    if (left <= 0 || ++i >= h.n_tiles) break;
     piece = 0;
     t = load_record<Tile>(a.plan + a.tiles + i * static_cast<int64_t>(sizeof(Tile)));
   }
@@ -1168,8 +1231,7 @@ extern "C" int fp_shared_decode_plan(const int64_t* batch_idx, const void* input
   const Layout l = layout_of(B, S, Hq, Hc);
   const PlanArgs a{batch_idx, input_pos, pos_index_type, prefix_ids, prefix_lens, B, S, Hq, Hc, Hq / Hc, max_batch, max_context,
                    l.n_wg, static_cast<char*>(plan), l.seqs, l.tokens, l.place, l.shares, l.tiles};
-  int threads = (B + 63) / 64 * 64;
-  threads = S > 1 || threads > 1024 ? 1024 : threads < 256 ? 256 : threads;  // a wavefront a sequence, or a thread
+  const int threads = S > 1 || B > 64 ? 1024 : 256;
   const size_t lds = kPlanArrays * static_cast<size_t>((B + 3) & ~3) * sizeof(int);
   if (lds > 64 * 1024) {
     static const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(shared_plan_kernel),
