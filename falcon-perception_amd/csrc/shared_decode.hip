@@ -564,6 +564,12 @@ __device__ __forceinline__ s16x4 lds_read_tr(const char* p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p));
 }
 
+// fp::load_to_lds for rows that no other workgroup reads (non-temporal).
+__device__ __forceinline__ void load_once(const char* base, uint32_t offset, uint32_t own, uint32_t constant) {
+  asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3 nt"
+               : : "s"(own), "s"(constant), "v"(offset), "s"(base) : "memory", "scc");
+}
+
 // this wavefront's staging loads but the `kLater` issued last have landed in LDS
 template <int kLater>
 __device__ __forceinline__ void wait_staged() {
@@ -617,9 +623,11 @@ struct Shared {
   int tainted;  // an element of V that is not finite was left out
 };
 
-// x, worked out again where it is used: what follows from it is not kept in registers through the loops around.
-__device__ __forceinline__ int anew(int x) {
-  asm volatile("" : "+v"(x));
+// This lane's number, worked out where it is used: kept through the loop over the keys it would be a register of the loop, and so
+// would all that follows from it.
+__device__ __forceinline__ int lane_id() {
+  int x;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(x));
   return x;
 }
 
@@ -664,14 +672,13 @@ __device__ __forceinline__ void add_infinities(const SharedArgs& a, const Tile& 
 // One piece: the rows of a tile over its keys [t0, t1).  CB blocks of 16 columns; kSplit: at most 8 rows, in columns 0 .. 7 and again in
 // 8 .. 15, whose probabilities carry what the rounding of the first left over.
 template <typename E, int D, int CB, bool kSplit>
-__device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh, const Tile& tile, const int piece, const int t0,
-                                          const int t1) {
+__device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh, const int wave, const Tile& tile, const int piece,
+                                          const int t0, const int t1) {
   using G = Geo<E, D>;
-  const int tid = anew(threadIdx.x), lane = tid & 63, hc = blockIdx.x;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int col = lane & 15, grp = lane >> 4;
+  const int hc = blockIdx.x;
   const bool prefix = tile.shared != 0;
   char* const ring = sh.ring[wave];
+  const uint32_t lds_ring = fp::lds_address(ring);
   const char* const kplane = a.pool_k + static_cast<int64_t>(hc) * a.n_slots * G::ROWB;
   const char* const vplane = a.pool_v + static_cast<int64_t>(hc) * a.n_slots * G::ROWB;
   const int64_t* const table = a.page_table + static_cast<int64_t>(tile.slot) * a.pt_row_stride;
@@ -681,6 +688,7 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
   int least = INT32_MAX;
   {
     // two trips to memory: the tokens, then what they name
+    const int lane = lane_id(), col = lane & 15, grp = lane >> 4;
     const SharedArgs& a = reread();
     const int* const tokens = reinterpret_cast<const int*>(a.plan + a.tokens) + tile.base;
     int x[CB], token[CB];
@@ -717,7 +725,7 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
     }
   }
   least = -fp::wave_max(-least);
-  if (tid == 0) sh.tainted = 0;  // ahead of the barriers of the first segment
+  if (wave == 0 && lane_id() == 0) sh.tainted = 0;  // ahead of the barriers of the first segment
 
   f32x4 o[CB][G::DB];
   float m[CB], l[CB];
@@ -729,11 +737,6 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
     for (int db = 0; db < G::DB; ++db) o[cb][db] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  // byte offset inside row r of a stage of what goes to position p of the row
-  const auto k_off = [](int p, int r) { return static_cast<uint32_t>((p ^ G::k_swz(r)) * 16); };
-  const auto v_off = [](int p, int r) {
-    return static_cast<uint32_t>(G::k16 ? (p ^ G::v_swz(r) * 2) * 16 : p * 16);
-  };
   const bool aligned_pages = a.pd.shift >= 0 && a.pd.page_size % G::TS == 0;
 
   for (int seg0 = t0; seg0 < t1;) {
@@ -747,7 +750,7 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
       int unused;
       a.pd.split(seg1 - 1, last, unused);
       __syncthreads();  // the page ids before are no longer read
-      for (int i = tid; i <= static_cast<int>(last - blk0); i += kThreads) {
+      for (int i = wave * 64 + lane_id(); i <= static_cast<int>(last - blk0); i += kThreads) {
         int64_t page = 0;
         if (blk0 + i < a.n_pages) page = table[blk0 + i];
         if (page < 0 || page >= a.pool_pages) page = 0;  // as paged_decode: the reserved page
@@ -762,61 +765,74 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
         for (int kk = 0; kk < G::QV; ++kk) asm volatile("" : "+v"(q[cb][kk]));
     }
 
-    const auto issue = [&](int c0, char* stage) {
-      const int at_lane = anew(lane), lrow = at_lane / G::CPR, lpos = at_lane % G::CPR;
-      if (aligned_pages && c0 % G::TS == 0 && c0 + G::TS <= seg1) {
-        const int page = __builtin_amdgcn_readfirstlane(sh.pages[(c0 >> a.pd.shift) - static_cast<int>(blk0)]);
-        const int64_t slot = static_cast<int64_t>(page) * a.pd.page_size + (c0 & (a.pd.page_size - 1));
+    // pool row of the first key of a stage that lies in one page and in the segment, -1: not such a stage
+    const auto locate = [&](int c0) {
+      if (!aligned_pages || c0 % G::TS != 0 || c0 + G::TS > seg1) return static_cast<int64_t>(-1);
+      const int page = __builtin_amdgcn_readfirstlane(sh.pages[(c0 >> a.pd.shift) - static_cast<int>(blk0)]);
+      return static_cast<int64_t>(page) * a.pd.page_size + (c0 & (a.pd.page_size - 1));
+    };
+    const auto issue = [&](int64_t slot, int c0, uint32_t stage) {
+      // Instruction i brings rows i * RPI + lrow, position lpos of each.  The permutations of a row are those of i * RPI and of lrow
+      // together, so a load's offset is one exclusive or and one sum away from the first one's.
+      const int at = lane_id(), lrow = at / G::CPR, lpos = at % G::CPR;
+      const uint32_t k_at = lrow * G::ROWB + (lpos ^ G::k_swz(lrow)) * 16, v_at = lrow * G::ROWB + (lpos ^ G::v_swz(lrow) * 2) * 16;
+      if (slot >= 0) {
+        const char* const k = kplane + slot * G::ROWB;
+        const char* const v = vplane + slot * G::ROWB;
         if (prefix) {  // other tiles read these rows, too
 #pragma unroll
-          for (int i = 0; i < G::NI; ++i) fp::load_to_lds(kplane + slot * G::ROWB, (i * G::RPI + lrow) * G::ROWB + k_off(lpos, i * G::RPI + lrow), stage + i * 1024);
+          for (int i = 0; i < G::NI; ++i) fp::load_to_lds(k, (k_at ^ (G::k_swz(i * G::RPI) * 16)) + i * 1024, stage, i * 1024);
 #pragma unroll
-          for (int i = 0; i < G::NI; ++i)
-            fp::load_to_lds(vplane + slot * G::ROWB, (i * G::RPI + lrow) * G::ROWB + v_off(lpos, i * G::RPI + lrow), stage + G::HALF + i * 1024);
+          for (int i = 0; i < G::NI; ++i) fp::load_to_lds(v, (v_at ^ (G::v_swz(i * G::RPI) * 32)) + i * 1024, stage, G::HALF + i * 1024);
         } else {
 #pragma unroll
-          for (int i = 0; i < G::NI; ++i) fp::load_to_lds_nt(kplane + slot * G::ROWB, (i * G::RPI + lrow) * G::ROWB + k_off(lpos, i * G::RPI + lrow), stage + i * 1024);
+          for (int i = 0; i < G::NI; ++i) load_once(k, (k_at ^ (G::k_swz(i * G::RPI) * 16)) + i * 1024, stage, i * 1024);
 #pragma unroll
-          for (int i = 0; i < G::NI; ++i)
-            fp::load_to_lds_nt(vplane + slot * G::ROWB, (i * G::RPI + lrow) * G::ROWB + v_off(lpos, i * G::RPI + lrow), stage + G::HALF + i * 1024);
+          for (int i = 0; i < G::NI; ++i) load_once(v, (v_at ^ (G::v_swz(i * G::RPI) * 32)) + i * 1024, stage, G::HALF + i * 1024);
         }
       } else {  // pages that do not hold whole stages, the last keys: row by row.  A row past the range repeats its last one and is masked
 #pragma nounroll
         for (int i = 0; i < G::NI; ++i) {  // one at a time: their addresses would be registers of the whole loop
-          const int r = i * G::RPI + lrow;
-          const int t = min(c0 + r, seg1 - 1);
+          const int t = min(c0 + i * G::RPI + lrow, seg1 - 1);
           int64_t blk;
           int off;
           a.pd.split(t, blk, off);
-          const int64_t at = (static_cast<int64_t>(sh.pages[blk - blk0]) * a.pd.page_size + off) * G::ROWB;
-          fp::load_to_lds(kplane + at + k_off(lpos, r), stage + i * 1024);
-          fp::load_to_lds(vplane + at + v_off(lpos, r), stage + G::HALF + i * 1024);
+          const int64_t row = (static_cast<int64_t>(sh.pages[blk - blk0]) * a.pd.page_size + off) * G::ROWB;
+          fp::load_to_lds(kplane + row + ((lpos ^ G::k_swz(i * G::RPI + lrow)) * 16), stage + i * 1024, 0u);
+          fp::load_to_lds(vplane + row + ((lpos ^ G::v_swz(i * G::RPI + lrow) * 2) * 16), stage + G::HALF + i * 1024, 0u);
         }
       }
     };
 
     // stages wave, wave + 4, ... of the segment
     const int n_stages = (seg1 - seg0 + G::TS - 1) / G::TS;
-    if (wave < n_stages) issue(seg0 + wave * G::TS, ring);
-    if (wave + kWaves < n_stages) issue(seg0 + (wave + kWaves) * G::TS, ring + 2 * G::HALF);
+    if (wave < n_stages) issue(locate(seg0 + wave * G::TS), seg0 + wave * G::TS, lds_ring);
+    if (wave + kWaves < n_stages) issue(locate(seg0 + (wave + kWaves) * G::TS), seg0 + (wave + kWaves) * G::TS, lds_ring + 2 * G::HALF);
 #pragma nounroll
     for (int s = wave, buf = 0; s < n_stages; s += kWaves, buf ^= 1) {
       const int c0 = seg0 + s * G::TS;
       char* const k_lds = ring + buf * 2 * G::HALF;
       char* const v_lds = k_lds + G::HALF;
+      const int64_t next = s + 2 * kWaves < n_stages ? locate(c0 + 2 * kWaves * G::TS) : -1;
       if (s + kWaves < n_stages) wait_staged<2 * G::NI>(); else wait_staged<0>();
       // scores of this lane's columns: keys 16 * blk + 4 * grp + 0 .. 3
       f32x4 sc[CB][G::NB];
-      const int lane_now = anew(lane);
+      const int lane_now = lane_id();
 #pragma unroll
       for (int blk = 0; blk < G::NB; ++blk) {
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) sc[cb][blk] = f32x4{0.f, 0.f, 0.f, 0.f};
         const int r = blk * 16 + (lane_now & 15);
         const uint32_t at = r * G::ROWB + ((lane_now >> 4) ^ G::k_swz(r)) * 16;
+        constexpr int kAhead = CB == 4 ? 2 : 4;  // operands on their way ahead of the products that use them
+        v4u ahead[G::QV];
+#pragma unroll
+        for (int kk = 0; kk < kAhead && kk < G::QV; ++kk) ahead[kk] = *reinterpret_cast<const v4u*>(k_lds + (at ^ (kk * 64)));
 #pragma unroll
         for (int kk = 0; kk < G::QV; ++kk) {
-          const v4u ka = *reinterpret_cast<const v4u*>(k_lds + (at ^ (kk * 64)));
+          if (kk + kAhead < G::QV) ahead[kk + kAhead] = *reinterpret_cast<const v4u*>(k_lds + (at ^ ((kk + kAhead) * 64)));
+          __builtin_amdgcn_sched_barrier(0);
+          const v4u ka = ahead[kk];
 #pragma unroll
           for (int cb = 0; cb < CB; ++cb) {
             if constexpr (G::k16) {
@@ -834,20 +850,20 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
       if (c0 + G::TS > min(seg1, least)) {
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) {
-          const int end = min(sh.limit[wave][cb * 16 + col], seg1);
+          const int end = min(sh.limit[wave][cb * 16 + (lane_now & 15)], seg1);
 #pragma unroll
           for (int blk = 0; blk < G::NB; ++blk)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-              if (c0 + blk * 16 + grp * 4 + j >= end) sc[cb][blk][j] = -INFINITY;
+              if (c0 + blk * 16 + (lane_now >> 4) * 4 + j >= end) sc[cb][blk][j] = -INFINITY;
         }
         // V rows past the range become 0: a probability of 0 against an infinity would be NaN.  So do the elements that are not
         // finite of rows which only some columns see; these columns get them at the end.
 #pragma nounroll
         for (int i = 0; i < G::NI; ++i) {
-          const int t = c0 + i * G::RPI + anew(lane) / G::CPR;
+          const int t = c0 + i * G::RPI + lane_now / G::CPR;
           if (t < least) continue;
-          v4u* const at = reinterpret_cast<v4u*>(v_lds + i * 1024 + lane * 16);
+          v4u* const at = reinterpret_cast<v4u*>(v_lds + i * 1024 + lane_now * 16);
           v4u w = {0, 0, 0, 0};
           if (t < seg1) {
             w = *at;
@@ -865,6 +881,22 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
         }
         asm volatile("" : : : "memory");  // a wavefront's LDS instructions are executed in order
       }
+      // The first V operands leave LDS while the exponentials are worked out.
+      constexpr int kReadsV = G::k16 ? G::NB * G::DB : G::NB * 4 * (D / 64);  // reads of a stage
+      constexpr int kAheadV = CB == 4 ? 4 : 8 < kReadsV ? 8 : kReadsV;
+      const auto read_v = [&](int n) {
+        if constexpr (G::k16) {
+          // lanes 4 j + c of a 16-lane block name elements 4 c .. of key 4 * grp + j and receive element `col` of the four keys
+          const int r = n / G::DB * 16 + (lane_now >> 4) * 4 + ((lane_now & 15) >> 2);
+          return lds_read_tr(v_lds + ((r * G::ROWB + G::v_swz(r) * 32 + (lane_now & 3) * 8) ^ (n % G::DB * 32)));
+        } else {
+          const int r = n / (D / 64) / 4 * 16 + (lane_now >> 4) * 4 + n / (D / 64) % 4;
+          return *reinterpret_cast<const f32x4*>(v_lds + r * G::ROWB + n % (D / 64) * 256 + (lane_now & 15) * 16);
+        }
+      };
+      decltype(read_v(0)) v_ahead[kAheadV];
+#pragma unroll
+      for (int n = 0; n < kAheadV; ++n) v_ahead[n] = read_v(n);
       // Reference point of the exponentials, per column: moves only when the column's maximum has outgrown it by kMaxSlack, so most
       // stages need no exchange between the lanes of a column and no rescale.
       float cand[CB];
@@ -916,47 +948,44 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
               w[j] = E::pack2(E::above_zero(p0), E::above_zero(p1));
               if constexpr (kSplit) {
                 const uint32_t rest = E::pack2(p0 - E::to_float(w[j] & 0xffffu), p1 - E::to_float(w[j] >> 16));
-                if (col >= 8) w[j] = rest;
+                if ((lane_now & 15) >= 8) w[j] = rest;
               }
             }
             pb[cb] = __builtin_bit_cast(s16x4, uint2{w[0], w[1]});
           }
-          // lanes 4 j + c of a 16-lane block name elements 4 c .. of key 4 * grp + j and receive element `col` of the four keys
-          const int r = blk * 16 + (lane_now >> 4) * 4 + ((lane_now & 15) >> 2);
-          const uint32_t at = r * G::ROWB + G::v_swz(r) * 32 + (lane_now & 3) * 8;
 #pragma unroll
           for (int db = 0; db < G::DB; ++db) {
-            const s16x4 va = lds_read_tr(v_lds + (at ^ (db * 32)));
+            const s16x4 va = v_ahead[(blk * G::DB + db) % kAheadV];
 #pragma unroll
             for (int cb = 0; cb < CB; ++cb) o[cb][db] = E::mfma_k16(va, pb[cb], o[cb][db]);
+            if (blk * G::DB + db + kAheadV < G::NB * G::DB) v_ahead[(blk * G::DB + db) % kAheadV] = read_v(blk * G::DB + db + kAheadV);
+            __builtin_amdgcn_sched_barrier(0);
           }
         }
       } else {
         // element e of four neighbours of a V row is the operand of block e of O^T: row i of block 4 h + e is d = 64 h + 4 i + e
 #pragma unroll
-        for (int blk = 0; blk < G::NB; ++blk)
+        for (int n = 0; n < kReadsV; ++n) {
+          const int h = n % (D / 64), j = n / (D / 64) % 4, blk = n / (D / 64) / 4;
+          const f32x4 va = v_ahead[n % kAheadV];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int r = blk * 16 + (lane_now >> 4) * 4 + j;
+          for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
-            for (int h = 0; h < D / 64; ++h) {
-              const f32x4 va = *reinterpret_cast<const f32x4*>(v_lds + r * G::ROWB + h * 256 + (lane_now & 15) * 16);
-#pragma unroll
-              for (int cb = 0; cb < CB; ++cb)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  o[cb][4 * h + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(va[e], sc[cb][blk][j], o[cb][4 * h + e], 0, 0, 0);
-            }
-          }
+            for (int e = 0; e < 4; ++e)
+              o[cb][4 * h + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(va[e], sc[cb][blk][j], o[cb][4 * h + e], 0, 0, 0);
+          if (n + kAheadV < kReadsV) v_ahead[n % kAheadV] = read_v(n + kAheadV);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
       if (s + 2 * kWaves < n_stages) {
         asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // every operand of this stage has left LDS
-        issue(c0 + 2 * kWaves * G::TS, ring + buf * 2 * G::HALF);
+        issue(next, c0 + 2 * kWaves * G::TS, lds_ring + buf * 2 * G::HALF);
       }
     }
     seg0 = seg1;
   }
 
+  const int lane = lane_id(), tid = wave * 64 + lane, col = lane & 15, grp = lane >> 4;
   // The wavefronts' states meet in LDS: maxima and sums first, then the accumulators, scaled to the common maximum, PASS column blocks
   // at a time, chunks permuted against bank conflicts.
 #pragma unroll
@@ -1070,6 +1099,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(Shared<E, D>) <= 80 * 1024 ? 2 : 
   const Header h = load_record<Header>(a.plan);
   const Share share = load_record<Share>(a.plan + a.shares + w * static_cast<int64_t>(sizeof(Share)));
   if (!plan_fits(a, h) || w >= h.n_wg) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int left = share.units, offset = share.offset, piece = share.piece;
   bool busy = false;
   Tile t = share.first;
@@ -1083,13 +1113,13 @@ __global__ __launch_bounds__(kThreads, (sizeof(Shared<E, D>) <= 80 * 1024 ? 2 : 
     if (busy) __syncthreads();  // the piece before has left LDS
     busy = true;
     if (Geo<E, D>::k16 && t.n_rows <= 8)
-      run_piece<E, D, 1, Geo<E, D>::k16>(a, sh, t, piece, t0, t1);
+      run_piece<E, D, 1, Geo<E, D>::k16>(a, sh, wave, t, piece, t0, t1);
     else if (t.n_rows <= 16)
-      run_piece<E, D, 1, false>(a, sh, t, piece, t0, t1);
+      run_piece<E, D, 1, false>(a, sh, wave, t, piece, t0, t1);
     else if (t.n_rows <= 32)
-      run_piece<E, D, 2, false>(a, sh, t, piece, t0, t1);
+      run_piece<E, D, 2, false>(a, sh, wave, t, piece, t0, t1);
     else
-      run_piece<E, D, 4, false>(a, sh, t, piece, t0, t1);
+      run_piece<E, D, 4, false>(a, sh, wave, t, piece, t0, t1);
     }
     if (left <= 0 || ++i >= h.n_tiles) break;
     piece = 0;
