@@ -669,6 +669,10 @@ __device__ __forceinline__ void add_infinities(const SharedArgs& a, const Tile& 
   }
 }
 
+// A barrier of the workgroup behind this wavefront's LDS instructions.  (__syncthreads also waits for stores to global memory, 1 to 2 us
+// for partial results that nobody here reads.)
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory"); }
+
 // One piece: the rows of a tile over its keys [t0, t1).  CB blocks of 16 columns; kSplit: at most 8 rows, in columns 0 .. 7 and again in
 // 8 .. 15, whose probabilities carry what the rounding of the first left over.
 template <typename E, int D, int CB, bool kSplit>
@@ -683,8 +687,20 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
   const char* const vplane = a.pool_v + static_cast<int64_t>(hc) * a.n_slots * G::ROWB;
   const int64_t* const table = a.page_table + static_cast<int64_t>(tile.slot) * a.pt_row_stride;
 
+  // the page ids of the first segment are on their way before the rows are asked for
+  int64_t early = 0;
+  {
+    int64_t first, last;
+    int unused;
+    a.pd.split(t0, first, unused);
+    a.pd.split(t1 - 1, last, unused);
+    const int64_t blk = first + wave * 64 + lane_id();
+    if (blk <= last && blk < a.n_pages) early = table[blk];
+  }
+
   // rows: query operands and limits of this lane's columns.  A column without a row repeats row 0, sees everything and is not stored.
   v4u q[CB][G::QV];
+  int64_t pos[CB];
   int least = INT32_MAX;
   {
     // two trips to memory: the tokens, then what they name
@@ -698,7 +714,6 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
       x[cb] = tile.row0 + (r < tile.n_rows ? r : 0);
       token[cb] = tokens[x[cb] >> a.group_shift];
     }
-    int64_t pos[CB];
     const auto at = [&](int cb) { return static_cast<int64_t>(token[cb] >> kTokenShift) * a.S + (token[cb] & ((1 << kTokenShift) - 1)); };
     if (a.pos_i64) {
 #pragma unroll
@@ -715,16 +730,7 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
       for (int kk = 0; kk < G::QV; ++kk) q[cb][kk] = *reinterpret_cast<const v4u*>(src + kk * 64);
     }
     __builtin_amdgcn_sched_barrier(0);  // all of them are on their way before the first is waited for
-#pragma unroll
-    for (int cb = 0; cb < CB; ++cb) {
-      const int r = kSplit ? col & 7 : cb * 16 + col;
-      const int64_t keys = pos[cb] < 0 ? 0 : pos[cb] >= a.max_context ? a.max_context : pos[cb] + 1;
-      const int lim = r < tile.n_rows ? static_cast<int>(keys) : INT32_MAX;
-      least = min(least, lim);
-      if (grp == 0) sh.limit[wave][cb * 16 + col] = lim;
-    }
   }
-  least = -fp::wave_max(-least);
   if (wave == 0 && lane_id() == 0) sh.tainted = 0;  // ahead of the barriers of the first segment
 
   f32x4 o[CB][G::DB];
@@ -749,20 +755,17 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
       int64_t last;
       int unused;
       a.pd.split(seg1 - 1, last, unused);
-      __syncthreads();  // the page ids before are no longer read
+      lds_barrier();  // the page ids before are no longer read
       for (int i = wave * 64 + lane_id(); i <= static_cast<int>(last - blk0); i += kThreads) {
         int64_t page = 0;
-        if (blk0 + i < a.n_pages) page = table[blk0 + i];
+        if (seg0 == t0 && i < kThreads)
+          page = early;
+        else if (blk0 + i < a.n_pages)
+          page = table[blk0 + i];
         if (page < 0 || page >= a.pool_pages) page = 0;  // as paged_decode: the reserved page
         sh.pages[i] = static_cast<int>(page);
       }
-      __syncthreads();
-      // The query rows are waited for here.  At their first use, inside the loop over the stages, the wait would be one of every
-      // stage, and for the stages on their way, too, of which the compiler does not know.
-#pragma unroll
-      for (int cb = 0; cb < CB; ++cb)
-#pragma unroll
-        for (int kk = 0; kk < G::QV; ++kk) asm volatile("" : "+v"(q[cb][kk]));
+      lds_barrier();
     }
 
     // pool row of the first key of a stage that lies in one page and in the segment, -1: not such a stage
@@ -808,6 +811,24 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
     const int n_stages = (seg1 - seg0 + G::TS - 1) / G::TS;
     if (wave < n_stages) issue(locate(seg0 + wave * G::TS), seg0 + wave * G::TS, lds_ring);
     if (wave + kWaves < n_stages) issue(locate(seg0 + (wave + kWaves) * G::TS), seg0 + (wave + kWaves) * G::TS, lds_ring + 2 * G::HALF);
+    if (seg0 == t0) {  // the rows' limits, now that the first stages are on their way
+      const int lane = lane_id(), col = lane & 15, max_context = a.max_context;
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb) {
+        const int r = kSplit ? col & 7 : cb * 16 + col;
+        const int64_t keys = pos[cb] < 0 ? 0 : pos[cb] >= max_context ? max_context : pos[cb] + 1;
+        const int lim = r < tile.n_rows ? static_cast<int>(keys) : INT32_MAX;
+        least = min(least, lim);
+        if (lane < 16) sh.limit[wave][cb * 16 + col] = lim;
+      }
+      least = -fp::wave_max(-least);
+    }
+    // The query rows are waited for here.  At their first use, inside the loop over the stages, the wait would be one of every stage, and
+    // for the stages on their way, too, of which the compiler does not know.
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+      for (int kk = 0; kk < G::QV; ++kk) asm volatile("" : "+v"(q[cb][kk]));
 #pragma nounroll
     for (int s = wave, buf = 0; s < n_stages; s += kWaves, buf ^= 1) {
       const int c0 = seg0 + s * G::TS;
@@ -1005,7 +1026,7 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
     l[cb] += __shfl_xor(l[cb], 32);
     if (grp == 0) *reinterpret_cast<float2*>(sh.ml[wave][cb * 16 + col]) = float2{m[cb], l[cb]};
   }
-  __syncthreads();
+  lds_barrier();
 #pragma unroll
   for (int cb = 0; cb < CB; ++cb) {
     float2 ml[kWaves];
@@ -1028,7 +1049,7 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
   constexpr int C4 = D / 4;  // 16-byte chunks of a row of O
 #pragma unroll
   for (int cb0 = 0; cb0 < CB; cb0 += G::PASS) {
-    if (cb0 > 0) __syncthreads();  // the pass before has been read
+    if (cb0 > 0) lds_barrier();  // the pass before has been read
 #pragma unroll
     for (int i = 0; i < G::PASS && cb0 + i < CB; ++i) {
       const int cb = cb0 + i;
@@ -1044,7 +1065,7 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
         }
       }
     }
-    __syncthreads();
+    lds_barrier();
     constexpr int kRows = G::PASS < CB ? G::PASS * 16 : CB * 16;
     for (int i = tid; i < kRows * C4; i += kThreads) {
       const int row = i / C4, c = i % C4, r = cb0 * 16 + row;
@@ -1110,7 +1131,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(Shared<E, D>) <= 80 * 1024 ? 2 : 
     left -= t.lead + all - offset;
     offset = 0;
     if (to > from) {
-    if (busy) __syncthreads();  // the piece before has left LDS
+    if (busy) lds_barrier();  // the piece before has left LDS
     busy = true;
     if (Geo<E, D>::k16 && t.n_rows <= 8)
       run_piece<E, D, 1, Geo<E, D>::k16>(a, sh, wave, t, piece, t0, t1);
