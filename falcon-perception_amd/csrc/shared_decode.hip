@@ -1027,22 +1027,26 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
     if (grp == 0) *reinterpret_cast<float2*>(sh.ml[wave][cb * 16 + col]) = float2{m[cb], l[cb]};
   }
   lds_barrier();
+  {
+    float2 ml[CB][kWaves];
 #pragma unroll
-  for (int cb = 0; cb < CB; ++cb) {
-    float2 ml[kWaves];
-    float mn = -INFINITY, den = 0.f;
+    for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      ml[w] = *reinterpret_cast<const float2*>(sh.ml[w][cb * 16 + col]);
-      mn = fmaxf(mn, ml[w].x);
+      for (int w = 0; w < kWaves; ++w) ml[cb][w] = *reinterpret_cast<const float2*>(sh.ml[w][cb * 16 + col]);
+    __builtin_amdgcn_sched_barrier(0);  // all reads on their way
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) {
+      float mn = -INFINITY, den = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) mn = fmaxf(mn, ml[cb][w].x);
+      const float ms = safe_max(mn);
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) den += ml[cb][w].y * fast_exp2(ml[cb][w].x - ms);
+      if (wave == 0 && grp == 0) *reinterpret_cast<float2*>(sh.joined[cb * 16 + col]) = float2{mn, den};
+      const float scale = fast_exp2(m[cb] - ms);
+#pragma unroll
+      for (int db = 0; db < G::DB; ++db) o[cb][db] *= scale;
     }
-    const float ms = safe_max(mn);
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) den += ml[w].y * fast_exp2(ml[w].x - ms);
-    if (wave == 0 && grp == 0) *reinterpret_cast<float2*>(sh.joined[cb * 16 + col]) = float2{mn, den};
-    const float scale = fast_exp2(m[cb] - ms);
-#pragma unroll
-    for (int db = 0; db < G::DB; ++db) o[cb][db] *= scale;
   }
   const SharedArgs& e = reread();
   const bool sole = !prefix && tile.n_pieces == 1 && tile.t_begin == 0;  // nothing to join: the result itself
@@ -1066,31 +1070,55 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
       }
     }
     lds_barrier();
-    constexpr int kRows = G::PASS < CB ? G::PASS * 16 : CB * 16;
-    for (int i = tid; i < kRows * C4; i += kThreads) {
-      const int row = i / C4, c = i % C4, r = cb0 * 16 + row;
-      if (r >= tile.n_rows) break;
-      const float2 ml = *reinterpret_cast<const float2*>(sh.joined[r]);
-      const float mn = ml.x, den = ml.y;
-      f32x4 num = {0.f, 0.f, 0.f, 0.f};
+    // a thread has one chunk of every kStep-th row
+    constexpr int kRows = G::PASS < CB ? G::PASS * 16 : CB * 16, kStep = kThreads / C4, kTurns = kRows / kStep;
+    const int c = tid % C4, row0 = tid / C4, r0 = cb0 * 16 + row0;
+    f32x4 num[kTurns];
+    float2 ml[kTurns];
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) num += reinterpret_cast<const f32x4*>(sh.ring[w])[row * C4 + (c ^ (row & 15))];
-      if (sh.tainted) add_infinities<E, D>(e, tile, r, max(t0, least), t1, e.pool_v + static_cast<int64_t>(hc) * e.n_slots * G::ROWB, c, num);
-      if (sole) {
+    for (int k = 0; k < kTurns; ++k) {
+      const int row = row0 + k * kStep;
+      ml[k] = *reinterpret_cast<const float2*>(sh.joined[cb0 * 16 + row]);
+      num[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) num[k] += reinterpret_cast<const f32x4*>(sh.ring[w])[row * C4 + (c ^ (row & 15))];
+    }
+    if (sh.tainted) {
+#pragma nounroll
+      for (int k = 0; k < kTurns; ++k)
+        if (r0 + k * kStep < tile.n_rows) {
+          f32x4 more = {0.f, 0.f, 0.f, 0.f};
+          add_infinities<E, D>(e, tile, r0 + k * kStep, max(t0, least), t1, e.pool_v + static_cast<int64_t>(hc) * e.n_slots * G::ROWB, c, more);
+#pragma unroll
+          for (int n = 0; n < kTurns; ++n)
+            if (n == k) num[n] += more;
+        }
+    }
+    if (sole) {
+#pragma unroll
+      for (int k = 0; k < kTurns; ++k) {
+        if (r0 + k * kStep >= tile.n_rows) break;
         int b, j, g;
-        find_row(e, tile, r, &b, &j, &g);
+        find_row(e, tile, r0 + k * kStep, &b, &j, &g);
         const int h = hc * e.group + g;
         const bool any = keys_of(e, b, j) > 0;
-        const float lse = (mn + log2f(den)) * kLn2;
+        const float lse = (ml[k].x + log2f(ml[k].y)) * kLn2;
         f32x4 res;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) res[k] = any ? fp_decode::sink_gate<E>(num[k] / den, lse, e.sinks, h) : 0.f;
+        for (int n = 0; n < 4; ++n) res[n] = any ? fp_decode::sink_gate<E>(num[k][n] / ml[k].y, lse, e.sinks, h) : 0.f;
         store4<E>(e.out + b * e.os_b + h * e.os_h + j * e.os_s + c * 4 * E::kBytes, res);
         if (c == 0) e.lse[(static_cast<int64_t>(b) * e.Hq + h) * e.S + j] = any ? lse : -INFINITY;
-      } else {
-        const int64_t p = (static_cast<int64_t>(tile.part) + static_cast<int64_t>(piece) * tile.n_rows + r) * e.Hc + hc;
-        *reinterpret_cast<f32x4*>(e.ws_acc + p * D + c * 4) = num;
-        if (c == 0) *reinterpret_cast<float2*>(e.ws_ml + p * 2) = float2{mn, den};
+      }
+    } else {
+      const int64_t first = (static_cast<int64_t>(tile.part) + static_cast<int64_t>(piece) * tile.n_rows + r0) * e.Hc + hc;
+      float* const acc = e.ws_acc + first * D + c * 4;
+      float* const mls = e.ws_ml + first * 2;
+      const int64_t step = static_cast<int64_t>(kStep) * e.Hc;
+#pragma unroll
+      for (int k = 0; k < kTurns; ++k) {
+        if (r0 + k * kStep >= tile.n_rows) break;
+        *reinterpret_cast<f32x4*>(acc + k * step * D) = num[k];
+        if (c == 0) *reinterpret_cast<float2*>(mls + k * step * 2) = ml[k];
       }
     }
   }
