@@ -36,8 +36,7 @@ constexpr int kMaxRows = 1 << 20;      // B * S * heads of a group
 constexpr int kMaxContext = 1 << 21;   // with the rows: units of all tiles fit 31 bits
 constexpr int kTileRows = 64;
 constexpr int kUnit = 64;              // keys: what the cut is made of
-constexpr int kMinUnits = 4;           // a workgroup's share at least
-constexpr int kMinShared = 64;         // keys of a prefix that are worth a tile of their own
+constexpr int kMinUnits = 3;           // a workgroup's share at least
 constexpr int kSegPages = 1024;        // page ids held in LDS
 constexpr float kMaxSlack = 6.f;       // the reference point of the exponentials may lag the maximum by this much (log2)
 constexpr int kMagic = 0x5ade0001;
@@ -72,7 +71,8 @@ struct Tile {
   int part;            // workspace row of the first piece's first row; piece after piece
   int shared;          // of a group
   int lead;            // units that stand for what it costs before its first key and behind its last
-  int pad[2];
+  int again;           // other tiles read the same keys
+  int pad;
 };
 struct Share {
   int tile, offset, units;  // first tile, units of it (lead included) that belong to workgroups before, units to do
@@ -121,7 +121,7 @@ struct PlanArgs {
 };
 
 // What a tile costs before its first key and behind its last, in units.
-__device__ __forceinline__ int lead_of(int rows) { return rows <= 32 ? 3 : 5; }
+__device__ __forceinline__ int lead_of(int rows) { return rows <= 16 ? 2 : rows <= 32 ? 3 : 5; }
 
 __device__ __forceinline__ int units_of(int keys) { return (keys + kUnit - 1) / kUnit; }
 
@@ -247,8 +247,10 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   }
   __syncthreads();
   for (int b = tid; b < a.B; b += n_thr) {
-    const int lead = s_lead[b], shared = s_members[lead] >= 2 ? min(s_shortest[lead], s_longest[lead]) : 0;
-    const bool shares = s_tok[b] > 0 && s_id[b] > 0 && shared >= kMinShared;
+    // Whole units: what is behind them counts as each one's own, up to 63 keys that are read once a sequence.  Own keys then begin
+    // with a stage that lies in one page; from anywhere else they would be staged row by row (64 sequences on 9 pictures: %s us a layer).
+    const int lead = s_lead[b], shared = s_members[lead] >= 2 ? min(s_shortest[lead], s_longest[lead]) / kUnit * kUnit : 0;
+    const bool shares = s_tok[b] > 0 && s_id[b] > 0 && shared > 0;
     s_shared[b] = shares ? shared : 0;
     if (!shares) s_rank[b] = 0;
     if (!shares || lead != b) s_count[b] = 0;
@@ -396,6 +398,7 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
       t.t_begin = 0;
       t.t_end = s_shared[b];
       t.shared = 1;
+      t.again = tiles_of(s_count[b]) > 1;
       rows_before = s_base[b] * a.group + t.row0 + (cut > 0 ? 0 : rest_part);
     } else {
       const int b = last_at_or_below(s_stile, a.B, i - p_tiles), k = i - p_tiles - s_stile[b];
@@ -409,6 +412,7 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
       t.t_begin = s_shared[b];
       t.t_end = s_keys[b];
       t.shared = 0;
+      t.again = tiles_of(s_tok[b]) > 1;
       rows_before = rest_part + (shared_tokens + s_len[b]) * a.group + t.row0;
     }
     if (cut > 0) {
@@ -419,7 +423,7 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
       t.part = first;
     }
     t.part = rows_before + kTileRows * t.part;
-    t.pad[0] = t.pad[1] = 0;
+    t.pad = 0;
     return t;
   };
   for (int i = tid; i < n_wg + n_tiles; i += n_thr) {
@@ -743,7 +747,7 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
     for (int db = 0; db < G::DB; ++db) o[cb][db] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  const bool aligned_pages = a.pd.shift >= 0 && a.pd.page_size % G::TS == 0;
+  const bool aligned_pages = a.pd.page_size % G::TS == 0;
 
   for (int seg0 = t0; seg0 < t1;) {
     int64_t blk0;
@@ -771,8 +775,9 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
     // pool row of the first key of a stage that lies in one page and in the segment, -1: not such a stage
     const auto locate = [&](int c0) {
       if (!aligned_pages || c0 % G::TS != 0 || c0 + G::TS > seg1) return static_cast<int64_t>(-1);
-      const int page = __builtin_amdgcn_readfirstlane(sh.pages[(c0 >> a.pd.shift) - static_cast<int>(blk0)]);
-      return static_cast<int64_t>(page) * a.pd.page_size + (c0 & (a.pd.page_size - 1));
+      const int blk = a.pd.shift >= 0 ? c0 >> a.pd.shift : c0 / a.pd.page_size;
+      const int page = __builtin_amdgcn_readfirstlane(sh.pages[blk - static_cast<int>(blk0)]);
+      return static_cast<int64_t>(page) * a.pd.page_size + (c0 - blk * a.pd.page_size);
     };
     const auto issue = [&](int64_t slot, int c0, uint32_t stage) {
       // Instruction i brings rows i * RPI + lrow, position lpos of each.  The permutations of a row are those of i * RPI and of lrow
@@ -782,7 +787,7 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
       if (slot >= 0) {
         const char* const k = kplane + slot * G::ROWB;
         const char* const v = vplane + slot * G::ROWB;
-        if (prefix) {  // other tiles read these rows, too
+        if (tile.again) {  // other tiles read these rows, too
 #pragma unroll
           for (int i = 0; i < G::NI; ++i) fp::load_to_lds(k, (k_at ^ (G::k_swz(i * G::RPI) * 16)) + i * 1024, stage, i * 1024);
 #pragma unroll
