@@ -31,7 +31,7 @@ using fp_decode::safe_max;
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int kMaxSequences = 2048;
+constexpr int kMaxSequences = 1536;
 constexpr int kMaxRows = 1 << 20;      // B * S * heads of a group
 constexpr int kMaxContext = 1 << 21;   // with the rows: units of all tiles fit 31 bits
 constexpr int kTileRows = 64;
@@ -72,7 +72,7 @@ struct Tile {
   int shared;          // of a group
   int lead;            // units that stand for what it costs before its first key and behind its last
   int again;           // other tiles read the same keys
-  int pad;
+  int next;            // the tile behind it on the axis that it is cut on
 };
 struct Share {
   int tile, offset, units;  // first tile, units of it (lead included) that belong to workgroups before, units to do
@@ -101,7 +101,7 @@ Layout layout_of(int B, int S, int Hq, int Hc) {
   l.shares = l.place + list;
   l.tiles = l.shares + static_cast<int64_t>(l.n_wg) * sizeof(Share);
   l.bytes = l.tiles + static_cast<int64_t>(l.max_tiles) * sizeof(Tile);
-  l.part_rows = 3ll * B * l.rows + static_cast<int64_t>(kTileRows) * l.n_wg;
+  l.part_rows = 4ll * B * l.rows + static_cast<int64_t>(kTileRows) * l.n_wg;
   return l;
 }
 
@@ -161,7 +161,7 @@ __device__ __forceinline__ void block_sums(const int (&x)[N], int (&before)[N], 
   __syncthreads();
 }
 
-constexpr int kPlanArrays = 15;
+constexpr int kPlanArrays = 20;
 
 __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   extern __shared__ int s_mem[];
@@ -180,7 +180,12 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   int* const s_stile = s_base + Bp;    //   tiles of own keys,
   int* const s_unit = s_stile + Bp;    //   units of prefixes that are cut with everything else,
   int* const s_own = s_unit + Bp;      //   units of own keys,
-  int* const s_wg = s_own + Bp;        //   workgroups of prefixes that are cut by themselves
+  int* const s_wide = s_own + Bp;      // place of a group of several tiles in the lists of these:
+  int* const s_at = s_wide + Bp;       //   its first sequence,
+  int* const s_pos = s_at + Bp;        //   its place on the axis of its kind,
+  int* const s_end = s_pos + Bp;       //   length of that axis, at the first of a kind, elsewhere 0,
+  int* const s_next = s_end + Bp;      //   the next of its kind, -1: none,
+  int* const s_part = s_next + Bp;     //   pieces of the groups before
   __shared__ int s_sum[16 * 7], s_pick[1];
   const int tid = threadIdx.x, n_thr = blockDim.x, lane = tid & 63, wave = tid >> 6, n_waves = n_thr / 64;
   Sequence* const seqs = reinterpret_cast<Sequence*>(a.plan + a.seqs);
@@ -287,62 +292,83 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
     s_base[b] = s_shared[b] > 0 ? x[1] : shared_tokens + x[3];  // of a group: right at its leader
     s_stile[b] = x[2];
     s_len[b] = x[6];  // tokens of the sequences before; the prefix lengths are no longer needed
-    if (s_count[b] > 0 && tiles_of(s_count[b]) > 1) s_wg[x[5]] = b;  // a list for the moment
+    if (s_count[b] > 0 && tiles_of(s_count[b]) > 1) {
+      s_wide[b] = x[5];
+      s_at[x[5]] = b;
+    }
     add(b);
   }
   if (tid == 0) s_pick[0] = -1;
   __syncthreads();
 
-  // The cut: `len` units a workgroup.  A prefix of several tiles is cut by itself, all its tiles at the same keys, and the pieces of one
-  // range of keys go to consecutive workgroups, which run at the same time and find what the first of them loads in their XCD's L2.
-  // (Laid end to end its tiles read all keys once each from beyond L2.)  That takes some more workgroups, so `len` is the
-  // shortest of 64 lengths, a lane each, for which there are enough.
+  // The cut: `len` units a workgroup.  Prefixes of several tiles are cut apart from everything else: those with the same number of tiles
+  // lie on one axis, every cut of it is a workgroup for each of the tiles, and these run at the same time and find what the first of
+  // them loads in their XCD's L2.  (With its tiles one behind the other all of them read the keys from beyond L2.)  That takes a few
+  // more workgroups, so `len` is the shortest of 64 lengths, a lane each, for which there are enough.
+  const auto tiles_at = [&](int m) { return tiles_of(s_count[s_at[m]]); };
+  const auto units_at = [&](int m) { return lead_for(s_count[s_at[m]]) + units_of(s_shared[s_at[m]]); };
+  for (int m = tid; m < n_multi; m += n_thr) {
+    const int n = tiles_at(m);
+    int pos = 0, all = 0, next = -1, first = 1;
+    for (int i = 0; i < n_multi; ++i) {
+      if (tiles_at(i) != n) continue;
+      const int u = units_at(i);
+      all += u;
+      if (i < m) {
+        pos += u;
+        first = 0;
+      } else if (i > m && next < 0) {
+        next = i;
+      }
+    }
+    s_pos[m] = pos;
+    s_end[m] = first ? all : 0;
+    s_next[m] = next;
+  }
+  __syncthreads();
   const int shortest_len = max(kMinUnits, (all_units + a.n_wg - 1) / a.n_wg);
-  const auto pieces_at = [&](int b, int len) {  // 0: cut with everything else
-    const int n = units_of(s_shared[b]);
-    const int lead = lead_for(s_count[b]), room = max(1, len - lead);
-    return tiles_of(s_count[b]) > 1 && 2 * (lead + n) >= len ? (n + room - 1) / room : 0;
-  };
+  const auto cuts = [](int units, int len) { return (units + len - 1) / len; };
   if (wave == 0 && n_multi > 0) {
     const int len = shortest_len + (shortest_len * lane + 31) / 32;
     int need = 0, rest = all_units;
-    for (int i = 0; i < n_multi; ++i) {
-      const int b = s_wg[i], n = pieces_at(b, len);
-      need += n * tiles_of(s_count[b]);
-      if (n > 0) rest -= tiles_of(s_count[b]) * (lead_for(s_count[b]) + units_of(s_shared[b]));
+    for (int m = 0; m < n_multi; ++m) {
+      need += tiles_at(m) * cuts(s_end[m], len);
+      rest -= tiles_at(m) * units_at(m);
     }
-    const unsigned long long enough = __ballot(need + (rest + len - 1) / len <= a.n_wg);
+    const unsigned long long enough = __ballot(need + cuts(rest, len) <= a.n_wg);
     if (enough != 0 && lane == 0) s_pick[0] = __builtin_ctzll(enough);
   }
   __syncthreads();
   const int pick = s_pick[0];
-  const int len = pick < 0 ? shortest_len : shortest_len + (shortest_len * pick + 31) / 32;
-  const auto pieces_of = [&](int b) { return pick < 0 ? 0 : pieces_at(b, len); };
-  int y[4] = {0, 0, 0, 0}, y_before[4], y_total[4];
+  const bool apart = pick >= 0;  // else there are too many kinds of groups: all on one axis
+  const int len = apart ? shortest_len + (shortest_len * pick + 31) / 32 : shortest_len;
+  const auto pieces_at = [&](int m) {  // of a tile: from the cut of its first key to that of its last
+    const int lead = lead_for(s_count[s_at[m]]);
+    return (s_pos[m] + units_at(m) - 1) / len - (s_pos[m] + lead) / len + 1;
+  };
+  int wg0 = 0, wide_parts = 0;  // workgroups and pieces of these prefixes
+  if (apart) {
+    for (int m = 0; m < n_multi; ++m) {
+      if (tid == 0) s_part[m] = wide_parts;
+      wg0 += tiles_at(m) * cuts(s_end[m], len);
+      wide_parts += tiles_at(m) * pieces_at(m);
+    }
+  }
+  const auto stands_apart = [&](int b) { return apart && tiles_of(s_count[b]) > 1; };
+  int y[2] = {0, 0}, y_before[2], y_total[2];
   const auto add_cut = [&](int b) {
     const int c = s_count[b], own = s_keys[b] - s_shared[b];
-    if (c > 0) {
-      const int n = pieces_of(b);
-      if (n > 0) {
-        y[0] += n * tiles_of(c);
-        y[3] += (n - 1) * tiles_of(c);
-      } else {
-        y[1] += tiles_of(c) * (lead_for(c) + units_of(s_shared[b]));
-      }
-    }
-    if (own > 0) y[2] += tiles_of(s_tok[b]) * (lead_for(s_tok[b]) + units_of(own));
+    if (c > 0 && !stands_apart(b)) y[0] += tiles_of(c) * (lead_for(c) + units_of(s_shared[b]));
+    if (own > 0) y[1] += tiles_of(s_tok[b]) * (lead_for(s_tok[b]) + units_of(own));
   };
   for (int b = b0; b < b1; ++b) add_cut(b);
   block_sums(y, y_before, y_total, s_sum);
-  const int wg0 = y_total[0], prefix_units = y_total[1], units = prefix_units + y_total[2];
-  const int n_wg = wg0 + (units + len - 1) / len;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) y[i] = y_before[i];
+  const int prefix_units = y_total[0], units = prefix_units + y_total[1];
+  const int n_wg = wg0 + cuts(units, len);
+  y[0] = y_before[0], y[1] = y_before[1];
   for (int b = b0; b < b1; ++b) {
-    s_wg[b] = y[0];
-    s_unit[b] = y[1];
-    s_own[b] = y[2];
-    if (s_count[b] > 0) s_id[b] = y[3];  // cuts of the groups before; the ids are no longer needed
+    s_unit[b] = y[0];
+    s_own[b] = y[1];
     add_cut(b);
   }
   __syncthreads();
@@ -378,19 +404,16 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
       }
     }
   }
-  // Workspace rows: behind those of the tiles before it, each once, and 64 for every cut up to a tile's first key; tiles that are cut by
-  // themselves first, then the others along their axis.
-  const int rest_part = shared_tokens * a.group + kTileRows * wg0;
+  // Workspace rows.  Prefixes that are cut apart: 64 a piece.  Behind them, along the other axis: those of the tiles before, each once, and
+  // 64 for every cut up to a tile's first key.
+  const int rest_part = kTileRows * wide_parts;
   const auto tile_at = [&](int i) {
     Tile t;
-    int n_units, from = 0, cut = 0, rows_before;
+    int n_units, from, rows_before;
     if (i < p_tiles) {
-      const int b = last_at_or_below(s_ptile, a.B, i), k = i - s_ptile[b];
+      const int b = last_at_or_below(s_ptile, a.B, i), k = i - s_ptile[b], n = tiles_of(s_count[b]);
       n_units = units_of(s_shared[b]);
-      cut = pieces_of(b);
-      t.part = cut > 0 ? s_id[b] + k * (cut - 1) : 0;
       t.lead = lead_for(s_count[b]);
-      from = s_unit[b] + k * (t.lead + n_units);
       t.base = s_base[b];
       t.slot = s_slot[b];
       t.row0 = k * kTileRows;
@@ -398,8 +421,18 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
       t.t_begin = 0;
       t.t_end = s_shared[b];
       t.shared = 1;
-      t.again = tiles_of(s_count[b]) > 1;
-      rows_before = s_base[b] * a.group + t.row0 + (cut > 0 ? 0 : rest_part);
+      t.again = n > 1;
+      if (stands_apart(b)) {
+        const int m = s_wide[b], next = s_next[m];
+        t.n_pieces = pieces_at(m);
+        t.part = kTileRows * (s_part[m] + k * t.n_pieces);
+        t.next = next < 0 ? n_tiles : s_ptile[s_at[next]] + k;
+        return t;
+      }
+      from = s_unit[b] + k * (t.lead + n_units);
+      const int end = from + t.lead + n_units;
+      t.next = k + 1 < n ? i + 1 : end < prefix_units ? s_ptile[last_at_or_below(s_unit, a.B, end)] : p_tiles;
+      rows_before = s_base[b] * a.group + t.row0;
     } else {
       const int b = last_at_or_below(s_stile, a.B, i - p_tiles), k = i - p_tiles - s_stile[b];
       n_units = units_of(s_keys[b] - s_shared[b]);
@@ -413,17 +446,12 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
       t.t_end = s_keys[b];
       t.shared = 0;
       t.again = tiles_of(s_tok[b]) > 1;
-      rows_before = rest_part + (shared_tokens + s_len[b]) * a.group + t.row0;
+      t.next = i + 1;
+      rows_before = (shared_tokens + s_len[b]) * a.group + t.row0;
     }
-    if (cut > 0) {
-      t.n_pieces = cut;
-    } else {
-      const int first = (from + t.lead) / len;
-      t.n_pieces = (from + t.lead + n_units - 1) / len - first + 1;
-      t.part = first;
-    }
-    t.part = rows_before + kTileRows * t.part;
-    t.pad = 0;
+    const int first = (from + t.lead) / len;
+    t.n_pieces = (from + t.lead + n_units - 1) / len - first + 1;
+    t.part = rest_part + rows_before + kTileRows * first;
     return t;
   };
   for (int i = tid; i < n_wg + n_tiles; i += n_thr) {
@@ -433,17 +461,24 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
     }
     const int w = i;
     Share s;
+    int start, from;  // of the first tile's first key and of this workgroup, on their axis
     if (w < wg0) {
-      const int b = last_at_or_below(s_wg, a.B, w), n = tiles_of(s_count[b]), k = (w - s_wg[b]) / n;
-      const int all = units_of(s_shared[b]), n_pieces = pieces_of(b);
-      const int from = static_cast<int>(static_cast<int64_t>(all) * k / n_pieces);
-      s.tile = s_ptile[b] + (w - s_wg[b]) % n;
-      s.offset = lead_for(s_count[b]) + from;
-      s.units = static_cast<int>(static_cast<int64_t>(all) * (k + 1) / n_pieces) - from;
-      s.piece = k;
+      int m = 0, rest = w;  // the first group of the kind, workgroups of the kind before this one
+      for (;; ++m) {
+        const int here = tiles_at(m) * cuts(s_end[m], len);
+        if (rest < here) break;
+        rest -= here;
+      }
+      const int n = tiles_at(m), all = s_end[m];
+      from = rest / n * len;
+      while (s_pos[m] + units_at(m) <= from) m = s_next[m];
+      s.tile = s_ptile[s_at[m]] + rest % n;
+      s.offset = from - s_pos[m];
+      s.units = min(len, all - from);
+      start = s_pos[m] + lead_for(s_count[s_at[m]]);
     } else {
-      const int from = (w - wg0) * len;
-      int lead, start;
+      from = (w - wg0) * len;
+      int lead;
       s.units = min(len, units - from);
       if (from < prefix_units) {
         const int b = last_at_or_below(s_unit, a.B, from), n = lead_for(s_count[b]) + units_of(s_shared[b]), off = from - s_unit[b];
@@ -457,9 +492,9 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
         s.tile = p_tiles + s_stile[b] + off / n;
         s.offset = off % n;
       }
-      start = from - s.offset + lead;  // of the tile's first key
-      s.piece = max(0, (from - start / len * len) / len);
+      start = from - s.offset + lead;
     }
+    s.piece = max(0, from / len - start / len);
     s.first = tile_at(s.tile);
     reinterpret_cast<Share*>(a.plan + a.shares)[w] = s;
   }
@@ -1175,7 +1210,8 @@ __global__ __launch_bounds__(kThreads, (sizeof(Shared<E, D>) <= 80 * 1024 ? 2 : 
     else
       run_piece<E, D, 4, false>(a, sh, wave, t, piece, t0, t1);
     }
-    if (left <= 0 || ++i >= h.n_tiles) break;
+    i = t.next;
+    if (left <= 0 || i >= h.n_tiles) break;
     piece = 0;
     t = load_record<Tile>(a.plan + a.tiles + i * static_cast<int64_t>(sizeof(Tile)));
   }

@@ -609,7 +609,7 @@ int fp_copy_pages(void* pool, const int64_t* src, const int64_t* dst, const int3
  * same B, S, Hq, Hc, D and max_context takes the plan.  batch_idx, input_pos and the rows of page_table must not change in between: a launch
  * that meets a plan of another shape, or of other slots or positions for a row, leaves NaN in out and lse there.
  * Plan and workspace are memory of the caller (16-byte aligned), one launch at a time; nothing in them needs clearing.
- * Hq / Hc in {1, 2, 4, 8}, D in {64, 128}, B <= 2048, B * S * Hq / Hc <= 2^20, max_context <= 2^21.  Both may be captured in a graph.
+ * Hq / Hc in {1, 2, 4, 8}, D in {64, 128}, B <= 1536, B * S * Hq / Hc <= 2^20, max_context <= 2^21.  Both may be captured in a graph.
  */
 int64_t fp_shared_decode_plan_bytes(int32_t B, int32_t S, int32_t Hq, int32_t Hc, int32_t D);
 int64_t fp_shared_decode_workspace_bytes(int32_t B, int32_t S, int32_t Hq, int32_t Hc, int32_t D);
