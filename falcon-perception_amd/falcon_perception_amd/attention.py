@@ -255,6 +255,8 @@ def compiled_flex_attn_decode(q: Tensor, k: Tensor, v: Tensor, score_mod=None, b
         raise RuntimeError(
             f"the mask was converted for {tuple(block_mask.batch_idx.shape)} sequences but the last insert_kv of this "
             f"cache appended {tuple(step.batch_idx.shape)}: attention must follow the insert_kv of its own step")
+    if getattr(cache, "prefix_sharing", False):
+        return _result(*_shared_decode(q, k, v, block_mask, step, scale, sinks), return_aux, return_lse)
     kv_rep = getattr(cache, "kv_rep", 1)
     B, Hq, _, D = q.shape
     Hc = k.shape[1]
@@ -301,6 +303,25 @@ def compiled_flex_attn_decode(q: Tensor, k: Tensor, v: Tensor, score_mod=None, b
         got = ops.paged_decode(*args, scale=scale, workspace=workspace, split_tokens=split_tokens, sinks=sinks, kv_rep=kv_rep,
                                k_new=k_new, v_new=v_new, plan=plan, arrivals=arrivals, next_arrivals=after)
     return _result(*got, return_aux, return_lse)
+
+
+def _shared_decode(q: Tensor, k: Tensor, v: Tensor, mask: PagedDecodeMask, step, scale, sinks) -> tuple[Tensor, Tensor]:
+    """The decode call of a cache with `prefix_sharing`: its append goes first, the plan is made by the first layer of a step."""
+    cache = mask.cache
+    cache.flush()
+    (B, Hq, _, D), Hc = q.shape, k.shape[1]
+    pools = cache._pools[step.layer_id]
+    pool_k, pool_v = cache._planes[step.layer_id] if k is pools[0] and v is pools[1] else (k[0], v[0])
+    plan, workspace = cache.shared_decode_buffers(B, Hq, Hc, D)
+    args = (mask.batch_idx, step.input_pos, cache.prefix_ids, cache.prefix_lens)
+    shape = (B, Hq, D, Hc, step.input_pos.data_ptr())
+    if cache._decode_plan_owner is not mask or mask._plan_shape != shape or step.layer_id <= mask._plan_layer:
+        ops.shared_decode_plan(*args, q_heads=Hq, cached_heads=Hc, head_dim=D, max_context=mask.max_context, plan=plan)
+        cache._decode_plan_owner = mask
+        mask._plan_shape = shape
+    mask._plan_layer = step.layer_id
+    return ops.paged_decode_shared(q, pool_k, pool_v, cache.page_table, *args, cache.page_size, mask.max_context, scale=scale,
+                                   sinks=sinks, plan=plan, workspace=workspace)
 
 
 def compiled_flex_attn_prefill(q: Tensor, k: Tensor, v: Tensor, score_mod=None, block_mask=None,

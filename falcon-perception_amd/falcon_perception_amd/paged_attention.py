@@ -48,6 +48,11 @@ class PagedKVCache(KVCacheBase):
       page_table_cpu, capacity, free_pages, free_batch_idx   host mirrors (:60-67);
                           page 0 and batch slot 0 are reserved and never handed out
 
+    `prefix_sharing` (not an argument of the reference's class either) is for batches of requests about one picture: `fork`
+    makes sequences that begin with a cached one's tokens and share its pages, and decode attention reads such a
+    prefix once for all of them (`ops.paged_decode_shared`).  Every decode call of the cache then goes that way, captured
+    in a graph or not: which sequences share is found on the GPU, from `prefix_ids` and `prefix_lens` [max_batch].
+
     `max_blocks_per_seq` (not an argument of the reference's class) makes the tables sparse:
     page_table becomes [max_batch, max_blocks_per_seq] and the inverse table is not kept.  The
     reference's dense [max_batch, n_pages] int64 pair grows with pool size times batch size
@@ -64,7 +69,8 @@ class PagedKVCache(KVCacheBase):
     def __init__(self, n_pages: int, page_size: int, max_batch_size: int, n_heads: int, head_dim: int,
                  num_layers: int, dtype: torch.dtype, device: str | torch.device = "cuda",
                  max_blocks_per_seq: int | None = None, *, kv_rep: int | None = None,
-                 qk_normalised: bool | None = None, fuse_decode_append: bool | None = None):
+                 qk_normalised: bool | None = None, fuse_decode_append: bool | None = None,
+                 prefix_sharing: bool = False):
         self.n_pages = n_pages
         self.page_size = page_size
         self.max_batch_size = max_batch_size
@@ -133,6 +139,15 @@ class PagedKVCache(KVCacheBase):
         self._table_view: tuple[Tensor, int, Tensor] | None = None  # of `table_for`
         self._prefill_need: dict[tuple, tuple[int, int]] = {}
         self._prefill_tile_rows: dict[tuple, int] = {}
+        # prefix sharing: pages that several slots map (page -> slots), what each slot shares (id, tokens, whether it is a
+        # fork), and the same by slot on the GPU for the decode kernel's plan
+        self.prefix_sharing = bool(prefix_sharing)
+        self._page_slots: dict[int, int] = {}
+        self._prefixes: dict[int, tuple[int, int, bool]] = {}
+        self._last_prefix_id = 0
+        self.prefix_ids = torch.zeros(max_batch_size, dtype=torch.int32, device=device) if prefix_sharing else None
+        self.prefix_lens = torch.zeros(max_batch_size, dtype=torch.int32, device=device) if prefix_sharing else None
+        self._shared_buffers: dict[tuple, tuple[Tensor, Tensor, int]] = {}
         # status word of the last prefill mask, on its way to the host (`check_prefill_masks`)
         self._mask_status_host: Tensor | None = None
         self._mask_status_event = None
@@ -326,12 +341,132 @@ class PagedKVCache(KVCacheBase):
         self.flush()
         self.check_prefill_masks(wait=False)
         self.free_batch_idx.append(batch_idx)
-        self.free_pages.extend(reversed(self.page_table_cpu[batch_idx]))
+        pages = self.page_table_cpu[batch_idx]
+        if self._page_slots:  # pages that other slots map stay theirs
+            kept = {page for page in pages if self._page_slots.get(page, 1) > 1}
+            for page in kept:
+                self._page_slots[page] -= 1
+                if self._page_slots[page] == 1:
+                    del self._page_slots[page]
+            pages = [page for page in pages if page not in kept]
+        self.free_pages.extend(reversed(pages))
+        if self._prefixes.pop(batch_idx, None) is not None and self.prefix_sharing:
+            self.prefix_ids[batch_idx].zero_()
         self.page_table_cpu[batch_idx] = []
         self.page_table[batch_idx].fill_(-1)
         if self.physical_to_logical is not None:
             self.physical_to_logical[batch_idx].fill_(-1)
         self.capacity[batch_idx] = 0
+
+    # ----------------------------------------------------- steps of many requests
+    def step_tables(self, slots: list[int], old_lens: list[int], new_lens: list[int], *,
+                    row_multiple: int = 1) -> "ops.StepTables":
+        """Reserve the step of a batch and make its packed rows: slot `slots[i]` grows from `old_lens[i]` cached tokens to
+        `new_lens[i]`.  What `reserve`, called for each of them in turn, does to the page table and the free list, in one
+        upload and one launch instead of an upload and two index writes a request; the rows (`batch_idx`, `input_pos`,
+        `slot_map`, see `ops.step_tables`) are what a packed prefill step is given, each request's padded to `row_multiple`.
+        Not a method of the reference's class.  Raises, and changes nothing, where the pool or the table is short."""
+        return self._step(slots, old_lens, new_lens, [0] * len(slots), row_multiple)
+
+    def fork(self, parent: int, n_tokens: int, count: int = 1) -> list[int]:
+        """`count` new slots that begin with the first `n_tokens` cached tokens of slot `parent` and share its whole pages;
+        of the page the prefix ends in, each gets a copy.  The parent, and a fork of a fork, live on independently: a page
+        goes back to the free list with the last slot that maps it.  Nothing may be written to the shared positions of
+        any of them afterwards.  Not a method of the reference's class."""
+        ops.N.require_cuda(self.page_table)
+        if not 0 < parent < self.max_batch_size:
+            raise RuntimeError(f"Slot {parent} cannot be forked.")
+        if not 0 < n_tokens <= self.capacity[parent]:
+            raise RuntimeError(f"Cannot fork {n_tokens} tokens of slot {parent}, which holds {self.capacity[parent]}.")
+        if count > len(self.free_batch_idx):
+            raise RuntimeError(f"Cannot fork {count} sequences. Only {len(self.free_batch_idx)} slots available.")
+        if count < 1:
+            return []
+        self.flush()
+        whole = n_tokens // self.page_size
+        tail = n_tokens > whole * self.page_size
+        if tail and self.num_free_pages < count:
+            raise RuntimeError(f"Cannot reserve {count} pages for forks of slot {parent}. Only {self.num_free_pages} pages available.")
+        slots = [self.free_batch_idx.pop() for _ in range(count)]
+        self.page_table[slots] = -1
+        if self.physical_to_logical is not None:
+            self.physical_to_logical[slots] = -1
+        shared = self.page_table_cpu[parent][:whole]
+        for slot in slots:
+            self.page_table_cpu[slot] = list(shared)
+            self.capacity[slot] = whole * self.page_size
+        for page in shared:
+            self._page_slots[page] = self._page_slots.get(page, 1) + count
+        made = self._step(slots, [n_tokens] * count, [n_tokens] * count, [parent] * count, 1)
+        if tail:
+            ops.copy_pages(self._kv, made.copy_src, made.copy_dst, made.copy_rows, self.page_size)
+        # Slots with one id share at least the smaller of their two lengths: a fork's length is what it shares with the first sequence
+        # of its line, and that one's is the longest of its own forks'.
+        root_id, root_len, forked = self._prefixes.get(parent, (0, 0, False))
+        if root_id == 0:
+            self._last_prefix_id += 1
+            root_id = self._last_prefix_id
+        length = min(n_tokens, root_len) if forked else n_tokens
+        if not forked:
+            self._prefixes[parent] = (root_id, max(root_len, n_tokens), False)
+        for slot in slots:
+            self._prefixes[slot] = (root_id, length, True)
+        if self.prefix_sharing:
+            rows = [*slots, parent]
+            values = torch.tensor([rows, [self._prefixes[r][0] for r in rows], [self._prefixes[r][1] for r in rows]], device=self.device)
+            self.prefix_ids[values[0]] = values[1].int()
+            self.prefix_lens[values[0]] = values[2].int()
+        return slots
+
+    def _step(self, slots, old_lens, new_lens, parents, row_multiple) -> "ops.StepTables":
+        ops.N.require_cuda(self.page_table)
+        P, B = self.page_size, len(slots)
+        if len(old_lens) != B or len(new_lens) != B:
+            raise ValueError("slots, old_lens and new_lens must have one entry per request")
+        if len(set(slots)) != B or any(not 0 < s < self.max_batch_size for s in slots):
+            raise ValueError("slots must be different cache slots other than 0")
+        if any(not 0 <= o <= n for o, n in zip(old_lens, new_lens)):
+            raise ValueError("a step cannot make a sequence shorter")
+        if row_multiple < 1:
+            raise ValueError("row_multiple must be at least 1")
+        grow = [max(0, _cdiv(n, P) - len(self.page_table_cpu[s])) for s, n in zip(slots, new_lens)]
+        if sum(grow) > self.num_free_pages:
+            raise RuntimeError(f"Cannot reserve {sum(grow)} pages for a step of {B} sequences. Only {self.num_free_pages} pages available.")
+        if any(_cdiv(n, P) > self.table_cols for n in new_lens):
+            raise RuntimeError(f"Cannot reserve a sequence of length {max(new_lens)}: the page table holds {self.table_cols} blocks of "
+                               f"{P} tokens per sequence.")
+        if any(o > len(self.page_table_cpu[s]) * P for s, o, p in zip(slots, old_lens, parents) if p == 0):
+            raise RuntimeError("a sequence has no pages for the tokens it is said to have cached")
+        # the pages each request gets, in the place where the kernel looks for them: the last request's first.  Pages that were reserved
+        # ahead of the step are written again as they are.
+        pages: list[int] = []
+        for s, o, n, p, more in zip(slots, old_lens, new_lens, parents, grow):
+            if more:
+                self.page_table_cpu[s] += self.free_pages[-more:]
+                del self.free_pages[-more:]
+                self.capacity[s] = len(self.page_table_cpu[s]) * P
+            have = o // P if p > 0 else _cdiv(o, P)
+            pages = self.page_table_cpu[s][have:_cdiv(n, P)] + pages
+        packed = torch.tensor([*slots, *old_lens, *new_lens, *parents, *pages, len(pages)], dtype=torch.int64, device=self.device)
+        ids, old, new, par = (packed[i * B:(i + 1) * B] for i in range(4))
+        rows = sum(-(-(n - o) // row_multiple) * row_multiple for o, n in zip(old_lens, new_lens))
+        return ops.step_tables(ids, old, new, packed[4 * B:-1], packed[-1:].view(torch.int32)[:1], self.page_table, P, rows,
+                               parents=par, row_multiple=row_multiple, inverse=self.physical_to_logical)
+
+    def shared_decode_buffers(self, B: int, Hq: int, Hc: int, D: int) -> tuple[Tensor, Tensor]:
+        """Plan and workspace of the decode launches over shared prefixes, for every batch up to the cache's largest: graphs
+        captured with them stay valid."""
+        key = (Hq, Hc, D)
+        hit = self._shared_buffers.get(key)
+        if hit is None or hit[2] < B:
+            most = max(B, min(self.max_batch_size, 1536))
+            shape = dict(q_heads=Hq, cached_heads=Hc, head_dim=D)
+            sizes = ops.shared_decode_plan_bytes(most, 1, **shape), ops.shared_decode_workspace_bytes(most, 1, **shape)
+            if hit is not None:
+                self._retired_workspaces.extend(hit[:2])
+            plan, workspace = (torch.zeros(n, dtype=torch.uint8, device=self._kv.device) for n in sizes)
+            hit = self._shared_buffers[key] = (plan, workspace, most)
+        return hit[0], hit[1]
 
     # ------------------------------------------------------------------- masks
     def convert_logical_block_mask(self, block_mask: BlockMask, batch_idx: Tensor | None = None) -> PagedDecodeMask:
