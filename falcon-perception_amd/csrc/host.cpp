@@ -315,6 +315,14 @@ PyObject* shared_unguarded(PyObject* const* args) {
   return pair(out, lse);
 }
 
+// n elements of a byte buffer's memory, from `offset` bytes on, as a tensor that shares it
+at::Tensor part(const at::Tensor& buffer, int64_t offset, int64_t n, at::ScalarType type) {
+  at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buffer.storage()), buffer.key_set(), c10::scalarTypeToTypeMeta(type));
+  t.unsafeGetTensorImpl()->set_storage_offset(buffer.storage_offset() + offset / static_cast<int64_t>(c10::elementSize(type)));
+  t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  return t;
+}
+
 // slots, old_lens, new_lens, free_pages, free_count, page_table, page_size, max_rows, parents, row_multiple, inverse, device, stream ->
 // the nine tensors of StepTables
 PyObject* tables_unguarded(PyObject* const* args) {
@@ -338,10 +346,19 @@ PyObject* tables_unguarded(PyObject* const* args) {
   int rc;
   {
     const Unlocked others;
-    const auto options = slots->options(), whole = options.dtype(at::kInt);
-    const int64_t sizes[9] = {rows, rows, rows, B + 1, 1, B, B, B, 1};
-    const bool is_long[9] = {true, false, true, false, false, true, true, false, false};
-    for (int i = 0; i < 9; ++i) made[i] = at::empty({sizes[i]}, is_long[i] ? options : whole);
+    // two allocations, the rows and the rest: nine cost as much as the launch
+    const auto bytes = slots->options().dtype(at::kByte);
+    const int64_t wide = (rows + 3) / 4 * 4;
+    const at::Tensor big = at::empty({20 * wide}, bytes), small = at::empty({16 * B + 4 * (2 * B + 3)}, bytes);
+    made[0] = part(big, 0, rows, at::kLong);
+    made[2] = part(big, 8 * wide, rows, at::kLong);
+    made[1] = part(big, 16 * wide, rows, at::kInt);
+    made[5] = part(small, 0, B, at::kLong);
+    made[6] = part(small, 8 * B, B, at::kLong);
+    made[3] = part(small, 16 * B, B + 1, at::kInt);
+    made[7] = part(small, 20 * B + 4, B, at::kInt);
+    made[4] = part(small, 24 * B + 4, 1, at::kInt);
+    made[8] = part(small, 24 * B + 8, 1, at::kInt);
     const auto at = [&](int i) { return made[i].data_ptr(); };
     rc = fp_step_tables(static_cast<const int64_t*>(slots->data_ptr()), before->data_ptr(), after->data_ptr(), index_code(*before),
                         parents ? static_cast<const int64_t*>(parents->data_ptr()) : nullptr, static_cast<const int64_t*>(pages->data_ptr()),

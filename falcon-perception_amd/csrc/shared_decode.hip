@@ -1354,8 +1354,8 @@ extern "C" int fp_shared_decode_plan(const int64_t* batch_idx, const void* input
   const int threads = S > 1 || B > 64 ? 1024 : 256;
   const size_t lds = kPlanArrays * static_cast<size_t>((B + 3) & ~3) * sizeof(int);
   if (lds > 64 * 1024) {
-    static const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(shared_plan_kernel),
-                                                          hipFuncAttributeMaxDynamicSharedMemorySize, kPlanArrays * kMaxSequences * sizeof(int));
+    const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(shared_plan_kernel),
+                                                   hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
     if (allowed != hipSuccess) return fp::fail(FP_ERR_LAUNCH, "%s: %s", what, hipGetErrorString(allowed));
   }
   hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3(threads), lds, static_cast<hipStream_t>(stream), a);

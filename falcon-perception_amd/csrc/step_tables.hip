@@ -18,6 +18,8 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kMaxRequests = 4096;
 constexpr int kMaxSlots = 1 << 17;
+typedef int64_t v2l __attribute__((ext_vector_type(2)));
+typedef int v4i __attribute__((ext_vector_type(4)));
 
 struct TablesArgs {
   const int64_t* slots;
@@ -41,7 +43,13 @@ struct TablesArgs {
   int32_t* copy_rows;
   int32_t* status;
   int B, max_rows, row_multiple, columns, max_batch, n_free;
+  int wide;  // the rows' arrays are 16-byte aligned
   fp::PageDiv pd;
+};
+
+// What the rows of a request need of it, in LDS.
+struct Record {
+  int slot, old_len, new_len, have;
 };
 
 struct Request {
@@ -74,17 +82,27 @@ __device__ __forceinline__ int64_t padded_rows(const TablesArgs& a, const Reques
   return (n + a.row_multiple - 1) / a.row_multiple * a.row_multiple;
 }
 
+__device__ __forceinline__ int64_t pages_of_request(const TablesArgs& a, const Record& r) {
+  int64_t end;
+  int rest;
+  a.pd.split(r.new_len, end, rest);
+  end += rest > 0;
+  return end > r.have ? end - r.have : 0;
+}
+
 // page of block c of a request: its own row, its parent's or the free list, none of which this launch writes there
 __device__ __forceinline__ int64_t page_of(const TablesArgs& a, const Request& r, int64_t c, int64_t first_free) {
   if (c >= r.have) return a.free_pages[first_free + c - r.have];
   return a.page_table[(r.parent > 0 ? r.parent : r.slot) * a.pt_row_stride + c];
 }
 
+template <int kRows>  // neighbours that a thread has
 __global__ __launch_bounds__(kThreads) void step_tables_kernel(const TablesArgs a) {
-  extern __shared__ int s_mem[];
+  extern __shared__ __attribute__((aligned(16))) int s_mem[];
   int* const s_start = s_mem;                      // [B + 1] first row of every request
   int* const s_free = s_mem + a.B + 1;             // [B] pages taken by the requests before
   uint32_t* const s_named = reinterpret_cast<uint32_t*>(s_free + a.B);  // bit per slot: named by a request
+  Record* const s_rec = reinterpret_cast<Record*>(s_mem + (2 * a.B + 1 + (a.max_batch + 31) / 32 + 3) / 4 * 4);
   const int words = (a.max_batch + 31) / 32;
   __shared__ int64_t s_sum[kWaves][2];
   __shared__ int s_bad;
@@ -99,18 +117,31 @@ __global__ __launch_bounds__(kThreads) void step_tables_kernel(const TablesArgs 
   const int64_t count = *a.free_count;
   int64_t rows = 0, pages = 0;
   int bad = count < 0 || count > a.n_free ? 8 : 0;
-  for (int b = b0; b < b1; ++b) {
-    const Request r = load_request(a, b);
-    if (r.slot <= 0 || r.slot >= a.max_batch || r.parent >= a.max_batch || r.old_len < 0 || r.new_len < r.old_len ||
-        r.new_len > INT32_MAX) {
-      bad |= 8;
-      continue;
+  for (int b4 = b0; b4 < b1; b4 += 4) {
+    Request four[4];  // on their way together
+#pragma unroll
+    for (int k = 0; k < 4; ++k) four[k] = load_request(a, min(b4 + k, b1 - 1));
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int b = b4 + k;
+      if (b >= b1) break;
+      const Request& r = four[k];
+      if (r.slot <= 0 || r.slot >= a.max_batch || r.parent >= a.max_batch || r.old_len < 0 || r.new_len < r.old_len ||
+          r.new_len > INT32_MAX) {
+        bad |= 8;
+        continue;
+      }
+      const uint32_t bit = 1u << (r.slot & 31);
+      if (atomicOr(&s_named[r.slot >> 5], bit) & bit) bad |= 8;  // a slot that two requests name
+      if (r.blocks > a.columns) bad |= 2;
+      const int64_t n = padded_rows(a, r);
+      if (n > a.max_rows) bad |= 4;
+      rows += n;
+      pages += r.need();
+      s_start[b] = static_cast<int>(n);  // its own rows and pages for now, below those of the requests before it
+      s_free[b] = static_cast<int>(r.need());
+      s_rec[b] = Record{static_cast<int>(r.slot), static_cast<int>(r.old_len), static_cast<int>(r.new_len), static_cast<int>(r.have)};
     }
-    const uint32_t bit = 1u << (r.slot & 31);
-    if (atomicOr(&s_named[r.slot >> 5], bit) & bit) bad |= 8;  // a slot that two requests name
-    if (r.blocks > a.columns) bad |= 2;
-    rows += padded_rows(a, r);
-    pages += r.need();
   }
   int64_t rows_upto = rows, pages_upto = pages;
 #pragma unroll
@@ -129,14 +160,15 @@ __global__ __launch_bounds__(kThreads) void step_tables_kernel(const TablesArgs 
   }
   if (rows_all > a.max_rows) bad |= 4;
   if (pages_all > count) bad |= 1;
-  for (int b = b0; b < b1; ++b) {
-    const Request r = load_request(a, b);
-    if (r.parent > 0 && r.parent < a.max_batch && s_named[r.parent >> 5] >> (r.parent & 31) & 1) bad |= 8;
-    s_start[b] = static_cast<int>(rows_upto);
-    s_free[b] = static_cast<int>(pages_upto);
-    if (r.slot > 0 && r.slot < a.max_batch && r.parent < a.max_batch && r.old_len >= 0 && r.new_len >= r.old_len) {
-      rows_upto += padded_rows(a, r);
-      pages_upto += r.need();
+  if (!bad) {  // else nothing is done
+    for (int b = b0; b < b1; ++b) {
+      const int64_t parent = a.parents ? a.parents[b] : 0;
+      if (parent > 0 && s_named[parent >> 5] >> (parent & 31) & 1) bad |= 8;
+      const int n = s_start[b], need = s_free[b];
+      s_start[b] = static_cast<int>(rows_upto);
+      s_free[b] = static_cast<int>(pages_upto);
+      rows_upto += n;
+      pages_upto += need;
     }
   }
   if (bad) atomicOr(&s_bad, bad);
@@ -180,29 +212,67 @@ __global__ __launch_bounds__(kThreads) void step_tables_kernel(const TablesArgs 
   }
 
   // packed rows
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kThreads + tid; row < a.max_rows; row += static_cast<int64_t>(gridDim.x) * kThreads) {
-    int64_t slot = 0, where = 0;
-    int pos = 0;
-    if (row < n_rows) {
-      int lo = 0, hi = a.B - 1;  // the last request that starts at or before the row and is not empty
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * kThreads * kRows;
+  for (int64_t row0 = (static_cast<int64_t>(blockIdx.x) * kThreads + tid) * kRows; row0 < a.max_rows; row0 += stride) {
+    int64_t slot[kRows] = {}, where[kRows] = {};
+    int pos[kRows] = {};
+    if (row0 < n_rows) {
+      int lo = 0, hi = a.B - 1;  // the last request that starts at or before the row
       while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (s_start[mid] <= row) lo = mid; else hi = mid - 1;
+        if (s_start[mid] <= row0) lo = mid; else hi = mid - 1;
       }
-      const Request r = load_request(a, lo);
-      const int64_t p = r.old_len + row - s_start[lo];
-      if (p < r.new_len) {
+      Record r = s_rec[lo];
+      int64_t blk_now = -1, page = 0;
+#pragma unroll
+      for (int k = 0; k < kRows; ++k) {
+        const int64_t row = row0 + k;
+        if (row >= n_rows) break;
+        if (row >= s_start[lo + 1]) {
+          do ++lo; while (row >= s_start[lo + 1]);
+          r = s_rec[lo];
+          blk_now = -1;
+        }
+        const int64_t p = r.old_len + (row - s_start[lo]);
+        if (p >= r.new_len) continue;
         int64_t blk;
         int off;
         a.pd.split(p, blk, off);
-        slot = r.slot;
-        pos = static_cast<int>(p);
-        where = page_of(a, r, blk, count - s_free[lo] - r.need()) * a.pd.page_size + off;
+        if (blk != blk_now) {
+          blk_now = blk;
+          // behind the blocks it has, the free list; else its own row, which this launch does not write there (a fork's rows begin
+          // behind its shared blocks)
+          const int64_t need = pages_of_request(a, r);
+          page = (blk >= r.have ? a.free_pages[count - s_free[lo] - need + blk - r.have]
+                                : a.page_table[r.slot * a.pt_row_stride + blk]) * a.pd.page_size;
+        }
+        slot[k] = r.slot;
+        pos[k] = static_cast<int>(p);
+        where[k] = page + off;
       }
     }
-    a.batch_idx[row] = slot;
-    a.input_pos[row] = pos;
-    a.slot_map[row] = where;
+    bool stored = false;
+    if constexpr (kRows == 4) {
+      if (a.wide && row0 + 4 <= a.max_rows) {
+      v2l* const to_slot = reinterpret_cast<v2l*>(a.batch_idx + row0);
+      v2l* const to_where = reinterpret_cast<v2l*>(a.slot_map + row0);
+      to_slot[0] = v2l{slot[0], slot[1]};
+      to_slot[1] = v2l{slot[2], slot[3]};
+      to_where[0] = v2l{where[0], where[1]};
+      to_where[1] = v2l{where[2], where[3]};
+      *reinterpret_cast<v4i*>(a.input_pos + row0) = v4i{pos[0], pos[1], pos[2], pos[3]};
+        stored = true;
+      }
+    }
+    if (!stored) {
+#pragma unroll
+      for (int k = 0; k < kRows; ++k) {
+        if (row0 + k >= a.max_rows) break;
+        a.batch_idx[row0 + k] = slot[k];
+        a.input_pos[row0 + k] = pos[k];
+        a.slot_map[row0 + k] = where[k];
+      }
+    }
   }
 }
 
@@ -232,13 +302,22 @@ extern "C" int fp_step_tables(const int64_t* slots, const void* old_lens, const 
   const TablesArgs a{slots, old_lens, new_lens, len_index_type, parents, free_pages, free_count, page_table, pt_row_stride,
                      inverse, inv_row_stride, inv_cols, batch_idx, input_pos, slot_map, row_starts, free_left, copy_src,
                      copy_dst, copy_rows, status, B, max_rows, row_multiple, n_pages, max_batch, n_free,
-                     fp::PageDiv(page_size)};
-  const int64_t work = max_rows > 64ll * B ? max_rows : 64ll * B;  // threads that find something to do at once
-  const int64_t most = 8ll * fp::compute_units();
+                     fp::aligned(batch_idx, 16) && fp::aligned(input_pos, 16) && fp::aligned(slot_map, 16), fp::PageDiv(page_size)};
+  // A row a thread while that many threads run at once: a decode step's rows belong to as many requests, whose numbers four rows of one
+  // thread would fetch one after the other (64 requests 5.4 us, 7.8 with four).  Beyond, four: one request and one page, mostly, and
+  // stores of 16 bytes (2 million rows @@).
+  const int64_t most = 2ll * fp::compute_units();  // workgroups; each of them reads all requests
+  const bool few = max_rows <= most * kThreads;
+  const int64_t turns = few ? max_rows : (max_rows + 3) / 4, work = turns > 64ll * B ? turns : 64ll * B;
   int64_t grid = (work + kThreads - 1) / kThreads;
   grid = grid < 1 ? 1 : grid > most ? most : grid;
-  const size_t lds = (2 * static_cast<size_t>(B) + 1 + (max_batch + 31) / 32) * sizeof(int);
-  hipLaunchKernelGGL(step_tables_kernel, dim3(static_cast<unsigned>(grid)), dim3(kThreads), lds,
-                     static_cast<hipStream_t>(stream), a);
+  const size_t lds = (2 * static_cast<size_t>(B) + 1 + (max_batch + 31) / 32 + 3) / 4 * 16 + B * sizeof(Record);
+  const auto go = [&](auto kernel) {
+    if (lds > 64 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                               static_cast<int>(lds)) != hipSuccess)
+      return;  // the launch below would be refused: check_launch says so
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(kThreads), lds, static_cast<hipStream_t>(stream), a);
+  };
+  few ? go(step_tables_kernel<1>) : go(step_tables_kernel<4>);
   return fp::check_launch("fp_step_tables");
 }
