@@ -121,7 +121,7 @@ struct PlanArgs {
 };
 
 // What a tile costs before its first key and behind its last, in units.
-__device__ __forceinline__ int lead_of(int rows) { return rows <= 16 ? 2 : rows <= 32 ? 3 : 5; }
+__device__ __forceinline__ int lead_of(int rows) { return rows <= 16 ? 2 : rows <= 32 ? 3 : 6; }
 
 __device__ __forceinline__ int units_of(int keys) { return (keys + kUnit - 1) / kUnit; }
 
@@ -161,7 +161,7 @@ __device__ __forceinline__ void block_sums(const int (&x)[N], int (&before)[N], 
   __syncthreads();
 }
 
-constexpr int kPlanArrays = 20;
+constexpr int kPlanArrays = 23;
 
 __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   extern __shared__ int s_mem[];
@@ -182,7 +182,10 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   int* const s_own = s_unit + Bp;      //   units of own keys,
   int* const s_wide = s_own + Bp;      // place of a group of several tiles in the lists of these:
   int* const s_at = s_wide + Bp;       //   its first sequence,
-  int* const s_pos = s_at + Bp;        //   its place on the axis of its kind,
+  int* const s_n = s_at + Bp;          //   its tiles,
+  int* const s_u = s_n + Bp;           //   units of each, with the lead
+  int* const s_lu = s_u + Bp;          //   the lead,
+  int* const s_pos = s_lu + Bp;        //   its place on the axis of its kind,
   int* const s_end = s_pos + Bp;       //   length of that axis, at the first of a kind, elsewhere 0,
   int* const s_next = s_end + Bp;      //   the next of its kind, -1: none,
   int* const s_part = s_next + Bp;     //   pieces of the groups before
@@ -295,6 +298,9 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
     if (s_count[b] > 0 && tiles_of(s_count[b]) > 1) {
       s_wide[b] = x[5];
       s_at[x[5]] = b;
+      s_n[x[5]] = tiles_of(s_count[b]);
+      s_lu[x[5]] = lead_for(s_count[b]);
+      s_u[x[5]] = lead_for(s_count[b]) + units_of(s_shared[b]);
     }
     add(b);
   }
@@ -305,14 +311,12 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   // lie on one axis, every cut of it is a workgroup for each of the tiles, and these run at the same time and find what the first of
   // them loads in their XCD's L2.  (With its tiles one behind the other all of them read the keys from beyond L2.)  That takes a few
   // more workgroups, so `len` is the shortest of 64 lengths, a lane each, for which there are enough.
-  const auto tiles_at = [&](int m) { return tiles_of(s_count[s_at[m]]); };
-  const auto units_at = [&](int m) { return lead_for(s_count[s_at[m]]) + units_of(s_shared[s_at[m]]); };
   for (int m = tid; m < n_multi; m += n_thr) {
-    const int n = tiles_at(m);
+    const int n = s_n[m];
     int pos = 0, all = 0, next = -1, first = 1;
     for (int i = 0; i < n_multi; ++i) {
-      if (tiles_at(i) != n) continue;
-      const int u = units_at(i);
+      if (s_n[i] != n) continue;
+      const int u = s_u[i];
       all += u;
       if (i < m) {
         pos += u;
@@ -332,8 +336,8 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
     const int len = shortest_len + (shortest_len * lane + 31) / 32;
     int need = 0, rest = all_units;
     for (int m = 0; m < n_multi; ++m) {
-      need += tiles_at(m) * cuts(s_end[m], len);
-      rest -= tiles_at(m) * units_at(m);
+      need += s_n[m] * cuts(s_end[m], len);
+      rest -= s_n[m] * s_u[m];
     }
     const unsigned long long enough = __ballot(need + cuts(rest, len) <= a.n_wg);
     if (enough != 0 && lane == 0) s_pick[0] = __builtin_ctzll(enough);
@@ -343,15 +347,14 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   const bool apart = pick >= 0;  // else there are too many kinds of groups: all on one axis
   const int len = apart ? shortest_len + (shortest_len * pick + 31) / 32 : shortest_len;
   const auto pieces_at = [&](int m) {  // of a tile: from the cut of its first key to that of its last
-    const int lead = lead_for(s_count[s_at[m]]);
-    return (s_pos[m] + units_at(m) - 1) / len - (s_pos[m] + lead) / len + 1;
+    return (s_pos[m] + s_u[m] - 1) / len - (s_pos[m] + s_lu[m]) / len + 1;
   };
   int wg0 = 0, wide_parts = 0;  // workgroups and pieces of these prefixes
   if (apart) {
     for (int m = 0; m < n_multi; ++m) {
       if (tid == 0) s_part[m] = wide_parts;
-      wg0 += tiles_at(m) * cuts(s_end[m], len);
-      wide_parts += tiles_at(m) * pieces_at(m);
+      wg0 += s_n[m] * cuts(s_end[m], len);
+      wide_parts += s_n[m] * pieces_at(m);
     }
   }
   const auto stands_apart = [&](int b) { return apart && tiles_of(s_count[b]) > 1; };
@@ -465,17 +468,17 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
     if (w < wg0) {
       int m = 0, rest = w;  // the first group of the kind, workgroups of the kind before this one
       for (;; ++m) {
-        const int here = tiles_at(m) * cuts(s_end[m], len);
+        const int here = s_n[m] * cuts(s_end[m], len);
         if (rest < here) break;
         rest -= here;
       }
-      const int n = tiles_at(m), all = s_end[m];
+      const int n = s_n[m], all = s_end[m];
       from = rest / n * len;
-      while (s_pos[m] + units_at(m) <= from) m = s_next[m];
+      while (s_pos[m] + s_u[m] <= from) m = s_next[m];
       s.tile = s_ptile[s_at[m]] + rest % n;
       s.offset = from - s_pos[m];
       s.units = min(len, all - from);
-      start = s_pos[m] + lead_for(s_count[s_at[m]]);
+      start = s_pos[m] + s_lu[m];
     } else {
       from = (w - wg0) * len;
       int lead;
