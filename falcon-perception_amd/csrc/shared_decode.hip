@@ -29,6 +29,11 @@ using fp_decode::kLn2;
 using fp_decode::kLog2e;
 using fp_decode::safe_max;
 
+// The sink gate (model.py:122-128) in 32 bits: the product is rounded once, when it is stored.
+__device__ __forceinline__ float gated(float o, float lse, const float* sinks, int h) {
+  return sinks == nullptr ? o : o / (1.f + __expf(sinks[h] - lse));
+}
+
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kMaxSequences = 1536;
@@ -565,16 +570,18 @@ struct BF16 {
   static __device__ __forceinline__ f32x4 mfma_k32(const v4u& a, const v4u& b, const f32x4& c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vec8, a), __builtin_bit_cast(vec8, b), c, 0, 0, 0);
   }
-  static __device__ __forceinline__ f32x4 mfma_k16(const s16x4& a, const s16x4& b, const f32x4& c) {
-    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0);
-  }
   static __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     typedef __bf16 vec2 __attribute__((ext_vector_type(2)));
     const vec2 v = {static_cast<__bf16>(lo), static_cast<__bf16>(hi)};
     return __builtin_bit_cast(uint32_t, v);
   }
-  static __device__ __forceinline__ float above_zero(float p) { return p; }  // fp32's exponents: no p rounds to 0
-  static __device__ __forceinline__ float to_float(uint32_t bits) { return __uint_as_float(bits << 16); }
+  // p0 and p1 as sums of two numbers of the type, none below 0 (and above it where p is), so that against an infinite V element
+  // they give infinity: truncated, and what is left over, with 2^-23 of p on top.
+  static __device__ __forceinline__ void split(float p0, float p1, uint32_t& hi, uint32_t& lo) {
+    const uint32_t b0 = __float_as_uint(p0), b1 = __float_as_uint(p1);
+    hi = __builtin_amdgcn_perm(b1, b0, 0x07060302);
+    lo = pack2(fmaf(p0, 1.f + 0x1p-23f, -__uint_as_float(b0 & 0xffff0000u)), fmaf(p1, 1.f + 0x1p-23f, -__uint_as_float(b1 & 0xffff0000u)));
+  }
   static __device__ __forceinline__ float round(float v) { return static_cast<float>(static_cast<__bf16>(v)); }
 };
 struct F16 {
@@ -592,19 +599,17 @@ struct F16 {
   static __device__ __forceinline__ f32x4 mfma_k32(const v4u& a, const v4u& b, const f32x4& c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vec8, a), __builtin_bit_cast(vec8, b), c, 0, 0, 0);
   }
-  static __device__ __forceinline__ f32x4 mfma_k16(const s16x4& a, const s16x4& b, const f32x4& c) {
-    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(vec4, a), __builtin_bit_cast(vec4, b), c, 0, 0, 0);
-  }
   static __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     typedef _Float16 vec2 __attribute__((ext_vector_type(2)));
     const vec2 v = {static_cast<_Float16>(lo), static_cast<_Float16>(hi)};
     return __builtin_bit_cast(uint32_t, v);
   }
-  // a probability that would round to 0 becomes the smallest number of the type (2^-32 of the largest), so that an infinite V
-  // element still meets something above 0
-  static __device__ __forceinline__ float above_zero(float p) { return fmaxf(p, fminf(p * 0x1p+102f, 0x1p-24f)); }
-  static __device__ __forceinline__ float to_float(uint32_t bits) {
-    return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(bits)));
+  // As above.  Neither part of a p above 0 is below the smallest number of the type, 2^-32 of the largest p.
+  static __device__ __forceinline__ void split(float p0, float p1, uint32_t& hi, uint32_t& lo) {
+    const float l0 = fminf(p0 * 0x1p+102f, 0x1p-24f), l1 = fminf(p1 * 0x1p+102f, 0x1p-24f);
+    const auto h = __builtin_amdgcn_cvt_pkrtz(fmaxf(p0, l0), fmaxf(p1, l1));
+    hi = __builtin_bit_cast(uint32_t, h);
+    lo = pack2(fmaxf(p0 - static_cast<float>(h[0]), l0), fmaxf(p1 - static_cast<float>(h[1]), l1));
   }
   static __device__ __forceinline__ float round(float v) { return static_cast<float>(static_cast<_Float16>(v)); }
 };
@@ -652,6 +657,7 @@ struct Geo {
   static constexpr int NB = TS / 16;               // blocks of 16 keys
   static constexpr int DB = D / 16;                // blocks of 16 rows of O^T
   static constexpr int QV = ROWB / 64;             // 16-byte operand registers of a query row
+  static constexpr bool QTAIL = k16 && D == 128;
   static constexpr int RING = 2 * 2 * HALF;        // two stages a wavefront
   static constexpr int PASS = RING / (16 * D * 4) < 4 ? RING / (16 * D * 4) : 4;  // column blocks whose states fit a ring
   static __device__ __forceinline__ int k_swz(int r) { return CPR == 8 ? (r >> 1) & 7 : r & 15; }
@@ -680,6 +686,7 @@ struct Shared {
   __attribute__((aligned(8))) float ml[kWaves][kTileRows][2];
   float joined[kTileRows][2];    // maximum and sum of all wavefronts
   int limit[kWaves][kTileRows];  // keys of the columns' rows, each wavefront's own copy
+  __attribute__((aligned(16))) v4u q_tail[G::QTAIL ? 4 * 64 : 1];  // last quarter of the query rows, by column block and lane
   int tainted;  // an element of V that is not finite was left out
 };
 
@@ -733,9 +740,8 @@ __device__ __forceinline__ void add_infinities(const SharedArgs& a, const Tile& 
 // for partial results that nobody here reads.)
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory"); }
 
-// One piece: the rows of a tile over its keys [t0, t1).  CB blocks of 16 columns; kSplit: at most 8 rows, in columns 0 .. 7 and again in
-// 8 .. 15, whose probabilities carry what the rounding of the first left over.
-template <typename E, int D, int CB, bool kSplit>
+// One piece: the rows of a tile over its keys [t0, t1).  CB blocks of 16 columns.
+template <typename E, int D, int CB>
 __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh, const int wave, const Tile& tile, const int piece,
                                           const int t0, const int t1) {
   using G = Geo<E, D>;
@@ -759,7 +765,10 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
   }
 
   // rows: query operands and limits of this lane's columns.  A column without a row repeats row 0, sees everything and is not stored.
-  v4u q[CB][G::QV];
+  // Of four column blocks at head_dim 128 the last quarter of the query rows stays in LDS: with it the registers would not hold the rest.
+  constexpr bool kTail = CB == 4 && G::QTAIL;
+  constexpr int QR = kTail ? G::QV - 1 : G::QV;
+  v4u q[CB][QR], tail = {0, 0, 0, 0};
   int64_t pos[CB];
   int least = INT32_MAX;
   {
@@ -770,7 +779,7 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
     int x[CB], token[CB];
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb) {
-      const int r = kSplit ? col & 7 : cb * 16 + col;
+      const int r = cb * 16 + col;
       x[cb] = tile.row0 + (r < tile.n_rows ? r : 0);
       token[cb] = tokens[x[cb] >> a.group_shift];
     }
@@ -787,7 +796,8 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
       const int b = token[cb] >> kTokenShift, j = token[cb] & ((1 << kTokenShift) - 1), h = hc * a.group + (x[cb] & (a.group - 1));
       const char* const src = a.q + b * a.qs_b + h * a.qs_h + j * a.qs_s + grp * 16;
 #pragma unroll
-      for (int kk = 0; kk < G::QV; ++kk) q[cb][kk] = *reinterpret_cast<const v4u*>(src + kk * 64);
+      for (int kk = 0; kk < QR; ++kk) q[cb][kk] = *reinterpret_cast<const v4u*>(src + kk * 64);
+      if (kTail && cb == wave) tail = *reinterpret_cast<const v4u*>(src + QR * 64);  // a block a wavefront
     }
     __builtin_amdgcn_sched_barrier(0);  // all of them are on their way before the first is waited for
   }
@@ -876,20 +886,24 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
       const int lane = lane_id(), col = lane & 15, max_context = a.max_context;
 #pragma unroll
       for (int cb = 0; cb < CB; ++cb) {
-        const int r = kSplit ? col & 7 : cb * 16 + col;
+        const int r = cb * 16 + col;
         const int64_t keys = pos[cb] < 0 ? 0 : pos[cb] >= max_context ? max_context : pos[cb] + 1;
         const int lim = r < tile.n_rows ? static_cast<int>(keys) : INT32_MAX;
         least = min(least, lim);
         if (lane < 16) sh.limit[wave][cb * 16 + col] = lim;
       }
       least = -fp::wave_max(-least);
+      if constexpr (kTail) {
+        sh.q_tail[wave * 64 + lane] = tail;
+        lds_barrier();
+      }
     }
     // The query rows are waited for here.  At their first use, inside the loop over the stages, the wait would be one of every stage, and
     // for the stages on their way, too, of which the compiler does not know.
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
-      for (int kk = 0; kk < G::QV; ++kk) asm volatile("" : "+v"(q[cb][kk]));
+      for (int kk = 0; kk < QR; ++kk) asm volatile("" : "+v"(q[cb][kk]));
 #pragma nounroll
     for (int s = wave, buf = 0; s < n_stages; s += kWaves, buf ^= 1) {
       const int c0 = seg0 + s * G::TS;
@@ -918,7 +932,8 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
 #pragma unroll
           for (int cb = 0; cb < CB; ++cb) {
             if constexpr (G::k16) {
-              sc[cb][blk] = E::mfma_k32(ka, q[cb][kk], sc[cb][blk]);
+              const v4u qb = kk < QR ? q[cb][kk < QR ? kk : 0] : sh.q_tail[cb * 64 + lane_now];
+              sc[cb][blk] = E::mfma_k32(ka, qb, sc[cb][blk]);
             } else {
 #pragma unroll
               for (int e = 0; e < 4; ++e)
@@ -963,9 +978,9 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
         }
         asm volatile("" : : : "memory");  // a wavefront's LDS instructions are executed in order
       }
-      // The first V operands leave LDS while the exponentials are worked out.
+      // The first V operands leave LDS while the exponentials are worked out, where there are registers for them.
       constexpr int kReadsV = G::k16 ? G::NB * G::DB : G::NB * 4 * (D / 64);  // reads of a stage
-      constexpr int kAheadV = CB == 4 ? 4 : 8 < kReadsV ? 8 : kReadsV;
+      constexpr int kAheadV = CB == 4 ? 2 : 8 < kReadsV ? 8 : kReadsV;
       const auto read_v = [&](int n) {
         if constexpr (G::k16) {
           // lanes 4 j + c of a 16-lane block name elements 4 c .. of key 4 * grp + j and receive element `col` of the four keys
@@ -977,8 +992,11 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
         }
       };
       decltype(read_v(0)) v_ahead[kAheadV];
+      const auto first_v = [&] {
 #pragma unroll
-      for (int n = 0; n < kAheadV; ++n) v_ahead[n] = read_v(n);
+        for (int n = 0; n < kAheadV; ++n) v_ahead[n] = read_v(n);
+      };
+      if constexpr (CB < 4) first_v();
       // Reference point of the exponentials, per column: moves only when the column's maximum has outgrown it by kMaxSlack, so most
       // stages need no exchange between the lanes of a column and no rescale.
       float cand[CB];
@@ -1017,29 +1035,25 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
             l[cb] += sc[cb][blk][j];
           }
       }
+      if constexpr (CB == 4) first_v();
       if constexpr (G::k16) {
 #pragma unroll
         for (int blk = 0; blk < G::NB; ++blk) {
-          s16x4 pb[CB];
+          // 16 keys and the same 16 again: the probabilities are the sum of two parts of 16 bits, of which one product takes both
+          v4u pb[CB];
 #pragma unroll
           for (int cb = 0; cb < CB; ++cb) {
-            uint32_t w[2];
+            uint32_t hi[2], lo[2];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const float p0 = sc[cb][blk][2 * j], p1 = sc[cb][blk][2 * j + 1];
-              w[j] = E::pack2(E::above_zero(p0), E::above_zero(p1));
-              if constexpr (kSplit) {
-                const uint32_t rest = E::pack2(p0 - E::to_float(w[j] & 0xffffu), p1 - E::to_float(w[j] >> 16));
-                if ((lane_now & 15) >= 8) w[j] = rest;
-              }
-            }
-            pb[cb] = __builtin_bit_cast(s16x4, uint2{w[0], w[1]});
+            for (int j = 0; j < 2; ++j) E::split(sc[cb][blk][2 * j], sc[cb][blk][2 * j + 1], hi[j], lo[j]);
+            pb[cb] = v4u{hi[0], hi[1], lo[0], lo[1]};
           }
 #pragma unroll
           for (int db = 0; db < G::DB; ++db) {
-            const s16x4 va = v_ahead[(blk * G::DB + db) % kAheadV];
+            const uint2 half = __builtin_bit_cast(uint2, v_ahead[(blk * G::DB + db) % kAheadV]);
+            const v4u va = {half.x, half.y, half.x, half.y};
 #pragma unroll
-            for (int cb = 0; cb < CB; ++cb) o[cb][db] = E::mfma_k16(va, pb[cb], o[cb][db]);
+            for (int cb = 0; cb < CB; ++cb) o[cb][db] = E::mfma_k32(va, pb[cb], o[cb][db]);
             if (blk * G::DB + db + kAheadV < G::NB * G::DB) v_ahead[(blk * G::DB + db) % kAheadV] = read_v(blk * G::DB + db + kAheadV);
             __builtin_amdgcn_sched_barrier(0);
           }
@@ -1072,17 +1086,6 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
   // at a time, chunks permuted against bank conflicts.
 #pragma unroll
   for (int cb = 0; cb < CB; ++cb) {
-    if constexpr (kSplit) {
-      // both halves of the columns together.  Against an infinite V element what rounding left over is 0 or negative, and the sum would
-      // be NaN: the upper half stands.
-#pragma unroll
-      for (int db = 0; db < G::DB; ++db)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float rest = fp_decode::dpp<0x128>(o[cb][db][j]);  // row_ror:8, lane ^ 8
-          if ((__float_as_uint(o[cb][db][j]) & 0x7f800000u) != 0x7f800000u) o[cb][db][j] += rest;
-        }
-    }
     l[cb] += __shfl_xor(l[cb], 16);
     l[cb] += __shfl_xor(l[cb], 32);
     if (grp == 0) *reinterpret_cast<float2*>(sh.ml[wave][cb * 16 + col]) = float2{m[cb], l[cb]};
@@ -1166,7 +1169,7 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
         const float lse = (ml[k].x + log2f(ml[k].y)) * kLn2;
         f32x4 res;
 #pragma unroll
-        for (int n = 0; n < 4; ++n) res[n] = any ? fp_decode::sink_gate<E>(num[k][n] / ml[k].y, lse, e.sinks, h) : 0.f;
+        for (int n = 0; n < 4; ++n) res[n] = any ? gated(num[k][n] / ml[k].y, lse, e.sinks, h) : 0.f;
         store4<E>(e.out + b * e.os_b + h * e.os_h + j * e.os_s + c * 4 * E::kBytes, res);
         if (c == 0) e.lse[(static_cast<int64_t>(b) * e.Hq + h) * e.S + j] = any ? lse : -INFINITY;
       }
@@ -1222,14 +1225,12 @@ __global__ __launch_bounds__(kThreads, (sizeof(Shared<E, D>) <= 80 * 1024 ? 2 : 
     if (to > from) {
     if (busy) lds_barrier();  // the piece before has left LDS
     busy = true;
-    if (Geo<E, D>::k16 && t.n_rows <= 8)
-      run_piece<E, D, 1, Geo<E, D>::k16>(a, sh, wave, t, piece, t0, t1);
-    else if (t.n_rows <= 16)
-      run_piece<E, D, 1, false>(a, sh, wave, t, piece, t0, t1);
+    if (t.n_rows <= 16)
+      run_piece<E, D, 1>(a, sh, wave, t, piece, t0, t1);
     else if (t.n_rows <= 32)
-      run_piece<E, D, 2, false>(a, sh, wave, t, piece, t0, t1);
+      run_piece<E, D, 2>(a, sh, wave, t, piece, t0, t1);
     else
-      run_piece<E, D, 4, false>(a, sh, wave, t, piece, t0, t1);
+      run_piece<E, D, 4>(a, sh, wave, t, piece, t0, t1);
     }
     i = t.next;
     if (left <= 0 || i >= h.n_tiles) break;
@@ -1320,7 +1321,7 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(const SharedArgs 
     }
     lse = (m + log2f(den)) * kLn2;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) res[k] = fp_decode::sink_gate<E>(num[k] / den, lse, a.sinks, h);
+    for (int k = 0; k < 4; ++k) res[k] = gated(num[k] / den, lse, a.sinks, h);
   }
   store4<E>(a.out + b * a.os_b + h * a.os_h + j * a.os_s + c * 4 * E::kBytes, res);
   if (c == 0) a.lse[(static_cast<int64_t>(b) * a.Hq + h) * a.S + j] = lse;

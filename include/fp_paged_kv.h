@@ -602,7 +602,8 @@ int fp_copy_pages(void* pool, const int64_t* src, const int64_t* dst, const int3
  *              0 .. (smallest of their prefix_lens) - 1, be it in the same pages or in copies of them.  An id <= 0 shares with nobody
  *   out        [B, Hq, S, D], element strides (b, h, s); lse [B, Hq, S] float32 contiguous
  *   sinks, scale, page_table, batch_idx, pool_k, pool_v, n_slots  as fp_paged_decode
- * Results are those of fp_paged_decode for each token, up to the order of the sums; with a false prefix_ids they are not: a shared key
+ * Results are those of fp_paged_decode for each token, up to the order of the sums and, behind a sink gate, one rounding instead of
+ * two; with a false prefix_ids they are not: a shared key
  * is read through the table row of any of the sequences.
  *
  * fp_shared_decode_plan, once per step, finds the sequences that share and cuts the work; every layer's fp_paged_decode_shared with the

@@ -74,9 +74,10 @@ class SharedBatch:
 
         With u half a step of the type, n keys and c = scale * sum |q k| (natural units):
         a score is off by at most d = (D + 2) 2^-24 c (sums and the scale in fp32), its exponential by that, by the rounding of
-        its argument (2^-23 of it, at most c * 2^-22) and 2^-22 of its own; the probabilities are rounded once to 16 bits (u), and
-        sums over n keys, in parts that are joined, are off by (n + 64) 2^-24 of the sum of magnitudes.  The result is rounded
-        once, with a sink gate twice."""
+        its argument (2^-23 of it, at most c * 2^-22) and 2^-22 of its own; the probabilities of the 16-bit types are sums of two
+        numbers of the type, the second below 2u of the first and rounded by u of itself, so off by 2 u^2 (and in f16 by at
+        most 2^-31 of the largest, where a part would vanish); sums over n keys, in parts that are joined, are off by
+        (n + 64) 2^-24 of the sum of magnitudes.  The result is rounded once, also behind a sink gate."""
         u, scale = HALF_STEP[self.dtype], self.D ** -0.5 if scale is None else scale
         G = self.Hq // self.Hc
         pos = self.pos if pos is None else pos
@@ -102,12 +103,12 @@ class SharedBatch:
                     d = (self.D + 2) * 2.0 ** -24 * c + 2 * c * 2.0 ** -22 + 2.0 ** -21
                     sums = (n + 64) * 2.0 ** -24
                     mag = w @ np.abs(vv) / den
-                    rounding = u if self.dtype != torch.float32 else 0.0
+                    rounding = 0.0 if self.dtype == torch.float32 else 2 * u * u + (n * 2.0 ** -31 / den if self.dtype == torch.float16 else 0.0)
                     o_tol[b, h, j] = mag * (2 * d + 2 * sums + rounding) * 1.01 + u * np.abs(out[b, h, j]) + 1e-30
                     l_tol[b, h, j] = d + sums + 2.0 ** -22 * (1 + abs(lse[b, h, j]))
         if sinks is not None:
             gate = 1.0 / (1.0 + np.exp(sinks.double().numpy()[None, :, None] - lse))
-            o_tol = o_tol * gate[..., None] + np.abs(out) * gate[..., None] * (2 * u + l_tol[..., None] + 2.0 ** -21)
+            o_tol = (o_tol - u * np.abs(out)) * gate[..., None] + u * np.abs(out) * gate[..., None] + np.abs(out) * gate[..., None] * (l_tol[..., None] + 2.0 ** -21)
             out = out * gate[..., None]
         if self.dtype == torch.float16:
             o_tol = o_tol + 2.0 ** -24  # results below the normal numbers
