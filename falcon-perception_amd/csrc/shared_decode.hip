@@ -1419,8 +1419,8 @@ extern "C" int fp_paged_decode_shared(const void* q, int64_t q_stride_b, int64_t
       q_stride_b * e % 16 || q_stride_h * e % 16 || q_stride_s * e % 16 || out_stride_b * e % 16 || out_stride_h * e % 16 ||
       out_stride_s * e % 16)
     return fp::fail(FP_ERR_INVALID_ARGUMENT, "%s: rows of q, out and the pools must be 16-byte aligned", what);
-  if (plan_bytes < fp_shared_decode_plan_bytes(B, S, Hq, Hc, D))
-    return fp::fail(FP_ERR_WORKSPACE, "%s: plan of %lld bytes is too small", what, static_cast<long long>(plan_bytes));
+  if (plan_bytes < fp_shared_decode_plan_bytes(B, S, Hq, Hc, D) || !fp::aligned(plan, 16))
+    return fp::fail(FP_ERR_WORKSPACE, "%s: plan of %lld bytes is too small, or not 16-byte aligned", what, static_cast<long long>(plan_bytes));
   const int64_t need = fp_shared_decode_workspace_bytes(B, S, Hq, Hc, D);
   if (!workspace || workspace_bytes < need || !fp::aligned(workspace, 16))
     return fp::fail(FP_ERR_WORKSPACE, "%s: workspace of %lld bytes, 16-byte aligned, is needed (got %lld)", what,

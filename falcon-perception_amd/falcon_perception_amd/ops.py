@@ -727,13 +727,15 @@ def paged_decode_shared(q: Tensor, pool_k: Tensor, pool_v: Tensor, page_table: T
     if prefix_ids.shape[0] != page_table.shape[0]:
         raise RuntimeError(f"{what}: prefix_ids and prefix_lens need one entry per row of page_table ({page_table.shape[0]})")
     q = _rows(q)
+    if q.data_ptr() % 16 or any(s * q.element_size() % 16 for s in q.stride()[:3]):
+        q = q.contiguous()  # the kernel loads 16 bytes at once
     shape = dict(q_heads=Hq, cached_heads=Hc, head_dim=D)
     with _on(device):
         if plan is None:
             plan = shared_decode_plan(batch_idx, input_pos, prefix_ids, prefix_lens, max_context=max_context, **shape)
         workspace = _byte_buffer(what, "workspace", workspace, shared_decode_workspace_bytes(B, S, **shape), device)
         if out is None:
-            out = torch.empty_like(q)
+            out = torch.empty(q.shape, dtype=q.dtype, device=device)
         elif out.shape != q.shape or out.dtype != q.dtype or out.stride(3) != 1:
             raise RuntimeError(f"{what}: out must be like q, with dense rows")
         if lse is None:

@@ -307,3 +307,71 @@ def test_tokens_in_any_places():
     case.on()
     case.check(case.call(ops))
     case.check(case.call(ops, pos=case.pos_d.long()))
+
+
+def test_far_pages():
+    """Pages behind 2^32 bytes of a plane, and rows whose number passes 2^24."""
+    P, D, n_pages = 128, 128, 150_000
+    case = SharedBatch(33, [300], one_each([0, 0, -1], [20, 90, 400]), Hq=4, Hc=1, D=D, P=P, dtype=BF16)
+    pool = torch.empty(2, 1, n_pages * P, D, dtype=BF16, device="cuda")
+    shift = n_pages - case.n_pages
+    pool[:, :, shift * P:] = case.pool.cuda()
+    pool[:, :, :P] = float("nan")
+    case.on()
+    case.pool_d = pool
+    case.table_d[case.table_d > 0] += shift
+    case.check(case.call(ops))
+    src, dst, rows = (torch.tensor([v], device="cuda") for v in (n_pages - 1, n_pages - 2, 100))
+    ops.copy_pages(pool, src, dst, rows.int(), P)
+    a, b = pool[:, :, (n_pages - 2) * P:(n_pages - 2) * P + 100], pool[:, :, (n_pages - 1) * P:(n_pages - 1) * P + 100]
+    assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+def test_a_query_that_is_not_finite(value):
+    """It spoils its own row only."""
+    case = SharedBatch(34, [200], one_each([0] * 40, [1 + i for i in range(40)]), Hq=4, Hc=2, D=128, P=64, dtype=BF16).on()
+    want = case.call(ops)
+    case.q_d[7, 1] = value
+    got = case.call(ops)
+    keep = torch.ones(40, 4, dtype=torch.bool, device="cuda")
+    keep[7, 1] = False
+    assert torch.equal(got[0].squeeze(2)[keep], want[0].squeeze(2)[keep]) and torch.equal(got[1].squeeze(2)[keep], want[1].squeeze(2)[keep])
+    assert got[0][7, 1].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_an_infinite_value_that_all_rows_see(dtype):
+    """Infinity, whatever the weight of its key: the first is far below the largest."""
+    case = SharedBatch(35, [150], one_each([0] * 20, [1 + i for i in range(20)]), Hq=4, Hc=1, D=64, P=32, dtype=dtype)
+    k = case.keys[0][0]
+    far = int((k[0, :128].double() @ case.q[0, 0, 0].double()).argmin())  # in a page that all of them map
+    page = int(case.table[case.batch_idx[0], far // 32])
+    case.pool[1][0, page * 32 + far % 32, 3] = float("inf")
+    case.pool[1][0, page * 32 + far % 32, 4] = float("-inf")
+    assert (case.table[case.batch_idx, far // 32] == page).all()
+    case.q *= 3  # weights down to e^-20 and below
+    case.on()
+    want = torch.tensor([float("inf"), float("-inf")], dtype=dtype, device="cuda")
+    out = case.call(ops)[0]
+    assert (out[..., 3:5] == want).all()
+    assert out[..., [0, 1, 2, 5]].isfinite().all()
+
+
+def test_the_same_slot_twice():
+    case = SharedBatch(36, [200], one_each([0, 0, -1], [30, 9, 50]), Hq=4, Hc=2, D=128, P=64, dtype=BF16).on()
+    want = case.call(ops)
+    order = [2, 0, 1, 0, 2]
+    case.q_d, case.batch_idx_d = case.q_d[order], case.batch_idx_d[order]
+    got = case.call(ops, pos=case.pos_d[order])
+    assert torch.equal(got[1], want[1][order]) or torch.allclose(got[1], want[1][order], atol=2e-6)
+    assert torch.equal(got[0][1], got[0][3]) and torch.equal(got[0][0], got[0][4])
+
+
+def test_rows_that_are_not_aligned():
+    case = SharedBatch(37, [90], one_each([0, 0], [20, 90]), Hq=4, Hc=2, D=64, P=32, dtype=BF16).on()
+    want = case.call(ops)
+    wide = torch.zeros(2, 4, 1, 67, dtype=BF16, device="cuda")
+    wide[..., 3:] = case.q_d
+    got = case.call(ops, q=wide[..., 3:])
+    assert torch.equal(got[0], want[0])

@@ -262,3 +262,50 @@ def test_copy_pages_refusals():
                         ((pool.double(), one, one, rows, 16), "unsupported KV dtype")]:
         with pytest.raises(RuntimeError, match=match):
             ops.copy_pages(*args)
+
+
+def test_steps_and_copies_from_a_graph():
+    """Captured once, replayed over lengths that change: every replay is what the eager call makes of them."""
+    P, slots = 16, [3, 1, 4, 7]
+    dev = lambda x, t: torch.tensor(x, dtype=t, device="cuda")
+    table = torch.full((9, 12), -1, dtype=torch.int64, device="cuda")
+    table[0] = 0
+    table[5, :4] = dev([40, 41, 42, 43], torch.int64)
+    free, count = dev(list(range(1, 30)), torch.int64), dev([29], torch.int32)
+    pool = torch.randn(2, 2, 50 * P, 64, device="cuda")
+    old, new, parents = dev([0, 0, 37, 50], torch.int32), dev([0, 0, 0, 0], torch.int32), dev([0, 0, 5, 5], torch.int64)
+    ids = dev(slots, torch.int64)
+
+    def step(table, pool):
+        made = ops.step_tables(ids, old, new, free, count, table, P, 200, parents=parents, row_multiple=8)
+        ops.copy_pages(pool, made.copy_src, made.copy_dst, made.copy_rows, P)
+        return made
+
+    new.copy_(dev([5, 30, 40, 50], torch.int32))
+    step(table.clone(), pool.clone())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        made = step(table, pool)
+    for lens in ([5, 30, 40, 50], [1, 1, 37, 90], [100, 0, 80, 51], [300, 0, 80, 51], [0, 0, 37, 50]):
+        new.copy_(dev(lens, torch.int32))
+        before = table.clone(), pool.clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step(*before)
+        for a, b in zip(made, want):
+            assert torch.equal(a, b)
+        assert torch.equal(table, before[0]) and torch.equal(pool, before[1])
+        assert bool(made.status) == (lens[0] == 300)
+
+
+def test_under_inference_mode():
+    case = make(11, 20, old_hi=400, add_hi=70, P=32, forks=8, parents=3)
+    with torch.inference_mode():
+        check(case, 32, 3000)
+        t, made = run(case, 32, 3000)
+        assert made.batch_idx.is_inference() and made.free_left.is_inference()
+    t, made = run(case, 32, 3000)
+    assert not made.batch_idx.is_inference()
+    made.batch_idx[0] = 5  # an ordinary tensor
+    assert made.batch_idx._version == 1 or made.batch_idx.requires_grad is False
