@@ -4,7 +4,7 @@
 //
 // HBM-bound: every byte is read once and written once.  A workgroup copies one entry's rows of one plane, which are
 // contiguous on both sides, 16 bytes a lane and 32 KB on their way at once; the stores go past the caches, which the sources of
-// several forks are read from.  24 pages through 28 layers of 16 heads, D 128, bf16 (679 MB read and written): 117 us, 5.8 TB/s, where a
+// several forks are read from.  24 pages through 28 layers of 16 heads, D 128, bf16 (678 MB read and written): 116 us, 5.8 TB/s, where a
 // large copy reaches 5.2 on this GPU; with plain stores 143, one chunk at a time 138, with non-temporal loads as well 148.
 #include "fp_common.h"
 

@@ -15,9 +15,18 @@
 //      S^T = K Q^T    keys are the M rows of the matrix product and queries its columns, so a lane has the scores of
 //                     one query and a K operand read from LDS serves up to four blocks of 16 columns
 //      O^T += V^T P^T  P^T is in the B operand's layout as the scores leave the first product; V^T comes out of LDS
-//                     through the transpose read (fp32: by reading four neighbours of a row for four blocks of O^T)
+//                     through the transpose read (fp32: by reading four neighbours of a row for four blocks of O^T).
+//                     Of 16-bit types a probability is the sum of two numbers of the type, which one product of depth 32
+//                     takes against 16 keys twice: rounded once to 16 bits they cost f16 most of its precision
 //    The states of the four wavefronts meet in LDS at the end of a piece.
 //  * Join: a row's pieces, by their maxima and sums, in 32 bits.
+//
+// Bound by HBM where the keys are many.  64 sequences, most on one of 9 prefixes, 16 query heads on 8 cached ones, D 128, bf16, 473 MB a
+// layer: products 81.5 us (5.8 TB/s; a large copy reaches 5.2 on this GPU), join 4.9, plan 12.6 once a step; fp_paged_decode, which
+// reads a prefix once a sequence, takes 141.  192 sequences on 8 prefixes of up to 12288 keys, 4 query heads a cached one, 2.0 GB a layer:
+// 330 us, 6.0 TB/s (1153 once a sequence).  Small batches are bound by the trips to memory in front of the first key and by two
+// launches (3 sequences, 1.5 MB: 8.5 and 3.6 us), many tokens a sequence by LDS and the instructions between the matrix products
+// (40 sequences of 24 tokens, 11.6 GFLOP: 46 us).
 #include "decode_common.h"
 
 #include <math.h>
@@ -265,7 +274,8 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   __syncthreads();
   for (int b = tid; b < a.B; b += n_thr) {
     // Whole units: what is behind them counts as each one's own, up to 63 keys that are read once a sequence.  Own keys then begin
-    // with a stage that lies in one page; from anywhere else they would be staged row by row (64 sequences on 9 pictures: %s us a layer).
+    // with a stage that lies in one page; from anywhere else they would be staged row by row (64 sequences on 9 pictures: 86 us a
+    // layer instead of 82).
     const int lead = s_lead[b], shared = s_members[lead] >= 2 ? min(s_shortest[lead], s_longest[lead]) / kUnit * kUnit : 0;
     const bool shares = s_tok[b] > 0 && s_id[b] > 0 && shared > 0;
     s_shared[b] = shares ? shared : 0;
@@ -1223,14 +1233,14 @@ __global__ __launch_bounds__(kThreads, (sizeof(Shared<E, D>) <= 80 * 1024 ? 2 : 
     left -= t.lead + all - offset;
     offset = 0;
     if (to > from) {
-    if (busy) lds_barrier();  // the piece before has left LDS
-    busy = true;
-    if (t.n_rows <= 16)
-      run_piece<E, D, 1>(a, sh, wave, t, piece, t0, t1);
-    else if (t.n_rows <= 32)
-      run_piece<E, D, 2>(a, sh, wave, t, piece, t0, t1);
-    else
-      run_piece<E, D, 4>(a, sh, wave, t, piece, t0, t1);
+      if (busy) lds_barrier();  // the piece before has left LDS
+      busy = true;
+      if (t.n_rows <= 16)
+        run_piece<E, D, 1>(a, sh, wave, t, piece, t0, t1);
+      else if (t.n_rows <= 32)
+        run_piece<E, D, 2>(a, sh, wave, t, piece, t0, t1);
+      else
+        run_piece<E, D, 4>(a, sh, wave, t, piece, t0, t1);
     }
     i = t.next;
     if (left <= 0 || i >= h.n_tiles) break;

@@ -9,7 +9,9 @@
 //
 // Bound by latency for a decode step (one launch: load, scan, store) and by the stores of the rows (20 bytes each) for an
 // admission step.  One launch: every workgroup works out the sums of all requests by itself - 20 bytes a request, from L2 -
-// instead of waiting for a launch that does; nothing that one workgroup writes is read by another.
+// instead of waiting for a launch that does; nothing that one workgroup writes is read by another.  64 requests of one token: 6.0 us;
+// 48 forks, 16 thousand rows: 7.0; 1000 requests, 2 million rows, 41 MB: 20.2, about 8
+// of them before the first row.
 #include "fp_common.h"
 
 namespace {
@@ -18,6 +20,7 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kMaxRequests = 4096;
 constexpr int kMaxSlots = 1 << 17;
+constexpr int64_t kLdsBytes = 160 * 1024;  // of a CU
 typedef int64_t v2l __attribute__((ext_vector_type(2)));
 typedef int v4i __attribute__((ext_vector_type(4)));
 
@@ -254,13 +257,13 @@ __global__ __launch_bounds__(kThreads) void step_tables_kernel(const TablesArgs 
     bool stored = false;
     if constexpr (kRows == 4) {
       if (a.wide && row0 + 4 <= a.max_rows) {
-      v2l* const to_slot = reinterpret_cast<v2l*>(a.batch_idx + row0);
-      v2l* const to_where = reinterpret_cast<v2l*>(a.slot_map + row0);
-      to_slot[0] = v2l{slot[0], slot[1]};
-      to_slot[1] = v2l{slot[2], slot[3]};
-      to_where[0] = v2l{where[0], where[1]};
-      to_where[1] = v2l{where[2], where[3]};
-      *reinterpret_cast<v4i*>(a.input_pos + row0) = v4i{pos[0], pos[1], pos[2], pos[3]};
+        v2l* const to_slot = reinterpret_cast<v2l*>(a.batch_idx + row0);
+        v2l* const to_where = reinterpret_cast<v2l*>(a.slot_map + row0);
+        __builtin_nontemporal_store(v2l{slot[0], slot[1]}, to_slot);
+        __builtin_nontemporal_store(v2l{slot[2], slot[3]}, to_slot + 1);
+        __builtin_nontemporal_store(v2l{where[0], where[1]}, to_where);
+        __builtin_nontemporal_store(v2l{where[2], where[3]}, to_where + 1);
+        __builtin_nontemporal_store(v4i{pos[0], pos[1], pos[2], pos[3]}, reinterpret_cast<v4i*>(a.input_pos + row0));
         stored = true;
       }
     }
@@ -304,14 +307,15 @@ extern "C" int fp_step_tables(const int64_t* slots, const void* old_lens, const 
                      copy_dst, copy_rows, status, B, max_rows, row_multiple, n_pages, max_batch, n_free,
                      fp::aligned(batch_idx, 16) && fp::aligned(input_pos, 16) && fp::aligned(slot_map, 16), fp::PageDiv(page_size)};
   // A row a thread while that many threads run at once: a decode step's rows belong to as many requests, whose numbers four rows of one
-  // thread would fetch one after the other (64 requests 5.4 us, 7.8 with four).  Beyond, four: one request and one page, mostly, and
-  // stores of 16 bytes (2 million rows @@).
-  const int64_t most = 2ll * fp::compute_units();  // workgroups; each of them reads all requests
-  const bool few = max_rows <= most * kThreads;
+  // thread would fetch one after the other (64 requests: 5.9 us, 7.8 with four).  Beyond, four: mostly one request and one page, and
+  // stores of 16 bytes past the caches (1000 requests, 2 million rows, 41 MB: a row a thread 35 us, four 22.6, stores past the caches
+  // 21.5, three workgroups a CU 20.3).  Every workgroup reads all requests, so there are no more of them than run at once.
+  const size_t lds = (2 * static_cast<size_t>(B) + 1 + (max_batch + 31) / 32 + 3) / 4 * 16 + B * sizeof(Record);
+  const bool few = max_rows <= 2ll * fp::compute_units() * kThreads;
+  const int64_t fit = kLdsBytes / (lds + 1024), a_cu = few ? 2 : fit < 1 ? 1 : fit > 3 ? 3 : fit, most = a_cu * fp::compute_units();
   const int64_t turns = few ? max_rows : (max_rows + 3) / 4, work = turns > 64ll * B ? turns : 64ll * B;
   int64_t grid = (work + kThreads - 1) / kThreads;
   grid = grid < 1 ? 1 : grid > most ? most : grid;
-  const size_t lds = (2 * static_cast<size_t>(B) + 1 + (max_batch + 31) / 32 + 3) / 4 * 16 + B * sizeof(Record);
   const auto go = [&](auto kernel) {
     if (lds > 64 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
                                                static_cast<int>(lds)) != hipSuccess)

@@ -98,6 +98,11 @@ def test_the_most_requests():
     check(make(3, 4096, old_hi=40, add_hi=5, P=16, forks=2000, parents=50, max_batch=9000), 16, 30000)
 
 
+def test_the_most_requests_and_slots_and_many_rows():
+    """A workgroup a CU, several turns of four rows a thread."""
+    check(make(7, 4096, old_hi=60, add_hi=160, P=64, forks=900, parents=50, max_batch=1 << 17), 64, 400001)
+
+
 def test_no_requests_and_no_rows():
     slots, old, new, par, free, count, table = make(4, 3, old_hi=40, add_hi=0, P=16)
     check((slots, old, old, par, free, count, table), 16, 0)
