@@ -1,5 +1,5 @@
-// The calls an eager layer or step makes (append, decode step, prefill attention, tables and attention of shared prefixes) from PyTorch tensors to the C ABI of
-// include/fp_paged_kv.h, as a Python module.
+// The calls an eager layer or step makes (append, decode step, prefill attention; tables, page copies and attention of shared
+// prefixes) from PyTorch tensors to the C ABI of include/fp_paged_kv.h, as a Python module.
 //
 // Bound by the host: a layer of a small eager step is shorter on the GPU than its calls are in Python, where every pointer, size
 // and stride is an attribute look-up and the foreign call converts forty arguments one by one.  Here they are read from the tensors in C++:
@@ -52,6 +52,13 @@ bool dense_rows(const at::Tensor& t) { return t.stride(t.dim() - 1) == 1; }
 bool on_device(int64_t device, std::initializer_list<const at::Tensor*> tensors) {
   for (const at::Tensor* t : tensors)
     if (t && t->get_device() != device) return false;
+  return true;
+}
+
+// Each is a number that the C ABI takes as int32_t.
+bool fits(std::initializer_list<int64_t> sizes) {
+  for (const int64_t n : sizes)
+    if (n != static_cast<int32_t>(n)) return false;
   return true;
 }
 
@@ -263,7 +270,8 @@ PyObject* shared_plan_unguarded(PyObject* const* args) {
   const int64_t Hq = a.integer(), Hc = a.integer(), D = a.integer(), max_context = a.integer();
   const at::Tensor* plan = a.tensor();
   const int64_t device = a.integer(), stream = a.integer();
-  if (!a.ok || !is_shared_step(*bidx, *pos, *ids, *lens) || !is_bytes(*plan) || !on_device(device, {bidx, pos, ids, lens, plan}))
+  if (!a.ok || !is_shared_step(*bidx, *pos, *ids, *lens) || !is_bytes(*plan) || !on_device(device, {bidx, pos, ids, lens, plan}) ||
+      !fits({bidx->size(0), pos->size(pos->dim() - 1), Hq, Hc, D, ids->size(0), max_context}))
     Py_RETURN_NONE;
   int rc;
   {
@@ -295,7 +303,8 @@ PyObject* shared_unguarded(PyObject* const* args) {
     Py_RETURN_NONE;
   const int64_t B = q->size(0), Hq = q->size(1), S = q->size(2), D = q->size(3), Hc = pk->size(0);
   if (bidx->size(0) != B || (pos->dim() == 2 ? pos->size(1) : 1) != S || ids->size(0) != table->size(0) ||
-      (sinks && !is_vector(*sinks, at::kFloat, Hq)) || !on_device(device, {q, pk, pv, table, bidx, pos, ids, lens, sinks, plan, ws}))
+      (sinks && !is_vector(*sinks, at::kFloat, Hq)) || !fits({B, S, Hq, Hc, D, page_size, table->size(0), table->size(1), max_context}) ||
+      !on_device(device, {q, pk, pv, table, bidx, pos, ids, lens, sinks, plan, ws}))
     Py_RETURN_NONE;
   at::Tensor out, lse;
   int rc;
@@ -340,13 +349,14 @@ PyObject* tables_unguarded(PyObject* const* args) {
       !is_vector(*after, before->scalar_type(), B) || !is_vector(*pages, at::kLong, pages->size(0)) || !is_vector(*count, at::kInt, 1) ||
       !is_table(*table) || (parents && !is_vector(*parents, at::kLong, B)) ||
       (inverse && (!is_table(*inverse) || inverse->size(0) != table->size(0))) ||
+      !fits({pages->size(0), B, rows, multiple, page_size, table->size(0), table->size(1)}) ||
       !on_device(device, {slots, before, after, pages, count, table, parents, inverse}))
     Py_RETURN_NONE;
   at::Tensor made[9];
   int rc;
   {
     const Unlocked others;
-    // two allocations, the rows and the rest: nine cost as much as the launch
+    // two allocations, the rows and the rest: with nine a call is 13.6 us of the host, with two 8.1
     const auto bytes = slots->options().dtype(at::kByte);
     const int64_t wide = (rows + 3) / 4 * 4;
     const at::Tensor big = at::empty({20 * wide}, bytes), small = at::empty({16 * B + 4 * (2 * B + 3)}, bytes);
@@ -384,7 +394,8 @@ PyObject* copy_unguarded(PyObject* const* args) {
   const int64_t page_size = a.integer(), device = a.integer(), stream = a.integer();
   if (!a.ok || dtype_code(*pool) < 0 || pool->dim() < 2 || !pool->is_contiguous() || pool->numel() == 0 || src->dim() != 1 ||
       !is_vector(*src, at::kLong, src->size(0)) || !is_vector(*dst, at::kLong, src->size(0)) ||
-      !is_vector(*rows, at::kInt, src->size(0)) || page_size < 1 || !on_device(device, {pool, src, dst, rows}))
+      !is_vector(*rows, at::kInt, src->size(0)) || page_size < 1 || !fits({src->size(0), pool->size(-1), page_size}) ||
+      !on_device(device, {pool, src, dst, rows}))
     Py_RETURN_NONE;
   const int64_t D = pool->size(-1), n_slots = pool->size(-2);
   int rc;

@@ -518,9 +518,19 @@ def _vector(what: str, name: str, t: Tensor, n: int | None, *dtypes: torch.dtype
     return t.contiguous()
 
 
+def _int32(what: str, **sizes: int) -> None:
+    """What the C ABI takes as int32_t."""
+    for name, n in sizes.items():
+        if not -2 ** 31 <= n < 2 ** 31:
+            raise RuntimeError(f"{what}: {name} {n} does not fit 32 bits")
+
+
 def _page_table(what: str, page_table: Tensor) -> None:
     if page_table.dtype != torch.int64 or page_table.dim() != 2 or page_table.stride(1) != 1:
         raise RuntimeError(f"{what}: page_table must be int64 [max_batch, blocks] with a dense last axis")
+
+
+STEP_REQUESTS, STEP_SLOTS = 4096, 1 << 17  # that one `step_tables` call serves
 
 
 class StepTables(NamedTuple):
@@ -588,6 +598,7 @@ def step_tables(slots: Tensor, old_lens: Tensor, new_lens: Tensor, free_pages: T
         raise RuntimeError(f"{what}: inverse must be int64 [max_batch, pages] with a dense last axis")
     if max_rows < 0 or row_multiple < 1:
         raise RuntimeError(f"{what}: max_rows {max_rows}, row_multiple {row_multiple}")
+    _int32(what, max_rows=max_rows, row_multiple=row_multiple, page_size=page_size, free_pages=free_pages.shape[0], requests=B)
     with _on(device):
         long = lambda n: torch.empty(n, dtype=torch.int64, device=device)
         whole = lambda n: torch.empty(n, dtype=torch.int32, device=device)
@@ -623,6 +634,7 @@ def copy_pages(pool: Tensor, src: Tensor, dst: Tensor, rows: Tensor, page_size: 
     dst = _vector(what, "dst", dst, n, torch.int64)
     rows = _vector(what, "rows", rows, n, torch.int32)
     n_slots, D = pool.shape[-2:]
+    _int32(what, entries=n, page_size=page_size, head_dim=D)
     if pool.numel() == 0:
         return
     with _on(device):
@@ -634,6 +646,7 @@ def copy_pages(pool: Tensor, src: Tensor, dst: Tensor, rows: Tensor, page_size: 
 
 def shared_decode_plan_bytes(B: int, S: int, *, q_heads: int, cached_heads: int, head_dim: int) -> int:
     """Bytes of the plan of a `paged_decode_shared` step of this shape."""
+    _int32("fp_shared_decode_plan_bytes", B=B, S=S, q_heads=q_heads, cached_heads=cached_heads, head_dim=head_dim)
     n = int(N.lib().fp_shared_decode_plan_bytes(B, S, q_heads, cached_heads, head_dim))
     N.check(n, "fp_shared_decode_plan_bytes")
     return n
@@ -641,6 +654,7 @@ def shared_decode_plan_bytes(B: int, S: int, *, q_heads: int, cached_heads: int,
 
 def shared_decode_workspace_bytes(B: int, S: int, *, q_heads: int, cached_heads: int, head_dim: int) -> int:
     """Bytes of workspace that `paged_decode_shared` needs for this shape, whatever the lengths are."""
+    _int32("fp_shared_decode_workspace_bytes", B=B, S=S, q_heads=q_heads, cached_heads=cached_heads, head_dim=head_dim)
     n = int(N.lib().fp_shared_decode_workspace_bytes(B, S, q_heads, cached_heads, head_dim))
     N.check(n, "fp_shared_decode_workspace_bytes")
     return n
@@ -676,6 +690,7 @@ def shared_decode_plan(batch_idx: Tensor, input_pos: Tensor, prefix_ids: Tensor,
     device = _same_device(what, batch_idx, input_pos, prefix_ids, prefix_lens, plan)
     batch_idx, input_pos, prefix_ids, prefix_lens, S = _shared_step(what, batch_idx, input_pos, prefix_ids, prefix_lens)
     B, shape = batch_idx.shape[0], dict(q_heads=q_heads, cached_heads=cached_heads, head_dim=head_dim)
+    _int32(what, max_context=max_context, slots=prefix_ids.shape[0])
     with _on(device):
         plan = _byte_buffer(what, "plan", plan, shared_decode_plan_bytes(B, S, **shape), device)
         rc = N.lib().fp_shared_decode_plan(
@@ -730,6 +745,7 @@ def paged_decode_shared(q: Tensor, pool_k: Tensor, pool_v: Tensor, page_table: T
     if q.data_ptr() % 16 or any(s * q.element_size() % 16 for s in q.stride()[:3]):
         q = q.contiguous()  # the kernel loads 16 bytes at once
     shape = dict(q_heads=Hq, cached_heads=Hc, head_dim=D)
+    _int32(what, page_size=page_size, max_context=max_context)
     with _on(device):
         if plan is None:
             plan = shared_decode_plan(batch_idx, input_pos, prefix_ids, prefix_lens, max_context=max_context, **shape)

@@ -382,6 +382,9 @@ class PagedKVCache(KVCacheBase):
             raise RuntimeError(f"Cannot fork {count} sequences. Only {len(self.free_batch_idx)} slots available.")
         if count < 1:
             return []
+        self._check_step(count)
+        if self._kv.shape[-1] * self._kv.element_size() % 16:
+            raise RuntimeError(f"Pages of {self._kv.shape[-1]} elements of {self._kv.dtype} a row cannot be copied.")
         self.flush()
         whole = n_tokens // self.page_size
         tail = n_tokens > whole * self.page_size
@@ -418,6 +421,11 @@ class PagedKVCache(KVCacheBase):
             self.prefix_lens[values[0]] = values[2].int()
         return slots
 
+    def _check_step(self, B: int) -> None:
+        if B > ops.STEP_REQUESTS or self.max_batch_size > ops.STEP_SLOTS:
+            raise RuntimeError(f"A step is of at most {ops.STEP_REQUESTS} sequences in a cache of at most {ops.STEP_SLOTS} (got {B} and "
+                               f"{self.max_batch_size}).")
+
     def _step(self, slots, old_lens, new_lens, parents, row_multiple) -> "ops.StepTables":
         ops.N.require_cuda(self.page_table)
         P, B = self.page_size, len(slots)
@@ -429,6 +437,10 @@ class PagedKVCache(KVCacheBase):
             raise ValueError("a step cannot make a sequence shorter")
         if row_multiple < 1:
             raise ValueError("row_multiple must be at least 1")
+        self._check_step(B)
+        rows = sum(-(-(n - o) // row_multiple) * row_multiple for o, n in zip(old_lens, new_lens))
+        if max(rows, row_multiple) >= 2 ** 31:
+            raise ValueError(f"a step of {rows} rows, in multiples of {row_multiple}, does not fit 31 bits")
         grow = [max(0, _cdiv(n, P) - len(self.page_table_cpu[s])) for s, n in zip(slots, new_lens)]
         if sum(grow) > self.num_free_pages:
             raise RuntimeError(f"Cannot reserve {sum(grow)} pages for a step of {B} sequences. Only {self.num_free_pages} pages available.")
@@ -449,7 +461,6 @@ class PagedKVCache(KVCacheBase):
             pages = self.page_table_cpu[s][have:_cdiv(n, P)] + pages
         packed = torch.tensor([*slots, *old_lens, *new_lens, *parents, *pages, len(pages)], dtype=torch.int64, device=self.device)
         ids, old, new, par = (packed[i * B:(i + 1) * B] for i in range(4))
-        rows = sum(-(-(n - o) // row_multiple) * row_multiple for o, n in zip(old_lens, new_lens))
         return ops.step_tables(ids, old, new, packed[4 * B:-1], packed[-1:].view(torch.int32)[:1], self.page_table, P, rows,
                                parents=par, row_multiple=row_multiple, inverse=self.physical_to_logical)
 

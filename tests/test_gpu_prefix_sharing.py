@@ -218,6 +218,32 @@ def test_refusals_change_nothing():
     s.check_pool()
 
 
+def test_steps_that_one_launch_does_not_serve_change_nothing():
+    s = Server(n_pages=20, slots=4200, max_blocks_per_seq=2)
+    cat = s.picture(40)
+    before = ([list(x) for x in s.cache.page_table_cpu], list(s.cache.free_pages), list(s.cache.free_batch_idx), list(s.cache.capacity))
+    many = [i for i in range(1, 4199) if i != cat][:4097]
+    for call, error, text in [(lambda: s.cache.step_tables(many, [0] * 4097, [0] * 4097), RuntimeError, "at most 4096"),
+                              (lambda: s.cache.fork(cat, 32, 4097), RuntimeError, "at most 4096"),
+                              (lambda: s.cache.step_tables(many[:3], [0] * 3, [1] * 3, row_multiple=1 << 30), ValueError, "31 bits"),
+                              (lambda: s.cache.step_tables(many[:3], [0] * 3, [0] * 3, row_multiple=1 << 32), ValueError, "31 bits")]:
+        with pytest.raises(error, match=text):
+            call()
+        assert before == ([list(x) for x in s.cache.page_table_cpu], list(s.cache.free_pages), list(s.cache.free_batch_idx),
+                          list(s.cache.capacity))
+    s.check_pool()
+
+
+def test_pages_whose_rows_are_not_whole_chunks_are_not_forked():
+    cache = PagedKVCache(16, 16, 5, 2, 4, 1, torch.bfloat16, device="cuda")
+    slot = cache.allocate()
+    cache.reserve(slot, None, 40)
+    before = (list(cache.free_pages), list(cache.free_batch_idx))
+    with pytest.raises(RuntimeError, match="cannot be copied"):
+        cache.fork(slot, 20)
+    assert before == (cache.free_pages, cache.free_batch_idx)
+
+
 def test_decode_from_a_graph():
     """A decode step captured before any fork serves the forks that come later, also when they go."""
     s = Server(slots=12)

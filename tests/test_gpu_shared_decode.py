@@ -375,3 +375,17 @@ def test_rows_that_are_not_aligned():
     wide[..., 3:] = case.q_d
     got = case.call(ops, q=wide[..., 3:])
     assert torch.equal(got[0], want[0])
+
+
+@pytest.mark.parametrize("with_plan", [False, True])
+def test_a_context_of_more_than_32_bits_is_refused(with_plan):
+    case = SharedBatch(24, [64], [(0, 3, 1), (0, 5, 1)], Hq=4, Hc=2, D=128, P=64, dtype=BF16).on()
+    kw = {}
+    if with_plan:
+        shape = dict(q_heads=4, cached_heads=2, head_dim=128)
+        kw = dict(plan=torch.zeros(ops.shared_decode_plan_bytes(2, 1, **shape), dtype=torch.uint8, device="cuda"),
+                  workspace=torch.zeros(ops.shared_decode_workspace_bytes(2, 1, **shape), dtype=torch.uint8, device="cuda"))
+        with pytest.raises(RuntimeError, match="does not fit 32 bits"):
+            ops.shared_decode_plan(case.batch_idx_d, case.pos_d, case.ids_d, case.lens_d, max_context=(1 << 32) + 200, plan=kw["plan"], **shape)
+    with pytest.raises(RuntimeError, match="does not fit 32 bits"):
+        case.call(ops, max_context=(1 << 32) + 200, **kw)

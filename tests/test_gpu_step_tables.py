@@ -257,6 +257,20 @@ def test_copy_many_pages():
     ops.copy_pages(got, src.cuda()[:0], dst.cuda()[:0], rows.cuda()[:0], P)
 
 
+@pytest.mark.parametrize("change", [dict(rows=(1 << 32) + 10), dict(row_multiple=(1 << 32) + 1), dict(P=(1 << 32) + 16), dict(P=-(1 << 33))])
+def test_numbers_of_more_than_32_bits_are_refused(change):
+    slots, old, new, par, free, count, table = make(9, 4, old_hi=200, add_hi=40, P=16)
+    dev = lambda x, t: torch.tensor(x, dtype=t, device="cuda")
+    sizes = dict(P=16, rows=200, row_multiple=1) | change
+    with pytest.raises(RuntimeError, match="does not fit 32 bits"):
+        ops.step_tables(dev(slots, torch.int64), dev(old, torch.int32), dev(new, torch.int32), dev(free, torch.int64),
+                        dev([count], torch.int32), table.cuda(), sizes["P"], sizes["rows"], row_multiple=sizes["row_multiple"])
+    if "P" in change:
+        one = torch.tensor([1], device="cuda")
+        with pytest.raises(RuntimeError, match="does not fit 32 bits" if change["P"] > 0 else "page_size"):
+            ops.copy_pages(torch.zeros(2, 64, 64, device="cuda"), one, one, one.int(), change["P"])
+
+
 def test_copy_pages_refusals():
     pool = torch.zeros(2, 64, 64, device="cuda")
     one = torch.tensor([1], device="cuda")

@@ -108,3 +108,11 @@ def test_operators_refuse_the_cpu():
         with pytest.raises(RuntimeError, match="GPU only"):
             call()
     assert before == (cache.free_pages, cache.free_batch_idx)
+
+
+def test_shapes_of_more_than_32_bits_are_refused(native_lib):
+    shape = dict(q_heads=8, cached_heads=8, head_dim=64)
+    for size in (ops.shared_decode_plan_bytes, ops.shared_decode_workspace_bytes):
+        for B, S, change in ((1 << 32) + 2, 1, {}), (2, (1 << 32) + 1, {}), (2, 1, dict(q_heads=(1 << 32) + 8)), (2, 1, dict(head_dim=(1 << 32) + 64)):
+            with pytest.raises(RuntimeError, match="does not fit 32 bits"):
+                size(B, S, **(shape | change))
