@@ -22,7 +22,7 @@
 //  * Join: a row's pieces, by their maxima and sums, in 32 bits.
 //
 // Bound by HBM where the keys are many.  64 sequences, most on one of 9 prefixes, 16 query heads on 8 cached ones, D 128, bf16, 473 MB a
-// layer: products 81.5 us (5.8 TB/s; a large copy reaches 5.2 on this GPU), join 4.9, plan 12.6 once a step; fp_paged_decode, which
+// layer: products 81.5 us (5.8 TB/s; a large copy reaches 5.2 on this GPU), join 4.9, plan 10.9 once a step; fp_paged_decode, which
 // reads a prefix once a sequence, takes 141.  192 sequences on 8 prefixes of up to 12288 keys, 4 query heads a cached one, 2.0 GB a layer:
 // 330 us, 6.0 TB/s (1153 once a sequence).  Small batches are bound by the trips to memory in front of the first key and by two
 // launches (3 sequences, 1.5 MB: 8.5 and 3.6 us), many tokens a sequence by LDS and the instructions between the matrix products
@@ -472,67 +472,62 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
     t.part = rest_part + rows_before + kTileRows * first;
     return t;
   };
-  for (int i = tid; i < n_wg + n_tiles + a.B; i += n_thr) {
-    if (i >= n_wg + n_tiles) {
-      const int b = i - n_wg - n_tiles, lead = s_lead[b];
-      const bool shares = s_shared[b] > 0;
-      Sequence q{s_slot[b], s_keys[b], shares ? s_ptile[lead] : -1, s_rank[b] * a.group,
-                 s_keys[b] > s_shared[b] ? p_tiles + s_stile[b] : -1};
-      if (a.S == 1) {
-        if (shares) {
-          const Tile t = tile_at(q.prefix_tile + q.prefix_row / kTileRows);
-          q.at = t.part + q.prefix_row % kTileRows, q.step = t.n_rows, q.n = t.n_pieces;
+  // Shares, tiles, and two items a sequence: its prefix and its own keys.  Lanes of all three work out the tile that they need together
+  // (in a branch for each they would do so one after the other: 16 sequences 11.2 us instead of 8.6).
+  for (int i = tid; i < n_wg + n_tiles + 2 * a.B; i += n_thr) {
+    const int k = i - n_wg - n_tiles, b = k >> 1;
+    const bool is_share = i < n_wg, is_tile = !is_share && k < 0, of_own = k & 1;
+    int index = -1, offset = 0, units_to_do = 0, piece = 0;
+    if (is_share) {
+      int start, from;  // of the first tile's first key and of this workgroup, on their axis
+      if (i < wg0) {
+        int m = 0, rest = i;  // the first group of the kind, workgroups of the kind before this one
+        for (;; ++m) {
+          const int here = s_n[m] * cuts(s_end[m], len);
+          if (rest < here) break;
+          rest -= here;
         }
-        if (q.own_tile >= 0) {
-          const Tile t = tile_at(q.own_tile);
-          q.own_at = t.part, q.own_step = t.n_rows, q.own_n = t.n_pieces;
-        }
-      }
-      seqs[b] = q;
-      continue;
-    }
-    if (i >= n_wg) {
-      reinterpret_cast<Tile*>(a.plan + a.tiles)[i - n_wg] = tile_at(i - n_wg);
-      continue;
-    }
-    const int w = i;
-    Share s;
-    int start, from;  // of the first tile's first key and of this workgroup, on their axis
-    if (w < wg0) {
-      int m = 0, rest = w;  // the first group of the kind, workgroups of the kind before this one
-      for (;; ++m) {
-        const int here = s_n[m] * cuts(s_end[m], len);
-        if (rest < here) break;
-        rest -= here;
-      }
-      const int n = s_n[m], all = s_end[m];
-      from = rest / n * len;
-      while (s_pos[m] + s_u[m] <= from) m = s_next[m];
-      s.tile = s_ptile[s_at[m]] + rest % n;
-      s.offset = from - s_pos[m];
-      s.units = min(len, all - from);
-      start = s_pos[m] + s_lu[m];
-    } else {
-      from = (w - wg0) * len;
-      int lead;
-      s.units = min(len, units - from);
-      if (from < prefix_units) {
-        const int b = last_at_or_below(s_unit, a.B, from), n = lead_for(s_count[b]) + units_of(s_shared[b]), off = from - s_unit[b];
-        lead = lead_for(s_count[b]);
-        s.tile = s_ptile[b] + off / n;
-        s.offset = off % n;
+        const int n = s_n[m], all = s_end[m];
+        from = rest / n * len;
+        while (s_pos[m] + s_u[m] <= from) m = s_next[m];
+        index = s_ptile[s_at[m]] + rest % n;
+        offset = from - s_pos[m];
+        units_to_do = min(len, all - from);
+        start = s_pos[m] + s_lu[m];
       } else {
-        const int b = last_at_or_below(s_own, a.B, from - prefix_units), n = lead_for(s_tok[b]) + units_of(s_keys[b] - s_shared[b]);
-        lead = lead_for(s_tok[b]);
-        const int off = from - prefix_units - s_own[b];
-        s.tile = p_tiles + s_stile[b] + off / n;
-        s.offset = off % n;
+        from = (i - wg0) * len;
+        units_to_do = min(len, units - from);
+        const bool own = from >= prefix_units;
+        const int at = own ? from - prefix_units : from, of = last_at_or_below(own ? s_own : s_unit, a.B, at);
+        const int lead = lead_for(own ? s_tok[of] : s_count[of]);
+        const int n = lead + units_of(own ? s_keys[of] - s_shared[of] : s_shared[of]), off = at - (own ? s_own : s_unit)[of];
+        index = (own ? p_tiles + s_stile[of] : s_ptile[of]) + off / n;
+        offset = off % n;
+        start = from - offset + lead;
       }
-      start = from - s.offset + lead;
+      piece = max(0, from / len - start / len);
+    } else if (is_tile) {
+      index = i - n_wg;
+    } else if (of_own) {
+      index = s_keys[b] > s_shared[b] ? p_tiles + s_stile[b] : -1;
+    } else {
+      index = s_shared[b] > 0 ? s_ptile[s_lead[b]] + s_rank[b] * a.group / kTileRows : -1;
     }
-    s.piece = max(0, from / len - start / len);
-    s.first = tile_at(s.tile);
-    reinterpret_cast<Share*>(a.plan + a.shares)[w] = s;
+    Tile t{};
+    if (index >= 0) t = tile_at(index);
+    if (is_share) {
+      reinterpret_cast<Share*>(a.plan + a.shares)[i] = Share{index, offset, units_to_do, piece, t};
+    } else if (is_tile) {
+      reinterpret_cast<Tile*>(a.plan + a.tiles)[index] = t;
+    } else if (of_own) {
+      seqs[b].own_tile = index;
+      seqs[b].own_at = t.part, seqs[b].own_step = t.n_rows, seqs[b].own_n = t.n_pieces;
+    } else {
+      const int row = s_rank[b] * a.group;
+      seqs[b].slot = s_slot[b], seqs[b].keys = s_keys[b];
+      seqs[b].prefix_tile = index < 0 ? -1 : index - row / kTileRows, seqs[b].prefix_row = row;
+      seqs[b].at = t.part + row % kTileRows, seqs[b].step = t.n_rows, seqs[b].n = t.n_pieces;
+    }
   }
 }
 
@@ -1390,7 +1385,8 @@ extern "C" int fp_shared_decode_plan(const int64_t* batch_idx, const void* input
   const Layout l = layout_of(B, S, Hq, Hc);
   const PlanArgs a{batch_idx, input_pos, pos_index_type, prefix_ids, prefix_lens, B, S, Hq, Hc, Hq / Hc, max_batch, max_context,
                    l.n_wg, static_cast<char*>(plan), l.seqs, l.tokens, l.place, l.shares, l.tiles};
-  const int threads = S > 1 || B > 64 ? 1024 : 256;
+  // as many as there are shares, tiles and sequences to write: 64 sequences 2 us less with 512 than with 256, a few no more
+  const int threads = S > 1 || B > 64 ? 1024 : B > 24 ? 512 : 256;
   const size_t lds = kPlanArrays * static_cast<size_t>((B + 3) & ~3) * sizeof(int);
   if (lds > 64 * 1024) {
     const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(shared_plan_kernel),
