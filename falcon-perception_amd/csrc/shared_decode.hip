@@ -350,9 +350,12 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   }
   __syncthreads();
   const int shortest_len = max(kMinUnits, (all_units + a.n_wg - 1) / a.n_wg);
-  const auto cuts = [](int units, int len) { return (units + len - 1) / len; };
+  const auto cuts = [](int units, int len) { return units > 0 ? (units - 1) / len + 1 : 0; };  // (two such sums may pass 31 bits)
+  const auto length_at = [&](int i) {  // the i-th of the 64: up to three times the shortest, at most everything
+    return static_cast<int>(min(static_cast<int64_t>(max(kMinUnits, all_units)), shortest_len + (static_cast<int64_t>(shortest_len) * i + 31) / 32));
+  };
   if (wave == 0 && n_multi > 0) {
-    const int len = shortest_len + (shortest_len * lane + 31) / 32;
+    const int len = length_at(lane);
     int need = 0, rest = all_units;
     for (int m = 0; m < n_multi; ++m) {
       need += s_n[m] * cuts(s_end[m], len);
@@ -364,7 +367,7 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   __syncthreads();
   const int pick = s_pick[0];
   const bool apart = pick >= 0;  // else there are too many kinds of groups: all on one axis
-  const int len = apart ? shortest_len + (shortest_len * pick + 31) / 32 : shortest_len;
+  const int len = apart ? length_at(pick) : shortest_len;
   const auto pieces_at = [&](int m) {  // of a tile: from the cut of its first key to that of its last
     return (s_pos[m] + s_u[m] - 1) / len - (s_pos[m] + s_lu[m]) / len + 1;
   };

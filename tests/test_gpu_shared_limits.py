@@ -1,0 +1,148 @@
+"""Attention over shared prefixes at its limits: sequences, rows of a cached head, keys."""
+
+import math
+
+import pytest
+import torch
+
+from falcon_perception_amd import ops
+from tests.shared_cases import HALF_STEP, SharedBatch
+
+pytestmark = pytest.mark.gpu
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def test_the_most_sequences():
+    B = 1536
+    groups = [b % 17 - 1 for b in range(B)]
+    case = SharedBatch(41, [64 + 9 * g for g in range(16)], [(g, 1 + b % 70, 1) for b, g in enumerate(groups)], Hq=8, Hc=1, D=64, P=32,
+                       dtype=BF16).on()
+    case.check(case.call(ops))
+    shape = dict(q_heads=8, cached_heads=1, head_dim=64)
+    with pytest.raises(RuntimeError, match="at most 1536 sequences"):
+        ops.shared_decode_plan_bytes(B + 1, 1, **shape)
+
+
+@pytest.mark.parametrize("shared", [True, False])
+def test_the_most_rows(shared):
+    """2^20 rows of one cached head, their positions anywhere: 16 sequences of 8192 tokens, 8 query heads."""
+    B, S, G, D, P, keys = 16, 8192, 8, 64, 32, 208
+    gen = torch.Generator(device="cuda").manual_seed(42)
+    rnd = lambda *shape: torch.randn(shape, generator=gen, device="cuda").to(BF16)
+    prefix = 130 if shared else 0
+    k, v = rnd(B, keys, D), rnd(B, keys, D)
+    k[:, :prefix], v[:, :prefix] = k[0, :prefix], v[0, :prefix]
+    blocks = keys // P + 1
+    pool = torch.full((2, 1, (B * blocks + 1) * P, D), float("nan"), dtype=BF16, device="cuda")
+    table = torch.zeros(B + 1, blocks, dtype=torch.int64, device="cuda")
+    order = torch.randperm(B * blocks, generator=gen, device="cuda") + 1
+    table[1:] = order.view(B, blocks)
+    slots = torch.arange(1, B + 1, device="cuda")
+    at = (table[1:, :, None] * P + torch.arange(P, device="cuda")).reshape(B, -1)[:, :keys]
+    pool[0, 0, at], pool[1, 0, at] = k, v
+    ids = torch.full((B + 1,), int(shared) * 5, dtype=torch.int32, device="cuda")
+    lens = torch.full((B + 1,), prefix, dtype=torch.int32, device="cuda")
+    pos = torch.randint(-1, keys, (B, S), generator=gen, device="cuda", dtype=torch.int32)
+    q = rnd(B, G, S, D)
+    out, lse = ops.paged_decode_shared(q, pool[0], pool[1], table, slots, pos, ids, lens, P, keys)
+    # Off by (tests/shared_cases.py): a score by d = (D + 2) 2^-24 c with c = scale * sum |q k|, its exponential by that, 2^-22 c and 2^-22;
+    # the two parts of a probability by 2 u^2; sums by (n + 64) 2^-24; the result by half a step.  c is taken at its largest.
+    u = HALF_STEP[BF16]
+    for b in range(B):
+        qd, kd, vd = q[b].double().reshape(G * S, D), k[b].double(), v[b].double()
+        scores = qd @ kd.T.contiguous() / math.sqrt(D)
+        c = (qd.abs() @ kd.abs().T.contiguous() / math.sqrt(D)).max().item()
+        seen = torch.arange(keys, device="cuda") <= pos[b].repeat(G)[:, None]
+        scores = scores.masked_fill(~seen, -math.inf)
+        want_lse = torch.logsumexp(scores, 1)
+        p = torch.where(seen, (scores - want_lse[:, None]).exp(), 0.0)
+        want, mass = p @ vd, p @ vd.abs()
+        rel = 2 * ((D + 2) * 2.0 ** -24 * c + 2.0 ** -22 * (c + 1)) + 2 * u * u + 2 * (keys + 64) * 2.0 ** -24
+        off = (out[b].reshape(G * S, D).double() - want).abs()
+        assert bool((off <= u * want.abs() + (1 + u) * rel * mass).all())
+        none = pos[b].repeat(G) < 0
+        got_lse = lse[b].reshape(-1).double()
+        assert bool(torch.isneginf(got_lse[none]).all()) and bool((out[b].reshape(G * S, D)[none] == 0).all())
+        assert bool(((got_lse - want_lse).abs()[~none] <= rel + 2.0 ** -22 * (c + 1 + math.log(keys))).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_the_longest_context(dtype):
+    """2^21 keys.  Every query head looks for one key: its score is 40 above all others, whose weights together are below
+    2^21 e^-40 = 9e-12 of its own, so that the result is that key's V but for this, a rounding of the score (40 is a sum of one product:
+    exact) and half a step."""
+    P, D, G, L = 128, 64, 8, 1 << 21
+    blocks = L // P
+    gen = torch.Generator(device="cuda").manual_seed(43)
+    shared = L - 200  # the prefix ends inside a page
+    whole = shared // P
+    own = blocks - whole
+    pool = torch.zeros(2, 1, (1 + whole + 2 * own) * P, D, dtype=dtype, device="cuda")
+    pages = torch.randperm(whole + 2 * own, generator=gen, device="cuda") + 1
+    table = torch.zeros(3, blocks, dtype=torch.int64, device="cuda")
+    table[1:, :whole] = pages[:whole]
+    table[1:, whole:] = pages[whole:].view(2, own)
+    pool[1, 0, P:] = torch.randn((whole + 2 * own) * P, D, generator=gen, device="cuda").to(dtype)
+    row = lambda b, t: int(table[b + 1, t // P]) * P + t % P
+    for t in range(whole * P, shared):  # the rest of the prefix: the same values in both copies
+        pool[:, 0, row(1, t)] = pool[:, 0, row(0, t)]
+    marks = [[0, 1, 1024 * P - 1, 1024 * P, shared - 1, shared, L - 2, L - 1],
+             [5, 63 * 64 - 1, 1500 * P + 77, L // 2, shared - 3, shared + 1, L - 130, L - 2]]
+    q = torch.zeros(2, G, 1, D, dtype=dtype, device="cuda")
+    for b in range(2):
+        for h, t in enumerate(marks[b]):
+            d = b * G + h
+            q[b, h, 0, d] = 16
+            for other in range(2) if t < shared else (b,):
+                pool[0, 0, row(other, t), d] = 20
+    got, lse = ops.paged_decode_shared(
+        q, pool[0], pool[1], table, torch.tensor([1, 2], device="cuda"), torch.tensor([L - 1, L - 2], device="cuda"),
+        torch.tensor([0, 9, 9], dtype=torch.int32, device="cuda"), torch.tensor([0, shared, shared], dtype=torch.int32, device="cuda"), P, L)
+    for b in range(2):
+        for h, t in enumerate(marks[b]):
+            want = pool[1, 0, row(b, t)].double()
+            # weights of other keys, exponential and quotient (2^-21), sums of three parts; half a step of the type
+            tol = (HALF_STEP[dtype] + 2.0 ** -19) * want.abs() + 1e-10 + 2 * HALF_STEP[dtype] ** 2 * want.abs()
+            assert bool(((got[b, h, 0].double() - want).abs() <= tol).all()), (b, h, t)
+            assert abs(float(lse[b, h, 0]) - 40) <= 40 * 2.0 ** -20
+    with pytest.raises(RuntimeError, match="at most 2097152"):
+        ops.paged_decode_shared(q, pool[0], pool[1], table, torch.tensor([1, 2], device="cuda"), torch.tensor([L, L], device="cuda"),
+                                torch.zeros(3, dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda"), P, L + 1)
+
+
+def test_large_steps_are_captured():
+    """Plans and tables whose working memory is beyond the default of a launch, captured and replayed over other positions."""
+    B = 1200
+    groups = [b % 9 - 1 for b in range(B)]
+    case = SharedBatch(44, [100 + 9 * g for g in range(8)], [(g, 30 + b % 40, 1) for b, g in enumerate(groups)], Hq=2, Hc=1, D=64, P=32,
+                       dtype=BF16).on()
+    R = 4096
+    slots = torch.arange(1, R + 1, device="cuda")
+    old, new = torch.zeros(R, dtype=torch.int32, device="cuda"), torch.ones(R, dtype=torch.int32, device="cuda")
+    free, count = torch.arange(1, 2 * R + 1, device="cuda"), torch.tensor([2 * R], dtype=torch.int32, device="cuda")
+    table = torch.zeros(1 << 16, 2, dtype=torch.int64, device="cuda")
+
+    def step():
+        return case.call(ops), ops.step_tables(slots, old, new, free, count, table, 16, 2 * R)
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        (out, lse), made = step()
+    for shift, tokens in ((0, 1), (7, 2), (21, 1)):
+        case.pos_d.copy_((case.pos - shift).cuda())
+        new.fill_(tokens)
+        table.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = case.call(ops)
+        assert torch.equal(out, eager[0]) and torch.equal(lse, eager[1])
+        case.check((out, lse), pos=case.pos - shift)
+        made.check()
+        assert made.row_starts.tolist() == [tokens * i for i in range(R + 1)] and made.free_left.tolist() == [R]
+        assert torch.equal(table[1:R + 1, 0], free.flip(0)[:R]) and not table[1:, 1].any()
