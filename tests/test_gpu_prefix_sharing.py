@@ -292,3 +292,46 @@ def test_decode_from_a_graph():
     new = s.picture(90)  # takes the slot
     assert new == a[1]
     s.decode([new, cat, a[0], a[2]])
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 128), (torch.float16, 64), (torch.float32, 64)])
+def test_prompts_attend_over_a_forked_prefix(dtype, D):
+    """A packed prefill step of forks is bit for bit that of sequences which were given the same prefix each for itself."""
+    n, prompts, layers, Hc, Hq = 133, [3, 17, 40], 2, 2, 4
+    gen = torch.Generator().manual_seed(5)
+    rnd = lambda *shape: torch.randn(shape, generator=gen).to(dtype).to(DEV)
+    first = [(rnd(1, Hc, n, D), rnd(1, Hc, n, D)) for _ in range(layers)]
+    new, q = None, None
+    got = []
+    for forked in (True, False):
+        cache = PagedKVCache(60, 32, 9, Hc, D, layers, dtype, device=DEV, prefix_sharing=forked)
+        heads = 1 if forked else 3
+        slots = [cache.allocate() for _ in range(heads)]
+        made = cache.step_tables(slots, [0] * heads, [n] * heads).check()
+        for layer, (k, v) in enumerate(first):
+            cache.insert_kv(layer, k.repeat(1, 1, heads, 1), v.repeat(1, 1, heads, 1), input_pos=made.input_pos[None], batch_idx=made.batch_idx[None])
+        if forked:
+            slots = cache.fork(slots[0], n, 3)
+        made = cache.step_tables(slots, [n] * 3, [n + p for p in prompts], row_multiple=128).check()
+        L = made.batch_idx.shape[0]
+        if new is None:
+            new, q = [(rnd(1, Hc, L, D), rnd(1, Hc, L, D)) for _ in range(layers)], rnd(1, Hq, L, D)
+        mask = cache.create_prefill_blockmask(made.batch_idx[None], torch.ones(1, L, dtype=torch.int64, device=DEV), 998, 999, validate=True)
+        for layer, (k, v) in enumerate(new):
+            K, V = cache.insert_kv(layer, k, v, input_pos=made.input_pos[None], batch_idx=made.batch_idx[None])
+            out, aux = A.compiled_flex_attn_prefill(q, K, V, block_mask=mask, return_aux=AuxRequest(lse=True))
+            got.append((out, aux.lse, made.row_starts.tolist(), made.input_pos, made.batch_idx > 0))
+    starts = got[0][2]
+    assert starts == [0, 128, 256, 384]
+    for a, b in zip(got[:layers], got[layers:]):
+        assert a[2] == b[2] and torch.equal(a[3], b[3]) and torch.equal(a[4], b[4])
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    # the first row of a prompt sees the prefix and itself: in float64, within what probabilities of the type and sums may be off
+    u = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -16}[dtype]
+    for layer in range(layers):
+        for at in starts[:3]:
+            k, v = (torch.cat([first[layer][i], new[layer][i][:, :, at:at + 1]], 2)[0].double().repeat_interleave(Hq // Hc, 0) for i in range(2))
+            scores = (k @ q[0, :, at, :, None].double())[..., 0] / D ** 0.5
+            p = torch.softmax(scores, -1)
+            want, mass = (p[..., None] * v).sum(1), (p[..., None] * v.abs()).sum(1)
+            assert bool(((got[layer][0][0, :, at].double() - want).abs() <= 3 * u * mass).all())
