@@ -1248,15 +1248,22 @@ __global__ __launch_bounds__(kThreads, (sizeof(Shared<E, D>) <= 80 * 1024 ? 2 : 
 }
 
 // ------------------------------------------------------------------------------------------------------------ join
-// D / 4 lanes a row.
+// D / 4 lanes have a row, kBatch of its pieces on their way at once.  A row has as many pieces as its keys are cut into, up to one a
+// workgroup.  kWide: a workgroup has one row, and where that has more pieces than a batch all of its groups of lanes take some, so
+// that they are one trip to memory.
 constexpr int kBatch = 8;
-template <typename E, int D>
+// Up to here a row a workgroup: 4 sequences on a prefix of 16000 keys, 64 pieces a row, 16 heads, D 128: a layer 28.3 -> 20.7 us; with pieces in
+// one batch it costs 0.2 us a layer (16 sequences, 256 rows) and with 6144 rows 10.
+constexpr int kWideRows = 2048;
+template <typename E, int D, bool kWide>
 __global__ __launch_bounds__(kThreads) void shared_join_kernel(const SharedArgs a) {
-  constexpr int LPR = D / 4;
+  constexpr int LPR = D / 4, kGroups = kThreads / LPR, kRowsHere = kWide ? 1 : kGroups;
+  __shared__ float2 s_ml[kGroups];
+  __shared__ f32x4 s_acc[kWide ? kGroups : 1][LPR];
+  const int c = threadIdx.x % LPR, group = threadIdx.x / LPR, here = kWide ? 0 : group, part = kWide ? group : 0;
   // (32 bits: a division of 64 is a thousand cycles in front of the first load)
-  const uint32_t row = blockIdx.x * (kThreads / LPR) + threadIdx.x / LPR;
-  const int c = threadIdx.x % LPR;
-  if (row >= static_cast<uint32_t>(a.B * a.S) * a.Hq) return;
+  const uint32_t rows = static_cast<uint32_t>(a.B * a.S) * a.Hq, row = blockIdx.x * kRowsHere + here;
+  if (row >= rows) return;
   const uint32_t bj = row / static_cast<uint32_t>(a.Hq);
   const int h = static_cast<int>(row - bj * a.Hq);
   const int b = a.S == 1 ? static_cast<int>(bj) : static_cast<int>(bj / static_cast<uint32_t>(a.S)), j = static_cast<int>(bj) - b * a.S;
@@ -1268,17 +1275,16 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(const SharedArgs 
   const bool valid = slot >= 0 && slot < a.max_batch;
   const int at_b = !fits || a.S == 1 ? 0 : reinterpret_cast<const int*>(a.plan + a.place)[bj];  // place among the sequence's tokens
   const bool missing = at_b < 0;
-  f32x4 res = {0.f, 0.f, 0.f, 0.f};
-  float lse = -INFINITY;
-  if (!fits || (valid && (s.slot != slot || keys > s.keys || (keys > 0 && missing))) || (!valid && s.slot >= 0)) {
-    lse = NAN;  // the plan is of another step
-    res = f32x4{NAN, NAN, NAN, NAN};
-  } else if (valid && keys > 0) {
+  // of another step: the plan
+  const bool foreign = !fits || (valid && (s.slot != slot || keys > s.keys || (keys > 0 && missing))) || (!valid && s.slot >= 0);
+  const bool any = !foreign && valid && keys > 0;
+  float m = -INFINITY, den = 0.f;
+  f32x4 num = {0.f, 0.f, 0.f, 0.f};
+  bool shared_out = false;
+  if (any) {
     const Tile* const tiles = reinterpret_cast<const Tile*>(a.plan + a.tiles);
     const int hc = h >> a.group_shift, x = (at_b << a.group_shift) + (h & (a.group - 1));
-    float m = -INFINITY, den = 0.f;
-    f32x4 num = {0.f, 0.f, 0.f, 0.f};
-    // the prefix's pieces, then those of its own keys: kBatch of them are on their way at once
+    // the prefix's pieces, then those of its own keys
     int n_shared = 0, n_own = 0;
     int64_t at = 0, step = 0, own_at = 0, own_step = 0;  // rows of the workspace
     if (a.S == 1) {
@@ -1302,31 +1308,64 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(const SharedArgs 
     }
     if (n_shared == 0 && n_own == 1) return;  // stored already
     const int n = n_shared + n_own;
-    for (int k0 = 0; k0 < n; k0 += kBatch) {
+    shared_out = kWide && n > kBatch;
+    if (!shared_out && part > 0) return;
+    const int stride = shared_out ? kGroups : 1;
+    for (int k0 = part; k0 < n; k0 += kBatch * stride) {
       float2 ml[kBatch];
       f32x4 acc[kBatch];
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
-        const int k = min(k0 + i, n - 1);
+        const int k = min(k0 + i * stride, n - 1);
         const int64_t p = (k < n_shared ? at + k * step : own_at + (k - n_shared) * own_step) * a.Hc + hc;
         ml[i] = *reinterpret_cast<const float2*>(a.ws_ml + p * 2);
         acc[i] = *reinterpret_cast<const f32x4*>(a.ws_acc + p * D + c * 4);
       }
       float mn = m;
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) mn = fmaxf(mn, ml[i].x);
+      for (int i = 0; i < kBatch; ++i) mn = fmaxf(mn, k0 + i * stride < n ? ml[i].x : -INFINITY);
       const float ms = safe_max(mn), keep = fast_exp2(m - ms);
       den *= keep;
       num *= keep;
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
-        if (k0 + i >= n) break;
+        if (k0 + i * stride >= n) break;
         const float w = fast_exp2(ml[i].x - ms);
         den += ml[i].y * w;
         num += acc[i] * w;
       }
       m = mn;
     }
+  } else if (part > 0) {
+    return;
+  }
+  if (kWide && shared_out) {
+    if (c == 0) s_ml[part] = float2{m, den};
+    s_acc[part][c] = num;
+    __syncthreads();
+    if (part > 0) return;
+    float2 ml[kGroups];
+    f32x4 acc[kGroups];
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) ml[i] = s_ml[i], acc[i] = s_acc[kWide ? i : 0][c];
+#pragma unroll
+    for (int i = 1; i < kGroups; ++i) m = fmaxf(m, ml[i].x);
+    const float ms = safe_max(m);
+    den = 0.f;
+    num = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) {
+      const float w = fast_exp2(ml[i].x - ms);
+      den += ml[i].y * w;
+      num += acc[i] * w;
+    }
+  }
+  f32x4 res = {0.f, 0.f, 0.f, 0.f};
+  float lse = -INFINITY;
+  if (foreign) {
+    lse = NAN;
+    res = f32x4{NAN, NAN, NAN, NAN};
+  } else if (any) {
     lse = (m + log2f(den)) * kLn2;
 #pragma unroll
     for (int k = 0; k < 4; ++k) res[k] = gated(num[k] / den, lse, a.sinks, h);
@@ -1338,8 +1377,14 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(const SharedArgs 
 template <typename E, int D>
 void launch(const SharedArgs& a, int n_wg, hipStream_t st) {
   hipLaunchKernelGGL((shared_products_kernel<E, D>), dim3(a.Hc, n_wg), dim3(kThreads), 0, st, a);
-  const int64_t rows = static_cast<int64_t>(a.B) * a.S * a.Hq, per = kThreads / (D / 4);
-  hipLaunchKernelGGL((shared_join_kernel<E, D>), dim3(static_cast<unsigned>((rows + per - 1) / per)), dim3(kThreads), 0, st, a);
+  const int64_t rows = static_cast<int64_t>(a.B) * a.S * a.Hq;
+  const auto join = [&](auto kernel, int here) {
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((rows + here - 1) / here)), dim3(kThreads), 0, st, a);
+  };
+  if (rows <= kWideRows)
+    join(shared_join_kernel<E, D, true>, 1);
+  else
+    join(shared_join_kernel<E, D, false>, kThreads / (D / 4));
 }
 
 int check_shape(const char* what, int B, int S, int Hq, int Hc, int D) {

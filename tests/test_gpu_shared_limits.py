@@ -146,3 +146,21 @@ def test_large_steps_are_captured():
         made.check()
         assert made.row_starts.tolist() == [tokens * i for i in range(R + 1)] and made.free_left.tolist() == [R]
         assert torch.equal(table[1:R + 1, 0], free.flip(0)[:R]) and not table[1:, 1].any()
+
+
+@pytest.mark.parametrize("D,Hq,Hc,dtype", [(64, 2, 1, F16), (128, 4, 2, BF16), (64, 8, 8, F32)])
+def test_few_sequences_cut_into_many_pieces(D, Hq, Hc, dtype):
+    """A row's pieces are one to about all workgroups; rows beside each other have few and many, and results that need no join."""
+    for seed, prefixes, sequences in [(45, [], [(-1, 20000, 1)]), (46, [9000], [(0, 5, 1), (0, 1, 1), (-1, 3, 1), (-1, 6000, 1)]),
+                                      (47, [700], [(0, 2, 1), (-1, 1, 1), (0, 2500, 1)])]:
+        case = SharedBatch(seed, prefixes, sequences, Hq=Hq, Hc=Hc, D=D, P=64, dtype=dtype).on()
+        got = case.call(ops)
+        case.check(got)
+        again = case.call(ops)
+        assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+        case.check(case.call(ops, sinks=torch.linspace(-2, 2, Hq, device="cuda")), sinks=torch.linspace(-2, 2, Hq))
+
+
+def test_several_tokens_of_one_sequence_over_many_keys():
+    case = SharedBatch(48, [], [(-1, 15000, 5)], Hq=4, Hc=2, D=128, P=128, dtype=BF16).on()
+    case.check(case.call(ops))
