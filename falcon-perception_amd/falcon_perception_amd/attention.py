@@ -255,7 +255,8 @@ def compiled_flex_attn_decode(q: Tensor, k: Tensor, v: Tensor, score_mod=None, b
         raise RuntimeError(
             f"the mask was converted for {tuple(block_mask.batch_idx.shape)} sequences but the last insert_kv of this "
             f"cache appended {tuple(step.batch_idx.shape)}: attention must follow the insert_kv of its own step")
-    if getattr(cache, "prefix_sharing", False):
+    # (one sequence shares with nobody: 16 heads, D 128, 1030 keys 7.8 us a layer below, 12.0 there)
+    if getattr(cache, "prefix_sharing", False) and q.shape[0] > 1:
         return _result(*_shared_decode(q, k, v, block_mask, step, scale, sinks), return_aux, return_lse)
     kv_rep = getattr(cache, "kv_rep", 1)
     B, Hq, _, D = q.shape

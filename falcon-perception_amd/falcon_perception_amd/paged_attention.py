@@ -50,8 +50,9 @@ class PagedKVCache(KVCacheBase):
 
     `prefix_sharing` (not an argument of the reference's class either) is for batches of requests about one picture: `fork`
     makes sequences that begin with a cached one's tokens and share its pages, and decode attention reads such a
-    prefix once for all of them (`ops.paged_decode_shared`).  Every decode call of the cache then goes that way, captured
-    in a graph or not: which sequences share is found on the GPU, from `prefix_ids` and `prefix_lens` [max_batch].
+    prefix once for all of them (`ops.paged_decode_shared`).  Every decode call of the cache for two sequences or more then
+    goes that way, captured in a graph or not: which of them share is found on the GPU, from `prefix_ids` and `prefix_lens`
+    [max_batch].
 
     `max_blocks_per_seq` (not an argument of the reference's class) makes the tables sparse:
     page_table becomes [max_batch, max_blocks_per_seq] and the inverse table is not kept.  The

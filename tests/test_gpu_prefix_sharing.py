@@ -335,3 +335,26 @@ def test_prompts_attend_over_a_forked_prefix(dtype, D):
             p = torch.softmax(scores, -1)
             want, mass = (p[..., None] * v).sum(1), (p[..., None] * v.abs()).sum(1)
             assert bool(((got[layer][0][0, :, at].double() - want).abs() <= 3 * u * mass).all())
+
+
+def test_one_sequence_decodes_as_without_sharing():
+    """A step of one sequence, alone and between steps of several, is that of a cache without prefix_sharing bit for bit."""
+    outs = []
+    for sharing in (True, False):
+        s = Server(prefix_sharing=sharing, seed=9)
+        seen = []
+        cat = s.picture(133)
+        forks = s.fork(cat, 133, 2)
+        s.decode([forks[0]])
+        s.decode([forks[0], cat, forks[1]])
+        s.decode([cat])
+        pos = torch.tensor([s.length(cat)], dtype=torch.int32, device=DEV)
+        s.cache.reserve(cat, None, int(pos) + 1)
+        mask, idx, gen = s.mask([cat], pos), torch.tensor([cat], device=DEV), torch.Generator().manual_seed(3)
+        rnd = lambda heads: torch.randn(1, heads, 1, s.D, generator=gen).to(s.dtype).to(DEV)
+        for layer in range(s.layers):
+            K, V = s.cache.insert_kv(layer, rnd(s.Hc), rnd(s.Hc), input_pos=pos.view(-1, 1), batch_idx=idx)
+            out, aux = A.compiled_flex_attn_decode(rnd(s.Hq), K, V, block_mask=mask, return_aux=AuxRequest(lse=True))
+            seen += [out, aux.lse]
+        outs.append(seen)
+    assert all(torch.equal(x, y) for x, y in zip(*outs))
