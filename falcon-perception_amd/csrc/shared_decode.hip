@@ -22,10 +22,10 @@
 //  * Join: a row's pieces, by their maxima and sums, in 32 bits.
 //
 // Bound by HBM where the keys are many.  64 sequences, most on one of 9 prefixes, 16 query heads on 8 cached ones, D 128, bf16, 473 MB a
-// layer: products 81.5 us (5.8 TB/s; a large copy reaches 5.2 on this GPU), join 4.9, plan 10.9 once a step; fp_paged_decode, which
+// layer: products 81.5 us (5.8 TB/s; a large copy reaches 5.2 on this GPU), join 5.0, plan 10.9 once a step; fp_paged_decode, which
 // reads a prefix once a sequence, takes 141.  192 sequences on 8 prefixes of up to 12288 keys, 4 query heads a cached one, 2.0 GB a layer:
 // 330 us, 6.0 TB/s (1153 once a sequence).  Small batches are bound by the trips to memory in front of the first key and by two
-// launches (3 sequences, 1.5 MB: 8.5 and 3.6 us), many tokens a sequence by LDS and the instructions between the matrix products
+// launches (3 sequences, 1.5 MB: 8.9 and 4.1 us), many tokens a sequence by LDS and the instructions between the matrix products
 // (40 sequences of 24 tokens, 11.6 GFLOP: 46 us).
 #include "decode_common.h"
 
