@@ -255,8 +255,10 @@ def compiled_flex_attn_decode(q: Tensor, k: Tensor, v: Tensor, score_mod=None, b
         raise RuntimeError(
             f"the mask was converted for {tuple(block_mask.batch_idx.shape)} sequences but the last insert_kv of this "
             f"cache appended {tuple(step.batch_idx.shape)}: attention must follow the insert_kv of its own step")
-    # (one sequence shares with nobody: 16 heads, D 128, 1030 keys 7.8 us a layer below, 12.0 there)
-    if getattr(cache, "prefix_sharing", False) and q.shape[0] > 1:
+    # (one sequence shares with nobody: 16 heads, D 128, 1030 keys 7.8 us a layer below, 12.0 there; steps that are larger than one call
+    # over shared prefixes serves go below as well: there is no such limit there)
+    if (getattr(cache, "prefix_sharing", False) and 1 < q.shape[0] <= ops.SHARED_SEQUENCES
+            and block_mask.max_context <= ops.SHARED_CONTEXT):
         return _result(*_shared_decode(q, k, v, block_mask, step, scale, sinks), return_aux, return_lse)
     kv_rep = getattr(cache, "kv_rep", 1)
     B, Hq, _, D = q.shape

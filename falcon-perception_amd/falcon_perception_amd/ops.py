@@ -644,6 +644,9 @@ def copy_pages(pool: Tensor, src: Tensor, dst: Tensor, rows: Tensor, page_size: 
     N.check(rc, "fp_copy_pages")
 
 
+SHARED_SEQUENCES, SHARED_CONTEXT = 1536, 1 << 21  # that one `paged_decode_shared` call serves
+
+
 def shared_decode_plan_bytes(B: int, S: int, *, q_heads: int, cached_heads: int, head_dim: int) -> int:
     """Bytes of the plan of a `paged_decode_shared` step of this shape."""
     _int32("fp_shared_decode_plan_bytes", B=B, S=S, q_heads=q_heads, cached_heads=cached_heads, head_dim=head_dim)

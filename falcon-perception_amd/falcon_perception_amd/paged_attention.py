@@ -50,9 +50,9 @@ class PagedKVCache(KVCacheBase):
 
     `prefix_sharing` (not an argument of the reference's class either) is for batches of requests about one picture: `fork`
     makes sequences that begin with a cached one's tokens and share its pages, and decode attention reads such a
-    prefix once for all of them (`ops.paged_decode_shared`).  Every decode call of the cache for two sequences or more then
-    goes that way, captured in a graph or not: which of them share is found on the GPU, from `prefix_ids` and `prefix_lens`
-    [max_batch].
+    prefix once for all of them (`ops.paged_decode_shared`).  Every decode call of the cache for two sequences or more that one
+    such call serves (`ops.SHARED_SEQUENCES`, `ops.SHARED_CONTEXT`) then goes that way, captured in a graph or not: which of them share is
+    found on the GPU, from `prefix_ids` and `prefix_lens` [max_batch].
 
     `max_blocks_per_seq` (not an argument of the reference's class) makes the tables sparse:
     page_table becomes [max_batch, max_blocks_per_seq] and the inverse table is not kept.  The
@@ -471,7 +471,7 @@ class PagedKVCache(KVCacheBase):
         key = (Hq, Hc, D)
         hit = self._shared_buffers.get(key)
         if hit is None or hit[2] < B:
-            most = max(B, min(self.max_batch_size, 1536))
+            most = max(B, min(self.max_batch_size, ops.SHARED_SEQUENCES))
             shape = dict(q_heads=Hq, cached_heads=Hc, head_dim=D)
             sizes = ops.shared_decode_plan_bytes(most, 1, **shape), ops.shared_decode_workspace_bytes(most, 1, **shape)
             if hit is not None:

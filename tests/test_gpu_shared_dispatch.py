@@ -1,0 +1,53 @@
+"""Which decode calls of a cache with prefix_sharing go over shared prefixes, and what the others do instead."""
+
+import pytest
+import torch
+from torch.nn.attention.flex_attention import AuxRequest, BlockMask
+
+from falcon_perception_amd import attention as A
+from falcon_perception_amd import ops
+from falcon_perception_amd.paged_attention import PagedKVCache
+from tests.test_gpu_prefix_sharing import DEV, Server
+
+pytestmark = pytest.mark.gpu
+
+
+def decode_alike(monkeypatch, B, room, n_pages, slots, P, *, shared):
+    """Two layers of a decode step of B forks of 40 tokens, on a cache with prefix_sharing and on one without it: bit for bit alike
+    where the step does not go over shared prefixes."""
+    calls = []
+    real = ops.paged_decode_shared
+    monkeypatch.setattr(ops, "paged_decode_shared", lambda *a, **kw: calls.append(1) or real(*a, **kw))
+    got = []
+    for sharing in (True, False):
+        s = Server(prefix_sharing=sharing, n_pages=n_pages, P=P, slots=slots, Hc=1, Hq=2, layers=2, max_blocks_per_seq=-(-room // P), seed=3)
+        idx = [s.picture(40)]
+        idx += s.fork(idx[0], 40, B - 1)
+        s.cache.step_tables(idx, [40] * B, [41] * B)
+        pos = torch.full((B,), 40, dtype=torch.int32, device=DEV)
+        n = torch.full((B, 1, 1), 40 // P + 1, dtype=torch.int32, device=DEV)
+        logical = BlockMask.from_kv_blocks(n, torch.zeros(B, 1, 1, 2, dtype=torch.int32, device=DEV), None, None,
+                                           BLOCK_SIZE=(P, P), mask_mod=lambda b, h, q, kv: q + pos[b] >= kv, seq_lengths=(1, room))
+        mask = s.cache.convert_logical_block_mask(logical, torch.tensor(idx, device=DEV))
+        assert mask.max_context == room
+        for layer in range(2):
+            q, k, v = s.rnd(B, 2, 1, s.D), s.rnd(B, 1, 1, s.D), s.rnd(B, 1, 1, s.D)
+            K, V = s.cache.insert_kv(layer, k.to(DEV), v.to(DEV), input_pos=pos.view(-1, 1), batch_idx=mask.batch_idx)
+            out, aux = A.compiled_flex_attn_decode(q.to(DEV), K, V, block_mask=mask, return_aux=AuxRequest(lse=True))
+            got += [out, aux.lse]
+            if sharing:
+                keys = [tuple(torch.cat([old, new[i]], 1) for old, new in zip(s.keys[x][layer], (k, v))) for i, x in enumerate(idx)]
+                s.expected(q, keys, pos.cpu()).check((out, aux.lse))
+    assert len(calls) == 2 * shared
+    if not shared:
+        assert all(torch.equal(x, y) for x, y in zip(got[:4], got[4:]))
+
+
+@pytest.mark.parametrize("B,shared", [(1536, True), (1537, False), (1700, False)])
+def test_batches_of_any_size_decode(monkeypatch, B, shared):
+    decode_alike(monkeypatch, B, 128, 2 * 1800, 1800, 32, shared=shared)
+
+
+@pytest.mark.parametrize("room,shared", [(1 << 21, True), ((1 << 21) + 128, False)])
+def test_contexts_of_any_size_decode(monkeypatch, room, shared):
+    decode_alike(monkeypatch, 3, room, (1 << 14) + 2, 5, 128, shared=shared)

@@ -116,3 +116,10 @@ def test_shapes_of_more_than_32_bits_are_refused(native_lib):
         for B, S, change in ((1 << 32) + 2, 1, {}), (2, (1 << 32) + 1, {}), (2, 1, dict(q_heads=(1 << 32) + 8)), (2, 1, dict(head_dim=(1 << 32) + 64)):
             with pytest.raises(RuntimeError, match="does not fit 32 bits"):
                 size(B, S, **(shape | change))
+
+
+def test_the_limits_have_one_name_each(native_lib):
+    """What the decode path of a sharing cache takes as the limits of one call are those of the library."""
+    for B, room, code in ((ops.SHARED_SEQUENCES, ops.SHARED_CONTEXT, -1), (ops.SHARED_SEQUENCES + 1, ops.SHARED_CONTEXT, -2),
+                          (ops.SHARED_SEQUENCES, ops.SHARED_CONTEXT + 1, -2)):
+        assert attend(native_lib, B=B, room=room, q=None) == code
