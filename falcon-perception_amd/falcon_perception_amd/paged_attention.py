@@ -476,7 +476,8 @@ class PagedKVCache(KVCacheBase):
             sizes = ops.shared_decode_plan_bytes(most, 1, **shape), ops.shared_decode_workspace_bytes(most, 1, **shape)
             if hit is not None:
                 self._retired_workspaces.extend(hit[:2])
-            plan, workspace = (torch.zeros(n, dtype=torch.uint8, device=self._kv.device) for n in sizes)
+            # not cleared: nothing in them needs it, and of a first use inside a graph's capture every replay would clear them again
+            plan, workspace = (torch.empty(n, dtype=torch.uint8, device=self._kv.device) for n in sizes)
             hit = self._shared_buffers[key] = (plan, workspace, most)
         return hit[0], hit[1]
 

@@ -51,3 +51,35 @@ def test_batches_of_any_size_decode(monkeypatch, B, shared):
 @pytest.mark.parametrize("room,shared", [(1 << 21, True), ((1 << 21) + 128, False)])
 def test_contexts_of_any_size_decode(monkeypatch, room, shared):
     decode_alike(monkeypatch, 3, room, (1 << 14) + 2, 5, 128, shared=shared)
+
+
+def test_a_first_use_inside_a_capture_clears_nothing_in_replays():
+    """The buffers of a step whose first call is a graph's: a replay writes what the launch writes, not the whole buffers (some 70 MB
+    for a cache of 1536 slots)."""
+    s = Server(slots=400)
+    cat = s.picture(133)
+    idx = [cat, *s.fork(cat, 133, 2)]
+    s.cache.step_tables(idx, [133] * 3, [134] * 3)
+    pos = torch.full((3,), 133, dtype=torch.int32, device=DEV)
+    mask, ids = s.mask(idx, pos), torch.tensor(idx, device=DEV)
+    q, k, v = (s.rnd(3, h, 1, s.D).to(DEV) for h in (s.Hq, s.Hc, s.Hc))
+
+    def step():
+        K, V = s.cache.insert_kv(0, k, v, input_pos=pos.view(-1, 1), batch_idx=ids)
+        return A.compiled_flex_attn_decode(q, K, V, block_mask=mask)
+
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    plan, workspace = s.cache.shared_decode_buffers(3, s.Hq, s.Hc, s.D)
+    assert workspace.numel() > 1 << 20
+    for _ in range(3):
+        plan.fill_(0x5b)
+        workspace.fill_(0x5b)
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert bool((workspace[-4096:] == 0x5b).all()) and bool((plan[-256:] == 0x5b).all())
+        want = step()
+        assert torch.equal(out, want) and bool(torch.isfinite(want).all())
