@@ -452,14 +452,15 @@ class PagedKVCache(KVCacheBase):
             raise RuntimeError("a sequence has no pages for the tokens it is said to have cached")
         # the pages each request gets, in the place where the kernel looks for them: the last request's first.  Pages that were reserved
         # ahead of the step are written again as they are.
-        pages: list[int] = []
+        taken: list[list[int]] = []
         for s, o, n, p, more in zip(slots, old_lens, new_lens, parents, grow):
             if more:
                 self.page_table_cpu[s] += self.free_pages[-more:]
                 del self.free_pages[-more:]
                 self.capacity[s] = len(self.page_table_cpu[s]) * P
             have = o // P if p > 0 else _cdiv(o, P)
-            pages = self.page_table_cpu[s][have:_cdiv(n, P)] + pages
+            taken.append(self.page_table_cpu[s][have:_cdiv(n, P)])
+        pages = [page for of_request in reversed(taken) for page in of_request]
         packed = torch.tensor([*slots, *old_lens, *new_lens, *parents, *pages, len(pages)], dtype=torch.int64, device=self.device)
         ids, old, new, par = (packed[i * B:(i + 1) * B] for i in range(4))
         return ops.step_tables(ids, old, new, packed[4 * B:-1], packed[-1:].view(torch.int32)[:1], self.page_table, P, rows,
