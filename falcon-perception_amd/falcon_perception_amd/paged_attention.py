@@ -423,6 +423,8 @@ class PagedKVCache(KVCacheBase):
         return slots
 
     def _check_step(self, B: int) -> None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("fork and step_tables run on the host, between steps: they cannot be captured in a graph.")
         if B > ops.STEP_REQUESTS or self.max_batch_size > ops.STEP_SLOTS:
             raise RuntimeError(f"A step is of at most {ops.STEP_REQUESTS} sequences in a cache of at most {ops.STEP_SLOTS} (got {B} and "
                                f"{self.max_batch_size}).")

@@ -67,3 +67,18 @@ def test_the_time_of_a_step_grows_with_its_requests(launches):
 
     seconds(64)
     assert seconds(4096) < 24 * seconds(512)
+
+
+def test_a_step_inside_a_capture_changes_nothing(launches, monkeypatch):
+    cache = cache_of(8, 60, columns=30, prefix_sharing=True)
+    slot = cache.allocate()
+    cache.reserve(slot, None, 40)
+    state = lambda: ([list(x) for x in cache.page_table_cpu], list(cache.free_pages), list(cache.free_batch_idx), list(cache.capacity),
+                     dict(cache._prefixes), dict(cache._page_slots), cache.page_table.tolist())
+    before = state()
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    for call in (lambda: cache.fork(slot, 40, 2), lambda: cache.fork(slot, 32), lambda: cache.step_tables([slot], [40], [50])):
+        with pytest.raises(RuntimeError, match="cannot be captured"):
+            call()
+        assert state() == before and not launches
+    monkeypatch.undo()
