@@ -52,7 +52,9 @@ class PagedKVCache(KVCacheBase):
     makes sequences that begin with a cached one's tokens and share its pages, and decode attention reads such a
     prefix once for all of them (`ops.paged_decode_shared`).  Every decode call of the cache for two sequences or more that one
     such call serves (`ops.SHARED_SEQUENCES`, `ops.SHARED_CONTEXT`) then goes that way, captured in a graph or not: which of them share is
-    found on the GPU, from `prefix_ids` and `prefix_lens` [max_batch].
+    found on the GPU, from `prefix_ids` and `prefix_lens` [max_batch].  A slot shares with one line of forks at a time: of a system
+    prompt, pictures forked from it and questions forked from a picture, the questions share their picture (prompt included), and the prompt is
+    read once a picture.
 
     `max_blocks_per_seq` (not an argument of the reference's class) makes the tables sparse:
     page_table becomes [max_batch, max_blocks_per_seq] and the inverse table is not kept.  The
@@ -140,11 +142,12 @@ class PagedKVCache(KVCacheBase):
         self._table_view: tuple[Tensor, int, Tensor] | None = None  # of `table_for`
         self._prefill_need: dict[tuple, tuple[int, int]] = {}
         self._prefill_tile_rows: dict[tuple, int] = {}
-        # prefix sharing: pages that several slots map (page -> slots), what each slot shares (id, tokens, whether it is a
-        # fork), and the same by slot on the GPU for the decode kernel's plan
+        # prefix sharing: pages that several slots map (page -> slots), what each slot shares (id, tokens, whether with the first
+        # sequence of its line or as that one, tokens its own forks do not share with it by that), and the first two by slot on
+        # the GPU for the decode kernel's plan
         self.prefix_sharing = bool(prefix_sharing)
         self._page_slots: dict[int, int] = {}
-        self._prefixes: dict[int, tuple[int, int, bool]] = {}
+        self._prefixes: dict[int, tuple[int, int, bool, int]] = {}
         self._last_prefix_id = 0
         self.prefix_ids = torch.zeros(max_batch_size, dtype=torch.int32, device=device) if prefix_sharing else None
         self.prefix_lens = torch.zeros(max_batch_size, dtype=torch.int32, device=device) if prefix_sharing else None
@@ -405,16 +408,25 @@ class PagedKVCache(KVCacheBase):
         if tail:
             ops.copy_pages(self._kv, made.copy_src, made.copy_dst, made.copy_rows, self.page_size)
         # Slots with one id share at least the smaller of their two lengths: a fork's length is what it shares with the first sequence
-        # of its line, and that one's is the longest of its own forks'.
-        root_id, root_len, forked = self._prefixes.get(parent, (0, 0, False))
+        # of its line, and that one's is the longest of its own forks'.  Forks of a fork behind what it shares with its line (a picture
+        # behind a system prompt, questions behind the picture) share more with it than with the line.  Once the keys that they would
+        # read several times are more than those the line shares, the fork begins a line of its own: its forks from then on have
+        # its id, and what the old line shares is read once more for the new one.
+        root_id, root_len, forked, apart = self._prefixes.get(parent, (0, 0, False, 0))
+        if forked:
+            apart += count * max(0, n_tokens - root_len)
+            if apart > root_len:
+                root_id, root_len, forked = 0, 0, False
+            else:
+                self._prefixes[parent] = (root_id, root_len, True, apart)
         if root_id == 0:
             self._last_prefix_id += 1
             root_id = self._last_prefix_id
         length = min(n_tokens, root_len) if forked else n_tokens
         if not forked:
-            self._prefixes[parent] = (root_id, max(root_len, n_tokens), False)
+            self._prefixes[parent] = (root_id, max(root_len, n_tokens), False, 0)
         for slot in slots:
-            self._prefixes[slot] = (root_id, length, True)
+            self._prefixes[slot] = (root_id, length, True, 0)
         if self.prefix_sharing:
             rows = [*slots, parent]
             values = torch.tensor([rows, [self._prefixes[r][0] for r in rows], [self._prefixes[r][1] for r in rows]], device=self.device)
