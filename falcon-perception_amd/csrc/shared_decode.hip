@@ -6,8 +6,8 @@
 // head - are the columns of one matrix product, so that a shared key is read once for up to 64 rows, not once a sequence.
 //
 // Three launches: the plan once per step, then for every layer the products and the join.
-//  * Plan (one workgroup): finds the groups, and makes tiles of up to 64 rows over one range of keys: the prefix of a group
-//    by its rows, the keys behind it by the rows of one sequence.  The tiles' keys, in units of 64, are laid end to end and
+//  * Plan (one workgroup): finds the groups, leaves out members whose prefix is too short, and makes tiles of up to 64 rows over
+//    one range of keys: the prefix of a group by its rows, the keys behind it by the rows of one sequence.  The tiles' keys, in units of 64, are laid end to end and
 //    cut evenly over two workgroups a CU, so a workgroup streams the same number of keys whatever the lengths are; a tile
 //    that a cut goes through leaves a partial result for each of its pieces.
 //  * Products: a workgroup of 4 wavefronts takes the pieces of its cut, one cached head.  The wavefronts have the same rows
@@ -207,26 +207,32 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   int* const s_end = s_pos + Bp;       //   length of that axis, at the first of a kind, elsewhere 0,
   int* const s_next = s_end + Bp;      //   the next of its kind, -1: none,
   int* const s_part = s_next + Bp;     //   pieces of the groups before
-  __shared__ int s_sum[16 * 7], s_pick[1];
+  __shared__ int s_sum[16 * 7], s_pick[1], s_turn[2];
   const int tid = threadIdx.x, n_thr = blockDim.x, lane = tid & 63, wave = tid >> 6, n_waves = n_thr / 64;
   Sequence* const seqs = reinterpret_cast<Sequence*>(a.plan + a.seqs);
   // until the sums below, these three hold a group's sequences, shortest prefix length and most keys, at its first sequence
   int* const s_members = s_ptile;
   int* const s_shortest = s_base;
   int* const s_longest = s_stile;
+  // and these its longest prefix length, the most units that a length spares, and that length
+  int* const s_furthest = s_unit;
+  int* const s_best = s_own;
+  int* const s_cut = s_wide;
   for (int b = tid; b < Bp; b += n_thr) {
     const int64_t slot = b < a.B ? a.batch_idx[b] : -1;
     const bool valid = slot >= 0 && slot < a.max_batch;
     const int keys = a.S == 1 && valid ? plan_keys(a, b, 0) : 0;
-    s_id[b] = valid ? max(a.ids[slot], 0) : 0;
-    s_len[b] = valid ? max(a.lens[slot], 0) : 0;
+    const int id = valid ? max(a.ids[slot], 0) : 0, length = valid ? max(a.lens[slot], 0) : 0;
+    s_id[b] = length >= kUnit ? id : 0;
+    s_len[b] = length;
     s_keys[b] = keys;
     s_tok[b] = keys > 0;
     s_slot[b] = valid ? static_cast<int>(slot) : -1;
     s_lead[b] = b;
-    s_rank[b] = s_count[b] = s_members[b] = s_longest[b] = 0;
+    s_rank[b] = s_count[b] = s_members[b] = s_longest[b] = s_furthest[b] = 0;
     s_shortest[b] = INT32_MAX;
   }
+  if (tid < 2) s_turn[tid] = 0;
   __syncthreads();
   if (a.S > 1) {
     for (int i = tid; i < a.B * a.S; i += n_thr) {
@@ -241,7 +247,11 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
 
   // Groups.  The first sequence with the same id leads, and a sequence's place is behind the tokens of those before it: sequences
   // look at all before them, four at a time, some threads a sequence.  A sequence without a token belongs to no group.
-  {
+  const auto usable = [&](int b) { return min(s_len[b], s_longest[s_lead[b]]) / kUnit; };  // units of its prefix
+  const auto mixed = [&](int lead) {
+    return s_members[lead] > 2 && min(s_shortest[lead], s_longest[lead]) / kUnit < min(s_furthest[lead], s_longest[lead]) / kUnit;
+  };
+  for (int turn = 0;; ++turn) {
     const int wide = (a.B + 63) & ~63, parts = max(1, n_thr / wide), part = tid / wide;
     const int quads = (Bp / 4 + parts - 1) / parts;  // that a thread looks at
     for (int b = parts > 1 ? tid - part * wide : tid; b < a.B && part < parts; b += n_thr) {
@@ -261,28 +271,94 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
       if (lead < b) atomicMin(&s_lead[b], lead);
       if (rank > 0) atomicAdd(&s_rank[b], rank);
     }
+    __syncthreads();
+    for (int b = tid; b < a.B; b += n_thr) {
+      if (s_id[b] == 0 || s_tok[b] == 0) continue;
+      const int lead = s_lead[b];
+      atomicAdd(&s_count[lead], s_tok[b]);
+      atomicAdd(&s_members[lead], 1);
+      atomicMin(&s_shortest[lead], s_len[b]);
+      atomicMax(&s_furthest[lead], s_len[b]);
+      atomicMax(&s_longest[lead], s_keys[b]);
+    }
+    __syncthreads();
+    for (int b = tid; b < a.B; b += n_thr) {
+      // Whole units: what is behind them counts as each one's own, up to 63 keys that are read once a sequence.  Own keys then begin
+      // with a stage that lies in one page; from anywhere else they would be staged row by row (64 sequences on 9 pictures: 86 us a
+      // layer instead of 82).
+      const int lead = s_lead[b], shared = s_members[lead] >= 2 ? min(s_shortest[lead], s_longest[lead]) / kUnit * kUnit : 0;
+      const bool shares = s_tok[b] > 0 && s_id[b] > 0 && shared > 0;
+      s_shared[b] = shares ? shared : 0;
+      if (!shares) s_rank[b] = 0;
+      if (!shares || lead != b) s_count[b] = 0;
+      if (turn == 0 && mixed(b)) s_turn[0] = 1;
+    }
+    __syncthreads();
+    if (turn == 1 || s_turn[0] == 0) break;
+
+    // The shortest prefix length is what all of a group share.  Where lengths differ, those take part whose length is at least the
+    // one that spares most keys, length * (members of that length or more - 1), and the others share with nobody: a single short one
+    // would leave the others little or nothing.  The members of such groups, sorted by leader and length, say how many there are; the second
+    // turn makes the groups without those that were left out.  (16 sequences of one group 8.8 us where lengths are alike, 128 of four
+    // 12.0, and 20.9 where a fifth of them is short.)
+    int* const s_sorted = s_n;  // as many as the next power of two, below 2 B, of the 7 B behind it
+    int n_sort = 1;
+    while (n_sort < a.B) n_sort *= 2;
+    const auto of_mixed = [&](int b) { return s_id[b] > 0 && s_tok[b] > 0 && mixed(s_lead[b]); };
+    constexpr int kLengthBits = 16;
+    static_assert(kMaxContext / kUnit < 1 << kLengthBits && kMaxSequences < 1 << (31 - kLengthBits), "leader and length are one int");
+    for (int b = tid; b < a.B; b += n_thr) {
+      s_best[b] = 0;
+      s_cut[b] = INT32_MAX;
+    }
+    for (int i = tid; i < n_sort; i += n_thr) s_sorted[i] = i < a.B && of_mixed(i) ? s_lead[i] << kLengthBits | usable(i) : INT32_MAX;
+    __syncthreads();
+    for (int k = 2; k <= n_sort; k *= 2)
+      for (int j = k / 2; j > 0; j /= 2) {
+        for (int i = tid; i < n_sort; i += n_thr) {
+          const int at = i ^ j;
+          if (at < i) continue;
+          const int x = s_sorted[i], y = s_sorted[at];
+          if ((x > y) == ((i & k) == 0)) {
+            s_sorted[i] = y;
+            s_sorted[at] = x;
+          }
+        }
+        __syncthreads();
+      }
+    const auto spared = [&](int i, int* lead, int* units) {  // by the length at place i
+      *lead = s_sorted[i] >> kLengthBits, *units = s_sorted[i] & ((1 << kLengthBits) - 1);
+      int begin = 0, end = i;  // the leader's first place
+      while (begin < end) {
+        const int mid = (begin + end) >> 1;
+        if (s_sorted[mid] >= *lead << kLengthBits) end = mid; else begin = mid + 1;
+      }
+      return *units * (begin + s_members[*lead] - i - 1);
+    };
+    int lead, units;
+    for (int i = tid; i < a.B; i += n_thr)
+      if (s_sorted[i] != INT32_MAX) {
+        const int keys = spared(i, &lead, &units);
+        atomicMax(&s_best[lead], keys);
+      }
+    __syncthreads();
+    for (int i = tid; i < a.B; i += n_thr)
+      if (s_sorted[i] != INT32_MAX && spared(i, &lead, &units) == s_best[lead]) atomicMin(&s_cut[lead], units);
+    __syncthreads();
+    for (int b = tid; b < a.B; b += n_thr)
+      if (of_mixed(b) && usable(b) < s_cut[s_lead[b]]) {
+        s_id[b] = 0;
+        s_turn[1] = 1;
+      }
+    __syncthreads();
+    if (s_turn[1] == 0) break;
+    for (int b = tid; b < a.B; b += n_thr) {
+      s_lead[b] = b;
+      s_rank[b] = s_count[b] = s_members[b] = s_longest[b] = s_furthest[b] = 0;
+      s_shortest[b] = INT32_MAX;
+    }
+    __syncthreads();
   }
-  __syncthreads();
-  for (int b = tid; b < a.B; b += n_thr) {
-    if (s_id[b] == 0 || s_tok[b] == 0) continue;
-    const int lead = s_lead[b];
-    atomicAdd(&s_count[lead], s_tok[b]);
-    atomicAdd(&s_members[lead], 1);
-    atomicMin(&s_shortest[lead], s_len[b]);
-    atomicMax(&s_longest[lead], s_keys[b]);
-  }
-  __syncthreads();
-  for (int b = tid; b < a.B; b += n_thr) {
-    // Whole units: what is behind them counts as each one's own, up to 63 keys that are read once a sequence.  Own keys then begin
-    // with a stage that lies in one page; from anywhere else they would be staged row by row (64 sequences on 9 pictures: 86 us a
-    // layer instead of 82).
-    const int lead = s_lead[b], shared = s_members[lead] >= 2 ? min(s_shortest[lead], s_longest[lead]) / kUnit * kUnit : 0;
-    const bool shares = s_tok[b] > 0 && s_id[b] > 0 && shared > 0;
-    s_shared[b] = shares ? shared : 0;
-    if (!shares) s_rank[b] = 0;
-    if (!shares || lead != b) s_count[b] = 0;
-  }
-  __syncthreads();
 
   const auto lead_for = [&](int tokens) { return lead_of(tokens * a.group); };
   const auto tiles_of = [&](int tokens) { return (tokens * a.group + kTileRows - 1) / kTileRows; };

@@ -600,6 +600,8 @@ int fp_copy_pages(void* pool, const int64_t* src, const int64_t* dst, const int3
  *              max_context - 1); every such key is in the cache already.  input_pos < 0: no token, out = 0, lse = -inf
  *   prefix_ids, prefix_lens  [max_batch] int32 by cache slot: slots with the same id > 0 have the same keys and values at the positions
  *              0 .. (smallest of their prefix_lens) - 1, be it in the same pages or in copies of them.  An id <= 0 shares with nobody
+ *              Where the lengths of three or more sequences with one id differ, those share whose length is at least the one that
+ *              spares most keys; lengths count in whole units of 64 keys
  *   out        [B, Hq, S, D], element strides (b, h, s); lse [B, Hq, S] float32 contiguous
  *   sinks, scale, page_table, batch_idx, pool_k, pool_v, n_slots  as fp_paged_decode
  * Results are those of fp_paged_decode for each token, up to the order of the sums and, behind a sink gate, one rounding instead of
