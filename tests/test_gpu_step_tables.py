@@ -328,3 +328,24 @@ def test_under_inference_mode():
     assert not made.batch_idx.is_inference()
     made.batch_idx[0] = 5  # an ordinary tensor
     assert made.batch_idx._version == 1 or made.batch_idx.requires_grad is False
+
+
+@pytest.mark.parametrize("B,rows,native", [(1, 0, True), (3, 7, True), (20, 3001, True), (21, 3002, True), (5, 4, False), (33, 1001, False)])
+def test_the_returned_tensors_are_apart(monkeypatch, B, rows, native):
+    """Nine tensors in two allocations: writing to one changes none of the others, and each counts its own versions."""
+    slots, old, new, par, free, count, table = make(12, B, old_hi=200, add_hi=1 if rows < 100 else 40, P=16)
+    if rows < 100:
+        new = list(old)
+    if not native:
+        monkeypatch.setattr(ops, "_current", lambda t: -1)
+    dev = lambda x, t: torch.tensor(x, dtype=t, device="cuda")
+    made = ops.step_tables(dev(slots, torch.int64), dev(old, torch.int32), dev(new, torch.int32), dev(free, torch.int64), dev([count], torch.int32),
+                           table.cuda(), 16, rows).check()
+    sizes = dict(batch_idx=rows, input_pos=rows, slot_map=rows, row_starts=B + 1, free_left=1, copy_src=B, copy_dst=B, copy_rows=B, status=1)
+    for i, (name, t) in enumerate(made._asdict().items()):
+        assert t.shape == (sizes[name],) and t._version == 0
+        before = [x.clone() for x in made]
+        t.fill_(i + 70)
+        assert t._version == 1 and bool((t == i + 70).all())
+        for j, (x, y) in enumerate(zip(made, before)):
+            assert j == i or (torch.equal(x, y) and x._version == (j < i))
