@@ -83,3 +83,59 @@ def test_a_first_use_inside_a_capture_clears_nothing_in_replays():
         assert bool((workspace[-4096:] == 0x5b).all()) and bool((plan[-256:] == 0x5b).all())
         want = step()
         assert torch.equal(out, want) and bool(torch.isfinite(want).all())
+
+
+@pytest.mark.parametrize("dtype,D,heads,rep", [(torch.bfloat16, 128, 16, 2), (torch.float16, 64, 8, 4), (torch.float32, 64, 4, 2)])
+@pytest.mark.parametrize("graph", [False, True])
+def test_a_cache_whose_heads_are_copies(dtype, D, heads, rep, graph):
+    """One cached head a query head, V (and K) the same in groups of `kv_rep`, as an engine caches them; the append left to the attention."""
+    s = Server(Hc=heads, Hq=heads, D=D, dtype=dtype, kv_rep=rep, fuse_decode_append=True, layers=2, seed=12)
+    rnd = s.rnd
+
+    def copies(*shape):  # rows of K and V: groups of heads are alike; [.., heads, tokens, D]
+        if len(shape) == 4 and shape[1] == heads:
+            return rnd(shape[0], heads // rep, *shape[2:]).repeat_interleave(rep, 1)
+        return rnd(*shape)
+
+    s.rnd = copies
+    cat, dog = s.picture(133), s.picture(70)
+    idx = [cat, *s.fork(cat, 133, 4), dog, *s.fork(dog, 64, 2)]
+    s.extend(idx, [1 + 5 * i for i in range(len(idx))])
+    assert s.cache.v_copies_are_identical(0) and s.cache.v_copies_are_identical(1)
+    if not graph:
+        for batch in (idx, idx[::-1], idx[2:4]):
+            s.decode(batch)
+        s.check_pool()
+        return
+    lens = [s.length(x) for x in idx]
+    for x, n in zip(idx, lens):
+        s.cache.reserve(x, None, n + 3)
+    pos = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    mask, ids = s.mask(idx, pos), torch.tensor(idx, device=DEV)
+    q, k, v = (torch.zeros(2, len(idx), heads, 1, D, dtype=dtype, device=DEV) for _ in range(3))
+
+    def step():
+        got = []
+        for layer in range(2):
+            K, V = s.cache.insert_kv(layer, k[layer], v[layer], input_pos=pos.view(-1, 1), batch_idx=ids)
+            out, aux = A.compiled_flex_attn_decode(q[layer], K, V, block_mask=mask, return_aux=AuxRequest(lse=True))
+            got.append((out, aux.lse))
+        return got
+
+    step()
+    torch.cuda.synchronize()
+    captured = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(captured):
+        made = step()
+    for turn in range(3):
+        for t in (q, k, v):
+            for layer in range(2):
+                t[layer].copy_(s.rnd(len(idx), heads, 1, D))
+        captured.replay()
+        torch.cuda.synchronize()
+        for layer in range(2):
+            for i, x in enumerate(idx):
+                s.keys[x][layer] = tuple(torch.cat([old, new[layer, i].cpu()], 1) for old, new in zip(s.keys[x][layer], (k, v)))
+            s.expected(q[layer].cpu(), [s.keys[x][layer] for x in idx], pos.cpu()).check(made[layer])
+        pos.add_(1)
+    s.check_pool()
