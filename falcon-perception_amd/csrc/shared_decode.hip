@@ -59,7 +59,6 @@ typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef short s16x8 __attribute__((ext_vector_type(8)));
 
 // ------------------------------------------------------------------------------------------------------------ plan
 // ints: header, sequences, tokens of the groups and of the other sequences, each token's place, workgroups, tiles
@@ -666,11 +665,9 @@ struct BF16 {
     hi = __builtin_amdgcn_perm(b1, b0, 0x07060302);
     lo = pack2(fmaf(p0, 1.f + 0x1p-23f, -__uint_as_float(b0 & 0xffff0000u)), fmaf(p1, 1.f + 0x1p-23f, -__uint_as_float(b1 & 0xffff0000u)));
   }
-  static __device__ __forceinline__ float round(float v) { return static_cast<float>(static_cast<__bf16>(v)); }
 };
 struct F16 {
   using type = _Float16;
-  typedef _Float16 vec4 __attribute__((ext_vector_type(4)));
   typedef _Float16 vec8 __attribute__((ext_vector_type(8)));
   static constexpr int kBytes = 2;
   static __device__ __forceinline__ bool drop_infinities(uint32_t& w) {
@@ -688,14 +685,16 @@ struct F16 {
     const vec2 v = {static_cast<_Float16>(lo), static_cast<_Float16>(hi)};
     return __builtin_bit_cast(uint32_t, v);
   }
-  // As above.  Neither part of a p above 0 is below the smallest number of the type, 2^-32 of the largest p.
+  // As above.  Neither part of a p above 0 is below the smallest number of the type, 2^-24, where a wavefront's largest p is 2^8 or more
+  // (kHeadroom): each key of vanishing weight counts for up to 2^-31 of the largest one's.  A wavefront has a quarter of a piece's stages,
+  // so in a context of n keys they come to n * 2^-33 of the largest |V| at most, 2^-12 at kMaxContext, half of what rounding an f16 of
+  // that size may cost.
   static __device__ __forceinline__ void split(float p0, float p1, uint32_t& hi, uint32_t& lo) {
     const float l0 = fminf(p0 * 0x1p+102f, 0x1p-24f), l1 = fminf(p1 * 0x1p+102f, 0x1p-24f);
     const auto h = __builtin_amdgcn_cvt_pkrtz(fmaxf(p0, l0), fmaxf(p1, l1));
     hi = __builtin_bit_cast(uint32_t, h);
     lo = pack2(fmaxf(p0 - static_cast<float>(h[0]), l0), fmaxf(p1 - static_cast<float>(h[1]), l1));
   }
-  static __device__ __forceinline__ float round(float v) { return static_cast<float>(static_cast<_Float16>(v)); }
 };
 struct F32 {
   using type = float;
@@ -706,7 +705,6 @@ struct F32 {
     if (odd) w = 0;
     return odd;
   }
-  static __device__ __forceinline__ float round(float v) { return v; }
 };
 
 __device__ __forceinline__ s16x4 lds_read_tr(const char* p) {

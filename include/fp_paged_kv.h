@@ -609,9 +609,12 @@ int fp_copy_pages(void* pool, const int64_t* src, const int64_t* dst, const int3
  * is read through the table row of any of the sequences.
  *
  * fp_shared_decode_plan, once per step, finds the sequences that share and cuts the work; every layer's fp_paged_decode_shared with the
- * same B, S, Hq, Hc, D and max_context takes the plan.  batch_idx, input_pos and the rows of page_table must not change in between: a launch
- * that meets a plan of another shape, or of other slots or positions for a row, leaves NaN in out and lse there.
+ * same B, S, Hq, Hc, D and max_context takes the plan.  batch_idx, input_pos and the rows of page_table must not change in between.  A launch
+ * that meets a plan of another shape leaves NaN in out and lse; one whose sequence has another slot than the plan's, a token where the
+ * plan has none or a position behind all that the plan has for it leaves NaN in that row.  Positions in front of the planned ones are served
+ * as they are.
  * Plan and workspace are memory of the caller (16-byte aligned), one launch at a time; nothing in them needs clearing.
+ * Of f16, keys of vanishing weight come to at most n * 2^-33 of the largest |V| in a context of n keys (2^-12 at 2^21).
  * Hq / Hc in {1, 2, 4, 8}, D in {64, 128}, B <= 1536, B * S * Hq / Hc <= 2^20, max_context <= 2^21.  Both may be captured in a graph.
  */
 int64_t fp_shared_decode_plan_bytes(int32_t B, int32_t S, int32_t Hq, int32_t Hc, int32_t D);

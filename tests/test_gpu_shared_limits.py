@@ -164,3 +164,34 @@ def test_few_sequences_cut_into_many_pieces(D, Hq, Hc, dtype):
 def test_several_tokens_of_one_sequence_over_many_keys():
     case = SharedBatch(48, [], [(-1, 15000, 5)], Hq=4, Hc=2, D=128, P=128, dtype=BF16).on()
     case.check(case.call(ops))
+
+
+def test_the_longest_context_in_half_precision():
+    """2^21 keys in f16, all V but the marked ones 1.  A key of vanishing weight keeps 2^-23 beside a largest one of 2^8 or more in its
+    wavefront, which has a quarter of the keys or less: all of them together are below 2^21 / 4 * 2^-31 = 2^-12 of what they weigh."""
+    P, D, G, L = 128, 64, 8, 1 << 21
+    blocks = L // P
+    pool = torch.zeros(2, 1, (1 + blocks) * P, D, dtype=F16, device="cuda")
+    pool[1, 0, P:] = 1
+    pages = torch.randperm(blocks, generator=torch.Generator(device="cuda").manual_seed(49), device="cuda") + 1
+    table = torch.zeros(3, blocks, dtype=torch.int64, device="cuda")
+    table[1:] = pages  # both the same sequence, all of it shared
+    row = lambda t: int(table[1, t // P]) * P + t % P
+    marks = [0, 1, 1024 * P - 1, 1024 * P, L // 2 + 5, L - 130, L - 2, L - 1]
+    q = torch.zeros(2, G, 1, D, dtype=F16, device="cuda")
+    values = torch.linspace(-3, 3, D, dtype=torch.float64).to(F16)
+    for h, t in enumerate(marks):
+        q[:, h, 0, h] = 16
+        pool[0, 0, row(t), h] = 20  # 40 above all others
+        pool[1, 0, row(t)] = values.cuda() * (h - 4)
+    args = (table, torch.tensor([1, 2], device="cuda"), torch.tensor([L - 1, L - 1], device="cuda"))
+    for ids in ([0, 9, 9], [0, 0, 0]):
+        got, lse = ops.paged_decode_shared(q, pool[0], pool[1], *args, torch.tensor(ids, dtype=torch.int32, device="cuda"),
+                                           torch.tensor([0, L, L], dtype=torch.int32, device="cuda"), P, L)
+        for h in range(G):
+            want = (values * (h - 4)).double()
+            # the weights of all others; exponential, quotient and sums; half a step of the type
+            tol = 2.0 ** -12 + (HALF_STEP[F16] + 2.0 ** -19) * want.abs()
+            for b in range(2):
+                assert bool(((got[b, h, 0].double().cpu() - want).abs() <= tol).all()), (b, h)
+                assert abs(float(lse[b, h, 0]) - 40) <= 40 * 2.0 ** -20
