@@ -8,7 +8,7 @@
 //   row start_b + j -> (slot_b, old_b + j, page * P + position % P)
 //
 // Bound by latency for a decode step (one launch: load, scan, store) and by the stores of the rows (20 bytes each) for an
-// admission step.  One launch: every workgroup works out the sums of all requests by itself - 20 bytes a request, from L2 -
+// admission step.  One launch: every workgroup works out the sums of all requests by itself - 16 to 32 bytes a request, from L2 -
 // instead of waiting for a launch that does; nothing that one workgroup writes is read by another.  64 requests of one token: 6.0 us;
 // 48 forks, 16 thousand rows: 7.0; 1000 requests, 2 million rows, 41 MB: 20.2, about 8
 // of them before the first row.
