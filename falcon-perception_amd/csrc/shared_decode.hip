@@ -285,21 +285,22 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
       // Whole units: what is behind them counts as each one's own, up to 63 keys that are read once a sequence.  Own keys then begin
       // with a stage that lies in one page; from anywhere else they would be staged row by row (64 sequences on 9 pictures: 86 us a
       // layer instead of 82).
-      const int lead = s_lead[b], shared = s_members[lead] >= 2 ? min(s_shortest[lead], s_longest[lead]) / kUnit * kUnit : 0;
+      const int lead = s_lead[b], members = s_members[lead], shortest = s_shortest[lead], longest = s_longest[lead], furthest = s_furthest[lead];
+      const int shared = members >= 2 ? min(shortest, longest) / kUnit * kUnit : 0;
       const bool shares = s_tok[b] > 0 && s_id[b] > 0 && shared > 0;
       s_shared[b] = shares ? shared : 0;
       if (!shares) s_rank[b] = 0;
       if (!shares || lead != b) s_count[b] = 0;
-      if (turn == 0 && mixed(b)) s_turn[0] = 1;
+      if (turn == 0 && members > 2 && shared < min(furthest, longest) / kUnit * kUnit) s_turn[0] = 1;
     }
     __syncthreads();
-    if (turn == 1 || s_turn[0] == 0) break;
+    if (__builtin_expect(turn == 1 || s_turn[0] == 0, 1)) break;
 
     // The shortest prefix length is what all of a group share.  Where lengths differ, those take part whose length is at least the
     // one that spares most keys, length * (members of that length or more - 1), and the others share with nobody: a single short one
     // would leave the others little or nothing.  The members of such groups, sorted by leader and length, say how many there are; the second
-    // turn makes the groups without those that were left out.  (16 sequences of one group 8.8 us where lengths are alike, 128 of four
-    // 12.0, and 20.9 where a fifth of them is short.)
+    // turn makes the groups without those that were left out.  (The plan of 128 sequences of four groups: 11.8 us where lengths are alike,
+    // 21.2 where a fifth of them is short; of 1536 282 and 518.)
     int* const s_sorted = s_n;  // as many as the next power of two, below 2 B, of the 7 B behind it
     int n_sort = 1;
     while (n_sort < a.B) n_sort *= 2;
