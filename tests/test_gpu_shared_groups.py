@@ -167,3 +167,36 @@ def test_questions_about_pictures_behind_one_prompt_decode():
     s.forget(system)
     s.decode(everyone)
     s.check_pool()
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_a_server_with_forks_of_forks(seed):
+    """Any order of pictures, forks, prompts, decode steps and releases; every step against float64, the pool at the end."""
+    r = random.Random(seed)
+    s = Server(n_pages=300, slots=26, P=r.choice([16, 32, 48]), layers=2, dtype=r.choice([torch.bfloat16, torch.float16, torch.float32]), seed=seed)
+    room = 16 * s.P - 8
+    for _ in range(40):
+        live, what = list(s.keys), r.random()
+        pages = s.cache.num_free_pages
+        if not live or (what < 0.12 and len(live) < 20 and pages > 40):
+            s.picture(r.randrange(1, 2 * room // 3))
+        elif what < 0.45 and len(live) < 20 and pages > 40:
+            parent = r.choice(live)
+            n = s.length(parent) - (r.randrange(s.length(parent)) if r.random() < 0.4 else 0)
+            s.fork(parent, n, r.randrange(1, min(5, 25 - len(live))))
+        elif what < 0.6 and pages > 60:
+            some = [x for x in r.sample(live, min(len(live), 4)) if s.length(x) < room - 30]
+            if some:
+                s.extend(some, [r.randrange(0, 30) for _ in some], row_multiple=r.choice([1, 8]))
+        elif what < 0.85:
+            batch = [x for x in live if s.length(x) < room]
+            r.shuffle(batch)
+            if batch and pages >= len(batch):
+                s.decode(batch[:r.randrange(1, len(batch) + 1)])
+        else:
+            s.forget(r.choice(live))
+    s.check_pool()
+    for x in list(s.keys):
+        s.forget(x)
+    assert not s.cache._page_slots and not s.cache._prefixes and not s.cache.prefix_ids.any()
+    assert sorted(s.cache.free_pages) == list(range(1, 300))
