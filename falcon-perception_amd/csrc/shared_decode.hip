@@ -47,6 +47,7 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kMaxSequences = 1536;
 constexpr int kMaxRows = 1 << 20;      // B * S * heads of a group
+constexpr int kTreeTokens = 64;        // bits of a mask
 constexpr int kMaxContext = 1 << 21;   // with the rows: units of all tiles fit 31 bits
 constexpr int kTileRows = 64;
 constexpr int kUnit = 64;              // keys: what the cut is made of
@@ -130,7 +131,7 @@ struct PlanArgs {
   const int64_t* batch_idx;
   const void* input_pos;
   int pos_i64;
-  const int32_t* ids;
+  const int32_t* ids;  // null: no two sequences share keys
   const int32_t* lens;
   int B, S, Hq, Hc, group, max_batch, max_context, n_wg;
   char* plan;
@@ -221,7 +222,7 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
     const int64_t slot = b < a.B ? a.batch_idx[b] : -1;
     const bool valid = slot >= 0 && slot < a.max_batch;
     const int keys = a.S == 1 && valid ? plan_keys(a, b, 0) : 0;
-    const int id = valid ? max(a.ids[slot], 0) : 0, length = valid ? max(a.lens[slot], 0) : 0;
+    const int id = valid && a.ids ? max(a.ids[slot], 0) : 0, length = valid && a.ids ? max(a.lens[slot], 0) : 0;
     s_id[b] = length >= kUnit ? id : 0;
     s_len[b] = length;
     s_keys[b] = keys;
@@ -636,6 +637,7 @@ struct SharedArgs {
   int64_t seqs, tokens, place, shares, tiles;
   float* ws_acc;  // [part rows, Hc, D]
   float* ws_ml;   // [part rows, Hc, 2]
+  const int64_t* masks;  // [B, S], of a tree of drafts: bit i is the key of draft i
 };
 
 struct BF16 {
@@ -761,7 +763,22 @@ __device__ __forceinline__ int keys_of(const SharedArgs& a, int b, int j) {
   return p < 0 ? 0 : p > a.max_context ? a.max_context : static_cast<int>(p);
 }
 
-template <typename E, int D>
+// Trees of drafts: token j of a sequence is the key at position input_pos[b, j], so draft 0 is the one at input_pos[b, j] - j, and all keys
+// in front of that are seen by every token.  Of the drafts it sees those whose bits its mask has, up to its own.
+__device__ __forceinline__ int tree_base(int64_t pos, int j) {
+  return pos < j ? 0 : pos - j > INT32_MAX ? INT32_MAX : static_cast<int>(pos - j);
+}
+
+// Whether token j of sequence b, which is there, sees a key: with `keys` of the cache in front of it and itself
+template <bool kTree>
+__device__ __forceinline__ bool sees_any(const SharedArgs& a, int b, int j, int keys) {
+  if (!kTree || keys <= 0) return keys > 0;
+  const int64_t at = static_cast<int64_t>(b) * a.S + j;
+  const int base = tree_base(fp::load_index(a.input_pos, at, a.pos_i64), j);
+  return base > 0 || (static_cast<uint64_t>(a.masks[at]) << (64 - min(keys, 64))) != 0;
+}
+
+template <typename E, int D, bool kTree>
 struct Shared {
   using G = Geo<E, D>;
   __attribute__((aligned(1024))) char ring[kWaves][G::RING];
@@ -769,6 +786,8 @@ struct Shared {
   __attribute__((aligned(8))) float ml[kWaves][kTileRows][2];
   float joined[kTileRows][2];    // maximum and sum of all wavefronts
   int limit[kWaves][kTileRows];  // keys of the columns' rows, each wavefront's own copy
+  int base[kTree ? kWaves : 1][kTree ? kTileRows : 1];  // of a tree: keys in front of the drafts, and the drafts they see
+  __attribute__((aligned(8))) uint64_t mask[kTree ? kWaves : 1][kTree ? kTileRows : 1];
   __attribute__((aligned(16))) v4u q_tail[G::QTAIL ? 4 * 64 : 1];  // last quarter of the query rows, by column block and lane
   int tainted;  // an element of V that is not finite was left out
 };
@@ -798,13 +817,21 @@ __device__ __forceinline__ void find_row(const SharedArgs& a, const Tile& tile, 
 }
 
 // What the products left out of row r: the infinities and NaN of the V rows of keys [t0, t1) that it sees, elements 4 c .. 4 c + 3.
-template <typename E, int D>
+template <typename E, int D, bool kTree>
 __device__ __forceinline__ void add_infinities(const SharedArgs& a, const Tile& tile, int r, int t0, int t1,
                                                          const char* vplane, int c, f32x4& num) {
   int b, j, g;
   find_row(a, tile, r, &b, &j, &g);
   const int end = min(t1, keys_of(a, b, j));
+  int base = INT32_MAX;
+  uint64_t mask = 0;
+  if constexpr (kTree) {
+    const int64_t at = static_cast<int64_t>(b) * a.S + j;
+    base = tree_base(fp::load_index(a.input_pos, at, a.pos_i64), j);
+    mask = a.masks[at];
+  }
   for (int t = t0; t < end; ++t) {
+    if (kTree && t >= base && !(mask >> (t - base) & 1)) continue;
     int64_t blk;
     int off;
     a.pd.split(t, blk, off);
@@ -824,8 +851,8 @@ __device__ __forceinline__ void add_infinities(const SharedArgs& a, const Tile& 
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory"); }
 
 // One piece: the rows of a tile over its keys [t0, t1).  CB blocks of 16 columns.
-template <typename E, int D, int CB>
-__device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh, const int wave, const Tile& tile, const int piece,
+template <typename E, int D, bool kTree, int CB>
+__device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D, kTree>& sh, const int wave, const Tile& tile, const int piece,
                                           const int t0, const int t1) {
   using G = Geo<E, D>;
   const int hc = blockIdx.x;
@@ -852,7 +879,9 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
   constexpr bool kTail = CB == 4 && G::QTAIL;
   constexpr int QR = kTail ? G::QV - 1 : G::QV;
   v4u q[CB][QR], tail = {0, 0, 0, 0};
-  int64_t pos[CB];
+  int64_t pos[kTree ? 1 : CB];  // of a tree: a row a lane, whose limit, base and mask it brings to LDS
+  uint64_t mask = 0;
+  int draft = 0;
   int least = INT32_MAX;
   {
     // two trips to memory: the tokens, then what they name
@@ -866,8 +895,14 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
       x[cb] = tile.row0 + (r < tile.n_rows ? r : 0);
       token[cb] = tokens[x[cb] >> a.group_shift];
     }
-    const auto at = [&](int cb) { return static_cast<int64_t>(token[cb] >> kTokenShift) * a.S + (token[cb] & ((1 << kTokenShift) - 1)); };
-    if (a.pos_i64) {
+    const auto place = [&](int token) { return static_cast<int64_t>(token >> kTokenShift) * a.S + (token & ((1 << kTokenShift) - 1)); };
+    const auto at = [&](int cb) { return place(token[cb]); };
+    if constexpr (kTree) {
+      const int mine = tokens[(tile.row0 + (lane < tile.n_rows ? lane : 0)) >> a.group_shift];
+      pos[0] = fp::load_index(a.input_pos, place(mine), a.pos_i64);
+      mask = a.masks[place(mine)];
+      draft = mine & ((1 << kTokenShift) - 1);
+    } else if (a.pos_i64) {
 #pragma unroll
       for (int cb = 0; cb < CB; ++cb) pos[cb] = static_cast<const int64_t*>(a.input_pos)[at(cb)];
     } else {
@@ -967,13 +1002,23 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
     if (wave + kWaves < n_stages) issue(locate(seg0 + (wave + kWaves) * G::TS), seg0 + (wave + kWaves) * G::TS, lds_ring + 2 * G::HALF);
     if (seg0 == t0) {  // the rows' limits, now that the first stages are on their way
       const int lane = lane_id(), col = lane & 15, max_context = a.max_context;
+      const auto limit_of = [&](int64_t p, int r) {
+        const int64_t keys = p < 0 ? 0 : p >= max_context ? max_context : p + 1;
+        return r < tile.n_rows ? static_cast<int>(keys) : INT32_MAX;
+      };
+      if constexpr (kTree) {
+        const int lim = limit_of(pos[0], lane), base = lane < tile.n_rows ? tree_base(pos[0], draft) : INT32_MAX;
+        least = min(lim, base);
+        sh.limit[wave][lane] = lim;
+        sh.base[wave][lane] = base;
+        sh.mask[wave][lane] = mask;
+      } else {
 #pragma unroll
-      for (int cb = 0; cb < CB; ++cb) {
-        const int r = cb * 16 + col;
-        const int64_t keys = pos[cb] < 0 ? 0 : pos[cb] >= max_context ? max_context : pos[cb] + 1;
-        const int lim = r < tile.n_rows ? static_cast<int>(keys) : INT32_MAX;
-        least = min(least, lim);
-        if (lane < 16) sh.limit[wave][cb * 16 + col] = lim;
+        for (int cb = 0; cb < CB; ++cb) {
+          const int lim = limit_of(pos[cb], cb * 16 + col);
+          least = min(least, lim);
+          if (lane < 16) sh.limit[wave][cb * 16 + col] = lim;
+        }
       }
       least = -fp::wave_max(-least);
       if constexpr (kTail) {
@@ -1032,10 +1077,21 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
         for (int cb = 0; cb < CB; ++cb) {
           const int end = min(sh.limit[wave][cb * 16 + (lane_now & 15)], seg1);
 #pragma unroll
-          for (int blk = 0; blk < G::NB; ++blk)
+          for (int blk = 0; blk < G::NB; ++blk) {
+            uint32_t seen = 15;  // of this lane's four keys
+            if constexpr (kTree) {
+              const int ahead = c0 + blk * 16 + (lane_now >> 4) * 4 - sh.base[wave][cb * 16 + (lane_now & 15)];
+              const uint64_t mask = sh.mask[wave][cb * 16 + (lane_now & 15)];
+              // (at 64 and beyond the limit hides them)
+              if (ahead >= 0)
+                seen = static_cast<uint32_t>(mask >> min(ahead, 63));
+              else if (ahead > -4)
+                seen = static_cast<uint32_t>(mask << -ahead) | ((1u << -ahead) - 1);
+            }
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-              if (c0 + blk * 16 + (lane_now >> 4) * 4 + j >= end) sc[cb][blk][j] = -INFINITY;
+              if (c0 + blk * 16 + (lane_now >> 4) * 4 + j >= end || (kTree && !(seen >> j & 1))) sc[cb][blk][j] = -INFINITY;
+          }
         }
         // V rows past the range become 0: a probability of 0 against an infinity would be NaN.  So do the elements that are not
         // finite of rows which only some columns see; these columns get them at the end.
@@ -1235,7 +1291,7 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
       for (int k = 0; k < kTurns; ++k)
         if (r0 + k * kStep < tile.n_rows) {
           f32x4 more = {0.f, 0.f, 0.f, 0.f};
-          add_infinities<E, D>(e, tile, r0 + k * kStep, max(t0, least), t1, e.pool_v + static_cast<int64_t>(hc) * e.n_slots * G::ROWB, c, more);
+          add_infinities<E, D, kTree>(e, tile, r0 + k * kStep, max(t0, least), t1, e.pool_v + static_cast<int64_t>(hc) * e.n_slots * G::ROWB, c, more);
 #pragma unroll
           for (int n = 0; n < kTurns; ++n)
             if (n == k) num[n] += more;
@@ -1248,7 +1304,7 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D>& sh,
         int b, j, g;
         find_row(e, tile, r0 + k * kStep, &b, &j, &g);
         const int h = hc * e.group + g;
-        const bool any = keys_of(e, b, j) > 0;
+        const bool any = sees_any<kTree>(e, b, j, keys_of(e, b, j));
         const float lse = (ml[k].x + log2f(ml[k].y)) * kLn2;
         f32x4 res;
 #pragma unroll
@@ -1288,9 +1344,9 @@ __device__ __forceinline__ T load_record(const char* p) {
   return t;
 }
 
-template <typename E, int D>
-__global__ __launch_bounds__(kThreads, (sizeof(Shared<E, D>) <= 80 * 1024 ? 2 : 1)) void shared_products_kernel(const SharedArgs a) {
-  __shared__ Shared<E, D> sh;
+template <typename E, int D, bool kTree>
+__global__ __launch_bounds__(kThreads, (sizeof(Shared<E, D, kTree>) <= 80 * 1024 ? 2 : 1)) void shared_products_kernel(const SharedArgs a) {
+  __shared__ Shared<E, D, kTree> sh;
   const int w = blockIdx.y;
   const Header h = load_record<Header>(a.plan);
   const Share share = load_record<Share>(a.plan + a.shares + w * static_cast<int64_t>(sizeof(Share)));
@@ -1309,11 +1365,11 @@ __global__ __launch_bounds__(kThreads, (sizeof(Shared<E, D>) <= 80 * 1024 ? 2 : 
       if (busy) lds_barrier();  // the piece before has left LDS
       busy = true;
       if (t.n_rows <= 16)
-        run_piece<E, D, 1>(a, sh, wave, t, piece, t0, t1);
+        run_piece<E, D, kTree, 1>(a, sh, wave, t, piece, t0, t1);
       else if (t.n_rows <= 32)
-        run_piece<E, D, 2>(a, sh, wave, t, piece, t0, t1);
+        run_piece<E, D, kTree, 2>(a, sh, wave, t, piece, t0, t1);
       else
-        run_piece<E, D, 4>(a, sh, wave, t, piece, t0, t1);
+        run_piece<E, D, kTree, 4>(a, sh, wave, t, piece, t0, t1);
     }
     i = t.next;
     if (left <= 0 || i >= h.n_tiles) break;
@@ -1330,7 +1386,7 @@ constexpr int kBatch = 8;
 // Up to here a row a workgroup: 4 sequences on a prefix of 16000 keys, 64 pieces a row, 16 heads, D 128: a layer 28.3 -> 20.7 us; with pieces in
 // one batch it costs 0.2 us a layer (16 sequences, 256 rows) and with 6144 rows 10.
 constexpr int kWideRows = 2048;
-template <typename E, int D, bool kWide>
+template <typename E, int D, bool kWide, bool kTree>
 __global__ __launch_bounds__(kThreads) void shared_join_kernel(const SharedArgs a) {
   constexpr int LPR = D / 4, kGroups = kThreads / LPR, kRowsHere = kWide ? 1 : kGroups;
   __shared__ float2 s_ml[kGroups];
@@ -1352,7 +1408,7 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(const SharedArgs 
   const bool missing = at_b < 0;
   // of another step: the plan
   const bool foreign = !fits || (valid && (s.slot != slot || keys > s.keys || (keys > 0 && missing))) || (!valid && s.slot >= 0);
-  const bool any = !foreign && valid && keys > 0;
+  const bool any = !foreign && valid && sees_any<kTree>(a, b, j, keys);
   float m = -INFINITY, den = 0.f;
   f32x4 num = {0.f, 0.f, 0.f, 0.f};
   bool shared_out = false;
@@ -1449,17 +1505,17 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(const SharedArgs 
   if (c == 0) a.lse[(static_cast<int64_t>(b) * a.Hq + h) * a.S + j] = lse;
 }
 
-template <typename E, int D>
+template <typename E, int D, bool kTree>
 void launch(const SharedArgs& a, int n_wg, hipStream_t st) {
-  hipLaunchKernelGGL((shared_products_kernel<E, D>), dim3(a.Hc, n_wg), dim3(kThreads), 0, st, a);
+  hipLaunchKernelGGL((shared_products_kernel<E, D, kTree>), dim3(a.Hc, n_wg), dim3(kThreads), 0, st, a);
   const int64_t rows = static_cast<int64_t>(a.B) * a.S * a.Hq;
   const auto join = [&](auto kernel, int here) {
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((rows + here - 1) / here)), dim3(kThreads), 0, st, a);
   };
   if (rows <= kWideRows)
-    join(shared_join_kernel<E, D, true>, 1);
+    join(shared_join_kernel<E, D, true, kTree>, 1);
   else
-    join(shared_join_kernel<E, D, false>, kThreads / (D / 4));
+    join(shared_join_kernel<E, D, false, kTree>, kThreads / (D / 4));
 }
 
 int check_shape(const char* what, int B, int S, int Hq, int Hc, int D) {
@@ -1487,11 +1543,12 @@ extern "C" int64_t fp_shared_decode_workspace_bytes(int32_t B, int32_t S, int32_
   return layout_of(B, S, Hq, Hc).part_rows * Hc * (D + 2) * static_cast<int64_t>(sizeof(float));
 }
 
-extern "C" int fp_shared_decode_plan(const int64_t* batch_idx, const void* input_pos, int pos_index_type,
-                                     const int32_t* prefix_ids, const int32_t* prefix_lens, int32_t B, int32_t S, int32_t Hq,
-                                     int32_t Hc, int32_t D, int32_t max_batch, int32_t max_context, void* plan,
-                                     int64_t plan_bytes, void* stream) {
-  const char* const what = "fp_shared_decode_plan";
+namespace {
+
+// (`alone`: prefix_ids and prefix_lens may be null)
+int make_plan(const char* what, bool alone, const int64_t* batch_idx, const void* input_pos, int pos_index_type, const int32_t* prefix_ids,
+              const int32_t* prefix_lens, int32_t B, int32_t S, int32_t Hq, int32_t Hc, int32_t D, int32_t max_batch,
+              int32_t max_context, void* plan, int64_t plan_bytes, void* stream) {
   if (const int rc = check_shape(what, B, S, Hq, Hc, D)) return rc;
   if (max_batch <= 0 || max_context <= 0)
     return fp::fail(FP_ERR_INVALID_ARGUMENT, "%s: max_batch %d, max_context %d", what, max_batch, max_context);
@@ -1500,7 +1557,7 @@ extern "C" int fp_shared_decode_plan(const int64_t* batch_idx, const void* input
   if (pos_index_type != FP_INDEX_I32 && pos_index_type != FP_INDEX_I64)
     return fp::fail(FP_ERR_INVALID_ARGUMENT, "%s: pos_index_type %d", what, pos_index_type);
   if (B == 0) return FP_OK;
-  if (!batch_idx || !input_pos || !prefix_ids || !prefix_lens || !plan)
+  if (!batch_idx || !input_pos || (alone ? !prefix_ids != !prefix_lens : !prefix_ids || !prefix_lens) || !plan)
     return fp::fail(FP_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
   if (plan_bytes < fp_shared_decode_plan_bytes(B, S, Hq, Hc, D) || !fp::aligned(plan, 16))
     return fp::fail(FP_ERR_WORKSPACE, "%s: the plan needs %lld bytes, 16-byte aligned (got %lld)", what,
@@ -1520,16 +1577,12 @@ extern "C" int fp_shared_decode_plan(const int64_t* batch_idx, const void* input
   return fp::check_launch(what);
 }
 
-extern "C" int fp_paged_decode_shared(const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_s,
-                                      const void* pool_k, const void* pool_v, const int64_t* page_table,
-                                      int64_t pt_row_stride, const int64_t* batch_idx, const void* input_pos,
-                                      int pos_index_type, void* out, int64_t out_stride_b, int64_t out_stride_h,
-                                      int64_t out_stride_s, float* lse, const float* sinks, void* workspace,
-                                      int64_t workspace_bytes, const void* plan, int64_t plan_bytes, int32_t B, int32_t S,
-                                      int32_t Hq, int32_t Hc, int32_t D, int32_t page_size, int32_t n_pages,
-                                      int32_t max_batch, int64_t n_slots, int32_t max_context, float scale, int dtype,
-                                      void* stream) {
-  const char* const what = "fp_paged_decode_shared";
+int attend(const char* what, bool tree, const int64_t* masks, const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_s,
+           const void* pool_k, const void* pool_v, const int64_t* page_table, int64_t pt_row_stride, const int64_t* batch_idx,
+           const void* input_pos, int pos_index_type, void* out, int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_s,
+           float* lse, const float* sinks, void* workspace, int64_t workspace_bytes, const void* plan, int64_t plan_bytes, int32_t B,
+           int32_t S, int32_t Hq, int32_t Hc, int32_t D, int32_t page_size, int32_t n_pages, int32_t max_batch, int64_t n_slots,
+           int32_t max_context, float scale, int dtype, void* stream) {
   if (const int rc = check_shape(what, B, S, Hq, Hc, D)) return rc;
   const int e = fp::elem_bytes(dtype);
   if (e == 0) return fp::fail(FP_ERR_UNSUPPORTED, "%s: dtype code %d", what, dtype);
@@ -1542,7 +1595,7 @@ extern "C" int fp_paged_decode_shared(const void* q, int64_t q_stride_b, int64_t
   if (pos_index_type != FP_INDEX_I32 && pos_index_type != FP_INDEX_I64)
     return fp::fail(FP_ERR_INVALID_ARGUMENT, "%s: pos_index_type %d", what, pos_index_type);
   if (B == 0) return FP_OK;
-  if (!q || !pool_k || !pool_v || !page_table || !batch_idx || !input_pos || !out || !lse || !plan)
+  if (!q || !pool_k || !pool_v || !page_table || !batch_idx || !input_pos || !out || !lse || !plan || (tree && !masks))
     return fp::fail(FP_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
   if (!fp::aligned(q, 16) || !fp::aligned(pool_k, 16) || !fp::aligned(pool_v, 16) || !fp::aligned(out, 16) ||
       q_stride_b * e % 16 || q_stride_h * e % 16 || q_stride_s * e % 16 || out_stride_b * e % 16 || out_stride_h * e % 16 ||
@@ -1562,14 +1615,15 @@ extern "C" int fp_paged_decode_shared(const void* q, int64_t q_stride_b, int64_t
                      input_pos, pos_index_type, static_cast<char*>(out), out_stride_b * e, out_stride_h * e, out_stride_s * e,
                      lse, sinks, B, S, Hq, Hc, fp::PageDiv(page_size), n_pages, max_batch,
                      static_cast<int>(n_slots / page_size), n_slots, max_context, scale * kLog2e, G, fp::log2_exact(G),
-                     static_cast<const char*>(plan), l.seqs, l.tokens, l.place, l.shares, l.tiles, acc, acc + l.part_rows * Hc * D};
+                     static_cast<const char*>(plan), l.seqs, l.tokens, l.place, l.shares, l.tiles, acc, acc + l.part_rows * Hc * D,
+                     masks};
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const auto go = [&](auto element) {
     using E = decltype(element);
-    if (D == 64)
-      launch<E, 64>(a, l.n_wg, st);
+    if (tree)
+      D == 64 ? launch<E, 64, true>(a, l.n_wg, st) : launch<E, 128, true>(a, l.n_wg, st);
     else
-      launch<E, 128>(a, l.n_wg, st);
+      D == 64 ? launch<E, 64, false>(a, l.n_wg, st) : launch<E, 128, false>(a, l.n_wg, st);
   };
   if (dtype == FP_DTYPE_F32)
     go(F32{});
@@ -1578,4 +1632,56 @@ extern "C" int fp_paged_decode_shared(const void* q, int64_t q_stride_b, int64_t
   else
     go(F16{});
   return fp::check_launch(what);
+}
+
+}  // namespace
+
+extern "C" int fp_shared_decode_plan(const int64_t* batch_idx, const void* input_pos, int pos_index_type,
+                                     const int32_t* prefix_ids, const int32_t* prefix_lens, int32_t B, int32_t S, int32_t Hq,
+                                     int32_t Hc, int32_t D, int32_t max_batch, int32_t max_context, void* plan,
+                                     int64_t plan_bytes, void* stream) {
+  return make_plan("fp_shared_decode_plan", false, batch_idx, input_pos, pos_index_type, prefix_ids, prefix_lens, B, S, Hq, Hc, D,
+                max_batch, max_context, plan, plan_bytes, stream);
+}
+
+extern "C" int fp_paged_decode_shared(const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_s,
+                                      const void* pool_k, const void* pool_v, const int64_t* page_table,
+                                      int64_t pt_row_stride, const int64_t* batch_idx, const void* input_pos,
+                                      int pos_index_type, void* out, int64_t out_stride_b, int64_t out_stride_h,
+                                      int64_t out_stride_s, float* lse, const float* sinks, void* workspace,
+                                      int64_t workspace_bytes, const void* plan, int64_t plan_bytes, int32_t B, int32_t S,
+                                      int32_t Hq, int32_t Hc, int32_t D, int32_t page_size, int32_t n_pages,
+                                      int32_t max_batch, int64_t n_slots, int32_t max_context, float scale, int dtype,
+                                      void* stream) {
+  return attend("fp_paged_decode_shared", false, nullptr, q, q_stride_b, q_stride_h, q_stride_s, pool_k, pool_v, page_table,
+                pt_row_stride, batch_idx, input_pos, pos_index_type, out, out_stride_b, out_stride_h, out_stride_s, lse, sinks,
+                workspace, workspace_bytes, plan, plan_bytes, B, S, Hq, Hc, D, page_size, n_pages, max_batch, n_slots,
+                max_context, scale, dtype, stream);
+}
+
+extern "C" int fp_tree_decode_plan(const int64_t* batch_idx, const void* input_pos, int pos_index_type,
+                                   const int32_t* prefix_ids, const int32_t* prefix_lens, int32_t B, int32_t S, int32_t Hq,
+                                   int32_t Hc, int32_t D, int32_t max_batch, int32_t max_context, void* plan,
+                                   int64_t plan_bytes, void* stream) {
+  if (S > kTreeTokens)
+    return fp::fail(FP_ERR_UNSUPPORTED, "%s: at most %d tokens a tree (got %d)", "fp_tree_decode_plan", kTreeTokens, S);
+  return make_plan("fp_tree_decode_plan", true, batch_idx, input_pos, pos_index_type, prefix_ids, prefix_lens, B, S, Hq, Hc, D,
+                max_batch, max_context, plan, plan_bytes, stream);
+}
+
+extern "C" int fp_paged_decode_tree(const int64_t* masks, const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_s,
+                                    const void* pool_k, const void* pool_v, const int64_t* page_table,
+                                    int64_t pt_row_stride, const int64_t* batch_idx, const void* input_pos,
+                                    int pos_index_type, void* out, int64_t out_stride_b, int64_t out_stride_h,
+                                    int64_t out_stride_s, float* lse, const float* sinks, void* workspace,
+                                    int64_t workspace_bytes, const void* plan, int64_t plan_bytes, int32_t B, int32_t S,
+                                    int32_t Hq, int32_t Hc, int32_t D, int32_t page_size, int32_t n_pages,
+                                    int32_t max_batch, int64_t n_slots, int32_t max_context, float scale, int dtype,
+                                    void* stream) {
+  if (S > kTreeTokens)
+    return fp::fail(FP_ERR_UNSUPPORTED, "%s: at most %d tokens a tree (got %d)", "fp_paged_decode_tree", kTreeTokens, S);
+  return attend("fp_paged_decode_tree", true, masks, q, q_stride_b, q_stride_h, q_stride_s, pool_k, pool_v, page_table,
+                pt_row_stride, batch_idx, input_pos, pos_index_type, out, out_stride_b, out_stride_h, out_stride_s, lse, sinks,
+                workspace, workspace_bytes, plan, plan_bytes, B, S, Hq, Hc, D, page_size, n_pages, max_batch, n_slots,
+                max_context, scale, dtype, stream);
 }

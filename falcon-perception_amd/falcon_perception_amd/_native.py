@@ -19,7 +19,7 @@ _LIB_DIR = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib")
 LIB_PATH = os.path.join(_LIB_DIR, "libfp_paged_kv.so")
 HOST_PATH = os.path.join(_LIB_DIR, "fp_host.so")
 
-FP_ABI_VERSION = 11
+FP_ABI_VERSION = 12
 NOALLOC_SCRATCH_BYTES = 64 << 20  # FP_NOALLOC_SCRATCH_BYTES
 FP_DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 FP_INDEX = {torch.int32: 0, torch.int64: 1}
@@ -94,6 +94,17 @@ SIGNATURES["fp_paged_decode_shared"] = (c_int, [
     c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int,
     c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64,
     c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int64, c_int32, c_float, c_int, c_void_p])
+
+SIGNATURES["fp_draft_tree"] = (c_int, [c_void_p, c_void_p, c_int, c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p])
+SIGNATURES["fp_tree_decode_plan"] = SIGNATURES["fp_shared_decode_plan"]
+SIGNATURES["fp_paged_decode_tree"] = (c_int, [c_void_p] + SIGNATURES["fp_paged_decode_shared"][1])
+SIGNATURES["fp_verify_drafts_workspace_bytes"] = (c_int64, [c_int32] * 3)
+SIGNATURES["fp_verify_drafts"] = (c_int, [
+    c_void_p, c_int64, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int,
+    c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_int32, c_int32, c_void_p])
+SIGNATURES["fp_keep_rows"] = (c_int, [
+    c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int32, c_int32, c_int64, c_int64, c_int32,
+    c_int32, c_int32, c_int32, c_int, c_void_p])
 
 SIGNATURES["fp_probe_mfma_softmax"] = (c_int, [c_int, c_int, c_int, c_int, c_void_p, c_int64, c_void_p])
 SIGNATURES["fp_paged_decode_plan"] = SIGNATURES["fp_paged_decode"]

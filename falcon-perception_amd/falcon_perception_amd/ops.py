@@ -772,3 +772,262 @@ def paged_decode_shared(q: Tensor, pool_k: Tensor, pool_v: Tensor, page_table: T
             N.stream_ptr(device))
     N.check(rc, "fp_paged_decode_shared")
     return out, lse
+
+
+# --------------------------------------------------------------------------------------------- answering with drafted tokens
+
+TREE_TOKENS = 64  # of a sequence, in one step
+
+
+class DraftTree(NamedTuple):
+    """What `draft_tree` makes of a step's drafts; see there."""
+
+    masks: Tensor
+    input_pos: Tensor
+    rope_pos: Tensor
+
+
+def _matrix(what: str, name: str, t: Tensor, shape: tuple[int, int], dtype: torch.dtype) -> Tensor:
+    if t.dtype != dtype or t.shape != shape:
+        raise RuntimeError(f"{what}: {name} must be {str(dtype)[6:]} {list(shape)}, got {str(t.dtype)[6:]} {list(t.shape)}")
+    return t.contiguous()
+
+
+def _tree_shape(what: str, parents: Tensor) -> tuple[int, int]:
+    if parents.dtype != torch.int32 or parents.dim() != 2 or not 0 < parents.shape[1] <= TREE_TOKENS:
+        raise RuntimeError(f"{what}: parents must be int32 [B, S] with S of 1 to {TREE_TOKENS}, got {str(parents.dtype)[6:]} "
+                           f"{list(parents.shape)}")
+    return parents.shape[0], parents.shape[1]
+
+
+def draft_tree(parents: Tensor, cached: Tensor) -> DraftTree:
+    """The trees of a step's tokens, once for all layers.
+
+    `parents` [B, S] int32: token 0 of a sequence is its last one, whose keys are not cached yet (-1: right behind the cached
+    keys), the others are drafts, each naming the row, in front of its own, of the token that it continues; anything else, -2 say,
+    is no token.  `cached` [B] (int32 or int64): keys in front of the step.
+
+    Returns `masks` [B, S] int64 (bit i of masks[b, j]: token j sees token i, its ancestors and itself; 0 no token), `input_pos`
+    [B, S] int32, the position in the cache that each token's keys go to (cached + j; -1 no token: `kv_append` leaves it out), and
+    `rope_pos` [B, S] int32, its place in the text (cached + number of ancestors)."""
+    what = "draft_tree"
+    device = _same_device(what, parents, cached)
+    B, S = _tree_shape(what, parents)
+    parents = parents.contiguous()
+    cached = _vector(what, "cached", cached, B, torch.int32, torch.int64)
+    _int32(what, sequences=B)
+    with _on(device):
+        made = DraftTree(torch.empty((B, S), dtype=torch.int64, device=device), torch.empty((B, S), dtype=torch.int32, device=device),
+                         torch.empty((B, S), dtype=torch.int32, device=device))
+        rc = N.lib().fp_draft_tree(parents.data_ptr(), cached.data_ptr(), N.index_code(cached), B, S, *(t.data_ptr() for t in made),
+                                   N.stream_ptr(device))
+    N.check(rc, "fp_draft_tree")
+    return made
+
+
+def _tree(what: str, tree: DraftTree) -> tuple[Tensor, Tensor]:
+    """Its masks and positions, [B, S] each."""
+    masks, input_pos = tree[0], tree[1]
+    if masks.dtype != torch.int64 or masks.dim() != 2 or not 0 < masks.shape[1] <= TREE_TOKENS:
+        raise RuntimeError(f"{what}: masks must be int64 [B, S] with S of 1 to {TREE_TOKENS}, got {str(masks.dtype)[6:]} {list(masks.shape)}")
+    if input_pos.dtype not in (torch.int32, torch.int64) or input_pos.shape != masks.shape:
+        raise RuntimeError(f"{what}: input_pos must be int32 or int64 {list(masks.shape)}, got {str(input_pos.dtype)[6:]} "
+                           f"{list(input_pos.shape)}")
+    return masks.contiguous(), input_pos.contiguous()
+
+
+def _prefixes(what: str, page_table: Tensor, prefix_ids: Tensor | None, prefix_lens: Tensor | None):
+    if (prefix_ids is None) != (prefix_lens is None):
+        raise RuntimeError(f"{what}: prefix_ids and prefix_lens are given together")
+    if prefix_ids is None:
+        return None, None
+    n = page_table.shape[0]
+    return _vector(what, "prefix_ids", prefix_ids, n, torch.int32), _vector(what, "prefix_lens", prefix_lens, n, torch.int32)
+
+
+def _pointer(t: Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def tree_decode_plan(batch_idx: Tensor, tree: DraftTree, page_table: Tensor, *, q_heads: int, cached_heads: int, head_dim: int,
+                     max_context: int, prefix_ids: Tensor | None = None, prefix_lens: Tensor | None = None,
+                     plan: Tensor | None = None) -> Tensor:
+    """The plan of a `paged_decode_tree` step, made once for all layers: how the work is cut and which sequences share a
+    prefix.  Arguments as there; `plan`: a uint8 tensor of `shared_decode_plan_bytes(B, S, ...)` bytes to write it to."""
+    what = "tree_decode_plan"
+    device = _same_device(what, batch_idx, tree[0], tree[1], page_table, prefix_ids, prefix_lens, plan)
+    masks, input_pos = _tree(what, tree)
+    B, S = masks.shape
+    batch_idx = _vector(what, "batch_idx", batch_idx, B, torch.int64)
+    _page_table(what, page_table)
+    prefix_ids, prefix_lens = _prefixes(what, page_table, prefix_ids, prefix_lens)
+    shape = dict(q_heads=q_heads, cached_heads=cached_heads, head_dim=head_dim)
+    _int32(what, max_context=max_context, slots=page_table.shape[0])
+    with _on(device):
+        plan = _byte_buffer(what, "plan", plan, shared_decode_plan_bytes(B, S, **shape), device)
+        rc = N.lib().fp_tree_decode_plan(
+            batch_idx.data_ptr(), input_pos.data_ptr(), N.index_code(input_pos), _pointer(prefix_ids), _pointer(prefix_lens), B, S,
+            q_heads, cached_heads, head_dim, page_table.shape[0], max_context, plan.data_ptr(), plan.numel(), N.stream_ptr(device))
+    N.check(rc, "fp_tree_decode_plan")
+    return plan
+
+
+def paged_decode_tree(q: Tensor, pool_k: Tensor, pool_v: Tensor, page_table: Tensor, batch_idx: Tensor, tree: DraftTree,
+                      page_size: int, max_context: int, *, prefix_ids: Tensor | None = None, prefix_lens: Tensor | None = None,
+                      scale: float | None = None, sinks: Tensor | None = None, plan: Tensor | None = None,
+                      workspace: Tensor | None = None, out: Tensor | None = None,
+                      lse: Tensor | None = None) -> tuple[Tensor, Tensor]:
+    """Attention of trees of drafted tokens over the paged cache, to which their keys have been appended (`tree.input_pos`).
+
+    q [B, Hq, S, D], pools [Hc, N, D], `tree` what `draft_tree` made (its masks and input_pos are read): token j of sequence b sees
+    the positions below input_pos[b, j] - j, its ancestors and itself.  A token that sees nothing, or is none: out 0, lse -inf.
+    `prefix_ids`, `prefix_lens` [max_batch] int32, both or none: as `paged_decode_shared`, a prefix that sequences have in common is
+    read once.  Returns out like q and lse [B, Hq, S].
+
+    `plan`: what `tree_decode_plan` made for this step (with the same prefixes; positions, slots and table unchanged since); without
+    one the call makes it.  `workspace`: `shared_decode_workspace_bytes(B, S, ...)` bytes, for one launch at a time.  `sinks`
+    [Hq] float32 gates the output as in `paged_decode`."""
+    what = "paged_decode_tree"
+    device = _same_device(what, q, pool_k, pool_v, page_table, batch_idx, tree[0], tree[1], prefix_ids, prefix_lens, sinks, plan,
+                          workspace, out, lse)
+    masks, input_pos = _tree(what, tree)
+    if q.dim() != 4 or pool_k.dim() != 3:
+        raise RuntimeError(f"{what}: q must be [B, Hq, S, D] and the pools [Hc, N, D]")
+    B, Hq, S, D = q.shape
+    Hc, n_slots, Dp = pool_k.shape
+    if Dp != D or pool_v.shape != pool_k.shape or pool_k.dtype != q.dtype or pool_v.dtype != q.dtype:
+        raise RuntimeError(f"{what}: q / pool shape or dtype mismatch")
+    if not (pool_k.is_contiguous() and pool_v.is_contiguous()):
+        raise RuntimeError(f"{what}: pool planes must be contiguous [H, N, D]")
+    if masks.shape != (B, S):
+        raise RuntimeError(f"{what}: the tree is of {list(masks.shape)} tokens, q of {[B, S]}")
+    batch_idx = _vector(what, "batch_idx", batch_idx, B, torch.int64)
+    _page_table(what, page_table)
+    prefix_ids, prefix_lens = _prefixes(what, page_table, prefix_ids, prefix_lens)
+    q = _rows(q)
+    if q.data_ptr() % 16 or any(s * q.element_size() % 16 for s in q.stride()[:3]):
+        q = q.contiguous()  # the kernel loads 16 bytes at once
+    shape = dict(q_heads=Hq, cached_heads=Hc, head_dim=D)
+    _int32(what, page_size=page_size, max_context=max_context)
+    with _on(device):
+        if plan is None:
+            plan = tree_decode_plan(batch_idx, DraftTree(masks, input_pos, tree[2]), page_table, max_context=max_context,
+                                    prefix_ids=prefix_ids, prefix_lens=prefix_lens, **shape)
+        workspace = _byte_buffer(what, "workspace", workspace, shared_decode_workspace_bytes(B, S, **shape), device)
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.stride(3) != 1:
+            raise RuntimeError(f"{what}: out must be like q, with dense rows")
+        if lse is None:
+            lse = torch.empty((B, Hq, S), dtype=torch.float32, device=device)
+        elif lse.shape != (B, Hq, S) or lse.dtype != torch.float32 or not lse.is_contiguous():
+            raise RuntimeError(f"{what}: lse must be contiguous float32 [B, Hq, S]")
+        if plan.dtype != torch.uint8 or not plan.is_contiguous():
+            raise RuntimeError(f"{what}: plan must be a contiguous uint8 tensor")
+        rc = N.lib().fp_paged_decode_tree(
+            masks.data_ptr(), q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), pool_k.data_ptr(), pool_v.data_ptr(),
+            page_table.data_ptr(), page_table.stride(0), batch_idx.data_ptr(), input_pos.data_ptr(), N.index_code(input_pos),
+            out.data_ptr(), out.stride(0), out.stride(1), out.stride(2), lse.data_ptr(), _sinks_ptr(sinks, Hq, device),
+            workspace.data_ptr(), workspace.numel(), plan.data_ptr(), plan.numel(), B, S, Hq, Hc, D, page_size, page_table.shape[1],
+            page_table.shape[0], n_slots, max_context, 1.0 / math.sqrt(D) if scale is None else scale, N.dtype_code(q.dtype),
+            N.stream_ptr(device))
+    N.check(rc, "fp_paged_decode_tree")
+    return out, lse
+
+
+class VerifiedDrafts(NamedTuple):
+    """What `verify_drafts` decides; see there."""
+
+    accepted: Tensor
+    path: Tensor
+    tokens: Tensor
+    logprobs: Tensor
+
+
+def verify_workspace_bytes(B: int, S: int, V: int) -> int:
+    """Bytes of workspace of a `verify_drafts` call on logits [B, S, V]."""
+    _int32("verify_workspace_bytes", B=B, S=S, V=V)
+    n = int(N.lib().fp_verify_drafts_workspace_bytes(B, S, V))
+    N.check(n, "fp_verify_drafts_workspace_bytes")
+    return n
+
+
+def verify_drafts(logits: Tensor, tokens: Tensor, parents: Tensor, uniforms: Tensor, *, temperatures: Tensor | None = None,
+                  draft_probs: Tensor | None = None, workspace: Tensor | None = None) -> VerifiedDrafts:
+    """Which drafted tokens stand by the target's distribution, and the token behind them, from given random numbers.
+
+    logits [B, S, V]: row j is what the target says behind token j of the step; `tokens` [B, S] int64 and `parents` [B, S] int32 are
+    the step's (row 0 the last token of the sequence, as `draft_tree`).  `uniforms` [B, S] float32 in [0, 1): that of row j for draft
+    j, that of row 0 for the drawn token.  `temperatures` [B] float32 (all 1 without; not above 0: greedy).  `draft_probs` [B, S, V]
+    (float32 or 16 bits): the distribution that the child of token j was drawn from; the drafts are then a chain.
+
+    From row 0 on, p the softmax of the row's logits / temperature, a child stands if u * r < p(its token), r what the children
+    refused before it leave of 1, or if u * q(its token) < p(its token).  Behind the last that stands a token is drawn from what is left, p
+    without the refused tokens or max(0, p - q).  In distribution the answer is that of drawing token by token from p.  Without drafts
+    (S = 1) it is a draw from p.
+
+    Returns `accepted` [B] int32, the number of drafts that stand; `path` [B, S] int32, row 0 and theirs, -1 behind (for `keep_rows`);
+    `tokens` [B, S] int64, those that stand and the drawn one, -1 behind; `logprobs` [B, S] float32, the log of p of each.  Decisions
+    are taken in 64 bits and do not depend on the batch.  A sequence whose parents[b, 0] is not -1 has no step: 0, -1, -1, 0.
+
+    `workspace`: `verify_workspace_bytes(B, S, V)` bytes, for one call at a time."""
+    what = "verify_drafts"
+    device = _same_device(what, logits, tokens, parents, uniforms, temperatures, draft_probs, workspace)
+    B, S = _tree_shape(what, parents)
+    if logits.dim() != 3 or logits.shape[:2] != (B, S) or logits.shape[2] < 1:
+        raise RuntimeError(f"{what}: logits must be [B, S, V] = [{B}, {S}, ...], got {list(logits.shape)}")
+    V = logits.shape[2]
+    code = N.dtype_code(logits.dtype)
+    parents = parents.contiguous()
+    tokens = _matrix(what, "tokens", tokens, (B, S), torch.int64)
+    uniforms = _matrix(what, "uniforms", uniforms, (B, S), torch.float32)
+    if temperatures is not None:
+        temperatures = _vector(what, "temperatures", temperatures, B, torch.float32)
+    logits = _rows(logits)
+    probs, probs_code, probs_strides = None, 0, (0, 0)
+    if draft_probs is not None:
+        if draft_probs.shape != logits.shape:
+            raise RuntimeError(f"{what}: draft_probs must be {list(logits.shape)}, got {list(draft_probs.shape)}")
+        probs = _rows(draft_probs)
+        probs_code, probs_strides = N.dtype_code(probs.dtype), probs.stride()[:2]
+    with _on(device):
+        workspace = _byte_buffer(what, "workspace", workspace, verify_workspace_bytes(B, S, V), device)
+        made = VerifiedDrafts(torch.empty(B, dtype=torch.int32, device=device), torch.empty((B, S), dtype=torch.int32, device=device),
+                              torch.empty((B, S), dtype=torch.int64, device=device),
+                              torch.empty((B, S), dtype=torch.float32, device=device))
+        rc = N.lib().fp_verify_drafts(
+            logits.data_ptr(), logits.stride(0), logits.stride(1), code, tokens.data_ptr(), parents.data_ptr(), uniforms.data_ptr(),
+            _pointer(temperatures), _pointer(probs), *probs_strides, probs_code, *(t.data_ptr() for t in made), workspace.data_ptr(),
+            workspace.numel(), B, S, V, N.stream_ptr(device))
+    N.check(rc, "fp_verify_drafts")
+    return made
+
+
+def keep_rows(pool: Tensor, page_table: Tensor, batch_idx: Tensor, cached: Tensor, path: Tensor, page_size: int) -> None:
+    """Move the cached rows of the tokens that stand together, in every plane of `pool` [..., n_slots, D].
+
+    For the leading entries of `path` [B, S] (int32, `VerifiedDrafts.path`) that rise, position cached[b] + i of slot batch_idx[b] gets the
+    rows of position cached[b] + path[b, i], as they were before the call; `cached` [B] (int32 or int64): keys in front of the
+    step.  An entry whose slot is outside the table, or named by an entry before it, is left out."""
+    what = "keep_rows"
+    device = _same_device(what, pool, page_table, batch_idx, cached, path)
+    if pool.dim() < 2 or not pool.is_contiguous():
+        raise RuntimeError(f"{what}: the pool must be contiguous [..., n_slots, D]")
+    if page_size < 1:
+        raise RuntimeError(f"{what}: page_size {page_size}")
+    _page_table(what, page_table)
+    if path.dtype != torch.int32 or path.dim() != 2 or not 0 < path.shape[1] <= TREE_TOKENS:
+        raise RuntimeError(f"{what}: path must be int32 [B, S] with S of 1 to {TREE_TOKENS}, got {str(path.dtype)[6:]} {list(path.shape)}")
+    B, S = path.shape
+    path = path.contiguous()
+    batch_idx = _vector(what, "batch_idx", batch_idx, B, torch.int64)
+    cached = _vector(what, "cached", cached, B, torch.int32, torch.int64)
+    n_slots, D = pool.shape[-2:]
+    _int32(what, entries=B, page_size=page_size, head_dim=D, columns=page_table.shape[1], slots=page_table.shape[0])
+    if pool.numel() == 0:
+        return
+    with _on(device):
+        rc = N.lib().fp_keep_rows(pool.data_ptr(), page_table.data_ptr(), page_table.stride(0), batch_idx.data_ptr(), cached.data_ptr(),
+                                  N.index_code(cached), path.data_ptr(), B, S, pool.numel() // (n_slots * D), n_slots, D, page_size,
+                                  page_table.shape[1], page_table.shape[0], N.dtype_code(pool.dtype), N.stream_ptr(device))
+    N.check(rc, "fp_keep_rows")

@@ -44,7 +44,7 @@
 extern "C" {
 #endif
 
-#define FP_ABI_VERSION 11
+#define FP_ABI_VERSION 12
 
 /* element types of pool / q / k / v */
 #define FP_DTYPE_F32 0
@@ -634,6 +634,101 @@ int fp_paged_decode_shared(const void* q, int64_t q_stride_b, int64_t q_stride_h
                            int32_t B, int32_t S, int32_t Hq, int32_t Hc, int32_t D,
                            int32_t page_size, int32_t n_pages, int32_t max_batch, int64_t n_slots,
                            int32_t max_context, float scale, int dtype, void* stream);
+
+/* ---- answering with drafted tokens (ABI 12; the reference has no counterpart) ---- */
+
+/*
+ * Trees of drafted tokens.  The tokens of a sequence's step are rows 0 .. S - 1: row 0 its last token, whose keys are not cached yet, the
+ * others drafts, each behind the token that it continues.
+ *
+ *   parents    [B, S] contiguous int32: -1 a token right behind the cached keys, 0 .. j - 1 the row that token j continues.  Anything else,
+ *              and whatever continues it: no token
+ *   cached     [B] int32/int64: keys in front of the step.  A negative one, or one past 2^31 - 65: the sequence has no tokens
+ *   masks      [B, S] int64: bit i of masks[b, j] says that token j sees token i: its ancestors and itself; 0 where there is no token
+ *   input_pos  [B, S] int32: cached[b] + j, the row of the cache that token j's keys go to (what fp_kv_append takes); -1 no token
+ *   rope_pos   [B, S] int32: cached[b] + number of ancestors, its place in the text; 0 no token
+ * S <= 64.
+ */
+int fp_draft_tree(const int32_t* parents, const void* cached, int cached_index_type, int32_t B, int32_t S,
+                  int64_t* masks, int32_t* input_pos, int32_t* rope_pos, void* stream);
+
+/*
+ * Attention of trees of drafted tokens over the paged cache: fp_paged_decode_shared for tokens that do not see all keys in front of them.
+ *
+ *   masks      [B, S] contiguous int64.  Token j of sequence b sees the positions below input_pos[b, j] - j and, for every bit i <= j of
+ *              masks[b, j], position input_pos[b, j] - j + i (of all these, those below max_context).  Bits behind j count for nothing.
+ *              A token that sees no key: out = 0, lse = -inf
+ * Everything else is as there, for fp_tree_decode_plan, too, whose prefix_ids and prefix_lens may both be NULL: no two sequences share
+ * keys.  Plan and workspace have the sizes of fp_shared_decode_plan_bytes and fp_shared_decode_workspace_bytes.  K and V rows of keys that
+ * a token does not see have no part in its result, whatever they hold.
+ * S <= 64.
+ */
+int fp_tree_decode_plan(const int64_t* batch_idx, const void* input_pos, int pos_index_type,
+                        const int32_t* prefix_ids, const int32_t* prefix_lens,
+                        int32_t B, int32_t S, int32_t Hq, int32_t Hc, int32_t D,
+                        int32_t max_batch, int32_t max_context,
+                        void* plan, int64_t plan_bytes, void* stream);
+int fp_paged_decode_tree(const int64_t* masks, const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_s,
+                         const void* pool_k, const void* pool_v,
+                         const int64_t* page_table, int64_t pt_row_stride,
+                         const int64_t* batch_idx, const void* input_pos, int pos_index_type,
+                         void* out, int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_s,
+                         float* lse, const float* sinks,
+                         void* workspace, int64_t workspace_bytes, const void* plan, int64_t plan_bytes,
+                         int32_t B, int32_t S, int32_t Hq, int32_t Hc, int32_t D,
+                         int32_t page_size, int32_t n_pages, int32_t max_batch, int64_t n_slots,
+                         int32_t max_context, float scale, int dtype, void* stream);
+
+/*
+ * Which drafted tokens the target model's distribution lets stand, and the token behind them, from given random numbers.
+ *
+ *   logits     [B, S, V], element strides (b, s), rows dense: row j is what the target says behind token j.  NaN counts as -inf
+ *   tokens     [B, S] contiguous int64; of row 0 not read
+ *   parents    [B, S] contiguous int32, as fp_draft_tree; row 0 must be -1, else the sequence has no step.  Logits of rows that are no token
+ *              are not read
+ *   uniforms   [B, S] contiguous float32, each used once, in 0 <= u < 1: u[b, j] for draft j, u[b, 0] for the drawn token
+ *   temperatures  NULL (all 1) or [B] float32; not above 0: the largest logit decides, of equal ones the first
+ *   draft_probs   NULL, or [B, S, V] of probs_dtype, element strides (b, s): row j is the distribution that the child of token j was
+ *              drawn from.  The drafts are then a chain: of a token's children only the first is looked at
+ *
+ * With p the softmax of a row's logits / temperature, from row 0 on: the children of the token are looked at in rising order, and child c
+ * stands if u_c * r < p(token_c), where r is 1 less the p of the children refused before it (of one token once); with draft_probs if
+ * u_c * q(token_c) < p(token_c).  Below the last that stands a token is drawn: the lowest i at which the sum of
+ * the weights up to it exceeds u_0 times the sum of all.  The weights are p without the refused tokens, or max(0, p - q) (p where that is
+ * 0 everywhere, or where no child was refused).  A draft outside 0 .. V - 1 never stands.  Sums and probabilities are in 64 bits: the
+ * result does not depend on how the work is cut.
+ *
+ *   accepted   [B] int32: drafts that stand
+ *   path       [B, S] int32: row 0 and the rows of those that stand, -1 behind them (what fp_keep_rows takes)
+ *   answer     [B, S] int64: the tokens that stand, then the drawn one, -1 behind them; -1 in its place too where the row has no logit
+ *              above -inf, or every token that has one was refused
+ *   logprobs   [B, S] float32: log p of every answered token where it stands (greedy: at temperature 1), 0 where there is none
+ * A sequence without a step: accepted 0, path and answer -1, logprobs 0.
+ * Workspace: memory of the caller, 16-byte aligned, one call at a time; nothing in it needs clearing.
+ * S <= 64, V <= 2^24.
+ */
+int64_t fp_verify_drafts_workspace_bytes(int32_t B, int32_t S, int32_t V);
+int fp_verify_drafts(const void* logits, int64_t logits_stride_b, int64_t logits_stride_s, int dtype,
+                     const int64_t* tokens, const int32_t* parents, const float* uniforms, const float* temperatures,
+                     const void* draft_probs, int64_t probs_stride_b, int64_t probs_stride_s, int probs_dtype,
+                     int32_t* accepted, int32_t* path, int64_t* answer, float* logprobs,
+                     void* workspace, int64_t workspace_bytes, int32_t B, int32_t S, int32_t V, void* stream);
+
+/*
+ * Moves the cached rows of the tokens that stand together, in every plane of a pool (all layers, K and V, all heads): for the leading
+ * entries of path[b] that rise (each above the one before, in 0 .. S - 1)
+ *   pool[p, row(cached[b] + i), :] = pool[p, row(cached[b] + path[b, i]), :],   row(t) = page_table[slot, t / P] * P + t % P
+ * as the rows were before the call.  cached[b] + (number of those entries) is the sequence's new length; what is behind it is left as it is.
+ *
+ *   pool       [n_planes, n_slots, D] contiguous, 16-byte aligned; rows of whole 16-byte chunks, 4096 bytes at most
+ *   batch_idx  [B] int64 cache slots; an entry with a slot outside the table, or one that an entry before it has, is left out
+ *   cached     [B] int32/int64; a negative one, or one past 2^31 - 1, leaves the entry out
+ *   path       [B, S] contiguous int32
+ * A row that lies in no page of the pool is neither read nor written.  S <= 64, B <= 65535.
+ */
+int fp_keep_rows(void* pool, const int64_t* page_table, int64_t pt_row_stride, const int64_t* batch_idx, const void* cached,
+                 int cached_index_type, const int32_t* path, int32_t B, int32_t S, int64_t n_planes, int64_t n_slots, int32_t D,
+                 int32_t page_size, int32_t n_pages, int32_t max_batch, int dtype, void* stream);
 
 #ifdef __cplusplus
 }
