@@ -6,13 +6,17 @@
 //                      u_c q[token_c] Z < w[token_c]                      (the drafts were drawn from q)
 // Behind the last that stands one more token is drawn: the first i whose cumulative weight is above u_0 times the total, of
 //   w without the refused tokens, or of max(0, w / Z - q).
-// Which token that is depends on sums over the whole vocabulary to the last bits: next to the border between two tokens, and with
-// 65536 of them there is always one near, sums in 32 bits would answer by the order they are taken in.  Weights and sums are
-// in 64 bits, the exponential to 2^-51 (a polynomial; on this GPU as many instructions a second as in 32 bits).
 //
-// Two launches.  The first has every row's maximum and sum, a chunk a workgroup, from one read of the logits.  In the second every
-// workgroup puts the chunks of its request's rows together, walks down the tree and sums the weights of a chunk of the row it ends at; the
-// last one of a request draws.  The first launch sets the counters of the second to 0: nothing is kept between calls.
+// Which token that is depends on sums over the whole vocabulary to the last bits: next to the border between two tokens, and with
+// 65536 of them there is always one near, sums in 32 bits would answer by the order they are taken in.  So the row that is drawn from is
+// weighed in 64 bits, the exponential to 2^-51.  All other rows have to say no more than on which side of a draft's weight u (Z - R) lies:
+//  * rows: every row's maximum and sum, a chunk a workgroup, from one read of the logits.  Weights in 32 bits, their arguments in
+//    two parts, off by kBand at most, summed in 64.
+//  * walk: every workgroup puts the chunks of its request's rows together and walks down the tree; a comparison within kBand of its
+//    border is made again with the row's sum in 64 bits (a few in a million).  Then it sums the weights of its part of the row that the walk
+//    ends at, and the last workgroup of a request draws.
+//  * rest: where the drafts were drawn, what is left of the target's distribution needs Z first: the same once more, with Z.
+// The first launch sets the counters of the others to 0: nothing is kept between calls.
 #include "fp_common.h"
 
 #include <math.h>
@@ -22,6 +26,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kMaxTokens = 64;
+constexpr float kBand = 0x1p-18f;  // what a row's sum may be off by, relatively
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
 struct BF16 {
@@ -51,9 +56,10 @@ struct Part {   // of a chunk of a row
   float peak;
   int best;     // the first place of `peak`, where the request is greedy
 };
-struct Sums {   // of a chunk of the row that is drawn from
-  double left;  // what is drawn from
-  double all;   // the weights themselves
+struct End {    // of a request's walk
+  int node, count;
+  int rest;     // something is taken away: what is left is weighed by the third launch
+  float peak;
 };
 
 struct VerifyArgs {
@@ -70,9 +76,12 @@ struct VerifyArgs {
   int32_t* path;
   int64_t* answer;
   float* logprobs;
-  Part* parts;   // [B * S, chunks]
-  Sums* sums;    // [B, draws]
-  int* arrivals;  // [B]
+  Part* parts;     // [B * S, chunks]
+  double* sums;    // [B, draws * NV]: weights of every 256 vectors of the row that is drawn from
+  double* rests;   // [B, draws * NV]: what is left of them
+  End* ends;       // [B]
+  double* totals;  // [B]: Z of the row that is drawn from, for the logarithm
+  int* arrivals;   // [2, B]
   int B, S, V, chunks, draws;
 };
 
@@ -124,13 +133,68 @@ struct Row {
 // Whether row j of the request is a token that can be reached.
 __device__ __forceinline__ bool is_token(int j, int parent) { return j == 0 ? parent == -1 : parent >= 0 && parent < j; }
 
+// Sum over the lanes up to this one, without a trip through LDS (row_shr:1, 2, 4, 8, then row_bcast:15, 31).
+template <int kControl, int kRows>
+__device__ __forceinline__ double from_lane(double x) {
+  const uint64_t bits = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(bits), kControl, kRows, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(bits >> 32), kControl, kRows, 0xf, false);
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+__device__ __forceinline__ double scan_lanes(double x) {
+  x += from_lane<0x111, 0xf>(x);
+  x += from_lane<0x112, 0xf>(x);
+  x += from_lane<0x114, 0xf>(x);
+  x += from_lane<0x118, 0xf>(x);
+  x += from_lane<0x142, 0xa>(x);
+  x += from_lane<0x143, 0xc>(x);
+  return x;
+}
+__device__ __forceinline__ double lane_of(double x, int lane) {
+  const uint64_t bits = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(bits), lane), hi = __builtin_amdgcn_readlane(static_cast<int>(bits >> 32), lane);
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+__device__ __forceinline__ double sum_lanes(double x) { return lane_of(scan_lanes(x), 63); }
+
 template <typename T, typename Op>
 __device__ __forceinline__ T reduce_lanes(T x, int width, Op op) {
   for (int d = 1; d < width; d <<= 1) x = op(x, __shfl_xor(x, d));
   return x;
 }
 
+// The elements of a row that belong to its v-th vector, in order, to f(x, i, place in the vector): of the first one those in front of it,
+// too, and of the last one those behind (place -1).
+template <typename E, typename F>
+__device__ __forceinline__ void each(const Row<E>& r, int v, const v4u& x, F f) {
+  if (r.head > 0 && v == 0)
+    for (int i = 0; i < r.head; ++i) f(r.one(i), i, -1);
+  if (v < r.vectors)
+#pragma unroll
+    for (int i = 0; i < E::kVec; ++i) f(E::get(x, i), r.head + v * E::kVec + i, i);
+  if (r.tail > 0 && v == max(r.vectors - 1, 0))
+    for (int i = 0; i < r.tail; ++i) f(r.one(r.behind() + i), r.behind() + i, -1);
+}
+
 // ---------------------------------------------------------------------------------------------------------------- rows
+// A weight in 32 bits.  Its exponent (x - peak) * rate is p + e: p rounded to 32 bits, e what the product and the difference were rounded
+// by (16-bit logits whose difference is not exact are off by 2^-24 of the larger one, and so is the exponent); 2^e = 1 + e ln 2.
+struct Rate {
+  float hi, lo;
+};
+template <typename E>
+__device__ __forceinline__ float weight32(float x, float peak, Rate rate) {
+  const float d = x - peak, p = fmaxf(d * rate.hi, -200.f);  // (-200: also of -inf and NaN)
+  float e = fmaf(d, rate.lo, fmaf(d, rate.hi, -p));
+  if constexpr (E::kBytes == 4) {
+    const float back = x - d, there = d + back;
+    e = fmaf((x - there) + (back - peak), rate.hi, e);
+  }
+  e = __builtin_amdgcn_fmed3f(e, -1.f, 1.f);
+  const float w = __builtin_amdgcn_exp2f(p);
+  return fmaf(w, e * 0x1.62e430p-1f, w);
+}
+
 template <typename E, int NV>  // vectors a thread
 __global__ __launch_bounds__(kThreads) void verify_rows_kernel(const VerifyArgs a) {
   __shared__ float s_peak[kWaves];
@@ -139,7 +203,7 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(const VerifyArgs 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint32_t row = blockIdx.x / static_cast<uint32_t>(a.chunks), b = row / static_cast<uint32_t>(a.S);
   const int c = blockIdx.x - row * a.chunks, j = row - b * a.S;
-  if (c == 0 && j == 0 && tid == 0) a.arrivals[b] = 0;
+  if (c == 0 && j == 0 && tid < 2) a.arrivals[tid * a.B + b] = 0;
   if (!is_token(j, a.parents[row]) || a.parents[static_cast<int64_t>(b) * a.S] != -1) return;
   const Row<E> r(a.logits + b * a.ls_b + j * a.ls_s, a.V);
   const int v0 = c * (kThreads * NV) + tid;
@@ -147,19 +211,11 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(const VerifyArgs 
 #pragma unroll
   for (int k = 0; k < NV; ++k)
     if (v0 + k * kThreads < r.vectors) x[k] = r.load(v0 + k * kThreads);
-  // the elements outside the whole 16 bytes: the first chunk's first threads and the last one's next 8
-  int extra = -1;
-  if (c == 0 && tid < r.head) extra = tid;
-  if (c == a.chunks - 1 && tid >= 8 && tid - 8 < r.tail) extra = r.behind() + tid - 8;
-  const float loose = extra >= 0 ? r.one(extra) : -INFINITY;
   const float heat = heat_of(a, b);
 
-  float peak = fmaxf(loose, -INFINITY);
+  float peak = -INFINITY;
 #pragma unroll
-  for (int k = 0; k < NV; ++k)
-    if (v0 + k * kThreads < r.vectors)
-#pragma unroll
-      for (int i = 0; i < E::kVec; ++i) peak = fmaxf(peak, E::get(x[k], i));
+  for (int k = 0; k < NV; ++k) each<E>(r, v0 + k * kThreads, x[k], [&](float y, int, int) { peak = fmaxf(peak, y); });
   peak = reduce_lanes(peak, 64, [](float p, float q) { return fmaxf(p, q); });
   if (lane == 0) s_peak[wave] = peak;
   __syncthreads();
@@ -168,33 +224,24 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(const VerifyArgs 
 
   int best = INT32_MAX;
   if (!(heat > 0.f)) {
-    if (loose == peak && extra >= 0) best = extra;
 #pragma unroll
     for (int k = 0; k < NV; ++k)
-      if (v0 + k * kThreads < r.vectors)
-#pragma unroll
-        for (int i = 0; i < E::kVec; ++i)
-          if (E::get(x[k], i) == peak) best = min(best, r.head + (v0 + k * kThreads) * E::kVec + i);
+      each<E>(r, v0 + k * kThreads, x[k], [&](float y, int i, int) { best = y == peak ? min(best, i) : best; });
     best = reduce_lanes(best, 64, [](int p, int q) { return min(p, q); });
   }
   double sum = 0.0;
-  if (fabsf(peak) < INFINITY) {
-    const double rate = kLog2e / (heat > 0.f ? heat : 1.0), top = peak;
-    if (extra >= 0) sum = power2((loose - top) * rate);
+  const double rate = kLog2e / (heat > 0.f ? heat : 1.0);
+  if (fabsf(peak) < INFINITY && rate > 0x1p-40 && rate < 0x1p40) {
+    const Rate parts{static_cast<float>(rate), static_cast<float>(rate - static_cast<float>(rate))};
 #pragma unroll
+    for (int k = 0; k < NV; ++k) each<E>(r, v0 + k * kThreads, x[k], [&](float y, int, int) { sum += weight32<E>(y, peak, parts); });
+  } else {  // infinite logits, temperatures out of all measure
+#pragma nounroll
     for (int k = 0; k < NV; ++k)
-      if (v0 + k * kThreads < r.vectors)
-#pragma unroll
-        for (int i = 0; i < E::kVec; ++i) sum += power2((E::get(x[k], i) - top) * rate);
-  } else if (peak > 0.f) {  // only infinite logits count
-    sum = extra >= 0 && loose == peak;
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-      if (v0 + k * kThreads < r.vectors)
-#pragma unroll
-        for (int i = 0; i < E::kVec; ++i) sum += E::get(x[k], i) == peak;
+      each<E>(r, v0 + k * kThreads, v0 + k * kThreads < r.vectors ? r.load(v0 + k * kThreads) : v4u{0, 0, 0, 0},
+              [&](float y, int, int) { sum += weight(y, peak, rate); });
   }
-  sum = reduce_lanes(sum, 64, [](double p, double q) { return p + q; });
+  sum = sum_lanes(sum);
   if (lane == 0) {
     s_sum[wave] = sum;
     s_best[wave] = best;
@@ -218,38 +265,139 @@ __device__ __forceinline__ double take(const double* p) {
   return __builtin_bit_cast(double, __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
 }
 
-// What the row that is drawn from weighs, element by element.
-struct Drawn {
-  const char* probs;   // of the draft, null: not taken away
-  float peak;
-  double rate, share;  // share: 1 / Z
+// log p of a token with logit x; slope: 1 / temperature
+__device__ __forceinline__ float log_share(float x, float peak, double slope, double total) {
+  return static_cast<float>((x == peak ? 0.0 : (static_cast<double>(x) - static_cast<double>(peak)) * slope) - log(total));
+}
+
+struct DrawShared {
+  double sum[kWaves];
+  int place, flag;
 };
 
+// The sums of this workgroup's 256 vectors each go to `to`; whether it is the last of `n` workgroups to say so.
+template <int NV>
+__device__ __forceinline__ bool last_with_sums(const double (&sum)[NV], double* to, int* counter, int n, double (*s_sum)[NV], int* flag) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const double all = sum_lanes(sum[k]);
+    if (lane == 0) s_sum[wave][k] = all;
+  }
+  __syncthreads();
+  if (wave == 0) {
+    if (lane < NV) publish(to + lane, s_sum[0][lane] + s_sum[1][lane] + s_sum[2][lane] + s_sum[3][lane]);
+    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // they have arrived before the count does
+    if (lane == 0) *flag = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
+  }
+  __syncthreads();
+  return *flag != 0;
+}
+
+// All of n published sums together, by each wavefront: the same in every one that asks.
+__device__ __forceinline__ double total_of(const double* sums, int n) {
+  double all = 0.0;
+  for (int k = threadIdx.x & 63; k < n; k += 64) all += take(sums + k);
+  return sum_lanes(all);
+}
+
+// The first token at which the weights of the row pass u times their total: `n` sums of 256 vectors each, `weigh(x, i)` a token's weight.
+// What it is goes to answer(token, x), by one thread; -1 if nothing weighs anything.
+template <typename E, typename W, typename A>
+__device__ __forceinline__ void draw(const Row<E>& r, const double* sums, int n, double total, float u, DrawShared& sh, W weigh, A answer) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const double goal = (u < 0.f ? 0.0 : static_cast<double>(u)) * total;  // (NaN passes nothing: the last token)
+  double before = 0.0, before_last = 0.0;
+  int part = -1, last = -1;
+  for (int k0 = 0; k0 < n && part < 0; k0 += 64) {
+    const double s = k0 + lane < n ? take(sums + k0 + lane) : 0.0, upto = scan_lanes(s);
+    const uint64_t past = __ballot(before + upto > goal), some = __ballot(s > 0.0);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      part = k0 + l;
+      before += lane_of(upto - s, l);
+    } else {
+      if (some) {
+        const int l = 63 - __builtin_clzll(some);
+        last = k0 + l;
+        before_last = before + lane_of(upto - s, l);
+      }
+      before += lane_of(upto, 63);
+    }
+  }
+  if (part < 0) part = last, before = before_last;
+  if (part < 0) {
+    if (tid == 0) answer(-1, 0.f);
+    return;
+  }
+  const int v = part * kThreads + tid;
+  const v4u x = v < r.vectors ? r.load(v) : v4u{0, 0, 0, 0};
+  double sum = 0.0;
+  int found = -1;
+  float its = 0.f;
+  each<E>(r, v, x, [&](float y, int i, int) {
+    const double w = weigh(y, i);
+    sum += w;
+    if (w > 0.0) found = i, its = y;  // the last that weighs something
+  });
+  const double upto = scan_lanes(sum);
+  if (lane == 63) sh.sum[wave] = upto;
+  if (tid == 0) sh.place = INT32_MAX;
+  __syncthreads();
+  double at = before;
+  for (int w = 0; w < wave; ++w) at += sh.sum[w];
+  at += upto - sum;
+  const bool passes = sum > 0.0 && at + sum > goal;
+  if (passes) {
+    bool done = false;
+    each<E>(r, v, x, [&](float y, int i, int) {
+      const double w = weigh(y, i);
+      at += w;
+      if (!done && w > 0.0 && at > goal) done = true, found = i, its = y;
+    });
+    atomicMin(&sh.place, found);
+  }
+  __syncthreads();
+  if (sh.place == INT32_MAX) {  // u at its very end: the last token that weighs something
+    __syncthreads();
+    if (tid == 0) sh.place = -1;
+    __syncthreads();
+    if (found >= 0) atomicMax(&sh.place, found);
+    __syncthreads();
+  }
+  if (found >= 0 && found == sh.place) answer(found, its);
+}
+
 template <typename E, int NV>
-__global__ __launch_bounds__(kThreads) void verify_draw_kernel(const VerifyArgs a) {
-  constexpr int kVectors = kThreads * NV, kMarks = kVectors * E::kVec + 2 * 8;
+__global__ __launch_bounds__(kThreads) void verify_walk_kernel(const VerifyArgs a) {
   __shared__ float s_peak[kMaxTokens];
   __shared__ int s_best[kMaxTokens];
   __shared__ double s_total[kMaxTokens];
-  __shared__ int64_t s_out[kMaxTokens];             // refused tokens
-  __shared__ uint32_t s_mark[(kMarks + 31) / 32];   // of the chunk's elements
-  __shared__ int s_node, s_count, s_n_out, s_refused, s_flag, s_place;
-  __shared__ double s_sum[kWaves][2];
+  __shared__ int s_out[kMaxTokens];  // refused tokens
+  __shared__ int s_node, s_count, s_n_out, s_refused, s_again;
+  __shared__ double s_sums[kWaves][NV];
+  __shared__ DrawShared sh;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint32_t b = blockIdx.x / static_cast<uint32_t>(a.draws);
   const int c = blockIdx.x - b * a.draws, S = a.S;
   const int64_t first = static_cast<int64_t>(b) * S;
   const bool there = a.parents[first] == -1;
-  const float heat = heat_of(a, b);
+  const float heat = heat_of(a, b), u0 = a.uniforms[first];
   const bool greedy = !(heat > 0.f);
   const double rate = kLog2e / (greedy ? 1.0 : heat), slope = 1.0 / (greedy ? 1.0 : heat);
 
-  // every row's maximum and sum: `per` lanes a row
+  // a token a lane
+  const int parent = lane < S ? a.parents[first + lane] : -2;
+  const int64_t token = lane < S ? a.tokens[first + lane] : -1;
+  const float u = lane < S ? a.uniforms[first + lane] : 0.f;
+
+  // every row's maximum and sum, `per` lanes a row
   int per = 64;
   while (per > kThreads / S) per >>= 1;
-  for (int j = tid / per; j < S; j += kThreads / per) {
-    Part t{0.0, -INFINITY, INT32_MAX};
-    if (there && is_token(j, a.parents[first + j])) {
+  {
+    const int j = tid / per;
+    if (j < S && there && is_token(j, a.parents[first + j])) {
+      Part t{0.0, -INFINITY, INT32_MAX};
       const Part* const parts = a.parts + (first + j) * a.chunks;
       for (int k = tid % per; k < a.chunks; k += per) {
         const Part p = parts[k];
@@ -262,304 +410,256 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(const VerifyArgs 
           if (p.peak == t.peak) t.best = min(t.best, p.best);
         }
       }
-    }
-    const float peak = reduce_lanes(t.peak, per, [](float p, float q) { return fmaxf(p, q); });
-    const double total = reduce_lanes(t.sum * weight(t.peak, peak, rate), per, [](double p, double q) { return p + q; });
-    const int best = reduce_lanes(t.peak == peak ? t.best : INT32_MAX, per, [](int p, int q) { return min(p, q); });
-    if (tid % per == 0) {
-      s_peak[j] = peak;
-      s_total[j] = total;
-      s_best[j] = peak == -INFINITY ? -1 : best;
-    }
-  }
-  __syncthreads();
-
-  // the walk down the tree: a token a lane
-  if (wave == 0) {
-    const int parent = lane < S ? a.parents[first + lane] : -2;
-    const int64_t token = lane < S ? a.tokens[first + lane] : -1;
-    const float u = lane < S ? a.uniforms[first + lane] : 0.f;
-    const bool child = there && lane > 0 && lane < S && parent >= 0 && parent < lane, known = token >= 0 && token < a.V;
-    const int at = child ? parent : 0;
-    double w = 0.0, q = 0.0;
-    float x = -INFINITY;
-    if (child && known) {
-      x = E::at(a.logits + b * a.ls_b + at * a.ls_s + token * E::kBytes);
-      if (a.probs) q = probability(a, a.probs + b * a.ps_b + at * a.ps_s, token);
-      w = weight(x, s_peak[at], rate);
-    }
-    double refused = 0.0;
-    bool eldest = true;
-    for (int i = 1; i < S; ++i) {  // the siblings before this token: what they weigh, the same token once
-      const bool sibling = i < lane && __builtin_amdgcn_readlane(parent, i) == parent;
-      const int64_t name = __shfl(token, i);
-      const double theirs = __shfl(w, i);
-      if (sibling) {
-        eldest = false;
-        if (name == token) w = 0.0; else refused += theirs;
+      const float peak = reduce_lanes(t.peak, per, [](float p, float q) { return fmaxf(p, q); });
+      const double total = reduce_lanes(t.sum * weight(t.peak, peak, rate), per, [](double p, double q) { return p + q; });
+      const int best = reduce_lanes(t.peak == peak ? t.best : INT32_MAX, per, [](int p, int q) { return min(p, q); });
+      if (tid % per == 0) {
+        s_peak[j] = peak;
+        s_total[j] = total;
+        s_best[j] = peak == -INFINITY ? -1 : best;
       }
     }
-    const double z = s_total[at];
-    const bool takes = child && known && (greedy ? token == s_best[at] : a.probs ? eldest && u * q * z < w : u * (z - refused) < w);
-    int node = 0, count = 0, mine = lane == 0 ? 0 : -1;  // mine: the lane-th of the path
-    if (there) {
+  }
+  const bool child = there && lane > 0 && lane < S && parent >= 0 && parent < lane, known = token >= 0 && token < a.V;
+  const int at = child ? parent : 0;
+  float x = -INFINITY;
+  double q = 0.0;
+  if (wave == 0 && child && known) {
+    x = E::at(a.logits + b * a.ls_b + at * a.ls_s + token * E::kBytes);
+    if (a.probs) q = probability(a, a.probs + b * a.ps_b + at * a.ps_s, token);
+  }
+  __syncthreads();
+  if (!there) {
+    if (c == 0 && tid < S) {
+      a.path[first + tid] = -1;
+      a.answer[first + tid] = -1;
+      a.logprobs[first + tid] = 0.f;
+      if (tid == 0) a.accepted[b] = 0;
+    }
+    if (c == 0 && tid == 0) a.ends[b] = End{0, 0, 0, 0.f};
+    return;
+  }
+
+  // the walk down the tree
+  uint64_t exact = 0;  // rows whose sums are in 64 bits
+  double w = 0.0, refused = 0.0;
+  bool eldest = true;
+  if (wave == 0) {
+    if (child && known) w = weight(x, s_peak[at], rate);
+    for (int i = 1; i < S; ++i) {  // the siblings before this token: what they weigh, the same token once
+      const bool sibling = i < lane && __builtin_amdgcn_readlane(parent, i) == parent;
+      const bool same = __builtin_amdgcn_readlane(known ? static_cast<int>(token) : -1, i) == static_cast<int>(token);
+      const double theirs = lane_of(w, i);
+      if (sibling) {
+        eldest = false;
+        if (same) w = 0.0; else refused += theirs;
+      }
+    }
+  }
+  for (;;) {
+    if (wave == 0) {
+      const double z = s_total[at], side = a.probs ? u * q * z : u * (z - refused);
+      const bool asked = child && known && w > 0.0 && (!a.probs || eldest);
+      const bool takes = child && known && greedy ? token == s_best[at] : asked && side < w;
+      const bool near = asked && !greedy && !(exact >> at & 1) && fabs(side - w) <= kBand * (a.probs ? side : z);
+      int node = 0, count = 0, mine = lane == 0 ? 0 : -1, again = -1;  // mine: the lane-th of the path
       for (;;) {
-        const uint64_t stand = __ballot(takes && parent == node);
+        const uint64_t doubt = __ballot(near && parent == node), stand = __ballot(takes && parent == node);
+        // (a child that stands hides doubts about those behind it)
+        if (doubt && (stand == 0 || __builtin_ctzll(doubt) <= __builtin_ctzll(stand))) {
+          again = node;
+          break;
+        }
         if (stand == 0) break;
         node = __builtin_ctzll(stand);
         ++count;
         if (lane == count) mine = node;
       }
-    }
-    const uint64_t out = __ballot(child && known && parent == node);
-    if (child && known && parent == node) s_out[__builtin_popcountll(out & ((1ull << lane) - 1))] = token;
-    const bool any = __ballot(child && parent == node) != 0;
-    if (lane == 0) {
-      s_node = node;
-      s_count = count;
-      s_n_out = __builtin_popcountll(out);
-      s_refused = any;
-    }
-    if (c == 0) {
-      // the token of path[lane + 1] answers at place lane; the last place is the drawn one's
-      const int next = __shfl_down(mine, 1);
-      const int from = lane < count ? next : 0;
-      const int64_t name = __shfl(token, from);
-      const float its = __shfl(x, from);
-      const int under = __shfl(at, from);
-      if (lane < S) {
-        a.path[first + lane] = there ? mine : -1;
-        if (lane != count || !there) {
-          const bool says = there && lane < count;
-          a.answer[first + lane] = says ? name : -1;
-          const float peak = s_peak[under];
-          a.logprobs[first + lane] = says ? static_cast<float>((its == peak ? 0.0 : (static_cast<double>(its) - peak) * slope) - log(s_total[under])) : 0.f;
-        }
+      const bool here = child && parent == node, gone = here && known;
+      const uint64_t out = __ballot(gone);
+      if (gone) s_out[__builtin_popcountll(out & ((1ull << lane) - 1))] = static_cast<int>(token);
+      const bool any = __ballot(here) != 0;
+      if (lane == 0) {
+        s_node = node;
+        s_count = count;
+        s_n_out = __builtin_popcountll(out);
+        s_refused = any;
+        s_again = again;
       }
-      if (lane == 0) a.accepted[b] = count;
+      if (c == 0 && again < 0) {
+        // the token of path[lane + 1] answers at place lane; the last place is the drawn one's
+        const int next = __shfl_down(mine, 1);
+        const int from = lane < count ? next : 0;
+        const int64_t name = __shfl(token, from);
+        const float its = __shfl(x, from);
+        const int under = __shfl(at, from);
+        if (lane < S) {
+          a.path[first + lane] = mine;
+          if (lane != count) {
+            const bool says = lane < count;
+            a.answer[first + lane] = says ? name : -1;
+            a.logprobs[first + lane] = says ? log_share(its, s_peak[under], slope, s_total[under]) : 0.f;
+          }
+        }
+        if (lane == 0) a.accepted[b] = count;
+      }
     }
+    __syncthreads();
+    const int again = s_again;
+    if (again < 0) break;
+    // too near to its border: the row's sum once more, in 64 bits
+    const Row<E> r(a.logits + b * a.ls_b + again * a.ls_s, a.V);
+    const float peak = s_peak[again];
+    double sum = 0.0;
+    for (int v = tid; v < max(r.vectors, 1); v += kThreads)
+      each<E>(r, v, v < r.vectors ? r.load(v) : v4u{0, 0, 0, 0}, [&](float y, int, int) { sum += weight(y, peak, rate); });
+    sum = sum_lanes(sum);
+    if (lane == 0) sh.sum[wave] = sum;
+    __syncthreads();
+    if (tid == 0) s_total[again] = sh.sum[0] + sh.sum[1] + sh.sum[2] + sh.sum[3];
+    exact |= 1ull << again;
+    __syncthreads();
   }
-  __syncthreads();
-  if (!there) return;
+
   const int node = s_node, count = s_count;
+  const float peak = s_peak[node];
+  const double total = s_total[node];
   const Row<E> r(a.logits + b * a.ls_b + node * a.ls_s, a.V);
-  const auto answer = [&](int64_t token) {
+  const auto answer = [&](int token, float x) {
     a.answer[first + count] = token;
-    float says = 0.f;
-    if (token >= 0) {
-      const float x = r.one(token), peak = s_peak[node];
-      says = static_cast<float>((x == peak ? 0.0 : (static_cast<double>(x) - peak) * slope) - log(s_total[node]));
-    }
-    a.logprobs[first + count] = says;
+    a.logprobs[first + count] = token < 0 ? 0.f : log_share(x, peak, slope, total);
   };
-  if (greedy || s_peak[node] == -INFINITY) {
-    if (c == 0 && tid == 0) answer(s_best[node]);
+  const bool rest = a.probs && s_refused && !greedy && peak > -INFINITY;
+  if (c == 0 && tid == 0) {
+    a.ends[b] = End{node, count, rest, peak};
+    a.totals[b] = total;
+  }
+  if (greedy || peak == -INFINITY) {
+    if (c == 0 && tid == 0) answer(s_best[node], peak);
     return;
   }
-
-  const Drawn drawn{a.probs && s_refused ? a.probs + b * a.ps_b + node * a.ps_s : nullptr, s_peak[node], rate, 1.0 / s_total[node]};
   const int n_out = a.probs ? 0 : s_n_out;
-  // Marks of the refused tokens among the elements of a chunk: those in front of the whole 16 bytes have the first 8 places, those behind
-  // them the next 8.
-  const auto mark = [&](int chunk) {
-    if (n_out == 0) return;
-    __syncthreads();
-    for (int i = tid; i < (kMarks + 31) / 32; i += kThreads) s_mark[i] = 0;
-    __syncthreads();
-    if (tid < n_out) {
-      const int64_t t = s_out[tid], inside = t - r.head - static_cast<int64_t>(chunk) * kVectors * E::kVec;
-      int place = -1;
-      if (t < r.head)
-        place = chunk == 0 ? static_cast<int>(t) : -1;
-      else if (t >= r.behind())
-        place = chunk == a.draws - 1 ? static_cast<int>(8 + t - r.behind()) : -1;
-      else if (inside >= 0 && inside < kVectors * E::kVec)
-        place = static_cast<int>(16 + inside);
-      if (place >= 0) atomicOr(&s_mark[place >> 5], 1u << (place & 31));
-    }
-    __syncthreads();
+  // the weight of token i, 0 if it was refused
+  const auto weigh = [&](float y, int i) {
+    double w = weight(y, peak, rate);
+    for (int k = 0; k < n_out; ++k) w = s_out[k] == i ? 0.0 : w;
+    return w;
   };
-  const auto marked = [&](int place) { return n_out > 0 && (s_mark[place >> 5] >> (place & 31) & 1); };
-  // weight of element i of the row, whose place among the marks is given
-  const auto left_of = [&](float x, int64_t i, int place, bool take_away) {
-    if (marked(place)) return 0.0;
-    const double w = weight(x, drawn.peak, drawn.rate);
-    return take_away ? fmax(0.0, w * drawn.share - static_cast<double>(probability(a, drawn.probs, i))) : w;
-  };
-
-  mark(c);
   {
-    double left = 0.0, all = 0.0;
-    const auto add = [&](float x, int64_t i, int place) {
-      const double w = left_of(x, i, place, false);
-      all += w;
-      if (drawn.probs) left += fmax(0.0, w * drawn.share - static_cast<double>(probability(a, drawn.probs, i)));
-    };
     v4u x[NV];
+    double sum[NV];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int v = c * kVectors + k * kThreads + tid;
+      const int v = (c * NV + k) * kThreads + tid;
       if (v < r.vectors) x[k] = r.load(v);
     }
-    if (c == 0 && tid < r.head) add(r.one(tid), tid, tid);
-    if (c == a.draws - 1 && tid >= 8 && tid - 8 < r.tail) add(r.one(r.behind() + tid - 8), r.behind() + tid - 8, tid);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int v = c * kVectors + k * kThreads + tid;
-      if (v < r.vectors)
-#pragma unroll
-        for (int i = 0; i < E::kVec; ++i)
-          add(E::get(x[k], i), r.head + static_cast<int64_t>(v) * E::kVec + i, 16 + (k * kThreads + tid) * E::kVec + i);
+      const int v = (c * NV + k) * kThreads + tid;
+      sum[k] = 0.0;
+      each<E>(r, v, x[k], [&](float y, int i, int) { sum[k] += weigh(y, i); });
     }
-    const auto plus = [](double p, double q) { return p + q; };
-    all = reduce_lanes(all, 64, plus);
-    left = reduce_lanes(left, 64, plus);
-    if (lane == 0) s_sum[wave][0] = drawn.probs ? left : all, s_sum[wave][1] = all;
-    __syncthreads();
-    if (tid == 0) {
-      Sums* const to = a.sums + static_cast<int64_t>(b) * a.draws + c;
-      publish(&to->left, s_sum[0][0] + s_sum[1][0] + s_sum[2][0] + s_sum[3][0]);
-      publish(&to->all, s_sum[0][1] + s_sum[1][1] + s_sum[2][1] + s_sum[3][1]);
-      asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // they have arrived before the count does
-      s_flag = __hip_atomic_fetch_add(a.arrivals + b, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.draws - 1;
-    }
-    __syncthreads();
-    if (!s_flag) return;
+    if (!last_with_sums<NV>(sum, a.sums + (static_cast<int64_t>(b) * a.draws + c) * NV, a.arrivals + b, a.draws, s_sums, &sh.flag) || rest) return;
   }
+  const double* const sums = a.sums + static_cast<int64_t>(b) * a.draws * NV;
+  draw<E>(r, sums, a.draws * NV, total_of(sums, a.draws * NV), u0, sh, weigh, answer);
+}
 
-  // The last workgroup of the request: the chunk in which the cumulative weight passes u_0 times the total, by one wavefront
-  __shared__ int s_chunk, s_all;
-  __shared__ double s_before, s_goal;
-  if (wave == 0) {
-    const Sums* const sums = a.sums + static_cast<int64_t>(b) * a.draws;
-    double left = 0.0, all = 0.0;
-    for (int k = lane; k < a.draws; k += 64) left += take(&sums[k].left), all += take(&sums[k].all);
-    const auto plus = [](double p, double q) { return p + q; };
-    left = reduce_lanes(left, 64, plus);
-    all = reduce_lanes(all, 64, plus);
-    const bool whole = !(left > 0.0);  // nothing is left: the target's own distribution
-    const float u = a.uniforms[first];
-    const double goal = (u < 0.f ? 0.0 : static_cast<double>(u)) * (whole ? all : left);  // (NaN passes nothing: the last token)
-    double before = 0.0;
-    int chunk = -1, last = -1;
-    double before_last = 0.0;
-    for (int k0 = 0; k0 < a.draws && chunk < 0; k0 += 64) {
-      const int k = k0 + lane;
-      const double s = k < a.draws ? take(whole ? &sums[k].all : &sums[k].left) : 0.0;
-      double upto = s;
+// Element i0 .. of a row of the draft's probabilities; `aligned`: kVec of them at once
+template <int kVec>
+__device__ __forceinline__ void load_probs(const VerifyArgs& a, const char* row, int64_t i0, bool aligned, float (&out)[kVec]) {
+  if (aligned && a.probs_dtype == FP_DTYPE_F32) {
 #pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const double y = __shfl_up(upto, d);
-        if (lane >= d) upto += y;
-      }
-      const uint64_t past = __ballot(before + upto > goal), some = __ballot(s > 0.0);
-      if (past) {
-        const int l = __builtin_ctzll(past);
-        chunk = k0 + l;
-        before += __shfl(upto - s, l);
-      } else {
-        if (some) {
-          const int l = 63 - __builtin_clzll(some);
-          last = k0 + l;
-          before_last = before + __shfl(upto - s, l);
-        }
-        before += __shfl(upto, 63);
-      }
+    for (int h = 0; h < kVec / 4; ++h) {
+      const v4u four = *reinterpret_cast<const v4u*>(row + (i0 + h * 4) * 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) out[h * 4 + i] = F32::get(four, i);
     }
-    if (lane == 0) {
-      s_chunk = chunk >= 0 ? chunk : last;
-      s_before = chunk >= 0 ? before : before_last;
-      s_goal = goal;
-      s_all = whole;
-      s_place = -1;
-    }
-  }
-  __syncthreads();
-  const int chunk = s_chunk;
-  if (chunk < 0) {  // every token is refused
-    if (tid == 0) answer(-1);
-    return;
-  }
-  const bool take_away = drawn.probs && !s_all;
-  mark(chunk);
-  // its elements in order, a segment at a time: those in front, the vectors by rows of threads, those behind
-  double before = s_before;
-  const double goal = s_goal;
-  int last = -1;  // of this thread's elements, the last that weighs something
-  for (int seg = 0; seg < NV + 2; ++seg) {
-    int n = 0, place = 0;
-    int64_t i0 = 0;
-    float x[E::kVec];
-    if (seg == 0) {
-      if (chunk == 0 && tid < r.head) n = 1, i0 = tid, place = tid;
-    } else if (seg == NV + 1) {
-      if (chunk == a.draws - 1 && tid < r.tail) n = 1, i0 = r.behind() + tid, place = 8 + tid;
+  } else if (aligned) {
+    uint32_t two[kVec / 2];
+    if constexpr (kVec == 8) {
+      const v4u all = *reinterpret_cast<const v4u*>(row + i0 * 2);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) two[i] = all[i];
     } else {
-      const int v = chunk * kVectors + (seg - 1) * kThreads + tid;
-      if (v < r.vectors) n = E::kVec, i0 = r.head + static_cast<int64_t>(v) * E::kVec, place = 16 + ((seg - 1) * kThreads + tid) * E::kVec;
+      const uint2 all = *reinterpret_cast<const uint2*>(row + i0 * 2);
+      two[0] = all.x, two[1] = all.y;
     }
-    double w[E::kVec], sum = 0.0;
-    if (n == 1) x[0] = r.one(i0);
-    if (n > 1) {
-      const v4u all = *reinterpret_cast<const v4u*>(r.at + i0 * E::kBytes);
+    const bool bf16 = a.probs_dtype == FP_DTYPE_BF16;
 #pragma unroll
-      for (int i = 0; i < E::kVec; ++i) x[i] = E::get(all, i);
+    for (int i = 0; i < kVec; ++i) {
+      const v4u pack = {two[i / 2], 0, 0, 0};
+      out[i] = bf16 ? BF16::get(pack, i & 1) : F16::get(pack, i & 1);
     }
+  } else {
 #pragma unroll
-    for (int i = 0; i < E::kVec; ++i) {
-      w[i] = i < n ? left_of(x[i], i0 + i, place + i, take_away) : 0.0;
-      sum += w[i];
-      if (w[i] > 0.0) last = static_cast<int>(i0 + i);
-    }
-    double upto = sum;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const double y = __shfl_up(upto, d);
-      if (lane >= d) upto += y;
-    }
-    __syncthreads();  // the segment before has been read
-    if (lane == 63) s_sum[wave][0] = upto;
-    __syncthreads();
-    double ahead = before;
-    for (int k = 0; k < wave; ++k) ahead += s_sum[k][0];
-    for (int k = 0; k < kWaves; ++k) before += s_sum[k][0];
-    // the thread in which the weight passes the goal: the first one whose elements reach beyond it
-    double at = ahead + (upto - sum);
-    if (sum > 0.0 && at + sum > goal) {
-      int found = -1;
-#pragma unroll
-      for (int i = 0; i < E::kVec; ++i) {
-        at += w[i];
-        if (found < 0 && w[i] > 0.0 && at > goal) found = static_cast<int>(i0 + i);
-      }
-      if (found >= 0) atomicMin(reinterpret_cast<uint32_t*>(&s_place), static_cast<uint32_t>(found));
-    }
-    __syncthreads();
-    if (s_place >= 0) break;
+    for (int i = 0; i < kVec; ++i) out[i] = probability(a, row, i0 + i);
   }
-  if (s_place < 0) {  // u_0 at the very end: the last token that weighs something
-    last = reduce_lanes(last, 64, [](int p, int q) { return max(p, q); });
-    __syncthreads();
-    if (lane == 0) atomicMax(&s_place, last);
-    __syncthreads();
+}
+
+template <typename E, int NV>
+__global__ __launch_bounds__(kThreads) void verify_rest_kernel(const VerifyArgs a) {
+  __shared__ double s_sums[kWaves][NV];
+  __shared__ DrawShared sh;
+  const int tid = threadIdx.x;
+  const uint32_t b = blockIdx.x / static_cast<uint32_t>(a.draws);
+  const int c = blockIdx.x - b * a.draws, n = a.draws * NV;
+  const int64_t first = static_cast<int64_t>(b) * a.S;
+  const End end = a.ends[b];
+  if (!end.rest) return;
+  const float heat = heat_of(a, b), u0 = a.uniforms[first];
+  const double rate = kLog2e / heat;
+  const Row<E> r(a.logits + b * a.ls_b + end.node * a.ls_s, a.V);
+  const char* const probs = a.probs + b * a.ps_b + end.node * a.ps_s;
+  const int pe = a.probs_dtype == FP_DTYPE_F32 ? 4 : 2;
+  const bool aligned = reinterpret_cast<uintptr_t>(probs + r.head * pe) % (E::kVec * pe < 16 ? E::kVec * pe : 16) == 0;
+  v4u x[NV];
+  float q[NV][E::kVec];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int v = (c * NV + k) * kThreads + tid;
+    if (v < r.vectors) {
+      x[k] = r.load(v);
+      load_probs<E::kVec>(a, probs, r.head + static_cast<int64_t>(v) * E::kVec, aligned, q[k]);
+    }
   }
-  if (tid == 0) answer(s_place);
+  const double* const sums = a.sums + static_cast<int64_t>(b) * n;
+  double* const rests = a.rests + static_cast<int64_t>(b) * n;
+  const double all = total_of(sums, n), share = 1.0 / all;
+  const auto left_of = [&](float y, float p) { return fmax(0.0, weight(y, end.peak, rate) * share - static_cast<double>(p)); };
+  double sum[NV];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int v = (c * NV + k) * kThreads + tid;
+    sum[k] = 0.0;
+    each<E>(r, v, x[k], [&](float y, int i, int place) { sum[k] += left_of(y, place >= 0 ? q[k][place] : probability(a, probs, i)); });
+  }
+  if (!last_with_sums<NV>(sum, rests + c * NV, a.arrivals + a.B + b, a.draws, s_sums, &sh.flag)) return;
+  const auto answer = [&](int token, float x) {
+    a.answer[first + end.count] = token;
+    a.logprobs[first + end.count] = token < 0 ? 0.f : log_share(x, end.peak, 1.0 / heat, a.totals[b]);
+  };
+  const double left = total_of(rests, n);
+  if (left > 0.0)
+    draw<E>(r, rests, n, left, u0, sh, [&](float y, int i) { return left_of(y, probability(a, probs, i)); }, answer);
+  else  // nothing is left: the target's own distribution
+    draw<E>(r, sums, n, all, u0, sh, [&](float y, int) { return weight(y, end.peak, rate); }, answer);
 }
 
 struct Cut {
   int nv, chunks;
 };
-// Vectors a thread: as many as leave `wanted` workgroups, 8 (rows) or 4 (draws) at most.
-Cut cut_of(int64_t rows, int V, int vec, int most, int64_t wanted) {
+// Vectors a thread: as many as leave `wanted` workgroups, 4 at most.
+Cut cut_of(int64_t rows, int V, int vec, int64_t wanted) {
   const int64_t vectors = (static_cast<int64_t>(V) + vec - 1) / vec;
-  Cut c{most, 0};
+  Cut c{4, 0};
   for (;; c.nv /= 2) {
     c.chunks = static_cast<int>((vectors + kThreads * c.nv - 1) / (kThreads * c.nv));
     if (c.nv == 1 || rows * c.chunks >= wanted) return c;
   }
 }
-Cut rows_cut(int B, int S, int V, int vec) { return cut_of(static_cast<int64_t>(B) * S, V, vec, 8, 4ll * fp::compute_units()); }
-Cut draw_cut(int B, int V, int vec) { return cut_of(B, V, vec, 4, 2ll * fp::compute_units()); }
+Cut rows_cut(int B, int S, int V, int vec) { return cut_of(static_cast<int64_t>(B) * S, V, vec, 4ll * fp::compute_units()); }
+Cut draw_cut(int B, int V, int vec) { return cut_of(B, V, vec, 2ll * fp::compute_units()); }
 
 int check_shape(const char* what, int B, int S, int V) {
   if (B < 0 || S <= 0 || V <= 0) return fp::fail(FP_ERR_INVALID_ARGUMENT, "%s: bad sizes (B=%d S=%d V=%d)", what, B, S, V);
@@ -572,13 +672,16 @@ int check_shape(const char* what, int B, int S, int V) {
 }
 
 struct Layout {
-  int64_t parts, sums, bytes;
+  int64_t ends, totals, parts, sums, rests, bytes;
 };
-Layout layout_of(int B, int S, int64_t chunks, int64_t draws) {
+Layout layout_of(int64_t B, int S, const Cut& rows, const Cut& draw) {
   Layout l;
-  l.parts = (static_cast<int64_t>(B) * 4 + 15) / 16 * 16;
-  l.sums = l.parts + static_cast<int64_t>(B) * S * chunks * sizeof(Part);
-  l.bytes = l.sums + B * draws * static_cast<int64_t>(sizeof(Sums));
+  l.ends = (B * 8 + 15) / 16 * 16;
+  l.totals = l.ends + B * static_cast<int64_t>(sizeof(End));
+  l.parts = l.totals + (B * 8 + 15) / 16 * 16;
+  l.sums = l.parts + B * S * rows.chunks * static_cast<int64_t>(sizeof(Part));
+  l.rests = l.sums + B * draw.chunks * draw.nv * 8;
+  l.bytes = l.rests + B * draw.chunks * draw.nv * 8;
   return l;
 }
 
@@ -588,7 +691,7 @@ extern "C" int64_t fp_verify_drafts_workspace_bytes(int32_t B, int32_t S, int32_
   if (const int rc = check_shape("fp_verify_drafts_workspace_bytes", B, S, V)) return rc;
   int64_t most = 0;
   for (const int vec : {4, 8}) {
-    const int64_t n = layout_of(B, S, rows_cut(B, S, V, vec).chunks, draw_cut(B, V, vec).chunks).bytes;
+    const int64_t n = layout_of(B, S, rows_cut(B, S, V, vec), draw_cut(B, V, vec)).bytes;
     most = n > most ? n : most;
   }
   return most;
@@ -609,15 +712,16 @@ extern "C" int fp_verify_drafts(const void* logits, int64_t logits_stride_b, int
   if (!fp::aligned(logits, e) || !fp::aligned(draft_probs, pe))
     return fp::fail(FP_ERR_INVALID_ARGUMENT, "%s: logits and draft_probs must be aligned to their elements", what);
   const Cut rows = rows_cut(B, S, V, 16 / e), draw = draw_cut(B, V, 16 / e);
-  const Layout l = layout_of(B, S, rows.chunks, draw.chunks);
+  const Layout l = layout_of(B, S, rows, draw);
   if (!workspace || workspace_bytes < l.bytes || !fp::aligned(workspace, 16))
     return fp::fail(FP_ERR_WORKSPACE, "%s: workspace of %lld bytes, 16-byte aligned, is needed (got %lld)", what,
                     static_cast<long long>(l.bytes), static_cast<long long>(workspace_bytes));
   char* const ws = static_cast<char*>(workspace);
   const VerifyArgs a{static_cast<const char*>(logits), logits_stride_b * e, logits_stride_s * e, tokens, parents, uniforms, temperatures,
                      static_cast<const char*>(draft_probs), probs_stride_b * pe, probs_stride_s * pe, probs_dtype, accepted, path, answer,
-                     logprobs, reinterpret_cast<Part*>(ws + l.parts), reinterpret_cast<Sums*>(ws + l.sums), reinterpret_cast<int*>(ws), B, S, V,
-                     rows.chunks, draw.chunks};
+                     logprobs, reinterpret_cast<Part*>(ws + l.parts), reinterpret_cast<double*>(ws + l.sums),
+                     reinterpret_cast<double*>(ws + l.rests), reinterpret_cast<End*>(ws + l.ends), reinterpret_cast<double*>(ws + l.totals),
+                     reinterpret_cast<int*>(ws), B, S, V, rows.chunks, draw.chunks};
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const auto go = [&](auto kernel, int64_t grid) {
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, st, a);
@@ -626,16 +730,19 @@ extern "C" int fp_verify_drafts(const void* logits, int64_t logits_stride_b, int
     using E = decltype(element);
     const int64_t grid = static_cast<int64_t>(B) * S * rows.chunks;
     switch (rows.nv) {
-      case 8: go(verify_rows_kernel<E, 8>, grid); break;
       case 4: go(verify_rows_kernel<E, 4>, grid); break;
       case 2: go(verify_rows_kernel<E, 2>, grid); break;
       default: go(verify_rows_kernel<E, 1>, grid);
     }
     const int64_t draws = static_cast<int64_t>(B) * draw.chunks;
+    const auto decide = [&](auto walk, auto rest) {
+      go(walk, draws);
+      if (draft_probs) go(rest, draws);
+    };
     switch (draw.nv) {
-      case 4: go(verify_draw_kernel<E, 4>, draws); break;
-      case 2: go(verify_draw_kernel<E, 2>, draws); break;
-      default: go(verify_draw_kernel<E, 1>, draws);
+      case 4: decide(verify_walk_kernel<E, 4>, verify_rest_kernel<E, 4>); break;
+      case 2: decide(verify_walk_kernel<E, 2>, verify_rest_kernel<E, 2>); break;
+      default: decide(verify_walk_kernel<E, 1>, verify_rest_kernel<E, 1>);
     }
   };
   if (dtype == FP_DTYPE_F32)

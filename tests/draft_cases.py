@@ -135,7 +135,8 @@ class DraftBatch(SharedBatch):
 
 
 def verify(logits, tokens, parents, uniforms, temperatures=None, probs=None):
-    """One sequence's decision in float64: (accepted rows, answer, logprobs) and how near the nearest border lay, relative to the whole.
+    """One sequence's decision in float64: (accepted rows, answer, (log p, weight of the row's other tokens than its largest) of each) and
+    how near the nearest border lay, relative to the whole.
 
     logits [S, V] as float64, probs likewise or None."""
     S, V = logits.shape
@@ -163,6 +164,7 @@ def verify(logits, tokens, parents, uniforms, temperatures=None, probs=None):
             log_p = np.log(w / z) if z > 0 else np.full(V, -np.inf)
             if top < np.inf and z > 0:
                 log_p = (x - top) / heat - np.log(z)
+        others = (z - (w == 1).sum()) / z if z > 0 else 0.0
         left, stands, tested = w.copy(), None, False
         for j in [j for j in range(1, S) if parents[j] == node]:
             name, known = int(tokens[j]), 0 <= tokens[j] < V
@@ -187,7 +189,7 @@ def verify(logits, tokens, parents, uniforms, temperatures=None, probs=None):
         if stands is not None:
             rows.append(stands)
             answer.append(int(tokens[stands]))
-            says.append(log_p[int(tokens[stands])])
+            says.append((log_p[int(tokens[stands])], others))
             node = stands
             continue
         if greedy:
@@ -203,7 +205,7 @@ def verify(logits, tokens, parents, uniforms, temperatures=None, probs=None):
                 name = min(int(np.searchsorted(sums, goal, side="right")), int(np.nonzero(left)[0][-1]))
                 near = min(near, np.abs(sums[:-1][left[:-1] > 0] - goal).min(initial=np.inf) / sums[-1])
         answer.append(name)
-        says.append(log_p[name] if name >= 0 else 0.0)
+        says.append((log_p[name] if name >= 0 else 0.0, others))
         return rows, answer, says, near
 
 
@@ -228,8 +230,11 @@ def check_verified(got, logits, tokens, parents, uniforms, temperatures=None, pr
         assert accepted[b] == len(rows), (b, accepted[b], rows)
         assert path[b].tolist() == pad([0] + rows, -1), (b, path[b], rows)
         assert answer[b].tolist() == pad(words, -1), (b, answer[b], words)
-        want = np.array(pad(says, 0.0))
+        want, others = np.array(pad(says, (0.0, 0.0))).T
         off = np.abs(logprobs[b].double().numpy() - want)
-        # rounded once to 32 bits, from a logarithm of sums that are exact to 2^-50 V
-        assert (off <= np.abs(want) * 2.0 ** -24 + V * 2.0 ** -49 + 1e-300).all(), (b, off.max())
+        # Rounded once to 32 bits, from the logarithm of a row's sum.  In that the largest weights are 1 and the others are in 32 bits: off
+        # by 2^-23 (the exponential) and 2^-24 (a product), and where the difference of two 16-bit logits is not exact by 2^-24 ln 2 of
+        # their exponent p.  Weights of 2^-p count for V 2^-p at most, so that p is log2 V where it matters: 16 of 65536 tokens.
+        relative = 1.5 * 2.0 ** -23 + math.log2(max(V, 2)) * math.log(2) * 2.0 ** -24
+        assert (off <= np.abs(want) * 2.0 ** -24 + others * relative + V * 2.0 ** -49 + 1e-300).all(), (b, off.max())
     assert skipped <= B // 16
