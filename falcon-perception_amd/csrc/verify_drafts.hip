@@ -10,8 +10,8 @@
 // Which token that is depends on sums over the whole vocabulary to the last bits: next to the border between two tokens, and with
 // 65536 of them there is always one near, sums in 32 bits would answer by the order they are taken in.  So the row that is drawn from is
 // weighed in 64 bits, the exponential to 2^-51.  All other rows have to say no more than on which side of a draft's weight u (Z - R) lies:
-//  * rows: every row's maximum and sum, a chunk a workgroup, from one read of the logits.  Weights in 32 bits, their arguments in
-//    two parts, off by kBand at most, summed in 64.
+//  * rows: every row's maximum and sum, a chunk a workgroup, from one read of the logits.  Weights in 32 bits, off by kBand at
+//    most, summed in 64.
 //  * walk: every workgroup puts the chunks of its request's rows together and walks down the tree; a comparison within kBand of its
 //    border is made again with the row's sum in 64 bits (a few in a million).  Then it sums the weights of its part of the row that the walk
 //    ends at, and the last workgroup of a request draws.
@@ -26,7 +26,10 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kMaxTokens = 64;
-constexpr float kBand = 0x1p-18f;  // what a row's sum may be off by, relatively
+// What a row's sum may be off by, relatively.  A weight 2^-p in 32 bits is off by 2.5 p 2^-24 ln 2 (the difference, the product and the
+// rate rounded) and 2^-23 (the exponential), sums of 8 by 3 * 2^-24.  Weights of 2^-p are V 2^-p of a whole of 1 or more, so p counts up to
+// log2 V, 24: 2.9e-6 in all.
+constexpr float kBand = 0x1p-18f;
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
 struct BF16 {
@@ -82,7 +85,9 @@ struct VerifyArgs {
   End* ends;       // [B]
   double* totals;  // [B]: Z of the row that is drawn from, for the logarithm
   int* arrivals;   // [2, B]
-  int B, S, V, chunks, draws;
+  int B, S, V;
+  int chunks, chunk_vectors;  // of a row, and of a chunk
+  int draws;
 };
 
 // 2^t for t <= 0 (0 for NaN): t = n + f, 2^f by its Chebyshev interpolation of degree 10 on [-1/2, 1/2], off by 2^-51.
@@ -110,6 +115,17 @@ __device__ __forceinline__ double weight(float x, float peak, double rate) {
   if (x == peak) return peak == -INFINITY ? 0.0 : 1.0;
   return power2((static_cast<double>(x) - static_cast<double>(peak)) * rate);
 }
+
+// The same for many tokens of a row, without a branch between them where the largest logit is finite.
+struct Weights {
+  float peak;
+  double rate;
+  bool plain;
+  __device__ Weights(float peak, double rate) : peak(peak), rate(rate), plain(__builtin_amdgcn_readfirstlane(fabsf(peak) < INFINITY)) {}
+  __device__ __forceinline__ double operator()(float x) const {
+    return plain ? power2((static_cast<double>(x) - static_cast<double>(peak)) * rate) : weight(x, peak, rate);
+  }
+};
 
 __device__ __forceinline__ float heat_of(const VerifyArgs& a, int b) { return a.temperatures ? a.temperatures[b] : 1.f; }
 
@@ -177,25 +193,11 @@ __device__ __forceinline__ void each(const Row<E>& r, int v, const v4u& x, F f) 
 }
 
 // ---------------------------------------------------------------------------------------------------------------- rows
-// A weight in 32 bits.  Its exponent (x - peak) * rate is p + e: p rounded to 32 bits, e what the product and the difference were rounded
-// by (16-bit logits whose difference is not exact are off by 2^-24 of the larger one, and so is the exponent); 2^e = 1 + e ln 2.
-struct Rate {
-  float hi, lo;
-};
-template <typename E>
-__device__ __forceinline__ float weight32(float x, float peak, Rate rate) {
-  const float d = x - peak, p = fmaxf(d * rate.hi, -200.f);  // (-200: also of -inf and NaN)
-  float e = fmaf(d, rate.lo, fmaf(d, rate.hi, -p));
-  if constexpr (E::kBytes == 4) {
-    const float back = x - d, there = d + back;
-    e = fmaf((x - there) + (back - peak), rate.hi, e);
-  }
-  e = __builtin_amdgcn_fmed3f(e, -1.f, 1.f);
-  const float w = __builtin_amdgcn_exp2f(p);
-  return fmaf(w, e * 0x1.62e430p-1f, w);
-}
+// A thread has G vectors at a time, the next ones on their way meanwhile, and weighs by a logit of its own that moves only when a larger one
+// is more than 2^kSlack heavier: no exchange between threads before the end of the chunk.
+constexpr double kSlack = 20.0;
 
-template <typename E, int NV>  // vectors a thread
+template <typename E, int G>
 __global__ __launch_bounds__(kThreads) void verify_rows_kernel(const VerifyArgs a) {
   __shared__ float s_peak[kWaves];
   __shared__ int s_best[kWaves];
@@ -204,44 +206,95 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(const VerifyArgs 
   const uint32_t row = blockIdx.x / static_cast<uint32_t>(a.chunks), b = row / static_cast<uint32_t>(a.S);
   const int c = blockIdx.x - row * a.chunks, j = row - b * a.S;
   if (c == 0 && j == 0 && tid < 2) a.arrivals[tid * a.B + b] = 0;
-  if (!is_token(j, a.parents[row]) || a.parents[static_cast<int64_t>(b) * a.S] != -1) return;
-  const Row<E> r(a.logits + b * a.ls_b + j * a.ls_s, a.V);
-  const int v0 = c * (kThreads * NV) + tid;
-  v4u x[NV];
-#pragma unroll
-  for (int k = 0; k < NV; ++k)
-    if (v0 + k * kThreads < r.vectors) x[k] = r.load(v0 + k * kThreads);
+  const int parent = a.parents[row], root = a.parents[static_cast<int64_t>(b) * a.S];
   const float heat = heat_of(a, b);
+  if (!is_token(j, parent) || root != -1) return;
+  const Row<E> r(a.logits + b * a.ls_b + j * a.ls_s, a.V);
+  const int v_end = min((c + 1) * a.chunk_vectors, r.vectors);
+  int v = c * a.chunk_vectors + tid;
+  const bool greedy = !(heat > 0.f);
+  const double rate = kLog2e / (greedy ? 1.0 : heat);
+  const float rate32 = static_cast<float>(rate), slack = static_cast<float>(kSlack / rate);
 
-  float peak = -INFINITY;
+  float peak = -INFINITY, by = -INFINITY;  // by: what the thread weighs by
+  int best = INT32_MAX;
+  double sum = 0.0;
+  const auto load = [&](v4u (&x)[G], int v) {
 #pragma unroll
-  for (int k = 0; k < NV; ++k) each<E>(r, v0 + k * kThreads, x[k], [&](float y, int, int) { peak = fmaxf(peak, y); });
-  peak = reduce_lanes(peak, 64, [](float p, float q) { return fmaxf(p, q); });
-  if (lane == 0) s_peak[wave] = peak;
+    for (int k = 0; k < G; ++k) {
+      x[k] = v4u{0, 0, 0, 0};
+      if (v + k * kThreads < v_end) x[k] = r.load(v + k * kThreads);
+    }
+  };
+  const auto grow = [&](float top) {  // of the elements to come
+    if (top > by + slack) {
+      sum *= weight(by, top, rate);
+      by = top;
+    }
+  };
+  v4u x[G];
+  load(x, v);
+  for (; v < v_end; v += G * kThreads) {
+    v4u next[G];
+    load(next, v + G * kThreads);
+    float top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < G; ++k)
+      if (k == 0 || v + k * kThreads < v_end)
+#pragma unroll
+        for (int i = 0; i < E::kVec; ++i) top = fmaxf(top, E::get(x[k], i));
+    if (greedy && top > peak) {
+#pragma unroll
+      for (int k = G - 1; k >= 0; --k)
+        if (v + k * kThreads < v_end)
+#pragma unroll
+          for (int i = E::kVec - 1; i >= 0; --i) best = E::get(x[k], i) == top ? r.head + (v + k * kThreads) * E::kVec + i : best;
+    }
+    peak = fmaxf(peak, top);
+    grow(top);
+    const float zero = by == -INFINITY ? 0.f : by;
+#pragma unroll
+    for (int k = 0; k < G; ++k)
+      if (k == 0 || v + k * kThreads < v_end) {
+        float w[E::kVec];
+#pragma unroll
+        for (int i = 0; i < E::kVec; ++i) w[i] = __builtin_amdgcn_exp2f(fmaxf((E::get(x[k], i) - zero) * rate32, -200.f));  // (-inf, NaN: 0)
+#pragma unroll
+        for (int d = 1; d < E::kVec; d *= 2)
+#pragma unroll
+          for (int i = 0; i < E::kVec; i += 2 * d) w[i] += w[i + d];
+        sum += w[0];
+      }
+#pragma unroll
+    for (int k = 0; k < G; ++k) x[k] = next[k];
+  }
+  // the elements outside the whole 16 bytes: the first chunk's first threads and the last one's next 8
+  int loose = -1;
+  if (c == 0 && tid < r.head) loose = tid;
+  if (c == a.chunks - 1 && tid >= 8 && tid - 8 < r.tail) loose = r.behind() + tid - 8;
+  if (loose >= 0) {
+    const float y = r.one(loose);
+    if (y > peak || (y == peak && loose < best)) best = loose;
+    peak = fmaxf(peak, y);
+    grow(y);
+    sum += y > by ? 1.0 / weight(by, y, rate) : weight(y, by, rate);
+  }
+  float all = reduce_lanes(peak, 64, [](float p, float q) { return fmaxf(p, q); });
+  if (lane == 0) s_peak[wave] = all;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) peak = fmaxf(peak, s_peak[w]);
-
-  int best = INT32_MAX;
-  if (!(heat > 0.f)) {
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-      each<E>(r, v0 + k * kThreads, x[k], [&](float y, int i, int) { best = y == peak ? min(best, i) : best; });
-    best = reduce_lanes(best, 64, [](int p, int q) { return min(p, q); });
-  }
-  double sum = 0.0;
-  const double rate = kLog2e / (heat > 0.f ? heat : 1.0);
-  if (fabsf(peak) < INFINITY && rate > 0x1p-40 && rate < 0x1p40) {
-    const Rate parts{static_cast<float>(rate), static_cast<float>(rate - static_cast<float>(rate))};
-#pragma unroll
-    for (int k = 0; k < NV; ++k) each<E>(r, v0 + k * kThreads, x[k], [&](float y, int, int) { sum += weight32<E>(y, peak, parts); });
-  } else {  // infinite logits, temperatures out of all measure
+  for (int w = 0; w < kWaves; ++w) all = fmaxf(all, s_peak[w]);
+  if (fabsf(all) < INFINITY && rate > 0x1p-40 && rate < 0x1p40) {
+    sum *= weight(by, all, rate);
+  } else {  // infinite logits, temperatures out of all measure: once more, in 64 bits
+    sum = loose >= 0 ? weight(r.one(loose), all, rate) : 0.0;
+    for (int u = c * a.chunk_vectors + tid; u < v_end; u += kThreads) {
 #pragma nounroll
-    for (int k = 0; k < NV; ++k)
-      each<E>(r, v0 + k * kThreads, v0 + k * kThreads < r.vectors ? r.load(v0 + k * kThreads) : v4u{0, 0, 0, 0},
-              [&](float y, int, int) { sum += weight(y, peak, rate); });
+      for (int i = 0; i < E::kVec; ++i) sum += weight(r.one(r.head + u * E::kVec + i), all, rate);
+    }
   }
   sum = sum_lanes(sum);
+  if (greedy) best = reduce_lanes(peak == all ? best : INT32_MAX, 64, [](int p, int q) { return min(p, q); });
   if (lane == 0) {
     s_sum[wave] = sum;
     s_best[wave] = best;
@@ -249,7 +302,7 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(const VerifyArgs 
   __syncthreads();
   if (tid == 0) {
     for (int w = 1; w < kWaves; ++w) sum += s_sum[w], best = min(best, s_best[w]);
-    a.parts[blockIdx.x] = Part{sum, peak, best};
+    a.parts[blockIdx.x] = Part{sum, all, best};
   }
 }
 
@@ -301,10 +354,12 @@ __device__ __forceinline__ double total_of(const double* sums, int n) {
   return sum_lanes(all);
 }
 
-// The first token at which the weights of the row pass u times their total: `n` sums of 256 vectors each, `weigh(x, i)` a token's weight.
-// What it is goes to answer(token, x), by one thread; -1 if nothing weighs anything.
-template <typename E, typename W, typename A>
-__device__ __forceinline__ void draw(const Row<E>& r, const double* sums, int n, double total, float u, DrawShared& sh, W weigh, A answer) {
+// The first token at which the weights of the row pass u times their total: `n` sums of 256 vectors each, weigh(x, i, place, prepare(v)) the
+// weight of token i, which has this place in vector v (-1: in none).  What it is goes to answer(token, x), by one thread; -1 if nothing
+// weighs anything.
+template <typename E, typename P, typename W, typename A>
+__device__ __forceinline__ void draw(const Row<E>& r, const double* sums, int n, double total, float u, DrawShared& sh, P prepare, W weigh,
+                                     A answer) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const double goal = (u < 0.f ? 0.0 : static_cast<double>(u)) * total;  // (NaN passes nothing: the last token)
   double before = 0.0, before_last = 0.0;
@@ -332,13 +387,18 @@ __device__ __forceinline__ void draw(const Row<E>& r, const double* sums, int n,
   }
   const int v = part * kThreads + tid;
   const v4u x = v < r.vectors ? r.load(v) : v4u{0, 0, 0, 0};
-  double sum = 0.0;
+  double sum = 0.0, weights[E::kVec];
   int found = -1;
   float its = 0.f;
-  each<E>(r, v, x, [&](float y, int i, int) {
-    const double w = weigh(y, i);
+  const auto ready = prepare(v);
+#pragma unroll
+  for (int i = 0; i < E::kVec; ++i) weights[i] = v < r.vectors ? weigh(E::get(x, i), r.head + v * E::kVec + i, i, ready) : 0.0;
+  const auto weight_of = [&](float y, int i, int place) { return place >= 0 ? weights[place] : weigh(y, i, -1, ready); };
+  each<E>(r, v, x, [&](float y, int i, int place) {
+    const double w = weight_of(y, i, place);
     sum += w;
-    if (w > 0.0) found = i, its = y;  // the last that weighs something
+    found = w > 0.0 ? i : found;  // the last that weighs something
+    its = w > 0.0 ? y : its;
   });
   const double upto = scan_lanes(sum);
   if (lane == 63) sh.sum[wave] = upto;
@@ -350,10 +410,13 @@ __device__ __forceinline__ void draw(const Row<E>& r, const double* sums, int n,
   const bool passes = sum > 0.0 && at + sum > goal;
   if (passes) {
     bool done = false;
-    each<E>(r, v, x, [&](float y, int i, int) {
-      const double w = weigh(y, i);
+    each<E>(r, v, x, [&](float y, int i, int place) {
+      const double w = weight_of(y, i, place);
       at += w;
-      if (!done && w > 0.0 && at > goal) done = true, found = i, its = y;
+      const bool here = !done && w > 0.0 && at > goal;
+      found = here ? i : found;
+      its = here ? y : its;
+      done |= here;
     });
     atomicMin(&sh.place, found);
   }
@@ -391,42 +454,44 @@ __global__ __launch_bounds__(kThreads) void verify_walk_kernel(const VerifyArgs 
   const int64_t token = lane < S ? a.tokens[first + lane] : -1;
   const float u = lane < S ? a.uniforms[first + lane] : 0.f;
 
-  // every row's maximum and sum, `per` lanes a row
+  // every row's maximum and sum, `per` lanes a row: the first chunks are on their way before it is known which rows are tokens
   int per = 64;
   while (per > kThreads / S) per >>= 1;
-  {
-    const int j = tid / per;
-    if (j < S && there && is_token(j, a.parents[first + j])) {
-      Part t{0.0, -INFINITY, INT32_MAX};
-      const Part* const parts = a.parts + (first + j) * a.chunks;
-      for (int k = tid % per; k < a.chunks; k += per) {
-        const Part p = parts[k];
-        if (p.peak > t.peak) {
-          t.sum = t.sum * weight(t.peak, p.peak, rate) + p.sum;
-          t.best = p.best;
-          t.peak = p.peak;
-        } else {
-          t.sum += p.sum * weight(p.peak, t.peak, rate);
-          if (p.peak == t.peak) t.best = min(t.best, p.best);
-        }
-      }
-      const float peak = reduce_lanes(t.peak, per, [](float p, float q) { return fmaxf(p, q); });
-      const double total = reduce_lanes(t.sum * weight(t.peak, peak, rate), per, [](double p, double q) { return p + q; });
-      const int best = reduce_lanes(t.peak == peak ? t.best : INT32_MAX, per, [](int p, int q) { return min(p, q); });
-      if (tid % per == 0) {
-        s_peak[j] = peak;
-        s_total[j] = total;
-        s_best[j] = peak == -INFINITY ? -1 : best;
-      }
-    }
-  }
+  const int mine = tid / per, row = mine < S ? mine : 0;
+  const Part* const parts = a.parts + (first + row) * a.chunks;
+  Part t = parts[min(tid % per, a.chunks - 1)];
+  const bool is_row = mine < S && there && is_token(row, a.parents[first + row]);
   const bool child = there && lane > 0 && lane < S && parent >= 0 && parent < lane, known = token >= 0 && token < a.V;
-  const int at = child ? parent : 0;
+  const int at = child ? parent : 0, name = known ? static_cast<int>(token) : -1;
   float x = -INFINITY;
   double q = 0.0;
   if (wave == 0 && child && known) {
     x = E::at(a.logits + b * a.ls_b + at * a.ls_s + token * E::kBytes);
     if (a.probs) q = probability(a, a.probs + b * a.ps_b + at * a.ps_s, token);
+  }
+  if (tid % per >= a.chunks || !is_row) t = Part{0.0, -INFINITY, INT32_MAX};
+  if (is_row) {
+    for (int k = tid % per + per; k < a.chunks; k += per) {
+      const Part p = parts[k];
+      if (p.peak > t.peak) {
+        t.sum = t.sum * weight(t.peak, p.peak, rate) + p.sum;
+        t.best = p.best;
+        t.peak = p.peak;
+      } else {
+        t.sum += p.sum * weight(p.peak, t.peak, rate);
+        if (p.peak == t.peak) t.best = min(t.best, p.best);
+      }
+    }
+  }
+  {
+    const float peak = reduce_lanes(t.peak, per, [](float p, float q) { return fmaxf(p, q); });
+    const double total = reduce_lanes(t.sum * weight(t.peak, peak, rate), per, [](double p, double q) { return p + q; });
+    const int best = greedy ? reduce_lanes(t.peak == peak ? t.best : INT32_MAX, per, [](int p, int q) { return min(p, q); }) : 0;
+    if (is_row && tid % per == 0) {
+      s_peak[row] = peak;
+      s_total[row] = total;
+      s_best[row] = peak == -INFINITY ? -1 : best;
+    }
   }
   __syncthreads();
   if (!there) {
@@ -442,42 +507,43 @@ __global__ __launch_bounds__(kThreads) void verify_walk_kernel(const VerifyArgs 
 
   // the walk down the tree
   uint64_t exact = 0;  // rows whose sums are in 64 bits
-  double w = 0.0, refused = 0.0;
-  bool eldest = true;
-  if (wave == 0) {
-    if (child && known) w = weight(x, s_peak[at], rate);
-    for (int i = 1; i < S; ++i) {  // the siblings before this token: what they weigh, the same token once
-      const bool sibling = i < lane && __builtin_amdgcn_readlane(parent, i) == parent;
-      const bool same = __builtin_amdgcn_readlane(known ? static_cast<int>(token) : -1, i) == static_cast<int>(token);
-      const double theirs = lane_of(w, i);
-      if (sibling) {
-        eldest = false;
-        if (same) w = 0.0; else refused += theirs;
-      }
-    }
-  }
+  const double w = wave == 0 && child && known ? weight(x, s_peak[at], rate) : 0.0;
   for (;;) {
     if (wave == 0) {
-      const double z = s_total[at], side = a.probs ? u * q * z : u * (z - refused);
-      const bool asked = child && known && w > 0.0 && (!a.probs || eldest);
-      const bool takes = child && known && greedy ? token == s_best[at] : asked && side < w;
-      const bool near = asked && !greedy && !(exact >> at & 1) && fabs(side - w) <= kBand * (a.probs ? side : z);
-      int node = 0, count = 0, mine = lane == 0 ? 0 : -1, again = -1;  // mine: the lane-th of the path
-      for (;;) {
-        const uint64_t doubt = __ballot(near && parent == node), stand = __ballot(takes && parent == node);
-        // (a child that stands hides doubts about those behind it)
-        if (doubt && (stand == 0 || __builtin_ctzll(doubt) <= __builtin_ctzll(stand))) {
-          again = node;
-          break;
+      int node = 0, count = 0, path = lane == 0 ? 0 : -1, again = -1;  // path: its lane-th row
+      for (bool stands = true; stands;) {
+        // the children in turn: what those refused weigh, the same token once
+        const double z = s_total[node], doubt = exact >> node & 1 ? -1.0 : kBand * z;
+        const int best = s_best[node];
+        double refused = 0.0;
+        bool out = false;  // this lane's token is refused at this node
+        stands = false;
+        for (uint64_t left = __ballot(child && parent == node); left && !stands && again < 0; left &= left - 1) {
+          const int i = __builtin_ctzll(left), token_i = __builtin_amdgcn_readlane(name, i);
+          if (greedy) {
+            stands = token_i >= 0 && token_i == best;
+          } else if (a.probs) {
+            const double side = lane_of(static_cast<double>(u) * q, i) * z, w_i = lane_of(w, i);
+            if (w_i > 0.0 && fabs(side - w_i) <= (doubt < 0.0 ? -1.0 : kBand * side)) again = node;
+            stands = again < 0 && w_i > 0.0 && side < w_i;
+            if (!stands) break;  // of drafts that were drawn the first child only
+          } else if (token_i >= 0 && __ballot(out && name == token_i) == 0) {
+            const double side = lane_of(static_cast<double>(u), i) * (z - refused), w_i = lane_of(w, i);
+            if (w_i > 0.0 && fabs(side - w_i) <= doubt) again = node;
+            stands = again < 0 && w_i > 0.0 && side < w_i;
+            refused += w_i;
+          }
+          out |= lane == i;
+          if (stands) {
+            node = i;
+            ++count;
+            if (lane == count) path = i;
+          }
         }
-        if (stand == 0) break;
-        node = __builtin_ctzll(stand);
-        ++count;
-        if (lane == count) mine = node;
       }
       const bool here = child && parent == node, gone = here && known;
       const uint64_t out = __ballot(gone);
-      if (gone) s_out[__builtin_popcountll(out & ((1ull << lane) - 1))] = static_cast<int>(token);
+      if (gone) s_out[__builtin_popcountll(out & ((1ull << lane) - 1))] = name;
       const bool any = __ballot(here) != 0;
       if (lane == 0) {
         s_node = node;
@@ -488,16 +554,16 @@ __global__ __launch_bounds__(kThreads) void verify_walk_kernel(const VerifyArgs 
       }
       if (c == 0 && again < 0) {
         // the token of path[lane + 1] answers at place lane; the last place is the drawn one's
-        const int next = __shfl_down(mine, 1);
+        const int next = __shfl_down(path, 1);
         const int from = lane < count ? next : 0;
-        const int64_t name = __shfl(token, from);
+        const int64_t says_token = __shfl(token, from);
         const float its = __shfl(x, from);
         const int under = __shfl(at, from);
         if (lane < S) {
-          a.path[first + lane] = mine;
+          a.path[first + lane] = path;
           if (lane != count) {
             const bool says = lane < count;
-            a.answer[first + lane] = says ? name : -1;
+            a.answer[first + lane] = says ? says_token : -1;
             a.logprobs[first + lane] = says ? log_share(its, s_peak[under], slope, s_total[under]) : 0.f;
           }
         }
@@ -510,9 +576,10 @@ __global__ __launch_bounds__(kThreads) void verify_walk_kernel(const VerifyArgs 
     // too near to its border: the row's sum once more, in 64 bits
     const Row<E> r(a.logits + b * a.ls_b + again * a.ls_s, a.V);
     const float peak = s_peak[again];
+    const Weights weigh(peak, rate);
     double sum = 0.0;
     for (int v = tid; v < max(r.vectors, 1); v += kThreads)
-      each<E>(r, v, v < r.vectors ? r.load(v) : v4u{0, 0, 0, 0}, [&](float y, int, int) { sum += weight(y, peak, rate); });
+      each<E>(r, v, v < r.vectors ? r.load(v) : v4u{0, 0, 0, 0}, [&](float y, int, int) { sum += weigh(y); });
     sum = sum_lanes(sum);
     if (lane == 0) sh.sum[wave] = sum;
     __syncthreads();
@@ -539,11 +606,23 @@ __global__ __launch_bounds__(kThreads) void verify_walk_kernel(const VerifyArgs 
     return;
   }
   const int n_out = a.probs ? 0 : s_n_out;
-  // the weight of token i, 0 if it was refused
-  const auto weigh = [&](float y, int i) {
-    double w = weight(y, peak, rate);
-    for (int k = 0; k < n_out; ++k) w = s_out[k] == i ? 0.0 : w;
-    return w;
+  const Weights weights(peak, rate);
+  // which of a vector's tokens were refused, a bit each; and the weight of token i, 0 if it was
+  const auto prepare = [&](int v) {
+    uint32_t out = 0;
+    for (int k = 0; k < n_out; ++k) {
+      const uint32_t place = s_out[k] - (r.head + v * E::kVec);
+      if (place < E::kVec) out |= 1u << place;
+    }
+    return out;
+  };
+  const auto weigh = [&](float y, int i, int place, uint32_t out) {
+    bool refused = false;
+    if (place >= 0)
+      refused = out >> place & 1;
+    else
+      for (int k = 0; k < n_out; ++k) refused |= s_out[k] == i;
+    return refused ? 0.0 : weights(y);
   };
   {
     v4u x[NV];
@@ -557,12 +636,13 @@ __global__ __launch_bounds__(kThreads) void verify_walk_kernel(const VerifyArgs 
     for (int k = 0; k < NV; ++k) {
       const int v = (c * NV + k) * kThreads + tid;
       sum[k] = 0.0;
-      each<E>(r, v, x[k], [&](float y, int i, int) { sum[k] += weigh(y, i); });
+      const uint32_t out = prepare(v);
+      each<E>(r, v, x[k], [&](float y, int i, int place) { sum[k] += weigh(y, i, place, out); });
     }
     if (!last_with_sums<NV>(sum, a.sums + (static_cast<int64_t>(b) * a.draws + c) * NV, a.arrivals + b, a.draws, s_sums, &sh.flag) || rest) return;
   }
   const double* const sums = a.sums + static_cast<int64_t>(b) * a.draws * NV;
-  draw<E>(r, sums, a.draws * NV, total_of(sums, a.draws * NV), u0, sh, weigh, answer);
+  draw<E>(r, sums, a.draws * NV, total_of(sums, a.draws * NV), u0, sh, prepare, weigh, answer);
 }
 
 // Element i0 .. of a row of the draft's probabilities; `aligned`: kVec of them at once
@@ -626,7 +706,8 @@ __global__ __launch_bounds__(kThreads) void verify_rest_kernel(const VerifyArgs 
   const double* const sums = a.sums + static_cast<int64_t>(b) * n;
   double* const rests = a.rests + static_cast<int64_t>(b) * n;
   const double all = total_of(sums, n), share = 1.0 / all;
-  const auto left_of = [&](float y, float p) { return fmax(0.0, weight(y, end.peak, rate) * share - static_cast<double>(p)); };
+  const Weights weights(end.peak, rate);
+  const auto left_of = [&](float y, float p) { return fmax(0.0, weights(y) * share - static_cast<double>(p)); };
   double sum[NV];
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
@@ -639,27 +720,38 @@ __global__ __launch_bounds__(kThreads) void verify_rest_kernel(const VerifyArgs 
     a.answer[first + end.count] = token;
     a.logprobs[first + end.count] = token < 0 ? 0.f : log_share(x, end.peak, 1.0 / heat, a.totals[b]);
   };
+  struct Probs {
+    float of[E::kVec];
+  };
+  // nothing left: the target's own distribution
   const double left = total_of(rests, n);
-  if (left > 0.0)
-    draw<E>(r, rests, n, left, u0, sh, [&](float y, int i) { return left_of(y, probability(a, probs, i)); }, answer);
-  else  // nothing is left: the target's own distribution
-    draw<E>(r, sums, n, all, u0, sh, [&](float y, int) { return weight(y, end.peak, rate); }, answer);
+  const bool whole = !(left > 0.0);
+  const auto prepare = [&](int v) {
+    Probs p = {};
+    if (v < r.vectors && !whole) load_probs<E::kVec>(a, probs, r.head + static_cast<int64_t>(v) * E::kVec, aligned, p.of);
+    return p;
+  };
+  const auto weigh = [&](float y, int i, int place, const Probs& p) {
+    if (whole) return weights(y);
+    return left_of(y, place >= 0 ? p.of[place] : probability(a, probs, i));
+  };
+  draw<E>(r, whole ? sums : rests, n, whole ? all : left, u0, sh, prepare, weigh, answer);
 }
 
 struct Cut {
   int nv, chunks;
 };
-// Vectors a thread: as many as leave `wanted` workgroups, 4 at most.
-Cut cut_of(int64_t rows, int V, int vec, int64_t wanted) {
+// Vectors a thread: as many as leave `wanted` workgroups, `most` at most.
+Cut cut_of(int64_t rows, int V, int vec, int most, int64_t wanted) {
   const int64_t vectors = (static_cast<int64_t>(V) + vec - 1) / vec;
-  Cut c{4, 0};
+  Cut c{most, 0};
   for (;; c.nv /= 2) {
     c.chunks = static_cast<int>((vectors + kThreads * c.nv - 1) / (kThreads * c.nv));
     if (c.nv == 1 || rows * c.chunks >= wanted) return c;
   }
 }
-Cut rows_cut(int B, int S, int V, int vec) { return cut_of(static_cast<int64_t>(B) * S, V, vec, 4ll * fp::compute_units()); }
-Cut draw_cut(int B, int V, int vec) { return cut_of(B, V, vec, 2ll * fp::compute_units()); }
+Cut rows_cut(int B, int S, int V, int vec) { return cut_of(static_cast<int64_t>(B) * S, V, vec, 16, 6ll * fp::compute_units()); }
+Cut draw_cut(int B, int V, int vec) { return cut_of(B, V, vec, 4, 2ll * fp::compute_units()); }
 
 int check_shape(const char* what, int B, int S, int V) {
   if (B < 0 || S <= 0 || V <= 0) return fp::fail(FP_ERR_INVALID_ARGUMENT, "%s: bad sizes (B=%d S=%d V=%d)", what, B, S, V);
@@ -721,7 +813,7 @@ extern "C" int fp_verify_drafts(const void* logits, int64_t logits_stride_b, int
                      static_cast<const char*>(draft_probs), probs_stride_b * pe, probs_stride_s * pe, probs_dtype, accepted, path, answer,
                      logprobs, reinterpret_cast<Part*>(ws + l.parts), reinterpret_cast<double*>(ws + l.sums),
                      reinterpret_cast<double*>(ws + l.rests), reinterpret_cast<End*>(ws + l.ends), reinterpret_cast<double*>(ws + l.totals),
-                     reinterpret_cast<int*>(ws), B, S, V, rows.chunks, draw.chunks};
+                     reinterpret_cast<int*>(ws), B, S, V, rows.chunks, rows.nv * kThreads, draw.chunks};
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const auto go = [&](auto kernel, int64_t grid) {
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, st, a);
@@ -730,9 +822,9 @@ extern "C" int fp_verify_drafts(const void* logits, int64_t logits_stride_b, int
     using E = decltype(element);
     const int64_t grid = static_cast<int64_t>(B) * S * rows.chunks;
     switch (rows.nv) {
-      case 4: go(verify_rows_kernel<E, 4>, grid); break;
+      default: go(verify_rows_kernel<E, 4>, grid); break;
       case 2: go(verify_rows_kernel<E, 2>, grid); break;
-      default: go(verify_rows_kernel<E, 1>, grid);
+      case 1: go(verify_rows_kernel<E, 1>, grid);
     }
     const int64_t draws = static_cast<int64_t>(B) * draw.chunks;
     const auto decide = [&](auto walk, auto rest) {

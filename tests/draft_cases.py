@@ -209,6 +209,22 @@ def verify(logits, tokens, parents, uniforms, temperatures=None, probs=None):
         return rows, answer, says, near
 
 
+def sum_bounds(V):
+    """How far the logarithm of a row's sum may be off, in parts of what its smaller logits weigh, and in all.
+
+    The sum's weights are in 32 bits.  A weight 2^-p is off by 2.5 p 2^-24 ln 2 (difference, product and rate rounded) and 2^-23 (the
+    exponential); weights of 2^-p are V 2^-p of the whole at most, so that p is log2 V where it matters, 16 of 65536 tokens.  Sums of 8 are off by
+    3 * 2^-24, the largest weight and all, and that by 2^-22 where a thread weighs by a logit with up to 2^20 to spare."""
+    return 2.0 ** -23 + 2.5 * math.log2(max(V, 2)) * math.log(2) * 2.0 ** -24, 3 * 2.0 ** -24 + 2.0 ** -22
+
+
+def same_answers(one, other, V):
+    """Whether two calls on the same logits, cut differently, decide alike; logprobs are within what each may be off by."""
+    for x, y in zip(one[:3], other[:3]):
+        assert torch.equal(x, y)
+    assert torch.allclose(one[3], other[3], rtol=2.0 ** -23, atol=2 * sum(sum_bounds(V)))
+
+
 def check_verified(got, logits, tokens, parents, uniforms, temperatures=None, probs=None):
     """A `VerifiedDrafts` against `verify`, decision by decision.  The decisions of two float64 computations can differ where a border
     is nearer than their sums are exact (weights to 2^-50, sums over V terms): such inputs are not compared, and there are hardly any."""
@@ -232,9 +248,6 @@ def check_verified(got, logits, tokens, parents, uniforms, temperatures=None, pr
         assert answer[b].tolist() == pad(words, -1), (b, answer[b], words)
         want, others = np.array(pad(says, (0.0, 0.0))).T
         off = np.abs(logprobs[b].double().numpy() - want)
-        # Rounded once to 32 bits, from the logarithm of a row's sum.  In that the largest weights are 1 and the others are in 32 bits: off
-        # by 2^-23 (the exponential) and 2^-24 (a product), and where the difference of two 16-bit logits is not exact by 2^-24 ln 2 of
-        # their exponent p.  Weights of 2^-p count for V 2^-p at most, so that p is log2 V where it matters: 16 of 65536 tokens.
-        relative = 1.5 * 2.0 ** -23 + math.log2(max(V, 2)) * math.log(2) * 2.0 ** -24
-        assert (off <= np.abs(want) * 2.0 ** -24 + others * relative + V * 2.0 ** -49 + 1e-300).all(), (b, off.max())
+        relative, whole = sum_bounds(V)
+        assert (off <= np.abs(want) * 2.0 ** -24 + others * relative + whole + V * 2.0 ** -49).all(), (b, off.max())
     assert skipped <= B // 16

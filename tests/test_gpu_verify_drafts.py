@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from falcon_perception_amd import ops
-from tests.draft_cases import check_verified, random_tree
+from tests.draft_cases import check_verified, random_tree, same_answers
 
 pytestmark = pytest.mark.gpu
 BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
@@ -215,12 +215,8 @@ def test_alignments_and_strides(dtype):
         view.copy_(step.logits)
         q = torch.full((B, S + 1, V + 11), float("nan"), dtype=dtype, device="cuda")
         q[:, 1:, offset:offset + V] = step.probs.cuda()
-        got = step.call(logits=view, draft_probs=q[:, 1:, offset:offset + V])
-        for w, g in zip(want, got):
-            assert torch.equal(w, g)
-    got = step.call(logits=step.logits.cuda().transpose(1, 2).contiguous().transpose(1, 2))
-    for w, g in zip(want, got):
-        assert torch.equal(w, g)
+        same_answers(want, step.call(logits=view, draft_probs=q[:, 1:, offset:offset + V]), V)
+    same_answers(want, step.call(logits=step.logits.cuda().transpose(1, 2).contiguous().transpose(1, 2)), V)
     one = Step(15, 1, 1, V, dtype)
     rows = one.logits.cuda().expand(300, 1, V)
     u = torch.rand(300, 1)
@@ -229,16 +225,13 @@ def test_alignments_and_strides(dtype):
 
 
 def test_the_answer_does_not_depend_on_the_batch():
-    """One request alone, in a batch of many, and with rows cut otherwise: the same decisions, and logprobs up to what a row's sum is off
-    by (check_verified: 2^-21 twice)."""
+    """One request alone, in a batch of many, and with rows cut otherwise: the same decisions."""
     step = Step(16, 64, 5, 30000, BF16, counts=[5, 4, 2])
     all_of = step.call()
     step.check(all_of)
     for b in (0, 17, 63):
         alone = ops.verify_drafts(step.logits[b:b + 1].cuda(), step.tokens[b:b + 1].cuda(), step.parents[b:b + 1].cuda(), step.uniforms[b:b + 1].cuda())
-        for w, g in zip(all_of[:3], alone[:3]):
-            assert torch.equal(w[b:b + 1], g)
-        assert torch.allclose(all_of.logprobs[b:b + 1], alone.logprobs, rtol=2.0 ** -23, atol=2.0 ** -19)
+        same_answers([t[b:b + 1] for t in all_of], alone, 30000)
 
 
 def test_draws_have_the_targets_distribution():
