@@ -80,14 +80,14 @@ struct VerifyArgs {
   int64_t* answer;
   float* logprobs;
   Part* parts;     // [B * S, chunks]
-  double* sums;    // [B, draws * NV]: weights of every 256 vectors of the row that is drawn from
-  double* rests;   // [B, draws * NV]: what is left of them
+  double* sums;    // [B, pieces]: weights of every 64 vectors of the row that is drawn from
+  double* rests;   // [B, pieces]: what is left of them
   End* ends;       // [B]
   double* totals;  // [B]: Z of the row that is drawn from, for the logarithm
   int* arrivals;   // [2, B]
   int B, S, V;
   int chunks, chunk_vectors;  // of a row, and of a chunk
-  int draws;
+  int draws, pieces;          // workgroups of a request, and pieces of 64 vectors
 };
 
 // 2^t for t <= 0 (0 for NaN): t = n + f, 2^f by its Chebyshev interpolation of degree 10 on [-1/2, 1/2], off by 2^-51.
@@ -328,21 +328,14 @@ struct DrawShared {
   int place, flag;
 };
 
-// The sums of this workgroup's 256 vectors each go to `to`; whether it is the last of `n` workgroups to say so.
-template <int NV>
-__device__ __forceinline__ bool last_with_sums(const double (&sum)[NV], double* to, int* counter, int n, double (*s_sum)[NV], int* flag) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-#pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const double all = sum_lanes(sum[k]);
-    if (lane == 0) s_sum[wave][k] = all;
-  }
+// Weights are summed by pieces of 64 vectors, a wavefront's.  The last workgroup of a request runs what follows alone, its instructions come from
+// memory as they are needed: loops, not copies of their bodies.
+
+// Whether this is the last of `n` workgroups whose sums are on their way.
+__device__ __forceinline__ bool last_to_arrive(int* counter, int n, int* flag) {
+  asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // this wavefront's have arrived
   __syncthreads();
-  if (wave == 0) {
-    if (lane < NV) publish(to + lane, s_sum[0][lane] + s_sum[1][lane] + s_sum[2][lane] + s_sum[3][lane]);
-    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // they have arrived before the count does
-    if (lane == 0) *flag = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
-  }
+  if (threadIdx.x == 0) *flag = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
   __syncthreads();
   return *flag != 0;
 }
@@ -354,16 +347,16 @@ __device__ __forceinline__ double total_of(const double* sums, int n) {
   return sum_lanes(all);
 }
 
-// The first token at which the weights of the row pass u times their total: `n` sums of 256 vectors each, weigh(x, i, place, prepare(v)) the
-// weight of token i, which has this place in vector v (-1: in none).  What it is goes to answer(token, x), by one thread; -1 if nothing
-// weighs anything.
-template <typename E, typename P, typename W, typename A>
-__device__ __forceinline__ void draw(const Row<E>& r, const double* sums, int n, double total, float u, DrawShared& sh, P prepare, W weigh,
-                                     A answer) {
+// The first token at which the weights of the row pass u times their total: sums of n pieces, weigh(x, i) the weight of token i.  What it is
+// goes to answer(token, x), by one thread; -1 if nothing weighs anything.
+template <typename E, typename W, typename A>
+__device__ __forceinline__ void draw(const Row<E>& r, int V, const double* sums, int n, double total, float u, DrawShared& sh, W weigh, A answer) {
+  constexpr int kEach = (64 * E::kVec + 2 * (E::kVec - 1) + kThreads - 1) / kThreads;  // elements of a piece, by threads
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const double goal = (u < 0.f ? 0.0 : static_cast<double>(u)) * total;  // (NaN passes nothing: the last token)
   double before = 0.0, before_last = 0.0;
   int part = -1, last = -1;
+#pragma nounroll
   for (int k0 = 0; k0 < n && part < 0; k0 += 64) {
     const double s = k0 + lane < n ? take(sums + k0 + lane) : 0.0, upto = scan_lanes(s);
     const uint64_t past = __ballot(before + upto > goal), some = __ballot(s > 0.0);
@@ -385,39 +378,40 @@ __device__ __forceinline__ void draw(const Row<E>& r, const double* sums, int n,
     if (tid == 0) answer(-1, 0.f);
     return;
   }
-  const int v = part * kThreads + tid;
-  const v4u x = v < r.vectors ? r.load(v) : v4u{0, 0, 0, 0};
-  double sum = 0.0, weights[E::kVec];
+  // its elements: those in front of the whole 16 bytes are the first piece's, those behind them the last one's
+  const int pieces = max((r.vectors + 63) / 64, 1), first = part == 0 ? 0 : r.head + part * 64 * E::kVec,
+            end = part == pieces - 1 ? V : r.head + (part + 1) * 64 * E::kVec, mine = first + tid * kEach;
+  double w[kEach], sum = 0.0;
+  float x[kEach];
   int found = -1;
   float its = 0.f;
-  const auto ready = prepare(v);
 #pragma unroll
-  for (int i = 0; i < E::kVec; ++i) weights[i] = v < r.vectors ? weigh(E::get(x, i), r.head + v * E::kVec + i, i, ready) : 0.0;
-  const auto weight_of = [&](float y, int i, int place) { return place >= 0 ? weights[place] : weigh(y, i, -1, ready); };
-  each<E>(r, v, x, [&](float y, int i, int place) {
-    const double w = weight_of(y, i, place);
-    sum += w;
-    found = w > 0.0 ? i : found;  // the last that weighs something
-    its = w > 0.0 ? y : its;
-  });
+  for (int i = 0; i < kEach; ++i) x[i] = mine + i < end ? r.one(mine + i) : 0.f;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    w[i] = mine + i < end ? weigh(x[i], mine + i) : 0.0;
+    sum += w[i];
+    found = w[i] > 0.0 ? mine + i : found;  // the last that weighs something
+    its = w[i] > 0.0 ? x[i] : its;
+  }
   const double upto = scan_lanes(sum);
   if (lane == 63) sh.sum[wave] = upto;
   if (tid == 0) sh.place = INT32_MAX;
   __syncthreads();
   double at = before;
-  for (int w = 0; w < wave; ++w) at += sh.sum[w];
+#pragma unroll
+  for (int k = 0; k < kWaves - 1; ++k) at += k < wave ? sh.sum[k] : 0.0;
   at += upto - sum;
-  const bool passes = sum > 0.0 && at + sum > goal;
-  if (passes) {
+  if (sum > 0.0 && at + sum > goal) {
     bool done = false;
-    each<E>(r, v, x, [&](float y, int i, int place) {
-      const double w = weight_of(y, i, place);
-      at += w;
-      const bool here = !done && w > 0.0 && at > goal;
-      found = here ? i : found;
-      its = here ? y : its;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      at += w[i];
+      const bool here = !done && w[i] > 0.0 && at > goal;
+      found = here ? mine + i : found;
+      its = here ? x[i] : its;
       done |= here;
-    });
+    }
     atomicMin(&sh.place, found);
   }
   __syncthreads();
@@ -431,14 +425,13 @@ __device__ __forceinline__ void draw(const Row<E>& r, const double* sums, int n,
   if (found >= 0 && found == sh.place) answer(found, its);
 }
 
-template <typename E, int NV>
+template <typename E>
 __global__ __launch_bounds__(kThreads) void verify_walk_kernel(const VerifyArgs a) {
   __shared__ float s_peak[kMaxTokens];
   __shared__ int s_best[kMaxTokens];
   __shared__ double s_total[kMaxTokens];
   __shared__ int s_out[kMaxTokens];  // refused tokens
   __shared__ int s_node, s_count, s_n_out, s_refused, s_again;
-  __shared__ double s_sums[kWaves][NV];
   __shared__ DrawShared sh;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint32_t b = blockIdx.x / static_cast<uint32_t>(a.draws);
@@ -607,42 +600,32 @@ __global__ __launch_bounds__(kThreads) void verify_walk_kernel(const VerifyArgs 
   }
   const int n_out = a.probs ? 0 : s_n_out;
   const Weights weights(peak, rate);
-  // which of a vector's tokens were refused, a bit each; and the weight of token i, 0 if it was
-  const auto prepare = [&](int v) {
-    uint32_t out = 0;
+  double* const sums = a.sums + static_cast<int64_t>(b) * a.pieces;
+  const auto is_out = [&](int i) {  // refused
+    bool out = false;
+#pragma nounroll
+    for (int k = 0; k < n_out; ++k) out |= s_out[k] == i;
+    return out;
+  };
+  for (int piece = c * kWaves + wave; piece < a.pieces; piece += a.draws * kWaves) {
+    const int v = piece * 64 + lane;
+    const v4u x = v < r.vectors ? r.load(v) : v4u{0, 0, 0, 0};
+    uint32_t out = 0;  // the vector's refused tokens, a bit each
+#pragma nounroll
     for (int k = 0; k < n_out; ++k) {
       const uint32_t place = s_out[k] - (r.head + v * E::kVec);
       if (place < E::kVec) out |= 1u << place;
     }
-    return out;
-  };
-  const auto weigh = [&](float y, int i, int place, uint32_t out) {
-    bool refused = false;
-    if (place >= 0)
-      refused = out >> place & 1;
-    else
-      for (int k = 0; k < n_out; ++k) refused |= s_out[k] == i;
-    return refused ? 0.0 : weights(y);
-  };
-  {
-    v4u x[NV];
-    double sum[NV];
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int v = (c * NV + k) * kThreads + tid;
-      if (v < r.vectors) x[k] = r.load(v);
-    }
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int v = (c * NV + k) * kThreads + tid;
-      sum[k] = 0.0;
-      const uint32_t out = prepare(v);
-      each<E>(r, v, x[k], [&](float y, int i, int place) { sum[k] += weigh(y, i, place, out); });
-    }
-    if (!last_with_sums<NV>(sum, a.sums + (static_cast<int64_t>(b) * a.draws + c) * NV, a.arrivals + b, a.draws, s_sums, &sh.flag) || rest) return;
+    double sum = 0.0;
+    each<E>(r, v, x, [&](float y, int i, int place) {
+      const double w = weights(y);
+      sum += (place >= 0 ? out >> place & 1 : is_out(i)) ? 0.0 : w;
+    });
+    sum = sum_lanes(sum);
+    if (lane == 0) publish(sums + piece, sum);
   }
-  const double* const sums = a.sums + static_cast<int64_t>(b) * a.draws * NV;
-  draw<E>(r, sums, a.draws * NV, total_of(sums, a.draws * NV), u0, sh, prepare, weigh, answer);
+  if (!last_to_arrive(a.arrivals + b, a.draws, &sh.flag) || rest) return;
+  draw<E>(r, a.V, sums, a.pieces, total_of(sums, a.pieces), u0, sh, [&](float y, int i) { return is_out(i) ? 0.0 : weights(y); }, answer);
 }
 
 // Element i0 .. of a row of the draft's probabilities; `aligned`: kVec of them at once
@@ -677,13 +660,12 @@ __device__ __forceinline__ void load_probs(const VerifyArgs& a, const char* row,
   }
 }
 
-template <typename E, int NV>
+template <typename E>
 __global__ __launch_bounds__(kThreads) void verify_rest_kernel(const VerifyArgs a) {
-  __shared__ double s_sums[kWaves][NV];
   __shared__ DrawShared sh;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint32_t b = blockIdx.x / static_cast<uint32_t>(a.draws);
-  const int c = blockIdx.x - b * a.draws, n = a.draws * NV;
+  const int c = blockIdx.x - b * a.draws, n = a.pieces;
   const int64_t first = static_cast<int64_t>(b) * a.S;
   const End end = a.ends[b];
   if (!end.rest) return;
@@ -693,49 +675,39 @@ __global__ __launch_bounds__(kThreads) void verify_rest_kernel(const VerifyArgs 
   const char* const probs = a.probs + b * a.ps_b + end.node * a.ps_s;
   const int pe = a.probs_dtype == FP_DTYPE_F32 ? 4 : 2;
   const bool aligned = reinterpret_cast<uintptr_t>(probs + r.head * pe) % (E::kVec * pe < 16 ? E::kVec * pe : 16) == 0;
-  v4u x[NV];
-  float q[NV][E::kVec];
-#pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int v = (c * NV + k) * kThreads + tid;
-    if (v < r.vectors) {
-      x[k] = r.load(v);
-      load_probs<E::kVec>(a, probs, r.head + static_cast<int64_t>(v) * E::kVec, aligned, q[k]);
-    }
-  }
   const double* const sums = a.sums + static_cast<int64_t>(b) * n;
   double* const rests = a.rests + static_cast<int64_t>(b) * n;
-  const double all = total_of(sums, n), share = 1.0 / all;
   const Weights weights(end.peak, rate);
+  double all = 0.0, share = 0.0;
   const auto left_of = [&](float y, float p) { return fmax(0.0, weights(y) * share - static_cast<double>(p)); };
-  double sum[NV];
-#pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int v = (c * NV + k) * kThreads + tid;
-    sum[k] = 0.0;
-    each<E>(r, v, x[k], [&](float y, int i, int place) { sum[k] += left_of(y, place >= 0 ? q[k][place] : probability(a, probs, i)); });
+  for (int piece = c * kWaves + wave; piece < n; piece += a.draws * kWaves) {
+    const int v = piece * 64 + lane;
+    v4u x = {0, 0, 0, 0};
+    float q[E::kVec];
+    if (v < r.vectors) {
+      x = r.load(v);
+      load_probs<E::kVec>(a, probs, r.head + static_cast<int64_t>(v) * E::kVec, aligned, q);
+    }
+    if (share == 0.0) {  // with the first ones on their way
+      all = total_of(sums, n);
+      share = 1.0 / all;
+    }
+    double sum = 0.0;
+    each<E>(r, v, x, [&](float y, int i, int place) { sum += left_of(y, place >= 0 ? q[place] : probability(a, probs, i)); });
+    sum = sum_lanes(sum);
+    if (lane == 0) publish(rests + piece, sum);
   }
-  if (!last_with_sums<NV>(sum, rests + c * NV, a.arrivals + a.B + b, a.draws, s_sums, &sh.flag)) return;
+  if (!last_to_arrive(a.arrivals + a.B + b, a.draws, &sh.flag)) return;
   const auto answer = [&](int token, float x) {
     a.answer[first + end.count] = token;
     a.logprobs[first + end.count] = token < 0 ? 0.f : log_share(x, end.peak, 1.0 / heat, a.totals[b]);
   };
-  struct Probs {
-    float of[E::kVec];
-  };
+  all = total_of(sums, n), share = 1.0 / all;  // (of a wavefront without a piece, too)
   // nothing left: the target's own distribution
   const double left = total_of(rests, n);
   const bool whole = !(left > 0.0);
-  const auto prepare = [&](int v) {
-    Probs p = {};
-    if (v < r.vectors && !whole) load_probs<E::kVec>(a, probs, r.head + static_cast<int64_t>(v) * E::kVec, aligned, p.of);
-    return p;
-  };
-  const auto weigh = [&](float y, int i, int place, const Probs& p) {
-    if (whole) return weights(y);
-    return left_of(y, place >= 0 ? p.of[place] : probability(a, probs, i));
-  };
-  draw<E>(r, whole ? sums : rests, n, whole ? all : left, u0, sh, prepare, weigh, answer);
+  draw<E>(r, a.V, whole ? sums : rests, n, whole ? all : left, u0, sh,
+          [&](float y, int i) { return whole ? weights(y) : left_of(y, probability(a, probs, i)); }, answer);
 }
 
 struct Cut {
@@ -751,7 +723,9 @@ Cut cut_of(int64_t rows, int V, int vec, int most, int64_t wanted) {
   }
 }
 Cut rows_cut(int B, int S, int V, int vec) { return cut_of(static_cast<int64_t>(B) * S, V, vec, 16, 6ll * fp::compute_units()); }
+// Workgroups of a request for the row that is drawn from: four pieces each, more where there are two for every CU without.
 Cut draw_cut(int B, int V, int vec) { return cut_of(B, V, vec, 4, 2ll * fp::compute_units()); }
+int pieces_of(int V, int vec) { return static_cast<int>((static_cast<int64_t>(V) + vec * 64 - 1) / (vec * 64)); }
 
 int check_shape(const char* what, int B, int S, int V) {
   if (B < 0 || S <= 0 || V <= 0) return fp::fail(FP_ERR_INVALID_ARGUMENT, "%s: bad sizes (B=%d S=%d V=%d)", what, B, S, V);
@@ -766,14 +740,14 @@ int check_shape(const char* what, int B, int S, int V) {
 struct Layout {
   int64_t ends, totals, parts, sums, rests, bytes;
 };
-Layout layout_of(int64_t B, int S, const Cut& rows, const Cut& draw) {
+Layout layout_of(int64_t B, int S, const Cut& rows, int64_t pieces) {
   Layout l;
   l.ends = (B * 8 + 15) / 16 * 16;
   l.totals = l.ends + B * static_cast<int64_t>(sizeof(End));
   l.parts = l.totals + (B * 8 + 15) / 16 * 16;
   l.sums = l.parts + B * S * rows.chunks * static_cast<int64_t>(sizeof(Part));
-  l.rests = l.sums + B * draw.chunks * draw.nv * 8;
-  l.bytes = l.rests + B * draw.chunks * draw.nv * 8;
+  l.rests = l.sums + B * pieces * 8;
+  l.bytes = l.rests + B * pieces * 8;
   return l;
 }
 
@@ -783,7 +757,7 @@ extern "C" int64_t fp_verify_drafts_workspace_bytes(int32_t B, int32_t S, int32_
   if (const int rc = check_shape("fp_verify_drafts_workspace_bytes", B, S, V)) return rc;
   int64_t most = 0;
   for (const int vec : {4, 8}) {
-    const int64_t n = layout_of(B, S, rows_cut(B, S, V, vec), draw_cut(B, V, vec)).bytes;
+    const int64_t n = layout_of(B, S, rows_cut(B, S, V, vec), pieces_of(V, vec)).bytes;
     most = n > most ? n : most;
   }
   return most;
@@ -804,7 +778,8 @@ extern "C" int fp_verify_drafts(const void* logits, int64_t logits_stride_b, int
   if (!fp::aligned(logits, e) || !fp::aligned(draft_probs, pe))
     return fp::fail(FP_ERR_INVALID_ARGUMENT, "%s: logits and draft_probs must be aligned to their elements", what);
   const Cut rows = rows_cut(B, S, V, 16 / e), draw = draw_cut(B, V, 16 / e);
-  const Layout l = layout_of(B, S, rows, draw);
+  const int pieces = pieces_of(V, 16 / e);
+  const Layout l = layout_of(B, S, rows, pieces);
   if (!workspace || workspace_bytes < l.bytes || !fp::aligned(workspace, 16))
     return fp::fail(FP_ERR_WORKSPACE, "%s: workspace of %lld bytes, 16-byte aligned, is needed (got %lld)", what,
                     static_cast<long long>(l.bytes), static_cast<long long>(workspace_bytes));
@@ -813,7 +788,7 @@ extern "C" int fp_verify_drafts(const void* logits, int64_t logits_stride_b, int
                      static_cast<const char*>(draft_probs), probs_stride_b * pe, probs_stride_s * pe, probs_dtype, accepted, path, answer,
                      logprobs, reinterpret_cast<Part*>(ws + l.parts), reinterpret_cast<double*>(ws + l.sums),
                      reinterpret_cast<double*>(ws + l.rests), reinterpret_cast<End*>(ws + l.ends), reinterpret_cast<double*>(ws + l.totals),
-                     reinterpret_cast<int*>(ws), B, S, V, rows.chunks, rows.nv * kThreads, draw.chunks};
+                     reinterpret_cast<int*>(ws), B, S, V, rows.chunks, rows.nv * kThreads, draw.chunks, pieces};
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const auto go = [&](auto kernel, int64_t grid) {
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, st, a);
@@ -827,15 +802,8 @@ extern "C" int fp_verify_drafts(const void* logits, int64_t logits_stride_b, int
       case 1: go(verify_rows_kernel<E, 1>, grid);
     }
     const int64_t draws = static_cast<int64_t>(B) * draw.chunks;
-    const auto decide = [&](auto walk, auto rest) {
-      go(walk, draws);
-      if (draft_probs) go(rest, draws);
-    };
-    switch (draw.nv) {
-      case 4: decide(verify_walk_kernel<E, 4>, verify_rest_kernel<E, 4>); break;
-      case 2: decide(verify_walk_kernel<E, 2>, verify_rest_kernel<E, 2>); break;
-      default: decide(verify_walk_kernel<E, 1>, verify_rest_kernel<E, 1>);
-    }
+    go(verify_walk_kernel<E>, draws);
+    if (draft_probs) go(verify_rest_kernel<E>, draws);
   };
   if (dtype == FP_DTYPE_F32)
     launch(F32{});
