@@ -13,10 +13,11 @@
 //  * rows: every row's maximum and sum, a chunk a workgroup, from one read of the logits.  Weights in 32 bits, off by kBand at
 //    most, summed in 64.
 //  * walk: every workgroup puts the chunks of its request's rows together and walks down the tree; a comparison within kBand of its
-//    border is made again with the row's sum in 64 bits (a few in a million).  Then it sums the weights of its part of the row that the walk
-//    ends at, and the last workgroup of a request draws.
-//  * rest: where the drafts were drawn, what is left of the target's distribution needs Z first: the same once more, with Z.
-// The first launch sets the counters of the others to 0: nothing is kept between calls.
+//    border is made again with the row's sum in 64 bits (a few in a million).  Then it sums the weights of its pieces of the row that the walk
+//    ends at, and the last workgroup of a request draws.  Where the drafts were drawn, Z is known only then: until then a piece has the
+//    sums of w and of q over the tokens that surely have something left, and one with a token within kBand of its border (every 100 pieces,
+//    if p and q have nothing to do with each other) is weighed again by the last workgroup.
+// The first launch sets the counters of the second to 0: nothing is kept between calls.
 #include "fp_common.h"
 
 #include <math.h>
@@ -59,10 +60,9 @@ struct Part {   // of a chunk of a row
   float peak;
   int best;     // the first place of `peak`, where the request is greedy
 };
-struct End {    // of a request's walk
-  int node, count;
-  int rest;     // something is taken away: what is left is weighed by the third launch
-  float peak;
+struct Piece {  // of 64 vectors of the row that is drawn from
+  double all;   // the weights
+  double kept, taken;  // of the tokens that surely have something left: weights, and the draft's probabilities; kept < 0: of some it is not sure
 };
 
 struct VerifyArgs {
@@ -80,11 +80,9 @@ struct VerifyArgs {
   int64_t* answer;
   float* logprobs;
   Part* parts;     // [B * S, chunks]
-  double* sums;    // [B, pieces]: weights of every 64 vectors of the row that is drawn from
+  Piece* sums;     // [B, pieces]
   double* rests;   // [B, pieces]: what is left of them
-  End* ends;       // [B]
-  double* totals;  // [B]: Z of the row that is drawn from, for the logarithm
-  int* arrivals;   // [2, B]
+  int* arrivals;   // [B]
   int B, S, V;
   int chunks, chunk_vectors;  // of a row, and of a chunk
   int draws, pieces;          // workgroups of a request, and pieces of 64 vectors
@@ -205,7 +203,7 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(const VerifyArgs 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint32_t row = blockIdx.x / static_cast<uint32_t>(a.chunks), b = row / static_cast<uint32_t>(a.S);
   const int c = blockIdx.x - row * a.chunks, j = row - b * a.S;
-  if (c == 0 && j == 0 && tid < 2) a.arrivals[tid * a.B + b] = 0;
+  if (c == 0 && j == 0 && tid == 0) a.arrivals[b] = 0;
   const int parent = a.parents[row], root = a.parents[static_cast<int64_t>(b) * a.S];
   const float heat = heat_of(a, b);
   if (!is_token(j, parent) || root != -1) return;
@@ -340,25 +338,32 @@ __device__ __forceinline__ bool last_to_arrive(int* counter, int n, int* flag) {
   return *flag != 0;
 }
 
-// All of n published sums together, by each wavefront: the same in every one that asks.
-__device__ __forceinline__ double total_of(const double* sums, int n) {
-  double all = 0.0;
-  for (int k = threadIdx.x & 63; k < n; k += 64) all += take(sums + k);
-  return sum_lanes(all);
+// Elements of a piece, by threads; and the first and the end of piece k: what is in front of the whole 16 bytes is the first one's, what is behind
+// them the last one's.
+template <typename E>
+constexpr int elements_each() { return (64 * E::kVec + 2 * (E::kVec - 1) + kThreads - 1) / kThreads; }
+template <typename E>
+__device__ __forceinline__ int2 piece_range(const Row<E>& r, int V, int k) {
+  const int pieces = max((r.vectors + 63) / 64, 1);
+  return int2{k == 0 ? 0 : r.head + k * 64 * E::kVec, k == pieces - 1 ? V : r.head + (k + 1) * 64 * E::kVec};
 }
 
-// The first token at which the weights of the row pass u times their total: sums of n pieces, weigh(x, i) the weight of token i.  What it is
-// goes to answer(token, x), by one thread; -1 if nothing weighs anything.
-template <typename E, typename W, typename A>
-__device__ __forceinline__ void draw(const Row<E>& r, int V, const double* sums, int n, double total, float u, DrawShared& sh, W weigh, A answer) {
-  constexpr int kEach = (64 * E::kVec + 2 * (E::kVec - 1) + kThreads - 1) / kThreads;  // elements of a piece, by threads
+// The first token at which the weights of the row pass u times their total: sum_of(k) the sum of piece k of n, weigh(x, i) the weight of
+// token i.  What it is goes to answer(token, x), by one thread; -1 if nothing weighs anything.
+template <typename E, typename S, typename W, typename A>
+__device__ __forceinline__ void draw(const Row<E>& r, int V, S sum_of, int n, float u, DrawShared& sh, W weigh, A answer) {
+  constexpr int kEach = elements_each<E>();
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const double goal = (u < 0.f ? 0.0 : static_cast<double>(u)) * total;  // (NaN passes nothing: the last token)
+  // by every wavefront, which all get the same
+  double total = 0.0;
+#pragma nounroll
+  for (int k = lane; k < n; k += 64) total += sum_of(k);
+  const double goal = (u < 0.f ? 0.0 : static_cast<double>(u)) * sum_lanes(total);  // (NaN passes nothing: the last token)
   double before = 0.0, before_last = 0.0;
   int part = -1, last = -1;
 #pragma nounroll
   for (int k0 = 0; k0 < n && part < 0; k0 += 64) {
-    const double s = k0 + lane < n ? take(sums + k0 + lane) : 0.0, upto = scan_lanes(s);
+    const double s = n <= 64 ? total : k0 + lane < n ? sum_of(k0 + lane) : 0.0, upto = scan_lanes(s);
     const uint64_t past = __ballot(before + upto > goal), some = __ballot(s > 0.0);
     if (past) {
       const int l = __builtin_ctzll(past);
@@ -378,9 +383,8 @@ __device__ __forceinline__ void draw(const Row<E>& r, int V, const double* sums,
     if (tid == 0) answer(-1, 0.f);
     return;
   }
-  // its elements: those in front of the whole 16 bytes are the first piece's, those behind them the last one's
-  const int pieces = max((r.vectors + 63) / 64, 1), first = part == 0 ? 0 : r.head + part * 64 * E::kVec,
-            end = part == pieces - 1 ? V : r.head + (part + 1) * 64 * E::kVec, mine = first + tid * kEach;
+  const int2 range = piece_range(r, V, part);
+  const int mine = range.x + tid * kEach, end = range.y;
   double w[kEach], sum = 0.0;
   float x[kEach];
   int found = -1;
@@ -423,6 +427,38 @@ __device__ __forceinline__ void draw(const Row<E>& r, int V, const double* sums,
     __syncthreads();
   }
   if (found >= 0 && found == sh.place) answer(found, its);
+}
+
+// Element i0 .. of a row of the draft's probabilities; `aligned`: kVec of them at once
+template <int kVec>
+__device__ __forceinline__ void load_probs(const VerifyArgs& a, const char* row, int64_t i0, bool aligned, float (&out)[kVec]) {
+  if (aligned && a.probs_dtype == FP_DTYPE_F32) {
+#pragma unroll
+    for (int h = 0; h < kVec / 4; ++h) {
+      const v4u four = *reinterpret_cast<const v4u*>(row + (i0 + h * 4) * 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) out[h * 4 + i] = F32::get(four, i);
+    }
+  } else if (aligned) {
+    uint32_t two[kVec / 2];
+    if constexpr (kVec == 8) {
+      const v4u all = *reinterpret_cast<const v4u*>(row + i0 * 2);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) two[i] = all[i];
+    } else {
+      const uint2 all = *reinterpret_cast<const uint2*>(row + i0 * 2);
+      two[0] = all.x, two[1] = all.y;
+    }
+    const bool bf16 = a.probs_dtype == FP_DTYPE_BF16;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      const v4u pack = {two[i / 2], 0, 0, 0};
+      out[i] = bf16 ? BF16::get(pack, i & 1) : F16::get(pack, i & 1);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) out[i] = probability(a, row, i0 + i);
+  }
 }
 
 template <typename E>
@@ -494,7 +530,6 @@ __global__ __launch_bounds__(kThreads) void verify_walk_kernel(const VerifyArgs 
       a.logprobs[first + tid] = 0.f;
       if (tid == 0) a.accepted[b] = 0;
     }
-    if (c == 0 && tid == 0) a.ends[b] = End{0, 0, 0, 0.f};
     return;
   }
 
@@ -589,124 +624,124 @@ __global__ __launch_bounds__(kThreads) void verify_walk_kernel(const VerifyArgs 
     a.answer[first + count] = token;
     a.logprobs[first + count] = token < 0 ? 0.f : log_share(x, peak, slope, total);
   };
-  const bool rest = a.probs && s_refused && !greedy && peak > -INFINITY;
-  if (c == 0 && tid == 0) {
-    a.ends[b] = End{node, count, rest, peak};
-    a.totals[b] = total;
-  }
   if (greedy || peak == -INFINITY) {
     if (c == 0 && tid == 0) answer(s_best[node], peak);
     return;
   }
   const int n_out = a.probs ? 0 : s_n_out;
   const Weights weights(peak, rate);
-  double* const sums = a.sums + static_cast<int64_t>(b) * a.pieces;
-  const auto is_out = [&](int i) {  // refused
-    bool out = false;
+  Piece* const sums = a.sums + static_cast<int64_t>(b) * a.pieces;
+  const int step = a.draws * kWaves;
+  if (!(a.probs && s_refused)) {
+    const auto is_out = [&](int i) {  // refused
+      bool out = false;
 #pragma nounroll
-    for (int k = 0; k < n_out; ++k) out |= s_out[k] == i;
-    return out;
-  };
-  for (int piece = c * kWaves + wave; piece < a.pieces; piece += a.draws * kWaves) {
-    const int v = piece * 64 + lane;
-    const v4u x = v < r.vectors ? r.load(v) : v4u{0, 0, 0, 0};
-    uint32_t out = 0;  // the vector's refused tokens, a bit each
+      for (int k = 0; k < n_out; ++k) out |= s_out[k] == i;
+      return out;
+    };
+    int piece = c * kWaves + wave;
+    v4u x = {0, 0, 0, 0};
+    if (piece * 64 + lane < r.vectors) x = r.load(piece * 64 + lane);
+    for (; piece < a.pieces; piece += step) {
+      const int v = piece * 64 + lane;
+      v4u next = {0, 0, 0, 0};
+      if (v + step * 64 < r.vectors) next = r.load(v + step * 64);
+      uint32_t out = 0;  // the vector's refused tokens, a bit each
 #pragma nounroll
-    for (int k = 0; k < n_out; ++k) {
-      const uint32_t place = s_out[k] - (r.head + v * E::kVec);
-      if (place < E::kVec) out |= 1u << place;
+      for (int k = 0; k < n_out; ++k) {
+        const uint32_t place = s_out[k] - (r.head + v * E::kVec);
+        if (place < E::kVec) out |= 1u << place;
+      }
+      double sum = 0.0;
+      each<E>(r, v, x, [&](float y, int i, int place) {
+        const double w = weights(y);
+        sum += (place >= 0 ? out >> place & 1 : is_out(i)) ? 0.0 : w;
+      });
+      sum = sum_lanes(sum);
+      if (lane == 0) publish(&sums[piece].all, sum);
+      x = next;
     }
-    double sum = 0.0;
-    each<E>(r, v, x, [&](float y, int i, int place) {
-      const double w = weights(y);
-      sum += (place >= 0 ? out >> place & 1 : is_out(i)) ? 0.0 : w;
-    });
-    sum = sum_lanes(sum);
-    if (lane == 0) publish(sums + piece, sum);
+    if (!last_to_arrive(a.arrivals + b, a.draws, &sh.flag)) return;
+    draw<E>(r, a.V, [&](int k) { return take(&sums[k].all); }, a.pieces, u0, sh, [&](float y, int i) { return is_out(i) ? 0.0 : weights(y); }, answer);
+    return;
   }
-  if (!last_to_arrive(a.arrivals + b, a.draws, &sh.flag) || rest) return;
-  draw<E>(r, a.V, sums, a.pieces, total_of(sums, a.pieces), u0, sh, [&](float y, int i) { return is_out(i) ? 0.0 : weights(y); }, answer);
-}
 
-// Element i0 .. of a row of the draft's probabilities; `aligned`: kVec of them at once
-template <int kVec>
-__device__ __forceinline__ void load_probs(const VerifyArgs& a, const char* row, int64_t i0, bool aligned, float (&out)[kVec]) {
-  if (aligned && a.probs_dtype == FP_DTYPE_F32) {
-#pragma unroll
-    for (int h = 0; h < kVec / 4; ++h) {
-      const v4u four = *reinterpret_cast<const v4u*>(row + (i0 + h * 4) * 4);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) out[h * 4 + i] = F32::get(four, i);
-    }
-  } else if (aligned) {
-    uint32_t two[kVec / 2];
-    if constexpr (kVec == 8) {
-      const v4u all = *reinterpret_cast<const v4u*>(row + i0 * 2);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) two[i] = all[i];
-    } else {
-      const uint2 all = *reinterpret_cast<const uint2*>(row + i0 * 2);
-      two[0] = all.x, two[1] = all.y;
-    }
-    const bool bf16 = a.probs_dtype == FP_DTYPE_BF16;
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-      const v4u pack = {two[i / 2], 0, 0, 0};
-      out[i] = bf16 ? BF16::get(pack, i & 1) : F16::get(pack, i & 1);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) out[i] = probability(a, row, i0 + i);
-  }
-}
-
-template <typename E>
-__global__ __launch_bounds__(kThreads) void verify_rest_kernel(const VerifyArgs a) {
-  __shared__ DrawShared sh;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const uint32_t b = blockIdx.x / static_cast<uint32_t>(a.draws);
-  const int c = blockIdx.x - b * a.draws, n = a.pieces;
-  const int64_t first = static_cast<int64_t>(b) * a.S;
-  const End end = a.ends[b];
-  if (!end.rest) return;
-  const float heat = heat_of(a, b), u0 = a.uniforms[first];
-  const double rate = kLog2e / heat;
-  const Row<E> r(a.logits + b * a.ls_b + end.node * a.ls_s, a.V);
-  const char* const probs = a.probs + b * a.ps_b + end.node * a.ps_s;
+  // max(0, w / Z - q)
+  const char* const probs = a.probs + b * a.ps_b + node * a.ps_s;
   const int pe = a.probs_dtype == FP_DTYPE_F32 ? 4 : 2;
   const bool aligned = reinterpret_cast<uintptr_t>(probs + r.head * pe) % (E::kVec * pe < 16 ? E::kVec * pe : 16) == 0;
-  const double* const sums = a.sums + static_cast<int64_t>(b) * n;
-  double* const rests = a.rests + static_cast<int64_t>(b) * n;
-  const Weights weights(end.peak, rate);
-  double all = 0.0, share = 0.0;
-  const auto left_of = [&](float y, float p) { return fmax(0.0, weights(y) * share - static_cast<double>(p)); };
-  for (int piece = c * kWaves + wave; piece < n; piece += a.draws * kWaves) {
-    const int v = piece * 64 + lane;
+  const double about = 1.0 / total;
+  {
+    int piece = c * kWaves + wave;
     v4u x = {0, 0, 0, 0};
-    float q[E::kVec];
-    if (v < r.vectors) {
+    float q[E::kVec] = {};
+    const auto load = [&](int v, v4u& x, float (&q)[E::kVec]) {
+      if (v >= r.vectors) return;
       x = r.load(v);
       load_probs<E::kVec>(a, probs, r.head + static_cast<int64_t>(v) * E::kVec, aligned, q);
+    };
+    load(piece * 64 + lane, x, q);
+    for (; piece < a.pieces; piece += step) {
+      const int v = piece * 64 + lane;
+      v4u next = {0, 0, 0, 0};
+      float q_next[E::kVec] = {};
+      load(v + step * 64, next, q_next);
+      Piece sum = {0.0, 0.0, 0.0};
+      bool unsure = false;
+      each<E>(r, v, x, [&](float y, int i, int place) {
+        const double w = weights(y), taken = place >= 0 ? q[place] : probability(a, probs, i), left = w * about - taken;
+        sum.all += w;
+        const bool kept = left > 0.0;
+        sum.kept += kept ? w : 0.0;
+        sum.taken += kept ? taken : 0.0;
+        unsure |= fabs(left) <= 4.0 * kBand * taken && taken > 0.0;  // (NaN is not left)
+      });
+      sum.all = sum_lanes(sum.all), sum.kept = sum_lanes(sum.kept), sum.taken = sum_lanes(sum.taken);
+      const bool again = __ballot(unsure) != 0;
+      if (lane == 0) {
+        publish(&sums[piece].all, sum.all);
+        publish(&sums[piece].kept, again ? -1.0 : sum.kept);
+        publish(&sums[piece].taken, sum.taken);
+      }
+      x = next;
+#pragma unroll
+      for (int i = 0; i < E::kVec; ++i) q[i] = q_next[i];
     }
-    if (share == 0.0) {  // with the first ones on their way
-      all = total_of(sums, n);
-      share = 1.0 / all;
-    }
-    double sum = 0.0;
-    each<E>(r, v, x, [&](float y, int i, int place) { sum += left_of(y, place >= 0 ? q[place] : probability(a, probs, i)); });
-    sum = sum_lanes(sum);
-    if (lane == 0) publish(rests + piece, sum);
   }
-  if (!last_to_arrive(a.arrivals + a.B + b, a.draws, &sh.flag)) return;
-  const auto answer = [&](int token, float x) {
-    a.answer[first + end.count] = token;
-    a.logprobs[first + end.count] = token < 0 ? 0.f : log_share(x, end.peak, 1.0 / heat, a.totals[b]);
-  };
-  all = total_of(sums, n), share = 1.0 / all;  // (of a wavefront without a piece, too)
-  // nothing left: the target's own distribution
-  const double left = total_of(rests, n);
-  const bool whole = !(left > 0.0);
-  draw<E>(r, a.V, whole ? sums : rests, n, whole ? all : left, u0, sh,
+  if (!last_to_arrive(a.arrivals + b, a.draws, &sh.flag)) return;
+  double all = 0.0;
+#pragma nounroll
+  for (int k = lane; k < a.pieces; k += 64) all += take(&sums[k].all);
+  const double share = 1.0 / sum_lanes(all);
+  const auto left_of = [&](float y, float q) { return fmax(0.0, weights(y) * share - static_cast<double>(q)); };
+  // what is left of every piece; those of which it was not sure by all threads
+  double* const rests = a.rests + static_cast<int64_t>(b) * a.pieces;
+  bool some = false;
+  const int rounds = (a.pieces + kThreads - 1) / kThreads;
+#pragma nounroll
+  for (int round = 0; round < rounds; ++round) {
+    const int k = round * kThreads + tid;
+    bool unsure = false;
+    if (k < a.pieces) {
+      const double kept = take(&sums[k].kept), left = fmax(0.0, kept * share - take(&sums[k].taken));
+      unsure = kept < 0.0;
+      if (!unsure) publish(rests + k, left);
+      some |= !unsure && left > 0.0;
+    }
+    for (uint64_t again = __ballot(unsure); again; again &= again - 1) {  // by the wavefront that found it
+      const int piece = round * kThreads + wave * 64 + __builtin_ctzll(again);
+      const int2 range = piece_range(r, a.V, piece);
+      double sum = 0.0;
+#pragma nounroll
+      for (int i = range.x + lane; i < range.y; i += 64) sum += left_of(r.one(i), probability(a, probs, i));
+      sum = sum_lanes(sum);
+      if (lane == 0) publish(rests + piece, sum);
+      some |= sum > 0.0;
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+  const bool whole = !__syncthreads_or(some);  // nothing is left: the target's own distribution
+  draw<E>(r, a.V, [&](int k) { return whole ? take(&sums[k].all) : take(rests + k); }, a.pieces, u0, sh,
           [&](float y, int i) { return whole ? weights(y) : left_of(y, probability(a, probs, i)); }, answer);
 }
 
@@ -738,15 +773,13 @@ int check_shape(const char* what, int B, int S, int V) {
 }
 
 struct Layout {
-  int64_t ends, totals, parts, sums, rests, bytes;
+  int64_t parts, sums, rests, bytes;
 };
 Layout layout_of(int64_t B, int S, const Cut& rows, int64_t pieces) {
   Layout l;
-  l.ends = (B * 8 + 15) / 16 * 16;
-  l.totals = l.ends + B * static_cast<int64_t>(sizeof(End));
-  l.parts = l.totals + (B * 8 + 15) / 16 * 16;
+  l.parts = (B * 4 + 15) / 16 * 16;
   l.sums = l.parts + B * S * rows.chunks * static_cast<int64_t>(sizeof(Part));
-  l.rests = l.sums + B * pieces * 8;
+  l.rests = l.sums + B * pieces * static_cast<int64_t>(sizeof(Piece));
   l.bytes = l.rests + B * pieces * 8;
   return l;
 }
@@ -786,9 +819,9 @@ extern "C" int fp_verify_drafts(const void* logits, int64_t logits_stride_b, int
   char* const ws = static_cast<char*>(workspace);
   const VerifyArgs a{static_cast<const char*>(logits), logits_stride_b * e, logits_stride_s * e, tokens, parents, uniforms, temperatures,
                      static_cast<const char*>(draft_probs), probs_stride_b * pe, probs_stride_s * pe, probs_dtype, accepted, path, answer,
-                     logprobs, reinterpret_cast<Part*>(ws + l.parts), reinterpret_cast<double*>(ws + l.sums),
-                     reinterpret_cast<double*>(ws + l.rests), reinterpret_cast<End*>(ws + l.ends), reinterpret_cast<double*>(ws + l.totals),
-                     reinterpret_cast<int*>(ws), B, S, V, rows.chunks, rows.nv * kThreads, draw.chunks, pieces};
+                     logprobs, reinterpret_cast<Part*>(ws + l.parts), reinterpret_cast<Piece*>(ws + l.sums),
+                     reinterpret_cast<double*>(ws + l.rests), reinterpret_cast<int*>(ws), B, S, V, rows.chunks, rows.nv * kThreads, draw.chunks,
+                     pieces};
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const auto go = [&](auto kernel, int64_t grid) {
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, st, a);
@@ -801,9 +834,7 @@ extern "C" int fp_verify_drafts(const void* logits, int64_t logits_stride_b, int
       case 2: go(verify_rows_kernel<E, 2>, grid); break;
       case 1: go(verify_rows_kernel<E, 1>, grid);
     }
-    const int64_t draws = static_cast<int64_t>(B) * draw.chunks;
-    go(verify_walk_kernel<E>, draws);
-    if (draft_probs) go(verify_rest_kernel<E>, draws);
+    go(verify_walk_kernel<E>, static_cast<int64_t>(B) * draw.chunks);
   };
   if (dtype == FP_DTYPE_F32)
     launch(F32{});

@@ -202,6 +202,30 @@ def test_equal_distributions_always_stand():
     step.check()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [600, 5003, 40000])
+def test_distributions_that_differ_by_roundings(V, dtype):
+    """q is p rounded to 32 bits but for two tokens, the draft among them: what is left is mostly a token's and a little everybody's, and on
+    which side of 0 that little lies hangs on the last bits of Z."""
+    B = 24
+    step = Step(23, B, 2, V, dtype, probs=F32)
+    p = torch.softmax(step.logits.double(), 2)
+    q = p.clone()
+    for b in range(B):
+        much, less = p[b, 0].topk(2).indices.tolist()
+        if b % 3:  # of every third one the little is all there is
+            q[b, 0, much] += 0.5 * q[b, 0, less]
+            q[b, 0, less] *= 0.5
+        step.tokens[b, 1] = much
+        step.uniforms[b, 1] = 1.0 - 2.0 ** -24 if b % 2 else step.uniforms[b, 1]
+    step.probs = q.float()
+    for b in range(0, B, 3):
+        step.probs[b, 0, step.tokens[b, 1]] *= 4
+    got = step.call()
+    step.check(got)
+    assert got.accepted.min() == 0
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 def test_alignments_and_strides(dtype):
     """Rows that begin at any element, lie apart, or are broadcast; probabilities alike."""
