@@ -1,5 +1,5 @@
 // The calls an eager layer or step makes (append, decode step, prefill attention; tables, page copies and attention of shared
-// prefixes) from PyTorch tensors to the C ABI of include/fp_paged_kv.h, as a Python module.
+// prefixes; trees of drafts, their attention and verification, their rows) from PyTorch tensors to the C ABI of include/fp_paged_kv.h, as a Python module.
 //
 // Bound by the host: a layer of a small eager step is shorter on the GPU than its calls are in Python, where every pointer, size
 // and stride is an attribute look-up and the foreign call converts forty arguments one by one.  Here they are read from the tensors in C++:
@@ -324,12 +324,19 @@ PyObject* shared_unguarded(PyObject* const* args) {
   return pair(out, lse);
 }
 
-// n elements of a byte buffer's memory, from `offset` bytes on, as a tensor that shares it
-at::Tensor part(const at::Tensor& buffer, int64_t offset, int64_t n, at::ScalarType type) {
+// Elements of a byte buffer's memory, from `offset` bytes on, as a tensor of these sizes that shares it
+at::Tensor part(const at::Tensor& buffer, int64_t offset, at::IntArrayRef sizes, at::ScalarType type) {
   at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buffer.storage()), buffer.key_set(), c10::scalarTypeToTypeMeta(type));
   t.unsafeGetTensorImpl()->set_storage_offset(buffer.storage_offset() + offset / static_cast<int64_t>(c10::elementSize(type)));
-  t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
   return t;
+}
+
+PyObject* tuple_of(const at::Tensor* t, int n) {
+  PyObject* const made = PyTuple_New(n);
+  if (!made) return nullptr;
+  for (int i = 0; i < n; ++i) PyTuple_SET_ITEM(made, i, THPVariable_Wrap(t[i]));
+  return made;
 }
 
 // slots, old_lens, new_lens, free_pages, free_count, page_table, page_size, max_rows, parents, row_multiple, inverse, device, stream ->
@@ -360,15 +367,15 @@ PyObject* tables_unguarded(PyObject* const* args) {
     const auto bytes = slots->options().dtype(at::kByte);
     const int64_t wide = (rows + 3) / 4 * 4;
     const at::Tensor big = at::empty({20 * wide}, bytes), small = at::empty({16 * B + 4 * (2 * B + 3)}, bytes);
-    made[0] = part(big, 0, rows, at::kLong);
-    made[2] = part(big, 8 * wide, rows, at::kLong);
-    made[1] = part(big, 16 * wide, rows, at::kInt);
-    made[5] = part(small, 0, B, at::kLong);
-    made[6] = part(small, 8 * B, B, at::kLong);
-    made[3] = part(small, 16 * B, B + 1, at::kInt);
-    made[7] = part(small, 20 * B + 4, B, at::kInt);
-    made[4] = part(small, 24 * B + 4, 1, at::kInt);
-    made[8] = part(small, 24 * B + 8, 1, at::kInt);
+    made[0] = part(big, 0, {rows}, at::kLong);
+    made[2] = part(big, 8 * wide, {rows}, at::kLong);
+    made[1] = part(big, 16 * wide, {rows}, at::kInt);
+    made[5] = part(small, 0, {B}, at::kLong);
+    made[6] = part(small, 8 * B, {B}, at::kLong);
+    made[3] = part(small, 16 * B, {B + 1}, at::kInt);
+    made[7] = part(small, 20 * B + 4, {B}, at::kInt);
+    made[4] = part(small, 24 * B + 4, {1}, at::kInt);
+    made[8] = part(small, 24 * B + 8, {1}, at::kInt);
     const auto at = [&](int i) { return made[i].data_ptr(); };
     rc = fp_step_tables(static_cast<const int64_t*>(slots->data_ptr()), before->data_ptr(), after->data_ptr(), index_code(*before),
                         parents ? static_cast<const int64_t*>(parents->data_ptr()) : nullptr, static_cast<const int64_t*>(pages->data_ptr()),
@@ -381,10 +388,7 @@ PyObject* tables_unguarded(PyObject* const* args) {
                         reinterpret_cast<void*>(stream));
   }
   if (rc < 0) return fail("fp_step_tables", rc);
-  PyObject* const t = PyTuple_New(9);
-  if (!t) return nullptr;
-  for (int i = 0; i < 9; ++i) PyTuple_SET_ITEM(t, i, THPVariable_Wrap(made[i]));
-  return t;
+  return tuple_of(made, 9);
 }
 
 // pool, src, dst, rows, page_size, device, stream -> True
@@ -409,6 +413,160 @@ PyObject* copy_unguarded(PyObject* const* args) {
   Py_RETURN_TRUE;
 }
 
+// [B, S] of this type
+bool is_matrix(const at::Tensor& t, at::ScalarType type, int64_t B, int64_t S) {
+  return t.dim() == 2 && t.scalar_type() == type && t.is_contiguous() && t.size(0) == B && t.size(1) == S;
+}
+bool is_lengths(const at::Tensor& t, int64_t n) { return index_code(t) >= 0 && is_vector(t, t.scalar_type(), n); }
+bool is_tree(const at::Tensor& masks, const at::Tensor& pos) {
+  return masks.dim() == 2 && is_matrix(masks, at::kLong, masks.size(0), masks.size(1)) && index_code(pos) >= 0 &&
+         is_matrix(pos, pos.scalar_type(), masks.size(0), masks.size(1));
+}
+
+// parents, cached, device, stream -> masks, input_pos, rope_pos
+PyObject* draft_tree_unguarded(PyObject* const* args) {
+  Args a{args};
+  const at::Tensor *parents = a.tensor(), *cached = a.tensor();
+  const int64_t device = a.integer(), stream = a.integer();
+  if (!a.ok || parents->dim() != 2) Py_RETURN_NONE;
+  const int64_t B = parents->size(0), S = parents->size(1);
+  if (!is_matrix(*parents, at::kInt, B, S) || !is_lengths(*cached, B) || !fits({B, S}) || S < 1 || !on_device(device, {parents, cached}))
+    Py_RETURN_NONE;
+  at::Tensor made[3];
+  int rc;
+  {
+    const Unlocked others;
+    const at::Tensor all = at::empty({16 * B * S}, parents->options().dtype(at::kByte));
+    made[0] = part(all, 0, {B, S}, at::kLong);
+    made[1] = part(all, 8 * B * S, {B, S}, at::kInt);
+    made[2] = part(all, 12 * B * S, {B, S}, at::kInt);
+    rc = fp_draft_tree(static_cast<const int32_t*>(parents->data_ptr()), cached->data_ptr(), index_code(*cached), B, S,
+                       static_cast<int64_t*>(made[0].data_ptr()), static_cast<int32_t*>(made[1].data_ptr()),
+                       static_cast<int32_t*>(made[2].data_ptr()), reinterpret_cast<void*>(stream));
+  }
+  if (rc < 0) return fail("fp_draft_tree", rc);
+  return tuple_of(made, 3);
+}
+
+// batch_idx, masks, input_pos, page_table, q_heads, cached_heads, head_dim, max_context, prefix_ids, prefix_lens, plan, device, stream -> True
+PyObject* tree_plan_unguarded(PyObject* const* args) {
+  Args a{args};
+  const at::Tensor *bidx = a.tensor(), *masks = a.tensor(), *pos = a.tensor(), *table = a.tensor();
+  const int64_t Hq = a.integer(), Hc = a.integer(), D = a.integer(), max_context = a.integer();
+  const at::Tensor *ids = a.maybe_tensor(), *lens = a.maybe_tensor(), *plan = a.tensor();
+  const int64_t device = a.integer(), stream = a.integer();
+  if (!a.ok || !is_tree(*masks, *pos) || !is_vector(*bidx, at::kLong, masks->size(0)) || !is_table(*table) || !ids != !lens ||
+      (ids && (!is_vector(*ids, at::kInt, table->size(0)) || !is_vector(*lens, at::kInt, table->size(0)))) || !is_bytes(*plan) ||
+      !on_device(device, {bidx, masks, pos, table, ids, lens, plan}) || !fits({masks->size(0), masks->size(1), Hq, Hc, D, table->size(0), max_context}))
+    Py_RETURN_NONE;
+  int rc;
+  {
+    const Unlocked others;
+    rc = fp_tree_decode_plan(static_cast<const int64_t*>(bidx->data_ptr()), pos->data_ptr(), index_code(*pos),
+                             ids ? static_cast<const int32_t*>(ids->data_ptr()) : nullptr,
+                             ids ? static_cast<const int32_t*>(lens->data_ptr()) : nullptr, masks->size(0), masks->size(1), Hq, Hc, D,
+                             table->size(0), max_context, plan->data_ptr(), plan->numel(), reinterpret_cast<void*>(stream));
+  }
+  if (rc < 0) return fail("fp_tree_decode_plan", rc);
+  Py_RETURN_TRUE;
+}
+
+// q, pool_k, pool_v, page_table, batch_idx, masks, input_pos, page_size, max_context, scale, sinks, plan, workspace, device, stream -> (out, lse)
+PyObject* tree_unguarded(PyObject* const* args) {
+  Args a{args};
+  const at::Tensor *q = a.tensor(), *pk = a.tensor(), *pv = a.tensor(), *table = a.tensor(), *bidx = a.tensor(), *masks = a.tensor(),
+                   *pos = a.tensor();
+  const int64_t page_size = a.integer(), max_context = a.integer();
+  const double scale = a.number();
+  const at::Tensor *sinks = a.maybe_tensor(), *plan = a.tensor(), *ws = a.tensor();
+  const int64_t device = a.integer(), stream = a.integer();
+  if (!a.ok) Py_RETURN_NONE;
+  const int dt = dtype_code(*q);
+  if (dt < 0 || q->dim() != 4 || pk->dim() != 3 || pk->sizes() != pv->sizes() || pk->size(2) != q->size(3) ||
+      pk->scalar_type() != q->scalar_type() || pv->scalar_type() != q->scalar_type() || !pk->is_contiguous() || !pv->is_contiguous() ||
+      !q->is_contiguous() || reinterpret_cast<uintptr_t>(q->data_ptr()) % 16 != 0 || !is_table(*table) || !is_tree(*masks, *pos) ||
+      !is_bytes(*plan) || !is_bytes(*ws))
+    Py_RETURN_NONE;
+  const int64_t B = q->size(0), Hq = q->size(1), S = q->size(2), D = q->size(3), Hc = pk->size(0);
+  if (!is_vector(*bidx, at::kLong, B) || masks->size(0) != B || masks->size(1) != S || (sinks && !is_vector(*sinks, at::kFloat, Hq)) ||
+      !fits({B, S, Hq, Hc, D, page_size, table->size(0), table->size(1), max_context}) ||
+      !on_device(device, {q, pk, pv, table, bidx, masks, pos, sinks, plan, ws}))
+    Py_RETURN_NONE;
+  at::Tensor out, lse;
+  int rc;
+  {
+    const Unlocked others;
+    out = at::empty({B, Hq, S, D}, q->options());
+    lse = at::empty({B, Hq, S}, q->options().dtype(at::kFloat));
+    rc = fp_paged_decode_tree(
+        static_cast<const int64_t*>(masks->data_ptr()), q->data_ptr(), q->stride(0), q->stride(1), q->stride(2), pk->data_ptr(), pv->data_ptr(),
+        static_cast<const int64_t*>(table->data_ptr()), table->stride(0), static_cast<const int64_t*>(bidx->data_ptr()), pos->data_ptr(),
+        index_code(*pos), out.data_ptr(), out.stride(0), out.stride(1), out.stride(2), static_cast<float*>(lse.data_ptr()),
+        sinks ? static_cast<const float*>(sinks->data_ptr()) : nullptr, ws->data_ptr(), ws->numel(), plan->data_ptr(), plan->numel(), B,
+        S, Hq, Hc, D, page_size, table->size(1), table->size(0), pk->size(1), max_context, static_cast<float>(scale), dt,
+        reinterpret_cast<void*>(stream));
+  }
+  if (rc < 0) return fail("fp_paged_decode_tree", rc);
+  return pair(out, lse);
+}
+
+// logits, tokens, parents, uniforms, temperatures, draft_probs, workspace, device, stream -> accepted, path, tokens, logprobs
+PyObject* verify_unguarded(PyObject* const* args) {
+  Args a{args};
+  const at::Tensor *logits = a.tensor(), *tokens = a.tensor(), *parents = a.tensor(), *uniforms = a.tensor(), *heat = a.maybe_tensor(),
+                   *probs = a.maybe_tensor(), *ws = a.tensor();
+  const int64_t device = a.integer(), stream = a.integer();
+  if (!a.ok) Py_RETURN_NONE;
+  const int dt = dtype_code(*logits), pt = probs ? dtype_code(*probs) : 0;
+  if (dt < 0 || pt < 0 || logits->dim() != 3 || !dense_rows(*logits) || (probs && (probs->sizes() != logits->sizes() || !dense_rows(*probs))))
+    Py_RETURN_NONE;
+  const int64_t B = logits->size(0), S = logits->size(1), V = logits->size(2);
+  if (S < 1 || V < 1 || !is_matrix(*tokens, at::kLong, B, S) || !is_matrix(*parents, at::kInt, B, S) || !is_matrix(*uniforms, at::kFloat, B, S) ||
+      (heat && !is_vector(*heat, at::kFloat, B)) || !is_bytes(*ws) || !fits({B, S, V}) ||
+      !on_device(device, {logits, tokens, parents, uniforms, heat, probs, ws}))
+    Py_RETURN_NONE;
+  at::Tensor made[4];
+  int rc;
+  {
+    const Unlocked others;
+    const at::Tensor all = at::empty({B * (16 * S + 4)}, logits->options().dtype(at::kByte));
+    made[2] = part(all, 0, {B, S}, at::kLong);
+    made[1] = part(all, 8 * B * S, {B, S}, at::kInt);
+    made[3] = part(all, 12 * B * S, {B, S}, at::kFloat);
+    made[0] = part(all, 16 * B * S, {B}, at::kInt);
+    rc = fp_verify_drafts(logits->data_ptr(), logits->stride(0), logits->stride(1), dt, static_cast<const int64_t*>(tokens->data_ptr()),
+                          static_cast<const int32_t*>(parents->data_ptr()), static_cast<const float*>(uniforms->data_ptr()),
+                          heat ? static_cast<const float*>(heat->data_ptr()) : nullptr, probs ? probs->data_ptr() : nullptr,
+                          probs ? probs->stride(0) : 0, probs ? probs->stride(1) : 0, pt, static_cast<int32_t*>(made[0].data_ptr()),
+                          static_cast<int32_t*>(made[1].data_ptr()), static_cast<int64_t*>(made[2].data_ptr()),
+                          static_cast<float*>(made[3].data_ptr()), ws->data_ptr(), ws->numel(), B, S, V, reinterpret_cast<void*>(stream));
+  }
+  if (rc < 0) return fail("fp_verify_drafts", rc);
+  return tuple_of(made, 4);
+}
+
+// pool, page_table, batch_idx, cached, path, page_size, device, stream -> True
+PyObject* keep_unguarded(PyObject* const* args) {
+  Args a{args};
+  const at::Tensor *pool = a.tensor(), *table = a.tensor(), *bidx = a.tensor(), *cached = a.tensor(), *path = a.tensor();
+  const int64_t page_size = a.integer(), device = a.integer(), stream = a.integer();
+  if (!a.ok || dtype_code(*pool) < 0 || pool->dim() < 2 || !pool->is_contiguous() || pool->numel() == 0 || path->dim() != 2) Py_RETURN_NONE;
+  const int64_t B = path->size(0), S = path->size(1), D = pool->size(-1), n_slots = pool->size(-2);
+  if (S < 1 || !is_matrix(*path, at::kInt, B, S) || !is_table(*table) || !is_vector(*bidx, at::kLong, B) || !is_lengths(*cached, B) ||
+      page_size < 1 || !fits({B, S, D, page_size, table->size(0), table->size(1)}) || !on_device(device, {pool, table, bidx, cached, path}))
+    Py_RETURN_NONE;
+  int rc;
+  {
+    const Unlocked others;
+    rc = fp_keep_rows(pool->data_ptr(), static_cast<const int64_t*>(table->data_ptr()), table->stride(0),
+                      static_cast<const int64_t*>(bidx->data_ptr()), cached->data_ptr(), index_code(*cached),
+                      static_cast<const int32_t*>(path->data_ptr()), B, S, pool->numel() / (n_slots * D), n_slots, D, page_size, table->size(1),
+                      table->size(0), dtype_code(*pool), reinterpret_cast<void*>(stream));
+  }
+  if (rc < 0) return fail("fp_keep_rows", rc);
+  Py_RETURN_TRUE;
+}
+
 // A C++ exception (an allocation that failed) becomes a Python one.
 template <PyObject* (*kCall)(PyObject* const*), Py_ssize_t kArgs>
 PyObject* guarded(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -425,7 +583,10 @@ PyObject* guarded(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyMethodDef kMethods[] = {FP_METHOD("append", append_unguarded, 11), FP_METHOD("decode", decode_unguarded, 19),
                           FP_METHOD("prefill", prefill_unguarded, 14),
                           FP_METHOD("shared_plan", shared_plan_unguarded, 11), FP_METHOD("shared", shared_unguarded, 16),
-                          FP_METHOD("tables", tables_unguarded, 13), FP_METHOD("copy_pages", copy_unguarded, 7), {nullptr, nullptr, 0, nullptr}};
+                          FP_METHOD("tables", tables_unguarded, 13), FP_METHOD("copy_pages", copy_unguarded, 7),
+                          FP_METHOD("draft_tree", draft_tree_unguarded, 4), FP_METHOD("tree_plan", tree_plan_unguarded, 13),
+                          FP_METHOD("tree", tree_unguarded, 15), FP_METHOD("verify", verify_unguarded, 9), FP_METHOD("keep", keep_unguarded, 8),
+                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "fp_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

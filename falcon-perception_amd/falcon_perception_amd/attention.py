@@ -9,6 +9,8 @@ The reference binds `compiled_flex_attn_decode` / `compiled_flex_attn_prefill`
   the split-K paged decode kernel,
 * a `HybridPrefillMask` (what `PagedKVCache.create_prefill_blockmask` returns) runs
   the MFMA chunked-prefill kernel over the paged cache,
+* a `PagedTreeMask` (what `PagedKVCache.create_tree_mask` returns), given to the decode
+  callable, runs the attention of trees of drafted tokens,
 * any other mask is not part of the paged path (the reference's AnyUp upsampler
   uses a windowed torch BlockMask, `anyup.py:358`) and is handed to torch's own
   flex_attention untouched.
@@ -41,6 +43,7 @@ __all__ = [
     "offset_mask_mod",
     "PagedDecodeMask",
     "HybridPrefillMask",
+    "PagedTreeMask",
 ]
 
 
@@ -196,6 +199,30 @@ class HybridPrefillMask:
         return hit
 
 
+class PagedTreeMask:
+    """Mask of a step in which every sequence has its last token and drafts behind it, which form a tree.
+
+    Returned by `PagedKVCache.create_tree_mask`; `compiled_flex_attn_decode` takes it with q [B, Hq, S, D].  `input_pos` [B, S] is what
+    `insert_kv` is given, `rope_pos` [B, S] the tokens' places in the text."""
+
+    def __init__(self, cache, batch_idx: Tensor, parents: Tensor, cached: Tensor):
+        self.cache = cache
+        self.batch_idx = batch_idx
+        self.parents = parents
+        self.cached = cached
+        self.tree = ops.draft_tree(parents, cached)
+        self._plan_shape = None  # as a PagedDecodeMask's
+        self._plan_layer = -1
+
+    @property
+    def input_pos(self) -> Tensor:
+        return self.tree.input_pos
+
+    @property
+    def rope_pos(self) -> Tensor:
+        return self.tree.rope_pos
+
+
 # --------------------------------------------------------------------------
 # the two attention callables
 # --------------------------------------------------------------------------
@@ -236,7 +263,13 @@ def compiled_flex_attn_decode(q: Tensor, k: Tensor, v: Tensor, score_mod=None, b
     The kernel attends positions 0 .. input_pos[b] of every sequence, i.e. the causal mask the engine
     installs for a decode step (`q + input_pos[b] >= kv`, `paged_inference.py:797-801`); the `mask_mod` of
     the logical mask is not evaluated, so a mask that hides earlier positions is outside this path.
+
+    With a `PagedTreeMask` q is [B, Hq, S, D], the tokens of a step of drafts, whose keys `insert_kv` has appended.
     """
+    if isinstance(block_mask, PagedTreeMask):
+        if score_mod is not None:
+            raise RuntimeError("score_mod is not supported on the paged decode path")
+        return _result(*_tree_decode(q, k, v, block_mask, scale, sinks), return_aux, return_lse)
     if not isinstance(block_mask, PagedDecodeMask):
         if sinks is not None:
             raise RuntimeError("the fused sink gate needs a mask made by PagedKVCache")
@@ -327,6 +360,33 @@ def _shared_decode(q: Tensor, k: Tensor, v: Tensor, mask: PagedDecodeMask, step,
     mask._plan_layer = step.layer_id
     return ops.paged_decode_shared(q, pool_k, pool_v, cache.page_table, *args, cache.page_size, mask.max_context, scale=scale,
                                    sinks=sinks, plan=plan, workspace=workspace)
+
+
+def _tree_decode(q: Tensor, k: Tensor, v: Tensor, mask: PagedTreeMask, scale, sinks) -> tuple[Tensor, Tensor]:
+    """The decode call of a step of drafts: the plan is made by the first layer."""
+    cache = mask.cache
+    step = cache.last_decode_step
+    if step is None:
+        raise RuntimeError("attention of drafts called before PagedKVCache.insert_kv for this step")
+    if step.batch_idx.shape != mask.batch_idx.shape or step.input_pos.shape != mask.input_pos.shape:
+        raise RuntimeError(f"the mask is of {list(mask.input_pos.shape)} tokens but the last insert_kv of this cache appended "
+                           f"{list(step.input_pos.shape)}: attention must follow the insert_kv of its own step")
+    cache.flush()
+    (B, Hq, S, D), Hc = q.shape, k.shape[1]
+    pools = cache._pools[step.layer_id]
+    pool_k, pool_v = cache._planes[step.layer_id] if k is pools[0] and v is pools[1] else (k[0], v[0])
+    plan, workspace = cache.tree_decode_buffers(B, S, Hq, Hc, D)
+    max_context = cache.table_cols * cache.page_size
+    shared = dict(prefix_ids=cache.prefix_ids, prefix_lens=cache.prefix_lens)  # None, None without prefix_sharing
+    shape = (B, Hq, S, D, Hc)
+    if cache._tree_plan_owner is not mask or mask._plan_shape != shape or step.layer_id <= mask._plan_layer:
+        ops.tree_decode_plan(mask.batch_idx, mask.tree, cache.page_table, q_heads=Hq, cached_heads=Hc, head_dim=D, max_context=max_context,
+                             plan=plan, **shared)
+        cache._tree_plan_owner = mask
+        mask._plan_shape = shape
+    mask._plan_layer = step.layer_id
+    return ops.paged_decode_tree(q, pool_k, pool_v, cache.page_table, mask.batch_idx, mask.tree, cache.page_size, max_context, scale=scale,
+                                 sinks=sinks, plan=plan, workspace=workspace, **shared)
 
 
 def compiled_flex_attn_prefill(q: Tensor, k: Tensor, v: Tensor, score_mod=None, block_mask=None,

@@ -810,6 +810,11 @@ def draft_tree(parents: Tensor, cached: Tensor) -> DraftTree:
     Returns `masks` [B, S] int64 (bit i of masks[b, j]: token j sees token i, its ancestors and itself; 0 no token), `input_pos`
     [B, S] int32, the position in the cache that each token's keys go to (cached + j; -1 no token: `kv_append` leaves it out), and
     `rope_pos` [B, S] int32, its place in the text (cached + number of ancestors)."""
+    index = _current(parents)
+    if index >= 0:
+        made = N.host().draft_tree(parents, cached, index, N.raw_stream(index))
+        if made is not None:
+            return DraftTree(*made)
     what = "draft_tree"
     device = _same_device(what, parents, cached)
     B, S = _tree_shape(what, parents)
@@ -854,6 +859,10 @@ def tree_decode_plan(batch_idx: Tensor, tree: DraftTree, page_table: Tensor, *, 
                      plan: Tensor | None = None) -> Tensor:
     """The plan of a `paged_decode_tree` step, made once for all layers: how the work is cut and which sequences share a
     prefix.  Arguments as there; `plan`: a uint8 tensor of `shared_decode_plan_bytes(B, S, ...)` bytes to write it to."""
+    index = _current(batch_idx)
+    if index >= 0 and plan is not None and N.host().tree_plan(batch_idx, tree[0], tree[1], page_table, q_heads, cached_heads, head_dim, max_context,
+                                                              prefix_ids, prefix_lens, plan, index, N.raw_stream(index)):
+        return plan
     what = "tree_decode_plan"
     device = _same_device(what, batch_idx, tree[0], tree[1], page_table, prefix_ids, prefix_lens, plan)
     masks, input_pos = _tree(what, tree)
@@ -887,6 +896,12 @@ def paged_decode_tree(q: Tensor, pool_k: Tensor, pool_v: Tensor, page_table: Ten
     `plan`: what `tree_decode_plan` made for this step (with the same prefixes; positions, slots and table unchanged since); without
     one the call makes it.  `workspace`: `shared_decode_workspace_bytes(B, S, ...)` bytes, for one launch at a time.  `sinks`
     [Hq] float32 gates the output as in `paged_decode`."""
+    index = _current(q)
+    if index >= 0 and out is None and lse is None and plan is not None and workspace is not None:
+        got = N.host().tree(q, pool_k, pool_v, page_table, batch_idx, tree[0], tree[1], page_size, max_context,
+                            1.0 / math.sqrt(q.shape[-1]) if scale is None else scale, sinks, plan, workspace, index, N.raw_stream(index))
+        if got is not None:
+            return got
     what = "paged_decode_tree"
     device = _same_device(what, q, pool_k, pool_v, page_table, batch_idx, tree[0], tree[1], prefix_ids, prefix_lens, sinks, plan,
                           workspace, out, lse)
@@ -971,6 +986,11 @@ def verify_drafts(logits: Tensor, tokens: Tensor, parents: Tensor, uniforms: Ten
     are taken in 64 bits and do not depend on the batch.  A sequence whose parents[b, 0] is not -1 has no step: 0, -1, -1, 0.
 
     `workspace`: `verify_workspace_bytes(B, S, V)` bytes, for one call at a time."""
+    index = _current(logits)
+    if index >= 0 and workspace is not None:
+        made = N.host().verify(logits, tokens, parents, uniforms, temperatures, draft_probs, workspace, index, N.raw_stream(index))
+        if made is not None:
+            return VerifiedDrafts(*made)
     what = "verify_drafts"
     device = _same_device(what, logits, tokens, parents, uniforms, temperatures, draft_probs, workspace)
     B, S = _tree_shape(what, parents)
@@ -1009,6 +1029,9 @@ def keep_rows(pool: Tensor, page_table: Tensor, batch_idx: Tensor, cached: Tenso
     For the leading entries of `path` [B, S] (int32, `VerifiedDrafts.path`) that rise, position cached[b] + i of slot batch_idx[b] gets the
     rows of position cached[b] + path[b, i], as they were before the call; `cached` [B] (int32 or int64): keys in front of the
     step.  An entry whose slot is outside the table, or named by an entry before it, is left out."""
+    index = _current(pool)
+    if index >= 0 and N.host().keep(pool, page_table, batch_idx, cached, path, page_size, index, N.raw_stream(index)):
+        return
     what = "keep_rows"
     device = _same_device(what, pool, page_table, batch_idx, cached, path)
     if pool.dim() < 2 or not pool.is_contiguous():

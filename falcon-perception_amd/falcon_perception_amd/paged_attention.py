@@ -18,7 +18,7 @@ from torch import Tensor
 from torch.nn.attention.flex_attention import BlockMask, noop_mask
 
 from . import ops
-from .attention import HybridPrefillMask, PagedDecodeMask, get_causal_mask_mod
+from .attention import HybridPrefillMask, PagedDecodeMask, PagedTreeMask, get_causal_mask_mod
 from .kv_cache import KVCacheBase
 
 
@@ -152,6 +152,8 @@ class PagedKVCache(KVCacheBase):
         self.prefix_ids = torch.zeros(max_batch_size, dtype=torch.int32, device=device) if prefix_sharing else None
         self.prefix_lens = torch.zeros(max_batch_size, dtype=torch.int32, device=device) if prefix_sharing else None
         self._shared_buffers: dict[tuple, tuple[Tensor, Tensor, int]] = {}
+        self._tree_buffers: dict[tuple, tuple[Tensor, Tensor, int]] = {}
+        self._tree_plan_owner = None  # the mask whose plan is in them
         # status word of the last prefill mask, on its way to the host (`check_prefill_masks`)
         self._mask_status_host: Tensor | None = None
         self._mask_status_event = None
@@ -494,6 +496,43 @@ class PagedKVCache(KVCacheBase):
             # not cleared: nothing in them needs it, and of a first use inside a graph's capture every replay would clear them again
             plan, workspace = (torch.empty(n, dtype=torch.uint8, device=self._kv.device) for n in sizes)
             hit = self._shared_buffers[key] = (plan, workspace, most)
+        return hit[0], hit[1]
+
+    # --------------------------------------------------------- drafted tokens
+    def create_tree_mask(self, batch_idx: Tensor, parents: Tensor, cached: Tensor) -> PagedTreeMask:
+        """Mask of a step of drafted tokens: per sequence its last token, whose keys are not cached yet, and drafts behind it, each naming
+        the row of the token it continues (`ops.draft_tree`).  `batch_idx` [B] int64 slots, `parents` [B, S] int32, `cached` [B]: keys in
+        front of the step.  Pages for cached + S tokens have to be reserved.  Not a method of the reference's class.
+
+        A step of such an engine: `insert_kv(layer, k, v, input_pos=mask.input_pos, batch_idx=batch_idx)` and
+        `compiled_flex_attn_decode(q, *pools, block_mask=mask)` in every layer, `ops.verify_drafts` on the logits, then `keep_drafts`."""
+        if self.table_cols * self.page_size > ops.SHARED_CONTEXT:
+            raise RuntimeError(f"Trees of drafts are of contexts up to {ops.SHARED_CONTEXT}; the page table holds {self.table_cols} blocks of "
+                               f"{self.page_size} tokens per sequence.")
+        if batch_idx.dim() != 1 or parents.dim() != 2 or parents.shape[0] != batch_idx.shape[0]:
+            raise RuntimeError(f"batch_idx must be [B] and parents [B, S], got {list(batch_idx.shape)} and {list(parents.shape)}")
+        self.flush()
+        return PagedTreeMask(self, batch_idx, parents, cached)
+
+    def keep_drafts(self, mask: PagedTreeMask, path: Tensor) -> None:
+        """Move the cached rows of the tokens that stand (`path` of `ops.verify_drafts`) together behind the keys in front of the step, in
+        all layers (`ops.keep_rows`): the sequence then has `mask.cached` + (accepted + 1) keys.  The rows behind them are
+        left as they are and written over by the next step; reserved pages stay the slot's.  Not a method of the reference's class."""
+        self.flush()
+        ops.keep_rows(self._kv, self.page_table, mask.batch_idx, mask.cached, path, self.page_size)
+
+    def tree_decode_buffers(self, B: int, S: int, Hq: int, Hc: int, D: int) -> tuple[Tensor, Tensor]:
+        """Plan and workspace of the attention of a step of drafts.  They grow with the batch; graphs captured with smaller ones keep those."""
+        key = (S, Hq, Hc, D)
+        hit = self._tree_buffers.get(key)
+        if hit is None or hit[2] < B:
+            shape = dict(q_heads=Hq, cached_heads=Hc, head_dim=D)
+            if hit is not None:
+                self._retired_workspaces.extend(hit[:2])
+            self._tree_plan_owner = None
+            sizes = ops.shared_decode_plan_bytes(B, S, **shape), ops.shared_decode_workspace_bytes(B, S, **shape)
+            plan, workspace = (torch.empty(n, dtype=torch.uint8, device=self._kv.device) for n in sizes)
+            hit = self._tree_buffers[key] = (plan, workspace, B)
         return hit[0], hit[1]
 
     # ------------------------------------------------------------------- masks
