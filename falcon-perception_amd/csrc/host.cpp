@@ -430,7 +430,7 @@ PyObject* draft_tree_unguarded(PyObject* const* args) {
   const int64_t device = a.integer(), stream = a.integer();
   if (!a.ok || parents->dim() != 2) Py_RETURN_NONE;
   const int64_t B = parents->size(0), S = parents->size(1);
-  if (!is_matrix(*parents, at::kInt, B, S) || !is_lengths(*cached, B) || !fits({B, S}) || S < 1 || !on_device(device, {parents, cached}))
+  if (!is_matrix(*parents, at::kInt, B, S) || !is_lengths(*cached, B) || !fits({B, S}) || S < 1 || S > 64 || !on_device(device, {parents, cached}))
     Py_RETURN_NONE;
   at::Tensor made[3];
   int rc;
@@ -521,7 +521,7 @@ PyObject* verify_unguarded(PyObject* const* args) {
   if (dt < 0 || pt < 0 || logits->dim() != 3 || !dense_rows(*logits) || (probs && (probs->sizes() != logits->sizes() || !dense_rows(*probs))))
     Py_RETURN_NONE;
   const int64_t B = logits->size(0), S = logits->size(1), V = logits->size(2);
-  if (S < 1 || V < 1 || !is_matrix(*tokens, at::kLong, B, S) || !is_matrix(*parents, at::kInt, B, S) || !is_matrix(*uniforms, at::kFloat, B, S) ||
+  if (S < 1 || S > 64 || V < 1 || !is_matrix(*tokens, at::kLong, B, S) || !is_matrix(*parents, at::kInt, B, S) || !is_matrix(*uniforms, at::kFloat, B, S) ||
       (heat && !is_vector(*heat, at::kFloat, B)) || !is_bytes(*ws) || !fits({B, S, V}) ||
       !on_device(device, {logits, tokens, parents, uniforms, heat, probs, ws}))
     Py_RETURN_NONE;
@@ -552,7 +552,7 @@ PyObject* keep_unguarded(PyObject* const* args) {
   const int64_t page_size = a.integer(), device = a.integer(), stream = a.integer();
   if (!a.ok || dtype_code(*pool) < 0 || pool->dim() < 2 || !pool->is_contiguous() || pool->numel() == 0 || path->dim() != 2) Py_RETURN_NONE;
   const int64_t B = path->size(0), S = path->size(1), D = pool->size(-1), n_slots = pool->size(-2);
-  if (S < 1 || !is_matrix(*path, at::kInt, B, S) || !is_table(*table) || !is_vector(*bidx, at::kLong, B) || !is_lengths(*cached, B) ||
+  if (S < 1 || S > 64 || !is_matrix(*path, at::kInt, B, S) || !is_table(*table) || !is_vector(*bidx, at::kLong, B) || !is_lengths(*cached, B) ||
       page_size < 1 || !fits({B, S, D, page_size, table->size(0), table->size(1)}) || !on_device(device, {pool, table, bidx, cached, path}))
     Py_RETURN_NONE;
   int rc;

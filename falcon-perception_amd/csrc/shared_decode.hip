@@ -136,6 +136,7 @@ struct PlanArgs {
   int B, S, Hq, Hc, group, max_batch, max_context, n_wg;
   char* plan;
   int64_t seqs, tokens, place, shares, tiles;
+  int wide_own;  // own keys of several tiles are cut as prefixes of several tiles are
 };
 
 // What a tile costs before its first key and behind its last, in units.
@@ -179,7 +180,9 @@ __device__ __forceinline__ void block_sums(const int (&x)[N], int (&before)[N], 
   __syncthreads();
 }
 
-constexpr int kPlanArrays = 23;
+constexpr int kPlanArrays = 23, kWideArrays = 8;  // these hold a number for each sequence, or two of them with wide_own, and one array more
+constexpr int kWideOwn = 1024;  // sequences up to which they fit
+constexpr int kOwnEntry = 1 << 20;
 
 __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   extern __shared__ int s_mem[];
@@ -199,14 +202,16 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   int* const s_unit = s_stile + Bp;    //   units of prefixes that are cut with everything else,
   int* const s_own = s_unit + Bp;      //   units of own keys,
   int* const s_wide = s_own + Bp;      // place of a group of several tiles in the lists of these:
-  int* const s_at = s_wide + Bp;       //   its first sequence,
-  int* const s_n = s_at + Bp;          //   its tiles,
-  int* const s_u = s_n + Bp;           //   units of each, with the lead
-  int* const s_lu = s_u + Bp;          //   the lead,
-  int* const s_pos = s_lu + Bp;        //   its place on the axis of its kind,
-  int* const s_end = s_pos + Bp;       //   length of that axis, at the first of a kind, elsewhere 0,
-  int* const s_next = s_end + Bp;      //   the next of its kind, -1: none,
-  int* const s_part = s_next + Bp;     //   pieces of the groups before
+  const int Wp = a.wide_own ? 2 * Bp : Bp;
+  int* const s_at = s_wide + Bp;       //   its first sequence (with kOwnEntry: its own keys),
+  int* const s_n = s_at + Wp;          //   its tiles,
+  int* const s_u = s_n + Wp;           //   units of each, with the lead
+  int* const s_lu = s_u + Wp;          //   the lead,
+  int* const s_pos = s_lu + Wp;        //   its place on the axis of its kind,
+  int* const s_end = s_pos + Wp;       //   length of that axis, at the first of a kind, elsewhere 0,
+  int* const s_next = s_end + Wp;      //   the next of its kind, -1: none,
+  int* const s_part = s_next + Wp;     //   pieces of the groups before
+  int* const s_wide_own = s_part + Wp; // with wide_own: place of a sequence's own keys in the lists
   __shared__ int s_sum[16 * 7], s_pick[1], s_turn[2];
   const int tid = threadIdx.x, n_thr = blockDim.x, lane = tid & 63, wave = tid >> 6, n_waves = n_thr / 64;
   Sequence* const seqs = reinterpret_cast<Sequence*>(a.plan + a.seqs);
@@ -366,6 +371,7 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   // sums over the sequences before, consecutive ones a thread
   const int per = (a.B + n_thr - 1) / n_thr, b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
   int x[7] = {0, 0, 0, 0, 0, 0, 0}, before[7], total[7];
+  const auto own_wide = [&](int b) { return a.wide_own && s_keys[b] > s_shared[b] && tiles_of(s_tok[b]) > 1; };
   const auto add = [&](int b) {
     const int c = s_count[b], own = s_keys[b] - s_shared[b];
     if (c > 0) {
@@ -373,37 +379,48 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
       x[1] += c;
       x[4] += tiles_of(c) * (lead_for(c) + units_of(s_shared[b]));
       x[5] += tiles_of(c) > 1;
+      x[6] += tiles_of(c) > 1 ? tiles_of(c) * (lead_for(c) + units_of(s_shared[b])) : 0;
     }
     if (own > 0) {
       x[2] += tiles_of(s_tok[b]);
       x[4] += tiles_of(s_tok[b]) * (lead_for(s_tok[b]) + units_of(own));
+      if (own_wide(b)) {
+        ++x[5];
+        x[6] += tiles_of(s_tok[b]) * (lead_for(s_tok[b]) + units_of(own));
+      }
     }
     if (s_shared[b] == 0) x[3] += s_tok[b];
-    x[6] += s_tok[b];
   };
   for (int b = b0; b < b1; ++b) add(b);
   block_sums(x, before, total, s_sum);
-  const int p_tiles = total[0], n_tiles = p_tiles + total[2], shared_tokens = total[1], n_multi = total[5], all_units = total[4];
+  const int p_tiles = total[0], n_tiles = p_tiles + total[2], shared_tokens = total[1], n_multi = total[5], all_units = total[4], wide_units = total[6];
 #pragma unroll
   for (int i = 0; i < 7; ++i) x[i] = before[i];
   for (int b = b0; b < b1; ++b) {
     s_ptile[b] = x[0];
     s_base[b] = s_shared[b] > 0 ? x[1] : shared_tokens + x[3];  // of a group: right at its leader
     s_stile[b] = x[2];
-    s_len[b] = x[6];  // tokens of the sequences before; the prefix lengths are no longer needed
+    const auto enter = [&](int m, int of, int tokens, int keys) {
+      s_at[m] = of;
+      s_n[m] = tiles_of(tokens);
+      s_lu[m] = lead_for(tokens);
+      s_u[m] = lead_for(tokens) + units_of(keys);
+    };
+    int m = x[5];
     if (s_count[b] > 0 && tiles_of(s_count[b]) > 1) {
-      s_wide[b] = x[5];
-      s_at[x[5]] = b;
-      s_n[x[5]] = tiles_of(s_count[b]);
-      s_lu[x[5]] = lead_for(s_count[b]);
-      s_u[x[5]] = lead_for(s_count[b]) + units_of(s_shared[b]);
+      s_wide[b] = m;
+      enter(m++, b, s_count[b], s_shared[b]);
+    }
+    if (own_wide(b)) {
+      s_wide_own[b] = m;
+      enter(m, b | kOwnEntry, s_tok[b], s_keys[b] - s_shared[b]);
     }
     add(b);
   }
   if (tid == 0) s_pick[0] = -1;
   __syncthreads();
 
-  // The cut: `len` units a workgroup.  Prefixes of several tiles are cut apart from everything else: those with the same number of tiles
+  // The cut: `len` units a workgroup.  Prefixes (with wide_own also own keys) of several tiles are cut apart from everything else: those with the same number of tiles
   // lie on one axis, every cut of it is a workgroup for each of the tiles, and these run at the same time and find what the first of
   // them loads in their XCD's L2.  (With its tiles one behind the other all of them read the keys from beyond L2.)  That takes a few
   // more workgroups, so `len` is the shortest of 64 lengths, a lane each, for which there are enough.
@@ -433,12 +450,15 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   };
   if (wave == 0 && n_multi > 0) {
     const int len = length_at(lane);
-    int need = 0, rest = all_units;
-    for (int m = 0; m < n_multi; ++m) {
-      need += s_n[m] * cuts(s_end[m], len);
-      rest -= s_n[m] * s_u[m];
+    int need = 0;
+    for (int m0 = 0; m0 < n_multi; m0 += 64) {
+      const int end = m0 + lane < n_multi ? s_end[m0 + lane] : 0, n = m0 + lane < n_multi ? s_n[m0 + lane] : 0;
+      for (unsigned long long kinds = __ballot(end > 0); kinds; kinds &= kinds - 1) {
+        const int m = __builtin_ctzll(kinds);
+        need += __builtin_amdgcn_readlane(n, m) * cuts(__builtin_amdgcn_readlane(end, m), len);
+      }
     }
-    const unsigned long long enough = __ballot(need + cuts(rest, len) <= a.n_wg);
+    const unsigned long long enough = __ballot(need + cuts(all_units - wide_units, len) <= a.n_wg);
     if (enough != 0 && lane == 0) s_pick[0] = __builtin_ctzll(enough);
   }
   __syncthreads();
@@ -448,29 +468,44 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   const auto pieces_at = [&](int m) {  // of a tile: from the cut of its first key to that of its last
     return (s_pos[m] + s_u[m] - 1) / len - (s_pos[m] + s_lu[m]) / len + 1;
   };
-  int wg0 = 0, wide_parts = 0;  // workgroups and pieces of these prefixes
+  int wg0 = 0, wide_parts = 0;  // workgroups and pieces of these
   if (apart) {
-    for (int m = 0; m < n_multi; ++m) {
-      if (tid == 0) s_part[m] = wide_parts;
-      wg0 += s_n[m] * cuts(s_end[m], len);
-      wide_parts += s_n[m] * pieces_at(m);
+    const int per_m = (n_multi + n_thr - 1) / n_thr, m0 = min(n_multi, tid * per_m), m1 = min(n_multi, m0 + per_m);
+    int z[2] = {0, 0}, z_before[2], z_total[2];
+    for (int m = m0; m < m1; ++m) z[0] += s_n[m] * cuts(s_end[m], len), z[1] += s_n[m] * pieces_at(m);
+    block_sums(z, z_before, z_total, s_sum);
+    for (int m = m0; m < m1; ++m) {
+      s_part[m] = z_before[1];
+      z_before[1] += s_n[m] * pieces_at(m);
     }
+    wg0 = z_total[0], wide_parts = z_total[1];
   }
   const auto stands_apart = [&](int b) { return apart && tiles_of(s_count[b]) > 1; };
-  int y[2] = {0, 0}, y_before[2], y_total[2];
+  const auto own_apart = [&](int b) { return apart && own_wide(b); };
+  int* const s_rest = s_id;  // (the ids are no longer needed)
+  int y[4] = {0, 0, 0, 0}, y_before[4], y_total[4];
   const auto add_cut = [&](int b) {
     const int c = s_count[b], own = s_keys[b] - s_shared[b];
-    if (c > 0 && !stands_apart(b)) y[0] += tiles_of(c) * (lead_for(c) + units_of(s_shared[b]));
-    if (own > 0) y[1] += tiles_of(s_tok[b]) * (lead_for(s_tok[b]) + units_of(own));
+    if (c > 0 && !stands_apart(b)) {
+      y[0] += tiles_of(c) * (lead_for(c) + units_of(s_shared[b]));
+      y[2] += c;
+    }
+    if (own > 0 && !own_apart(b)) {
+      y[1] += tiles_of(s_tok[b]) * (lead_for(s_tok[b]) + units_of(own));
+      y[3] += s_tok[b];
+    }
   };
   for (int b = b0; b < b1; ++b) add_cut(b);
   block_sums(y, y_before, y_total, s_sum);
-  const int prefix_units = y_total[0], units = prefix_units + y_total[1];
+  const int prefix_units = y_total[0], units = prefix_units + y_total[1], rest_tokens = y_total[2];
   const int n_wg = wg0 + cuts(units, len);
-  y[0] = y_before[0], y[1] = y_before[1];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = y_before[i];
   for (int b = b0; b < b1; ++b) {
     s_unit[b] = y[0];
     s_own[b] = y[1];
+    s_rest[b] = y[2];  // tokens, on this axis, of the groups before
+    s_len[b] = y[3];   // and of the sequences before; the prefix lengths are no longer needed
     add_cut(b);
   }
   __syncthreads();
@@ -505,6 +540,12 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   // Workspace rows.  Prefixes that are cut apart: 64 a piece.  Behind them, along the other axis: those of the tiles before, each once, and
   // 64 for every cut up to a tile's first key.
   const int rest_part = kTileRows * wide_parts;
+  // first tile of an entry of the wide ones, and of what begins at a place of the common axis
+  const auto entry_tile = [&](int m) { return s_at[m] >= kOwnEntry ? p_tiles + s_stile[s_at[m] - kOwnEntry] : s_ptile[s_at[m]]; };
+  const auto tile_behind = [&](int end) {
+    return end >= units ? n_tiles : end < prefix_units ? s_ptile[last_at_or_below(s_unit, a.B, end)]
+                                                       : p_tiles + s_stile[last_at_or_below(s_own, a.B, end - prefix_units)];
+  };
   const auto tile_at = [&](int i) {
     Tile t;
     int n_units, from, rows_before;
@@ -524,18 +565,16 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
         const int m = s_wide[b], next = s_next[m];
         t.n_pieces = pieces_at(m);
         t.part = kTileRows * (s_part[m] + k * t.n_pieces);
-        t.next = next < 0 ? n_tiles : s_ptile[s_at[next]] + k;
+        t.next = next < 0 ? n_tiles : entry_tile(next) + k;
         return t;
       }
       from = s_unit[b] + k * (t.lead + n_units);
-      const int end = from + t.lead + n_units;
-      t.next = k + 1 < n ? i + 1 : end < prefix_units ? s_ptile[last_at_or_below(s_unit, a.B, end)] : p_tiles;
-      rows_before = s_base[b] * a.group + t.row0;
+      t.next = k + 1 < n ? i + 1 : tile_behind(from + t.lead + n_units);
+      rows_before = s_rest[b] * a.group + t.row0;
     } else {
       const int b = last_at_or_below(s_stile, a.B, i - p_tiles), k = i - p_tiles - s_stile[b];
       n_units = units_of(s_keys[b] - s_shared[b]);
       t.lead = lead_for(s_tok[b]);
-      from = prefix_units + s_own[b] + k * (t.lead + n_units);
       t.base = base_of(b);
       t.slot = s_slot[b];
       t.row0 = k * kTileRows;
@@ -544,8 +583,16 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
       t.t_end = s_keys[b];
       t.shared = 0;
       t.again = tiles_of(s_tok[b]) > 1;
-      t.next = i + 1;
-      rows_before = (shared_tokens + s_len[b]) * a.group + t.row0;
+      if (own_apart(b)) {
+        const int m = s_wide_own[b], next = s_next[m];
+        t.n_pieces = pieces_at(m);
+        t.part = kTileRows * (s_part[m] + k * t.n_pieces);
+        t.next = next < 0 ? n_tiles : entry_tile(next) + k;
+        return t;
+      }
+      from = prefix_units + s_own[b] + k * (t.lead + n_units);
+      t.next = !a.wide_own || k + 1 < tiles_of(s_tok[b]) ? i + 1 : tile_behind(from + t.lead + n_units);
+      rows_before = (rest_tokens + s_len[b]) * a.group + t.row0;
     }
     const int first = (from + t.lead) / len;
     t.n_pieces = (from + t.lead + n_units - 1) / len - first + 1;
@@ -570,7 +617,7 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
         const int n = s_n[m], all = s_end[m];
         from = rest / n * len;
         while (s_pos[m] + s_u[m] <= from) m = s_next[m];
-        index = s_ptile[s_at[m]] + rest % n;
+        index = entry_tile(m) + rest % n;
         offset = from - s_pos[m];
         units_to_do = min(len, all - from);
         start = s_pos[m] + s_lu[m];
@@ -1545,8 +1592,8 @@ extern "C" int64_t fp_shared_decode_workspace_bytes(int32_t B, int32_t S, int32_
 
 namespace {
 
-// (`alone`: prefix_ids and prefix_lens may be null)
-int make_plan(const char* what, bool alone, const int64_t* batch_idx, const void* input_pos, int pos_index_type, const int32_t* prefix_ids,
+// (`tree`: prefix_ids and prefix_lens may be null)
+int make_plan(const char* what, bool tree, const int64_t* batch_idx, const void* input_pos, int pos_index_type, const int32_t* prefix_ids,
               const int32_t* prefix_lens, int32_t B, int32_t S, int32_t Hq, int32_t Hc, int32_t D, int32_t max_batch,
               int32_t max_context, void* plan, int64_t plan_bytes, void* stream) {
   if (const int rc = check_shape(what, B, S, Hq, Hc, D)) return rc;
@@ -1557,17 +1604,18 @@ int make_plan(const char* what, bool alone, const int64_t* batch_idx, const void
   if (pos_index_type != FP_INDEX_I32 && pos_index_type != FP_INDEX_I64)
     return fp::fail(FP_ERR_INVALID_ARGUMENT, "%s: pos_index_type %d", what, pos_index_type);
   if (B == 0) return FP_OK;
-  if (!batch_idx || !input_pos || (alone ? !prefix_ids != !prefix_lens : !prefix_ids || !prefix_lens) || !plan)
+  if (!batch_idx || !input_pos || (tree ? !prefix_ids != !prefix_lens : !prefix_ids || !prefix_lens) || !plan)
     return fp::fail(FP_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
   if (plan_bytes < fp_shared_decode_plan_bytes(B, S, Hq, Hc, D) || !fp::aligned(plan, 16))
     return fp::fail(FP_ERR_WORKSPACE, "%s: the plan needs %lld bytes, 16-byte aligned (got %lld)", what,
                     static_cast<long long>(fp_shared_decode_plan_bytes(B, S, Hq, Hc, D)), static_cast<long long>(plan_bytes));
   const Layout l = layout_of(B, S, Hq, Hc);
   const PlanArgs a{batch_idx, input_pos, pos_index_type, prefix_ids, prefix_lens, B, S, Hq, Hc, Hq / Hc, max_batch, max_context,
-                   l.n_wg, static_cast<char*>(plan), l.seqs, l.tokens, l.place, l.shares, l.tiles};
+                   l.n_wg, static_cast<char*>(plan), l.seqs, l.tokens, l.place, l.shares, l.tiles,
+                   tree && S * (Hq / Hc) > kTileRows && B <= kWideOwn};
   // as many as there are shares, tiles and sequences to write: 64 sequences 2 us less with 512 than with 256, a few no more
   const int threads = S > 1 || B > 64 ? 1024 : B > 24 ? 512 : 256;
-  const size_t lds = kPlanArrays * static_cast<size_t>((B + 3) & ~3) * sizeof(int);
+  const size_t lds = (kPlanArrays + (a.wide_own ? kWideArrays + 1 : 0)) * static_cast<size_t>((B + 3) & ~3) * sizeof(int);
   if (lds > 64 * 1024) {
     const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(shared_plan_kernel),
                                                    hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));

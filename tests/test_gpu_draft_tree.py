@@ -199,6 +199,28 @@ def test_long_context_and_many_sequences():
     case.check(case.call(ops))
 
 
+@pytest.mark.parametrize("dtype,D,Hq,Hc", [(BF16, 128, 8, 1), (F16, 64, 16, 2), (F32, 128, 4, 2), (BF16, 128, 4, 1)])
+def test_trees_of_several_tiles_of_rows(dtype, D, Hq, Hc):
+    """Sequences of one to eight tiles of 64 rows, alone and in groups of as many, on long and short contexts: tiles of one sequence are cut at
+    the same keys."""
+    gen = torch.Generator().manual_seed(9)
+    seqs = []
+    for b in range(23):
+        n = (64, 1, 33, 17, 0, 48, 9, 64)[b % 8]
+        seqs.append((b % 4 - 1, (1500, 3, 0, 700, 64, 129, 2311)[b % 7], random_tree(gen, n, 1 + b % 5)))
+    case = DraftBatch(35, [64, 300, 1024], seqs, Hq=Hq, Hc=Hc, D=D, P=64, dtype=dtype, S=64).on()
+    case.check(case.call(ops))
+    case.check(case.call(ops, share=False))
+
+
+@pytest.mark.parametrize("B", [1024, 1030])
+def test_the_most_sequences_of_several_tiles(B):
+    gen = torch.Generator().manual_seed(10)
+    seqs = [(-1, b % 5, random_tree(gen, (9, 1, 12)[b % 3], 2)) for b in range(B)]
+    case = DraftBatch(36, [], seqs, Hq=8, Hc=1, D=64, P=16, dtype=BF16).on()
+    case.check(case.call(ops))
+
+
 def test_refusals():
     case = DraftBatch(34, [], [(-1, 5, chain(3))], Hq=4, Hc=2, D=64, P=32, dtype=BF16).on()
     T = ops.DraftTree
