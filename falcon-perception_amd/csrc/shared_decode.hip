@@ -367,6 +367,11 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   }
 
   const auto lead_for = [&](int tokens) { return lead_of(tokens * a.group); };
+  // rows of a tile of own keys: with wide_own as many in each, in blocks of 16, so that the workgroups that run together end together
+  const auto own_rows = [&](int tokens) {
+    const int rows = tokens * a.group, n = (rows + kTileRows - 1) / kTileRows;
+    return a.wide_own && n > 1 ? ((rows + n - 1) / n + 15) & ~15 : kTileRows;
+  };
   const auto tiles_of = [&](int tokens) { return (tokens * a.group + kTileRows - 1) / kTileRows; };
   // sums over the sequences before, consecutive ones a thread
   const int per = (a.B + n_thr - 1) / n_thr, b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
@@ -577,8 +582,9 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
       t.lead = lead_for(s_tok[b]);
       t.base = base_of(b);
       t.slot = s_slot[b];
-      t.row0 = k * kTileRows;
-      t.n_rows = min(kTileRows, s_tok[b] * a.group - t.row0);
+      const int rows = own_rows(s_tok[b]);
+      t.row0 = k * rows;
+      t.n_rows = min(rows, s_tok[b] * a.group - t.row0);
       t.t_begin = s_shared[b];
       t.t_end = s_keys[b];
       t.shared = 0;
@@ -1415,6 +1421,8 @@ __global__ __launch_bounds__(kThreads, (sizeof(Shared<E, D, kTree>) <= 80 * 1024
         run_piece<E, D, kTree, 1>(a, sh, wave, t, piece, t0, t1);
       else if (t.n_rows <= 32)
         run_piece<E, D, kTree, 2>(a, sh, wave, t, piece, t0, t1);
+      else if (kTree && t.n_rows <= 48)
+        run_piece<E, D, kTree, kTree ? 3 : 4>(a, sh, wave, t, piece, t0, t1);
       else
         run_piece<E, D, kTree, 4>(a, sh, wave, t, piece, t0, t1);
     }
@@ -1478,9 +1486,11 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(const SharedArgs 
         step = t.n_rows;
       }
       if (s.own_tile >= 0) {
-        const Tile t = tiles[s.own_tile + x / kTileRows];
+        // (own_step: rows of its first tile, as many as of every one but the last)
+        const int tile = kTree ? x / s.own_step : x / kTileRows;
+        const Tile t = tiles[s.own_tile + tile];
         n_own = t.n_pieces;
-        own_at = t.part + x % kTileRows;
+        own_at = t.part + x - tile * (kTree ? s.own_step : kTileRows);
         own_step = t.n_rows;
       }
     }
