@@ -690,7 +690,9 @@ struct SharedArgs {
   int64_t seqs, tokens, place, shares, tiles;
   float* ws_acc;  // [part rows, Hc, D]
   float* ws_ml;   // [part rows, Hc, 2]
-  const int64_t* masks;  // [B, S], of a tree of drafts: bit i is the key of draft i
+  // of a tree of drafts
+  const int64_t* masks;  // [B, S]: bit i is the key of draft i
+  uint32_t q_signs;      // what turns the signs of q around, if the scale is below 0 (qscale is above it)
 };
 
 struct BF16 {
@@ -749,7 +751,11 @@ struct F16 {
     const float l0 = fminf(p0 * 0x1p+102f, 0x1p-24f), l1 = fminf(p1 * 0x1p+102f, 0x1p-24f);
     const auto h = __builtin_amdgcn_cvt_pkrtz(fmaxf(p0, l0), fmaxf(p1, l1));
     hi = __builtin_bit_cast(uint32_t, h);
-    lo = pack2(fmaxf(p0 - static_cast<float>(h[0]), l0), fmaxf(p1 - static_cast<float>(h[1]), l1));
+    // p less its upper part, from the 16 bits of that (0 or above, as l0 and l1: the larger one also as a whole number)
+    int r0, r1;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(hi), "v"(p0));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r1) : "v"(hi), "v"(p1));
+    lo = pack2(__int_as_float(max(r0, __float_as_int(l0))), __int_as_float(max(r1, __float_as_int(l1))));
   }
 };
 struct F32 {
@@ -971,6 +977,13 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D, kTre
       if (kTail && cb == wave) tail = *reinterpret_cast<const v4u*>(src + QR * 64);  // a block a wavefront
     }
     __builtin_amdgcn_sched_barrier(0);  // all of them are on their way before the first is waited for
+    if (kTree && a.q_signs != 0) {
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+        for (int kk = 0; kk < QR; ++kk) q[cb][kk] ^= a.q_signs;
+      tail ^= a.q_signs;
+    }
   }
   if (wave == 0 && lane_id() == 0) sh.tainted = 0;  // ahead of the barriers of the first segment
 
@@ -1122,8 +1135,10 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D, kTre
             }
           }
         }
+        if constexpr (!kTree) {
 #pragma unroll
-        for (int cb = 0; cb < CB; ++cb) sc[cb][blk] *= a.qscale;
+          for (int cb = 0; cb < CB; ++cb) sc[cb][blk] *= a.qscale;
+        }
       }
       if (c0 + G::TS > min(seg1, least)) {
 #pragma unroll
@@ -1177,7 +1192,17 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D, kTre
         if constexpr (G::k16) {
           // lanes 4 j + c of a 16-lane block name elements 4 c .. of key 4 * grp + j and receive element `col` of the four keys
           const int r = n / G::DB * 16 + (lane_now >> 4) * 4 + ((lane_now & 15) >> 2);
-          return lds_read_tr(v_lds + ((r * G::ROWB + G::v_swz(r) * 32 + (lane_now & 3) * 8) ^ (n % G::DB * 32)));
+          const char* const from = v_lds + ((r * G::ROWB + G::v_swz(r) * 32 + (lane_now & 3) * 8) ^ (n % G::DB * 32));
+          if constexpr (kTree) {
+            // both halves of the operand from LDS, which has room for that where the vector pipe is what a stage waits for
+            auto at = (__attribute__((address_space(3))) s16x4*)from;
+            const s16x4 first = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at);
+            asm volatile("" : "+v"(at));
+            const s16x4 again = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at);
+            return __builtin_bit_cast(v4u, __builtin_shufflevector(first, again, 0, 1, 2, 3, 4, 5, 6, 7));
+          } else {
+            return lds_read_tr(from);
+          }
         } else {
           const int r = n / (D / 64) / 4 * 16 + (lane_now >> 4) * 4 + n / (D / 64) % 4;
           return *reinterpret_cast<const f32x4*>(v_lds + r * G::ROWB + n % (D / 64) * 256 + (lane_now & 15) * 16);
@@ -1200,6 +1225,7 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D, kTre
         for (int blk = 0; blk < G::NB; ++blk)
 #pragma unroll
           for (int j = 0; j < 4; ++j) cand[cb] = fmaxf(cand[cb], sc[cb][blk][j]);
+        if constexpr (kTree) cand[cb] *= a.qscale;  // one product for the largest; the others have it in the sum in front of the exponential
         grown |= cand[cb] > m[cb] + (E::kHeadroom + kMaxSlack);
       }
       if (__any(grown)) {
@@ -1223,7 +1249,7 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D, kTre
         for (int blk = 0; blk < G::NB; ++blk)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            sc[cb][blk][j] = fast_exp2(sc[cb][blk][j] - ms);
+            sc[cb][blk][j] = fast_exp2(kTree ? fmaf(sc[cb][blk][j], a.qscale, -ms) : sc[cb][blk][j] - ms);
             l[cb] += sc[cb][blk][j];
           }
       }
@@ -1242,8 +1268,13 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D, kTre
           }
 #pragma unroll
           for (int db = 0; db < G::DB; ++db) {
-            const uint2 half = __builtin_bit_cast(uint2, v_ahead[(blk * G::DB + db) % kAheadV]);
-            const v4u va = {half.x, half.y, half.x, half.y};
+            v4u va;
+            if constexpr (kTree) {
+              va = v_ahead[(blk * G::DB + db) % kAheadV];
+            } else {
+              const uint2 half = __builtin_bit_cast(uint2, v_ahead[(blk * G::DB + db) % kAheadV]);
+              va = v4u{half.x, half.y, half.x, half.y};
+            }
 #pragma unroll
             for (int cb = 0; cb < CB; ++cb) o[cb][db] = E::mfma_k32(va, pb[cb], o[cb][db]);
             if (blk * G::DB + db + kAheadV < G::NB * G::DB) v_ahead[(blk * G::DB + db) % kAheadV] = read_v(blk * G::DB + db + kAheadV);
@@ -1668,13 +1699,15 @@ int attend(const char* what, bool tree, const int64_t* masks, const void* q, int
   const Layout l = layout_of(B, S, Hq, Hc);
   const int G = Hq / Hc;
   float* const acc = static_cast<float*>(workspace);
+  const float qscale = scale * kLog2e;
+  const bool turned = tree && qscale < 0.f;
   const SharedArgs a{static_cast<const char*>(q), q_stride_b * e, q_stride_h * e, q_stride_s * e,
                      static_cast<const char*>(pool_k), static_cast<const char*>(pool_v), page_table, pt_row_stride, batch_idx,
                      input_pos, pos_index_type, static_cast<char*>(out), out_stride_b * e, out_stride_h * e, out_stride_s * e,
                      lse, sinks, B, S, Hq, Hc, fp::PageDiv(page_size), n_pages, max_batch,
-                     static_cast<int>(n_slots / page_size), n_slots, max_context, scale * kLog2e, G, fp::log2_exact(G),
+                     static_cast<int>(n_slots / page_size), n_slots, max_context, turned ? -qscale : tree && qscale == 0.f ? 0x1p-126f : qscale, G, fp::log2_exact(G),
                      static_cast<const char*>(plan), l.seqs, l.tokens, l.place, l.shares, l.tiles, acc, acc + l.part_rows * Hc * D,
-                     masks};
+                     masks, !turned ? 0u : dtype == FP_DTYPE_F32 ? 0x80000000u : 0x80008000u};
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const auto go = [&](auto element) {
     using E = decltype(element);
