@@ -136,6 +136,7 @@ struct PlanArgs {
   int B, S, Hq, Hc, group, max_batch, max_context, n_wg;
   char* plan;
   int64_t seqs, tokens, place, shares, tiles;
+  int tree;
   int wide_own;  // own keys of several tiles are cut as prefixes of several tiles are
 };
 
@@ -180,7 +181,8 @@ __device__ __forceinline__ void block_sums(const int (&x)[N], int (&before)[N], 
   __syncthreads();
 }
 
-constexpr int kPlanArrays = 23, kWideArrays = 8;  // these hold a number for each sequence, or two of them with wide_own, and one array more
+// Arrays of a number for each sequence; of the last 8 with wide_own two, and one array more; of trees one like the last 8 more
+constexpr int kPlanArrays = 23, kWideArrays = 8;
 constexpr int kWideOwn = 1024;  // sequences up to which they fit
 constexpr int kOwnEntry = 1 << 20;
 
@@ -211,7 +213,8 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   int* const s_end = s_pos + Wp;       //   length of that axis, at the first of a kind, elsewhere 0,
   int* const s_next = s_end + Wp;      //   the next of its kind, -1: none,
   int* const s_part = s_next + Wp;     //   pieces of the groups before
-  int* const s_wide_own = s_part + Wp; // with wide_own: place of a sequence's own keys in the lists
+  int* const s_cut_len = s_part + Wp;  // of trees: units between the cuts of its axis
+  int* const s_wide_own = s_cut_len + Wp;  // with wide_own: place of a sequence's own keys in the lists
   __shared__ int s_sum[16 * 7], s_pick[1], s_turn[2];
   const int tid = threadIdx.x, n_thr = blockDim.x, lane = tid & 63, wave = tid >> 6, n_waves = n_thr / 64;
   Sequence* const seqs = reinterpret_cast<Sequence*>(a.plan + a.seqs);
@@ -446,6 +449,7 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
     s_pos[m] = pos;
     s_end[m] = first ? all : 0;
     s_next[m] = next;
+    if (a.tree) s_cut_len[m] = all;
   }
   __syncthreads();
   const int shortest_len = max(kMinUnits, (all_units + a.n_wg - 1) / a.n_wg);
@@ -470,14 +474,23 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   const int pick = s_pick[0];
   const bool apart = pick >= 0;  // else there are too many kinds of groups: all on one axis
   const int len = apart ? length_at(pick) : shortest_len;
+  // An axis is cut into as many shares as that length makes of it.  Of trees they are equal ones, and the common axis, which is cut
+  // after the others, has all workgroups that are left (37 sequences on 4 pictures, 56 rows each, 1430 units a head: shares of 3 to 20 units
+  // were 33 us a layer).
+  if (a.tree && apart) {
+    for (int m = tid; m < n_multi; m += n_thr) s_cut_len[m] = (s_cut_len[m] - 1) / cuts(s_cut_len[m], len) + 1;
+    __syncthreads();
+  }
+  const auto len_of = [&](int m) { return a.tree ? s_cut_len[m] : len; };
   const auto pieces_at = [&](int m) {  // of a tile: from the cut of its first key to that of its last
+    const int len = len_of(m);
     return (s_pos[m] + s_u[m] - 1) / len - (s_pos[m] + s_lu[m]) / len + 1;
   };
   int wg0 = 0, wide_parts = 0;  // workgroups and pieces of these
   if (apart) {
     const int per_m = (n_multi + n_thr - 1) / n_thr, m0 = min(n_multi, tid * per_m), m1 = min(n_multi, m0 + per_m);
     int z[2] = {0, 0}, z_before[2], z_total[2];
-    for (int m = m0; m < m1; ++m) z[0] += s_n[m] * cuts(s_end[m], len), z[1] += s_n[m] * pieces_at(m);
+    for (int m = m0; m < m1; ++m) z[0] += s_n[m] * cuts(s_end[m], len_of(m)), z[1] += s_n[m] * pieces_at(m);
     block_sums(z, z_before, z_total, s_sum);
     for (int m = m0; m < m1; ++m) {
       s_part[m] = z_before[1];
@@ -503,7 +516,8 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   for (int b = b0; b < b1; ++b) add_cut(b);
   block_sums(y, y_before, y_total, s_sum);
   const int prefix_units = y_total[0], units = prefix_units + y_total[1], rest_tokens = y_total[2];
-  const int n_wg = wg0 + cuts(units, len);
+  const int rest_len = a.tree && units > 0 && a.n_wg > wg0 ? max(kMinUnits, (units - 1) / (a.n_wg - wg0) + 1) : len;
+  const int n_wg = wg0 + cuts(units, rest_len);
 #pragma unroll
   for (int i = 0; i < 4; ++i) y[i] = y_before[i];
   for (int b = b0; b < b1; ++b) {
@@ -600,8 +614,8 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
       t.next = !a.wide_own || k + 1 < tiles_of(s_tok[b]) ? i + 1 : tile_behind(from + t.lead + n_units);
       rows_before = (rest_tokens + s_len[b]) * a.group + t.row0;
     }
-    const int first = (from + t.lead) / len;
-    t.n_pieces = (from + t.lead + n_units - 1) / len - first + 1;
+    const int first = (from + t.lead) / rest_len;
+    t.n_pieces = (from + t.lead + n_units - 1) / rest_len - first + 1;
     t.part = rest_part + rows_before + kTileRows * first;
     return t;
   };
@@ -612,15 +626,16 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
     const bool is_share = i < n_wg, is_tile = !is_share && k < 0, of_own = k & 1;
     int index = -1, offset = 0, units_to_do = 0, piece = 0;
     if (is_share) {
-      int start, from;  // of the first tile's first key and of this workgroup, on their axis
+      int start, from, len = rest_len;  // of the first tile's first key and of this workgroup, on their axis
       if (i < wg0) {
         int m = 0, rest = i;  // the first group of the kind, workgroups of the kind before this one
         for (;; ++m) {
-          const int here = s_n[m] * cuts(s_end[m], len);
+          const int here = s_n[m] * cuts(s_end[m], len_of(m));
           if (rest < here) break;
           rest -= here;
         }
         const int n = s_n[m], all = s_end[m];
+        len = len_of(m);
         from = rest / n * len;
         while (s_pos[m] + s_u[m] <= from) m = s_next[m];
         index = entry_tile(m) + rest % n;
@@ -1653,10 +1668,10 @@ int make_plan(const char* what, bool tree, const int64_t* batch_idx, const void*
   const Layout l = layout_of(B, S, Hq, Hc);
   const PlanArgs a{batch_idx, input_pos, pos_index_type, prefix_ids, prefix_lens, B, S, Hq, Hc, Hq / Hc, max_batch, max_context,
                    l.n_wg, static_cast<char*>(plan), l.seqs, l.tokens, l.place, l.shares, l.tiles,
-                   tree && S * (Hq / Hc) > kTileRows && B <= kWideOwn};
+                   tree, tree && S * (Hq / Hc) > kTileRows && B <= kWideOwn};
   // as many as there are shares, tiles and sequences to write: 64 sequences 2 us less with 512 than with 256, a few no more
   const int threads = S > 1 || B > 64 ? 1024 : B > 24 ? 512 : 256;
-  const size_t lds = (kPlanArrays + (a.wide_own ? kWideArrays + 1 : 0)) * static_cast<size_t>((B + 3) & ~3) * sizeof(int);
+  const size_t lds = (kPlanArrays + (a.wide_own ? kWideArrays + 3 : tree ? 1 : 0)) * static_cast<size_t>((B + 3) & ~3) * sizeof(int);
   if (lds > 64 * 1024) {
     const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(shared_plan_kernel),
                                                    hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
