@@ -3,14 +3,19 @@
 //   pool[p, slot(cached_b + i), :] = pool[p, slot(cached_b + path_i), :]   for i < n_b, every plane p (layer, K or V, head)
 //
 // A path rises, so path_i >= i: a row is written over only where it is read for an earlier place.  A plane's rows are therefore all read
-// before the first is written.
+// before the first is written: by one wavefront, which has several planes' rows on their way at once and waits for no other.
+//
+// The bytes bound it, read and written once: 65 MB (64 sequences, 1 to 7 rows kept of up to 32, 28 layers of 16 heads of 256 bytes) in 14.9 us,
+// 4.4 TB/s, of which 3 us pass before the first row's address is known (slot, count, path, page: each in the one before); the smallest
+// calls take 3.8 us.  With a workgroup to a plane's rows, a division for every chunk and stores that stay in L2 it was 19.3 us; with 8 chunks
+// a lane instead of 4 (half the wavefronts) 19.2; with ordinary stores 16.0 (and 2 us more until the next kernel begins).
 #include "fp_common.h"
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kMaxPath = 64;
-constexpr int kAhead = 8;  // chunks a thread has on their way
+constexpr int kAhead = 4;  // chunks a lane has on their way
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
 struct KeepArgs {
@@ -24,6 +29,7 @@ struct KeepArgs {
   int64_t planes, plane_bytes, n_slots;
   int B, S, n_pages, max_batch, pool_pages;
   int chunks;  // 16-byte chunks of a row
+  uint32_t per_row;
   fp::PageDiv pd;
 };
 
@@ -36,6 +42,9 @@ __device__ __forceinline__ int64_t slot_of(const KeepArgs& a, int64_t row, int64
   const int64_t page = a.page_table[row * a.pt_row_stride + blk];
   return page < 0 || page >= a.pool_pages ? -1 : page * a.pd.page_size + off;
 }
+
+// i / d for i below 2^16 and d above 1, from m = 2^32 / d rounded up.
+__device__ __forceinline__ int over(int i, uint32_t m) { return static_cast<int>(__umulhi(static_cast<uint32_t>(i), m)); }
 
 __global__ __launch_bounds__(kThreads) void keep_rows_kernel(const KeepArgs a) {
   __shared__ int64_t s_from[kMaxPath], s_to[kMaxPath];  // byte offsets in a plane
@@ -65,53 +74,35 @@ __global__ __launch_bounds__(kThreads) void keep_rows_kernel(const KeepArgs a) {
   if (__syncthreads_or(twice)) return;
   const int n = s_n;
   if (n == 0) return;
-  const int items = n * a.chunks;  // of a plane
-  if (items <= kThreads * kAhead / 2) {
-    // several planes at once
-    const int at_once = kThreads * kAhead / items;
-    const int64_t groups = (a.planes + at_once - 1) / at_once;
-    for (int64_t g = blockIdx.x; g < groups; g += gridDim.x) {
-      const int64_t plane0 = g * at_once;
-      const int here = static_cast<int>(a.planes - plane0 < at_once ? a.planes - plane0 : at_once);
+  // A wavefront takes the rows of some planes at once, or those of one plane in turns in the order of the path: what one turn writes is
+  // read by no turn after it.
+  const int lane = tid & 63, wave = tid >> 6;
+  const int room = 64 * kAhead;  // chunks
+  const int rows = min(n, room / a.chunks), items = rows * a.chunks, at_once = rows < n ? 1 : room / items;
+  const uint32_t per_plane = 0xffffffffu / static_cast<uint32_t>(items) + 1;
+  const int64_t n_waves = static_cast<int64_t>(gridDim.x) * kWaves;
+  for (int64_t plane0 = (static_cast<int64_t>(blockIdx.x) * kWaves + wave) * at_once; plane0 < a.planes; plane0 += n_waves * at_once) {
+    char* const base_of = a.pool + plane0 * a.plane_bytes;
+    const int here = static_cast<int>(min<int64_t>(a.planes - plane0, at_once)) * items;
+    for (int r0 = 0; r0 < n; r0 += rows) {
       v4u chunk[kAhead];
-      int64_t to[kAhead];
+      char* to[kAhead];
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
-        const int i = tid + k * kThreads;
-        to[k] = -1;
-        if (i < here * items) {
-          const int plane = i / items, rest = i - plane * items, r = rest / a.chunks, c = rest - r * a.chunks;
-          const int64_t at = (plane0 + plane) * a.plane_bytes + c * 16;
-          chunk[k] = *reinterpret_cast<const v4u*>(a.pool + at + s_from[r]);
+        const int i = lane + k * 64;
+        const int plane = items == 1 ? i : over(i, per_plane), rest = i - plane * items;
+        const int turn = a.chunks == 1 ? rest : over(rest, a.per_row), c = rest - turn * a.chunks, r = r0 + turn;
+        to[k] = nullptr;
+        if (i < here && r < n) {
+          char* const at = base_of + plane * a.plane_bytes + c * 16;
+          chunk[k] = *reinterpret_cast<const v4u*>(at + s_from[r]);
           to[k] = at + s_to[r];
         }
       }
       asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // every row has been read
-      __syncthreads();
 #pragma unroll
       for (int k = 0; k < kAhead; ++k)
-        if (to[k] >= 0) *reinterpret_cast<v4u*>(a.pool + to[k]) = chunk[k];
-    }
-    return;
-  }
-  // Many rows: those of one plane, in the order of the path.  What one turn writes is read by no turn after it.
-  const int rows = kThreads * kAhead / a.chunks;
-  for (int64_t plane = blockIdx.x; plane < a.planes; plane += gridDim.x) {
-    char* const base_of = a.pool + plane * a.plane_bytes;
-    for (int r0 = 0; r0 < n; r0 += rows) {
-      v4u chunk[kAhead];
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        const int i = tid + k * kThreads, r = r0 + i / a.chunks, c = i % a.chunks;
-        if (i < rows * a.chunks && r < n) chunk[k] = *reinterpret_cast<const v4u*>(base_of + s_from[r] + c * 16);
-      }
-      asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        const int i = tid + k * kThreads, r = r0 + i / a.chunks, c = i % a.chunks;
-        if (i < rows * a.chunks && r < n) *reinterpret_cast<v4u*>(base_of + s_to[r] + c * 16) = chunk[k];
-      }
+        if (to[k]) __builtin_nontemporal_store(chunk[k], reinterpret_cast<v4u*>(to[k]));
     }
   }
 }
@@ -139,9 +130,9 @@ extern "C" int fp_keep_rows(void* pool, const int64_t* page_table, int64_t pt_ro
   const int64_t row_bytes = static_cast<int64_t>(D) * e;
   const KeepArgs a{static_cast<char*>(pool), page_table, pt_row_stride, batch_idx, cached, cached_index_type, path, n_planes,
                    n_slots * row_bytes, n_slots, B, S, n_pages, max_batch, static_cast<int>(n_slots / page_size),
-                   static_cast<int>(row_bytes / 16), fp::PageDiv(page_size)};
-  int64_t x = (8ll * fp::compute_units() + B - 1) / B;
-  if (x > n_planes) x = n_planes;
+                   static_cast<int>(row_bytes / 16), 0xffffffffu / static_cast<uint32_t>(row_bytes / 16) + 1, fp::PageDiv(page_size)};
+  int64_t x = (16ll * fp::compute_units() + B - 1) / B;
+  if (x > (n_planes + kWaves - 1) / kWaves) x = (n_planes + kWaves - 1) / kWaves;
   hipLaunchKernelGGL(keep_rows_kernel, dim3(static_cast<unsigned>(x), static_cast<unsigned>(B)), dim3(kThreads), 0,
                      static_cast<hipStream_t>(stream), a);
   return fp::check_launch(what);
