@@ -181,8 +181,8 @@ __device__ __forceinline__ void block_sums(const int (&x)[N], int (&before)[N], 
   __syncthreads();
 }
 
-// Arrays of a number for each sequence; of the last 8 with wide_own two, and one array more; of trees one like the last 8 more
-constexpr int kPlanArrays = 23, kWideArrays = 8;
+// Arrays of a number for each sequence; of the last 10 with wide_own two, and one array more; of trees one like the last 10 more
+constexpr int kPlanArrays = 25, kWideArrays = 10;
 constexpr int kWideOwn = 1024;  // sequences up to which they fit
 constexpr int kOwnEntry = 1 << 20;
 
@@ -213,7 +213,10 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   int* const s_end = s_pos + Wp;       //   length of that axis, at the first of a kind, elsewhere 0,
   int* const s_next = s_end + Wp;      //   the next of its kind, -1: none,
   int* const s_part = s_next + Wp;     //   pieces of the groups before
-  int* const s_cut_len = s_part + Wp;  // of trees: units between the cuts of its axis
+  int* const s_first = s_part + Wp;    //   the first of its kind,
+  int* const s_wgs = s_first + Wp;     //   workgroups of the kinds before, at the first of a kind
+  int* const s_begins = s_wgs + Wp;    // the group that a workgroup of theirs begins with
+  int* const s_cut_len = s_begins + ((a.n_wg + 3) & ~3);  // of trees: units between the cuts of its axis
   int* const s_wide_own = s_cut_len + Wp;  // with wide_own: place of a sequence's own keys in the lists
   __shared__ int s_sum[16 * 7], s_pick[1], s_turn[2];
   const int tid = threadIdx.x, n_thr = blockDim.x, lane = tid & 63, wave = tid >> 6, n_waves = n_thr / 64;
@@ -432,26 +435,43 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   // lie on one axis, every cut of it is a workgroup for each of the tiles, and these run at the same time and find what the first of
   // them loads in their XCD's L2.  (With its tiles one behind the other all of them read the keys from beyond L2.)  That takes a few
   // more workgroups, so `len` is the shortest of 64 lengths, a lane each, for which there are enough.
-  for (int m = tid; m < n_multi; m += n_thr) {
-    const int n = s_n[m];
-    int pos = 0, all = 0, next = -1, first = 1;
-    for (int i = 0; i < n_multi; ++i) {
-      if (s_n[i] != n) continue;
-      const int u = s_u[i];
-      all += u;
-      if (i < m) {
-        pos += u;
-        first = 0;
-      } else if (i > m && next < 0) {
-        next = i;
-      }
+  if (n_multi > 0) {  // an entry looks at all others, four at a time, some threads an entry
+    for (int m = tid; m < n_multi; m += n_thr) {
+      s_pos[m] = s_end[m] = 0;
+      s_next[m] = s_first[m] = INT32_MAX;
     }
-    s_pos[m] = pos;
-    s_end[m] = first ? all : 0;
-    s_next[m] = next;
-    if (a.tree) s_cut_len[m] = all;
+    __syncthreads();
+    const int wide = (n_multi + 63) & ~63, parts = max(1, n_thr / wide), part = tid / wide;
+    const int per_part = ((n_multi + 3) / 4 + parts - 1) / parts * 4;
+    for (int m = parts > 1 ? tid - part * wide : tid; m < n_multi && part < parts; m += n_thr) {
+      const int n = s_n[m], from = parts > 1 ? part * per_part : 0, to = min(n_multi, from + per_part);
+      int pos = 0, all = 0, next = INT32_MAX, first = INT32_MAX;
+      for (int i = from; i < to; i += 4) {
+        const i32x4 ns = *reinterpret_cast<const i32x4*>(s_n + i), us = *reinterpret_cast<const i32x4*>(s_u + i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const bool same = ns[k] == n && i + k < to;
+          all += same ? us[k] : 0;
+          pos += same && i + k < m ? us[k] : 0;
+          next = min(next, same && i + k > m ? i + k : INT32_MAX);
+          first = min(first, same ? i + k : INT32_MAX);
+        }
+      }
+      if (all > 0) {
+        atomicAdd(&s_end[m], all);
+        atomicMin(&s_next[m], next);
+        atomicMin(&s_first[m], first);
+      }
+      if (pos > 0) atomicAdd(&s_pos[m], pos);
+    }
+    __syncthreads();
+    for (int m = tid; m < n_multi; m += n_thr) {
+      if (a.tree) s_cut_len[m] = s_end[m];
+      if (s_first[m] != m) s_end[m] = 0;
+      if (s_next[m] == INT32_MAX) s_next[m] = -1;
+    }
+    __syncthreads();
   }
-  __syncthreads();
   const int shortest_len = max(kMinUnits, (all_units + a.n_wg - 1) / a.n_wg);
   const auto cuts = [](int units, int len) { return units > 0 ? (units - 1) / len + 1 : 0; };  // (two such sums may pass 31 bits)
   const auto length_at = [&](int i) {  // the i-th of the 64: up to three times the shortest, at most everything
@@ -495,8 +515,15 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
     for (int m = m0; m < m1; ++m) {
       s_part[m] = z_before[1];
       z_before[1] += s_n[m] * pieces_at(m);
+      s_wgs[m] = z_before[0];
+      z_before[0] += s_n[m] * cuts(s_end[m], len_of(m));
     }
     wg0 = z_total[0], wide_parts = z_total[1];
+    __syncthreads();
+    for (int m = wave; m < n_multi; m += n_waves) {  // the workgroups that begin with this entry
+      const int len = len_of(m), n = s_n[m], begin = (s_pos[m] + len - 1) / len, end = (s_pos[m] + s_u[m] - 1) / len + 1;
+      for (int i = begin * n + lane; i < end * n; i += 64) s_begins[s_wgs[s_first[m]] + i] = m;
+    }
   }
   const auto stands_apart = [&](int b) { return apart && tiles_of(s_count[b]) > 1; };
   const auto own_apart = [&](int b) { return apart && own_wide(b); };
@@ -628,16 +655,10 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
     if (is_share) {
       int start, from, len = rest_len;  // of the first tile's first key and of this workgroup, on their axis
       if (i < wg0) {
-        int m = 0, rest = i;  // the first group of the kind, workgroups of the kind before this one
-        for (;; ++m) {
-          const int here = s_n[m] * cuts(s_end[m], len_of(m));
-          if (rest < here) break;
-          rest -= here;
-        }
-        const int n = s_n[m], all = s_end[m];
+        const int m = s_begins[i], first = s_first[m], n = s_n[m], rest = i - s_wgs[first];  // workgroups of the kind before this one
+        const int all = s_end[first];
         len = len_of(m);
         from = rest / n * len;
-        while (s_pos[m] + s_u[m] <= from) m = s_next[m];
         index = entry_tile(m) + rest % n;
         offset = from - s_pos[m];
         units_to_do = min(len, all - from);
@@ -1671,7 +1692,7 @@ int make_plan(const char* what, bool tree, const int64_t* batch_idx, const void*
                    tree, tree && S * (Hq / Hc) > kTileRows && B <= kWideOwn};
   // as many as there are shares, tiles and sequences to write: 64 sequences 2 us less with 512 than with 256, a few no more
   const int threads = S > 1 || B > 64 ? 1024 : B > 24 ? 512 : 256;
-  const size_t lds = (kPlanArrays + (a.wide_own ? kWideArrays + 3 : tree ? 1 : 0)) * static_cast<size_t>((B + 3) & ~3) * sizeof(int);
+  const size_t lds = ((kPlanArrays + (a.wide_own ? kWideArrays + 3 : tree ? 1 : 0)) * static_cast<size_t>((B + 3) & ~3) + ((l.n_wg + 3) & ~3)) * sizeof(int);
   if (lds > 64 * 1024) {
     const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(shared_plan_kernel),
                                                    hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
