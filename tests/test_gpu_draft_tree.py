@@ -230,6 +230,14 @@ def test_the_most_sequences_of_several_tiles(B):
     case.check(case.call(ops))
 
 
+def test_the_most_sequences():
+    """Of one cached head: the plan's arrays fill the shared memory of a workgroup."""
+    gen = torch.Generator().manual_seed(12)
+    seqs = [((b % 9) - 3, b % 5, random_tree(gen, (9, 1, 12)[b % 3], 2)) for b in range(1536)]
+    case = DraftBatch(38, [64, 130, 70, 200, 64, 300], seqs, Hq=8, Hc=1, D=64, P=16, dtype=BF16).on()
+    case.check(case.call(ops))
+
+
 def test_refusals():
     case = DraftBatch(34, [], [(-1, 5, chain(3))], Hq=4, Hc=2, D=64, P=32, dtype=BF16).on()
     T = ops.DraftTree
