@@ -321,10 +321,42 @@ __device__ __forceinline__ float log_share(float x, float peak, double slope, do
   return static_cast<float>((x == peak ? 0.0 : (static_cast<double>(x) - static_cast<double>(peak)) * slope) - log(total));
 }
 
+// Sums of three numbers over the lanes: of the first in lanes 0 to 15, of the second in 16 to 31, of the third in 32 to 47.  While lanes of
+// the first halves add to one number, those of the second add to another: 21 instructions instead of the 90 of three sums.
+__device__ __forceinline__ double add_halves(double x, double y) {  // x in lanes 0 to 31, y in 32 to 63
+  const uint64_t p = __builtin_bit_cast(uint64_t, x), q = __builtin_bit_cast(uint64_t, y);
+  const auto lo = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(p), static_cast<uint32_t>(q), false, false);
+  const auto hi = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(p >> 32), static_cast<uint32_t>(q >> 32), false, false);
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi[0]) << 32 | lo[0]) + __builtin_bit_cast(double, static_cast<uint64_t>(hi[1]) << 32 | lo[1]);
+}
+__device__ __forceinline__ double add_rows(double x, double y) {  // x in lanes 0 to 15 and 32 to 47, y in the others
+  const uint64_t p = __builtin_bit_cast(uint64_t, x), q = __builtin_bit_cast(uint64_t, y);
+  const auto lo = __builtin_amdgcn_permlane16_swap(static_cast<uint32_t>(p), static_cast<uint32_t>(q), false, false);
+  const auto hi = __builtin_amdgcn_permlane16_swap(static_cast<uint32_t>(p >> 32), static_cast<uint32_t>(q >> 32), false, false);
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi[0]) << 32 | lo[0]) + __builtin_bit_cast(double, static_cast<uint64_t>(hi[1]) << 32 | lo[1]);
+}
+__device__ __forceinline__ double sum_three(double x, double y, double z) {
+  double s = add_rows(add_halves(x, z), add_halves(y, 0.0));
+  s += from_lane<0xb1, 0xf>(s);   // quad_perm: the neighbour,
+  s += from_lane<0x4e, 0xf>(s);   // the other pair of four,
+  s += from_lane<0x141, 0xf>(s);  // row_half_mirror: the other four of eight,
+  s += from_lane<0x140, 0xf>(s);  // row_mirror: the other eight
+  return s;
+}
+
+constexpr int kHeldEach = 4, kHeld = kHeldEach * kThreads;  // pieces whose sums the last workgroup holds in LDS
 struct DrawShared {
-  double sum[kWaves];
+  double all[kHeld], kept[kHeld], taken[kHeld];
+  double sum[kWaves], total[kWaves], rest[kWaves];
   int place, flag;
 };
+
+__device__ __forceinline__ double sum_threads(double x, double (&part)[kWaves]) {  // a part once between two barriers
+  x = sum_lanes(x);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
+  __syncthreads();
+  return part[0] + part[1] + part[2] + part[3];
+}
 
 // Weights are summed by pieces of 64 vectors, a wavefront's.  The last workgroup of a request runs what follows alone, its instructions come from
 // memory as they are needed: loops, not copies of their bodies.
@@ -348,22 +380,19 @@ __device__ __forceinline__ int2 piece_range(const Row<E>& r, int V, int k) {
   return int2{k == 0 ? 0 : r.head + k * 64 * E::kVec, k == pieces - 1 ? V : r.head + (k + 1) * 64 * E::kVec};
 }
 
-// The first token at which the weights of the row pass u times their total: sum_of(k) the sum of piece k of n, weigh(x, i) the weight of
-// token i.  What it is goes to answer(token, x), by one thread; -1 if nothing weighs anything.
-template <typename E, typename S, typename W, typename A>
-__device__ __forceinline__ void draw(const Row<E>& r, int V, S sum_of, int n, float u, DrawShared& sh, W weigh, A answer) {
+// The first token at which the weights of the row pass u times their total: sum_of(k) the sum of piece k of n, weigh(x, i, load(i)) the weight
+// of token i.  What it is goes to answer(token, x), by one thread; -1 if nothing weighs anything.
+template <typename E, typename S, typename L, typename W, typename A>
+__device__ __forceinline__ void draw(const Row<E>& r, int V, double total, S sum_of, int n, float u, DrawShared& sh, L load, W weigh, A answer) {
   constexpr int kEach = elements_each<E>();
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   // by every wavefront, which all get the same
-  double total = 0.0;
-#pragma nounroll
-  for (int k = lane; k < n; k += 64) total += sum_of(k);
-  const double goal = (u < 0.f ? 0.0 : static_cast<double>(u)) * sum_lanes(total);  // (NaN passes nothing: the last token)
+  const double goal = (u < 0.f ? 0.0 : static_cast<double>(u)) * total;  // (NaN passes nothing: the last token)
   double before = 0.0, before_last = 0.0;
   int part = -1, last = -1;
 #pragma nounroll
   for (int k0 = 0; k0 < n && part < 0; k0 += 64) {
-    const double s = n <= 64 ? total : k0 + lane < n ? sum_of(k0 + lane) : 0.0, upto = scan_lanes(s);
+    const double s = k0 + lane < n ? sum_of(k0 + lane) : 0.0, upto = scan_lanes(s);
     const uint64_t past = __ballot(before + upto > goal), some = __ballot(s > 0.0);
     if (past) {
       const int l = __builtin_ctzll(past);
@@ -386,14 +415,17 @@ __device__ __forceinline__ void draw(const Row<E>& r, int V, S sum_of, int n, fl
   const int2 range = piece_range(r, V, part);
   const int mine = range.x + tid * kEach, end = range.y;
   double w[kEach], sum = 0.0;
-  float x[kEach];
+  float x[kEach], with[kEach];
   int found = -1;
   float its = 0.f;
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) x[i] = mine + i < end ? r.one(mine + i) : 0.f;
+  for (int i = 0; i < kEach; ++i) {
+    x[i] = mine + i < end ? r.one(mine + i) : 0.f;
+    with[i] = mine + i < end ? load(mine + i) : 0.f;
+  }
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
-    w[i] = mine + i < end ? weigh(x[i], mine + i) : 0.0;
+    w[i] = mine + i < end ? weigh(x[i], mine + i, with[i]) : 0.0;
     sum += w[i];
     found = w[i] > 0.0 ? mine + i : found;  // the last that weighs something
     its = w[i] > 0.0 ? x[i] : its;
@@ -662,7 +694,18 @@ __global__ __launch_bounds__(kThreads) void verify_walk_kernel(const VerifyArgs 
       x = next;
     }
     if (!last_to_arrive(a.arrivals + b, a.draws, &sh.flag)) return;
-    draw<E>(r, a.V, [&](int k) { return take(&sums[k].all); }, a.pieces, u0, sh, [&](float y, int i) { return is_out(i) ? 0.0 : weights(y); }, answer);
+    double all[kHeldEach], total = 0.0;
+#pragma unroll
+    for (int i = 0; i < kHeldEach; ++i) all[i] = take(&sums[min(i * kThreads + tid, a.pieces - 1)].all);
+#pragma unroll
+    for (int i = 0; i < kHeldEach; ++i) {
+      sh.all[i * kThreads + tid] = all[i];
+      total += i * kThreads + tid < a.pieces ? all[i] : 0.0;
+    }
+#pragma nounroll
+    for (int k = kHeld + tid; k < a.pieces; k += kThreads) total += take(&sums[k].all);
+    draw<E>(r, a.V, sum_threads(total, sh.total), [&](int k) { return k < kHeld ? sh.all[k] : take(&sums[k].all); }, a.pieces, u0, sh,
+            [](int) { return 0.f; }, [&](float y, int i, float) { return is_out(i) ? 0.0 : weights(y); }, answer);
     return;
   }
 
@@ -696,53 +739,72 @@ __global__ __launch_bounds__(kThreads) void verify_walk_kernel(const VerifyArgs 
         sum.taken += kept ? taken : 0.0;
         unsure |= fabs(left) <= 4.0 * kBand * taken && taken > 0.0;  // (NaN is not left)
       });
-      sum.all = sum_lanes(sum.all), sum.kept = sum_lanes(sum.kept), sum.taken = sum_lanes(sum.taken);
+      const double its = sum_three(sum.all, sum.kept, sum.taken);
       const bool again = __ballot(unsure) != 0;
-      if (lane == 0) {
-        publish(&sums[piece].all, sum.all);
-        publish(&sums[piece].kept, again ? -1.0 : sum.kept);
-        publish(&sums[piece].taken, sum.taken);
-      }
+      if (lane % 16 == 0 && lane < 48) publish(&sums[piece].all + lane / 16, again && lane == 16 ? -1.0 : its);
       x = next;
 #pragma unroll
       for (int i = 0; i < E::kVec; ++i) q[i] = q_next[i];
     }
   }
   if (!last_to_arrive(a.arrivals + b, a.draws, &sh.flag)) return;
-  double all = 0.0;
+  double all[kHeldEach], kept[kHeldEach], taken[kHeldEach], sum = 0.0, rest = 0.0;
+#pragma unroll
+  for (int i = 0; i < kHeldEach; ++i) {  // all of them on their way at once
+    const Piece* const its = sums + min(i * kThreads + tid, a.pieces - 1);
+    all[i] = take(&its->all), kept[i] = take(&its->kept), taken[i] = take(&its->taken);
+  }
+#pragma unroll
+  for (int i = 0; i < kHeldEach; ++i) {
+    const int k = i * kThreads + tid;
+    sh.all[k] = all[i], sh.kept[k] = kept[i], sh.taken[k] = taken[i];
+    sum += k < a.pieces ? all[i] : 0.0;
+  }
 #pragma nounroll
-  for (int k = lane; k < a.pieces; k += 64) all += take(&sums[k].all);
-  const double share = 1.0 / sum_lanes(all);
+  for (int k = kHeld + tid; k < a.pieces; k += kThreads) sum += take(&sums[k].all);
+  const double whole_total = sum_threads(sum, sh.total), share = 1.0 / whole_total;
   const auto left_of = [&](float y, float q) { return fmax(0.0, weights(y) * share - static_cast<double>(q)); };
-  // what is left of every piece; those of which it was not sure by all threads
+  // what is left of every piece, in place of what was kept; those of which it was not sure by the wavefront that found it
   double* const rests = a.rests + static_cast<int64_t>(b) * a.pieces;
-  bool some = false;
+  const auto set_rest = [&](int k, double x) {
+    rest += x;
+    if (k < kHeld)
+      sh.kept[k] = x;
+    else
+      publish(rests + k, x);
+  };
   const int rounds = (a.pieces + kThreads - 1) / kThreads;
 #pragma nounroll
   for (int round = 0; round < rounds; ++round) {
     const int k = round * kThreads + tid;
     bool unsure = false;
     if (k < a.pieces) {
-      const double kept = take(&sums[k].kept), left = fmax(0.0, kept * share - take(&sums[k].taken));
+      const double kept = k < kHeld ? sh.kept[k] : take(&sums[k].kept), taken = k < kHeld ? sh.taken[k] : take(&sums[k].taken);
       unsure = kept < 0.0;
-      if (!unsure) publish(rests + k, left);
-      some |= !unsure && left > 0.0;
+      if (!unsure) set_rest(k, fmax(0.0, kept * share - taken));
     }
-    for (uint64_t again = __ballot(unsure); again; again &= again - 1) {  // by the wavefront that found it
+    for (uint64_t again = __ballot(unsure); again; again &= again - 1) {
       const int piece = round * kThreads + wave * 64 + __builtin_ctzll(again);
       const int2 range = piece_range(r, a.V, piece);
+      float y[E::kVec + 1], q[E::kVec + 1];  // (up to 2 (kVec - 1) more than 64 vectors)
+#pragma unroll
+      for (int i = 0; i <= E::kVec; ++i) {
+        const int at = min(range.x + i * 64 + lane, range.y - 1);
+        y[i] = r.one(at), q[i] = probability(a, probs, at);
+      }
       double sum = 0.0;
-#pragma nounroll
-      for (int i = range.x + lane; i < range.y; i += 64) sum += left_of(r.one(i), probability(a, probs, i));
+#pragma unroll
+      for (int i = 0; i <= E::kVec; ++i) sum += range.x + i * 64 + lane < range.y ? left_of(y[i], q[i]) : 0.0;
       sum = sum_lanes(sum);
-      if (lane == 0) publish(rests + piece, sum);
-      some |= sum > 0.0;
+      if (lane == 0) set_rest(piece, sum);
     }
   }
   asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
-  const bool whole = !__syncthreads_or(some);  // nothing is left: the target's own distribution
-  draw<E>(r, a.V, [&](int k) { return whole ? take(&sums[k].all) : take(rests + k); }, a.pieces, u0, sh,
-          [&](float y, int i) { return whole ? weights(y) : left_of(y, probability(a, probs, i)); }, answer);
+  const double left = sum_threads(rest, sh.rest);
+  const bool whole = !(left > 0.0);  // nothing is left: the target's own distribution
+  draw<E>(r, a.V, whole ? whole_total : left,
+          [&](int k) { return k < kHeld ? whole ? sh.all[k] : sh.kept[k] : take(whole ? &sums[k].all : rests + k); }, a.pieces, u0, sh,
+          [&](int i) { return probability(a, probs, i); }, [&](float y, int, float q) { return whole ? weights(y) : left_of(y, q); }, answer);
 }
 
 struct Cut {
