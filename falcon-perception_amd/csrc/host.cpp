@@ -523,8 +523,7 @@ PyObject* verify_unguarded(PyObject* const* args) {
   const int64_t B = logits->size(0), S = logits->size(1), V = logits->size(2);
   if (S < 1 || S > 64 || V < 1 || !is_matrix(*tokens, at::kLong, B, S) || !is_matrix(*parents, at::kInt, B, S) || !is_matrix(*uniforms, at::kFloat, B, S) ||
       (heat && !is_vector(*heat, at::kFloat, B)) || !is_bytes(*ws) || !fits({B, S, V}) ||
-      !on_device(device, {logits, tokens, parents, uniforms, heat, probs, ws}) || ws->numel() < fp_verify_drafts_workspace_bytes(B, S, V) ||
-      reinterpret_cast<uintptr_t>(ws->data_ptr()) % 16 != 0)
+      !on_device(device, {logits, tokens, parents, uniforms, heat, probs, ws}))
     Py_RETURN_NONE;
   at::Tensor made[4];
   int rc;

@@ -292,8 +292,10 @@ def test_workspace_of_the_caller_and_no_requests():
     for _ in range(3):
         for w, g in zip(want, step.call(workspace=workspace)):
             assert torch.equal(w, g)
-    with pytest.raises(RuntimeError, match="workspace must be"):
+    with pytest.raises(RuntimeError, match="workspace of [0-9]+ bytes, 16-byte aligned, is needed"):
         step.call(workspace=workspace[:-1])
+    with pytest.raises(RuntimeError, match="workspace must be"):
+        step.call(workspace=workspace.view(torch.int8))
     none = ops.verify_drafts(step.logits[:0].cuda(), step.tokens[:0].cuda(), step.parents[:0].cuda(), step.uniforms[:0].cuda())
     assert none.accepted.shape == (0,) and none.tokens.shape == (0, 5)
 
