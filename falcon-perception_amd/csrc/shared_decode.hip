@@ -27,6 +27,16 @@
 // 330 us, 6.0 TB/s (1153 once a sequence).  Small batches are bound by the trips to memory in front of the first key and by two
 // launches (3 sequences, 1.5 MB: 8.9 and 4.1 us), many tokens a sequence by LDS and the instructions between the matrix products
 // (40 sequences of 24 tokens, 11.6 GFLOP: 46 us).
+//
+// Trees of drafted tokens (kTree) go the same way: a row sees the keys in front of draft 0, and of the drafts, which lie behind one
+// another, those whose bits its mask has.  The mask is looked at in the last stages only, those that reach a draft.  Their rows are many a
+// sequence, so the vector instructions between the products bound them before the bytes do; two things differ from the above for it.  The
+// scale is a factor of the sum in front of the exponential, and both halves of a V operand are read from LDS (37 sequences on 4 pictures, 56 rows each, D 64, f16: 29.2
+// us instead of 30.6; 64 of 96 rows on 4 k to 12 k keys: 547 instead of 560).  And own keys of sequences with more than 64 rows a cached head are cut as
+// prefixes of several tiles are (wide_own), in tiles of as many rows each: these 64 sequences read 2.2 GB a layer and took 822 us with tiles one
+// behind the other, which read the keys twice from beyond L2, 655 cut at the same keys (64 + 32 rows), 547 as 48 + 48; without more than 64 rows no tile has a
+// second, and the plan would hold its arrays twice for nothing.  64 sequences of 2 to 5 tokens, 680 MB a layer: 112 us, 6.1 TB/s; 16 of 17 to
+// 32, 289 MB: 61, 4.7.
 #include "decode_common.h"
 
 #include <math.h>
@@ -136,7 +146,6 @@ struct PlanArgs {
   int B, S, Hq, Hc, group, max_batch, max_context, n_wg;
   char* plan;
   int64_t seqs, tokens, place, shares, tiles;
-  int tree;
   int wide_own;  // own keys of several tiles are cut as prefixes of several tiles are
 };
 
@@ -181,11 +190,14 @@ __device__ __forceinline__ void block_sums(const int (&x)[N], int (&before)[N], 
   __syncthreads();
 }
 
-// Arrays of a number for each sequence; of the last 10 with wide_own two, and one array more; of trees one like the last 10 more
-constexpr int kPlanArrays = 25, kWideArrays = 10;
+// Arrays of a number for each sequence; of trees there are three more, and with wide_own two numbers in each of the last 11 and one array more
+constexpr int kPlanArrays = 23, kTreeArrays = 3, kWideArrays = 12;
 constexpr int kWideOwn = 1024;  // sequences up to which they fit
 constexpr int kOwnEntry = 1 << 20;
 
+// kTree: trees of drafted tokens.  Each has a search of its own for the kinds of groups: of drafts several tiles are the rule, and an entry looks
+// at all others by several threads (136 entries: 10.7 us less than by one); without drafts there are few, and the plan of 4 takes 2.2 us less by one.
+template <bool kTree>
 __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   extern __shared__ int s_mem[];
   const int Bp = (a.B + 3) & ~3;
@@ -204,7 +216,8 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   int* const s_unit = s_stile + Bp;    //   units of prefixes that are cut with everything else,
   int* const s_own = s_unit + Bp;      //   units of own keys,
   int* const s_wide = s_own + Bp;      // place of a group of several tiles in the lists of these:
-  const int Wp = a.wide_own ? 2 * Bp : Bp;
+  const bool wide_own = kTree && a.wide_own;
+  const int Wp = wide_own ? 2 * Bp : Bp;
   int* const s_at = s_wide + Bp;       //   its first sequence (with kOwnEntry: its own keys),
   int* const s_n = s_at + Wp;          //   its tiles,
   int* const s_u = s_n + Wp;           //   units of each, with the lead
@@ -213,11 +226,12 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   int* const s_end = s_pos + Wp;       //   length of that axis, at the first of a kind, elsewhere 0,
   int* const s_next = s_end + Wp;      //   the next of its kind, -1: none,
   int* const s_part = s_next + Wp;     //   pieces of the groups before
+  // of trees
   int* const s_first = s_part + Wp;    //   the first of its kind,
-  int* const s_wgs = s_first + Wp;     //   workgroups of the kinds before, at the first of a kind
-  int* const s_begins = s_wgs + Wp;    // the group that a workgroup of theirs begins with
-  int* const s_cut_len = s_begins + ((a.n_wg + 3) & ~3);  // of trees: units between the cuts of its axis
-  int* const s_wide_own = s_cut_len + Wp;  // with wide_own: place of a sequence's own keys in the lists
+  int* const s_wgs = s_first + Wp;     //   workgroups of the kinds before, at the first of a kind,
+  int* const s_cut_len = s_wgs + Wp;   //   units between the cuts of its axis
+  int* const s_begins = s_cut_len + Wp;  // the group that a workgroup of theirs begins with
+  int* const s_wide_own = s_begins + ((a.n_wg + 3) & ~3);  // with wide_own: place of a sequence's own keys in the lists
   __shared__ int s_sum[16 * 7], s_pick[1], s_turn[2];
   const int tid = threadIdx.x, n_thr = blockDim.x, lane = tid & 63, wave = tid >> 6, n_waves = n_thr / 64;
   Sequence* const seqs = reinterpret_cast<Sequence*>(a.plan + a.seqs);
@@ -233,7 +247,11 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
     const int64_t slot = b < a.B ? a.batch_idx[b] : -1;
     const bool valid = slot >= 0 && slot < a.max_batch;
     const int keys = a.S == 1 && valid ? plan_keys(a, b, 0) : 0;
-    const int id = valid && a.ids ? max(a.ids[slot], 0) : 0, length = valid && a.ids ? max(a.lens[slot], 0) : 0;
+    int id = 0, length = 0;
+    if (valid && (!kTree || a.ids)) {
+      id = a.ids[slot], length = a.lens[slot];
+      id = max(id, 0), length = max(length, 0);
+    }
     s_id[b] = length >= kUnit ? id : 0;
     s_len[b] = length;
     s_keys[b] = keys;
@@ -376,13 +394,13 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   // rows of a tile of own keys: with wide_own as many in each, in blocks of 16, so that the workgroups that run together end together
   const auto own_rows = [&](int tokens) {
     const int rows = tokens * a.group, n = (rows + kTileRows - 1) / kTileRows;
-    return a.wide_own && n > 1 ? ((rows + n - 1) / n + 15) & ~15 : kTileRows;
+    return wide_own && n > 1 ? ((rows + n - 1) / n + 15) & ~15 : kTileRows;
   };
   const auto tiles_of = [&](int tokens) { return (tokens * a.group + kTileRows - 1) / kTileRows; };
   // sums over the sequences before, consecutive ones a thread
   const int per = (a.B + n_thr - 1) / n_thr, b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
   int x[7] = {0, 0, 0, 0, 0, 0, 0}, before[7], total[7];
-  const auto own_wide = [&](int b) { return a.wide_own && s_keys[b] > s_shared[b] && tiles_of(s_tok[b]) > 1; };
+  const auto own_wide = [&](int b) { return wide_own && s_keys[b] > s_shared[b] && tiles_of(s_tok[b]) > 1; };
   const auto add = [&](int b) {
     const int c = s_count[b], own = s_keys[b] - s_shared[b];
     if (c > 0) {
@@ -390,7 +408,7 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
       x[1] += c;
       x[4] += tiles_of(c) * (lead_for(c) + units_of(s_shared[b]));
       x[5] += tiles_of(c) > 1;
-      x[6] += tiles_of(c) > 1 ? tiles_of(c) * (lead_for(c) + units_of(s_shared[b])) : 0;
+      if (kTree) x[6] += tiles_of(c) > 1 ? tiles_of(c) * (lead_for(c) + units_of(s_shared[b])) : 0;
     }
     if (own > 0) {
       x[2] += tiles_of(s_tok[b]);
@@ -401,16 +419,18 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
       }
     }
     if (s_shared[b] == 0) x[3] += s_tok[b];
+    if (!kTree) x[6] += s_tok[b];
   };
   for (int b = b0; b < b1; ++b) add(b);
   block_sums(x, before, total, s_sum);
-  const int p_tiles = total[0], n_tiles = p_tiles + total[2], shared_tokens = total[1], n_multi = total[5], all_units = total[4], wide_units = total[6];
+  const int p_tiles = total[0], n_tiles = p_tiles + total[2], shared_tokens = total[1], n_multi = total[5], all_units = total[4];
 #pragma unroll
   for (int i = 0; i < 7; ++i) x[i] = before[i];
   for (int b = b0; b < b1; ++b) {
     s_ptile[b] = x[0];
     s_base[b] = s_shared[b] > 0 ? x[1] : shared_tokens + x[3];  // of a group: right at its leader
     s_stile[b] = x[2];
+    if (!kTree) s_len[b] = x[6];  // tokens of the sequences before; the prefix lengths are no longer needed
     const auto enter = [&](int m, int of, int tokens, int keys) {
       s_at[m] = of;
       s_n[m] = tiles_of(tokens);
@@ -435,7 +455,27 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   // lie on one axis, every cut of it is a workgroup for each of the tiles, and these run at the same time and find what the first of
   // them loads in their XCD's L2.  (With its tiles one behind the other all of them read the keys from beyond L2.)  That takes a few
   // more workgroups, so `len` is the shortest of 64 lengths, a lane each, for which there are enough.
-  if (n_multi > 0) {  // an entry looks at all others, four at a time, some threads an entry
+  if constexpr (!kTree) {
+    for (int m = tid; m < n_multi; m += n_thr) {
+      const int n = s_n[m];
+      int pos = 0, all = 0, next = -1, first = 1;
+      for (int i = 0; i < n_multi; ++i) {
+        if (s_n[i] != n) continue;
+        const int u = s_u[i];
+        all += u;
+        if (i < m) {
+          pos += u;
+          first = 0;
+        } else if (i > m && next < 0) {
+          next = i;
+        }
+      }
+      s_pos[m] = pos;
+      s_end[m] = first ? all : 0;
+      s_next[m] = next;
+    }
+    __syncthreads();
+  } else if (n_multi > 0) {  // an entry looks at all others, four at a time, some threads an entry
     for (int m = tid; m < n_multi; m += n_thr) {
       s_pos[m] = s_end[m] = 0;
       s_next[m] = s_first[m] = INT32_MAX;
@@ -466,7 +506,7 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
     }
     __syncthreads();
     for (int m = tid; m < n_multi; m += n_thr) {
-      if (a.tree) s_cut_len[m] = s_end[m];
+      s_cut_len[m] = s_end[m];
       if (s_first[m] != m) s_end[m] = 0;
       if (s_next[m] == INT32_MAX) s_next[m] = -1;
     }
@@ -479,15 +519,23 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   };
   if (wave == 0 && n_multi > 0) {
     const int len = length_at(lane);
-    int need = 0;
-    for (int m0 = 0; m0 < n_multi; m0 += 64) {
-      const int end = m0 + lane < n_multi ? s_end[m0 + lane] : 0, n = m0 + lane < n_multi ? s_n[m0 + lane] : 0;
-      for (unsigned long long kinds = __ballot(end > 0); kinds; kinds &= kinds - 1) {
-        const int m = __builtin_ctzll(kinds);
-        need += __builtin_amdgcn_readlane(n, m) * cuts(__builtin_amdgcn_readlane(end, m), len);
+    int need = 0, rest = all_units;
+    if constexpr (kTree) {
+      rest -= total[6];
+      for (int m0 = 0; m0 < n_multi; m0 += 64) {
+        const int end = m0 + lane < n_multi ? s_end[m0 + lane] : 0, n = m0 + lane < n_multi ? s_n[m0 + lane] : 0;
+        for (unsigned long long kinds = __ballot(end > 0); kinds; kinds &= kinds - 1) {
+          const int m = __builtin_ctzll(kinds);
+          need += __builtin_amdgcn_readlane(n, m) * cuts(__builtin_amdgcn_readlane(end, m), len);
+        }
+      }
+    } else {
+      for (int m = 0; m < n_multi; ++m) {
+        need += s_n[m] * cuts(s_end[m], len);
+        rest -= s_n[m] * s_u[m];
       }
     }
-    const unsigned long long enough = __ballot(need + cuts(all_units - wide_units, len) <= a.n_wg);
+    const unsigned long long enough = __ballot(need + cuts(rest, len) <= a.n_wg);
     if (enough != 0 && lane == 0) s_pick[0] = __builtin_ctzll(enough);
   }
   __syncthreads();
@@ -497,61 +545,72 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   // An axis is cut into as many shares as that length makes of it.  Of trees they are equal ones, and the common axis, which is cut
   // after the others, has all workgroups that are left (37 sequences on 4 pictures, 56 rows each, 1430 units a head: shares of 3 to 20 units
   // were 33 us a layer).
-  if (a.tree && apart) {
+  if (kTree && apart) {
     for (int m = tid; m < n_multi; m += n_thr) s_cut_len[m] = (s_cut_len[m] - 1) / cuts(s_cut_len[m], len) + 1;
     __syncthreads();
   }
-  const auto len_of = [&](int m) { return a.tree ? s_cut_len[m] : len; };
+  const auto len_of = [&](int m) { return kTree ? s_cut_len[m] : len; };
   const auto pieces_at = [&](int m) {  // of a tile: from the cut of its first key to that of its last
     const int len = len_of(m);
     return (s_pos[m] + s_u[m] - 1) / len - (s_pos[m] + s_lu[m]) / len + 1;
   };
   int wg0 = 0, wide_parts = 0;  // workgroups and pieces of these
-  if (apart) {
-    const int per_m = (n_multi + n_thr - 1) / n_thr, m0 = min(n_multi, tid * per_m), m1 = min(n_multi, m0 + per_m);
-    int z[2] = {0, 0}, z_before[2], z_total[2];
-    for (int m = m0; m < m1; ++m) z[0] += s_n[m] * cuts(s_end[m], len_of(m)), z[1] += s_n[m] * pieces_at(m);
-    block_sums(z, z_before, z_total, s_sum);
-    for (int m = m0; m < m1; ++m) {
-      s_part[m] = z_before[1];
-      z_before[1] += s_n[m] * pieces_at(m);
-      s_wgs[m] = z_before[0];
-      z_before[0] += s_n[m] * cuts(s_end[m], len_of(m));
+  if constexpr (kTree) {
+    if (apart) {
+      const int per_m = (n_multi + n_thr - 1) / n_thr, m0 = min(n_multi, tid * per_m), m1 = min(n_multi, m0 + per_m);
+      int z[2] = {0, 0}, z_before[2], z_total[2];
+      for (int m = m0; m < m1; ++m) z[0] += s_n[m] * cuts(s_end[m], len_of(m)), z[1] += s_n[m] * pieces_at(m);
+      block_sums(z, z_before, z_total, s_sum);
+      for (int m = m0; m < m1; ++m) {
+        s_wgs[m] = z_before[0];
+        s_part[m] = z_before[1];
+        z_before[0] += s_n[m] * cuts(s_end[m], len_of(m));
+        z_before[1] += s_n[m] * pieces_at(m);
+      }
+      wg0 = z_total[0], wide_parts = z_total[1];
+      __syncthreads();
+      for (int m = wave; m < n_multi; m += n_waves) {  // the workgroups that begin with this entry
+        const int len = len_of(m), n = s_n[m], begin = (s_pos[m] + len - 1) / len, end = (s_pos[m] + s_u[m] - 1) / len + 1;
+        for (int i = begin * n + lane; i < end * n; i += 64) s_begins[s_wgs[s_first[m]] + i] = m;
+      }
     }
-    wg0 = z_total[0], wide_parts = z_total[1];
-    __syncthreads();
-    for (int m = wave; m < n_multi; m += n_waves) {  // the workgroups that begin with this entry
-      const int len = len_of(m), n = s_n[m], begin = (s_pos[m] + len - 1) / len, end = (s_pos[m] + s_u[m] - 1) / len + 1;
-      for (int i = begin * n + lane; i < end * n; i += 64) s_begins[s_wgs[s_first[m]] + i] = m;
+  } else if (apart) {
+    for (int m = 0; m < n_multi; ++m) {
+      if (tid == 0) s_part[m] = wide_parts;
+      wg0 += s_n[m] * cuts(s_end[m], len);
+      wide_parts += s_n[m] * pieces_at(m);
     }
   }
   const auto stands_apart = [&](int b) { return apart && tiles_of(s_count[b]) > 1; };
   const auto own_apart = [&](int b) { return apart && own_wide(b); };
   int* const s_rest = s_id;  // (the ids are no longer needed)
-  int y[4] = {0, 0, 0, 0}, y_before[4], y_total[4];
+  constexpr int kSums = kTree ? 4 : 2;
+  int y[kSums] = {}, y_before[kSums], y_total[kSums];
   const auto add_cut = [&](int b) {
     const int c = s_count[b], own = s_keys[b] - s_shared[b];
     if (c > 0 && !stands_apart(b)) {
       y[0] += tiles_of(c) * (lead_for(c) + units_of(s_shared[b]));
-      y[2] += c;
+      if constexpr (kTree) y[2] += c;
     }
     if (own > 0 && !own_apart(b)) {
       y[1] += tiles_of(s_tok[b]) * (lead_for(s_tok[b]) + units_of(own));
-      y[3] += s_tok[b];
+      if constexpr (kTree) y[3] += s_tok[b];
     }
   };
   for (int b = b0; b < b1; ++b) add_cut(b);
   block_sums(y, y_before, y_total, s_sum);
-  const int prefix_units = y_total[0], units = prefix_units + y_total[1], rest_tokens = y_total[2];
-  const int rest_len = a.tree && units > 0 && a.n_wg > wg0 ? max(kMinUnits, (units - 1) / (a.n_wg - wg0) + 1) : len;
+  const int prefix_units = y_total[0], units = prefix_units + y_total[1], rest_tokens = kTree ? y_total[kSums - 2] : shared_tokens;
+  const int rest_len = kTree && units > 0 && a.n_wg > wg0 ? max(kMinUnits, (units - 1) / (a.n_wg - wg0) + 1) : len;
   const int n_wg = wg0 + cuts(units, rest_len);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) y[i] = y_before[i];
+  for (int i = 0; i < kSums; ++i) y[i] = y_before[i];
   for (int b = b0; b < b1; ++b) {
     s_unit[b] = y[0];
     s_own[b] = y[1];
-    s_rest[b] = y[2];  // tokens, on this axis, of the groups before
-    s_len[b] = y[3];   // and of the sequences before; the prefix lengths are no longer needed
+    if constexpr (kTree) {
+      s_rest[b] = y[2];  // tokens, on this axis, of the groups before
+      s_len[b] = y[3];   // and of the sequences before; the prefix lengths are no longer needed
+    }
     add_cut(b);
   }
   __syncthreads();
@@ -587,8 +646,9 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
   // 64 for every cut up to a tile's first key.
   const int rest_part = kTileRows * wide_parts;
   // first tile of an entry of the wide ones, and of what begins at a place of the common axis
-  const auto entry_tile = [&](int m) { return s_at[m] >= kOwnEntry ? p_tiles + s_stile[s_at[m] - kOwnEntry] : s_ptile[s_at[m]]; };
+  const auto entry_tile = [&](int m) { return kTree && s_at[m] >= kOwnEntry ? p_tiles + s_stile[s_at[m] - kOwnEntry] : s_ptile[s_at[m]]; };
   const auto tile_behind = [&](int end) {
+    if (!kTree && end >= prefix_units) return p_tiles;
     return end >= units ? n_tiles : end < prefix_units ? s_ptile[last_at_or_below(s_unit, a.B, end)]
                                                        : p_tiles + s_stile[last_at_or_below(s_own, a.B, end - prefix_units)];
   };
@@ -616,7 +676,7 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
       }
       from = s_unit[b] + k * (t.lead + n_units);
       t.next = k + 1 < n ? i + 1 : tile_behind(from + t.lead + n_units);
-      rows_before = s_rest[b] * a.group + t.row0;
+      rows_before = (kTree ? s_rest[b] : s_base[b]) * a.group + t.row0;
     } else {
       const int b = last_at_or_below(s_stile, a.B, i - p_tiles), k = i - p_tiles - s_stile[b];
       n_units = units_of(s_keys[b] - s_shared[b]);
@@ -638,7 +698,7 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
         return t;
       }
       from = prefix_units + s_own[b] + k * (t.lead + n_units);
-      t.next = !a.wide_own || k + 1 < tiles_of(s_tok[b]) ? i + 1 : tile_behind(from + t.lead + n_units);
+      t.next = !wide_own || k + 1 < tiles_of(s_tok[b]) ? i + 1 : tile_behind(from + t.lead + n_units);
       rows_before = (rest_tokens + s_len[b]) * a.group + t.row0;
     }
     const int first = (from + t.lead) / rest_len;
@@ -655,10 +715,20 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
     if (is_share) {
       int start, from, len = rest_len;  // of the first tile's first key and of this workgroup, on their axis
       if (i < wg0) {
-        const int m = s_begins[i], first = s_first[m], n = s_n[m], rest = i - s_wgs[first];  // workgroups of the kind before this one
-        const int all = s_end[first];
+        int m = kTree ? s_begins[i] : 0, first = kTree ? s_first[m] : 0, rest = kTree ? i - s_wgs[first] : i;  // rest: workgroups of the kind before this one
+        if constexpr (!kTree) {
+          for (;; ++first) {
+            const int here = s_n[first] * cuts(s_end[first], len);
+            if (rest < here) break;
+            rest -= here;
+          }
+          m = first;
+        }
+        const int n = s_n[m], all = s_end[first];
         len = len_of(m);
         from = rest / n * len;
+        if constexpr (!kTree)
+          while (s_pos[m] + s_u[m] <= from) m = s_next[m];
         index = entry_tile(m) + rest % n;
         offset = from - s_pos[m];
         units_to_do = min(len, all - from);
@@ -1689,16 +1759,18 @@ int make_plan(const char* what, bool tree, const int64_t* batch_idx, const void*
   const Layout l = layout_of(B, S, Hq, Hc);
   const PlanArgs a{batch_idx, input_pos, pos_index_type, prefix_ids, prefix_lens, B, S, Hq, Hc, Hq / Hc, max_batch, max_context,
                    l.n_wg, static_cast<char*>(plan), l.seqs, l.tokens, l.place, l.shares, l.tiles,
-                   tree, tree && S * (Hq / Hc) > kTileRows && B <= kWideOwn};
+                   tree && S * (Hq / Hc) > kTileRows && B <= kWideOwn};
   // as many as there are shares, tiles and sequences to write: 64 sequences 2 us less with 512 than with 256, a few no more
   const int threads = S > 1 || B > 64 ? 1024 : B > 24 ? 512 : 256;
-  const size_t lds = ((kPlanArrays + (a.wide_own ? kWideArrays + 3 : tree ? 1 : 0)) * static_cast<size_t>((B + 3) & ~3) + ((l.n_wg + 3) & ~3)) * sizeof(int);
+  const size_t lds = ((kPlanArrays + (tree ? kTreeArrays : 0) + (a.wide_own ? kWideArrays : 0)) * static_cast<size_t>((B + 3) & ~3) +
+                      (tree ? (l.n_wg + 3) & ~3 : 0)) * sizeof(int);
+  const auto kernel = tree ? shared_plan_kernel<true> : shared_plan_kernel<false>;
   if (lds > 64 * 1024) {
-    const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(shared_plan_kernel),
+    const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                    hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
     if (allowed != hipSuccess) return fp::fail(FP_ERR_LAUNCH, "%s: %s", what, hipGetErrorString(allowed));
   }
-  hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3(threads), lds, static_cast<hipStream_t>(stream), a);
+  hipLaunchKernelGGL(kernel, dim3(1), dim3(threads), lds, static_cast<hipStream_t>(stream), a);
   return fp::check_launch(what);
 }
 

@@ -695,14 +695,15 @@ int fp_paged_decode_tree(const int64_t* masks, const void* q, int64_t q_stride_b
  * stands if u_c * r < p(token_c), where r is 1 less the p of the children refused before it (of one token once); with draft_probs if
  * u_c * q(token_c) < p(token_c).  Below the last that stands a token is drawn: the lowest i at which the sum of
  * the weights up to it exceeds u_0 times the sum of all.  The weights are p without the refused tokens, or max(0, p - q) (p where that is
- * 0 everywhere, or where no child was refused).  A draft outside 0 .. V - 1 never stands.  Sums and probabilities are in 64 bits: the
- * result does not depend on how the work is cut.
+ * 0 everywhere, or where no child was refused).  A draft outside 0 .. V - 1 never stands.  Sums and probabilities that decide are
+ * in 64 bits: which tokens they are does not depend on how the work is cut.
  *
  *   accepted   [B] int32: drafts that stand
  *   path       [B, S] int32: row 0 and the rows of those that stand, -1 behind them (what fp_keep_rows takes)
  *   answer     [B, S] int64: the tokens that stand, then the drawn one, -1 behind them; -1 in its place too where the row has no logit
  *              above -inf, or every token that has one was refused
- *   logprobs   [B, S] float32: log p of every answered token where it stands (greedy: at temperature 1), 0 where there is none
+ *   logprobs   [B, S] float32: log p of every answered token where it stands (greedy: at temperature 1), 0 where there is none; p's sum to 2^-18 of
+ *              itself, by weights in 32 bits
  * A sequence without a step: accepted 0, path and answer -1, logprobs 0.
  * Workspace: memory of the caller, 16-byte aligned, one call at a time; nothing in it needs clearing.
  * S <= 64, V <= 2^24.
