@@ -230,6 +230,20 @@ def test_the_most_sequences_of_several_tiles(B):
     case.check(case.call(ops))
 
 
+@pytest.mark.parametrize("dtype,Hq", [(BF16, 4), (F32, 2), (F16, 16)])
+def test_drafts_in_front_of_the_end_of_a_prefix(dtype, Hq):
+    """Sequences that were set back: their tokens are at positions of the prefix that others read as theirs."""
+    gen = torch.Generator().manual_seed(13)
+    trees = [random_tree(gen, n, r) for n, r in ((9, 3), (17, 4), (40, 5), (64, 2), (1, 1), (30, 9))]
+    case = DraftBatch(39, [192, 130], [(0, 20, trees[0]), (0, 64, trees[1]), (0, 0, trees[2]), (0, 7, trees[3]), (1, 0, trees[4]), (1, 65, trees[5])],
+                      Hq=Hq, Hc=2, D=64, P=32, dtype=dtype, S=64)
+    case.cached[1], case.cached[2], case.cached[3], case.cached[5] = 100, 64, 130, 0
+    case.masks, case.pos, case.rope = tree_tensors(case.trees, case.S, case.cached.tolist())
+    case.on()
+    case.check(case.call(ops))
+    case.check(case.call(ops, share=False))
+
+
 def test_the_most_sequences():
     """Of one cached head: the plan's arrays fill the shared memory of a workgroup."""
     gen = torch.Generator().manual_seed(12)
