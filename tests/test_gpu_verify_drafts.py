@@ -280,6 +280,20 @@ def test_large_vocabularies(V):
     Step(19, 3, 3, V, F32, probs=F32).check()
 
 
+@pytest.mark.parametrize("dtype,probs", [(F32, F32), (BF16, F16), (F16, None)])
+def test_vocabularies_of_more_pieces_than_are_held(dtype, probs):
+    step = Step(22, 4, 3, 1100003, dtype, probs=probs, reach=1 if probs else 3)
+    step.uniforms[:, 0] = torch.tensor([0.01, 0.4, 0.95, 0.9999])
+    step.check()
+    step.uniforms[:, 1:] = 0.99999  # hardly any draft stands
+    step.check()
+
+
+def test_the_largest_vocabulary():
+    step = Step(23, 1, 1, 1 << 24, F32)
+    step.check()
+
+
 def test_many_requests():
     step = Step(20, 1300, 3, 513, F32, counts=[3, 2, 0, 1])
     step.check()
