@@ -19,11 +19,11 @@
 //    if p and q have nothing to do with each other) is weighed again by the last workgroup.
 // The first launch sets the counters of the second to 0: nothing is kept between calls.
 //
-// Rows is bound by the logits' bytes: 64 requests of 3 to 8 rows of 65536 in 32 bits, 92 MB, 19.9 us (4.6 TB/s), 32 of 17 to 33 in 16 bits, 104 MB,
-// 24.4 us (4.3 TB/s: an exponential for every two bytes).  With all weights in 64 bits the two were 60.7 and 50.4 us.  Walk is a line of trips and of
-// f64 instructions: of the first 25.0 us, 2.7 until a request's rows are put together, 1.6 the walk, 8.5 the 25 MB of the rows that are drawn from and
+// Rows is bound by the logits' bytes: 64 requests of 3 to 8 rows of 65536 in 32 bits, 92 MB, 19.2 us (4.8 TB/s), 32 of 17 to 33 in 16 bits, 104 MB,
+// 22.6 us (4.6 TB/s: an exponential for every two bytes).  With all weights in 64 bits the two were 60.7 and 50.4 us.  Walk is a line of trips and of
+// f64 instructions: of the first 25.2 us, 2.7 until a request's rows are put together, 1.6 the walk, 8.5 the 25 MB of the rows that are drawn from and
 // of their drafts' probabilities (35 instructions a token, 14 of them f64 products), 2 until the last workgroup has the sums, 2 for the pieces of which it
-// was not sure, and the draw; of the second 16.4.  One request of 5 rows: 3.9 and 12.0 us.
+// was not sure, and the draw; of the second 16.3.  One request of 5 rows: 3.8 and 11.9 us.
 #include "fp_common.h"
 
 #include <math.h>
@@ -33,9 +33,9 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kMaxTokens = 64;
-// What a row's sum may be off by, relatively.  A weight 2^-p in 32 bits is off by 2.5 p 2^-24 ln 2 (the difference, the product and the
-// rate rounded) and 2^-23 (the exponential), sums of 8 by 3 * 2^-24.  Weights of 2^-p are V 2^-p of a whole of 1 or more, so p counts up to
-// log2 V, 24: 2.9e-6 in all.
+// What a row's sum may be off by, relatively.  A weight 2^-p in 32 bits is off by 2 p 2^-24 ln 2 (the exponent and the rate
+// rounded) and 2^-23 (the exponential), sums of 8 by 3 * 2^-24.  Weights of 2^-p are V 2^-p of a whole of 1 or more, so p counts up to
+// log2 V, 24: 2.3e-6 in all.
 constexpr float kBand = 0x1p-18f;
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
@@ -94,7 +94,7 @@ struct VerifyArgs {
   int draws, pieces;          // workgroups of a request, and pieces of 64 vectors
 };
 
-// 2^t for t <= 0 (0 for NaN): t = n + f, 2^f by its Chebyshev interpolation of degree 10 on [-1/2, 1/2], off by 2^-51.
+// 2^t for t below 1000 (0 for NaN): t = n + f, 2^f by its Chebyshev interpolation of degree 10 on [-1/2, 1/2], off by 2^-51.
 __device__ __forceinline__ double power2(double t) {
   t = fmax(t, -1100.0);
   const double n = rint(t), f = t - n;
@@ -198,8 +198,12 @@ __device__ __forceinline__ void each(const Row<E>& r, int v, const v4u& x, F f) 
 
 // ---------------------------------------------------------------------------------------------------------------- rows
 // A thread has G vectors at a time, the next ones on their way meanwhile, and weighs by a logit of its own that moves only when a larger one
-// is more than 2^kSlack heavier: no exchange between threads before the end of the chunk.
+// is more than 2^kSlack heavier: no exchange between threads before the end of the chunk.  An exponent is x rate - shift in one
+// instruction, rate and shift in 32 bits: the weights are next to 2^reference, which has in 64 bits what the two were rounded by.  An
+// infinity that is not below, or NaN, makes a thread's sum NaN, and it weighs once more.  (32 requests of 17 to 33 rows of 65536 in 16 bits: 22.6 us,
+// 24.4 with a difference, a product and a bound for NaN.)
 constexpr double kSlack = 20.0;
+constexpr double kFar = 0x1p22;  // a shift up to this is rounded by 1/4 at most
 
 template <typename E, int G>
 __global__ __launch_bounds__(kThreads) void verify_rows_kernel(const VerifyArgs a) {
@@ -220,9 +224,9 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(const VerifyArgs 
   const double rate = kLog2e / (greedy ? 1.0 : heat);
   const float rate32 = static_cast<float>(rate), slack = static_cast<float>(kSlack / rate);
 
-  float peak = -INFINITY, by = -INFINITY;  // by: what the thread weighs by
+  float peak = -INFINITY, by = -INFINITY, shift = 0.f;  // by: what the thread weighs by
   int best = INT32_MAX;
-  double sum = 0.0;
+  double sum = 0.0, reference = 0.0;
   const auto load = [&](v4u (&x)[G], int v) {
 #pragma unroll
     for (int k = 0; k < G; ++k) {
@@ -232,7 +236,10 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(const VerifyArgs 
   };
   const auto grow = [&](float top) {  // of the elements to come
     if (top > by + slack) {
-      sum *= weight(by, top, rate);
+      shift = top * rate32;
+      const double next = static_cast<double>(shift) + static_cast<double>(top) * (rate - static_cast<double>(rate32));
+      sum = by == -INFINITY ? 0.0 : sum * power2(reference - next);  // (nothing weighs anything before: NaN alone)
+      reference = next;
       by = top;
     }
   };
@@ -256,13 +263,12 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(const VerifyArgs 
     }
     peak = fmaxf(peak, top);
     grow(top);
-    const float zero = by == -INFINITY ? 0.f : by;
 #pragma unroll
     for (int k = 0; k < G; ++k)
       if (k == 0 || v + k * kThreads < v_end) {
         float w[E::kVec];
 #pragma unroll
-        for (int i = 0; i < E::kVec; ++i) w[i] = __builtin_amdgcn_exp2f(fmaxf((E::get(x[k], i) - zero) * rate32, -200.f));  // (-inf, NaN: 0)
+        for (int i = 0; i < E::kVec; ++i) w[i] = __builtin_amdgcn_exp2f(fmaf(E::get(x[k], i), rate32, -shift));  // (-inf: 0)
 #pragma unroll
         for (int d = 1; d < E::kVec; d *= 2)
 #pragma unroll
@@ -281,16 +287,16 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(const VerifyArgs 
     if (y > peak || (y == peak && loose < best)) best = loose;
     peak = fmaxf(peak, y);
     grow(y);
-    sum += y > by ? 1.0 / weight(by, y, rate) : weight(y, by, rate);
+    sum += power2(static_cast<double>(y) * rate - reference);
   }
   float all = reduce_lanes(peak, 64, [](float p, float q) { return fmaxf(p, q); });
   if (lane == 0) s_peak[wave] = all;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) all = fmaxf(all, s_peak[w]);
-  if (fabsf(all) < INFINITY && rate > 0x1p-40 && rate < 0x1p40) {
-    sum *= weight(by, all, rate);
-  } else {  // infinite logits, temperatures out of all measure: once more, in 64 bits
+  if (fabs(all * rate) < kFar && rate > 0x1p-40 && rate < 0x1p40 && fabs(sum) < INFINITY) {
+    sum = by == -INFINITY ? 0.0 : sum * power2(reference - static_cast<double>(all) * rate);
+  } else {  // infinite and far logits, NaN, temperatures out of all measure: once more, in 64 bits
     sum = loose >= 0 ? weight(r.one(loose), all, rate) : 0.0;
     for (int u = c * a.chunk_vectors + tid; u < v_end; u += kThreads) {
 #pragma nounroll

@@ -294,6 +294,24 @@ def test_the_largest_vocabulary():
     step.check()
 
 
+@pytest.mark.parametrize("probs", [F32, None])
+@pytest.mark.parametrize("heat", [1.0, 0.7, 30.0])
+def test_far_logits(heat, probs):
+    """Rows far from 0, rows that rise and fall by more than an exponential holds, NaN in front."""
+    V = 9001
+    step = Step(24, 9, 3, V, F32, probs=probs)
+    x = step.logits
+    for b, far in enumerate((-1e4, 1e4, -1e6, 1e6, 1e30)):
+        x[b] += far
+    ramp = torch.arange(V, dtype=torch.float32)
+    x[5] += ramp
+    x[6] -= 0.5 * ramp
+    x[7] += 40.0 * (ramp % 2048 // 8)
+    x[8, :, :6000] = float("nan")
+    step.temperatures = torch.full((9,), heat)
+    step.check()
+
+
 def test_many_requests():
     step = Step(20, 1300, 3, 513, F32, counts=[3, 2, 0, 1])
     step.check()
