@@ -393,7 +393,9 @@ __device__ __forceinline__ int2 piece_range(const Row<E>& r, int V, int k) {
 }
 
 // The first token at which the weights of the row pass u times their total: sum_of(k) the sum of piece k of n, weigh(x, i, load(i)) the weight
-// of token i.  What it is goes to answer(token, x), by one thread; -1 if nothing weighs anything.
+// of token i.  What it is goes to answer(token, x), by one thread; -1 if nothing weighs anything.  Only a piece that weighs something is chosen:
+// behind the last of them the sums up to a lane, which every lane adds up in another order, still differ in their last bits, and a goal of the whole
+// total (u = 1) lies among them.
 template <typename E, typename S, typename L, typename W, typename A>
 __device__ __forceinline__ void draw(const Row<E>& r, int V, double total, S sum_of, int n, float u, DrawShared& sh, L load, W weigh, A answer) {
   constexpr int kEach = elements_each<E>();
@@ -405,7 +407,7 @@ __device__ __forceinline__ void draw(const Row<E>& r, int V, double total, S sum
 #pragma nounroll
   for (int k0 = 0; k0 < n && part < 0; k0 += 64) {
     const double s = k0 + lane < n ? sum_of(k0 + lane) : 0.0, upto = scan_lanes(s);
-    const uint64_t past = __ballot(before + upto > goal), some = __ballot(s > 0.0);
+    const uint64_t some = __ballot(s > 0.0), past = some & __ballot(before + upto > goal);
     if (past) {
       const int l = __builtin_ctzll(past);
       part = k0 + l;
@@ -470,7 +472,11 @@ __device__ __forceinline__ void draw(const Row<E>& r, int V, double total, S sum
     if (found >= 0) atomicMax(&sh.place, found);
     __syncthreads();
   }
-  if (found >= 0 && found == sh.place) answer(found, its);
+  if (sh.place < 0) {  // not a token of the piece
+    if (tid == 0) answer(-1, 0.f);
+    return;
+  }
+  if (found == sh.place) answer(found, its);
 }
 
 // Element i0 .. of a row of the draft's probabilities; `aligned`: kVec of them at once

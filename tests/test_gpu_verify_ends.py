@@ -1,0 +1,53 @@
+"""Verification of drafted tokens where a draw has nothing left to pass."""
+
+import pytest
+import torch
+
+from falcon_perception_amd import _native as N
+from falcon_perception_amd import ops
+from tests.test_gpu_verify_drafts import BF16, F32, Step
+
+pytestmark = pytest.mark.gpu
+
+
+def call_into(step, fill, answer=-77):
+    """`verify_drafts` by the C entry point: every result and the workspace hold something before the call."""
+    B, S, V = step.logits.shape
+    dev = lambda t: t.cuda().contiguous()
+    logits, tokens, parents, u = dev(step.logits), dev(step.tokens), dev(step.parents), dev(step.uniforms)
+    probs = None if step.probs is None else dev(step.probs)
+    heat = None if step.temperatures is None else dev(step.temperatures)
+    made = ops.VerifiedDrafts(torch.full((B,), answer, dtype=torch.int32, device="cuda"), torch.full((B, S), answer, dtype=torch.int32, device="cuda"),
+                              torch.full((B, S), answer, dtype=torch.int64, device="cuda"), torch.full((B, S), float(answer), device="cuda"))
+    ws = torch.full((ops.verify_workspace_bytes(B, S, V),), fill, dtype=torch.uint8, device="cuda")
+    rc = N.lib().fp_verify_drafts(
+        logits.data_ptr(), logits.stride(0), logits.stride(1), N.dtype_code(logits.dtype), tokens.data_ptr(), parents.data_ptr(), u.data_ptr(),
+        None if heat is None else heat.data_ptr(), None if probs is None else probs.data_ptr(), *((0, 0) if probs is None else probs.stride()[:2]),
+        0 if probs is None else N.dtype_code(probs.dtype), *(t.data_ptr() for t in made), ws.data_ptr(), ws.numel(), B, S, V, N.stream_ptr(logits.device))
+    N.check(rc, "fp_verify_drafts")
+    torch.cuda.synchronize()
+    return made, ws
+
+
+@pytest.mark.parametrize("u", [1.0, 3.0, float("nan")])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("probs", [False, True])
+def test_numbers_past_the_last_token(probs, dtype, u):
+    """From 1 on the last token that weighs something answers, whatever the sums round to: unequal weights, and pieces behind them that
+    weigh nothing."""
+    B, V, some = 256, 32768, 24000
+    step = Step(41, B, 2, V, dtype, probs=F32 if probs else None, spread=1.0)
+    step.logits[:, :, some:] = -float("inf")
+    step.logits[:, :, some - 1] = step.logits[:, :, :some].float().amax(2)
+    step.parents[:] = torch.tensor([-1, 0])
+    step.uniforms[:, 0] = u
+    step.uniforms[:, 1] = 1e9  # the draft is refused
+    step.tokens[:, 1] = 7
+    if probs:
+        step.probs[:, :, some - 1] = 0.0
+    got, _ = call_into(step, 255)
+    assert (got.accepted == 0).all()
+    assert (got.tokens[:, 0] == some - 1).all()
+    x = step.logits[:, 0, :].double()
+    want = x[:, some - 1] - torch.logsumexp(x, 1)
+    assert (got.logprobs[:, 0].cpu().double() - want).abs().max() <= 1e-5
