@@ -604,13 +604,13 @@ __global__ __launch_bounds__(kThreads) void verify_walk_kernel(const VerifyArgs 
             const double side = lane_of(static_cast<double>(u) * q, i) * z, w_i = lane_of(w, i);
             if (w_i > 0.0 && fabs(side - w_i) <= (doubt < 0.0 ? -1.0 : kBand * side)) again = node;
             stands = again < 0 && w_i > 0.0 && side < w_i;
-            if (!stands) break;  // of drafts that were drawn the first child only
           } else if (token_i >= 0 && __ballot(out && name == token_i) == 0) {
             const double side = lane_of(static_cast<double>(u), i) * (z - refused), w_i = lane_of(w, i);
             if (w_i > 0.0 && fabs(side - w_i) <= doubt) again = node;
             stands = again < 0 && w_i > 0.0 && side < w_i;
             refused += w_i;
           }
+          if (a.probs && !stands) break;  // of drafts that were drawn the first child only
           out |= lane == i;
           if (stands) {
             node = i;

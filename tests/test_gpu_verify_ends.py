@@ -1,4 +1,4 @@
-"""Verification of drafted tokens where a draw has nothing left to pass."""
+"""Verification of drafted tokens where a draw has nothing left to pass, and where a greedy request's drafts were drawn."""
 
 import pytest
 import torch
@@ -51,3 +51,18 @@ def test_numbers_past_the_last_token(probs, dtype, u):
     x = step.logits[:, 0, :].double()
     want = x[:, some - 1] - torch.logsumexp(x, 1)
     assert (got.logprobs[:, 0].cpu().double() - want).abs().max() <= 1e-5
+
+
+def test_of_drawn_drafts_the_first_child_alone_decides_for_greedy_requests_too():
+    step = Step(42, 12, 6, 400, F32, probs=F32, reach=6)
+    step.temperatures = torch.zeros(12)
+    step.parents[:] = torch.tensor([-1, 0, 0, 1, 1, 2])
+    best = step.logits.argmax(2)
+    step.tokens[:, 1] = (best[:, 0] + 1) % 400
+    step.tokens[:, 2] = best[:, 0]
+    step.tokens[::2, 1] = best[::2, 0]
+    step.tokens[:, 3] = (best[:, 1] + 1) % 400
+    step.tokens[:, 4] = best[:, 1]
+    got = step.call()
+    assert got.accepted.tolist() == [1, 0] * 6
+    step.check(got)
