@@ -150,8 +150,16 @@ struct Row {
   __device__ int behind() const { return head + vectors * E::kVec; }  // first element behind the whole ones
 };
 
-// Whether row j of the request is a token that can be reached.
-__device__ __forceinline__ bool is_token(int j, int parent) { return j == 0 ? parent == -1 : parent >= 0 && parent < j; }
+// The rows that the walk can reach from row 0, a bit each, for all lanes; lane j holds the parent of row j, -2 if there is none.  A turn for
+// every level of the tree.
+__device__ __forceinline__ uint64_t reachable(int parent, int lane) {
+  uint64_t rows = __ballot(lane == 0 && parent == -1);
+  for (uint64_t more = rows; more;) {
+    more = __ballot(parent >= 0 && parent < lane && (rows >> (parent & 63) & 1)) & ~rows;
+    rows |= more;
+  }
+  return rows;
+}
 
 // Sum over the lanes up to this one, without a trip through LDS (row_shr:1, 2, 4, 8, then row_bcast:15, 31).
 template <int kControl, int kRows>
@@ -214,9 +222,8 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(const VerifyArgs 
   const uint32_t row = blockIdx.x / static_cast<uint32_t>(a.chunks), b = row / static_cast<uint32_t>(a.S);
   const int c = blockIdx.x - row * a.chunks, j = row - b * a.S;
   if (c == 0 && j == 0 && tid == 0) a.arrivals[b] = 0;
-  const int parent = a.parents[row], root = a.parents[static_cast<int64_t>(b) * a.S];
   const float heat = heat_of(a, b);
-  if (!is_token(j, parent) || root != -1) return;
+  if (!(reachable(lane < a.S ? a.parents[static_cast<int64_t>(b) * a.S + lane] : -2, lane) >> j & 1)) return;
   const Row<E> r(a.logits + b * a.ls_b + j * a.ls_s, a.V);
   const int v_end = min((c + 1) * a.chunk_vectors, r.vectors);
   int v = c * a.chunk_vectors + tid;
@@ -523,7 +530,6 @@ __global__ __launch_bounds__(kThreads) void verify_walk_kernel(const VerifyArgs 
   const uint32_t b = blockIdx.x / static_cast<uint32_t>(a.draws);
   const int c = blockIdx.x - b * a.draws, S = a.S;
   const int64_t first = static_cast<int64_t>(b) * S;
-  const bool there = a.parents[first] == -1;
   const float heat = heat_of(a, b), u0 = a.uniforms[first];
   const bool greedy = !(heat > 0.f);
   const double rate = kLog2e / (greedy ? 1.0 : heat), slope = 1.0 / (greedy ? 1.0 : heat);
@@ -533,14 +539,16 @@ __global__ __launch_bounds__(kThreads) void verify_walk_kernel(const VerifyArgs 
   const int64_t token = lane < S ? a.tokens[first + lane] : -1;
   const float u = lane < S ? a.uniforms[first + lane] : 0.f;
 
-  // every row's maximum and sum, `per` lanes a row: the first chunks are on their way before it is known which rows are tokens
+  // every row's maximum and sum, `per` lanes a row: the first chunks are on their way before it is known which rows are reached
   int per = 64;
   while (per > kThreads / S) per >>= 1;
   const int mine = tid / per, row = mine < S ? mine : 0;
   const Part* const parts = a.parts + (first + row) * a.chunks;
   Part t = parts[min(tid % per, a.chunks - 1)];
-  const bool is_row = mine < S && there && is_token(row, a.parents[first + row]);
-  const bool child = there && lane > 0 && lane < S && parent >= 0 && parent < lane, known = token >= 0 && token < a.V;
+  const uint64_t rows = reachable(parent, lane);
+  const bool there = rows & 1;
+  const bool is_row = mine < S && (rows >> row & 1);
+  const bool child = lane > 0 && (rows >> lane & 1), known = token >= 0 && token < a.V;
   const int at = child ? parent : 0, name = known ? static_cast<int>(token) : -1;
   float x = -INFINITY;
   double q = 0.0;

@@ -683,9 +683,9 @@ int fp_paged_decode_tree(const int64_t* masks, const void* q, int64_t q_stride_b
  * Which drafted tokens the target model's distribution lets stand, and the token behind them, from given random numbers.
  *
  *   logits     [B, S, V], element strides (b, s), rows dense: row j is what the target says behind token j.  NaN counts as -inf
- *   tokens     [B, S] contiguous int64; of row 0 not read
- *   parents    [B, S] contiguous int32, as fp_draft_tree; row 0 must be -1, else the sequence has no step.  Logits of rows that are no token
- *              are not read
+ *   tokens     [B, S] contiguous int64; that of row 0 counts for nothing
+ *   parents    [B, S] contiguous int32, as fp_draft_tree; row 0 must be -1, else the sequence has no step.  Rows that do not lead back to row 0
+ *              (no token, behind one that is none, behind another first token) have no part in it: their logits and probabilities are not read
  *   uniforms   [B, S] contiguous float32, each used once, in 0 <= u < 1: u[b, j] for draft j, u[b, 0] for the drawn token
  *   temperatures  NULL (all 1) or [B] float32; not above 0: the largest logit decides, of equal ones the first
  *   draft_probs   NULL, or [B, S, V] of probs_dtype, element strides (b, s): row j is the distribution that the child of token j was

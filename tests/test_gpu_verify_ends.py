@@ -1,11 +1,12 @@
-"""Verification of drafted tokens where a draw has nothing left to pass, and where a greedy request's drafts were drawn."""
+"""Verification of drafted tokens where a draw has nothing left to pass, where a greedy request's drafts were drawn, and where a tree has
+rows that nothing reaches."""
 
 import pytest
 import torch
 
 from falcon_perception_amd import _native as N
 from falcon_perception_amd import ops
-from tests.test_gpu_verify_drafts import BF16, F32, Step
+from tests.test_gpu_verify_drafts import BF16, F16, F32, Step
 
 pytestmark = pytest.mark.gpu
 
@@ -65,4 +66,24 @@ def test_of_drawn_drafts_the_first_child_alone_decides_for_greedy_requests_too()
     step.tokens[:, 4] = best[:, 1]
     got = step.call()
     assert got.accepted.tolist() == [1, 0] * 6
+    step.check(got)
+
+
+@pytest.mark.parametrize("greedy", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_rows_that_nothing_reaches_are_not_read(dtype, greedy):
+    """Rows behind a hole, behind a second first token, and those of a sequence without a step: the workspace is left as it is for rows that name
+    no parent at all."""
+    step = Step(43, 4, 8, 3001, dtype)
+    reached = torch.tensor([[-1, -2, 0, -2, 2, -2, -2, -2], [-1, 0, 1, -2, -2, -2, -2, -2], [-2] * 8, [-1] + [-2] * 7], dtype=torch.int32)
+    others = torch.tensor([[-1, -2, 0, 1, 2, 3, -1, 6], [-1, 0, 1, -1, 3, 9, 5, 6], [-2, 0, 1, 2, 0, 0, -1, 6], [-1, 4, 1, 1, -1, 4, 5, 5]], dtype=torch.int32)
+    step.temperatures = torch.zeros(4) if greedy else None
+    results = []
+    for parents in (reached, others):
+        step.parents[:] = parents
+        results.append(call_into(step, 173))
+    (want, want_ws), (got, got_ws) = results
+    for w, g in zip(want, got):
+        assert torch.equal(w, g)
+    assert torch.equal(want_ws, got_ws)
     step.check(got)
