@@ -14,7 +14,7 @@
 //    most, summed in 64.
 //  * walk: every workgroup puts the chunks of its request's rows together and walks down the tree; a comparison within kBand of its
 //    border is made again with the row's sum in 64 bits (a few in a million).  Then it sums the weights of its pieces of the row that the walk
-//    ends at, and the last workgroup of a request draws.  Where the drafts were drawn, Z is known only then: until then a piece has the
+//    ends at, and the last workgroup of a request draws; the drawn token's logarithm is by that sum.  Where the drafts were drawn, Z is known only then: until then a piece has the
 //    sums of w and of q over the tokens that surely have something left, and one with a token within kBand of its border (every 100 pieces,
 //    if p and q have nothing to do with each other) is weighed again by the last workgroup.
 // The first launch sets the counters of the second to 0: nothing is kept between calls.
@@ -368,6 +368,7 @@ struct DrawShared {
   double all[kHeld], kept[kHeld], taken[kHeld];
   double sum[kWaves], total[kWaves], rest[kWaves];
   int place, flag;
+  double refused;  // weights of the tokens refused at the row that is drawn from
 };
 
 __device__ __forceinline__ double sum_threads(double x, double (&part)[kWaves]) {  // a part once between two barriers
@@ -597,11 +598,12 @@ __global__ __launch_bounds__(kThreads) void verify_walk_kernel(const VerifyArgs 
   for (;;) {
     if (wave == 0) {
       int node = 0, count = 0, path = lane == 0 ? 0 : -1, again = -1;  // path: its lane-th row
+      double refused = 0.0;
       for (bool stands = true; stands;) {
         // the children in turn: what those refused weigh, the same token once
         const double z = s_total[node], doubt = exact >> node & 1 ? -1.0 : kBand * z;
         const int best = s_best[node];
-        double refused = 0.0;
+        refused = 0.0;
         bool out = false;  // this lane's token is refused at this node
         stands = false;
         for (uint64_t left = __ballot(child && parent == node); left && !stands && again < 0; left &= left - 1) {
@@ -637,6 +639,7 @@ __global__ __launch_bounds__(kThreads) void verify_walk_kernel(const VerifyArgs 
         s_n_out = __builtin_popcountll(out);
         s_refused = any;
         s_again = again;
+        sh.refused = refused;
       }
       if (c == 0 && again < 0) {
         // the token of path[lane + 1] answers at place lane; the last place is the drawn one's
@@ -677,10 +680,11 @@ __global__ __launch_bounds__(kThreads) void verify_walk_kernel(const VerifyArgs 
   const int node = s_node, count = s_count;
   const float peak = s_peak[node];
   const double total = s_total[node];
+  double whole = total;  // what the drawn token's logarithm is by: the sum in 64 bits, as soon as that is known
   const Row<E> r(a.logits + b * a.ls_b + node * a.ls_s, a.V);
   const auto answer = [&](int token, float x) {
     a.answer[first + count] = token;
-    a.logprobs[first + count] = token < 0 ? 0.f : log_share(x, peak, slope, total);
+    a.logprobs[first + count] = token < 0 ? 0.f : log_share(x, peak, slope, whole);
   };
   if (greedy || peak == -INFINITY) {
     if (c == 0 && tid == 0) answer(s_best[node], peak);
@@ -730,7 +734,9 @@ __global__ __launch_bounds__(kThreads) void verify_walk_kernel(const VerifyArgs 
     }
 #pragma nounroll
     for (int k = kHeld + tid; k < a.pieces; k += kThreads) total += take(&sums[k].all);
-    draw<E>(r, a.V, sum_threads(total, sh.total), [&](int k) { return k < kHeld ? sh.all[k] : take(&sums[k].all); }, a.pieces, u0, sh,
+    total = sum_threads(total, sh.total);
+    whole = total + sh.refused;
+    draw<E>(r, a.V, total, [&](int k) { return k < kHeld ? sh.all[k] : take(&sums[k].all); }, a.pieces, u0, sh,
             [](int) { return 0.f; }, [&](float y, int i, float) { return is_out(i) ? 0.0 : weights(y); }, answer);
     return;
   }
@@ -788,7 +794,8 @@ __global__ __launch_bounds__(kThreads) void verify_walk_kernel(const VerifyArgs 
   }
 #pragma nounroll
   for (int k = kHeld + tid; k < a.pieces; k += kThreads) sum += take(&sums[k].all);
-  const double whole_total = sum_threads(sum, sh.total), share = 1.0 / whole_total;
+  whole = sum_threads(sum, sh.total);
+  const double share = 1.0 / whole;
   const auto left_of = [&](float y, float q) { return fmax(0.0, weights(y) * share - static_cast<double>(q)); };
   // what is left of every piece, in place of what was kept; those of which it was not sure by the wavefront that found it
   double* const rests = a.rests + static_cast<int64_t>(b) * a.pieces;
@@ -827,10 +834,10 @@ __global__ __launch_bounds__(kThreads) void verify_walk_kernel(const VerifyArgs 
   }
   asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
   const double left = sum_threads(rest, sh.rest);
-  const bool whole = !(left > 0.0);  // nothing is left: the target's own distribution
-  draw<E>(r, a.V, whole ? whole_total : left,
-          [&](int k) { return k < kHeld ? whole ? sh.all[k] : sh.kept[k] : take(whole ? &sums[k].all : rests + k); }, a.pieces, u0, sh,
-          [&](int i) { return probability(a, probs, i); }, [&](float y, int, float q) { return whole ? weights(y) : left_of(y, q); }, answer);
+  const bool own = !(left > 0.0);  // nothing is left: the target's own distribution
+  draw<E>(r, a.V, own ? whole : left,
+          [&](int k) { return k < kHeld ? own ? sh.all[k] : sh.kept[k] : take(own ? &sums[k].all : rests + k); }, a.pieces, u0, sh,
+          [&](int i) { return probability(a, probs, i); }, [&](float y, int, float q) { return own ? weights(y) : left_of(y, q); }, answer);
 }
 
 struct Cut {

@@ -982,8 +982,10 @@ def verify_drafts(logits: Tensor, tokens: Tensor, parents: Tensor, uniforms: Ten
     (S = 1) it is a draw from p.
 
     Returns `accepted` [B] int32, the number of drafts that stand; `path` [B, S] int32, row 0 and theirs, -1 behind (for `keep_rows`);
-    `tokens` [B, S] int64, those that stand and the drawn one, -1 behind; `logprobs` [B, S] float32, the log of p of each
-    (its sum to 2^-18 of itself).  Decisions are taken in 64 bits and do not depend on the batch.  A sequence whose parents[b, 0] is not -1 has no step: 0, -1, -1, 0.
+    `tokens` [B, S] int64, those that stand and the drawn one, -1 behind; `logprobs` [B, S] float32, the log of p of each.
+    Decisions, and the drawn token's logarithm, are of sums in 64 bits and do not depend on the batch.  For drafts that stand and for greedy requests p's
+    sum is of weights in 32 bits: to 2^-18 of itself, and by that much the logarithm may depend on the batch.  A sequence whose parents[b, 0] is not -1 has
+    no step: 0, -1, -1, 0.
 
     `workspace`: `verify_workspace_bytes(B, S, V)` bytes, for one call at a time."""
     index = _current(logits)

@@ -1,5 +1,7 @@
-"""Verification of drafted tokens where a draw has nothing left to pass, where a greedy request's drafts were drawn, and where a tree has
-rows that nothing reaches."""
+"""Verification of drafted tokens where a draw has nothing left to pass, where a greedy request's drafts were drawn, where a tree has
+rows that nothing reaches, and what the drawn token's logarithm may depend on."""
+
+import math
 
 import pytest
 import torch
@@ -87,3 +89,31 @@ def test_rows_that_nothing_reaches_are_not_read(dtype, greedy):
         assert torch.equal(w, g)
     assert torch.equal(want_ws, got_ws)
     step.check(got)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("probs", [False, True])
+def test_the_drawn_tokens_logarithm_is_of_64_bit_sums(probs, dtype):
+    """It is the same in every batch, bit for bit, and off by its own rounding: a token with half of the weight, 65536 others."""
+    B, V = 24, 65536
+    step = Step(44, B, 3, V, dtype, probs=F32 if probs else None, spread=1.0, counts=[3, 1, 2])
+    gen = torch.Generator().manual_seed(45)
+    x = torch.randn(B, 3, V, generator=gen)
+    x[:, :, 1234] = math.log(V) + 0.5
+    step.logits = x.to(dtype)
+    step.uniforms[:, 1:] = 1e9  # no draft stands; of three rows both name the same token
+    step.tokens[:, 1], step.tokens[:, 2] = 99, 99
+    step.parents[:, 2] = torch.where(step.parents[:, 2] >= 0, 0, -2)
+    if probs:
+        step.probs[:, :, 1234] = 0.0
+    got = step.call()
+    log_p = torch.log_softmax(step.logits[:, 0].double(), 1)
+    want = log_p.gather(1, got.tokens[:, :1].cpu())[:, 0]
+    off = (got.logprobs[:, 0].cpu().double() - want).abs()
+    # rounded once to 32 bits; weights to 2^-50 and sums over V terms
+    assert (off <= want.abs() * 2.0 ** -24 + V * 2.0 ** -49).all(), off.max()
+    assert (got.tokens[:, 0] == 1234).sum() >= 3
+    for b0, b1 in ((0, 1), (5, 6), (7, 10), (0, B)):
+        part = [step.logits[b0:b1].cuda(), step.tokens[b0:b1].cuda(), step.parents[b0:b1].cuda(), step.uniforms[b0:b1].cuda()]
+        alone = ops.verify_drafts(*part, draft_probs=None if not probs else step.probs[b0:b1].cuda())
+        assert torch.equal(alone.tokens, got.tokens[b0:b1]) and torch.equal(alone.logprobs, got.logprobs[b0:b1])
