@@ -840,6 +840,7 @@ __global__ __launch_bounds__(kThreads) void verify_walk_kernel(const VerifyArgs 
           [&](int i) { return probability(a, probs, i); }, [&](float y, int, float q) { return own ? weights(y) : left_of(y, q); }, answer);
 }
 
+constexpr int kRowVectors = 16;  // vectors a thread of the largest cut of rows
 struct Cut {
   int nv, chunks;
 };
@@ -852,7 +853,16 @@ Cut cut_of(int64_t rows, int V, int vec, int most, int64_t wanted) {
     if (c.nv == 1 || rows * c.chunks >= wanted) return c;
   }
 }
-Cut rows_cut(int B, int S, int V, int vec) { return cut_of(static_cast<int64_t>(B) * S, V, vec, 16, 6ll * fp::compute_units()); }
+int64_t rows_wanted() { return 6ll * fp::compute_units(); }
+Cut rows_cut(int B, int S, int V, int vec) { return cut_of(static_cast<int64_t>(B) * S, V, vec, kRowVectors, rows_wanted()); }
+// Chunks of up to this many rows of up to V logits: those of the largest cut, or, of a smaller one, less than twice what was wanted (the cut of twice
+// its size made too few).
+int64_t most_chunks(int64_t rows, int V, int vec) {
+  const int64_t vectors = (static_cast<int64_t>(V) + vec - 1) / vec;
+  const int64_t largest = rows * ((vectors + kThreads * kRowVectors - 1) / (kThreads * kRowVectors)), smallest = rows * ((vectors + kThreads - 1) / kThreads);
+  const int64_t finer = 2 * rows_wanted() < smallest ? 2 * rows_wanted() : smallest;
+  return largest > finer ? largest : finer;
+}
 // Workgroups of a request for the row that is drawn from: four pieces each, more where there are two for every CU without.
 Cut draw_cut(int B, int V, int vec) { return cut_of(B, V, vec, 4, 2ll * fp::compute_units()); }
 int pieces_of(int V, int vec) { return static_cast<int>((static_cast<int64_t>(V) + vec * 64 - 1) / (vec * 64)); }
@@ -870,25 +880,29 @@ int check_shape(const char* what, int B, int S, int V) {
 struct Layout {
   int64_t parts, sums, rests, bytes;
 };
-Layout layout_of(int64_t B, int S, const Cut& rows, int64_t pieces) {
+Layout layout_of(int64_t B, int64_t chunks, int64_t pieces) {
   Layout l;
   l.parts = (B * 4 + 15) / 16 * 16;
-  l.sums = l.parts + B * S * rows.chunks * static_cast<int64_t>(sizeof(Part));
+  l.sums = l.parts + chunks * static_cast<int64_t>(sizeof(Part));
   l.rests = l.sums + B * pieces * static_cast<int64_t>(sizeof(Piece));
   l.bytes = l.rests + B * pieces * 8;
   return l;
+}
+// What any call of this size or smaller, in any type, needs: fewer requests are cut finer and can have more chunks.
+int64_t workspace_of(int B, int S, int V) {
+  int64_t most = 0;
+  for (const int vec : {4, 8}) {
+    const int64_t n = layout_of(B, most_chunks(static_cast<int64_t>(B) * S, V, vec), pieces_of(V, vec)).bytes;
+    most = n > most ? n : most;
+  }
+  return most;
 }
 
 }  // namespace
 
 extern "C" int64_t fp_verify_drafts_workspace_bytes(int32_t B, int32_t S, int32_t V) {
   if (const int rc = check_shape("fp_verify_drafts_workspace_bytes", B, S, V)) return rc;
-  int64_t most = 0;
-  for (const int vec : {4, 8}) {
-    const int64_t n = layout_of(B, S, rows_cut(B, S, V, vec), pieces_of(V, vec)).bytes;
-    most = n > most ? n : most;
-  }
-  return most;
+  return workspace_of(B, S, V);
 }
 
 extern "C" int fp_verify_drafts(const void* logits, int64_t logits_stride_b, int64_t logits_stride_s, int dtype, const int64_t* tokens,
@@ -907,10 +921,11 @@ extern "C" int fp_verify_drafts(const void* logits, int64_t logits_stride_b, int
     return fp::fail(FP_ERR_INVALID_ARGUMENT, "%s: logits and draft_probs must be aligned to their elements", what);
   const Cut rows = rows_cut(B, S, V, 16 / e), draw = draw_cut(B, V, 16 / e);
   const int pieces = pieces_of(V, 16 / e);
-  const Layout l = layout_of(B, S, rows, pieces);
-  if (!workspace || workspace_bytes < l.bytes || !fp::aligned(workspace, 16))
+  const Layout l = layout_of(B, static_cast<int64_t>(B) * S * rows.chunks, pieces);
+  const int64_t needed = workspace_of(B, S, V);
+  if (!workspace || workspace_bytes < needed || !fp::aligned(workspace, 16))
     return fp::fail(FP_ERR_WORKSPACE, "%s: workspace of %lld bytes, 16-byte aligned, is needed (got %lld)", what,
-                    static_cast<long long>(l.bytes), static_cast<long long>(workspace_bytes));
+                    static_cast<long long>(needed), static_cast<long long>(workspace_bytes));
   char* const ws = static_cast<char*>(workspace);
   const VerifyArgs a{static_cast<const char*>(logits), logits_stride_b * e, logits_stride_s * e, tokens, parents, uniforms, temperatures,
                      static_cast<const char*>(draft_probs), probs_stride_b * pe, probs_stride_s * pe, probs_dtype, accepted, path, answer,

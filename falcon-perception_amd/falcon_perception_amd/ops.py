@@ -960,7 +960,7 @@ class VerifiedDrafts(NamedTuple):
 
 
 def verify_workspace_bytes(B: int, S: int, V: int) -> int:
-    """Bytes of workspace of a `verify_drafts` call on logits [B, S, V]."""
+    """Bytes of workspace of `verify_drafts` calls on logits up to [B, S, V], of any type."""
     _int32("verify_workspace_bytes", B=B, S=S, V=V)
     n = int(N.lib().fp_verify_drafts_workspace_bytes(B, S, V))
     N.check(n, "fp_verify_drafts_workspace_bytes")

@@ -706,7 +706,8 @@ int fp_paged_decode_tree(const int64_t* masks, const void* q, int64_t q_stride_b
  *              p's sum is in 64 bits, in an order that no cut changes: rounded once, the same in every batch.  Of drafts that stand, and of greedy
  *              requests, it is of weights in 32 bits, to 2^-18 of itself, and may differ by that much from batch to batch
  * A sequence without a step: accepted 0, path and answer -1, logprobs 0.
- * Workspace: memory of the caller, 16-byte aligned, one call at a time; nothing in it needs clearing.
+ * Workspace: memory of the caller, 16-byte aligned, one call at a time; nothing in it needs clearing.  What is asked for B, S and V serves every
+ * call that is not larger in any of them, in every type.
  * S <= 64, V <= 2^24.
  */
 int64_t fp_verify_drafts_workspace_bytes(int32_t B, int32_t S, int32_t V);

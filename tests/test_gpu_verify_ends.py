@@ -8,6 +8,7 @@ import torch
 
 from falcon_perception_amd import _native as N
 from falcon_perception_amd import ops
+from tests.draft_cases import check_verified
 from tests.test_gpu_verify_drafts import BF16, F16, F32, Step
 
 pytestmark = pytest.mark.gpu
@@ -117,3 +118,17 @@ def test_the_drawn_tokens_logarithm_is_of_64_bit_sums(probs, dtype):
         part = [step.logits[b0:b1].cuda(), step.tokens[b0:b1].cuda(), step.parents[b0:b1].cuda(), step.uniforms[b0:b1].cuda()]
         alone = ops.verify_drafts(*part, draft_probs=None if not probs else step.probs[b0:b1].cuda())
         assert torch.equal(alone.tokens, got.tokens[b0:b1]) and torch.equal(alone.logprobs, got.logprobs[b0:b1])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_the_workspace_of_the_largest_call_serves_all(dtype):
+    """Requests that end leave smaller calls behind, which are cut finer: one workspace, its bytes behind what was asked for untouched."""
+    S, V = 16, 32000
+    step = Step(46, 24, S, V, dtype, reach=3)
+    need = ops.verify_workspace_bytes(24, S, V)
+    whole = torch.full((need + 4096,), 91, dtype=torch.uint8, device="cuda")
+    for B, rows in ((24, S), (6, S), (5, S), (1, S), (3, 7), (1, 1), (23, 2)):
+        part = [t[:B, :rows].contiguous().cuda() for t in (step.logits, step.tokens, step.parents, step.uniforms)]
+        got = ops.verify_drafts(*part, workspace=whole[:need])
+        check_verified(got, *(t.cpu() for t in part))
+        assert (whole[need:] == 91).all()
