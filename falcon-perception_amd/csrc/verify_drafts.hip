@@ -867,13 +867,19 @@ int64_t most_chunks(int64_t rows, int V, int vec) {
 Cut draw_cut(int B, int V, int vec) { return cut_of(B, V, vec, 4, 2ll * fp::compute_units()); }
 int pieces_of(int V, int vec) { return static_cast<int>((static_cast<int64_t>(V) + vec * 64 - 1) / (vec * 64)); }
 
+// Whether both launches, a workgroup a chunk of a row and a workgroup a request's share of the row that is drawn from, are of fewer than 2^32 lanes.
+bool one_launch(int B, int S, int V, int vec) {
+  const int64_t rows = static_cast<int64_t>(B) * S * rows_cut(B, S, V, vec).chunks, draws = static_cast<int64_t>(B) * draw_cut(B, V, vec).chunks;
+  return (rows > draws ? rows : draws) < (1ll << 32) / kThreads;
+}
+int too_many(const char* what, int B, int S, int V) {
+  return fp::fail(FP_ERR_UNSUPPORTED, "%s: %d requests of %d rows of %d logits are too many for one call", what, B, S, V);
+}
 int check_shape(const char* what, int B, int S, int V) {
   if (B < 0 || S <= 0 || V <= 0) return fp::fail(FP_ERR_INVALID_ARGUMENT, "%s: bad sizes (B=%d S=%d V=%d)", what, B, S, V);
   if (S > kMaxTokens || V > 1 << 24)
     return fp::fail(FP_ERR_UNSUPPORTED, "%s: at most %d tokens a request and a vocabulary of %d (got %d and %d)", what, kMaxTokens, 1 << 24, S, V);
-  // one launch of workgroups of a chunk of a row each
-  if (static_cast<int64_t>(B) * S * ((V + kThreads * 4ll - 1) / (kThreads * 4)) > INT32_MAX)
-    return fp::fail(FP_ERR_UNSUPPORTED, "%s: %d requests of %d rows of %d logits are too many for one call", what, B, S, V);
+  if (!one_launch(B, S, V, 8)) return too_many(what, B, S, V);  // of 16 bits; fp_verify_drafts knows its type
   return FP_OK;
 }
 
@@ -914,6 +920,7 @@ extern "C" int fp_verify_drafts(const void* logits, int64_t logits_stride_b, int
   if (const int rc = check_shape(what, B, S, V)) return rc;
   const int e = fp::elem_bytes(dtype), pe = draft_probs ? fp::elem_bytes(probs_dtype) : 4;
   if (e == 0 || pe == 0) return fp::fail(FP_ERR_UNSUPPORTED, "%s: dtype code %d", what, e == 0 ? dtype : probs_dtype);
+  if (!one_launch(B, S, V, 16 / e)) return too_many(what, B, S, V);
   if (B == 0) return FP_OK;
   if (!logits || !tokens || !parents || !uniforms || !accepted || !path || !answer || !logprobs)
     return fp::fail(FP_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
@@ -935,22 +942,14 @@ extern "C" int fp_verify_drafts(const void* logits, int64_t logits_stride_b, int
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const auto go = [&](auto kernel, int64_t grid) {
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, st, a);
+    return fp::check_launch(what);
   };
   const auto launch = [&](auto element) {
     using E = decltype(element);
     const int64_t grid = static_cast<int64_t>(B) * S * rows.chunks;
-    switch (rows.nv) {
-      default: go(verify_rows_kernel<E, 4>, grid); break;
-      case 2: go(verify_rows_kernel<E, 2>, grid); break;
-      case 1: go(verify_rows_kernel<E, 1>, grid);
-    }
-    go(verify_walk_kernel<E>, static_cast<int64_t>(B) * draw.chunks);
+    const int rc = rows.nv >= 4 ? go(verify_rows_kernel<E, 4>, grid) : rows.nv == 2 ? go(verify_rows_kernel<E, 2>, grid) : go(verify_rows_kernel<E, 1>, grid);
+    // (the second reads what the first writes)
+    return rc != FP_OK ? rc : go(verify_walk_kernel<E>, static_cast<int64_t>(B) * draw.chunks);
   };
-  if (dtype == FP_DTYPE_F32)
-    launch(F32{});
-  else if (dtype == FP_DTYPE_BF16)
-    launch(BF16{});
-  else
-    launch(F16{});
-  return fp::check_launch(what);
+  return dtype == FP_DTYPE_F32 ? launch(F32{}) : dtype == FP_DTYPE_BF16 ? launch(BF16{}) : launch(F16{});
 }

@@ -708,7 +708,7 @@ int fp_paged_decode_tree(const int64_t* masks, const void* q, int64_t q_stride_b
  * A sequence without a step: accepted 0, path and answer -1, logprobs 0.
  * Workspace: memory of the caller, 16-byte aligned, one call at a time; nothing in it needs clearing.  What is asked for B, S and V serves every
  * call that is not larger in any of them, in every type.
- * S <= 64, V <= 2^24.
+ * S <= 64, V <= 2^24, and fewer than 2^24 workgroups a launch: B * S * ceil(V / 32768) and B * ceil(V / 8192), of 32 bits 16384 and 4096.
  */
 int64_t fp_verify_drafts_workspace_bytes(int32_t B, int32_t S, int32_t V);
 int fp_verify_drafts(const void* logits, int64_t logits_stride_b, int64_t logits_stride_s, int dtype,

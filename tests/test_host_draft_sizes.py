@@ -1,8 +1,12 @@
-"""Sizes of calls on drafted tokens: workspaces that serve smaller calls."""
+"""Sizes of calls on drafted tokens: workspaces that serve smaller calls, calls past one dispatch."""
+
+import ctypes
 
 import pytest
 
 from falcon_perception_amd import ops
+
+P = ctypes.c_void_p(4096)  # a pointer that is never followed
 
 
 @pytest.mark.parametrize("V", [1, 500, 4096, 32000, 65536, 150001, 1 << 24])
@@ -27,3 +31,25 @@ def test_a_workspace_is_not_much_larger_than_its_call(native_lib):
     assert ops.verify_workspace_bytes(1, 1, 1) < 1 << 17
     # 512 requests of 33 rows of 65536: 4 chunks of 16384 a row, 256 pieces of 256 a request
     assert ops.verify_workspace_bytes(512, 33, 65536) < 512 * (33 * 4 * 16 + 256 * 32) + (1 << 18)
+
+
+@pytest.mark.parametrize("B,S,V,fits", [(1 << 18, 64, 1000, False), ((1 << 18) - 1, 64, 1000, True), (1 << 24, 1, 5, False), ((1 << 24) - 1, 1, 5, True),
+                                        (1 << 19, 1, 1 << 18, False), (1 << 20, 64, 1, False), (1 << 30, 1, 1, False)])
+def test_verifications_past_one_dispatch(native_lib, B, S, V, fits):
+    """A dispatch has fewer than 2^32 lanes: 2^24 workgroups, of a row's chunk or of a request's share of the row that is drawn from."""
+    n = native_lib.fp_verify_drafts_workspace_bytes(B, S, V)
+    if fits:
+        assert n > 0
+        return
+    assert n == -2 and "too many" in native_lib.fp_last_error().decode()
+    for dtype in (0, 1, 2):
+        rc = native_lib.fp_verify_drafts(P, S * V, V, dtype, P, P, P, None, None, 0, 0, 0, P, P, P, P, P, 1 << 50, B, S, V, None)
+        assert rc == -2 and "too many" in native_lib.fp_last_error().decode()
+
+
+def test_elements_of_32_bits_reach_the_end_of_a_dispatch_first(native_lib):
+    """16 bits: 2^18 requests of 32 rows of 32768 are 2^23 workgroups; of 32 bits they are 2^24, and too many."""
+    B, S, V = 1 << 18, 32, 32768
+    assert native_lib.fp_verify_drafts_workspace_bytes(B, S, V) > 0
+    rc = native_lib.fp_verify_drafts(P, S * V, V, 0, P, P, P, None, None, 0, 0, 0, P, P, P, P, P, 1 << 50, B, S, V, None)
+    assert rc == -2 and "too many" in native_lib.fp_last_error().decode()
