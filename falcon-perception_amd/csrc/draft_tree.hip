@@ -41,6 +41,8 @@ extern "C" int fp_draft_tree(const int32_t* parents, const void* cached, int cac
                              int32_t* input_pos, int32_t* rope_pos, void* stream) {
   if (B < 0 || S <= 0) return fp::fail(FP_ERR_INVALID_ARGUMENT, "fp_draft_tree: bad sizes (B=%d S=%d)", B, S);
   if (S > 64) return fp::fail(FP_ERR_UNSUPPORTED, "fp_draft_tree: at most 64 tokens a tree (got %d)", S);
+  if (B > (1 << 26) - kWaves)  // a dispatch holds fewer than 2^32 lanes
+    return fp::fail(FP_ERR_UNSUPPORTED, "fp_draft_tree: %d sequences are too many for one call", B);
   if (cached_index_type != FP_INDEX_I32 && cached_index_type != FP_INDEX_I64)
     return fp::fail(FP_ERR_INVALID_ARGUMENT, "fp_draft_tree: cached_index_type %d", cached_index_type);
   if (B == 0) return FP_OK;

@@ -647,7 +647,7 @@ int fp_paged_decode_shared(const void* q, int64_t q_stride_b, int64_t q_stride_h
  *   masks      [B, S] int64: bit i of masks[b, j] says that token j sees token i: its ancestors and itself; 0 where there is no token
  *   input_pos  [B, S] int32: cached[b] + j, the row of the cache that token j's keys go to (what fp_kv_append takes); -1 no token
  *   rope_pos   [B, S] int32: cached[b] + number of ancestors, its place in the text; 0 no token
- * S <= 64.
+ * S <= 64, B <= 2^26 - 4.
  */
 int fp_draft_tree(const int32_t* parents, const void* cached, int cached_index_type, int32_t B, int32_t S,
                   int64_t* masks, int32_t* input_pos, int32_t* rope_pos, void* stream);

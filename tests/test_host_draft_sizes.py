@@ -53,3 +53,8 @@ def test_elements_of_32_bits_reach_the_end_of_a_dispatch_first(native_lib):
     assert native_lib.fp_verify_drafts_workspace_bytes(B, S, V) > 0
     rc = native_lib.fp_verify_drafts(P, S * V, V, 0, P, P, P, None, None, 0, 0, 0, P, P, P, P, P, 1 << 50, B, S, V, None)
     assert rc == -2 and "too many" in native_lib.fp_last_error().decode()
+
+
+def test_trees_past_one_dispatch(native_lib):
+    for B in (1 << 26, (1 << 26) - 3, 2 ** 31 - 1):
+        assert native_lib.fp_draft_tree(P, P, 0, B, 64, P, P, P, None) == -2 and "too many" in native_lib.fp_last_error().decode()
