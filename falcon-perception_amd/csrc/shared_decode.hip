@@ -1722,6 +1722,9 @@ int check_shape(const char* what, int B, int S, int Hq, int Hc, int D) {
   if (B > kMaxSequences || static_cast<int64_t>(B) * S * G > kMaxRows || static_cast<int64_t>(B) * S * Hq > INT32_MAX)
     return fp::fail(FP_ERR_UNSUPPORTED, "%s: at most %d sequences and %d rows a cached head (got %d of %d tokens, %d heads)", what,
                     kMaxSequences, kMaxRows, B, S, G);
+  // a dispatch holds fewer than 2^32 lanes: D / 4 a row of the join, a workgroup a cached head of the products
+  if ((static_cast<int64_t>(B) * S * Hq + kThreads) * (D / 4) >= 1ll << 32 || Hc >= (1ll << 32) / kThreads)
+    return fp::fail(FP_ERR_UNSUPPORTED, "%s: %d sequences of %d tokens and %d heads on %d are too many for one call", what, B, S, Hq, Hc);
   return FP_OK;
 }
 

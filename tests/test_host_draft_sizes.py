@@ -58,3 +58,11 @@ def test_elements_of_32_bits_reach_the_end_of_a_dispatch_first(native_lib):
 def test_trees_past_one_dispatch(native_lib):
     for B in (1 << 26, (1 << 26) - 3, 2 ** 31 - 1):
         assert native_lib.fp_draft_tree(P, P, 0, B, 64, P, P, P, None) == -2 and "too many" in native_lib.fp_last_error().decode()
+
+
+def test_attention_past_one_dispatch(native_lib):
+    """Rows of the join, D / 4 lanes each, and a workgroup a cached head of the products."""
+    for size in (native_lib.fp_shared_decode_plan_bytes, native_lib.fp_shared_decode_workspace_bytes):
+        assert size(1024, 64, 8 * 256, 256, 128) == -2 and "too many" in native_lib.fp_last_error().decode()
+        assert size(1024, 64, 8 * 255, 255, 128) > 0
+        assert size(1, 1, 1 << 24, 1 << 24, 64) == -2 and "too many" in native_lib.fp_last_error().decode()
