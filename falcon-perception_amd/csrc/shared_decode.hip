@@ -929,9 +929,10 @@ __device__ __forceinline__ int keys_of(const SharedArgs& a, int b, int j) {
 }
 
 // Trees of drafts: token j of a sequence is the key at position input_pos[b, j], so draft 0 is the one at input_pos[b, j] - j, and all keys
-// in front of that are seen by every token.  Of the drafts it sees those whose bits its mask has, up to its own.
+// in front of that are seen by every token.  Of the drafts it sees those whose bits its mask has, up to its own.  (A position below j, of a caller's
+// own: the base is negative, and bits that name what lies in front of position 0 name no key.)
 __device__ __forceinline__ int tree_base(int64_t pos, int j) {
-  return pos < j ? 0 : pos - j > INT32_MAX ? INT32_MAX : static_cast<int>(pos - j);
+  return pos < 0 ? 0 : pos - j > INT32_MAX ? INT32_MAX : static_cast<int>(pos - j);
 }
 
 // Whether token j of sequence b, which is there, sees a key: with `keys` of the cache in front of it and itself
@@ -940,7 +941,8 @@ __device__ __forceinline__ bool sees_any(const SharedArgs& a, int b, int j, int 
   if (!kTree || keys <= 0) return keys > 0;
   const int64_t at = static_cast<int64_t>(b) * a.S + j;
   const int base = tree_base(fp::load_index(a.input_pos, at, a.pos_i64), j);
-  return base > 0 || (static_cast<uint64_t>(a.masks[at]) << (64 - min(keys, 64))) != 0;
+  // (base <= 0: keys are j + 1 + base at most, and -base at most j)
+  return base > 0 || (static_cast<uint64_t>(a.masks[at]) >> -base << (64 - min(keys, 64))) != 0;
 }
 
 template <typename E, int D, bool kTree>

@@ -656,7 +656,7 @@ int fp_draft_tree(const int32_t* parents, const void* cached, int cached_index_t
  * Attention of trees of drafted tokens over the paged cache: fp_paged_decode_shared for tokens that do not see all keys in front of them.
  *
  *   masks      [B, S] contiguous int64.  Token j of sequence b sees the positions below input_pos[b, j] - j and, for every bit i <= j of
- *              masks[b, j], position input_pos[b, j] - j + i (of all these, those below max_context).  Bits behind j count for nothing.
+ *              masks[b, j], position input_pos[b, j] - j + i (of all these, those from 0 on and below max_context).  Bits behind j count for nothing.
  *              A token that sees no key: out = 0, lse = -inf
  * Everything else is as there, for fp_tree_decode_plan, too, whose prefix_ids and prefix_lens may both be NULL: no two sequences share
  * keys.  Plan and workspace have the sizes of fp_shared_decode_plan_bytes and fp_shared_decode_workspace_bytes.  K and V rows of keys that

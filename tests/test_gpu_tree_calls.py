@@ -1,0 +1,59 @@
+"""Attention of trees: positions of the caller's own, in front of a token's row in the step."""
+
+import pytest
+import torch
+
+from falcon_perception_amd import ops
+from tests.draft_cases import DraftBatch
+
+pytestmark = pytest.mark.gpu
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+class Early(DraftBatch):
+    """Tokens whose row in the step is beyond their position: what their masks name in front of position 0 is no key."""
+
+    def seen(self, b, j, max_context=None):
+        pos, mask = int(self.pos[b, j]), int(self.masks[b, j])
+        if pos < 0:
+            return []
+        base = pos - j
+        keys = list(range(base)) + [base + i for i in range(j + 1) if mask >> i & 1]
+        return [t for t in keys if 0 <= t and (max_context is None or t < max_context)]
+
+
+@pytest.mark.parametrize("share", [False, True])
+@pytest.mark.parametrize("index", [torch.int32, torch.int64])
+@pytest.mark.parametrize("dtype,Hq", [(BF16, 4), (F16, 16), (F32, 2)])
+def test_positions_in_front_of_a_tokens_row(dtype, Hq, index, share):
+    gen = torch.Generator().manual_seed(51)
+    case = Early(52, [64], [(-1, 0, [-1] * 64), (0, 20, [-1] * 64), (-1, 30, [-1] * 33), (-1, 0, [-1] * 6)], Hq=Hq, Hc=2, D=64, P=32, dtype=dtype, S=64)
+    case.masks = torch.randint(-(1 << 62), 1 << 62, (4, 64), generator=gen)
+    case.masks[0, 60:] = torch.tensor([-1, 1, 0, -(1 << 63)])
+    case.masks[3] = 0
+    case.masks[3, :6] = torch.tensor([1, 2, 4, 8, 16, 32])  # each sees itself alone
+    case.pos[0] = torch.randint(-1, 64, (64,), generator=gen, dtype=torch.int32)
+    case.pos[1] = torch.randint(0, 84, (64,), generator=gen, dtype=torch.int32)
+    case.pos[2] = torch.arange(64, dtype=torch.int32) // 2
+    case.pos[3] = torch.where(torch.arange(64) < 6, torch.tensor([0, 0, 0, 2, 2, 2] + [-1] * 58), torch.tensor(-1)).int()
+    case.on()
+    tree = ops.DraftTree(case.masks_d, case.pos_d.to(index), case.pos_d)
+    case.check(case.call(ops, share=share, tree=tree))
+    for room in (3, 40):
+        case.check(case.call(ops, share=share, tree=tree, max_context=room), max_context=room)
+
+
+def test_infinities_that_such_a_token_does_not_see():
+    """The value of a key is infinite: tokens whose mask names it, counted from the tree's first position, get to know and no others."""
+    case = Early(53, [], [(-1, 0, [-1] * 8)], Hq=2, Hc=1, D=64, P=16, dtype=BF16).on()
+    case.pos = torch.tensor([[0, 1, 1, 2, 2, 2, 6, 7]], dtype=torch.int32)
+    case.pos_d = case.pos.cuda()
+    case.masks = torch.tensor([[1, 0b11, 0b110, 0b1110, 0b11000, 0b100000, 0b1000010, 0b10000000]])
+    case.masks_d = case.masks.cuda()
+    case.check(case.call(ops))
+    at = int(case.table[case.batch_idx[0], 0]) * 16 + 1  # position 1
+    case.pool_d[1][:, at, 9] = float("inf")
+    out = case.call(ops)[0][0, 0, :, 9].float().cpu()
+    sees = [1 in case.seen(0, j) for j in range(8)]
+    assert sees.count(True) >= 3 and sees.count(False) >= 3
+    assert torch.isinf(out).tolist() == sees
