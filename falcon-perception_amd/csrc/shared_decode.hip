@@ -64,7 +64,7 @@ constexpr int kUnit = 64;              // keys: what the cut is made of
 constexpr int kMinUnits = 3;           // a workgroup's share at least
 constexpr int kSegPages = 1024;        // page ids held in LDS
 constexpr float kMaxSlack = 6.f;       // the reference point of the exponentials may lag the maximum by this much (log2)
-constexpr int kMagic = 0x5ade0001;
+constexpr int kMagic = 0x5ade0001;    // of a plan; of trees, whose tiles are others, the next number
 
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -617,7 +617,7 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const PlanArgs a) {
 
   if (tid == 0) {
     Header* const h = reinterpret_cast<Header*>(a.plan);
-    h->magic = kMagic;
+    h->magic = kMagic + kTree;
     h->B = a.B, h->S = a.S, h->Hq = a.Hq, h->Hc = a.Hc, h->max_batch = a.max_batch, h->max_context = a.max_context;
     h->n_wg = n_wg, h->n_tiles = n_tiles;
   }
@@ -1519,8 +1519,9 @@ __device__ __forceinline__ void run_piece(const SharedArgs& a, Shared<E, D, kTre
   }
 }
 
+template <bool kTree>
 __device__ __forceinline__ bool plan_fits(const SharedArgs& a, const Header& h) {
-  return h.magic == kMagic && h.B == a.B && h.S == a.S && h.Hq == a.Hq && h.Hc == a.Hc && h.max_batch == a.max_batch &&
+  return h.magic == kMagic + kTree && h.B == a.B && h.S == a.S && h.Hq == a.Hq && h.Hc == a.Hc && h.max_batch == a.max_batch &&
          h.max_context == a.max_context;
 }
 
@@ -1542,7 +1543,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(Shared<E, D, kTree>) <= 80 * 1024
   const int w = blockIdx.y;
   const Header h = load_record<Header>(a.plan);
   const Share share = load_record<Share>(a.plan + a.shares + w * static_cast<int64_t>(sizeof(Share)));
-  if (!plan_fits(a, h) || w >= h.n_wg) return;
+  if (!plan_fits<kTree>(a, h) || w >= h.n_wg) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int left = share.units, offset = share.offset, piece = share.piece;
   bool busy = false;
@@ -1593,7 +1594,7 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(const SharedArgs 
   const int h = static_cast<int>(row - bj * a.Hq);
   const int b = a.S == 1 ? static_cast<int>(bj) : static_cast<int>(bj / static_cast<uint32_t>(a.S)), j = static_cast<int>(bj) - b * a.S;
   const Header head = *reinterpret_cast<const Header*>(a.plan);
-  const bool fits = plan_fits(a, head);
+  const bool fits = plan_fits<kTree>(a, head);
   const Sequence s = reinterpret_cast<const Sequence*>(a.plan + a.seqs)[b];
   const int keys = keys_of(a, b, j);
   const int64_t slot = a.batch_idx[b];

@@ -610,7 +610,7 @@ int fp_copy_pages(void* pool, const int64_t* src, const int64_t* dst, const int3
  *
  * fp_shared_decode_plan, once per step, finds the sequences that share and cuts the work; every layer's fp_paged_decode_shared with the
  * same B, S, Hq, Hc, D and max_context takes the plan.  batch_idx, input_pos and the rows of page_table must not change in between.  A launch
- * that meets a plan of another shape leaves NaN in out and lse; one whose sequence has another slot than the plan's, a token where the
+ * that meets a plan of another shape, or of fp_tree_decode_plan, leaves NaN in out and lse; one whose sequence has another slot than the plan's, a token where the
  * plan has none or a position behind all that the plan has for it leaves NaN in that row.  Positions in front of the planned ones are served
  * as they are.
  * Plan and workspace are memory of the caller (16-byte aligned), one launch at a time; nothing in them needs clearing.
@@ -658,7 +658,7 @@ int fp_draft_tree(const int32_t* parents, const void* cached, int cached_index_t
  *   masks      [B, S] contiguous int64.  Token j of sequence b sees the positions below input_pos[b, j] - j and, for every bit i <= j of
  *              masks[b, j], position input_pos[b, j] - j + i (of all these, those from 0 on and below max_context).  Bits behind j count for nothing.
  *              A token that sees no key: out = 0, lse = -inf
- * Everything else is as there, for fp_tree_decode_plan, too, whose prefix_ids and prefix_lens may both be NULL: no two sequences share
+ * Everything else is as there (a plan of fp_shared_decode_plan leaves NaN here), for fp_tree_decode_plan, too, whose prefix_ids and prefix_lens may both be NULL: no two sequences share
  * keys.  Plan and workspace have the sizes of fp_shared_decode_plan_bytes and fp_shared_decode_workspace_bytes.  K and V rows of keys that
  * a token does not see have no part in its result, whatever they hold.
  * S <= 64.

@@ -1,10 +1,11 @@
-"""Attention of trees: positions of the caller's own, in front of a token's row in the step."""
+"""Attention of trees: positions of the caller's own, in front of a token's row in the step, and plans of the other kind."""
 
 import pytest
 import torch
 
 from falcon_perception_amd import ops
 from tests.draft_cases import DraftBatch
+from tests.shared_cases import SharedBatch
 
 pytestmark = pytest.mark.gpu
 BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
@@ -57,3 +58,18 @@ def test_infinities_that_such_a_token_does_not_see():
     sees = [1 in case.seen(0, j) for j in range(8)]
     assert sees.count(True) >= 3 and sees.count(False) >= 3
     assert torch.isinf(out).tolist() == sees
+
+
+def test_plans_of_the_other_kind_are_foreign():
+    """A plan says what it is of: with more than 64 rows of a sequence the two kinds cut them differently."""
+    gen = torch.Generator().manual_seed(54)
+    case = DraftBatch(55, [], [(-1, 200, list(range(-1, 39))), (-1, 9, list(range(-1, 33)))], Hq=8, Hc=2, D=64, P=32, dtype=BF16).on()
+    shape = dict(q_heads=8, cached_heads=2, head_dim=64)
+    room = case.columns * 32
+    tree = ops.DraftTree(case.masks_d, case.pos_d, case.pos_d)
+    of_trees = ops.tree_decode_plan(case.batch_idx_d, tree, case.table_d, max_context=room, prefix_ids=case.ids_d, prefix_lens=case.lens_d, **shape)
+    of_shared = ops.shared_decode_plan(case.batch_idx_d, case.pos_d, case.ids_d, case.lens_d, max_context=room, **shape)
+    case.check(case.call(ops, plan=of_trees))
+    case.check(SharedBatch.call(case, ops, plan=of_shared))
+    for got in (case.call(ops, plan=of_shared), SharedBatch.call(case, ops, plan=of_trees)):
+        assert torch.isnan(got[0].float()).all() and torch.isnan(got[1]).all()
