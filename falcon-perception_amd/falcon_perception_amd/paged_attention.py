@@ -152,7 +152,7 @@ class PagedKVCache(KVCacheBase):
         self.prefix_ids = torch.zeros(max_batch_size, dtype=torch.int32, device=device) if prefix_sharing else None
         self.prefix_lens = torch.zeros(max_batch_size, dtype=torch.int32, device=device) if prefix_sharing else None
         self._shared_buffers: dict[tuple, tuple[Tensor, Tensor, int]] = {}
-        self._tree_buffers: dict[tuple, tuple[Tensor, Tensor, int]] = {}
+        self._tree_buffers: dict[tuple, tuple[Tensor, Tensor, set]] = {}
         self._tree_plan_owner = None  # the mask whose plan is in them
         # status word of the last prefill mask, on its way to the host (`check_prefill_masks`)
         self._mask_status_host: Tensor | None = None
@@ -522,17 +522,24 @@ class PagedKVCache(KVCacheBase):
         ops.keep_rows(self._kv, self.page_table, mask.batch_idx, mask.cached, path, self.page_size)
 
     def tree_decode_buffers(self, B: int, S: int, Hq: int, Hc: int, D: int) -> tuple[Tensor, Tensor]:
-        """Plan and workspace of the attention of a step of drafts.  They grow with the batch; graphs captured with smaller ones keep those."""
-        key = (S, Hq, Hc, D)
-        hit = self._tree_buffers.get(key)
-        if hit is None or hit[2] < B:
+        """Plan and workspace of the attention of a step of drafts, one pair for steps of every batch and number of tokens.  They grow, each to
+        twice its size at least: graphs captured with smaller ones keep those, which all together are no more than the present ones."""
+        hit = self._tree_buffers.get((Hq, Hc, D))
+        if hit is None or (B, S) not in hit[2]:
             shape = dict(q_heads=Hq, cached_heads=Hc, head_dim=D)
-            if hit is not None:
-                self._retired_workspaces.extend(hit[:2])
-            self._tree_plan_owner = None
             sizes = ops.shared_decode_plan_bytes(B, S, **shape), ops.shared_decode_workspace_bytes(B, S, **shape)
-            plan, workspace = (torch.empty(n, dtype=torch.uint8, device=self._kv.device) for n in sizes)
-            hit = self._tree_buffers[key] = (plan, workspace, B)
+            pair = [None, None] if hit is None else list(hit[:2])
+            for i, (t, n) in enumerate(zip(pair, sizes)):
+                if t is None or t.numel() < n:
+                    # (not cleared, as in `shared_decode_buffers`)
+                    pair[i] = torch.empty(n if t is None else max(n, 2 * t.numel()), dtype=torch.uint8, device=self._kv.device)
+                    if t is not None:
+                        self._retired_workspaces.append(t)
+                    if i == 0:
+                        self._tree_plan_owner = None
+            served = set() if hit is None else hit[2]  # steps that they are known to serve
+            served.add((B, S))
+            hit = self._tree_buffers[(Hq, Hc, D)] = (*pair, served)
         return hit[0], hit[1]
 
     # ------------------------------------------------------------------- masks

@@ -1,10 +1,12 @@
-"""Attention of trees: positions of the caller's own, in front of a token's row in the step, and plans of the other kind."""
+"""Attention of trees: positions of the caller's own, in front of a token's row in the step, plans of the other kind, and buffers that grow."""
 
 import pytest
 import torch
 
 from falcon_perception_amd import ops
-from tests.draft_cases import DraftBatch
+from falcon_perception_amd.attention import compiled_flex_attn_decode
+from falcon_perception_amd.paged_attention import PagedKVCache
+from tests.draft_cases import DraftBatch, random_tree
 from tests.shared_cases import SharedBatch
 
 pytestmark = pytest.mark.gpu
@@ -73,3 +75,60 @@ def test_plans_of_the_other_kind_are_foreign():
     case.check(SharedBatch.call(case, ops, plan=of_shared))
     for got in (case.call(ops, plan=of_shared), SharedBatch.call(case, ops, plan=of_trees)):
         assert torch.isnan(got[0].float()).all() and torch.isnan(got[1]).all()
+
+
+def test_graphs_captured_before_the_buffers_grew():
+    """A step of one request in a graph; larger steps afterwards, which need other buffers, and smaller ones, which take them; the graph between
+    them all.  Every step against a cache of its own."""
+    gen = torch.Generator().manual_seed(57)
+    Hq, Hc, D, L = 8, 2, 64, 2
+    make = lambda: PagedKVCache(60, 32, 9, Hc, D, L, BF16)
+    cache, twins = make(), {}
+    slots = [cache.allocate() for _ in range(8)]
+    for s in slots:
+        cache.reserve(s, None, 200)
+    table = cache.page_table.clone()
+    rnd = lambda *s: torch.randn(s, generator=gen).to(BF16).cuda()
+    cache._kv.copy_(rnd(*cache._kv.shape))
+    start = cache._kv.clone()
+
+    def step(c, parents, cached, rows):
+        c._kv.copy_(start)
+        batch_idx = idx[:parents.shape[0]]
+        mask = c.create_tree_mask(batch_idx, parents, cached)
+        outs = []
+        for layer, (q, k, v) in enumerate(rows):
+            pools = c.insert_kv(layer, k, v, input_pos=mask.input_pos, batch_idx=batch_idx)
+            outs += compiled_flex_attn_decode(q, *pools, block_mask=mask, return_lse=True)
+        return outs
+
+    def inputs(B, S):
+        parents = torch.tensor([random_tree(gen, S, 1 + b % 4) for b in range(B)], dtype=torch.int32).cuda()
+        cached = torch.randint(0, 130, (B,), generator=gen, dtype=torch.int32).cuda()
+        return parents, cached, [(rnd(B, Hq, S, D), rnd(B, Hc, S, D), rnd(B, Hc, S, D)) for _ in range(L)]
+
+    def alone(B, S, args):
+        if (B, S) not in twins:
+            twins[B, S] = make()
+            twins[B, S].page_table.copy_(table)
+        return step(twins[B, S], *args)
+
+    idx = torch.tensor(slots, device="cuda")
+    one = inputs(1, 3)
+    step(cache, *one)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step(cache, *one)
+    for B, S in ((1, 3), (2, 5), (8, 20), (3, 7), (8, 64), (1, 1), (8, 20), (2, 64)):
+        args = inputs(B, S)
+        for x, y in zip(step(cache, *args), alone(B, S, args)):
+            assert torch.equal(x, y)
+        new = inputs(1, 3)
+        for x, y in zip((one[0], one[1], *(t for r in one[2] for t in r)), (new[0], new[1], *(t for r in new[2] for t in r))):
+            x.copy_(y)
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(captured, alone(1, 3, one)):
+            assert torch.equal(x, y)
+    assert len(cache._tree_buffers) == 1 and len(cache._retired_workspaces) >= 2

@@ -1,10 +1,12 @@
-"""Sizes of calls on drafted tokens: workspaces that serve smaller calls, calls past one dispatch."""
+"""Sizes of calls on drafted tokens: workspaces that serve smaller calls, calls past one dispatch, buffers of a cache that grow."""
 
 import ctypes
 
 import pytest
+import torch
 
 from falcon_perception_amd import ops
+from falcon_perception_amd.paged_attention import PagedKVCache
 
 P = ctypes.c_void_p(4096)  # a pointer that is never followed
 
@@ -66,3 +68,41 @@ def test_attention_past_one_dispatch(native_lib):
         assert size(1024, 64, 8 * 256, 256, 128) == -2 and "too many" in native_lib.fp_last_error().decode()
         assert size(1024, 64, 8 * 255, 255, 128) > 0
         assert size(1, 1, 1 << 24, 1 << 24, 64) == -2 and "too many" in native_lib.fp_last_error().decode()
+
+
+def retained(cache):
+    held = {t.data_ptr(): t.numel() for t in cache._retired_workspaces}
+    held.update({t.data_ptr(): t.numel() for hit in cache._tree_buffers.values() for t in hit[:2]})
+    return sum(held.values())
+
+
+@pytest.mark.parametrize("order", ["batch", "tokens", "down"])
+def test_buffers_of_trees_are_bounded(native_lib, order):
+    """Batches that grow one request at a time, steps of every number of tokens: what a cache holds on to is within four times what its
+    largest step needs."""
+    cache = PagedKVCache(8, 16, 80, 8, 128, 1, torch.bfloat16, device="cpu")
+    Hq, Hc, D = 32, 8, 128
+    shape = dict(q_heads=Hq, cached_heads=Hc, head_dim=D)
+    steps = {"batch": [(B, S) for B in range(1, 65) for S in (3, 24)], "tokens": [(B, S) for S in range(1, 65) for B in (2, 17, 64)],
+             "down": [(B, S) for B in range(64, 0, -9) for S in range(64, 0, -1)]}[order]
+    largest = 0
+    for B, S in steps:
+        plan, workspace = cache.tree_decode_buffers(B, S, Hq, Hc, D)
+        need = ops.shared_decode_plan_bytes(B, S, **shape), ops.shared_decode_workspace_bytes(B, S, **shape)
+        assert plan.numel() >= need[0] and workspace.numel() >= need[1] and plan.dtype == workspace.dtype == torch.uint8
+        again = cache.tree_decode_buffers(B, S, Hq, Hc, D)
+        assert again[0] is plan and again[1] is workspace
+        largest = max(largest, sum(need))
+    assert retained(cache) <= 4 * largest
+
+
+def test_a_plan_that_moved_is_made_again(native_lib):
+    """Of larger buffers the plan of the step in flight is not in the new one; where they stay, it stands."""
+    cache = PagedKVCache(8, 16, 80, 2, 64, 1, torch.bfloat16, device="cpu")
+    first = cache.tree_decode_buffers(8, 8, 4, 2, 64)
+    cache._tree_plan_owner = owner = object()
+    assert cache.tree_decode_buffers(3, 5, 4, 2, 64)[0] is first[0] and cache._tree_plan_owner is owner
+    more = cache.tree_decode_buffers(40, 64, 4, 2, 64)
+    assert more[0] is not first[0] and cache._tree_plan_owner is None
+    assert any(t is first[0] for t in cache._retired_workspaces)  # a graph captured with it still writes to it
+    assert cache.tree_decode_buffers(40, 64, 8, 2, 64)[0] is not more[0]
