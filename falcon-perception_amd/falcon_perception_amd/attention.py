@@ -363,7 +363,8 @@ def _shared_decode(q: Tensor, k: Tensor, v: Tensor, mask: PagedDecodeMask, step,
 
 
 def _tree_decode(q: Tensor, k: Tensor, v: Tensor, mask: PagedTreeMask, scale, sinks) -> tuple[Tensor, Tensor]:
-    """The decode call of a step of drafts: the plan is made by the first layer."""
+    """The decode call of a step of drafts: the plan is made by the first layer.  (`kv_rep` has no part in it: every cached V head is read, and a
+    tile has the rows of one cached head.)"""
     cache = mask.cache
     step = cache.last_decode_step
     if step is None:

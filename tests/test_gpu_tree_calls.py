@@ -1,4 +1,5 @@
-"""Attention of trees: positions of the caller's own, in front of a token's row in the step, plans of the other kind, and buffers that grow."""
+"""Attention of trees: positions of the caller's own, in front of a token's row in the step, plans of the other kind, buffers that
+grow, caches whose heads are copies."""
 
 import pytest
 import torch
@@ -132,3 +133,52 @@ def test_graphs_captured_before_the_buffers_grew():
         for x, y in zip(captured, alone(1, 3, one)):
             assert torch.equal(x, y)
     assert len(cache._tree_buffers) == 1 and len(cache._retired_workspaces) >= 2
+
+
+@pytest.mark.parametrize("sharing", [False, True])
+@pytest.mark.parametrize("fuse", [False, True])
+def test_a_cache_whose_heads_are_copies(fuse, sharing):
+    """One cached head a query head, V copied in pairs: trees read every cached head and answer as a cache of the heads by themselves."""
+    gen = torch.Generator().manual_seed(56)
+    H, Hkv, D, L = 8, 4, 64, 2
+    wide = PagedKVCache(40, 16, 5, H, D, L, BF16, kv_rep=2, prefix_sharing=sharing, fuse_decode_append=fuse)
+    plain = PagedKVCache(40, 16, 5, H, D, L, BF16, kv_rep=1, prefix_sharing=sharing, fuse_decode_append=fuse)
+    rnd = lambda *s: torch.randn(s, generator=gen).to(BF16).cuda()
+    lens, S = [37, 5, 0], 6
+    slots = []
+    for cache in (wide, plain):
+        slots.append([cache.allocate() for _ in lens])
+        for s, n in zip(slots[-1], lens):
+            cache.reserve(s, None, n + S)
+    assert slots[0] == slots[1]
+    batch_idx = torch.tensor(slots[0], device="cuda")
+    pair = lambda t: t.repeat_interleave(2, 1)
+    for i in range(max(lens)):
+        have = torch.tensor([[i] if i < n else [-1] for n in lens], dtype=torch.int32).cuda()
+        for layer in range(L):
+            k, v = rnd(3, H, 1, D), pair(rnd(3, Hkv, 1, D))
+            for cache in (wide, plain):
+                cache.assign(layer, batch_idx, have, k, v)
+                cache.flush()
+    parents = torch.tensor([random_tree(gen, S, r) for r in (1, 2, 6)], dtype=torch.int32).cuda()
+    cached = torch.tensor(lens, dtype=torch.int32).cuda()
+    masks = [cache.create_tree_mask(batch_idx, parents, cached) for cache in (wide, plain)]
+    for layer in range(L):
+        k, v, q = rnd(3, H, S, D), pair(rnd(3, Hkv, S, D)), rnd(3, H, S, D)
+        outs = []
+        for cache, mask in zip((wide, plain), masks):
+            pools = cache.insert_kv(layer, k, v, input_pos=mask.input_pos, batch_idx=batch_idx)
+            outs.append(compiled_flex_attn_decode(q, *pools, block_mask=mask, return_lse=True))
+        for x, y in zip(*outs):
+            assert torch.equal(x, y)
+        # against the definition, one request at a time
+        for b, n in enumerate(lens):
+            seen = masks[0].tree.masks[b].tolist()
+            rows = torch.arange(n + S, device="cuda")
+            at = wide.page_table[batch_idx[b], rows // 16] * 16 + rows % 16
+            kk, vv = (wide.kv_cache[layer, i, 0][:, at].double().cpu() for i in range(2))
+            hide = torch.tensor([[t >= n and not seen[j] >> (t - n) & 1 for t in range(n + S)] for j in range(S)])
+            x = torch.bmm(q[b].double().cpu(), kk.transpose(1, 2).contiguous()) * D ** -0.5
+            want = torch.bmm(torch.softmax(x.masked_fill(hide, -torch.inf), 2), vv)
+            # rounded once to bf16; sums of 50 keys in 32 bits
+            assert (outs[0][0][b].double().cpu() - want).abs().max() <= 2.0 ** -8 * want.abs().max() + 1e-4
