@@ -133,6 +133,16 @@ struct Weights {
 
 __device__ __forceinline__ float heat_of(const VerifyArgs& a, int b) { return a.temperatures ? a.temperatures[b] : 1.f; }
 
+// Whether the walk can reach row j, which is the same for all lanes: up from there, in scalar registers.
+__device__ __forceinline__ bool is_reachable(int parent, int j) {
+  while (j > 0) {
+    const int above = __builtin_amdgcn_readlane(parent, j);
+    if (above < 0 || above >= j) return false;
+    j = above;
+  }
+  return __builtin_amdgcn_readlane(parent, 0) == -1;
+}
+
 // A row: elements in front of the first whole 16 bytes, whole ones, elements behind them.
 template <typename E>
 struct Row {
@@ -223,7 +233,7 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(const VerifyArgs 
   const int c = blockIdx.x - row * a.chunks, j = row - b * a.S;
   if (c == 0 && j == 0 && tid == 0) a.arrivals[b] = 0;
   const float heat = heat_of(a, b);
-  if (!(reachable(lane < a.S ? a.parents[static_cast<int64_t>(b) * a.S + lane] : -2, lane) >> j & 1)) return;
+  if (!is_reachable(lane < a.S ? a.parents[static_cast<int64_t>(b) * a.S + lane] : -2, j)) return;
   const Row<E> r(a.logits + b * a.ls_b + j * a.ls_s, a.V);
   const int v_end = min((c + 1) * a.chunk_vectors, r.vectors);
   int v = c * a.chunk_vectors + tid;
