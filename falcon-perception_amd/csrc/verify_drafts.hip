@@ -14,16 +14,16 @@
 //    most, summed in 64.
 //  * walk: every workgroup puts the chunks of its request's rows together and walks down the tree; a comparison within kBand of its
 //    border is made again with the row's sum in 64 bits (a few in a million).  Then it sums the weights of its pieces of the row that the walk
-//    ends at, and the last workgroup of a request draws; the drawn token's logarithm is by that sum.  Where the drafts were drawn, Z is known only then: until then a piece has the
-//    sums of w and of q over the tokens that surely have something left, and one with a token within kBand of its border (every 100 pieces,
-//    if p and q have nothing to do with each other) is weighed again by the last workgroup.
+//    ends at, and the last workgroup of a request draws; the drawn token's logarithm is by that sum.  Where the drafts were drawn, Z is known
+//    only then: until then a piece has the sums of w and of q over the tokens that surely have something left, and one with a token within kBand
+//    of its border (every 100 pieces, if p and q have nothing to do with each other) is weighed again by the last workgroup.
 // The first launch sets the counters of the second to 0: nothing is kept between calls.
 //
-// Rows is bound by the logits' bytes: 64 requests of 3 to 8 rows of 65536 in 32 bits, 92 MB, 19.2 us (4.8 TB/s), 32 of 17 to 33 in 16 bits, 104 MB,
-// 22.6 us (4.6 TB/s: an exponential for every two bytes).  With all weights in 64 bits the two were 60.7 and 50.4 us.  Walk is a line of trips and of
-// f64 instructions: of the first 25.2 us, 2.7 until a request's rows are put together, 1.6 the walk, 8.5 the 25 MB of the rows that are drawn from and
-// of their drafts' probabilities (35 instructions a token, 14 of them f64 products), 2 until the last workgroup has the sums, 2 for the pieces of which it
-// was not sure, and the draw; of the second 16.3.  One request of 5 rows: 3.8 and 11.9 us.
+// Rows is bound by the logits' bytes: 64 requests of 3 to 8 rows of 65536 in 32 bits, 92 MB, 19.7 us (4.7 TB/s), 32 of 17 to 33 in 16 bits, 104 MB,
+// 24.6 us (4.2 TB/s: an exponential for every two bytes; 0.3 of it to find which rows the walk can reach).  With all weights in 64 bits the two were
+// 60.7 and 50.4 us.  Walk is a line of trips and of f64 instructions: of the first 25.0 us, 2.7 until a request's rows are put together, 1.6 the walk,
+// 8.5 the 25 MB of the rows that are drawn from and of their drafts' probabilities (35 instructions a token, 14 of them f64 products), 2 until the last
+// workgroup has the sums, 2 for the pieces of which it was not sure, and the draw; of the second 15.5.  One request of 5 rows: 3.7 and 11.5 us.
 #include "fp_common.h"
 
 #include <math.h>
@@ -218,8 +218,8 @@ __device__ __forceinline__ void each(const Row<E>& r, int v, const v4u& x, F f) 
 // A thread has G vectors at a time, the next ones on their way meanwhile, and weighs by a logit of its own that moves only when a larger one
 // is more than 2^kSlack heavier: no exchange between threads before the end of the chunk.  An exponent is x rate - shift in one
 // instruction, rate and shift in 32 bits: the weights are next to 2^reference, which has in 64 bits what the two were rounded by.  An
-// infinity that is not below, or NaN, makes a thread's sum NaN, and it weighs once more.  (32 requests of 17 to 33 rows of 65536 in 16 bits: 22.6 us,
-// 24.4 with a difference, a product and a bound for NaN.)
+// infinity that is not below, or NaN, makes a thread's sum NaN, and it weighs once more.  (32 requests of 17 to 33 rows of 65536 in 16 bits: 24.2 us,
+// 26.2 with a difference, a product and a bound for NaN.)
 constexpr double kSlack = 20.0;
 constexpr double kFar = 0x1p22;  // a shift up to this is rounded by 1/4 at most
 

@@ -660,7 +660,7 @@ int fp_draft_tree(const int32_t* parents, const void* cached, int cached_index_t
  *              A token that sees no key: out = 0, lse = -inf
  * Everything else is as there (a plan of fp_shared_decode_plan leaves NaN here), for fp_tree_decode_plan, too, whose prefix_ids and prefix_lens may both be NULL: no two sequences share
  * keys.  Plan and workspace have the sizes of fp_shared_decode_plan_bytes and fp_shared_decode_workspace_bytes.  K and V rows of keys that
- * a token does not see have no part in its result, whatever they hold.
+ * a token does not see have no part in its result, whatever they hold.  Cached heads that are copies of one another are each read.
  * S <= 64.
  */
 int fp_tree_decode_plan(const int64_t* batch_idx, const void* input_pos, int pos_index_type,
