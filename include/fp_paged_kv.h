@@ -703,8 +703,9 @@ int fp_paged_decode_tree(const int64_t* masks, const void* q, int64_t q_stride_b
  *   answer     [B, S] int64: the tokens that stand, then the drawn one, -1 behind them; -1 in its place too where the row has no logit
  *              above -inf, or every token that has one was refused
  *   logprobs   [B, S] float32: log p of every answered token where it stands (greedy: at temperature 1), 0 where there is none.  Of the drawn token
- *              p's sum is in 64 bits, in an order that no cut changes: rounded once, the same in every batch.  Of drafts that stand, and of greedy
- *              requests, it is of weights in 32 bits, to 2^-18 of itself, and may differ by that much from batch to batch
+ *              p's sum is in 64 bits, in an order that no cut changes: rounded once, and the same in every batch (of rows that begin at the same
+ *              place of 16 bytes; else the sum's last bits may differ).  Of drafts that stand, and of greedy requests, it is of weights in 32
+ *              bits, to 2^-18 of itself, and may differ by that much from batch to batch
  * A sequence without a step: accepted 0, path and answer -1, logprobs 0.
  * Workspace: memory of the caller, 16-byte aligned, one call at a time; nothing in it needs clearing.  What is asked for B, S and V serves every
  * call that is not larger in any of them, in every type.
